@@ -203,8 +203,9 @@ def _plain_pack(x):
     blocks = -(-width // BLOCK)
     v = torch.nn.functional.pad(x.float(), (0, blocks * BLOCK - width)).reshape(*x.shape[:-1], blocks, BLOCK)
     m = v.abs().amax(-1, keepdim=True).clamp_min(TINY)
-    code = torch.round(v * (127.0 / m))
-    value = (code * (m / 127.0)).reshape(*x.shape[:-1], blocks * BLOCK)[..., :width]
+    most = torch.full_like(m, 127.0)  # a tensor: torch turns divisions with a number into products
+    code = torch.round(v * (most / m))
+    value = (code * (m / most)).reshape(*x.shape[:-1], blocks * BLOCK)[..., :width]
     return value.to(x.dtype)
 
 
