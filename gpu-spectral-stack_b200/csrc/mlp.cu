@@ -1,0 +1,1268 @@
+// The gated feed-forward block, y = (act(x Wg^T) * (x Wu^T)) Wd^T, and its gradients, as tcgen05
+// matrix products with the pointwise work in their epilogues.
+//
+// Forward (M tokens, C channels, F hidden, D outputs):
+//   gate       G = x Wg^T and U = x Wu^T in one kernel (one MMA of N = 256 over the stacked tiles
+//              [Wg; Wu]); its epilogue stores h = act(G) * U, so neither product reaches HBM
+//   down       y = h Wd^T
+// Backward, from x (or its 8-bit checkpoint) and dy alone:
+//   gate back  G, U and dh = dy Wd in one kernel; its epilogue stores dU = dh act(G),
+//              dG = dh U act'(G) and h
+//   input      dx = dG Wg + dU Wu, one accumulator over both products
+//   weights    dWg = dG^T x, dWu = dU^T x, dWd = dy^T h, K = tokens: the token range is cut into
+//              parts, FP32 partial products are added up in a fixed order by a last kernel
+// Weights and activations are used as they lie: a product that needs a transposed operand reads
+// the same TMA tile through an MN-major descriptor (umma.cuh), nothing is transposed in memory.
+//
+// One kernel template serves the products: persistent CTAs (one per SM), a TMA warp, an MMA warp
+// (one elected lane issues) and eight epilogue warps; tiles of 128 rows, K in chunks of 64,
+// kStages chunks in flight; two accumulator sets in tensor memory, so a tile's epilogue runs under
+// the next tile's products. Every wait is bounded (tma.cuh).
+//
+// Types: bf16 and f16 run as they are, accumulated in FP32; h, dG and dU are rounded once to the
+// type, as they feed the next product. float32 operands are split into three bf16 parts
+// (24 significand bits, bf16 has FP32's range) and the six products of order up to 2 (hi hi, hi
+// mid, mid hi, mid mid, hi lo, lo hi) are taken: the dropped ones are below 2^-24 of the product.
+// The tensor core cuts its FP32 accumulator once per MMA, an error that grows with K, so float32
+// products run in passes of 128 values of K: the five small products first, hi hi last, and the
+// epilogue warps add the passes up in registers (rounded to nearest). One pass over all of K left
+// an error of 4.3e-6 at K = 100 and 270.
+//
+// A few tokens: matrix tiles would be mostly padding, and the weights are all there is to read.
+// Two kernels read each weight row once with 16-byte loads, all lanes of a warp on one row, h
+// in FP32 in between.
+
+#include "../../include/spectral_b200.h"
+
+#include "backend.hpp"
+#include "launch.cuh"
+#include "pointwise.cuh"
+#include "umma.cuh"
+
+#include <algorithm>
+#include <climits>
+
+namespace spectral {
+
+void unpack8(const signed char* codes, const float* scales, void* x, int dtype, long long rows, int width,
+             cudaStream_t stream);
+
+namespace {
+
+constexpr int kTileM = 128;
+constexpr int kChunk = umma::kAtom;  // K per stage
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kTileABytes = kTileM * umma::kRowBytes;
+constexpr int kMaxSmem = 227 * 1024;
+constexpr long long kMaxTokens = 0x7fffff00LL;  // 32-bit TMA coordinates
+
+// The type matrix products run in, and the parts an operand of T is split into.
+template <class T>
+struct Operand {
+    using Type = T;
+    static constexpr int kPlanes = 1;
+    static constexpr int kProducts = 1;
+    static constexpr int kPassChunks = 1 << 24;  // one pass over all of K
+};
+template <>
+struct Operand<float> {
+    using Type = bf16;
+    static constexpr int kPlanes = 3;
+    static constexpr int kProducts = 6;
+    static constexpr int kPassChunks = 2;
+};
+
+// Parts (a, b) of a float32 product's p-th MMA, the small ones first: (2,0) (0,2) (1,1) (1,0) (0,1)
+// (0,0), two bits each. Other types have one part.
+template <class T>
+__device__ __forceinline__ int part_a(int p) { return sizeof(T) == 4 ? (0b00'00'01'01'00'10 >> (2 * p)) & 3 : 0; }
+template <class T>
+__device__ __forceinline__ int part_b(int p) { return sizeof(T) == 4 ? (0b00'01'00'01'10'00 >> (2 * p)) & 3 : 0; }
+
+// v = hi + mid + lo in bf16 parts (exact but for parts below bf16's smallest). A hi that would round to
+// infinity is cut instead, and an infinity or NaN has no further parts.
+__device__ __forceinline__ void split3(float v, bf16& hi, bf16& mid, bf16& lo)
+{
+    hi = __float2bfloat16_rn(v);
+    if (fabsf(v) > 3.3895313892515355e38f && fabsf(v) <= 3.4028234663852886e38f) {
+        hi = __float2bfloat16_rz(v);
+    }
+    const float r = fabsf(v) <= 3.4028234663852886e38f ? v - __bfloat162float(hi) : 0.0f;
+    mid = __float2bfloat16_rn(r);
+    lo = __float2bfloat16_rn(r - __bfloat162float(mid));
+}
+
+// --- staging ---------------------------------------------------------------------------------------
+
+// Copies a rows x cols matrix of T into the operand form: planes of the operand type, `pitch`
+// values a row (a multiple of 8). For arrays TMA cannot read as they lie: float32, or rows that
+// are not 16-byte pieces.
+template <class T>
+__global__ void __launch_bounds__(256)
+    stage_kernel(const T* __restrict__ src, typename Operand<T>::Type* __restrict__ dst, long long rows, int cols, int pitch)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int pieces = pitch / 8;
+    const long long total = rows * pieces;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<long long>(gridDim.x) * 256) {
+        const long long row = i / pieces;
+        const int c0 = static_cast<int>(i - row * pieces) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = c0 + j < cols ? to_float(src[row * cols + c0 + j]) : 0.0f;
+        }
+        if constexpr (sizeof(T) == 4) {
+            Vec<bf16, 8> hi, mid, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                split3(v[j], hi.v[j], mid.v[j], lo.v[j]);
+            }
+            *reinterpret_cast<Vec<bf16, 8>*>(dst + row * pitch + c0) = hi;
+            *reinterpret_cast<Vec<bf16, 8>*>(dst + (rows + row) * pitch + c0) = mid;
+            *reinterpret_cast<Vec<bf16, 8>*>(dst + (2 * rows + row) * pitch + c0) = lo;
+        } else {
+            Vec<T, 8> out;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                out.v[j] = from_float<T>(v[j]);
+            }
+            *reinterpret_cast<Vec<T, 8>*>(dst + row * pitch + c0) = out;
+        }
+    }
+}
+
+// --- epilogue stores ---------------------------------------------------------------------------------
+
+// 32 bytes with one store; p is 32-byte aligned.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// A run of 32 values of one row; only the first `valid` exist.
+template <class T>
+__device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
+{
+    constexpr int kPer = 32 / static_cast<int>(sizeof(T));  // values per 32 bytes
+    if (valid >= 32 && (reinterpret_cast<std::uintptr_t>(p) & 31u) == 0) {
+#pragma unroll
+        for (int i = 0; i < 32 / kPer; ++i) {
+            uint32_t w[8];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = __float_as_uint(v[i * kPer + j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    Vec<T, 2> two{{v[i * kPer + 2 * j], v[i * kPer + 2 * j + 1]}};
+                    w[j] = *reinterpret_cast<uint32_t*>(&two);
+                }
+            }
+            store32(p + i * kPer, w);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (j < valid) {
+                p[j] = v[j];
+            }
+        }
+    }
+}
+
+// A run of hidden values in the operand form (planes `plane` values apart).
+template <class T>
+__device__ __forceinline__ void store_hidden(typename Operand<T>::Type* p, long long plane, const float (&v)[32], int valid)
+{
+    if constexpr (sizeof(T) == 4) {
+        bf16 hi[32], mid[32], lo[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            split3(v[j], hi[j], mid[j], lo[j]);
+        }
+        store_run(p, hi, valid);
+        store_run(p + plane, mid, valid);
+        store_run(p + 2 * plane, lo, valid);
+    } else {
+        T out[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            out[j] = from_float<T>(v[j]);
+        }
+        store_run(p, out, valid);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[32], int valid)
+{
+    T out[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        out[j] = from_float<T>(v[j]);
+    }
+    store_run(p, out, valid);
+}
+
+// --- the matrix-product kernel -----------------------------------------------------------------------
+
+enum class Kind {
+    kGate,      // A = x, B = [Wg; Wu] (K-major): h
+    kGateBack,  // A = x, B = [Wg; Wu], then A = dy, B = Wd (MN-major): dG, dU, h
+    kDown,      // A = h, B = Wd (K-major): y
+    kInput,     // A = dG, B = Wg, then A = dU, B = Wu (MN-major): dx
+    kWeight,    // three problems, A and B MN-major, K = tokens: FP32 partial products
+};
+
+struct Maps {
+    CUtensorMap a[3];
+    CUtensorMap b[3];
+};
+
+struct Args {
+    int rows = 0;         // of the output (M)
+    int cols = 0;         // per accumulator (N)
+    int m_tiles = 0;
+    int n_tiles = 0;
+    long long tiles = 0;
+    int chunks[2] = {0, 0};  // K chunks of the one or two operand pairs
+    void* out[3] = {nullptr, nullptr, nullptr};
+    long long pitch = 0;  // of the output rows, in values
+    long long plane = 0;  // of the hidden arrays, in values
+    // kWeight: problem p is rows_of[p] x cols_of[p]; tiles [first[p], first[p + 1]) of one part.
+    int rows_of[3] = {0, 0, 0};
+    int cols_of[3] = {0, 0, 0};
+    int n_tiles_of[3] = {0, 0, 0};
+    long long first[4] = {0, 0, 0, 0};
+    int parts = 1;
+    int part_chunks = 0;
+    long long part_size = 0;  // floats of one part's three products
+    long long offset[3] = {0, 0, 0};
+    unsigned* fault = nullptr;
+};
+
+template <Kind K, int BN>
+struct Config {
+    static constexpr bool kAMn = K == Kind::kWeight;
+    static constexpr int kSets = K == Kind::kGate ? 2 : K == Kind::kGateBack ? 3 : 1;  // accumulators of BN columns
+    static constexpr int kBRows = K == Kind::kGate || K == Kind::kGateBack ? 2 * BN : BN;
+    static constexpr int kBBytes = kBRows * umma::kRowBytes;
+    static constexpr int kStageBytes = kTileABytes + kBBytes;
+    static constexpr int kStages = (kMaxSmem - 2048) / kStageBytes > 6 ? 6 : (kMaxSmem - 2048) / kStageBytes;
+    static constexpr int kCols = kSets * BN;
+    static constexpr int kTmemCols = 2 * kCols <= 64 ? 64 : 2 * kCols <= 128 ? 128 : 2 * kCols <= 256 ? 256 : 512;
+    static constexpr int kSmem = kStages * kStageBytes + 2048;  // barriers, and slack for the 1 KiB base
+    static_assert(2 * kCols <= 512, "two accumulator sets in tensor memory");
+};
+
+// Tile t: output rows from m0, columns from n0, chunks [k0, k1) (kWeight: of problem p and part `part`).
+struct Tile {
+    int m0;
+    int n0;
+    int k0;
+    int k1;
+    int problem;
+    int part;
+    int passes;
+};
+
+// The chunks of operand pair `pair` that pass `pass` of a tile covers.
+template <class T>
+__device__ __forceinline__ void pass_range(const Args& g, const Tile& tile, int pair, int pass, int& begin, int& end)
+{
+    constexpr int kStep = Operand<T>::kPassChunks;
+    const int last = pair == 0 ? tile.k1 : g.chunks[1];
+    begin = min((pair == 0 ? tile.k0 : 0) + pass * kStep, last);
+    end = min(begin + kStep, last);
+}
+
+template <Kind K, int BN, class T>
+__device__ __forceinline__ Tile locate(const Args& g, long long t)
+{
+    Tile tile{0, 0, 0, g.chunks[0], 0, 0, 1};
+    if constexpr (K == Kind::kWeight) {
+        tile.part = static_cast<int>(t / g.first[3]);
+        const long long r = t - tile.part * g.first[3];
+        tile.problem = r >= g.first[2] ? 2 : r >= g.first[1] ? 1 : 0;
+        const int i = static_cast<int>(r - g.first[tile.problem]);
+        tile.m0 = i / g.n_tiles_of[tile.problem] * kTileM;
+        tile.n0 = i % g.n_tiles_of[tile.problem] * BN;
+        tile.k0 = tile.part * g.part_chunks;
+        tile.k1 = min(tile.k0 + g.part_chunks, g.chunks[0]);
+    } else {
+        tile.m0 = static_cast<int>(t / g.n_tiles) * kTileM;
+        tile.n0 = static_cast<int>(t % g.n_tiles) * BN;
+    }
+    if constexpr (sizeof(T) == 4) {
+        constexpr int kStep = Operand<T>::kPassChunks;
+        tile.passes = (max(tile.k1 - tile.k0, g.chunks[1]) + kStep - 1) / kStep;
+    }
+    return tile;
+}
+
+// The epilogue of 32 columns of one row, from col on: acc holds each accumulator's values.
+template <Kind K, class T, int Act, int Sets>
+__device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row, int col, int cols, float (&acc)[Sets][32])
+{
+    using Op = typename Operand<T>::Type;
+    const int valid = min(32, cols - col);
+    const long long at = row * g.pitch + col;
+    if constexpr (K == Kind::kGate) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            acc[0][j] = activate<Act>(acc[0][j]) * acc[1][j];
+        }
+        store_hidden<T>(static_cast<Op*>(g.out[0]) + at, g.plane, acc[0], valid);
+    } else if constexpr (K == Kind::kGateBack) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float slope;
+            const float a = activate_slope<Act>(acc[0][j], slope);
+            const float up = acc[1][j];
+            acc[0][j] = acc[2][j] * up * slope;  // dG
+            acc[1][j] = a * up;                  // h
+            acc[2][j] *= a;                      // dU
+        }
+        store_hidden<T>(static_cast<Op*>(g.out[0]) + at, g.plane, acc[0], valid);
+        store_hidden<T>(static_cast<Op*>(g.out[1]) + at, g.plane, acc[2], valid);
+        store_hidden<T>(static_cast<Op*>(g.out[2]) + at, g.plane, acc[1], valid);
+    } else if constexpr (K == Kind::kWeight) {
+        float* out = static_cast<float*>(g.out[0]) + tile.part * g.part_size + g.offset[tile.problem];
+        store_values<float>(out + static_cast<long long>(row) * cols + col, acc[0], valid);
+    } else {
+        store_values<T>(static_cast<T*>(g.out[0]) + at, acc[0], valid);
+    }
+}
+
+// This warp has read the accumulator set that `bar` guards.
+__device__ __forceinline__ void release(uint64_t* bar, int lane)
+{
+    umma::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) {
+        umma::arrive(bar);
+    }
+}
+
+template <Kind K, int BN, class T, int Act>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g)
+{
+    using Cfg = Config<K, BN>;
+    using Op = Operand<T>;
+    constexpr bool kBf16 = std::is_same_v<typename Op::Type, bf16>;
+    constexpr int kStages = Cfg::kStages;
+    allow_next_grid();
+    extern __shared__ unsigned char smem_base[];
+    const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
+    __shared__ uint64_t full[kStages], empty[kStages], done[2], freed[2], drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up;
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (warp == kEpilogueWarps) {
+        umma::alloc<Cfg::kTmemCols>(&tmem_slot);
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            tma::mbar_init(&full[s], 1);
+            tma::mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            tma::mbar_init(&done[s], 1);
+            tma::mbar_init(&freed[s], kEpilogueWarps);
+        }
+        tma::mbar_init(&drain, 1);
+        gave_up = 0;
+        tma::fence_mbar_init();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    wait_for_previous_grid();
+
+    if (warp == kEpilogueWarps) {
+        // The TMA warp. The previous kernels' plain stores come before these async-proxy reads.
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        int stage = 0;
+        unsigned phase = 0;
+        long long issued = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
+            const Tile tile = locate<K, BN, T>(g, t);
+            constexpr int kPairs = K == Kind::kGateBack || K == Kind::kInput ? 2 : 1;
+            for (int turn = 0; ok && turn < tile.passes * kPairs; ++turn) {
+                const int pair = turn % kPairs;
+                int k0, k1;
+                pass_range<T>(g, tile, pair, turn / kPairs, k0, k1);
+                for (int p = 0; ok && p < Op::kProducts; ++p) {
+                    const int pa = part_a<T>(p), pb = part_b<T>(p);
+                    for (int k = k0; k < k1; ++k) {
+                        ok = tma::mbar_wait(&empty[stage], phase ^ 1u);
+                        if (!ok) {
+                            break;
+                        }
+                        const uint32_t a = base + stage * Cfg::kStageBytes;
+                        const uint32_t b = a + kTileABytes;
+                        uint64_t* bar = &full[stage];
+                        if (umma::elect_one()) {
+                            const int kc = k * kChunk;
+                            if constexpr (K == Kind::kWeight) {
+                                const int q = tile.problem;
+                                tma::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+#pragma unroll
+                                for (int j = 0; j < kTileM / 64; ++j) {
+                                    umma::load_3d(a + j * 8192, &maps.a[q], tile.m0 + 64 * j, kc, pa, bar);
+                                }
+#pragma unroll
+                                for (int j = 0; j < BN / 64; ++j) {
+                                    umma::load_3d(b + j * 8192, &maps.b[q], tile.n0 + 64 * j, kc, pb, bar);
+                                }
+                            } else if constexpr (K == Kind::kInput) {
+                                tma::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+                                umma::load_3d(a, &maps.a[pair], kc, tile.m0, pa, bar);
+#pragma unroll
+                                for (int j = 0; j < BN / 64; ++j) {
+                                    umma::load_3d(b + j * 8192, &maps.b[pair], tile.n0 + 64 * j, kc, pb, bar);
+                                }
+                            } else if constexpr (K == Kind::kDown) {
+                                tma::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+                                umma::load_3d(a, &maps.a[0], kc, tile.m0, pa, bar);
+                                umma::load_3d(b, &maps.b[0], kc, tile.n0, pb, bar);
+                            } else if (pair == 0) {
+                                tma::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+                                umma::load_3d(a, &maps.a[0], kc, tile.m0, pa, bar);
+                                umma::load_3d(b, &maps.b[0], kc, tile.n0, pb, bar);
+                                umma::load_3d(b + BN * umma::kRowBytes, &maps.b[1], kc, tile.n0, pb, bar);
+                            } else {
+                                tma::mbar_arrive_expect_tx(bar, kTileABytes + BN * umma::kRowBytes);
+                                umma::load_3d(a, &maps.a[1], kc, tile.m0, pa, bar);
+#pragma unroll
+                                for (int j = 0; j < BN / 64; ++j) {
+                                    umma::load_3d(b + j * 8192, &maps.b[2], tile.n0 + 64 * j, kc, pb, bar);
+                                }
+                            }
+                        }
+                        __syncwarp();
+                        ++issued;
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+            }
+        }
+        if (!ok) {
+            // Let the loads in flight land (bounded) before the shared memory is given up.
+            bool drained = true;
+            for (long long i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+                drained = tma::mbar_wait(&full[i % kStages], static_cast<unsigned>(i / kStages) & 1u) && drained;
+            }
+            if (lane == 0) {
+                gave_up = 1;
+                if (!drained) {
+                    atomicOr(g.fault, tma::kFaultDrainTimeout);
+                }
+            }
+        }
+    } else if (warp == kEpilogueWarps + 1) {
+        // The MMA warp.
+        constexpr bool kBMnFirst = K == Kind::kWeight || K == Kind::kInput;
+        constexpr uint32_t kFirst = umma::instruction(kBf16, Cfg::kAMn, kBMnFirst, kTileM, Cfg::kBRows);
+        constexpr uint32_t kSecond =
+            K == Kind::kGateBack ? umma::instruction(kBf16, false, true, kTileM, BN) : kFirst;
+        int stage = 0;
+        unsigned phase = 0;
+        int slot = 0;
+        unsigned slot_phase = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
+            const Tile tile = locate<K, BN, T>(g, t);
+            constexpr int kPairs = K == Kind::kGateBack || K == Kind::kInput ? 2 : 1;
+            for (int pass = 0; ok && pass < tile.passes; ++pass) {
+                ok = tma::mbar_wait(&freed[slot], slot_phase ^ 1u);
+                if (!ok) {
+                    break;
+                }
+                umma::fence_after_sync();
+                for (int pair = 0; ok && pair < kPairs; ++pair) {
+                    int k0, k1;
+                    pass_range<T>(g, tile, pair, pass, k0, k1);
+                    const int steps = (k1 - k0) * Op::kProducts;
+                    // kInput's two products share an accumulator; kGateBack's second has its own.
+                    const bool fresh = pair == 0 || K == Kind::kGateBack;
+                    const uint32_t d = tmem + slot * Cfg::kCols + (K == Kind::kGateBack && pair == 1 ? 2 * BN : 0);
+                    for (int i = 0; i < steps; ++i) {
+                        ok = tma::mbar_wait(&full[stage], phase);
+                        if (!ok) {
+                            break;
+                        }
+                        umma::fence_after_sync();
+                        const uint32_t a = base + stage * Cfg::kStageBytes;
+                        const uint32_t b = a + kTileABytes;
+                        if (umma::elect_one()) {
+#pragma unroll
+                            for (int s = 0; s < kChunk / 16; ++s) {
+                                const bool more = !fresh || i > 0 || s > 0;
+                                const uint64_t da = Cfg::kAMn ? umma::desc_mn(a, s, 8192) : umma::desc_k(a, s);
+                                if (K == Kind::kGateBack && pair == 1) {
+                                    umma::mma(d, da, umma::desc_mn(b, s, 8192), kSecond, more);
+                                } else {
+                                    umma::mma(d, da, kBMnFirst ? umma::desc_mn(b, s, 8192) : umma::desc_k(b, s), kFirst,
+                                              more);
+                                }
+                            }
+                            umma::commit(&empty[stage]);
+                        }
+                        __syncwarp();
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                if (ok) {
+                    if (umma::elect_one()) {
+                        umma::commit(&done[slot]);
+                    }
+                    __syncwarp();
+                    slot ^= 1;
+                    slot_phase ^= slot == 0 ? 1u : 0u;
+                }
+            }
+        }
+        if (!ok) {
+            if (umma::elect_one()) {
+                umma::commit(&drain);
+            }
+            __syncwarp();
+            const bool drained = tma::mbar_wait(&drain, 0);
+            if (lane == 0) {
+                gave_up = 1;
+                if (!drained) {
+                    atomicOr(g.fault, tma::kFaultDrainTimeout);
+                }
+            }
+        }
+    } else {
+        // The epilogue warps: warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half the
+        // columns of each accumulator.
+        const int quad = warp & 3;
+        const int half = warp >> 2;
+        int slot = 0;
+        unsigned slot_phase = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
+            const Tile tile = locate<K, BN, T>(g, t);
+            const int row = tile.m0 + quad * 32 + lane;
+            const int rows = K == Kind::kWeight ? g.rows_of[tile.problem] : g.rows;
+            const int cols = K == Kind::kWeight ? g.cols_of[tile.problem] : g.cols;
+            if constexpr (sizeof(T) == 4) {
+                // The passes' accumulators add up in registers: BN = 64, 32 columns per warp.
+                static_assert(BN == 64, "one run of 32 columns per warp");
+                float acc[Cfg::kSets][32];
+#pragma unroll
+                for (int q = 0; q < Cfg::kSets; ++q) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        acc[q][j] = 0.0f;
+                    }
+                }
+                for (int pass = 0; ok && pass < tile.passes; ++pass) {
+                    ok = tma::mbar_wait(&done[slot], slot_phase);
+                    if (!ok) {
+                        break;
+                    }
+                    umma::fence_after_sync();
+                    const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16) + half * 32;
+#pragma unroll
+                    for (int q = 0; q < Cfg::kSets; ++q) {
+                        // An operand pair that ended in an earlier pass has nothing new here.
+                        int begin, end;
+                        pass_range<T>(g, tile, K == Kind::kGateBack && q == 2 ? 1 : 0, pass, begin, end);
+                        if (begin < end) {
+                            float v[32];
+                            umma::load32(d + q * BN, v);
+                            umma::load_wait(v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                acc[q][j] += v[j];
+                            }
+                        }
+                    }
+                    release(&freed[slot], lane);
+                    slot ^= 1;
+                    slot_phase ^= slot == 0 ? 1u : 0u;
+                }
+                const int col = tile.n0 + half * 32;
+                if (ok && row < rows && col < cols) {
+                    finish<K, T, Act>(g, tile, row, col, cols, acc);
+                }
+            } else {
+                ok = tma::mbar_wait(&done[slot], slot_phase);
+                if (ok) {
+                    umma::fence_after_sync();
+                    const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16);
+#pragma unroll 1
+                    for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                        if (tile.n0 + c >= cols) {
+                            break;
+                        }
+                        float acc[Cfg::kSets][32];
+#pragma unroll
+                        for (int q = 0; q < Cfg::kSets; ++q) {
+                            umma::load32(d + q * BN + c, acc[q]);
+                        }
+#pragma unroll
+                        for (int q = 0; q < Cfg::kSets; ++q) {
+                            umma::load_wait(acc[q]);
+                        }
+                        if (row < rows) {
+                            finish<K, T, Act>(g, tile, row, tile.n0 + c, cols, acc);
+                        }
+                        __syncwarp();
+                    }
+                    release(&freed[slot], lane);
+                    slot ^= 1;
+                    slot_phase ^= slot == 0 ? 1u : 0u;
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            gave_up = 1;
+        }
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    if (threadIdx.x == 0 && gave_up != 0) {
+        atomicOr(g.fault, tma::kFaultWaitTimeout);
+    }
+    if (warp == kEpilogueWarps) {
+        umma::dealloc<Cfg::kTmemCols>(tmem);
+    }
+}
+
+// The parts of the three weight products, added up in order and rounded once.
+template <class T>
+__global__ void __launch_bounds__(256)
+    weight_sum_kernel(const float* __restrict__ partial, T* __restrict__ w0, T* __restrict__ w1, T* __restrict__ w2,
+                      long long size0, long long size2, long long part_size, int parts)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const long long total = 2 * size0 + size2;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<long long>(gridDim.x) * 256) {
+        float s = 0.0f;
+        for (int p = 0; p < parts; ++p) {
+            s += partial[p * part_size + i];
+        }
+        if (i < size0) {
+            w0[i] = from_float<T>(s);
+        } else if (i < 2 * size0) {
+            w1[i - size0] = from_float<T>(s);
+        } else {
+            w2[i - 2 * size0] = from_float<T>(s);
+        }
+    }
+}
+
+// --- a few tokens --------------------------------------------------------------------------------------
+
+constexpr int kFewTokens = 8;
+constexpr int kFewThreads = 256;
+
+// acc[m] += sum over a warp's share of w[0 .. n) . v[m][0 .. n), lanes striding 16-byte pieces (or
+// single values where the rows are not whole aligned pieces).
+template <class W, class X, int M>
+__device__ __forceinline__ void row_dot(const W* __restrict__ w, const X* __restrict__ v, long long pitch, int n, int first,
+                                        int step, bool wide, float (&acc)[M])
+{
+    constexpr int kV = 16 / static_cast<int>(sizeof(W));
+    if (wide) {
+#pragma unroll 4
+        for (int c = first * kV; c < n; c += step * kV) {
+            const Vec<W, kV> p = *reinterpret_cast<const Vec<W, kV>*>(w + c);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+#pragma unroll
+                for (int j = 0; j < kV; ++j) {
+                    acc[m] = fmaf(to_float(p.v[j]), to_float(v[m * pitch + c + j]), acc[m]);
+                }
+            }
+        }
+    } else {
+        for (int c = first; c < n; c += step) {
+            const float p = to_float(w[c]);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                acc[m] = fmaf(p, to_float(v[m * pitch + c]), acc[m]);
+            }
+        }
+    }
+}
+
+// One warp per hidden value: h[m][f] = act(x_m . Wg_f) * (x_m . Wu_f), in FP32.
+template <class T, int Act, int M>
+__global__ void __launch_bounds__(kFewThreads)
+    few_gate_kernel(const T* __restrict__ x, const T* __restrict__ w_gate, const T* __restrict__ w_up, float* __restrict__ h,
+                    int channels, int hidden, bool wide)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int f = static_cast<int>(blockIdx.x) * (kFewThreads / 32) + static_cast<int>(threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (f >= hidden) {
+        return;
+    }
+    float a[M], b[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        a[m] = 0.0f;
+        b[m] = 0.0f;
+    }
+    row_dot<T, T, M>(w_gate + static_cast<long long>(f) * channels, x, channels, channels, lane, 32, wide, a);
+    row_dot<T, T, M>(w_up + static_cast<long long>(f) * channels, x, channels, channels, lane, 32, wide, b);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            a[m] += __shfl_xor_sync(0xffffffffu, a[m], o);
+            b[m] += __shfl_xor_sync(0xffffffffu, b[m], o);
+        }
+        if (lane == 0) {
+            h[static_cast<long long>(m) * hidden + f] = activate<Act>(a[m]) * b[m];
+        }
+    }
+}
+
+// One CTA per output: its warps share the row of Wd, the partial sums meet in shared memory.
+template <class T, int M>
+__global__ void __launch_bounds__(kFewThreads)
+    few_down_kernel(const float* __restrict__ h, const T* __restrict__ w_down, T* __restrict__ y, int hidden, int outputs,
+                    bool wide)
+{
+    __shared__ float sums[kFewThreads / 32][M];
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int o = blockIdx.x;
+    float a[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        a[m] = 0.0f;
+    }
+    row_dot<T, float, M>(w_down + static_cast<long long>(o) * hidden, h, hidden, hidden, static_cast<int>(threadIdx.x),
+                         kFewThreads, wide, a);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) {
+            a[m] += __shfl_xor_sync(0xffffffffu, a[m], k);
+        }
+        if ((threadIdx.x & 31) == 0) {
+            sums[threadIdx.x >> 5][m] = a[m];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < M) {
+        float s = 0.0f;
+        for (int k = 0; k < kFewThreads / 32; ++k) {
+            s += sums[k][threadIdx.x];
+        }
+        y[static_cast<long long>(threadIdx.x) * outputs + o] = from_float<T>(s);
+    }
+}
+
+// --- host side -----------------------------------------------------------------------------------------
+
+struct MlpShape {
+    long long tokens;
+    int channels;
+    int hidden;
+    int outputs;
+    int act;
+};
+
+int round_up(int v, int to) { return (v + to - 1) / to * to; }
+int tiles_of(long long v, int tile) { return static_cast<int>((v + tile - 1) / tile); }
+int hidden_pitch(const MlpShape& n) { return round_up(n.hidden, 16); }  // 32-byte rows for the epilogue's stores
+int planes_of(int dtype) { return dtype == SPECTRAL_FLOAT32 ? 3 : 1; }
+
+// A workspace handed out piece by piece, each 256-byte aligned; with a null base it only counts.
+struct Arena {
+    unsigned char* base;
+    std::size_t used = 0;
+
+    void* take(std::size_t bytes)
+    {
+        void* p = base != nullptr ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+// A matrix as the product kernel reads it.
+struct Matrix {
+    const void* base = nullptr;
+    long long rows = 0;
+    long long cols = 0;
+    long long pitch = 0;
+    int planes = 1;
+    bool is_bf16 = true;
+
+    CUtensorMap map(int box_rows) const
+    {
+        return umma::matrix_map(base, is_bf16, rows, cols, pitch, planes, rows * pitch, box_rows);
+    }
+};
+
+// TMA reads the array as it lies: 16-bit values in 16-byte aligned rows.
+template <class T>
+bool direct(const void* p, int cols)
+{
+    return sizeof(T) == 2 && cols % 8 == 0 && aligned_to(p, 16);
+}
+
+template <class T>
+std::size_t staged_bytes(long long rows, int cols)
+{
+    return static_cast<std::size_t>(rows) * round_up(cols, 8) * 2 * Operand<T>::kPlanes;
+}
+
+// The operand form of a rows x cols array, staged into the arena where TMA cannot read it in place.
+template <class T>
+Matrix operand(const void* p, long long rows, int cols, Arena& arena, cudaStream_t stream)
+{
+    constexpr bool kBf16 = std::is_same_v<typename Operand<T>::Type, bf16>;
+    if (direct<T>(p, cols)) {
+        return {p, rows, cols, cols, 1, kBf16};
+    }
+    const int pitch = round_up(cols, 8);
+    void* dst = arena.take(staged_bytes<T>(rows, cols));
+    const long long pieces = rows * (pitch / 8);
+    const unsigned grid = static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, 148 * 16));
+    launch_pdl(stage_kernel<T>, dim3(grid), dim3(256), 0, stream, static_cast<const T*>(p),
+               static_cast<typename Operand<T>::Type*>(dst), rows, cols, pitch);
+    return {dst, rows, cols, pitch, Operand<T>::kPlanes, kBf16};
+}
+
+// hidden values (tokens x hidden) in the arena, in the operand form.
+template <class T>
+Matrix hidden_matrix(const MlpShape& n, Arena& arena)
+{
+    const int pitch = hidden_pitch(n);
+    void* p = arena.take(static_cast<std::size_t>(n.tokens) * pitch * 2 * Operand<T>::kPlanes);
+    return {p, n.tokens, n.hidden, pitch, Operand<T>::kPlanes, std::is_same_v<typename Operand<T>::Type, bf16>};
+}
+
+template <Kind K, int BN, class T, int Act>
+void launch_product(const Maps& maps, Args& g, cudaStream_t stream)
+{
+    using Cfg = Config<K, BN>;
+    static std::atomic<bool> opted[kMaxDevices];
+    const int device = current_device();
+    const auto kernel = product_kernel<K, BN, T, Act>;
+    if (!opted[device].load(std::memory_order_relaxed)) {
+        SPECTRAL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+        opted[device].store(true, std::memory_order_relaxed);
+    }
+    g.fault = device_fault_word();
+    const long long grid = std::min<long long>(g.tiles, device_sm_count(device));
+    launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), static_cast<std::size_t>(Cfg::kSmem), stream, maps, g);
+}
+
+// Calls f(integral_constant<BN>) with the widest tile of 64, 128 or 256 columns that `cols` fills:
+// wider tiles read each row of A fewer times.
+template <class T, class F>
+void with_width(int cols, F&& f)
+{
+    if constexpr (sizeof(T) == 4) {
+        f(std::integral_constant<int, 64>{});  // the passes' sums stay in registers
+    } else if (cols <= 64) {
+        f(std::integral_constant<int, 64>{});
+    } else if (cols <= 128) {
+        f(std::integral_constant<int, 128>{});
+    } else {
+        f(std::integral_constant<int, 256>{});
+    }
+}
+
+void set_tiles(Args& g, long long rows, int cols, int bn)
+{
+    g.rows = static_cast<int>(rows);
+    g.cols = cols;
+    g.m_tiles = tiles_of(rows, kTileM);
+    g.n_tiles = tiles_of(cols, bn);
+    g.tiles = static_cast<long long>(g.m_tiles) * g.n_tiles;
+}
+
+template <class T, int Act>
+void mlp_few(const void* x, const void* wg, const void* wu, const void* wd, void* y, const MlpShape& n, float* h,
+             cudaStream_t stream)
+{
+    constexpr int kV = 16 / static_cast<int>(sizeof(T));
+    const bool wide_c = n.channels % kV == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
+    const bool wide_f = n.hidden % kV == 0 && aligned_to(wd, 16);
+    const auto run = [&](auto m) {
+        constexpr int M = decltype(m)::value;
+        launch_pdl(few_gate_kernel<T, Act, M>, dim3(static_cast<unsigned>(tiles_of(n.hidden, kFewThreads / 32))),
+                   dim3(kFewThreads), 0, stream, static_cast<const T*>(x), static_cast<const T*>(wg),
+                   static_cast<const T*>(wu), h, n.channels, n.hidden, wide_c);
+        launch_pdl(few_down_kernel<T, M>, dim3(static_cast<unsigned>(n.outputs)), dim3(kFewThreads), 0, stream,
+                   static_cast<const float*>(h), static_cast<const T*>(wd), static_cast<T*>(y), n.hidden, n.outputs, wide_f);
+    };
+    switch (n.tokens) {
+        case 1: run(std::integral_constant<int, 1>{}); return;
+        case 2: run(std::integral_constant<int, 2>{}); return;
+        case 3: run(std::integral_constant<int, 3>{}); return;
+        case 4: run(std::integral_constant<int, 4>{}); return;
+        case 5: run(std::integral_constant<int, 5>{}); return;
+        case 6: run(std::integral_constant<int, 6>{}); return;
+        case 7: run(std::integral_constant<int, 7>{}); return;
+        default: run(std::integral_constant<int, 8>{}); return;
+    }
+}
+
+template <class T>
+std::size_t forward_bytes(const MlpShape& n)
+{
+    Arena arena{nullptr};
+    arena.take(staged_bytes<T>(n.tokens, n.channels));
+    arena.take(staged_bytes<T>(n.hidden, n.channels));
+    arena.take(staged_bytes<T>(n.hidden, n.channels));
+    arena.take(staged_bytes<T>(n.outputs, n.hidden));
+    hidden_matrix<T>(n, arena);
+    arena.take(sizeof(float) * kFewTokens * static_cast<std::size_t>(n.hidden));
+    return arena.used + 256;
+}
+
+template <class T>
+void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, void* y, const MlpShape& n, void* work,
+                 cudaStream_t stream)
+{
+    Arena arena{reinterpret_cast<unsigned char*>((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255})};
+    if (n.tokens <= kFewTokens) {
+        float* h = static_cast<float*>(arena.take(sizeof(float) * kFewTokens * static_cast<std::size_t>(n.hidden)));
+        with_activation(n.act, [&](auto act) { mlp_few<T, decltype(act)::value>(x, wg, wu, wd, y, n, h, stream); });
+        return;
+    }
+    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, stream);
+    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, stream);
+    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, stream);
+    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, stream);
+    const Matrix mh = hidden_matrix<T>(n, arena);
+    {
+        constexpr int BN = sizeof(T) == 4 ? 64 : 128;
+        Maps maps;
+        maps.a[0] = mx.map(kTileM);
+        maps.b[0] = mg.map(BN);
+        maps.b[1] = mu.map(BN);
+        Args g;
+        set_tiles(g, n.tokens, n.hidden, BN);
+        g.chunks[0] = tiles_of(n.channels, kChunk);
+        g.out[0] = const_cast<void*>(mh.base);
+        g.pitch = mh.pitch;
+        g.plane = mh.rows * mh.pitch;
+        with_activation(n.act, [&](auto act) { launch_product<Kind::kGate, BN, T, decltype(act)::value>(maps, g, stream); });
+    }
+    with_width<T>(n.outputs, [&](auto width) {
+        constexpr int BN = decltype(width)::value;
+        Maps maps;
+        maps.a[0] = mh.map(kTileM);
+        maps.b[0] = md.map(BN);
+        Args g;
+        set_tiles(g, n.tokens, n.outputs, BN);
+        g.chunks[0] = tiles_of(n.hidden, kChunk);
+        g.out[0] = y;
+        g.pitch = n.outputs;
+        launch_product<Kind::kDown, BN, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+    });
+}
+
+template <class T>
+constexpr int kWeightBN = sizeof(T) == 4 ? 64 : 128;
+
+// The weight products' tiles and parts: as many parts as keep the SMs busy over whole waves, each
+// at least eight chunks (512 tokens) long.
+template <class T>
+void set_weight_tiles(Args& g, const MlpShape& n)
+{
+    const int rows[3] = {n.hidden, n.hidden, n.outputs};
+    const int cols[3] = {n.channels, n.channels, n.hidden};
+    g.first[0] = 0;
+    for (int p = 0; p < 3; ++p) {
+        g.rows_of[p] = rows[p];
+        g.cols_of[p] = cols[p];
+        g.n_tiles_of[p] = tiles_of(cols[p], kWeightBN<T>);
+        g.first[p + 1] = g.first[p] + static_cast<long long>(tiles_of(rows[p], kTileM)) * g.n_tiles_of[p];
+    }
+    const long long size = static_cast<long long>(n.hidden) * n.channels;
+    g.offset[0] = 0;
+    g.offset[1] = size;
+    g.offset[2] = 2 * size;
+    g.part_size = 2 * size + static_cast<long long>(n.outputs) * n.hidden;
+    g.chunks[0] = std::max(1, tiles_of(n.tokens, kChunk));  // no tokens: sized for, never launched
+    // A part of k chunks costs its tiles k units and an epilogue of about four.
+    double best = 0.0;
+    for (int parts = 1; parts <= 148 && (parts == 1 || g.chunks[0] / parts >= 8); ++parts) {
+        const int k = tiles_of(g.chunks[0], parts);
+        const long long waves = (g.first[3] * tiles_of(g.chunks[0], k) + 147) / 148;
+        const double cost = static_cast<double>(waves) * (k + 4);
+        if (parts == 1 || cost < 0.97 * best) {
+            best = cost;
+            g.parts = tiles_of(g.chunks[0], k);
+            g.part_chunks = k;
+        }
+    }
+    g.tiles = g.first[3] * g.parts;
+}
+
+template <class T>
+std::size_t backward_bytes(const MlpShape& n)
+{
+    Arena arena{nullptr};
+    arena.take(static_cast<std::size_t>(n.tokens) * n.channels * sizeof(T));  // x restored
+    arena.take(staged_bytes<T>(n.tokens, n.channels));
+    arena.take(staged_bytes<T>(n.tokens, n.outputs));
+    arena.take(staged_bytes<T>(n.hidden, n.channels));
+    arena.take(staged_bytes<T>(n.hidden, n.channels));
+    arena.take(staged_bytes<T>(n.outputs, n.hidden));
+    for (int i = 0; i < 3; ++i) {
+        hidden_matrix<T>(n, arena);
+    }
+    Args g;
+    set_weight_tiles<T>(g, n);
+    arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts);
+    return arena.used + 256;
+}
+
+template <class T>
+void mlp_backward(const void* dy, const void* x, const signed char* codes, const float* scales, const void* wg,
+                  const void* wu, const void* wd, void* dx, void* dwg, void* dwu, void* dwd, int dtype, const MlpShape& n,
+                  void* work, cudaStream_t stream)
+{
+    Arena arena{reinterpret_cast<unsigned char*>((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255})};
+    if (codes != nullptr) {
+        void* restored = arena.take(static_cast<std::size_t>(n.tokens) * n.channels * sizeof(T));
+        unpack8(codes, scales, restored, dtype, n.tokens, n.channels, stream);
+        x = restored;
+    }
+    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, stream);
+    const Matrix mdy = operand<T>(dy, n.tokens, n.outputs, arena, stream);
+    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, stream);
+    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, stream);
+    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, stream);
+    const Matrix mdg = hidden_matrix<T>(n, arena);
+    const Matrix mdu = hidden_matrix<T>(n, arena);
+    const Matrix mh = hidden_matrix<T>(n, arena);
+    {
+        constexpr int BN = 64;
+        Maps maps;
+        maps.a[0] = mx.map(kTileM);
+        maps.b[0] = mg.map(BN);
+        maps.b[1] = mu.map(BN);
+        maps.a[1] = mdy.map(kTileM);
+        maps.b[2] = md.map(kChunk);
+        Args g;
+        set_tiles(g, n.tokens, n.hidden, BN);
+        g.chunks[0] = tiles_of(n.channels, kChunk);
+        g.chunks[1] = tiles_of(n.outputs, kChunk);
+        g.out[0] = const_cast<void*>(mdg.base);
+        g.out[1] = const_cast<void*>(mdu.base);
+        g.out[2] = const_cast<void*>(mh.base);
+        g.pitch = mh.pitch;
+        g.plane = mh.rows * mh.pitch;
+        with_activation(n.act,
+                        [&](auto act) { launch_product<Kind::kGateBack, BN, T, decltype(act)::value>(maps, g, stream); });
+    }
+    with_width<T>(n.channels, [&](auto width) {
+        constexpr int BN = decltype(width)::value;
+        Maps maps;
+        maps.a[0] = mdg.map(kTileM);
+        maps.a[1] = mdu.map(kTileM);
+        maps.b[0] = mg.map(kChunk);
+        maps.b[1] = mu.map(kChunk);
+        Args g;
+        set_tiles(g, n.tokens, n.channels, BN);
+        g.chunks[0] = tiles_of(n.hidden, kChunk);
+        g.chunks[1] = g.chunks[0];
+        g.out[0] = dx;
+        g.pitch = n.channels;
+        launch_product<Kind::kInput, BN, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+    });
+    {
+        Maps maps;
+        maps.a[0] = mdg.map(kChunk);
+        maps.a[1] = mdu.map(kChunk);
+        maps.a[2] = mdy.map(kChunk);
+        maps.b[0] = mx.map(kChunk);
+        maps.b[1] = mx.map(kChunk);
+        maps.b[2] = mh.map(kChunk);
+        Args g;
+        set_weight_tiles<T>(g, n);
+        float* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts));
+        g.out[0] = partial;
+        launch_product<Kind::kWeight, kWeightBN<T>, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        const long long size0 = static_cast<long long>(n.hidden) * n.channels;
+        const long long size2 = static_cast<long long>(n.outputs) * n.hidden;
+        const unsigned grid = static_cast<unsigned>(std::min<long long>((g.part_size + 255) / 256, 148 * 8));
+        launch_pdl(weight_sum_kernel<T>, dim3(grid), dim3(256), 0, stream, static_cast<const float*>(partial),
+                   static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dwd), size0, size2, g.part_size, g.parts);
+    }
+}
+
+int invalid(const std::string& message)
+{
+    set_last_error(message);
+    return SPECTRAL_INVALID_ARGUMENT;
+}
+
+int check(const char* op, int dtype, long long tokens, int channels, int hidden, int outputs)
+{
+    const std::string name(op);
+    if (!dtype_known(dtype)) {
+        return invalid(name + ": dtype must be SPECTRAL_FLOAT32, SPECTRAL_BFLOAT16 or SPECTRAL_FLOAT16");
+    }
+    constexpr int kMost = 1 << 20;
+    if (tokens < 0 || tokens > kMaxTokens || channels < 1 || hidden < 1 || outputs < 1 || channels > kMost || hidden > kMost
+        || outputs > kMost) {
+        return invalid(name + ": need 0 <= tokens < 2^31 - 256 and channels, hidden and outputs from 1 to 2^20");
+    }
+    return SPECTRAL_OK;
+}
+
+bool overlap(const void* a, unsigned long long a_bytes, const void* b, unsigned long long b_bytes)
+{
+    const auto p = reinterpret_cast<unsigned long long>(a);
+    const auto q = reinterpret_cast<unsigned long long>(b);
+    return p < q + b_bytes && q < p + a_bytes;
+}
+
+}  // namespace
+}  // namespace spectral
+
+extern "C" int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs, size_t* count)
+{
+    using namespace spectral;
+    const int status = check("gated_mlp_workspace", dtype, tokens, channels, hidden, outputs);
+    if (status != SPECTRAL_OK || count == nullptr) {
+        return status != SPECTRAL_OK ? status : invalid("gated_mlp_workspace: null count");
+    }
+    const MlpShape n{tokens, channels, hidden, outputs, 0};
+    with_dtype(dtype, [&](auto t) { *count = (forward_bytes<decltype(t)>(n) + 7) / 8; });
+    return SPECTRAL_OK;
+}
+
+extern "C" int spectral_gated_mlp_backward_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
+                                                     size_t* count)
+{
+    using namespace spectral;
+    const int status = check("gated_mlp_backward_workspace", dtype, tokens, channels, hidden, outputs);
+    if (status != SPECTRAL_OK || count == nullptr) {
+        return status != SPECTRAL_OK ? status : invalid("gated_mlp_backward_workspace: null count");
+    }
+    const MlpShape n{tokens, channels, hidden, outputs, 0};
+    with_dtype(dtype, [&](auto t) { *count = (backward_bytes<decltype(t)>(n) + 7) / 8; });
+    return SPECTRAL_OK;
+}
+
+extern "C" int spectral_gated_mlp(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* y, int dtype,
+                                  long long tokens, int channels, int hidden, int outputs, int activation, void* work,
+                                  void* stream)
+{
+    using namespace spectral;
+    const int status = check("gated_mlp", dtype, tokens, channels, hidden, outputs);
+    if (status != SPECTRAL_OK) {
+        return status;
+    }
+    if (!activation_known(activation)) {
+        return invalid("gated_mlp: activation must be SPECTRAL_ACT_NONE, _SILU or _GELU");
+    }
+    if (tokens == 0) {
+        return SPECTRAL_OK;
+    }
+    if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || y == nullptr || work == nullptr) {
+        return invalid("gated_mlp: null array");
+    }
+    const std::size_t size = dtype_size(dtype);
+    for (const void* p : {x, w_gate, w_up, w_down, static_cast<const void*>(y)}) {
+        if (!aligned_to(p, size)) {
+            return invalid("gated_mlp: arrays must be aligned to their element size");
+        }
+    }
+    if (overlap(x, tokens * channels * size, y, tokens * outputs * size)) {
+        return invalid("gated_mlp: x and y must not overlap");
+    }
+    try {
+        const MlpShape n{tokens, channels, hidden, outputs, activation};
+        with_dtype(dtype, [&](auto t) {
+            mlp_forward<decltype(t)>(x, w_gate, w_up, w_down, y, n, work, static_cast<cudaStream_t>(stream));
+        });
+        return SPECTRAL_OK;
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return SPECTRAL_CUDA_ERROR;
+    }
+}
+
+extern "C" int spectral_gated_mlp_backward(const void* dy, const void* x, const void* codes, const float* scales,
+                                           const void* w_gate, const void* w_up, const void* w_down, void* dx,
+                                           void* dw_gate, void* dw_up, void* dw_down, int dtype, long long tokens,
+                                           int channels, int hidden, int outputs, int activation, void* work, void* stream)
+{
+    using namespace spectral;
+    const int status = check("gated_mlp_backward", dtype, tokens, channels, hidden, outputs);
+    if (status != SPECTRAL_OK) {
+        return status;
+    }
+    if (!activation_known(activation)) {
+        return invalid("gated_mlp_backward: activation must be SPECTRAL_ACT_NONE, _SILU or _GELU");
+    }
+    if (dw_gate == nullptr || dw_up == nullptr || dw_down == nullptr) {
+        return invalid("gated_mlp_backward: null array");
+    }
+    const std::size_t size = dtype_size(dtype);
+    const auto s = static_cast<cudaStream_t>(stream);
+    try {
+        if (tokens == 0) {  // sums over nothing
+            SPECTRAL_CUDA(cudaMemsetAsync(dw_gate, 0, size * hidden * channels, s));
+            SPECTRAL_CUDA(cudaMemsetAsync(dw_up, 0, size * hidden * channels, s));
+            SPECTRAL_CUDA(cudaMemsetAsync(dw_down, 0, size * outputs * hidden, s));
+            return SPECTRAL_OK;
+        }
+        if (dy == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || dx == nullptr || work == nullptr
+            || (x == nullptr) == (codes == nullptr) || (codes == nullptr) != (scales == nullptr)) {
+            return invalid("gated_mlp_backward: every array must be given, and either x or codes with scales");
+        }
+        for (const void* p : {dy, x, w_gate, w_up, w_down, static_cast<const void*>(dx), static_cast<const void*>(dw_gate),
+                              static_cast<const void*>(dw_up), static_cast<const void*>(dw_down)}) {
+            if (!aligned_to(p, size)) {
+                return invalid("gated_mlp_backward: arrays must be aligned to their element size");
+            }
+        }
+        if (overlap(dx, tokens * channels * size, dy, tokens * outputs * size)
+            || (x != nullptr && overlap(dx, tokens * channels * size, x, tokens * channels * size))) {
+            return invalid("gated_mlp_backward: dx must not overlap dy or x");
+        }
+        const MlpShape n{tokens, channels, hidden, outputs, activation};
+        with_dtype(dtype, [&](auto t) {
+            mlp_backward<decltype(t)>(dy, x, static_cast<const signed char*>(codes), scales, w_gate, w_up, w_down, dx,
+                                      dw_gate, dw_up, dw_down, dtype, n, work, s);
+        });
+        return SPECTRAL_OK;
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return SPECTRAL_CUDA_ERROR;
+    }
+}

@@ -23,6 +23,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <vector>
 
 namespace {
@@ -534,6 +535,308 @@ void flow_stage_cuda(const at::Tensor& x, const at::Tensor& w, at::Tensor& f0, a
                                      stream()));
 }
 
+// --- the pointwise half of an FNO block: additions of this library ------------------------------
+
+int dtype_code(const at::Tensor& t, const char* op, const char* name)
+{
+    TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be a CUDA tensor");
+    switch (t.scalar_type()) {
+        case at::kFloat: return SPECTRAL_FLOAT32;
+        case at::kBFloat16: return SPECTRAL_BFLOAT16;
+        case at::kHalf: return SPECTRAL_FLOAT16;
+        default: break;
+    }
+    TORCH_CHECK(false, op, ": ", name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+}
+
+int activation_code(c10::string_view activation, const char* op)
+{
+    if (activation == "none") {
+        return SPECTRAL_ACT_NONE;
+    }
+    if (activation == "silu") {
+        return SPECTRAL_ACT_SILU;
+    }
+    TORCH_CHECK(activation == "gelu", op, ": activation must be 'none', 'silu' or 'gelu', got '",
+                std::string(activation.data(), activation.size()), "'");
+    return SPECTRAL_ACT_GELU;
+}
+
+int small_int(int64_t v, const char* op, const char* name)
+{
+    TORCH_CHECK(v <= INT_MAX, op, ": ", name, " is too large: ", v);
+    return static_cast<int>(v);
+}
+
+// `t` must be of x's type and device.
+void check_like(const at::Tensor& t, const at::Tensor& x, const char* op, const char* name)
+{
+    TORCH_CHECK(t.is_cuda() && t.device() == x.device(), op, ": ", name, " must be on the device of x");
+    TORCH_CHECK(t.scalar_type() == x.scalar_type(), op, ": ", name, " must be ", x.scalar_type(), " as x, got ",
+                t.scalar_type());
+}
+
+// An optional per-channel parameter: `channels` float32 values, contiguous (undefined if not given).
+at::Tensor channel_parameter(const c10::optional<at::Tensor>& t, const at::Tensor& x, int64_t channels, const char* op,
+                             const char* name)
+{
+    if (!t.has_value() || !t->defined()) {
+        return at::Tensor();
+    }
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 1
+                    && t->size(0) == channels,
+                op, ": ", name, " must be a float32 tensor of ", channels, " values on the device of x");
+    return t->contiguous();
+}
+
+const float* fptr(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.const_data_ptr<float>() : nullptr; }
+
+std::vector<int64_t> scale_shape(const at::Tensor& x)
+{
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = (shape.back() + SPECTRAL_PACK8_BLOCK - 1) / SPECTRAL_PACK8_BLOCK;
+    return shape;
+}
+
+int64_t rows_of(const at::Tensor& x)
+{
+    int64_t rows = 1;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) {
+        rows *= x.size(d);
+    }
+    return rows;
+}
+
+// codes int8 of `like`'s shape with one float32 scale per row and block, contiguous.
+void check_packed(const at::Tensor& codes, const at::Tensor& scales, const char* op)
+{
+    TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() >= 1, op,
+                ": codes must be an int8 CUDA tensor with at least one dimension");
+    TORCH_CHECK(scales.is_cuda() && scales.device() == codes.device() && scales.scalar_type() == at::kFloat
+                    && scales.sizes() == at::IntArrayRef(scale_shape(codes)),
+                op, ": scales must be float32 of shape ", at::IntArrayRef(scale_shape(codes)), " on the device of codes");
+}
+
+std::tuple<at::Tensor, at::Tensor> pack8_cuda(const at::Tensor& x)
+{
+    const int dtype = dtype_code(x, "pack8", "x");
+    TORCH_CHECK(x.dim() >= 1, "pack8: x needs at least one dimension");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = x.contiguous();
+    at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    at::Tensor scales = at::empty(scale_shape(x), x.options().dtype(at::kFloat));
+    check_status(spectral_pack8(cptr(xc), dtype, mptr(codes), static_cast<float*>(mptr(scales)), rows_of(x),
+                                small_int(x.size(-1), "pack8", "the last dimension"), stream()));
+    return {codes, scales};
+}
+
+at::Tensor unpack8_cuda(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype)
+{
+    check_packed(codes, scales, "unpack8");
+    const c10::cuda::CUDAGuard guard(codes.device());
+    at::Tensor x = at::empty(codes.sizes(), codes.options().dtype(dtype));
+    const int code = dtype_code(x, "unpack8", "the result");
+    const at::Tensor cc = codes.contiguous();
+    const at::Tensor sc = scales.contiguous();
+    check_status(spectral_unpack8(cptr(cc), fptr(sc), mptr(x), code, rows_of(codes),
+                                  small_int(codes.size(-1), "unpack8", "the last dimension"), stream()));
+    return x;
+}
+
+struct NormSizes {
+    int64_t batch;
+    int64_t points;
+    int channels;
+    int groups;
+};
+
+NormSizes norm_sizes(const at::Tensor& x, int64_t groups, const char* op)
+{
+    TORCH_CHECK(x.dim() >= 2, op, ": x must be (batch, ..., channels)");
+    NormSizes s{x.size(0), 1, small_int(x.size(-1), op, "the number of channels"), small_int(groups, op, "groups")};
+    for (int64_t d = 1; d + 1 < x.dim(); ++d) {
+        s.points *= x.size(d);
+    }
+    TORCH_CHECK(groups >= 1 && s.channels >= 1 && s.channels % groups == 0, op, ": groups must divide the number of channels, got ",
+                groups, " groups of ", s.channels, " channels");
+    return s;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                    const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation, bool keep8)
+{
+    constexpr const char* op = "group_norm_act";
+    const int dtype = dtype_code(x, op, "x");
+    const NormSizes n = norm_sizes(x, groups, op);
+    const int act = activation_code(activation, op);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor w = channel_parameter(weight, x, n.channels, op, "weight");
+    const at::Tensor b = channel_parameter(bias, x, n.channels, op, "bias");
+    const at::Tensor xc = x.contiguous();
+    at::Tensor y = at::empty(x.sizes(), x.options());
+    at::Tensor mean = at::empty({n.batch, groups}, x.options().dtype(at::kFloat));
+    at::Tensor rstd = at::empty_like(mean);
+    at::Tensor codes = at::empty(keep8 ? x.sizes() : at::IntArrayRef({0}), x.options().dtype(at::kChar));
+    at::Tensor scales = at::empty(keep8 ? scale_shape(x) : std::vector<int64_t>{0}, x.options().dtype(at::kFloat));
+    if (x.numel() == 0) {
+        mean.zero_();
+        rstd.zero_();
+        return {y, mean, rstd, codes, scales};
+    }
+    size_t count = 0;
+    check_status(spectral_group_norm_act_workspace(n.batch, n.channels, n.groups, &count));
+    at::Tensor work = workspace(count, x);
+    check_status(spectral_group_norm_act(cptr(xc), fptr(w), fptr(b), mptr(y), static_cast<float*>(mptr(mean)),
+                                         static_cast<float*>(mptr(rstd)), keep8 ? mptr(codes) : nullptr,
+                                         keep8 ? static_cast<float*>(mptr(scales)) : nullptr, dtype, n.batch, n.points,
+                                         n.channels, n.groups, static_cast<float>(eps), act, mptr(work), stream()));
+    return {y, mean, rstd, codes, scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x,
+                             const c10::optional<at::Tensor>& codes, const c10::optional<at::Tensor>& scales,
+                             const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
+                             const at::Tensor& mean, const at::Tensor& rstd, int64_t groups, c10::string_view activation)
+{
+    constexpr const char* op = "group_norm_act_backward";
+    const int dtype = dtype_code(dy, op, "dy");
+    const NormSizes n = norm_sizes(dy, groups, op);
+    const int act = activation_code(activation, op);
+    TORCH_CHECK(x.has_value() != codes.has_value() && codes.has_value() == scales.has_value(), op,
+                ": needs either x or codes with scales");
+    const c10::cuda::CUDAGuard guard(dy.device());
+    at::Tensor xc;
+    at::Tensor cc;
+    at::Tensor sc;
+    if (x.has_value()) {
+        check_like(*x, dy, op, "x");
+        TORCH_CHECK(x->sizes() == dy.sizes(), op, ": x and dy must have one shape");
+        xc = x->contiguous();
+    } else {
+        check_packed(*codes, *scales, op);
+        TORCH_CHECK(codes->device() == dy.device() && codes->sizes() == dy.sizes(), op,
+                    ": codes must have the shape and device of dy");
+        cc = codes->contiguous();
+        sc = scales->contiguous();
+    }
+    for (const at::Tensor* t : {&mean, &rstd}) {
+        TORCH_CHECK(t->is_cuda() && t->device() == dy.device() && t->scalar_type() == at::kFloat && t->dim() == 2
+                        && t->size(0) == n.batch && t->size(1) == groups && t->is_contiguous(),
+                    op, ": mean and rstd must be contiguous float32 (batch, groups) on the device of dy");
+    }
+    const at::Tensor w = channel_parameter(weight, dy, n.channels, op, "weight");
+    const at::Tensor b = channel_parameter(bias, dy, n.channels, op, "bias");
+    const at::Tensor dyc = dy.contiguous();
+    at::Tensor dx = at::empty(dy.sizes(), dy.options());
+    at::Tensor dweight = at::empty({n.channels}, dy.options().dtype(at::kFloat));
+    at::Tensor dbias = at::empty_like(dweight);
+    size_t count = 0;
+    check_status(spectral_group_norm_act_backward_workspace(n.batch, n.channels, n.groups, &count));
+    at::Tensor work = workspace(count, dy);
+    check_status(spectral_group_norm_act_backward(
+        cptr(dyc), xc.defined() ? cptr(xc) : nullptr, cc.defined() ? cptr(cc) : nullptr, fptr(sc), fptr(w), fptr(b),
+        fptr(mean), fptr(rstd), mptr(dx), static_cast<float*>(mptr(dweight)), static_cast<float*>(mptr(dbias)), dtype,
+        n.batch, n.points, n.channels, n.groups, act, mptr(work), stream()));
+    return {dx, dweight, dbias};
+}
+
+struct MlpSizes {
+    int64_t tokens;
+    int channels;
+    int hidden;
+    int outputs;
+};
+
+// x is (..., channels); its rows are the tokens.
+MlpSizes mlp_sizes(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, const at::Tensor& w_down,
+                   const char* op)
+{
+    TORCH_CHECK(x.dim() >= 1, op, ": x needs at least one dimension");
+    TORCH_CHECK(w_gate.dim() == 2 && w_up.dim() == 2 && w_down.dim() == 2, op, ": the weights must be matrices");
+    TORCH_CHECK(w_gate.size(1) == x.size(-1) && w_up.sizes() == w_gate.sizes() && w_down.size(1) == w_gate.size(0), op,
+                ": x (..., channels), w_gate and w_up (hidden, channels) and w_down (outputs, hidden) do not match: ",
+                x.sizes(), ", ", w_gate.sizes(), ", ", w_up.sizes(), ", ", w_down.sizes());
+    return {rows_of(x), small_int(x.size(-1), op, "the number of channels"), small_int(w_gate.size(0), op, "hidden"),
+            small_int(w_down.size(0), op, "outputs")};
+}
+
+at::Tensor gated_mlp_cuda(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, const at::Tensor& w_down,
+                          c10::string_view activation)
+{
+    constexpr const char* op = "gated_mlp";
+    const int dtype = dtype_code(x, op, "x");
+    check_like(w_gate, x, op, "w_gate");
+    check_like(w_up, x, op, "w_up");
+    check_like(w_down, x, op, "w_down");
+    const MlpSizes n = mlp_sizes(x, w_gate, w_up, w_down, op);
+    const int act = activation_code(activation, op);
+    const c10::cuda::CUDAGuard guard(x.device());
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = n.outputs;
+    at::Tensor y = at::empty(shape, x.options());
+    const at::Tensor xc = x.contiguous();
+    const at::Tensor wg = w_gate.contiguous();
+    const at::Tensor wu = w_up.contiguous();
+    const at::Tensor wd = w_down.contiguous();
+    size_t count = 0;
+    check_status(spectral_gated_mlp_workspace(dtype, n.tokens, n.channels, n.hidden, n.outputs, &count));
+    at::Tensor work = workspace(count, x);
+    check_status(spectral_gated_mlp(cptr(xc), cptr(wg), cptr(wu), cptr(wd), mptr(y), dtype, n.tokens, n.channels, n.hidden,
+                                    n.outputs, act, mptr(work), stream()));
+    return y;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+gated_mlp_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x, const c10::optional<at::Tensor>& codes,
+                        const c10::optional<at::Tensor>& scales, const at::Tensor& w_gate, const at::Tensor& w_up,
+                        const at::Tensor& w_down, c10::string_view activation)
+{
+    constexpr const char* op = "gated_mlp_backward";
+    const int dtype = dtype_code(dy, op, "dy");
+    TORCH_CHECK(x.has_value() != codes.has_value() && codes.has_value() == scales.has_value(), op,
+                ": needs either x or codes with scales");
+    check_like(w_gate, dy, op, "w_gate");
+    check_like(w_up, dy, op, "w_up");
+    check_like(w_down, dy, op, "w_down");
+    const c10::cuda::CUDAGuard guard(dy.device());
+    at::Tensor xc;
+    at::Tensor cc;
+    at::Tensor sc;
+    if (x.has_value()) {
+        check_like(*x, dy, op, "x");
+        xc = x->contiguous();
+    } else {
+        check_packed(*codes, *scales, op);
+        TORCH_CHECK(codes->device() == dy.device(), op, ": codes must be on the device of dy");
+        cc = codes->contiguous();
+        sc = scales->contiguous();
+    }
+    const at::Tensor& input = x.has_value() ? *x : *codes;
+    const MlpSizes n = mlp_sizes(input, w_gate, w_up, w_down, op);
+    std::vector<int64_t> shape = input.sizes().vec();
+    shape.back() = n.outputs;
+    TORCH_CHECK(dy.sizes() == at::IntArrayRef(shape), op, ": dy must be ", at::IntArrayRef(shape), ", got ", dy.sizes());
+    const int act = activation_code(activation, op);
+    const at::Tensor dyc = dy.contiguous();
+    const at::Tensor wg = w_gate.contiguous();
+    const at::Tensor wu = w_up.contiguous();
+    const at::Tensor wd = w_down.contiguous();
+    at::Tensor dx = at::empty(input.sizes(), dy.options());
+    at::Tensor dwg = at::empty(wg.sizes(), dy.options());
+    at::Tensor dwu = at::empty(wg.sizes(), dy.options());
+    at::Tensor dwd = at::empty(wd.sizes(), dy.options());
+    size_t count = 0;
+    check_status(spectral_gated_mlp_backward_workspace(dtype, n.tokens, n.channels, n.hidden, n.outputs, &count));
+    at::Tensor work = workspace(count, dy);
+    check_status(spectral_gated_mlp_backward(cptr(dyc), xc.defined() ? cptr(xc) : nullptr, cc.defined() ? cptr(cc) : nullptr,
+                                             fptr(sc), cptr(wg), cptr(wu), cptr(wd), mptr(dx), mptr(dwg), mptr(dwu),
+                                             mptr(dwd), dtype, n.tokens, n.channels, n.hidden, n.outputs, act, mptr(work),
+                                             stream()));
+    return {dx, dwg, dwu, dwd};
+}
+
 // spectral._C.fft_impls(): the registry's names, in order, as a tuple of str.
 PyObject* py_fft_impls(PyObject*, PyObject*)
 {
@@ -581,6 +884,15 @@ TORCH_LIBRARY(spectral, m)
     m.def("flow_stage(Tensor x, Tensor w, Tensor(a!) f0, Tensor(b!) out, Tensor derive, Tensor forcing, Tensor mask,"
           " Tensor explicit_factor, Tensor implicit_factor, Tensor(c!) work, int n, int m, float dt, int stage,"
           " str impl=\"stockham_r8\") -> ()");
+    m.def("pack8(Tensor x) -> (Tensor, Tensor)");
+    m.def("unpack8(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
+    m.def("group_norm_act(Tensor x, int groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-5,"
+          " str activation=\"none\", bool keep8=False) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("group_norm_act_backward(Tensor dy, Tensor? x, Tensor? codes, Tensor? scales, Tensor? weight, Tensor? bias,"
+          " Tensor mean, Tensor rstd, int groups, str activation) -> (Tensor, Tensor, Tensor)");
+    m.def("gated_mlp(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation=\"silu\") -> Tensor");
+    m.def("gated_mlp_backward(Tensor dy, Tensor? x, Tensor? codes, Tensor? scales, Tensor w_gate, Tensor w_up,"
+          " Tensor w_down, str activation) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(spectral, CUDA, m)
@@ -599,6 +911,12 @@ TORCH_LIBRARY_IMPL(spectral, CUDA, m)
     m.impl("spectrum_frames", &spectrum_frames_cuda);
     m.impl("fir_overlap_save", &fir_overlap_save_cuda);
     m.impl("flow_stage", &flow_stage_cuda);
+    m.impl("pack8", &pack8_cuda);
+    m.impl("unpack8", &unpack8_cuda);
+    m.impl("group_norm_act", &group_norm_act_cuda);
+    m.impl("group_norm_act_backward", &group_norm_act_backward_cuda);
+    m.impl("gated_mlp", &gated_mlp_cuda);
+    m.impl("gated_mlp_backward", &gated_mlp_backward_cuda);
 }
 
 PyMODINIT_FUNC PyInit__C(void)

@@ -18,6 +18,7 @@ except ImportError as exc:  # pragma: no cover - exercised only on an unbuilt ch
 from . import nn
 from .ops import (
     FFT_IMPLS,
+    PACK8_BLOCK,
     fft2,
     fft_c2c,
     fft_truncated,
@@ -26,14 +27,17 @@ from .ops import (
     irfft2,
     irfft2_from_modes,
     mode_contract,
+    pack8,
     rfft,
     rfft2,
     rfft2_truncated,
     scale,
+    unpack8,
 )
 
 __all__ = [
     "FFT_IMPLS",
+    "PACK8_BLOCK",
     "fft2",
     "fft_c2c",
     "fft_truncated",
@@ -42,8 +46,10 @@ __all__ = [
     "irfft2",
     "irfft2_from_modes",
     "mode_contract",
+    "pack8",
     "rfft",
     "rfft2",
     "rfft2_truncated",
     "scale",
+    "unpack8",
 ]

@@ -79,6 +79,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spectral_ipc_free": (_i, [_p]),
     "spectral_mode_contract": (_i, [_p, _p, _p, _ll, _i, _i, _ll, _p]),
     "spectral_mode_contract_method": (_i, [_p, _p, _p, _ll, _i, _i, _ll, _i, _p]),
+    "spectral_pack8": (_i, [_p, _i, _p, _p, _ll, _i, _p]),
+    "spectral_unpack8": (_i, [_p, _p, _p, _i, _ll, _i, _p]),
+    "spectral_group_norm_act_workspace": (_i, [_ll, _i, _i, _szp]),
+    "spectral_group_norm_act": (_i, [_p] * 8 + [_i, _ll, _ll, _i, _i, _f, _i, _p, _p]),
+    "spectral_group_norm_act_backward_workspace": (_i, [_ll, _i, _i, _szp]),
+    "spectral_group_norm_act_backward": (_i, [_p] * 11 + [_i, _ll, _ll, _i, _i, _i, _p, _p]),
+    "spectral_gated_mlp_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),
+    "spectral_gated_mlp": (_i, [_p] * 5 + [_i, _ll, _i, _i, _i, _i, _p, _p]),
+    "spectral_gated_mlp_backward_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),
+    "spectral_gated_mlp_backward": (_i, [_p] * 11 + [_i, _ll, _i, _i, _i, _i, _p, _p]),
     "spectral_fp32_ceiling": (_i, [_p, _i, _i, _p, ctypes.POINTER(ctypes.c_double)]),
     "spectral_spectrum": (_i, [_s, _p, _p, _p, _ll, _i, _ll, _p]),
     "spectral_fir": (_i, [_s, _p, _p, _p, _ll, _i, _i, _ll, _p]),

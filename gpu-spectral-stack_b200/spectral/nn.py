@@ -1,5 +1,8 @@
-"""SpectralConv2d: the Fourier-neural-operator spectral convolution layer on this library's
-kernels, with a hand-derived backward.
+"""Layers of a Fourier neural operator on this library's kernels, with hand-derived backwards:
+SpectralConv2d, the spectral convolution, and the pointwise half of an FNO block around it
+(GroupNormAct, GatedMLP, and FNOBlock, which joins the three).
+
+SpectralConv2d.
 
 The reference plans this layer (docs/ROADMAP.md:71-76, tasks 3.4-3.6) on top of its pruned
 transforms but has no implementation. Forward, for real fields u of shape (b, c_in, n1, n2):
@@ -21,6 +24,11 @@ Backward (gradients in torch's convention for complex tensors, dL/dRe + i dL/dIm
 
 Every transform and contraction runs on this library's CUDA kernels; torch supplies only the
 transposes, conjugations and per-column weights.
+
+The pointwise half (additions of this library) works on channels-last fields (b, ..., c), float32,
+bfloat16 or float16. Each layer keeps only its input for the backward pass; with checkpoint8=True
+it keeps that input in 8 bits (ops.pack8), a half or a quarter of the memory, and the gradients
+are those at the restored input.
 """
 
 from __future__ import annotations
@@ -109,3 +117,135 @@ class SpectralConv2d(torch.nn.Module):
 
     def extra_repr(self) -> str:
         return f"{self.in_channels}, {self.out_channels}, m1={self.m1}, m2={self.m2}, impl={self.impl!r}"
+
+
+def _wants_grad(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _GroupNormActFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups: int, eps: float, activation: str, checkpoint8: bool):
+        y, mean, rstd, codes, scales = torch.ops.spectral.group_norm_act.default(
+            x, groups, weight, bias, eps, activation, checkpoint8)
+        kept = (codes, scales) if checkpoint8 else (x,)
+        ctx.save_for_backward(weight, bias, mean, rstd, *kept)
+        ctx.groups, ctx.activation = groups, activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad: torch.Tensor):
+        weight, bias, mean, rstd, *kept = ctx.saved_tensors
+        x, codes, scales = (None, *kept) if len(kept) == 2 else (kept[0], None, None)
+        dx, dweight, dbias = torch.ops.spectral.group_norm_act_backward.default(
+            grad, x, codes, scales, weight, bias, mean, rstd, ctx.groups, ctx.activation)
+        return (dx, dweight if weight is not None else None, dbias if bias is not None else None,
+                None, None, None, None)
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, *, eps: float = 1e-5, activation: str = "none",
+                   checkpoint8: bool = False) -> torch.Tensor:
+    """act(group_norm(x) * weight + bias) over channels-last fields: x (b, ..., c), statistics per
+    sample and group of c / groups channels over all points; weight and bias float32 (c,) or None;
+    activation "none", "silu" or "gelu" (the exact one). Returns a contiguous tensor of x's type.
+    Differentiable in x, weight and bias; checkpoint8=True keeps x for that in 8 bits."""
+    if _wants_grad(x, weight, bias):
+        return _GroupNormActFunction.apply(x, weight, bias, groups, eps, activation, checkpoint8)
+    return torch.ops.spectral.group_norm_act.default(x, groups, weight, bias, eps, activation, False)[0]
+
+
+class _GatedMLPFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation: str, checkpoint8: bool):
+        y = torch.ops.spectral.gated_mlp.default(x, w_gate, w_up, w_down, activation)
+        kept = torch.ops.spectral.pack8.default(x) if checkpoint8 else (x,)
+        ctx.save_for_backward(w_gate, w_up, w_down, *kept)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad: torch.Tensor):
+        w_gate, w_up, w_down, *kept = ctx.saved_tensors
+        x, codes, scales = (None, *kept) if len(kept) == 2 else (kept[0], None, None)
+        grads = torch.ops.spectral.gated_mlp_backward.default(
+            grad, x, codes, scales, w_gate, w_up, w_down, ctx.activation)
+        return (*grads, None, None)
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
+              activation: str = "silu", checkpoint8: bool = False) -> torch.Tensor:
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T over the last dimension of x (..., channels): w_gate
+    and w_up (hidden, channels), w_down (outputs, hidden), all of x's type. Differentiable in all
+    four; only x is kept for that (in 8 bits with checkpoint8=True), the hidden values are
+    recomputed."""
+    if _wants_grad(x, w_gate, w_up, w_down):
+        return _GatedMLPFunction.apply(x, w_gate, w_up, w_down, activation, checkpoint8)
+    return torch.ops.spectral.gated_mlp.default(x, w_gate, w_up, w_down, activation)
+
+
+class GroupNormAct(torch.nn.Module):
+    """Group norm with learned scale and offset per channel, then the activation, on channels-last
+    fields (group_norm_act)."""
+
+    def __init__(self, groups: int, channels: int, *, eps: float = 1e-5, activation: str = "gelu",
+                 checkpoint8: bool = False, device=None):
+        super().__init__()
+        self.groups, self.channels, self.eps = groups, channels, eps
+        self.activation, self.checkpoint8 = activation, checkpoint8
+        self.weight = torch.nn.Parameter(torch.ones(channels, device=device))
+        self.bias = torch.nn.Parameter(torch.zeros(channels, device=device))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return group_norm_act(x, self.groups, self.weight, self.bias, eps=self.eps, activation=self.activation,
+                              checkpoint8=self.checkpoint8)
+
+    def extra_repr(self) -> str:
+        return f"{self.groups}, {self.channels}, activation={self.activation!r}, checkpoint8={self.checkpoint8}"
+
+
+class GatedMLP(torch.nn.Module):
+    """The gated feed-forward block (gated_mlp) with learned weights, which start iid N(0, 1 / fan-in)."""
+
+    def __init__(self, channels: int, hidden: int, outputs: int | None = None, *, activation: str = "gelu",
+                 checkpoint8: bool = False, device=None, dtype=None):
+        super().__init__()
+        outputs = channels if outputs is None else outputs
+        self.activation, self.checkpoint8 = activation, checkpoint8
+
+        def weight(rows: int, cols: int) -> torch.nn.Parameter:
+            return torch.nn.Parameter(torch.randn(rows, cols, device=device, dtype=dtype) / math.sqrt(max(1, cols)))
+
+        self.w_gate, self.w_up, self.w_down = weight(hidden, channels), weight(hidden, channels), weight(outputs, hidden)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return gated_mlp(x, self.w_gate, self.w_up, self.w_down, activation=self.activation,
+                         checkpoint8=self.checkpoint8)
+
+    def extra_repr(self) -> str:
+        hidden, channels = self.w_gate.shape
+        return (f"{channels}, {hidden}, {self.w_down.shape[0]}, activation={self.activation!r}, "
+                f"checkpoint8={self.checkpoint8}")
+
+
+class FNOBlock(torch.nn.Module):
+    """One Fourier-neural-operator block on real fields u (b, channels, n1, n2), float32:
+
+        v = SpectralConv2d(u) as channels-last fields, in `dtype`
+        out = u + GatedMLP(GroupNormAct(v)), channels first again, float32
+
+    `dtype` is the pointwise half's type; checkpoint8=True keeps its two inputs in 8 bits."""
+
+    def __init__(self, channels: int, hidden: int, m1: int, m2: int, *, groups: int = 8, activation: str = "gelu",
+                 checkpoint8: bool = False, impl: str = "stockham_r8", device=None, dtype: torch.dtype = torch.float32):
+        super().__init__()
+        self.conv = SpectralConv2d(channels, channels, m1, m2, impl=impl, device=device)
+        self.norm = GroupNormAct(groups, channels, activation=activation, checkpoint8=checkpoint8, device=device)
+        self.mlp = GatedMLP(channels, hidden, activation=activation, checkpoint8=checkpoint8, device=device, dtype=dtype)
+        self.dtype = dtype
+
+    def forward(self, u: torch.Tensor) -> torch.Tensor:
+        v = self.conv(u).permute(0, 2, 3, 1).to(self.dtype)
+        return u + self.mlp(self.norm(v)).permute(0, 3, 1, 2).to(u.dtype)

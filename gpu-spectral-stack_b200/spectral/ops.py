@@ -96,3 +96,22 @@ def mode_contract(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     (batch, cin, *modes), w is (cin, cout, *modes). An addition of this library: the reference
     plans this step (its ROADMAP tasks 3.3-3.6) but does not implement it."""
     return torch.ops.spectral.mode_contract.default(x, w)
+
+
+# 8-bit activation checkpoints (an addition of this library): one byte per value and one float32
+# scale per block of PACK8_BLOCK values along the last dimension.
+
+PACK8_BLOCK = 64
+
+
+def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The 8-bit checkpoint of a float32, bfloat16 or float16 CUDA tensor: (codes, scales), int8
+    of x's shape and float32 of x's shape with the last dimension in blocks of 64. Per block, with
+    m = max(|v|, 2^-100): scale = m / 127, code = round(v * (127 / m)), restored as code * scale,
+    off by at most half a scale. A block with an infinity or NaN restores as NaN."""
+    return torch.ops.spectral.pack8.default(x)
+
+
+def unpack8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values a pack8 checkpoint stands for, as a new tensor of `dtype`."""
+    return torch.ops.spectral.unpack8.default(codes, scales, dtype)

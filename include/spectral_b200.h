@@ -305,6 +305,75 @@ SPECTRAL_API int spectral_mode_contract(const void* x, const void* w, void* out,
 SPECTRAL_API int spectral_mode_contract_method(const void* x, const void* w, void* out, long long batch,
                                                int cin, int cout, long long modes, int method, void* stream);
 
+/* --- the pointwise half of an FNO block -------------------------------------------------------- */
+/* Around its spectral convolution an FNO block normalises its fields, mixes their channels point
+ * by point, and keeps activations for the backward pass. No counterparts in the reference. Arrays
+ * are contiguous and channels last; values are one of three types, sums are FP32. Workspaces
+ * are in complex values (8 bytes), as everywhere in this header, and 8-byte aligned. */
+#define SPECTRAL_FLOAT32 0
+#define SPECTRAL_BFLOAT16 1
+#define SPECTRAL_FLOAT16 2
+#define SPECTRAL_ACT_NONE 0
+#define SPECTRAL_ACT_SILU 1 /* z / (1 + exp(-z)) */
+#define SPECTRAL_ACT_GELU 2 /* z Phi(z), Phi the normal distribution function */
+
+/* 8-bit activation checkpoints. Each of `rows` rows of `width` values is cut into blocks of
+ * SPECTRAL_PACK8_BLOCK values (the last may be shorter). With m = max(|v|, 2^-100) over a block,
+ *   scale = m / 127,  code = round(v * (127 / m)) to nearest, ties to even,  value = code * scale
+ * (each operation in FP32, the value at most the largest float), so a restored value is off by at
+ * most half a scale. A block with an
+ * infinity or NaN restores as NaN throughout. codes: rows x width int8; scales: rows x
+ * ceil(width / 64) floats. spectral_unpack8 writes the values in `dtype`. */
+#define SPECTRAL_PACK8_BLOCK 64
+SPECTRAL_API int spectral_pack8(const void* x, int dtype, void* codes, float* scales, long long rows, int width,
+                                void* stream);
+SPECTRAL_API int spectral_unpack8(const void* codes, const float* scales, void* x, int dtype, long long rows,
+                                  int width, void* stream);
+
+/* Group norm with an activation: x and y (batch, points, channels),
+ *   y = act((x - mean) rstd weight + bias),  rstd = 1 / sqrt(var + eps),
+ * mean and var (biased) per sample over the points x (channels / groups) values of each group.
+ * weight and bias: `channels` floats, or NULL for 1 and 0. mean and rstd (batch x groups floats)
+ * receive the statistics for the backward pass; both may be NULL. codes and scales (both or
+ * neither) receive x's 8-bit checkpoint (rows of `channels`). x and y must not overlap. */
+SPECTRAL_API int spectral_group_norm_act_workspace(long long batch, int channels, int groups, size_t* count);
+SPECTRAL_API int spectral_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean,
+                                         float* rstd, void* codes, float* scales, int dtype, long long batch,
+                                         long long points, int channels, int groups, float eps, int activation,
+                                         void* work, void* stream);
+/* Its gradients for the upstream gradient dy, from the forward call's mean and rstd and either x
+ * or its checkpoint (codes and scales, x NULL): dx, and dweight and dbias (`channels` floats each;
+ * either may be NULL). Every sum has a fixed order: equal inputs give equal bits. */
+SPECTRAL_API int spectral_group_norm_act_backward_workspace(long long batch, int channels, int groups,
+                                                            size_t* count);
+SPECTRAL_API int spectral_group_norm_act_backward(const void* dy, const void* x, const void* codes,
+                                                  const float* scales, const float* weight, const float* bias,
+                                                  const float* mean, const float* rstd, void* dx, float* dweight,
+                                                  float* dbias, int dtype, long long batch, long long points,
+                                                  int channels, int groups, int activation, void* work,
+                                                  void* stream);
+
+/* The gated feed-forward block on `tokens` rows:
+ *   y = (act(x w_gate^T) * (x w_up^T)) w_down^T
+ * x (tokens, channels), w_gate and w_up (hidden, channels), w_down (outputs, hidden),
+ * y (tokens, outputs), all of `dtype`. Products run on the tensor cores with FP32 accumulators;
+ * FP32 operands are split into three bf16 parts (FP32-level error). */
+SPECTRAL_API int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
+                                              size_t* count);
+SPECTRAL_API int spectral_gated_mlp(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* y,
+                                    int dtype, long long tokens, int channels, int hidden, int outputs,
+                                    int activation, void* work, void* stream);
+/* Its gradients for dy (tokens, outputs), from x or its 8-bit checkpoint (codes and scales, x NULL):
+ * dx (tokens, channels) and the three weights' gradients, of `dtype` and of their arrays' shapes.
+ * The products of the forward pass are recomputed, nothing but x is kept. Fixed summation order. */
+SPECTRAL_API int spectral_gated_mlp_backward_workspace(int dtype, long long tokens, int channels, int hidden,
+                                                       int outputs, size_t* count);
+SPECTRAL_API int spectral_gated_mlp_backward(const void* dy, const void* x, const void* codes, const float* scales,
+                                             const void* w_gate, const void* w_up, const void* w_down, void* dx,
+                                             void* dw_gate, void* dw_up, void* dw_down, int dtype, long long tokens,
+                                             int channels, int hidden, int outputs, int activation, void* work,
+                                             void* stream);
+
 /* The FP32 arithmetic ceiling, for the roofline of FP32-bound kernels such as the contraction
  * (reference: csrc/tools/peaks.cu:46-70, a separate tool there). Launches one full wave of CTAs
  * that run independent fused multiply-add chains and nothing else: scalar FFMA (packed == 0) or

@@ -1,0 +1,332 @@
+"""The gated feed-forward block: values and all gradients against the formula in float64
+(differentiated by torch's autograd), over types, sizes that are no multiple of a tile, one token to
+many, unaligned and strided operands, 8-bit checkpoints, non-finite values; against differences;
+and the refusals; and FNOBlock, which runs the pointwise operators around the spectral convolution.
+
+Tolerances, relative to the result's norm. 16-bit types round the hidden values and the result
+once each. Over many values a rounding is 2^-9 (bf16) or 2^-12 (f16) of the norm or less, so twice
+that bounds both; a result of a few values has to allow the worst case of each, 2^-8 or 2^-11, and
+f16's subnormal unit 2^-24. float32 products accumulate passes of 128 values, cut at 2^-23 per 16 of them: at most
+8 x 2^-23 a product, and a result is a chain of at most three."""
+
+import math
+
+import pytest
+import torch
+
+import spectral
+from spectral import native
+from spectral.nn import FNOBlock, GatedMLP, gated_mlp
+
+TOL = {torch.float32: 24 * 2.0 ** -23, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DTYPES = list(TOL)
+
+
+def act64(z, activation):
+    if activation == "silu":
+        return z * torch.sigmoid(z)
+    if activation == "gelu":
+        return 0.5 * z * (1.0 + torch.erf(z / math.sqrt(2.0)))
+    return z
+
+
+def formula(x, w_gate, w_up, w_down, activation):
+    return (act64(x @ w_gate.T, activation) * (x @ w_up.T)) @ w_down.T
+
+
+def inputs(tokens, channels, hidden, outputs, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + tokens + 7 * channels + 11 * hidden)
+    shapes = [(tokens, channels), (hidden, channels), (hidden, channels), (outputs, hidden), (tokens, outputs)]
+    scale = [1.0, channels ** -0.5, channels ** -0.5, hidden ** -0.5, 1.0]
+    return [(torch.randn(*s, generator=g) * k).to(dtype).cuda() for s, k in zip(shapes, scale)]
+
+
+def close(got, want, tol, name=""):
+    dtype, few = got.dtype, got.numel() < 16
+    got, want = got.detach().double(), want.detach().double()
+    err, size = float((got - want).norm()), float(want.norm())
+    least = 0.0
+    if few and dtype != torch.float32:
+        tol, least = 2 * tol, 2.0 ** -22 if dtype == torch.float16 else 0.0
+    assert err <= tol * size + least, f"{name}: {err / max(size, 1e-300):.3g} > {tol:.3g}"
+
+
+# tokens, channels, hidden, outputs: one of everything; the few-token form and its edge; sizes around
+# the tiles of 64, 128 and 256; unlike inputs and outputs; rows that are no 16-byte pieces.
+SIZES = [(1, 1, 1, 1), (1, 64, 128, 64), (3, 50, 33, 70), (8, 512, 96, 200), (9, 64, 64, 64), (17, 24, 40, 8),
+         (128, 64, 128, 64), (129, 65, 127, 33), (200, 130, 300, 129), (1000, 100, 270, 100), (513, 256, 512, 257),
+         (300, 64, 1024, 320), (2048, 16, 16, 16), (640, 520, 72, 264)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["none", "silu", "gelu"])
+@pytest.mark.parametrize(("tokens", "channels", "hidden", "outputs"), SIZES)
+def test_values_and_gradients(tokens, channels, hidden, outputs, activation, dtype):
+    *args, dy = inputs(tokens, channels, hidden, outputs, dtype)
+    want_y = formula(*[a.double() for a in args], activation)
+    close(gated_mlp(*args, activation=activation), want_y, TOL[dtype], "y without gradients")
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    y = gated_mlp(*leaves, activation=activation)
+    assert y.dtype == dtype and y.shape == (tokens, outputs)
+    got = torch.autograd.grad(y, leaves, dy)
+    ref = [a.double().requires_grad_(True) for a in args]
+    want = torch.autograd.grad(formula(*ref, activation), ref, dy.double())
+    close(y, want_y, TOL[dtype], "y")
+    # dx adds two products and the gate's slope may cancel against 1: bounded by the two parts' norms.
+    for name, g, w in zip(("dx", "dw_gate", "dw_up", "dw_down"), got, want):
+        assert g.dtype == dtype and g.shape == w.shape
+        close(g, w, TOL[dtype] * (2 if name == "dx" and channels * hidden < 64 else 1), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "channels", "hidden", "outputs"), [(5, 64, 96, 64), (700, 64, 128, 64), (333, 200, 130, 72),
+                                                                       (150, 37, 50, 37)])
+def test_gradients_from_an_8_bit_checkpoint(tokens, channels, hidden, outputs, dtype):
+    *args, dy = inputs(tokens, channels, hidden, outputs, dtype)
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    y = gated_mlp(*leaves, activation="gelu", checkpoint8=True)
+    assert torch.equal(y, gated_mlp(*args, activation="gelu"))
+    got = torch.autograd.grad(y, leaves, dy)
+    restored = spectral.unpack8(*spectral.pack8(args[0]), dtype=dtype)
+    ref = [a.double().requires_grad_(True) for a in (restored, *args[1:])]
+    want = torch.autograd.grad(formula(*ref, "gelu"), ref, dy.double())
+    for name, g, w in zip(("dx", "dw_gate", "dw_up", "dw_down"), got, want):
+        close(g, w, TOL[dtype], name)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    *args, dy = inputs(40, 24, 36, 20, torch.float32)
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    grads = torch.autograd.grad(gated_mlp(*leaves), leaves, dy)
+    step = 1e-2
+    for i, grad in enumerate(grads):
+        direction = torch.randn(args[i].shape, generator=torch.Generator().manual_seed(i)).cuda()
+        direction /= direction.norm() / args[i].norm()
+        ends = []
+        for sign in (1.0, -1.0):
+            moved = list(args)
+            moved[i] = args[i] + sign * step * direction
+            ends.append((gated_mlp(*moved).double() * dy.double()).sum())
+        slope = float(ends[0] - ends[1]) / (2 * step)
+        # The remainder is of order step^2, the values' rounding 1e-6 / step.
+        assert abs(slope - float((grad.double() * direction.double()).sum())) <= 2e-3 * float(grad.double().norm() * direction.double().norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_unaligned_and_batched_operands(dtype):
+    *args, dy = inputs(60, 40, 48, 40, dtype)
+    want = gated_mlp(*args)
+
+    def shifted(t):  # the same values one element off a 16-byte boundary
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    exact = 0.0 if dtype != torch.float32 else 1e-7
+    for variant in ([shifted(a) for a in args], [a.t().contiguous().t() for a in args], [args[0].view(3, 4, 5, 40), *args[1:]]):
+        close(gated_mlp(*variant).reshape(want.shape), want, exact)
+        leaves = [a.detach().requires_grad_(True) for a in variant]
+        y = gated_mlp(*leaves)
+        plain = [a.clone().requires_grad_(True) for a in args]
+        grads = torch.autograd.grad(y, leaves, dy.reshape(y.shape))
+        for g, w in zip(grads, torch.autograd.grad(gated_mlp(*plain), plain, dy)):
+            close(g.reshape(w.shape), w, exact)
+    one = [a.clone() for a in args]
+    close(gated_mlp(shifted(one[0][:2]), *map(shifted, one[1:])), gated_mlp(one[0][:2].clone(), *one[1:]), TOL[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [6, 300])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_non_finite_tokens_stay_in_their_rows(tokens, dtype):
+    *args, dy = inputs(tokens, 64, 96, 64, dtype)
+    clean = gated_mlp(*args)
+    args[0][2, 5] = float("nan")
+    args[0][4, 0] = float("inf")
+    leaf = args[0].clone().requires_grad_(True)
+    y = gated_mlp(leaf, *args[1:])
+    rest = [i for i in range(tokens) if i not in (2, 4)]
+    assert y[2].isnan().all() and not y[4].isfinite().any()
+    assert torch.equal(y[rest], clean[rest])
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    assert dx[rest].isfinite().all() and dx[2].isnan().all()
+
+
+@pytest.mark.gpu
+def test_float32_beyond_the_16_bit_ranges():
+    # The three parts of a float32 have its range: large and small operands keep float32's accuracy.
+    *args, _ = inputs(100, 40, 48, 40, torch.float32)
+    args[0] *= 1e18
+    args[1] *= 1e-20
+    args[2] *= 1e10
+    args[3] *= 1e-12
+    close(gated_mlp(*args, activation="none"), formula(*[a.double() for a in args], "none"), TOL[torch.float32])
+
+
+@pytest.mark.gpu
+def test_no_tokens():
+    *args, dy = inputs(0, 8, 16, 24, torch.bfloat16)
+    leaves = [a.requires_grad_(True) for a in args]
+    y = gated_mlp(*leaves)
+    assert y.shape == (0, 24)
+    for g, a in zip(torch.autograd.grad(y, leaves, dy), leaves):
+        assert g.shape == a.shape and float(g.abs().sum()) == 0.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_same_bits_every_time_and_on_a_side_stream(dtype):
+    *args, dy = inputs(5000, 96, 160, 96, dtype)
+
+    def step():
+        leaves = [a.clone().requires_grad_(True) for a in args]
+        y = gated_mlp(*leaves, activation="gelu", checkpoint8=True)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+@pytest.mark.gpu
+def test_past_two_to_the_31_values():
+    tokens = (1 << 25) + 77
+    x = torch.zeros(tokens, 64, dtype=torch.bfloat16, device="cuda")
+    *args, dy = inputs(200, 64, 16, 8, torch.bfloat16)
+    x[-200:] = args[0]
+    y = gated_mlp(x, *args[1:])
+    close(y[-200:], formula(*[a.double() for a in args], "silu"), TOL[torch.bfloat16])
+    assert float(y[:1000].abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_module_and_training_step():
+    torch.manual_seed(0)
+    mlp = GatedMLP(16, 48, activation="silu", checkpoint8=True, device="cuda")
+    x, target = torch.randn(500, 16, device="cuda"), torch.randn(500, 16, device="cuda")
+    opt = torch.optim.SGD(mlp.parameters(), lr=0.05)
+    losses = []
+    for _ in range(3):
+        loss = ((mlp(x) - target) ** 2).mean()
+        losses.append(loss.item())
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+    assert losses[2] < losses[1] < losses[0]
+    assert "16, 48, 16" in repr(mlp)
+
+
+def block64(block, u):
+    """FNOBlock in float64 with torch's FFT."""
+    conv, norm, mlp = block.conv, block.norm, block.mlp
+    n1, n2 = u.shape[-2:]
+    spec = torch.fft.rfft2(u)
+    modes = torch.cat([spec[..., :conv.m1, :conv.m2], spec[..., n1 - conv.m1:, :conv.m2]], dim=-2)
+    out = torch.einsum("bikl,iokl->bokl", modes, conv.weight.to(torch.complex128))
+    full = torch.zeros(*u.shape[:2], n1, n2 // 2 + 1, dtype=out.dtype, device=u.device)
+    full[..., :conv.m1, :conv.m2] = out[..., :conv.m1, :]
+    full[..., n1 - conv.m1:, :conv.m2] = out[..., conv.m1:, :]
+    v = torch.fft.irfft2(full, s=(n1, n2)).permute(0, 2, 3, 1)
+    g = v.reshape(v.shape[0], -1, norm.groups, v.shape[-1] // norm.groups)
+    mean = g.mean((1, 3), keepdim=True)
+    g = (g - mean) / torch.sqrt(((g - mean) ** 2).mean((1, 3), keepdim=True) + norm.eps)
+    z = act64(g.reshape(v.shape) * norm.weight.double() + norm.bias.double(), norm.activation)
+    z = formula(z, mlp.w_gate.double(), mlp.w_up.double(), mlp.w_down.double(), mlp.activation)
+    return u + z.permute(0, 3, 1, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("dtype", "tol"), [(torch.float32, 2e-5), (torch.bfloat16, 2e-2)])
+def test_fno_block(dtype, tol):
+    torch.manual_seed(1)
+    block = FNOBlock(16, 32, 8, 8, groups=4, device="cuda", dtype=dtype)
+    u = torch.randn(2, 16, 32, 32, device="cuda")
+    up = torch.randn_like(u)
+    leaf = u.clone().requires_grad_(True)
+    y = block(leaf)
+    params = [block.norm.weight, block.norm.bias, block.mlp.w_gate, block.mlp.w_up, block.mlp.w_down]
+    got = torch.autograd.grad(y, [leaf, *params], up)
+    ref = u.double().requires_grad_(True)
+    want_y = block64(block, ref)
+    want = torch.autograd.grad(want_y, [ref, *params], up.double())
+    close(y, want_y, tol)
+    for g, w in zip(got, want):
+        close(g, w, tol)
+
+
+@pytest.mark.gpu
+def test_fno_block_trains_with_8_bit_checkpoints():
+    torch.manual_seed(2)
+    block = FNOBlock(16, 32, 8, 8, groups=4, checkpoint8=True, device="cuda")
+    u, target = torch.randn(4, 16, 32, 32, device="cuda"), torch.randn(4, 16, 32, 32, device="cuda")
+    opt = torch.optim.SGD(block.parameters(), lr=0.05)
+    losses = []
+    for _ in range(3):
+        loss = ((block(u) - target) ** 2).mean()
+        losses.append(loss.item())
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+    assert losses[2] < losses[1] < losses[0]
+
+
+def arguments(**change):
+    a = dict(x=1 << 20, w_gate=1 << 21, w_up=1 << 22, w_down=1 << 23, y=1 << 24, dtype=1, tokens=4, channels=8, hidden=16,
+             outputs=8, activation=1, work=1 << 25, stream=None)
+    a.update(change)
+    return tuple(a.values())
+
+
+@pytest.mark.parametrize(
+    ("change", "message"),
+    [(dict(dtype=3), "dtype must be"), (dict(tokens=-1), "tokens"), (dict(hidden=0), "hidden"), (dict(activation=3), "activation must be"),
+     (dict(w_up=None), "null array"), (dict(x=(1 << 20) + 1), "aligned"), (dict(y=(1 << 20) + 32), "must not overlap"),
+     (dict(work=None), "null array"), (dict(tokens=1 << 31), "tokens")])
+def test_the_c_abi_refuses(change, message):
+    with pytest.raises(ValueError, match=message):
+        native.call("spectral_gated_mlp", *arguments(**change))
+
+
+@pytest.mark.parametrize(
+    ("change", "message"),
+    [(dict(x=None), "either x or codes"), (dict(codes=4096, scales=4096), "either x or codes"), (dict(dw_up=None), "null array"),
+     (dict(dx=1 << 20), "must not overlap"), (dict(dx=None), "must be given"), (dict(dtype=-1), "dtype must be"),
+     (dict(dw_down=(1 << 29) + 1), "aligned")])
+def test_the_c_abi_refuses_backward(change, message):
+    a = dict(dy=1 << 20, x=1 << 21, codes=None, scales=None, w_gate=1 << 22, w_up=1 << 23, w_down=1 << 24, dx=1 << 25,
+             dw_gate=1 << 26, dw_up=1 << 27, dw_down=1 << 29, dtype=1, tokens=4, channels=8, hidden=16, outputs=8, activation=1,
+             work=1 << 30, stream=None)
+    a.update(change)
+    with pytest.raises(ValueError, match=message):
+        native.call("spectral_gated_mlp_backward", *a.values())
+
+
+def test_cpu_tensors_are_refused():
+    w = torch.zeros(16, 8)
+    with pytest.raises(NotImplementedError, match="CPU"):
+        gated_mlp(torch.zeros(2, 8), w, w, w.t())
+
+
+@pytest.mark.gpu
+def test_wrong_arguments_are_refused():
+    x, w, d = torch.zeros(2, 8, device="cuda"), torch.zeros(16, 8, device="cuda"), torch.zeros(4, 16, device="cuda")
+    with pytest.raises(RuntimeError, match="do not match"):
+        gated_mlp(x, w, w[:8], d)
+    with pytest.raises(RuntimeError, match="do not match"):
+        gated_mlp(x[:, :4], w, w, d)
+    with pytest.raises(RuntimeError, match="w_down must be"):
+        gated_mlp(x, w, w, d.bfloat16())
+    with pytest.raises(RuntimeError, match="activation must be"):
+        gated_mlp(x, w, w, d, activation="tanh")
+    with pytest.raises(RuntimeError, match="must be matrices"):
+        gated_mlp(x, w[0], w, d)
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        gated_mlp(x.double(), w.double(), w.double(), d.double())

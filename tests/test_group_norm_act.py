@@ -1,0 +1,319 @@
+"""Group norm with an activation on channels-last fields: values, statistics and all gradients against
+the formula in float64 (differentiated by torch's autograd), over types, group sizes that do not
+fill a vector, sizes of both kernel forms (a group kept on chip, and two passes), checkpoints in 8
+bits, strided and unaligned inputs, empty and non-finite ones; against differences; and the refusals.
+
+Tolerances, relative to the result's norm: a 16-bit type rounds each value once, at most 2^-9
+(bf16) or 2^-12 (f16) of it; float32 outputs carry a few roundings of the statistics (2^-24 each,
+times 1 + |mean| / std for the difference from the mean) and about 4 units of the fast exponential:
+64 units in all."""
+
+import math
+
+import pytest
+import torch
+
+import spectral
+from spectral import native
+from spectral.nn import GroupNormAct, group_norm_act
+
+TOL = {torch.float32: 64 * 2.0 ** -24, torch.bfloat16: 2.0 ** -9 * 1.05, torch.float16: 2.0 ** -12 * 1.05}
+DTYPES = list(TOL)
+
+
+def act64(z, activation):
+    if activation == "silu":
+        return z * torch.sigmoid(z)
+    if activation == "gelu":
+        return 0.5 * z * (1.0 + torch.erf(z / math.sqrt(2.0)))
+    return z
+
+
+def formula(x, groups, weight, bias, eps, activation, at=None):
+    """The definition on float64 tensors; statistics of x, values at `at` (x if not given)."""
+    b, c = x.shape[0], x.shape[-1]
+    v = x.reshape(b, -1, groups, c // groups)
+    mean = v.mean((1, 3), keepdim=True)
+    rstd = 1.0 / torch.sqrt(((v - mean) ** 2).mean((1, 3), keepdim=True) + eps)
+    xhat = (v - mean) * rstd
+    z = xhat.reshape(b, -1, c)
+    if weight is not None:
+        z = z * weight
+    if bias is not None:
+        z = z + bias
+    return act64(z, activation).reshape(x.shape)
+
+
+def gradients_at(x8, x, groups, weight, bias, eps, activation, dy):
+    """dx, dweight, dbias at the restored input x8 with the statistics of x, in float64."""
+    b, c = x.shape[0], x.shape[-1]
+    v = x.reshape(b, -1, groups, c // groups)
+    mean = v.mean((1, 3), keepdim=True)
+    rstd = 1.0 / torch.sqrt(((v - mean) ** 2).mean((1, 3), keepdim=True) + eps)
+    xhat = ((x8.reshape(v.shape) - mean) * rstd).reshape(b, -1, c)
+    z = (xhat * weight + bias).requires_grad_(True)
+    (slope,) = torch.autograd.grad(act64(z, activation).sum(), z)
+    dz = dy.reshape(b, -1, c) * slope
+    t = (dz * weight).reshape(v.shape)
+    h = xhat.reshape(v.shape)
+    dx = rstd * (t - t.mean((1, 3), keepdim=True) - h * (t * h).mean((1, 3), keepdim=True))
+    return dx.reshape(x.shape), (dz * xhat).sum((0, 1)), dz.sum((0, 1))
+
+
+def close(got, want, tol, name=""):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    err, size = float((got - want).norm()), float(want.norm())
+    assert err <= tol * size, f"{name}: {err / max(size, 1e-300):.3g} > {tol:.3g}"
+
+
+def inputs(shape, dtype, seed, offset=1.0):
+    g = torch.Generator().manual_seed(seed)
+    c = shape[-1]
+    x = torch.randn(*shape, generator=g) * torch.exp(0.5 * torch.randn(c, generator=g)) + offset * torch.randn(c, generator=g)
+    weight, bias = 1.0 + 0.2 * torch.randn(c, generator=g), 0.3 * torch.randn(c, generator=g)
+    dy = torch.randn(*shape, generator=g)
+    return x.to(dtype).cuda(), weight.cuda(), bias.cuda(), dy.to(dtype).cuda()
+
+
+# shape (batch, ..., channels), groups. Whole vectors and not; one point; one channel a group; a
+# group of everything; several CTAs a cluster; the two-pass form (more than a cluster holds, or
+# a group wider than a CTA's threads).
+SHAPES = [((2, 1, 16), 4), ((3, 5, 7, 24), 3), ((1, 16, 16, 32), 8), ((2, 33, 30), 6), ((2, 19, 7), 7), ((4, 9, 64), 64),
+          ((2, 300, 12), 1), ((1, 70, 70, 64), 8), ((2, 4000, 60), 6), ((1, 20000, 48), 2), ((2, 3, 4608), 2),
+          ((1, 70000, 64), 1), ((1, 5, 5, 1), 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["none", "silu", "gelu"])
+@pytest.mark.parametrize(("shape", "groups"), SHAPES)
+def test_values_and_gradients(shape, groups, activation, dtype):
+    x, weight, bias, dy = inputs(shape, dtype, sum(shape) + groups)
+    leaves = [t.clone().requires_grad_(True) for t in (x, weight, bias)]
+    y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], eps=1e-5, activation=activation)
+    got = torch.autograd.grad(y, leaves, dy)
+    ref = [t.double().requires_grad_(True) for t in (x, weight, bias)]
+    want_y = formula(ref[0], groups, ref[1], ref[2], 1e-5, activation)
+    want = torch.autograd.grad(want_y, ref, dy.double())
+    assert y.dtype == dtype and y.is_contiguous()
+    v = x.double().reshape(shape[0], -1, groups, shape[-1] // groups)
+    std = (v.var((1, 3), unbiased=False) + 1e-5).sqrt()
+    worst = 1.0 + float((v.mean((1, 3)).abs() / std).max())
+    single = TOL[torch.float32] * worst
+    tol = TOL[dtype] + single
+    close(y, want_y, tol, "y")
+    # A group of few values has dx near zero against its terms: rstd (t - mean(t) - xhat mean(t xhat)).
+    terms = float(((1.0 / std)[:, None, :, None] * (dy.double() * weight.double()).reshape(v.shape)).norm())
+    err = float((got[0].double() - want[0]).norm())
+    assert err <= tol * float(want[0].norm()) + single * 2 * terms, f"dx: {err:.3g}"
+    # The parameters' gradients are float32 sums; bound by the sums of magnitudes.
+    for name, g, w, size in (("dweight", got[1], want[1], (dy.double().abs() * 4).sum()),
+                             ("dbias", got[2], want[2], (dy.double().abs() * 2).sum())):
+        assert float((g.double() - w).abs().max()) <= single * float(w.abs().max()) + single * float(size) / shape[-1] ** 0.5, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("shape", "groups"), [((3, 5, 7, 24), 3), ((2, 33, 30), 6), ((1, 70, 70, 64), 8), ((2, 11, 136), 2),
+                                               ((1, 70000, 64), 1), ((2, 500, 4608), 3)])
+def test_gradients_from_an_8_bit_checkpoint(shape, groups, dtype):
+    x, weight, bias, dy = inputs(shape, dtype, sum(shape) + groups)
+    leaves = [t.clone().requires_grad_(True) for t in (x, weight, bias)]
+    y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], activation="gelu", checkpoint8=True)
+    assert torch.equal(y, group_norm_act(x, groups, weight, bias, activation="gelu"))
+    got = torch.autograd.grad(y, leaves, dy)
+    restored = spectral.unpack8(*spectral.pack8(x), dtype=dtype)
+    want = gradients_at(restored.double(), x.double(), groups, weight.double(), bias.double(), 1e-5, "gelu", dy.double())
+    v = x.double().reshape(shape[0], -1, groups, shape[-1] // groups)
+    worst = 1.0 + float((v.mean((1, 3)).abs() / (v.var((1, 3), unbiased=False) + 1e-5).sqrt()).max())
+    single = TOL[torch.float32] * worst
+    close(got[0], want[0], TOL[dtype] + single, "dx")
+    for name, g, w, factor in (("dweight", got[1], want[1], 4), ("dbias", got[2], want[2], 2)):
+        size = float((dy.double().abs() * factor).sum()) / shape[-1] ** 0.5
+        assert float((g.double() - w).abs().max()) <= single * (float(w.abs().max()) + size), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_gradients_against_differences(activation):
+    x, weight, bias, dy = inputs((2, 40, 24), torch.float32, 3)
+    args = [x, weight, bias]
+    leaves = [t.clone().requires_grad_(True) for t in args]
+    grads = torch.autograd.grad(group_norm_act(leaves[0], 4, leaves[1], leaves[2], activation=activation), leaves, dy)
+    step = 1e-2
+    for i, grad in enumerate(grads):
+        direction = torch.randn(args[i].shape, generator=torch.Generator().manual_seed(i)).cuda()
+        ends = []
+        for sign in (1.0, -1.0):
+            moved = list(args)
+            moved[i] = args[i] + sign * step * direction
+            ends.append((group_norm_act(moved[0], 4, moved[1], moved[2], activation=activation).double() * dy.double()).sum())
+        slope = float(ends[0] - ends[1]) / (2 * step)
+        # Second-order remainder step^2 and rounding 1e-6 / step, against gradients of this norm.
+        assert abs(slope - float((grad.double() * direction.double()).sum())) <= 2e-3 * float(grad.double().norm() * direction.double().norm())
+
+
+@pytest.mark.gpu
+def test_statistics_of_a_large_mean_do_not_cancel():
+    # Offsets of 3000 standard deviations: the one-pass form sum x^2 - n mean^2 would lose the variance.
+    for shape in [(2, 600, 16), (1, 70000, 64)]:
+        g = torch.Generator().manual_seed(7)
+        x = (torch.randn(*shape, generator=g) + 3000.0).cuda()
+        y = group_norm_act(x, 1)
+        close(y, formula(x.double(), 1, None, None, 1e-5, "none"), 64 * 3001 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+def test_optional_parameters_constant_inputs_and_eps():
+    x = torch.full((2, 7, 8), 3.0, device="cuda")
+    bias = torch.arange(8.0, device="cuda")
+    assert torch.equal(group_norm_act(x, 2, None, bias), bias.expand(2, 7, 8))
+    x = inputs((2, 9, 8), torch.float32, 1)[0]
+    close(group_norm_act(x, 2, eps=0.5), formula(x.double(), 2, None, None, 0.5, "none"), 1e-5)
+    leaf = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(group_norm_act(leaf, 2, eps=0.5).sum(), leaf)
+    assert float(dx.abs().max()) < 1e-5  # a sum over a group of normalised values does not move
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["resident", "two passes"])
+def test_non_finite_values_stay_in_their_group(form):
+    shape, groups = ((2, 50, 16), 2) if form == "resident" else ((2, 70000, 128), 2)
+    x, weight, bias, dy = inputs(shape, torch.float32, 11)
+    clean = group_norm_act(x, groups, weight, bias, activation="silu")
+    x[0, 3, 1] = float("nan")
+    x[1, 4, shape[-1] - 1] = float("inf")
+    leaf = x.clone().requires_grad_(True)
+    y = group_norm_act(leaf, groups, weight, bias, activation="silu")
+    half = shape[-1] // 2
+    assert y[0, :, :half].isnan().all() and y[1, :, half:].isnan().all()
+    assert torch.equal(y[0, :, half:], clean[0, :, half:]) and torch.equal(y[1, :, :half], clean[1, :, :half])
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    assert dx[0, :, half:].isfinite().all() and dx[1, :, :half].isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_and_unaligned_inputs(dtype):
+    g = torch.Generator().manual_seed(2)
+    first = torch.randn(3, 24, 10, 9, generator=g).to(dtype).cuda()  # channels first in memory
+    weight, bias = torch.randn(24, generator=g).cuda(), torch.randn(24, generator=g).cuda()
+    flat = torch.randn(2 * 24 * 11 + 1, generator=g).to(dtype).cuda()
+    for x in (first.permute(0, 2, 3, 1), first[:, :, ::2].permute(0, 2, 3, 1), flat[1:].view(2, 11, 24),
+              first.permute(0, 2, 3, 1)[..., 8:16].repeat(1, 1, 1, 3)):
+        leaf = x.detach().requires_grad_(True)
+        y = group_norm_act(leaf, 4, weight, bias, activation="gelu")
+        same = x.contiguous().clone().requires_grad_(True)
+        want = group_norm_act(same, 4, weight, bias, activation="gelu")
+        close(y, want, TOL[torch.float32] + (0 if dtype == torch.float32 else TOL[dtype]))
+        dy = torch.randn(y.shape, generator=g).to(dtype).cuda()
+        close(torch.autograd.grad(y, leaf, dy)[0], torch.autograd.grad(want, same, dy)[0],
+              4 * TOL[torch.float32] + (0 if dtype == torch.float32 else TOL[dtype]))
+
+
+@pytest.mark.gpu
+def test_empty_inputs():
+    weight = torch.ones(8, device="cuda", requires_grad=True)
+    for shape in [(0, 5, 8), (2, 0, 8)]:
+        x = torch.zeros(shape, device="cuda", requires_grad=True)
+        y = group_norm_act(x, 2, weight, activation="silu")
+        assert y.shape == shape
+        dx, dw = torch.autograd.grad(y.sum(), (x, weight))
+        assert dx.shape == shape and torch.equal(dw, torch.zeros_like(dw))
+
+
+@pytest.mark.gpu
+def test_the_same_bits_every_time_and_on_a_side_stream():
+    for shape, groups in [((4, 4000, 64), 8), ((1, 70000, 64), 1)]:
+        x, weight, bias, dy = inputs(shape, torch.bfloat16, 4)
+
+        def step():
+            leaves = [t.clone().requires_grad_(True) for t in (x, weight, bias)]
+            y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], activation="gelu", checkpoint8=True)
+            return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+        first = step()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            second = step()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+@pytest.mark.gpu
+def test_past_two_to_the_31_values():
+    points = (1 << 24) + 5
+    x = torch.zeros(2, points, 64, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    x[1, -1000:] = torch.randn(1000, 64, generator=g).to(torch.bfloat16).cuda()
+    y = group_norm_act(x, 2)
+    v = x[1, -1000:].double().reshape(1000, 2, 32)
+    n = points * 32
+    mean = v.sum((0, 2)) / n
+    var = (v ** 2).sum((0, 2)) / n - mean ** 2
+    want = (v - mean[:, None]) / torch.sqrt(var[:, None] + 1e-5)
+    close(y[1, -1000:].reshape(1000, 2, 32), want, TOL[torch.bfloat16] + 2.0 ** -20)
+    assert float(y[0].abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_module():
+    norm = GroupNormAct(4, 16, activation="silu", checkpoint8=True, device="cuda")
+    x = inputs((2, 6, 6, 16), torch.bfloat16, 8)[0]
+    assert torch.equal(norm(x), group_norm_act(x, 4, norm.weight, norm.bias, activation="silu"))
+    norm(x).float().square().mean().backward()
+    assert norm.weight.grad.shape == (16,) and norm.bias.grad.shape == (16,)
+    assert "checkpoint8=True" in repr(norm)
+
+
+def forward_args(**change):
+    a = dict(x=4096, weight=None, bias=None, y=8192, mean=None, rstd=None, codes=None, scales=None, dtype=0, batch=1,
+             points=4, channels=8, groups=2, eps=1e-5, activation=0, work=65536, stream=None)
+    a.update(change)
+    return tuple(a.values())
+
+
+@pytest.mark.parametrize(
+    ("change", "message"),
+    [(dict(dtype=5), "dtype must be"), (dict(activation=9), "activation must be"), (dict(groups=3), "groups dividing channels"),
+     (dict(groups=0), "groups dividing channels"), (dict(batch=-1), "batch >= 0"), (dict(work=None), "must be given"),
+     (dict(mean=4096), "mean with rstd"), (dict(codes=4096), "codes with scales"), (dict(x=4098), "aligned"),
+     (dict(y=4096 + 64), "must not overlap"), (dict(batch=70000), "at most 65535 samples")])
+def test_the_c_abi_refuses(change, message):
+    with pytest.raises(ValueError, match=message):
+        native.call("spectral_group_norm_act", *forward_args(**change))
+
+
+@pytest.mark.parametrize(
+    ("change", "message"),
+    [(dict(x=None), "either x or codes"), (dict(codes=4096, scales=4096), "either x or codes"), (dict(mean=None), "must be given"),
+     (dict(dx=1 << 20), "must not overlap"), (dict(groups=5), "groups dividing channels"), (dict(dy=(1 << 20) + 1), "aligned")])
+def test_the_c_abi_refuses_backward(change, message):
+    a = dict(dy=1 << 20, x=1 << 21, codes=None, scales=None, weight=None, bias=None, mean=4096, rstd=8192, dx=1 << 22,
+             dweight=None, dbias=None, dtype=0, batch=1, points=4, channels=8, groups=2, activation=0, work=65536, stream=None)
+    a.update(change)
+    with pytest.raises(ValueError, match=message):
+        native.call("spectral_group_norm_act_backward", *a.values())
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(NotImplementedError, match="CPU"):
+        group_norm_act(torch.zeros(2, 4, 8), 2)
+
+
+@pytest.mark.gpu
+def test_wrong_arguments_are_refused():
+    x = torch.zeros(2, 4, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="groups must divide"):
+        group_norm_act(x, 3)
+    with pytest.raises(RuntimeError, match="activation must be"):
+        group_norm_act(x, 2, activation="relu")
+    with pytest.raises(RuntimeError, match="weight must be a float32 tensor of 8"):
+        group_norm_act(x, 2, torch.ones(4, device="cuda"))
+    with pytest.raises(RuntimeError, match="weight must be a float32 tensor of 8"):
+        group_norm_act(x, 2, torch.ones(8, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        group_norm_act(x.double(), 2)
+    with pytest.raises(RuntimeError, match="must be \\(batch"):
+        group_norm_act(x[0, 0], 2)
