@@ -137,14 +137,6 @@ __global__ void __launch_bounds__(256)
 
 // --- epilogue stores ---------------------------------------------------------------------------------
 
-// 32 bytes with one store; p is 32-byte aligned.
-__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8])
-{
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-
 // A run of 32 values of one row; only the first `valid` exist.
 template <class T>
 __device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
@@ -317,19 +309,26 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
     const long long at = row * g.pitch + col;
     if constexpr (K == Kind::kGate) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            acc[0][j] = activate<Act>(acc[0][j]) * acc[1][j];
+        for (int j = 0; j < 32; j += 2) {
+            const float2 h = activate2<Act, T>(make_float2(acc[0][j], acc[0][j + 1])) * make_float2(acc[1][j], acc[1][j + 1]);
+            acc[0][j] = h.x;
+            acc[0][j + 1] = h.y;
         }
         store_hidden<T>(static_cast<Op*>(g.out[0]) + at, g.plane, acc[0], valid);
     } else if constexpr (K == Kind::kGateBack) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            float slope;
-            const float a = activate_slope<Act>(acc[0][j], slope);
-            const float up = acc[1][j];
-            acc[0][j] = acc[2][j] * up * slope;  // dG
-            acc[1][j] = a * up;                  // h
-            acc[2][j] *= a;                      // dU
+        for (int j = 0; j < 32; j += 2) {
+            float2 slope;
+            const float2 up = make_float2(acc[1][j], acc[1][j + 1]);
+            const float2 dh = make_float2(acc[2][j], acc[2][j + 1]);
+            const float2 a = activate_slope2<Act>(make_float2(acc[0][j], acc[0][j + 1]), slope);
+            const float2 dg = dh * up * slope, h = a * up, du = dh * a;
+            acc[0][j] = dg.x;
+            acc[0][j + 1] = dg.y;
+            acc[1][j] = h.x;
+            acc[1][j + 1] = h.y;
+            acc[2][j] = du.x;
+            acc[2][j + 1] = du.y;
         }
         store_hidden<T>(static_cast<Op*>(g.out[0]) + at, g.plane, acc[0], valid);
         store_hidden<T>(static_cast<Op*>(g.out[1]) + at, g.plane, acc[2], valid);

@@ -8,6 +8,8 @@
 
 #include "common.cuh"
 
+#include <cstdint>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -54,62 +56,190 @@ void with_dtype(int dtype, F&& f)
     }
 }
 
+// --- pairs of floats -------------------------------------------------------------------------------
+
+// The pointwise kernels are close to bound by instruction issue, so they work on pairs: one packed
+// FP32x2 instruction does both (the same IEEE rounding as the scalar form).
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 operator+(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 operator*(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+// a - b: the product with -1 is exact, so there is one rounding.
+__device__ __forceinline__ float2 operator-(float2 a, float2 b) { return __ffma2_rn(b, pair(-1.0f), a); }
+
+// V values as pairs (an odd last one is paired with 0).
+template <int V>
+struct Floats {
+    static constexpr int kPairs = (V + 1) / 2;
+    float2 p[kPairs];
+
+    __device__ __forceinline__ float at(int j) const { return j % 2 == 0 ? p[j / 2].x : p[j / 2].y; }
+    __device__ __forceinline__ void set(int j, float v) { (j % 2 == 0 ? p[j / 2].x : p[j / 2].y) = v; }
+    __device__ __forceinline__ void fill(float v)
+    {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            p[i] = pair(v);
+        }
+    }
+};
+
+template <class T, int V>
+__device__ __forceinline__ Floats<V> widen(const Vec<T, V>& v)
+{
+    Floats<V> f;
+    if constexpr (V == 1) {
+        f.p[0] = make_float2(to_float(v.v[0]), 0.0f);
+    } else if constexpr (std::is_same_v<T, bf16>) {
+        const auto* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {  // bf16 is the upper half of a float
+            f.p[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        }
+    } else if constexpr (std::is_same_v<T, f16>) {
+        const auto* w = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            f.p[i] = __half22float2(w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            f.p[i] = make_float2(v.v[2 * i], v.v[2 * i + 1]);
+        }
+    }
+    return f;
+}
+
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(const Floats<V>& f)
+{
+    Vec<T, V> v;
+    if constexpr (V == 1) {
+        v.v[0] = from_float<T>(f.p[0].x);
+    } else if constexpr (std::is_same_v<T, bf16>) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            reinterpret_cast<__nv_bfloat162*>(&v)[i] = __float22bfloat162_rn(f.p[i]);
+        }
+    } else if constexpr (std::is_same_v<T, f16>) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            reinterpret_cast<__half2*>(&v)[i] = __float22half2_rn(f.p[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            v.v[2 * i] = f.p[i].x;
+            v.v[2 * i + 1] = f.p[i].y;
+        }
+    }
+    return v;
+}
+
 // --- activations ---------------------------------------------------------------------------------
 
-// 1 / (1 + exp(-z)) with the fast exponential and division (a few units in the last place; for
-// z < -87 the exponential overflows to infinity and the quotient is 0, the limit).
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-
-// The normal distribution function Phi(z), and exp(-z^2 / 2), which its density shares.
-// Q(|z|) = 1 - Phi(|z|) = exp(-z^2 / 2) t P(t) with t = 1 / (1 + 0.28 |z|), the classical form of
-// Hastings' approximations; P (degree 5) is a least-squares fit of this library's own, error
-// below 1.5e-8. One exponential and one reciprocal give both the value and the slope of gelu,
-// where erff and expf would cost about three times the instructions.
-__device__ __forceinline__ float normal_cdf(float z, float& e)
+// The hardware's 2^v and 1 / v (about one unit in the last place, subnormals as zero).
+__device__ __forceinline__ float exp2_fast(float v)
 {
-    e = __expf(-0.5f * z * z);
-    const float t = __fdividef(1.0f, fmaf(0.28f, fabsf(z), 1.0f));
-    float p = -0.10655131936073303f;
-    p = fmaf(p, t, 0.3929559588432312f);
-    p = fmaf(p, t, -0.2420753836631775f);
-    p = fmaf(p, t, 0.27307337522506714f);
-    p = fmaf(p, t, 0.06580273061990738f);
-    p = fmaf(p, t, 0.11679460108280182f);
-    const float q = p * t * e;
-    return z > 0.0f ? 1.0f - q : q;
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// 1 / (1 + exp(-z)). For z < -88 the power overflows to infinity and its reciprocal is 0, the limit.
+__device__ __forceinline__ float2 sigmoid2(float2 z)
+{
+    const float2 e = z * pair(-1.4426950408889634f);
+    const float2 d = make_float2(exp2_fast(e.x), exp2_fast(e.y)) + pair(1.0f);
+    return make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+}
+
+// The normal distribution function Phi(z), and e = exp(-z^2 / 2), which its density shares.
+// 1 - Phi(|z|) = e t P(t) with t = 1 / (1 + 0.28 |z|), the form of Hastings' approximations; P
+// (degree 5) is a least-squares fit of this library's own, off by less than 1.5e-8. One power and
+// one reciprocal give the value and the slope of gelu, about ten instructions a value; erff and
+// expf measured 47 against 22 for the whole normalisation of a value.
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2& e)
+{
+    const float2 x = (z * pair(-0.7213475204444817f)) * z;
+    e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+    const float2 t = make_float2(reciprocal_fast(fmaf(0.28f, fabsf(z.x), 1.0f)), reciprocal_fast(fmaf(0.28f, fabsf(z.y), 1.0f)));
+    float2 p = pair(-0.10655131936073303f);
+    p = fma2(p, t, pair(0.3929559588432312f));
+    p = fma2(p, t, pair(-0.2420753836631775f));
+    p = fma2(p, t, pair(0.27307337522506714f));
+    p = fma2(p, t, pair(0.06580273061990738f));
+    p = fma2(p, t, pair(0.11679460108280182f));
+    const float2 half = fma2(p * t, e * pair(-1.0f), pair(0.5f));  // Phi(|z|) - 1/2
+    return pair(0.5f) + make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y));
+}
+
+// Phi(z) for results that are rounded to 16 bits: the logistic function of z P(z^2), P (degree 6, a
+// least-squares fit of this library's own) the even part of log(Phi(z) / Phi(-z)) / z. z Phi(z) is off
+// by less than 6e-7 in all and by 5e-5 of its own size for z > -3 (a bf16 or f16 rounding: 2^-9, 2^-12).
+// Seven instructions a value against normal_cdf2's ten, every one of them packed.
+__device__ __forceinline__ float2 normal_cdf16(float2 z)
+{
+    const float2 u = z * z;
+    float2 p = pair(-4.304068657035032e-09f);  // times -log2(e)
+    p = fma2(p, u, pair(3.4366911449978943e-07f));
+    p = fma2(p, u, pair(-1.07983396446798e-05f));
+    p = fma2(p, u, pair(0.0001548998843645677f));
+    p = fma2(p, u, pair(0.00010911076969932765f));
+    p = fma2(p, u, pair(-0.1048540323972702f));
+    p = fma2(p, u, pair(-2.3022031784057617f));
+    p = p * z;
+    const float2 d = make_float2(exp2_fast(p.x), exp2_fast(p.y)) + pair(1.0f);
+    return make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+}
+
+// The activation of a value that is then rounded to T.
+template <int Act, class T = float>
+__device__ __forceinline__ float2 activate2(float2 z)
+{
+    if constexpr (Act == SPECTRAL_ACT_SILU) {
+        return z * sigmoid2(z);
+    } else if constexpr (Act == SPECTRAL_ACT_GELU && sizeof(T) == 2) {
+        return z * normal_cdf16(z);
+    } else if constexpr (Act == SPECTRAL_ACT_GELU) {
+        float2 e;
+        return z * normal_cdf2(z, e);
+    } else {
+        return z;
+    }
+}
+
+// The activation's values and slopes at z.
+template <int Act>
+__device__ __forceinline__ float2 activate_slope2(float2 z, float2& slope)
+{
+    if constexpr (Act == SPECTRAL_ACT_SILU) {
+        const float2 s = sigmoid2(z);
+        const float2 a = z * s;
+        slope = fma2(a, pair(1.0f) - s, s);
+        return a;
+    } else if constexpr (Act == SPECTRAL_ACT_GELU) {
+        float2 e;
+        const float2 phi = normal_cdf2(z, e);
+        slope = fma2(z * pair(0.3989422804014327f), e, phi);
+        return z * phi;
+    } else {
+        slope = pair(1.0f);
+        return z;
+    }
 }
 
 template <int Act>
 __device__ __forceinline__ float activate(float z)
 {
-    if constexpr (Act == SPECTRAL_ACT_SILU) {
-        return z * sigmoid(z);
-    } else if constexpr (Act == SPECTRAL_ACT_GELU) {
-        float e;
-        return z * normal_cdf(z, e);
-    } else {
-        return z;
-    }
-}
-
-// The activation's value and slope at z.
-template <int Act>
-__device__ __forceinline__ float activate_slope(float z, float& slope)
-{
-    if constexpr (Act == SPECTRAL_ACT_SILU) {
-        const float s = sigmoid(z);
-        const float a = z * s;
-        slope = fmaf(a, 1.0f - s, s);
-        return a;
-    } else if constexpr (Act == SPECTRAL_ACT_GELU) {
-        float e;
-        const float phi = normal_cdf(z, e);
-        slope = fmaf(0.3989422804014327f * z, e, phi);
-        return z * phi;
-    } else {
-        slope = 1.0f;
-        return z;
-    }
+    return activate2<Act>(make_float2(z, 0.0f)).x;
 }
 
 // Calls f(integral_constant<Act>) for an activation code.
@@ -128,16 +258,156 @@ void with_activation(int act, F&& f)
 constexpr int kPackBlock = SPECTRAL_PACK8_BLOCK;     // values of a row that share one scale
 constexpr float kPackTiny = 7.888609052210118e-31f;  // 2^-100: 127 / tiny is finite
 
-// The value a code stands for, in the checkpoint's type. 127 scale can round past the largest float32;
-// such a value is that largest one (the scale itself is never infinite).
-template <class T>
-__device__ __forceinline__ T restored(signed char code, float scale)
+// The values V codes stand for, in the checkpoint's type. A code's byte, offset by 128, becomes the low
+// bits of 2^23 + byte, so one subtraction converts it. 127 scale can round past the largest float32;
+// such a value is that largest one (the scale itself is never infinite; the 16-bit types are far
+// from it).
+template <class T, int V>
+__device__ __forceinline__ Floats<V> restored(const Vec<signed char, V>& codes, float scale)
 {
-    float v = static_cast<float>(code) * scale;
-    if (fabsf(v) > 3.4028234663852886e38f) {
-        v = copysignf(3.4028234663852886e38f, v);
+    Floats<V> f;
+    if constexpr (V >= 4) {
+        const auto* w = reinterpret_cast<const uint32_t*>(&codes);
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            const uint32_t u = w[j] ^ 0x80808080u;
+            f.p[2 * j] = make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)),
+                                     __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)));
+            f.p[2 * j + 1] = make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)),
+                                         __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)));
+        }
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            f.p[j] = (f.p[j] - pair(8388736.0f)) * pair(scale);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+            f.p[j].x = static_cast<float>(codes.v[2 * j]) * scale;
+            f.p[j].y = 2 * j + 1 < V ? static_cast<float>(codes.v[2 * j + 1 < V ? 2 * j + 1 : 0]) * scale : 0.0f;
+        }
     }
-    return from_float<T>(v);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float v = f.at(j);
+            f.set(j, fabsf(v) > 3.4028234663852886e38f ? copysignf(3.4028234663852886e38f, v) : v);
+        }
+        return f;
+    } else {
+        return widen(narrow<T>(f));
+    }
+}
+
+// The scale of a block whose largest magnitude has the bits `top` (a NaN's are above infinity's, and
+// those above every number's), and the factor that turns its values into codes. A block with an
+// infinity or NaN has the scale NaN and the codes 0.
+struct PackScale {
+    float scale;
+    float per_unit;
+};
+
+__device__ __forceinline__ PackScale pack_scale(unsigned top)
+{
+    const bool finite = top < 0x7f800000u;
+    const float m = finite ? fmaxf(__uint_as_float(top), kPackTiny) : 1.0f;
+    return {finite ? __fdiv_rn(m, 127.0f) : __uint_as_float(0x7fc00000u), finite ? __fdiv_rn(127.0f, m) : 0.0f};
+}
+
+// The bits of the largest magnitude among the values: whole numbers order as the magnitudes do, in
+// 16 bits as in 32.
+template <class T, int V>
+__device__ __forceinline__ unsigned top_bits(const Vec<T, V>& v)
+{
+    if constexpr (sizeof(T) == 4 || V == 1) {
+        unsigned top = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            top = max(top, __float_as_uint(to_float(v.v[j])) & 0x7fffffffu);
+        }
+        return top;
+    } else {
+        const auto* w = reinterpret_cast<const unsigned*>(&v);
+        unsigned two = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int j = 1; j < V / 2; ++j) {
+            two = __vmaxu2(two, w[j] & 0x7fff7fffu);
+        }
+        const unsigned short top = static_cast<unsigned short>(max(two & 0xffffu, two >> 16));
+        return __float_as_uint(to_float(*reinterpret_cast<const T*>(&top)));
+    }
+}
+
+// round(v * per_unit) as bytes. Adding 1.5 x 2^23 rounds to the nearest whole number, ties to even,
+// and leaves it in the low bits (two's complement). A per_unit of 0 gives codes 0 whatever v is.
+template <int V>
+__device__ __forceinline__ Vec<signed char, V> pack_codes(const Floats<V>& f, float per_unit)
+{
+    Vec<signed char, V> c;
+    uint32_t w[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        // The scalar intrinsics: the product is rounded before the sum (a packed multiply and add
+        // may be contracted, which moved codes at ties).
+        w[j] = __float_as_uint(__fadd_rn(__fmul_rn(f.at(j), per_unit), 12582912.0f));
+    }
+    const uint32_t keep = per_unit == 0.0f ? 0u : 0xffffffffu;
+    if constexpr (V >= 4) {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            const uint32_t lo = __byte_perm(w[4 * j], w[4 * j + 1], 0x0040);
+            const uint32_t hi = __byte_perm(w[4 * j + 2], w[4 * j + 3], 0x0040);
+            reinterpret_cast<uint32_t*>(&c)[j] = __byte_perm(lo, hi, 0x5410) & keep;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            c.v[j] = static_cast<signed char>(w[j] & keep);
+        }
+    }
+    return c;
+}
+
+// Packs K blocks at once. This lane holds one piece of each, v[k]; the kPackBlock / V lanes of a
+// block sit side by side in the warp. Each lane computes the scale of one block (scale_at(k) is
+// where it goes), the block's other lanes take it from there; put(k, codes) stores the codes.
+template <class T, int V, int K, class ScaleAt, class Put>
+__device__ __forceinline__ void pack_blocks(const Vec<T, V> (&v)[K], ScaleAt&& scale_at, Put&& put)
+{
+    constexpr int kLanes = kPackBlock / V;
+    static_assert(K <= kLanes && kLanes <= 32, "a lane per block");
+    const int lane = threadIdx.x & 31;
+    const int sub = lane % kLanes;
+    const unsigned mask = kLanes == 32 ? 0xffffffffu : ((1u << (kLanes % 32)) - 1u) << (lane / kLanes * kLanes);
+    unsigned mine = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        unsigned top = top_bits(v[k]);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o /= 2) {
+            top = max(top, __shfl_xor_sync(mask, top, o));
+        }
+        mine = k == 0 || sub == k ? top : mine;
+    }
+    const PackScale s = pack_scale(mine);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (sub == k) {
+            float* at = scale_at(k);
+            if (at != nullptr) {
+                *at = s.scale;
+            }
+        }
+        put(k, pack_codes<V>(widen(v[k]), __shfl_sync(mask, s.per_unit, k, kLanes)));
+    }
+}
+
+// 32 bytes with one store; p is 32-byte aligned.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // --- asynchronous copies -----------------------------------------------------------------------------

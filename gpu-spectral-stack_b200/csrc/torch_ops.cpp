@@ -662,6 +662,26 @@ NormSizes norm_sizes(const at::Tensor& x, int64_t groups, const char* op)
     return s;
 }
 
+// x (batch, ..., channels) lies in memory as (batch, channels, ...), in a shape and alignment that the
+// library's channels-first kernels take.
+bool channels_first(const at::Tensor& x, const NormSizes& n)
+{
+    const int64_t values = 16 / x.element_size();
+    return !x.is_contiguous() && n.channels % 8 == 0 && n.points % values == 0 && x.movedim(-1, 1).is_contiguous()
+           && (reinterpret_cast<uintptr_t>(x.const_data_ptr()) & 15u) == 0;
+}
+
+// x with its channels last in memory.
+at::Tensor last_contiguous(const at::Tensor& x, int dtype, const NormSizes& n)
+{
+    if (x.numel() == 0 || !channels_first(x, n)) {
+        return x.contiguous();
+    }
+    at::Tensor y = at::empty(x.sizes(), x.options());
+    check_status(spectral_channels_last(cptr(x), mptr(y), dtype, n.batch, n.points, n.channels, stream()));
+    return y;
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
                     const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation, bool keep8)
@@ -673,7 +693,8 @@ group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at:
     const c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor w = channel_parameter(weight, x, n.channels, op, "weight");
     const at::Tensor b = channel_parameter(bias, x, n.channels, op, "bias");
-    const at::Tensor xc = x.contiguous();
+    const bool first = x.numel() > 0 && !keep8 && channels_first(x, n);
+    const at::Tensor xc = first ? x : last_contiguous(x, dtype, n);
     at::Tensor y = at::empty(x.sizes(), x.options());
     at::Tensor mean = at::empty({n.batch, groups}, x.options().dtype(at::kFloat));
     at::Tensor rstd = at::empty_like(mean);
@@ -685,12 +706,12 @@ group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at:
         return {y, mean, rstd, codes, scales};
     }
     size_t count = 0;
-    check_status(spectral_group_norm_act_workspace(n.batch, n.channels, n.groups, &count));
+    check_status(spectral_group_norm_act_workspace(dtype, n.batch, n.points, n.channels, n.groups, &count));
     at::Tensor work = workspace(count, x);
     check_status(spectral_group_norm_act(cptr(xc), fptr(w), fptr(b), mptr(y), static_cast<float*>(mptr(mean)),
                                          static_cast<float*>(mptr(rstd)), keep8 ? mptr(codes) : nullptr,
-                                         keep8 ? static_cast<float*>(mptr(scales)) : nullptr, dtype, n.batch, n.points,
-                                         n.channels, n.groups, static_cast<float>(eps), act, mptr(work), stream()));
+                                         keep8 ? static_cast<float*>(mptr(scales)) : nullptr, dtype, first ? 1 : 0, n.batch,
+                                         n.points, n.channels, n.groups, static_cast<float>(eps), act, mptr(work), stream()));
     return {y, mean, rstd, codes, scales};
 }
 
@@ -713,7 +734,7 @@ group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tenso
     if (x.has_value()) {
         check_like(*x, dy, op, "x");
         TORCH_CHECK(x->sizes() == dy.sizes(), op, ": x and dy must have one shape");
-        xc = x->contiguous();
+        xc = last_contiguous(*x, dtype, n);
     } else {
         check_packed(*codes, *scales, op);
         TORCH_CHECK(codes->device() == dy.device() && codes->sizes() == dy.sizes(), op,
@@ -728,12 +749,12 @@ group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tenso
     }
     const at::Tensor w = channel_parameter(weight, dy, n.channels, op, "weight");
     const at::Tensor b = channel_parameter(bias, dy, n.channels, op, "bias");
-    const at::Tensor dyc = dy.contiguous();
+    const at::Tensor dyc = last_contiguous(dy, dtype, n);
     at::Tensor dx = at::empty(dy.sizes(), dy.options());
     at::Tensor dweight = at::empty({n.channels}, dy.options().dtype(at::kFloat));
     at::Tensor dbias = at::empty_like(dweight);
     size_t count = 0;
-    check_status(spectral_group_norm_act_backward_workspace(n.batch, n.channels, n.groups, &count));
+    check_status(spectral_group_norm_act_backward_workspace(dtype, n.batch, n.points, n.channels, n.groups, &count));
     at::Tensor work = workspace(count, dy);
     check_status(spectral_group_norm_act_backward(
         cptr(dyc), xc.defined() ? cptr(xc) : nullptr, cc.defined() ? cptr(cc) : nullptr, fptr(sc), fptr(w), fptr(b),

@@ -81,10 +81,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spectral_mode_contract_method": (_i, [_p, _p, _p, _ll, _i, _i, _ll, _i, _p]),
     "spectral_pack8": (_i, [_p, _i, _p, _p, _ll, _i, _p]),
     "spectral_unpack8": (_i, [_p, _p, _p, _i, _ll, _i, _p]),
-    "spectral_group_norm_act_workspace": (_i, [_ll, _i, _i, _szp]),
-    "spectral_group_norm_act": (_i, [_p] * 8 + [_i, _ll, _ll, _i, _i, _f, _i, _p, _p]),
-    "spectral_group_norm_act_backward_workspace": (_i, [_ll, _i, _i, _szp]),
+    "spectral_group_norm_act_workspace": (_i, [_i, _ll, _ll, _i, _i, _szp]),
+    "spectral_group_norm_act": (_i, [_p] * 8 + [_i, _i, _ll, _ll, _i, _i, _f, _i, _p, _p]),
+    "spectral_group_norm_act_backward_workspace": (_i, [_i, _ll, _ll, _i, _i, _szp]),
     "spectral_group_norm_act_backward": (_i, [_p] * 11 + [_i, _ll, _ll, _i, _i, _i, _p, _p]),
+    "spectral_channels_last": (_i, [_p, _p, _i, _ll, _ll, _i, _p]),
     "spectral_gated_mlp_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),
     "spectral_gated_mlp": (_i, [_p] * 5 + [_i, _ll, _i, _i, _i, _i, _p, _p]),
     "spectral_gated_mlp_backward_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),

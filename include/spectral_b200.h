@@ -335,23 +335,32 @@ SPECTRAL_API int spectral_unpack8(const void* codes, const float* scales, void* 
  * mean and var (biased) per sample over the points x (channels / groups) values of each group.
  * weight and bias: `channels` floats, or NULL for 1 and 0. mean and rstd (batch x groups floats)
  * receive the statistics for the backward pass; both may be NULL. codes and scales (both or
- * neither) receive x's 8-bit checkpoint (rows of `channels`). x and y must not overlap. */
-SPECTRAL_API int spectral_group_norm_act_workspace(long long batch, int channels, int groups, size_t* count);
+ * neither) receive x's 8-bit checkpoint (rows of `channels`). x and y must not overlap. With
+ * channels_first, x is (batch, channels, points), as a spectral convolution leaves it, and is read
+ * as it lies (y is channels last all the same): needs channels a multiple of 8, points of 16 bytes of
+ * values, 16-byte aligned x and y, and no checkpoint. */
+SPECTRAL_API int spectral_group_norm_act_workspace(int dtype, long long batch, long long points, int channels,
+                                                   int groups, size_t* count);
 SPECTRAL_API int spectral_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean,
-                                         float* rstd, void* codes, float* scales, int dtype, long long batch,
-                                         long long points, int channels, int groups, float eps, int activation,
-                                         void* work, void* stream);
+                                         float* rstd, void* codes, float* scales, int dtype, int channels_first,
+                                         long long batch, long long points, int channels, int groups, float eps,
+                                         int activation, void* work, void* stream);
 /* Its gradients for the upstream gradient dy, from the forward call's mean and rstd and either x
  * or its checkpoint (codes and scales, x NULL): dx, and dweight and dbias (`channels` floats each;
  * either may be NULL). Every sum has a fixed order: equal inputs give equal bits. */
-SPECTRAL_API int spectral_group_norm_act_backward_workspace(long long batch, int channels, int groups,
-                                                            size_t* count);
+SPECTRAL_API int spectral_group_norm_act_backward_workspace(int dtype, long long batch, long long points,
+                                                            int channels, int groups, size_t* count);
 SPECTRAL_API int spectral_group_norm_act_backward(const void* dy, const void* x, const void* codes,
                                                   const float* scales, const float* weight, const float* bias,
                                                   const float* mean, const float* rstd, void* dx, float* dweight,
                                                   float* dbias, int dtype, long long batch, long long points,
                                                   int channels, int groups, int activation, void* work,
                                                   void* stream);
+
+/* The transposing copy alone: x (batch, channels, points) to y (batch, points, channels), under the
+ * conditions of channels_first above. */
+SPECTRAL_API int spectral_channels_last(const void* x, void* y, int dtype, long long batch, long long points,
+                                        int channels, void* stream);
 
 /* The gated feed-forward block on `tokens` rows:
  *   y = (act(x w_gate^T) * (x w_up^T)) w_down^T

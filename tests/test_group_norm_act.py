@@ -1,6 +1,6 @@
 """Group norm with an activation on channels-last fields: values, statistics and all gradients against
 the formula in float64 (differentiated by torch's autograd), over types, group sizes that do not
-fill a vector, sizes of both kernel forms (a group kept on chip, and two passes), checkpoints in 8
+fill a vector, sizes of both kernel forms (a group kept on chip, and read twice), checkpoints in 8
 bits, strided and unaligned inputs, empty and non-finite ones; against differences; and the refusals.
 
 Tolerances, relative to the result's norm: a 16-bit type rounds each value once, at most 2^-9
@@ -268,7 +268,7 @@ def test_module():
 
 
 def forward_args(**change):
-    a = dict(x=4096, weight=None, bias=None, y=8192, mean=None, rstd=None, codes=None, scales=None, dtype=0, batch=1,
+    a = dict(x=4096, weight=None, bias=None, y=8192, mean=None, rstd=None, codes=None, scales=None, dtype=0, channels_first=0, batch=1,
              points=4, channels=8, groups=2, eps=1e-5, activation=0, work=65536, stream=None)
     a.update(change)
     return tuple(a.values())
@@ -279,7 +279,8 @@ def forward_args(**change):
     [(dict(dtype=5), "dtype must be"), (dict(activation=9), "activation must be"), (dict(groups=3), "groups dividing channels"),
      (dict(groups=0), "groups dividing channels"), (dict(batch=-1), "batch >= 0"), (dict(work=None), "must be given"),
      (dict(mean=4096), "mean with rstd"), (dict(codes=4096), "codes with scales"), (dict(x=4098), "aligned"),
-     (dict(y=4096 + 64), "must not overlap"), (dict(batch=70000), "at most 65535 samples")])
+     (dict(y=4096 + 64), "must not overlap"), (dict(channels_first=1, points=5), "channels first needs"),
+     (dict(channels_first=1, codes=1 << 20, scales=1 << 21), "channels first needs"), (dict(batch=1 << 31, x=1 << 60), "at most 2\\^30 samples")])
 def test_the_c_abi_refuses(change, message):
     with pytest.raises(ValueError, match=message):
         native.call("spectral_group_norm_act", *forward_args(**change))
