@@ -34,10 +34,7 @@
 
 #include "../../include/spectral_b200.h"
 
-#include "backend.hpp"
-#include "launch.cuh"
-#include "pointwise.cuh"
-#include "umma.cuh"
+#include "mlp.cuh"
 
 #include <algorithm>
 #include <climits>
@@ -49,49 +46,9 @@ void unpack8(const signed char* codes, const float* scales, void* x, int dtype, 
 
 namespace {
 
-constexpr int kTileM = 128;
-constexpr int kChunk = umma::kAtom;  // K per stage
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 32 * (kEpilogueWarps + 2);
-constexpr int kTileABytes = kTileM * umma::kRowBytes;
-constexpr int kMaxSmem = 227 * 1024;
+using namespace mlp;
+
 constexpr long long kMaxTokens = 0x7fffff00LL;  // 32-bit TMA coordinates
-
-// The type matrix products run in, and the parts an operand of T is split into.
-template <class T>
-struct Operand {
-    using Type = T;
-    static constexpr int kPlanes = 1;
-    static constexpr int kProducts = 1;
-    static constexpr int kPassChunks = 1 << 24;  // one pass over all of K
-};
-template <>
-struct Operand<float> {
-    using Type = bf16;
-    static constexpr int kPlanes = 3;
-    static constexpr int kProducts = 6;
-    static constexpr int kPassChunks = 2;
-};
-
-// Parts (a, b) of a float32 product's p-th MMA, the small ones first: (2,0) (0,2) (1,1) (1,0) (0,1)
-// (0,0), two bits each. Other types have one part.
-template <class T>
-__device__ __forceinline__ int part_a(int p) { return sizeof(T) == 4 ? (0b00'00'01'01'00'10 >> (2 * p)) & 3 : 0; }
-template <class T>
-__device__ __forceinline__ int part_b(int p) { return sizeof(T) == 4 ? (0b00'01'00'01'10'00 >> (2 * p)) & 3 : 0; }
-
-// v = hi + mid + lo in bf16 parts (exact but for parts below bf16's smallest). A hi that would round to
-// infinity is cut instead, and an infinity or NaN has no further parts.
-__device__ __forceinline__ void split3(float v, bf16& hi, bf16& mid, bf16& lo)
-{
-    hi = __float2bfloat16_rn(v);
-    if (fabsf(v) > 3.3895313892515355e38f && fabsf(v) <= 3.4028234663852886e38f) {
-        hi = __float2bfloat16_rz(v);
-    }
-    const float r = fabsf(v) <= 3.4028234663852886e38f ? v - __bfloat162float(hi) : 0.0f;
-    mid = __float2bfloat16_rn(r);
-    lo = __float2bfloat16_rn(r - __bfloat162float(mid));
-}
 
 // --- staging ---------------------------------------------------------------------------------------
 
@@ -137,39 +94,6 @@ __global__ void __launch_bounds__(256)
 
 // --- epilogue stores ---------------------------------------------------------------------------------
 
-// A run of 32 values of one row; only the first `valid` exist.
-template <class T>
-__device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
-{
-    constexpr int kPer = 32 / static_cast<int>(sizeof(T));  // values per 32 bytes
-    if (valid >= 32 && (reinterpret_cast<std::uintptr_t>(p) & 31u) == 0) {
-#pragma unroll
-        for (int i = 0; i < 32 / kPer; ++i) {
-            uint32_t w[8];
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[j] = __float_as_uint(v[i * kPer + j]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    Vec<T, 2> two{{v[i * kPer + 2 * j], v[i * kPer + 2 * j + 1]}};
-                    w[j] = *reinterpret_cast<uint32_t*>(&two);
-                }
-            }
-            store32(p + i * kPer, w);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            if (j < valid) {
-                p[j] = v[j];
-            }
-        }
-    }
-}
-
 // A run of hidden values in the operand form (planes `plane` values apart).
 template <class T>
 __device__ __forceinline__ void store_hidden(typename Operand<T>::Type* p, long long plane, const float (&v)[32], int valid)
@@ -191,17 +115,6 @@ __device__ __forceinline__ void store_hidden(typename Operand<T>::Type* p, long 
         }
         store_run(p, out, valid);
     }
-}
-
-template <class T>
-__device__ __forceinline__ void store_values(T* p, const float (&v)[32], int valid)
-{
-    T out[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        out[j] = from_float<T>(v[j]);
-    }
-    store_run(p, out, valid);
 }
 
 // --- the matrix-product kernel -----------------------------------------------------------------------
@@ -338,16 +251,6 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
         store_values<float>(out + static_cast<long long>(row) * cols + col, acc[0], valid);
     } else {
         store_values<T>(static_cast<T*>(g.out[0]) + at, acc[0], valid);
-    }
-}
-
-// This warp has read the accumulator set that `bar` guards.
-__device__ __forceinline__ void release(uint64_t* bar, int lane)
-{
-    umma::fence_before_sync();
-    __syncwarp();
-    if (lane == 0) {
-        umma::arrive(bar);
     }
 }
 
@@ -652,28 +555,44 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     }
 }
 
-// The parts of the three weight products, added up in order and rounded once.
+// The parts of the three weight products, added up and rounded once: 32 values side by side, eight
+// warps taking every eighth part, joined in order.
 template <class T>
 __global__ void __launch_bounds__(256)
     weight_sum_kernel(const float* __restrict__ partial, T* __restrict__ w0, T* __restrict__ w1, T* __restrict__ w2,
                       long long size0, long long size2, long long part_size, int parts)
 {
+    __shared__ float sums[8][32];
     allow_next_grid();
-    wait_for_previous_grid();
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     const long long total = 2 * size0 + size2;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
-         i += static_cast<long long>(gridDim.x) * 256) {
+    wait_for_previous_grid();
+    for (long long i0 = static_cast<long long>(blockIdx.x) * 32; i0 < total; i0 += static_cast<long long>(gridDim.x) * 32) {
+        const long long i = i0 + lane;
         float s = 0.0f;
-        for (int p = 0; p < parts; ++p) {
-            s += partial[p * part_size + i];
+        if (i < total) {
+#pragma unroll 8
+            for (int p = warp; p < parts; p += 8) {
+                s += partial[p * part_size + i];
+            }
         }
-        if (i < size0) {
-            w0[i] = from_float<T>(s);
-        } else if (i < 2 * size0) {
-            w1[i - size0] = from_float<T>(s);
-        } else {
-            w2[i - 2 * size0] = from_float<T>(s);
+        sums[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0 && i < total) {
+#pragma unroll
+            for (int k = 1; k < 8; ++k) {
+                s += sums[k][lane];
+            }
+            if (i < size0) {
+                w0[i] = from_float<T>(s);
+            } else if (i < 2 * size0) {
+                w1[i - size0] = from_float<T>(s);
+            } else {
+                w2[i - 2 * size0] = from_float<T>(s);
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -785,14 +704,6 @@ __global__ void __launch_bounds__(kFewThreads)
 
 // --- host side -----------------------------------------------------------------------------------------
 
-struct MlpShape {
-    long long tokens;
-    int channels;
-    int hidden;
-    int outputs;
-    int act;
-};
-
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 int tiles_of(long long v, int tile) { return static_cast<int>((v + tile - 1) / tile); }
 int hidden_pitch(const MlpShape& n) { return round_up(n.hidden, 16); }  // 32-byte rows for the epilogue's stores
@@ -808,21 +719,6 @@ struct Arena {
         void* p = base != nullptr ? base + used : nullptr;
         used += (bytes + 255) / 256 * 256;
         return p;
-    }
-};
-
-// A matrix as the product kernel reads it.
-struct Matrix {
-    const void* base = nullptr;
-    long long rows = 0;
-    long long cols = 0;
-    long long pitch = 0;
-    int planes = 1;
-    bool is_bf16 = true;
-
-    CUtensorMap map(int box_rows) const
-    {
-        return umma::matrix_map(base, is_bf16, rows, cols, pitch, planes, rows * pitch, box_rows);
     }
 };
 
@@ -947,8 +843,8 @@ std::size_t forward_bytes(const MlpShape& n)
 }
 
 template <class T>
-void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, void* y, const MlpShape& n, void* work,
-                 cudaStream_t stream)
+void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, void* y, int dtype, const MlpShape& n,
+                 void* work, cudaStream_t stream)
 {
     Arena arena{reinterpret_cast<unsigned char*>((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255})};
     if (n.tokens <= kFewTokens) {
@@ -960,6 +856,12 @@ void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, 
     const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, stream);
     const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, stream);
     const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, stream);
+    if constexpr (sizeof(T) == 2) {
+        if (narrow_forward_fits(n, dtype)) {
+            narrow_forward(mx, mg, mu, md, y, dtype, n, stream);
+            return;
+        }
+    }
     const Matrix mh = hidden_matrix<T>(n, arena);
     {
         constexpr int BN = sizeof(T) == 4 ? 64 : 128;
@@ -1042,7 +944,7 @@ std::size_t backward_bytes(const MlpShape& n)
     }
     Args g;
     set_weight_tiles<T>(g, n);
-    arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts);
+    arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * std::max(g.parts, narrow_backward_parts(n)));
     return arena.used + 256;
 }
 
@@ -1062,6 +964,23 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
     const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, stream);
     const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, stream);
     const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, stream);
+    const long long size0 = static_cast<long long>(n.hidden) * n.channels;
+    const long long size2 = static_cast<long long>(n.outputs) * n.hidden;
+    const long long part_size = 2 * size0 + size2;
+    const auto add_parts = [&](const float* partial, int parts) {
+        const unsigned grid = static_cast<unsigned>(std::min<long long>((part_size + 31) / 32, 148 * 8));
+        launch_pdl(weight_sum_kernel<T>, dim3(grid), dim3(256), 0, stream, partial, static_cast<T*>(dwg), static_cast<T*>(dwu),
+                   static_cast<T*>(dwd), size0, size2, part_size, parts);
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (narrow_backward_fits(n, dtype)) {
+            const int parts = narrow_backward_parts(n);
+            auto* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(part_size) * parts));
+            narrow_backward(mdy, mx, mg, mu, md, dx, partial, dtype, n, stream);
+            add_parts(partial, parts);
+            return;
+        }
+    }
     const Matrix mdg = hidden_matrix<T>(n, arena);
     const Matrix mdu = hidden_matrix<T>(n, arena);
     const Matrix mh = hidden_matrix<T>(n, arena);
@@ -1113,11 +1032,7 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         float* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts));
         g.out[0] = partial;
         launch_product<Kind::kWeight, kWeightBN<T>, T, SPECTRAL_ACT_NONE>(maps, g, stream);
-        const long long size0 = static_cast<long long>(n.hidden) * n.channels;
-        const long long size2 = static_cast<long long>(n.outputs) * n.hidden;
-        const unsigned grid = static_cast<unsigned>(std::min<long long>((g.part_size + 255) / 256, 148 * 8));
-        launch_pdl(weight_sum_kernel<T>, dim3(grid), dim3(256), 0, stream, static_cast<const float*>(partial),
-                   static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dwd), size0, size2, g.part_size, g.parts);
+        add_parts(partial, g.parts);
     }
 }
 
@@ -1206,7 +1121,7 @@ extern "C" int spectral_gated_mlp(const void* x, const void* w_gate, const void*
     try {
         const MlpShape n{tokens, channels, hidden, outputs, activation};
         with_dtype(dtype, [&](auto t) {
-            mlp_forward<decltype(t)>(x, w_gate, w_up, w_down, y, n, work, static_cast<cudaStream_t>(stream));
+            mlp_forward<decltype(t)>(x, w_gate, w_up, w_down, y, dtype, n, work, static_cast<cudaStream_t>(stream));
         });
         return SPECTRAL_OK;
     } catch (const std::exception& e) {

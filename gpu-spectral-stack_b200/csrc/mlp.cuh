@@ -1,0 +1,144 @@
+#pragma once
+
+// What the feed-forward block's kernels share: operand types and their splitting, the stores of
+// their epilogues, and the host's view of a matrix.
+
+#include "backend.hpp"
+#include "launch.cuh"
+#include "pointwise.cuh"
+#include "umma.cuh"
+
+namespace spectral::mlp {
+
+constexpr int kTileM = 128;
+constexpr int kChunk = umma::kAtom;  // K per stage
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kTileABytes = kTileM * umma::kRowBytes;
+constexpr int kMaxSmem = 227 * 1024;
+
+// The type matrix products run in, and the parts an operand of T is split into.
+template <class T>
+struct Operand {
+    using Type = T;
+    static constexpr int kPlanes = 1;
+    static constexpr int kProducts = 1;
+    static constexpr int kPassChunks = 1 << 24;  // one pass over all of K
+};
+template <>
+struct Operand<float> {
+    using Type = bf16;
+    static constexpr int kPlanes = 3;
+    static constexpr int kProducts = 6;
+    static constexpr int kPassChunks = 2;
+};
+
+// Parts (a, b) of a float32 product's p-th MMA, the small ones first: (2,0) (0,2) (1,1) (1,0) (0,1)
+// (0,0), two bits each. Other types have one part.
+template <class T>
+__device__ __forceinline__ int part_a(int p) { return sizeof(T) == 4 ? (0b00'00'01'01'00'10 >> (2 * p)) & 3 : 0; }
+template <class T>
+__device__ __forceinline__ int part_b(int p) { return sizeof(T) == 4 ? (0b00'01'00'01'10'00 >> (2 * p)) & 3 : 0; }
+
+// v = hi + mid + lo in bf16 parts (exact but for parts below bf16's smallest). A hi that would round to
+// infinity is cut instead, and an infinity or NaN has no further parts.
+__device__ __forceinline__ void split3(float v, bf16& hi, bf16& mid, bf16& lo)
+{
+    hi = __float2bfloat16_rn(v);
+    if (fabsf(v) > 3.3895313892515355e38f && fabsf(v) <= 3.4028234663852886e38f) {
+        hi = __float2bfloat16_rz(v);
+    }
+    const float r = fabsf(v) <= 3.4028234663852886e38f ? v - __bfloat162float(hi) : 0.0f;
+    mid = __float2bfloat16_rn(r);
+    lo = __float2bfloat16_rn(r - __bfloat162float(mid));
+}
+
+// A run of 32 values of one row; only the first `valid` exist.
+template <class T>
+__device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
+{
+    constexpr int kPer = 32 / static_cast<int>(sizeof(T));  // values per 32 bytes
+    if (valid >= 32 && (reinterpret_cast<std::uintptr_t>(p) & 31u) == 0) {
+#pragma unroll
+        for (int i = 0; i < 32 / kPer; ++i) {
+            uint32_t w[8];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = __float_as_uint(v[i * kPer + j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    Vec<T, 2> two{{v[i * kPer + 2 * j], v[i * kPer + 2 * j + 1]}};
+                    w[j] = *reinterpret_cast<uint32_t*>(&two);
+                }
+            }
+            store32(p + i * kPer, w);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (j < valid) {
+                p[j] = v[j];
+            }
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[32], int valid)
+{
+    T out[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        out[j] = from_float<T>(v[j]);
+    }
+    store_run(p, out, valid);
+}
+
+// This warp has read the accumulator set that `bar` guards.
+__device__ __forceinline__ void release(uint64_t* bar, int lane)
+{
+    umma::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) {
+        umma::arrive(bar);
+    }
+}
+
+struct MlpShape {
+    long long tokens;
+    int channels;
+    int hidden;
+    int outputs;
+    int act;
+};
+
+// A matrix as the product kernel reads it.
+struct Matrix {
+    const void* base = nullptr;
+    long long rows = 0;
+    long long cols = 0;
+    long long pitch = 0;
+    int planes = 1;
+    bool is_bf16 = true;
+
+    CUtensorMap map(int box_rows) const
+    {
+        return umma::matrix_map(base, is_bf16, rows, cols, pitch, planes, rows * pitch, box_rows);
+    }
+};
+
+// The forward and backward passes with everything but x, y, dy, dx and the weights on chip
+// (mlp_narrow.cu). The matrices are in the operand form, of type `dtype` (16 bits).
+bool narrow_forward_fits(const MlpShape& n, int dtype);
+void narrow_forward(const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd, void* y, int dtype,
+                    const MlpShape& n, cudaStream_t stream);
+bool narrow_backward_fits(const MlpShape& n, int dtype);
+// The CTAs of a backward call: each leaves its sums of the three weight gradients, back to back, in `partial`.
+int narrow_backward_parts(const MlpShape& n);
+void narrow_backward(const Matrix& dy, const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd, void* dx,
+                     float* partial, int dtype, const MlpShape& n, cudaStream_t stream);
+
+}  // namespace spectral::mlp
