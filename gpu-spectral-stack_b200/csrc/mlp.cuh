@@ -53,14 +53,14 @@ __device__ __forceinline__ void split3(float v, bf16& hi, bf16& mid, bf16& lo)
     lo = __float2bfloat16_rn(r - __bfloat162float(mid));
 }
 
-// A run of 32 values of one row; only the first `valid` exist.
-template <class T>
-__device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
+// A run of N (16 or 32) values of one row; only the first `valid` exist.
+template <class T, int N>
+__device__ __forceinline__ void store_run(T* p, const T (&v)[N], int valid)
 {
     constexpr int kPer = 32 / static_cast<int>(sizeof(T));  // values per 32 bytes
-    if (valid >= 32 && (reinterpret_cast<std::uintptr_t>(p) & 31u) == 0) {
+    if (valid >= N && (reinterpret_cast<std::uintptr_t>(p) & 31u) == 0) {
 #pragma unroll
-        for (int i = 0; i < 32 / kPer; ++i) {
+        for (int i = 0; i < N / kPer; ++i) {
             uint32_t w[8];
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -78,7 +78,7 @@ __device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             if (j < valid) {
                 p[j] = v[j];
             }
@@ -86,12 +86,12 @@ __device__ __forceinline__ void store_run(T* p, const T (&v)[32], int valid)
     }
 }
 
-template <class T>
-__device__ __forceinline__ void store_values(T* p, const float (&v)[32], int valid)
+template <class T, int N>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[N], int valid)
 {
-    T out[32];
+    T out[N];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < N; ++j) {
         out[j] = from_float<T>(v[j]);
     }
     store_run(p, out, valid);

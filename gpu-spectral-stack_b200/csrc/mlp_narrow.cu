@@ -3,7 +3,7 @@
 // SM, so HBM carries only x and y (backward: x, dy and dx).
 //
 // Both kernels are persistent, one CTA per SM, tiles of 128 tokens: a TMA warp, an MMA warp (one
-// elected lane issues) and eight epilogue warps; the hidden values in chunks of 64. The next chunk's
+// elected lane issues) and sixteen epilogue warps; the hidden values in chunks of 64. The next chunk's
 // products are issued before the current chunk's second ones, so the tensor cores work under the
 // epilogue. Every wait is bounded (tma.cuh).
 //
@@ -36,6 +36,10 @@ constexpr int kHiddenChunk = 64;
 constexpr int kTileBytes = kTileM * umma::kRowBytes;  // 128 tokens x 64 values: 16 KiB
 constexpr int kWeightBytes = kHiddenChunk * umma::kRowBytes;  // 64 x 64 weights: 8 KiB
 
+// Sixteen epilogue warps, the TMA warp, the MMA warp.
+constexpr int kWarps = 16;
+constexpr int kNarrowThreads = 32 * (kWarps + 2);
+
 struct NarrowMaps {
     CUtensorMap x;
     CUtensorMap dy;
@@ -62,12 +66,13 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece)
     return static_cast<uint32_t>(row * umma::kRowBytes + ((piece ^ (row & 7)) << 4));
 }
 
-// 32 values of one row, rounded to T, into columns [32 half, 32 half + 32) of a tile at shared address `tile`.
-template <class T>
-__device__ __forceinline__ void put_row(uint32_t tile, int row, int half, const float (&v)[32])
+// N (16 or 32) values of one row, rounded to T, into columns [N part, N part + N) of a tile at shared
+// address `tile`.
+template <class T, int N>
+__device__ __forceinline__ void put_row(uint32_t tile, int row, int part, const float (&v)[N])
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N / 8; ++i) {
         Floats<8> f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -75,7 +80,7 @@ __device__ __forceinline__ void put_row(uint32_t tile, int row, int half, const 
         }
         const Vec<T, 8> w = narrow<T>(f);
         const auto* u = reinterpret_cast<const uint32_t*>(&w);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + swizzled(row, 4 * half + i)), "r"(u[0]),
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + swizzled(row, N / 8 * part + i)), "r"(u[0]),
                      "r"(u[1]), "r"(u[2]), "r"(u[3])
                      : "memory");
     }
@@ -111,6 +116,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, bool writes)
 
 // --- forward -------------------------------------------------------------------------------------------
 
+// The epilogue warps work in two groups of eight, on every second chunk each: a chunk's way from the
+// accumulator through the activation to shared memory is mostly latency (one group took 1650 cycles a
+// chunk with no activation at all).
+constexpr int kGroupWarps = kWarps / 2;
+
 // CK and DK: channels and outputs in 64s (1 or 2).
 template <int CK, int DK>
 struct Forward {
@@ -122,7 +132,7 @@ struct Forward {
 };
 
 template <class T, int Act, int CK, int DK>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kNarrowThreads, 1)
     narrow_forward_kernel(const __grid_constant__ NarrowMaps maps, const __grid_constant__ NarrowArgs g)
 {
     using F = Forward<CK, DK>;
@@ -141,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ int gave_up;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == kEpilogueWarps) {
+    if (warp == kWarps) {
         umma::alloc<512>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
@@ -151,11 +161,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma::mbar_init(&x_full[i], 1);
             tma::mbar_init(&x_empty[i], 1);
             tma::mbar_init(&gu_full[i], 1);
-            tma::mbar_init(&gu_empty[i], kEpilogueWarps);
-            tma::mbar_init(&h_full[i], kEpilogueWarps);
+            tma::mbar_init(&gu_empty[i], kGroupWarps);
+            tma::mbar_init(&h_full[i], kGroupWarps);
             tma::mbar_init(&h_empty[i], 1);
             tma::mbar_init(&y_full[i], 1);
-            tma::mbar_init(&y_empty[i], kEpilogueWarps);
+            tma::mbar_init(&y_empty[i], kGroupWarps);
         }
         gave_up = 0;
         tma::fence_mbar_init();
@@ -169,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     wait_for_previous_grid();
     bool ok = true;
 
-    if (warp == kEpilogueWarps) {
+    if (warp == kWarps) {
         asm volatile("fence.proxy.async.global;" ::: "memory");
         if (umma::elect_one()) {
             tma::mbar_arrive_expect_tx(&weights_full, static_cast<unsigned>(chunks * F::kChunkBytes));
@@ -210,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 atomicOr(g.fault, tma::kFaultDrainTimeout);
             }
         }
-    } else if (warp == kEpilogueWarps + 1) {
+    } else if (warp == kWarps + 1) {
         Turn<2> x, gu, h, y;
         // [G U] of one chunk; the last chunk of a tile releases its x.
         const auto first = [&](int j) {
@@ -290,69 +300,69 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
+        const int group = warp / kGroupWarps;
         const int quad = warp & 3;
-        const int half = warp >> 2;
+        const int half = warp % kGroupWarps >> 2;
         const int row = quad * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-        Turn<2> gu, h, y;
-        // The outputs of tile t, once its last product is done.
-        const auto store_y = [&](int t) {
-            ok = tma::mbar_wait(&y_full[y.at], y.phase);
+        const int stride = static_cast<int>(gridDim.x);
+        const int mine = g.tiles > static_cast<int>(blockIdx.x) ? (g.tiles - static_cast<int>(blockIdx.x) + stride - 1) / stride : 0;
+        const int total = mine * chunks;
+        // The outputs of this CTA's k-th tile, once its last product is done. Group k % 2 stores them from
+        // accumulator k % 2.
+        const auto store_y = [&](int k) {
+            ok = tma::mbar_wait(&y_full[group], static_cast<unsigned>(k >> 1) & 1u);
             if (!ok) {
                 return;
             }
             umma::fence_after_sync();
-            const long long token = static_cast<long long>(t) * kTileM + row;
+            const long long token = (static_cast<long long>(blockIdx.x) + static_cast<long long>(k) * stride) * kTileM + row;
 #pragma unroll
             for (int d = 0; d < DK; ++d) {
                 float v[32];
                 const int col = 64 * d + 32 * half;
-                umma::load32(tmem_y + lanes + y.at * F::kYCols + col, v);
+                umma::load32(tmem_y + lanes + group * F::kYCols + col, v);
                 umma::load_wait(v);
                 if (token < g.tokens && col < g.outputs) {
                     store_values<T>(static_cast<T*>(g.out) + token * g.outputs + col, v, min(32, g.outputs - col));
                 }
             }
-            warp_arrive(&y_empty[y.at], false);
-            y.next();
+            warp_arrive(&y_empty[group], false);
         };
-        int before = -1;  // the tile whose outputs are still to be stored
-        for (int t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
-            for (int j = 0; ok && j < chunks; ++j) {
-                ok = tma::mbar_wait(&gu_full[gu.at], gu.phase);
-                if (!ok) {
-                    break;
-                }
-                umma::fence_after_sync();
-                float a[32], u[32];
-                umma::load32(tmem + lanes + gu.at * 128 + 32 * half, a);
-                umma::load32(tmem + lanes + gu.at * 128 + 64 + 32 * half, u);
-                umma::load_wait(a);
-                umma::load_wait(u);
-                warp_arrive(&gu_empty[gu.at], false);
-                gu.next();
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 v = activate2<Act, T>(make_float2(a[i], a[i + 1])) * make_float2(u[i], u[i + 1]);
-                    a[i] = v.x;
-                    a[i + 1] = v.y;
-                }
-                ok = tma::mbar_wait(&h_empty[h.at], h.phase ^ 1u);
-                if (!ok) {
-                    break;
-                }
-                put_row<T>(hs + h.at * kTileBytes, row, half, a);
-                warp_arrive(&h_full[h.at], true);
-                h.next();
-                if (j == 0 && before >= 0) {
-                    store_y(before);
-                    before = -1;
-                }
+        int stored = group;  // the group's next tile to store
+        for (int n = group; ok && n < total; n += 2) {
+            const unsigned phase = static_cast<unsigned>(n >> 1) & 1u;  // buffer n % 2 is this group's
+            ok = tma::mbar_wait(&gu_full[group], phase);
+            if (!ok) {
+                break;
             }
-            before = t;
+            umma::fence_after_sync();
+            float a[32], u[32];
+            umma::load32(tmem + lanes + group * 128 + 32 * half, a);
+            umma::load32(tmem + lanes + group * 128 + 64 + 32 * half, u);
+            umma::load_wait(a);
+            umma::load_wait(u);
+            warp_arrive(&gu_empty[group], false);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float2 v = activate2<Act, T>(make_float2(a[i], a[i + 1])) * make_float2(u[i], u[i + 1]);
+                a[i] = v.x;
+                a[i + 1] = v.y;
+            }
+            ok = tma::mbar_wait(&h_empty[group], phase ^ 1u);
+            if (!ok) {
+                break;
+            }
+            put_row<T>(hs + group * kTileBytes, row, half, a);
+            warp_arrive(&h_full[group], true);
+            // A tile whose last chunk is behind this one needs nothing more of this group.
+            if ((stored + 1) * chunks <= n) {
+                store_y(stored);
+                stored += 2;
+            }
         }
-        if (ok && before >= 0) {
-            store_y(before);
+        for (; ok && stored < mine; stored += 2) {
+            store_y(stored);
         }
     }
     if (!ok && lane == 0) {
@@ -364,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && gave_up != 0) {
         atomicOr(g.fault, tma::kFaultWaitTimeout);
     }
-    if (warp == kEpilogueWarps) {
+    if (warp == kWarps) {
         umma::dealloc<512>(tmem);
     }
 }
@@ -383,7 +393,7 @@ constexpr int kColGateUp = 320;    // two chunks of 64
 constexpr int kColDown = 448;
 
 template <class T, int Act>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kNarrowThreads, 1)
     narrow_backward_kernel(const __grid_constant__ NarrowMaps maps, const __grid_constant__ NarrowArgs g)
 {
     constexpr bool kBf16 = std::is_same_v<T, bf16>;
@@ -403,22 +413,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ int gave_up;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == kEpilogueWarps) {
+    if (warp == kWarps) {
         umma::alloc<512>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
         tma::mbar_init(&weights_full, 1);
         tma::mbar_init(&acc_full, 1);
-        tma::mbar_init(&acc_empty, kEpilogueWarps);
+        tma::mbar_init(&acc_empty, kWarps);
         tma::mbar_init(&all_done, 1);
         tma::mbar_init(&drain, 1);
         for (int i = 0; i < 2; ++i) {
             tma::mbar_init(&in_full[i], 1);
             tma::mbar_init(&in_empty[i], 1);
-            tma::mbar_init(&hidden_full[i], kEpilogueWarps);
+            tma::mbar_init(&hidden_full[i], kWarps);
             tma::mbar_init(&hidden_empty[i], 1);
             tma::mbar_init(&dx_full[i], 1);
-            tma::mbar_init(&dx_empty[i], kEpilogueWarps);
+            tma::mbar_init(&dx_empty[i], kWarps);
         }
         gave_up = 0;
         tma::fence_mbar_init();
@@ -434,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     wait_for_previous_grid();
     bool ok = true;
 
-    if (warp == kEpilogueWarps) {
+    if (warp == kWarps) {
         asm volatile("fence.proxy.async.global;" ::: "memory");
         if (umma::elect_one()) {
             tma::mbar_arrive_expect_tx(&weights_full, static_cast<unsigned>(chunks * kBackChunkWeights));
@@ -472,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 atomicOr(g.fault, tma::kFaultDrainTimeout);
             }
         }
-    } else if (warp == kEpilogueWarps + 1) {
+    } else if (warp == kWarps + 1) {
         Turn<2> ahead, in, dx;  // the input stage of the first products, of the second ones; the dx accumulator
         Turn<1> acc, hidden;    // phases of the chunk accumulator, and of a chunk's hidden tiles
         const auto first = [&](int j) {
@@ -575,12 +585,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         const int quad = warp & 3;
-        const int half = warp >> 2;
+        const int part = warp >> 2;  // 16 of a chunk's 64 columns
         const int row = quad * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         if (chunks == 1) {  // the other chunk's h takes part in the last product
-            const float zero[32] = {};
-            put_row<T>(hs + kTileBytes, row, half, zero);
+            const float zero[16] = {};
+            put_row<T>(hs + kTileBytes, row, part, zero);
         }
         Turn<1> acc, hidden;
         Turn<2> dx;
@@ -590,15 +600,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return;
             }
             umma::fence_after_sync();
-            float v[32];
-            umma::load32(tmem + lanes + kColDx + dx.at * 64 + 32 * half, v);
+            float v[16];
+            umma::load16(tmem + lanes + kColDx + dx.at * 64 + 16 * part, v);
             umma::load_wait(v);
             warp_arrive(&dx_empty[dx.at], false);
             dx.next();
             const long long token = static_cast<long long>(t) * kTileM + row;
-            const int col = 32 * half;
+            const int col = 16 * part;
             if (token < g.tokens && col < g.channels) {
-                store_values<T>(static_cast<T*>(g.out) + token * g.channels + col, v, min(32, g.channels - col));
+                store_values<T>(static_cast<T*>(g.out) + token * g.channels + col, v, min(16, g.channels - col));
             }
         };
         int before = -1;
@@ -609,17 +619,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 umma::fence_after_sync();
-                float a[32], u[32], dh[32];
-                umma::load32(tmem + lanes + 32 * half, a);
-                umma::load32(tmem + lanes + 64 + 32 * half, u);
-                umma::load32(tmem + lanes + 128 + 32 * half, dh);
+                float a[16], u[16], dh[16];
+                umma::load16(tmem + lanes + 16 * part, a);
+                umma::load16(tmem + lanes + 64 + 16 * part, u);
+                umma::load16(tmem + lanes + 128 + 16 * part, dh);
                 umma::load_wait(a);
                 umma::load_wait(u);
                 umma::load_wait(dh);
                 warp_arrive(&acc_empty, false);
                 acc.next();
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
+                for (int i = 0; i < 16; i += 2) {
                     float2 slope;
                     const float2 up = make_float2(u[i], u[i + 1]);
                     const float2 d = make_float2(dh[i], dh[i + 1]);
@@ -636,9 +646,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) {
                     break;
                 }
-                put_row<T>(dgs + j * 2 * kTileBytes, row, half, a);
-                put_row<T>(dgs + j * 2 * kTileBytes + kTileBytes, row, half, dh);
-                put_row<T>(hs + j * kTileBytes, row, half, u);
+                put_row<T>(dgs + j * 2 * kTileBytes, row, part, a);
+                put_row<T>(dgs + j * 2 * kTileBytes + kTileBytes, row, part, dh);
+                put_row<T>(hs + j * kTileBytes, row, part, u);
                 warp_arrive(&hidden_full[j], true);
                 if (j == 0 && before >= 0) {
                     store_dx(before);
@@ -658,31 +668,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok) {
             umma::fence_after_sync();
-            float* part = g.partial + blockIdx.x * g.part_size;
+            float* sums = g.partial + blockIdx.x * g.part_size;
             const long long size = static_cast<long long>(g.hidden) * g.channels;
-            const int col = 32 * half;
+            const int col = 16 * part;
             for (int j = 0; j < chunks; ++j) {
-                float v[32] = {};
+                float v[16] = {};
                 if (mine > 0) {
-                    umma::load32(tmem + lanes + kColGateUp + 64 * j + col, v);
+                    umma::load16(tmem + lanes + kColGateUp + 64 * j + col, v);
                     umma::load_wait(v);
                 }
                 const int f = 64 * j + (row & 63);
                 if (f < g.hidden && col < g.channels) {
-                    store_values<float>(part + (row >> 6) * size + static_cast<long long>(f) * g.channels + col, v,
-                                        min(32, g.channels - col));
+                    store_values<float>(sums + (row >> 6) * size + static_cast<long long>(f) * g.channels + col, v,
+                                        min(16, g.channels - col));
                 }
             }
-            float v[32] = {};
+            float v[16] = {};
             if (mine > 0) {
-                umma::load32(tmem + lanes + kColDown + col, v);
+                umma::load16(tmem + lanes + kColDown + col, v);
                 umma::load_wait(v);
             }
             if (row < g.hidden) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < 16; ++i) {
                     if (col + i < g.outputs) {
-                        part[2 * size + static_cast<long long>(col + i) * g.hidden + row] = v[i];
+                        sums[2 * size + static_cast<long long>(col + i) * g.hidden + row] = v[i];
                     }
                 }
             }
@@ -697,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && gave_up != 0) {
         atomicOr(g.fault, tma::kFaultWaitTimeout);
     }
-    if (warp == kEpilogueWarps) {
+    if (warp == kWarps) {
         umma::dealloc<512>(tmem);
     }
 }
@@ -728,7 +738,7 @@ void launch(int ctas, int smem, const NarrowMaps& maps, const NarrowArgs& g, cud
         SPECTRAL_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem - 1024));
         opted[device].store(true, std::memory_order_relaxed);
     }
-    launch_pdl(Kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), static_cast<std::size_t>(smem), stream, maps, g);
+    launch_pdl(Kernel, dim3(static_cast<unsigned>(ctas)), dim3(kNarrowThreads), static_cast<std::size_t>(smem), stream, maps, g);
 }
 
 int forward_smem(const MlpShape& n)
