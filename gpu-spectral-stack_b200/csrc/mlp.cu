@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             }
         }
     } else if (warp == kEpilogueWarps + 1) {
-        // The MMA warp.
+        // The MMA warp: converged, so that addresses and descriptors stay warp-uniform, one elected lane
+        // issues (one lane throughout measured 10 % slower).
         constexpr bool kBMnFirst = K == Kind::kWeight || K == Kind::kInput;
         constexpr uint32_t kFirst = umma::instruction(kBf16, Cfg::kAMn, kBMnFirst, kTileM, Cfg::kBRows);
         constexpr uint32_t kSecond =
@@ -413,15 +414,20 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         const uint32_t a = base + stage * Cfg::kStageBytes;
                         const uint32_t b = a + kTileABytes;
                         if (umma::elect_one()) {
+                            const uint64_t da = Cfg::kAMn ? umma::desc_mn<8192>(a) : umma::desc_k(a);
+                            constexpr uint64_t kStepA = Cfg::kAMn ? umma::kStepMn : umma::kStepK;
+                            if (K == Kind::kGateBack && pair == 1) {
+                                const uint64_t db = umma::desc_mn<8192>(b);
 #pragma unroll
-                            for (int s = 0; s < kChunk / 16; ++s) {
-                                const bool more = !fresh || i > 0 || s > 0;
-                                const uint64_t da = Cfg::kAMn ? umma::desc_mn(a, s, 8192) : umma::desc_k(a, s);
-                                if (K == Kind::kGateBack && pair == 1) {
-                                    umma::mma(d, da, umma::desc_mn(b, s, 8192), kSecond, more);
-                                } else {
-                                    umma::mma(d, da, kBMnFirst ? umma::desc_mn(b, s, 8192) : umma::desc_k(b, s), kFirst,
-                                              more);
+                                for (int s = 0; s < kChunk / 16; ++s) {
+                                    umma::mma(d, da + kStepA * s, db + umma::kStepMn * s, kSecond, !fresh || i > 0 || s > 0);
+                                }
+                            } else {
+                                const uint64_t db = kBMnFirst ? umma::desc_mn<8192>(b) : umma::desc_k(b);
+                                constexpr uint64_t kStepB = kBMnFirst ? umma::kStepMn : umma::kStepK;
+#pragma unroll
+                                for (int s = 0; s < kChunk / 16; ++s) {
+                                    umma::mma(d, da + kStepA * s, db + kStepB * s, kFirst, !fresh || i > 0 || s > 0);
                                 }
                             }
                             umma::commit(&empty[stage]);

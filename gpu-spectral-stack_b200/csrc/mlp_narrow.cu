@@ -2,10 +2,10 @@
 // channels, very many tokens. Its weights fit in shared memory and its hidden values never leave the
 // SM, so HBM carries only x and y (backward: x, dy and dx).
 //
-// Both kernels are persistent, one CTA per SM, tiles of 128 tokens: a TMA warp, an MMA warp (one
-// elected lane issues) and sixteen epilogue warps; the hidden values in chunks of 64. The next chunk's
-// products are issued before the current chunk's second ones, so the tensor cores work under the
-// epilogue. Every wait is bounded (tma.cuh).
+// Both kernels are persistent, one CTA per SM, tiles of 128 tokens: a TMA warp, two MMA warps (one for
+// the products that lead to the hidden values, one for those that use them, so that the first run
+// ahead while the epilogue works) and sixteen epilogue warps; the hidden values in chunks of 64.
+// Every wait is bounded (tma.cuh).
 //
 // Forward, chunk j:  [G U] = x [Wg_j; Wu_j]^T   (N = 128, one accumulator set of two)
 //                    h = act(G) * U, rounded, into shared memory as the next A operand
@@ -36,9 +36,12 @@ constexpr int kHiddenChunk = 64;
 constexpr int kTileBytes = kTileM * umma::kRowBytes;  // 128 tokens x 64 values: 16 KiB
 constexpr int kWeightBytes = kHiddenChunk * umma::kRowBytes;  // 64 x 64 weights: 8 KiB
 
-// Sixteen epilogue warps, the TMA warp, the MMA warp.
+// Sixteen epilogue warps, the TMA warp, and two that issue MMAs. The latter run as one lane each from
+// start to end: a wait costs it some 75 to 100 cycles even where nothing is left to wait for, a
+// commit 50, and as one warp with an elected lane per step the two products of a chunk took 1500 cycles
+// to issue, three times what they take to run.
 constexpr int kWarps = 16;
-constexpr int kNarrowThreads = 32 * (kWarps + 2);
+constexpr int kNarrowThreads = 32 * (kWarps + 3);
 
 struct NarrowMaps {
     CUtensorMap x;
@@ -114,6 +117,17 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, bool writes)
     }
 }
 
+// The end of an MMA warp that gave up: waits (bounded) for the MMAs it issued.
+__device__ __forceinline__ void drain_on_failure(bool ok, uint64_t* bar, unsigned* fault)
+{
+    if (!ok) {
+        umma::commit(bar);
+        if (!tma::mbar_wait(bar, 0)) {
+            atomicOr(fault, tma::kFaultDrainTimeout);
+        }
+    }
+}
+
 // --- forward -------------------------------------------------------------------------------------------
 
 // The epilogue warps work in two groups of eight, on every second chunk each: a chunk's way from the
@@ -125,8 +139,9 @@ constexpr int kGroupWarps = kWarps / 2;
 template <int CK, int DK>
 struct Forward {
     static constexpr int kXBytes = CK * kTileBytes;
+    static constexpr int kXStages = CK == 1 ? 4 : 2;  // tiles of x in flight or in use
     static constexpr int kChunkBytes = CK * 2 * kWeightBytes + DK * kWeightBytes;  // [Wg; Wu] per 64 channels, Wd
-    static constexpr int kFixed = 2 * kXBytes + 2 * kTileBytes + 2048;
+    static constexpr int kFixed = kXStages * kXBytes + 2 * kTileBytes + 2048;
     static constexpr int kYCols = DK * 64;
     static constexpr int smem(int chunks) { return kFixed + chunks * kChunkBytes; }
 };
@@ -142,11 +157,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     allow_next_grid();
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
-    const uint32_t xs = base;                       // two tiles of x
-    const uint32_t hs = xs + 2 * F::kXBytes;        // two chunks of h
+    const uint32_t xs = base;                       // tiles of x
+    const uint32_t hs = xs + F::kXStages * F::kXBytes;  // two chunks of h
     const uint32_t ws = hs + 2 * kTileBytes;        // the weights, by chunk
-    __shared__ uint64_t weights_full, x_full[2], x_empty[2], gu_full[2], gu_empty[2], h_full[2], h_empty[2], y_full[2],
-        y_empty[2], drain;
+    __shared__ uint64_t weights_full, x_full[F::kXStages], x_empty[F::kXStages], gu_full[2], gu_empty[2], h_full[2], h_empty[2], y_full[2],
+        y_empty[2], drain[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     const int warp = threadIdx.x >> 5;
@@ -156,16 +171,18 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     }
     if (threadIdx.x == 0) {
         tma::mbar_init(&weights_full, 1);
-        tma::mbar_init(&drain, 1);
         for (int i = 0; i < 2; ++i) {
-            tma::mbar_init(&x_full[i], 1);
-            tma::mbar_init(&x_empty[i], 1);
+            tma::mbar_init(&drain[i], 1);
             tma::mbar_init(&gu_full[i], 1);
             tma::mbar_init(&gu_empty[i], kGroupWarps);
             tma::mbar_init(&h_full[i], kGroupWarps);
             tma::mbar_init(&h_empty[i], 1);
             tma::mbar_init(&y_full[i], 1);
             tma::mbar_init(&y_empty[i], kGroupWarps);
+        }
+        for (int i = 0; i < F::kXStages; ++i) {
+            tma::mbar_init(&x_full[i], 1);
+            tma::mbar_init(&x_empty[i], 1);
         }
         gave_up = 0;
         tma::fence_mbar_init();
@@ -176,6 +193,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     const uint32_t tmem = tmem_slot;
     const uint32_t tmem_y = tmem + 256;
     const int chunks = (g.hidden + kHiddenChunk - 1) / kHiddenChunk;
+    const int stride = static_cast<int>(gridDim.x);
+    const int mine = g.tiles > static_cast<int>(blockIdx.x) ? (g.tiles - static_cast<int>(blockIdx.x) + stride - 1) / stride : 0;
     wait_for_previous_grid();
     bool ok = true;
 
@@ -195,7 +214,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
             }
         }
         __syncwarp();
-        Turn<2> x;
+        Turn<F::kXStages> x;
         int issued = 0;
         for (int t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
             ok = tma::mbar_wait(&x_empty[x.at], x.phase ^ 1u);
@@ -213,91 +232,72 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         }
         if (!ok) {  // let the loads in flight land (bounded) before the shared memory is given up
             bool drained = tma::mbar_wait(&weights_full, 0);
-            for (int i = issued > 2 ? issued - 2 : 0; i < issued; ++i) {
-                drained = tma::mbar_wait(&x_full[i % 2], static_cast<unsigned>(i / 2) & 1u) && drained;
+            for (int i = issued > F::kXStages ? issued - F::kXStages : 0; i < issued; ++i) {
+                drained = tma::mbar_wait(&x_full[i % F::kXStages], static_cast<unsigned>(i / F::kXStages) & 1u) && drained;
             }
             if (lane == 0 && !drained) {
                 atomicOr(g.fault, tma::kFaultDrainTimeout);
             }
         }
     } else if (warp == kWarps + 1) {
-        Turn<2> x, gu, h, y;
-        // [G U] of one chunk; the last chunk of a tile releases its x.
-        const auto first = [&](int j) {
-            ok = (j > 0 || tma::mbar_wait(&x_full[x.at], x.phase)) && tma::mbar_wait(&gu_empty[gu.at], gu.phase ^ 1u);
-            if (!ok) {
-                return;
+        if (lane == 0) {  // [G U] of every chunk; a tile's last chunk releases its x
+            Turn<F::kXStages> x;
+            Turn<2> gu;
+            ok = tma::mbar_wait(&weights_full, 0);
+            for (int k = 0; ok && k < mine; ++k) {
+                ok = tma::mbar_wait(&x_full[x.at], x.phase);
+                for (int j = 0; ok && j < chunks; ++j) {
+                    ok = tma::mbar_wait(&gu_empty[gu.at], gu.phase ^ 1u);
+                    if (!ok) {
+                        break;
+                    }
+                    umma::fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < CK; ++c) {
+                        const uint64_t da = umma::desc_k(xs + x.at * F::kXBytes + c * kTileBytes);
+                        const uint64_t db = umma::desc_k(ws + j * F::kChunkBytes + c * 2 * kWeightBytes);
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            umma::mma(tmem + gu.at * 128, da + umma::kStepK * s, db + umma::kStepK * s, kFirst, c > 0 || s > 0);
+                        }
+                    }
+                    umma::commit(&gu_full[gu.at]);
+                    gu.next();
+                }
+                if (ok) {
+                    umma::commit(&x_empty[x.at]);
+                    x.next();
+                }
             }
-            umma::fence_after_sync();
-            if (umma::elect_one()) {
-                for (int c = 0; c < CK; ++c) {
-                    const uint32_t a = xs + x.at * F::kXBytes + c * kTileBytes;
-                    const uint32_t b = ws + j * F::kChunkBytes + c * 2 * kWeightBytes;
+            drain_on_failure(ok, &drain[0], g.fault);
+        }
+    } else if (warp == kWarps + 2) {
+        if (lane == 0) {  // y += h Wd^T of every chunk
+            Turn<2> h, y;
+            ok = tma::mbar_wait(&weights_full, 0);
+            for (int k = 0; ok && k < mine; ++k) {
+                ok = tma::mbar_wait(&y_empty[y.at], y.phase ^ 1u);
+                for (int j = 0; ok && j < chunks; ++j) {
+                    ok = tma::mbar_wait(&h_full[h.at], h.phase);
+                    if (!ok) {
+                        break;
+                    }
+                    umma::fence_after_sync();
+                    const uint64_t da = umma::desc_k(hs + h.at * kTileBytes);
+                    const uint64_t db = umma::desc_k(ws + j * F::kChunkBytes + CK * 2 * kWeightBytes);
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
-                        umma::mma(tmem + gu.at * 128, umma::desc_k(a, s), umma::desc_k(b, s), kFirst, c > 0 || s > 0);
+                        umma::mma(tmem_y + y.at * F::kYCols, da + umma::kStepK * s, db + umma::kStepK * s, kSecond, j > 0 || s > 0);
                     }
+                    umma::commit(&h_empty[h.at]);
+                    h.next();
                 }
-                umma::commit(&gu_full[gu.at]);
-                if (j == chunks - 1) {
-                    umma::commit(&x_empty[x.at]);
-                }
-            }
-            __syncwarp();
-            gu.next();
-            if (j == chunks - 1) {
-                x.next();
-            }
-        };
-        // y += h Wd^T of one chunk.
-        const auto second = [&](int j) {
-            ok = (j > 0 || tma::mbar_wait(&y_empty[y.at], y.phase ^ 1u)) && tma::mbar_wait(&h_full[h.at], h.phase);
-            if (!ok) {
-                return;
-            }
-            umma::fence_after_sync();
-            if (umma::elect_one()) {
-                const uint32_t a = hs + h.at * kTileBytes;
-                const uint32_t b = ws + j * F::kChunkBytes + CK * 2 * kWeightBytes;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    umma::mma(tmem_y + y.at * F::kYCols, umma::desc_k(a, s), umma::desc_k(b, s), kSecond, j > 0 || s > 0);
-                }
-                umma::commit(&h_empty[h.at]);
-                if (j == chunks - 1) {
+                if (ok) {
                     umma::commit(&y_full[y.at]);
+                    y.next();
                 }
             }
-            __syncwarp();
-            h.next();
-            if (j == chunks - 1) {
-                y.next();
-            }
-        };
-        ok = tma::mbar_wait(&weights_full, 0);
-        const int mine = g.tiles > static_cast<int>(blockIdx.x)
-                             ? (g.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x)
-                             : 0;
-        const int total = mine * chunks;
-        if (ok && total > 0) {
-            first(0);
-        }
-        for (int n = 0; ok && n < total; ++n) {
-            if (n + 1 < total) {
-                first((n + 1) % chunks);
-            }
-            if (ok) {
-                second(n % chunks);
-            }
-        }
-        if (!ok) {
-            if (umma::elect_one()) {
-                umma::commit(&drain);
-            }
-            __syncwarp();
-            if (!tma::mbar_wait(&drain, 0) && lane == 0) {
-                atomicOr(g.fault, tma::kFaultDrainTimeout);
-            }
+            drain_on_failure(ok, &drain[1], g.fault);
         }
     } else {
         const int group = warp / kGroupWarps;
@@ -305,8 +305,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         const int half = warp % kGroupWarps >> 2;
         const int row = quad * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-        const int stride = static_cast<int>(gridDim.x);
-        const int mine = g.tiles > static_cast<int>(blockIdx.x) ? (g.tiles - static_cast<int>(blockIdx.x) + stride - 1) / stride : 0;
         const int total = mine * chunks;
         // The outputs of this CTA's k-th tile, once its last product is done. Group k % 2 stores them from
         // accumulator k % 2.
@@ -407,8 +405,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     const uint32_t ws = ins + 4 * kTileBytes;           // [chunk][Wg, Wu, Wd]
     const uint32_t dgs = ws + 2 * kBackChunkWeights;    // [chunk][dG, dU]
     const uint32_t hs = dgs + 4 * kTileBytes;           // [chunk]
-    __shared__ uint64_t weights_full, in_full[2], in_empty[2], acc_full, acc_empty, hidden_full[2], hidden_empty[2],
-        dx_full[2], dx_empty[2], all_done, drain;
+    __shared__ uint64_t weights_full, in_full[2], in_empty[2], acc_full, acc_empty, hidden_full[2], dgu_empty[2], h_empty,
+        dx_full[2], dx_empty[2], all_done, drain[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     const int warp = threadIdx.x >> 5;
@@ -421,12 +419,13 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         tma::mbar_init(&acc_full, 1);
         tma::mbar_init(&acc_empty, kWarps);
         tma::mbar_init(&all_done, 1);
-        tma::mbar_init(&drain, 1);
+        tma::mbar_init(&h_empty, 1);
         for (int i = 0; i < 2; ++i) {
             tma::mbar_init(&in_full[i], 1);
-            tma::mbar_init(&in_empty[i], 1);
+            tma::mbar_init(&in_empty[i], 2);  // both MMA warps
+            tma::mbar_init(&drain[i], 1);
             tma::mbar_init(&hidden_full[i], kWarps);
-            tma::mbar_init(&hidden_empty[i], 1);
+            tma::mbar_init(&dgu_empty[i], 1);
             tma::mbar_init(&dx_full[i], 1);
             tma::mbar_init(&dx_empty[i], kWarps);
         }
@@ -483,105 +482,101 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
             }
         }
     } else if (warp == kWarps + 1) {
-        Turn<2> ahead, in, dx;  // the input stage of the first products, of the second ones; the dx accumulator
-        Turn<1> acc, hidden;    // phases of the chunk accumulator, and of a chunk's hidden tiles
-        const auto first = [&](int j) {
-            ok = (j > 0 || tma::mbar_wait(&in_full[ahead.at], ahead.phase)) && tma::mbar_wait(&acc_empty, acc.phase ^ 1u);
-            if (!ok) {
-                return;
-            }
-            umma::fence_after_sync();
-            if (umma::elect_one()) {
-                const uint32_t x = ins + ahead.at * 2 * kTileBytes;
-                const uint32_t w = ws + j * kBackChunkWeights;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    umma::mma(tmem, umma::desc_k(x, s), umma::desc_k(w, s), kGateUp, s > 0);
-                }
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    umma::mma(tmem + 128, umma::desc_k(x + kTileBytes, s), umma::desc_mn(w + 2 * kWeightBytes, s, kWeightBytes),
-                              kThrough, s > 0);
-                }
-                umma::commit(&acc_full);
-            }
-            __syncwarp();
-            acc.next();
-            if (j == chunks - 1) {
-                ahead.next();
-            }
-        };
-        const auto second = [&](int j, bool fresh) {  // fresh: the CTA's first tile
-            ok = (j > 0 || tma::mbar_wait(&dx_empty[dx.at], dx.phase ^ 1u)) && tma::mbar_wait(&hidden_full[j], hidden.phase);
-            if (!ok) {
-                return;
-            }
-            umma::fence_after_sync();
-            if (umma::elect_one()) {
-                const uint32_t x = ins + in.at * 2 * kTileBytes;
-                const uint32_t w = ws + j * kBackChunkWeights;
-                const uint32_t dg = dgs + j * 2 * kTileBytes;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {  // dG Wg, then dU Wu
+        if (lane == 0) {  // G, U and dh of every chunk
+            Turn<2> in;
+            Turn<1> acc;
+            ok = tma::mbar_wait(&weights_full, 0);
+            for (int k = 0; ok && k < mine; ++k) {
+                ok = tma::mbar_wait(&in_full[in.at], in.phase);
+                const uint64_t dx = umma::desc_k(ins + in.at * 2 * kTileBytes);
+                const uint64_t ddy = umma::desc_k(ins + in.at * 2 * kTileBytes + kTileBytes);
+                for (int j = 0; ok && j < chunks; ++j) {
+                    ok = tma::mbar_wait(&acc_empty, acc.phase ^ 1u);
+                    if (!ok) {
+                        break;
+                    }
+                    umma::fence_after_sync();
+                    const uint64_t dw = umma::desc_k(ws + j * kBackChunkWeights);
+                    const uint64_t dwd = umma::desc_mn<kWeightBytes>(ws + j * kBackChunkWeights + 2 * kWeightBytes);
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
-                        umma::mma(tmem + kColDx + dx.at * 64, umma::desc_k(dg + k * kTileBytes, s),
-                                  umma::desc_mn(w + k * kWeightBytes, s, kWeightBytes), kThrough, j > 0 || k > 0 || s > 0);
+                        umma::mma(tmem, dx + umma::kStepK * s, dw + umma::kStepK * s, kGateUp, s > 0);
                     }
-                }
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    umma::mma(tmem + kColGateUp + j * 64, umma::desc_mn(dg, s, kTileBytes), umma::desc_mn(x, s, kTileBytes),
-                              kGradient, !fresh || s > 0);
-                }
-                if (j == chunks - 1) {
-                    umma::commit(&dx_full[dx.at]);
-                    // One chunk only: the second half of M reads the other chunk's tile, which the
-                    // epilogue zeroed.
-#pragma unroll
-                    for (int s = 0; s < 8; ++s) {
-                        umma::mma(tmem + kColDown, umma::desc_mn(hs, s, kTileBytes), umma::desc_mn(x + kTileBytes, s, kTileBytes),
-                                  kGradient, !fresh || s > 0);
+                    for (int s = 0; s < 4; ++s) {
+                        umma::mma(tmem + 128, ddy + umma::kStepK * s, dwd + umma::kStepMn * s, kThrough, s > 0);
                     }
+                    umma::commit(&acc_full);
+                    acc.next();
+                }
+                if (ok) {
                     umma::commit(&in_empty[in.at]);
-                    for (int k = 0; k < chunks; ++k) {
-                        umma::commit(&hidden_empty[k]);
-                    }
+                    in.next();
                 }
             }
-            __syncwarp();
-            if (j == chunks - 1) {
+            drain_on_failure(ok, &drain[0], g.fault);
+        }
+    } else if (warp == kWarps + 2) {
+        if (lane == 0) {  // dx and the weight gradients
+            Turn<2> in, dx;
+            Turn<1> hidden;
+            ok = tma::mbar_wait(&weights_full, 0);
+            for (int k = 0; ok && k < mine; ++k) {
+                ok = tma::mbar_wait(&in_full[in.at], in.phase) && tma::mbar_wait(&dx_empty[dx.at], dx.phase ^ 1u);
+                const uint32_t x = ins + in.at * 2 * kTileBytes;
+                const uint64_t x_mn = umma::desc_mn<kTileBytes>(x);
+                for (int j = 0; ok && j < chunks; ++j) {
+                    ok = tma::mbar_wait(&hidden_full[j], hidden.phase);
+                    if (!ok) {
+                        break;
+                    }
+                    umma::fence_after_sync();
+                    if (j == chunks - 1) {
+                        // First, as the next tile's first hidden values wait for it. With one chunk only,
+                        // the second half of M reads the other chunk's tile, which the epilogue zeroed.
+                        const uint64_t dh = umma::desc_mn<kTileBytes>(hs), dy_mn = umma::desc_mn<kTileBytes>(x + kTileBytes);
+#pragma unroll
+                        for (int s = 0; s < 8; ++s) {
+                            umma::mma(tmem + kColDown, dh + umma::kStepMn * s, dy_mn + umma::kStepMn * s, kGradient,
+                                      k > 0 || s > 0);
+                        }
+                        umma::commit(&h_empty);
+                    }
+                    const uint32_t w = ws + j * kBackChunkWeights;
+                    const uint32_t dg = dgs + j * 2 * kTileBytes;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {  // dG Wg, then dU Wu
+                        const uint64_t da = umma::desc_k(dg + i * kTileBytes);
+                        const uint64_t db = umma::desc_mn<kWeightBytes>(w + i * kWeightBytes);
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            umma::mma(tmem + kColDx + dx.at * 64, da + umma::kStepK * s, db + umma::kStepMn * s, kThrough,
+                                      j > 0 || i > 0 || s > 0);
+                        }
+                    }
+                    if (j == chunks - 1) {
+                        umma::commit(&dx_full[dx.at]);
+                    }
+                    const uint64_t dgu = umma::desc_mn<kTileBytes>(dg);
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) {
+                        umma::mma(tmem + kColGateUp + j * 64, dgu + umma::kStepMn * s, x_mn + umma::kStepMn * s, kGradient,
+                                  k > 0 || s > 0);
+                    }
+                    umma::commit(&dgu_empty[j]);
+                }
+                if (!ok) {
+                    break;
+                }
+                umma::commit(&in_empty[in.at]);
                 in.next();
                 dx.next();
                 hidden.next();
             }
-        };
-        ok = tma::mbar_wait(&weights_full, 0);
-        const int total = mine * chunks;
-        if (ok && total > 0) {
-            first(0);
-        }
-        for (int n = 0; ok && n < total; ++n) {
-            if (n + 1 < total) {
-                first((n + 1) % chunks);
-            }
             if (ok) {
-                second(n % chunks, n < chunks);
-            }
-        }
-        if (ok) {
-            if (umma::elect_one()) {
                 umma::commit(&all_done);
             }
-            __syncwarp();
-        } else {
-            if (umma::elect_one()) {
-                umma::commit(&drain);
-            }
-            __syncwarp();
-            if (!tma::mbar_wait(&drain, 0) && lane == 0) {
-                atomicOr(g.fault, tma::kFaultDrainTimeout);
-            }
+            drain_on_failure(ok, &drain[1], g.fault);
         }
     } else {
         const int quad = warp & 3;
@@ -642,12 +637,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
                     dh[i] = du.x;
                     dh[i + 1] = du.y;
                 }
-                ok = tma::mbar_wait(&hidden_empty[j], hidden.phase ^ 1u);
+                ok = tma::mbar_wait(&dgu_empty[j], hidden.phase ^ 1u);
                 if (!ok) {
                     break;
                 }
                 put_row<T>(dgs + j * 2 * kTileBytes, row, part, a);
                 put_row<T>(dgs + j * 2 * kTileBytes + kTileBytes, row, part, dh);
+                ok = j > 0 || tma::mbar_wait(&h_empty, hidden.phase ^ 1u);
+                if (!ok) {
+                    break;
+                }
                 put_row<T>(hs + j * kTileBytes, row, part, u);
                 warp_arrive(&hidden_full[j], true);
                 if (j == 0 && before >= 0) {

@@ -26,20 +26,28 @@ constexpr int kAtom = 64;          // 16-bit values per 128-byte row
 constexpr int kRowBytes = 128;
 constexpr int kGroupBytes = 1024;  // 8 rows
 
-// Shared-memory matrix descriptor: start address, leading and stride byte offsets (16-byte
-// units), version 1 at bit 46, 128-byte swizzle (2) at bit 61.
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t leading, uint32_t stride)
+// Shared-memory matrix descriptors: start address, leading and stride byte offsets (16-byte units),
+// version 1 at bit 46, 128-byte swizzle (2) at bit 61. Everything but the address is a constant, and a
+// step of 16 along K adds a constant to the address field: one descriptor per tile, one addition per
+// MMA. (Building each from its byte address cost the issuing warp some 150 cycles an MMA, more than
+// the MMA itself.)
+constexpr uint64_t constant_bits(uint32_t leading)
 {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((leading >> 4) & 0x3FFFu) << 16)
-           | (static_cast<uint64_t>((stride >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+    return (static_cast<uint64_t>(leading >> 4) << 16) | (static_cast<uint64_t>(kGroupBytes >> 4) << 32) | (1ull << 46)
+           | (2ull << 61);
 }
 
-// K step `step` (16 values of K) of a K-major tile at addr, or of an MN-major one whose next 64
-// rows of M or N are `next` bytes further.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr, int step) { return desc(addr + 32u * step, 16, kGroupBytes); }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, int step, uint32_t next)
+// A K-major tile at `addr`; K step s is + kStepK * s.
+constexpr uint64_t kStepK = 32 >> 4;
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return constant_bits(16) | (addr >> 4); }
+
+// An MN-major tile at `addr` whose next 64 rows of M or N are Next bytes further; K step s is
+// + kStepMn * s.
+constexpr uint64_t kStepMn = 2 * kGroupBytes >> 4;
+template <uint32_t Next>
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr)
 {
-    return desc(addr + 2u * kGroupBytes * step, next, kGroupBytes);
+    return constant_bits(Next) | (addr >> 4);
 }
 
 // Instruction descriptor of kind::f16 with an FP32 accumulator: operand type (0 f16, 1 bf16) at
