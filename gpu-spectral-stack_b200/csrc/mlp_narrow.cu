@@ -21,9 +21,11 @@
 // x, dy, the weights and the hidden tiles each serve as K-major and as MN-major operands from the
 // one copy in shared memory (umma.cuh).
 //
-// What bounds them: the activation. A tile's 16384 hidden values take two of the 16-a-cycle special
-// function results each (2048 cycles), the tensor cores 384 cycles forward and 1024 backward, HBM
-// 32 KiB and 48 KiB (about 750 and 1100 cycles of the SM's share).
+// What bounds them (64 channels, 128 hidden). Forward: gelu, whose two special functions a value (16 a cycle)
+// are 2048 of a tile's 2900 cycles; a polynomial without any measured the same, bound by its
+// multiply-adds (31 us against 18.5 us with no activation; HBM alone 10 us). Backward: the tensor
+// cores' reads of shared memory; a tile's 56 MMAs of N = 64 or 128 take some 85 cycles each, 4800 in
+// all, which is a tile's period (60 us with gelu, 50 us without).
 
 #include "mlp.cuh"
 
@@ -381,9 +383,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
 
 constexpr int kBackHidden = 128;   // at most: two chunks
 constexpr int kBackWidth = 64;     // channels and outputs, at most
-// Shared memory: two stages of x and dy, the weights (Wg, Wu, Wd of each chunk), dG, dU and h of each chunk.
+// Shared memory: three stages of x and dy (a tile's stage is held until its weight gradients are done), the weights (Wg, Wu, Wd of each chunk), one chunk's dG
+// and dU, both chunks' h.
+constexpr int kBackStages = 3;
 constexpr int kBackChunkWeights = 3 * kWeightBytes;
-constexpr int kBackSmem = 4 * kTileBytes + 2 * kBackChunkWeights + 6 * kTileBytes + 2048;
+constexpr int kBackSmem = 2 * kBackStages * kTileBytes + 2 * kBackChunkWeights + 4 * kTileBytes + 2048;
 static_assert(kBackSmem <= kMaxSmem, "shared memory");
 // Tensor memory columns.
 constexpr int kColDx = 192;        // two accumulators of 64
@@ -402,10 +406,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
     const uint32_t ins = base;                          // [stage][x, dy]
-    const uint32_t ws = ins + 4 * kTileBytes;           // [chunk][Wg, Wu, Wd]
-    const uint32_t dgs = ws + 2 * kBackChunkWeights;    // [chunk][dG, dU]
-    const uint32_t hs = dgs + 4 * kTileBytes;           // [chunk]
-    __shared__ uint64_t weights_full, in_full[2], in_empty[2], acc_full, acc_empty, hidden_full[2], dgu_empty[2], h_empty,
+    const uint32_t ws = ins + 2 * kBackStages * kTileBytes;  // [chunk][Wg, Wu, Wd]
+    const uint32_t dgs = ws + 2 * kBackChunkWeights;    // [dG, dU]
+    const uint32_t hs = dgs + 2 * kTileBytes;           // [chunk]
+    __shared__ uint64_t weights_full, in_full[kBackStages], in_empty[kBackStages], acc_full, acc_empty, hidden_full[2], dgu_empty, h_empty,
         dx_full[2], dx_empty[2], all_done, drain[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
@@ -420,12 +424,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         tma::mbar_init(&acc_empty, kWarps);
         tma::mbar_init(&all_done, 1);
         tma::mbar_init(&h_empty, 1);
-        for (int i = 0; i < 2; ++i) {
+        tma::mbar_init(&dgu_empty, 1);
+        for (int i = 0; i < kBackStages; ++i) {
             tma::mbar_init(&in_full[i], 1);
             tma::mbar_init(&in_empty[i], 2);  // both MMA warps
+        }
+        for (int i = 0; i < 2; ++i) {
             tma::mbar_init(&drain[i], 1);
             tma::mbar_init(&hidden_full[i], kWarps);
-            tma::mbar_init(&dgu_empty[i], 1);
             tma::mbar_init(&dx_full[i], 1);
             tma::mbar_init(&dx_empty[i], kWarps);
         }
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
             }
         }
         __syncwarp();
-        Turn<2> in;
+        Turn<kBackStages> in;
         int issued = 0;
         for (int k = 0; ok && k < mine; ++k) {
             ok = tma::mbar_wait(&in_empty[in.at], in.phase ^ 1u);
@@ -474,8 +480,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         }
         if (!ok) {
             bool drained = tma::mbar_wait(&weights_full, 0);
-            for (int i = issued > 2 ? issued - 2 : 0; i < issued; ++i) {
-                drained = tma::mbar_wait(&in_full[i % 2], static_cast<unsigned>(i / 2) & 1u) && drained;
+            for (int i = issued > kBackStages ? issued - kBackStages : 0; i < issued; ++i) {
+                drained = tma::mbar_wait(&in_full[i % kBackStages], static_cast<unsigned>(i / kBackStages) & 1u) && drained;
             }
             if (lane == 0 && !drained) {
                 atomicOr(g.fault, tma::kFaultDrainTimeout);
@@ -483,7 +489,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         }
     } else if (warp == kWarps + 1) {
         if (lane == 0) {  // G, U and dh of every chunk
-            Turn<2> in;
+            Turn<kBackStages> in;
             Turn<1> acc;
             ok = tma::mbar_wait(&weights_full, 0);
             for (int k = 0; ok && k < mine; ++k) {
@@ -518,7 +524,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         }
     } else if (warp == kWarps + 2) {
         if (lane == 0) {  // dx and the weight gradients
-            Turn<2> in, dx;
+            Turn<kBackStages> in;
+            Turn<2> dx;
             Turn<1> hidden;
             ok = tma::mbar_wait(&weights_full, 0);
             for (int k = 0; ok && k < mine; ++k) {
@@ -543,7 +550,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
                         umma::commit(&h_empty);
                     }
                     const uint32_t w = ws + j * kBackChunkWeights;
-                    const uint32_t dg = dgs + j * 2 * kTileBytes;
+                    const uint32_t dg = dgs;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {  // dG Wg, then dU Wu
                         const uint64_t da = umma::desc_k(dg + i * kTileBytes);
@@ -563,7 +570,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
                         umma::mma(tmem + kColGateUp + j * 64, dgu + umma::kStepMn * s, x_mn + umma::kStepMn * s, kGradient,
                                   k > 0 || s > 0);
                     }
-                    umma::commit(&dgu_empty[j]);
+                    umma::commit(&dgu_empty);
                 }
                 if (!ok) {
                     break;
@@ -587,7 +594,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
             const float zero[16] = {};
             put_row<T>(hs + kTileBytes, row, part, zero);
         }
-        Turn<1> acc, hidden;
+        Turn<1> acc, dgu, hidden;
         Turn<2> dx;
         const auto store_dx = [&](int t) {
             ok = tma::mbar_wait(&dx_full[dx.at], dx.phase);
@@ -637,12 +644,13 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
                     dh[i] = du.x;
                     dh[i + 1] = du.y;
                 }
-                ok = tma::mbar_wait(&dgu_empty[j], hidden.phase ^ 1u);
+                ok = tma::mbar_wait(&dgu_empty, dgu.phase ^ 1u);
                 if (!ok) {
                     break;
                 }
-                put_row<T>(dgs + j * 2 * kTileBytes, row, part, a);
-                put_row<T>(dgs + j * 2 * kTileBytes + kTileBytes, row, part, dh);
+                dgu.next();
+                put_row<T>(dgs, row, part, a);
+                put_row<T>(dgs + kTileBytes, row, part, dh);
                 ok = j > 0 || tma::mbar_wait(&h_empty, hidden.phase ^ 1u);
                 if (!ok) {
                     break;

@@ -6,7 +6,7 @@
 // made here raise RuntimeError (TORCH_CHECK), the C ABI's SPECTRAL_INVALID_ARGUMENT is rethrown
 // as std::invalid_argument (ValueError), as the reference's drivers do. Every operator is
 // registered for the CUDA dispatch key only, so CPU tensors get the dispatcher's
-// NotImplementedError. A binding checks, makes its input contiguous, allocates the output and
+// NotImplementedError (two also have gradients, through the AutogradCUDA key). A binding checks, makes its input contiguous, allocates the output and
 // any workspace with at::empty (torch's caching allocator, stream-ordered), and launches on the
 // current stream under a device guard. Nothing here runs on the CPU.
 
@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "../../include/spectral_b200.h"
@@ -682,9 +683,17 @@ at::Tensor last_contiguous(const at::Tensor& x, int dtype, const NormSizes& n)
     return y;
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
-group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
-                    const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation, bool keep8)
+// stats: (2, batch, groups), the means and the reciprocal standard deviations (undefined if not wanted).
+struct NormResult {
+    at::Tensor y;
+    at::Tensor stats;
+    at::Tensor codes;
+    at::Tensor scales;
+};
+
+NormResult norm_forward(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                        const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation, bool keep8,
+                        bool keep_stats)
 {
     constexpr const char* op = "group_norm_act";
     const int dtype = dtype_code(x, op, "x");
@@ -696,30 +705,46 @@ group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at:
     const bool first = x.numel() > 0 && !keep8 && channels_first(x, n);
     const at::Tensor xc = first ? x : last_contiguous(x, dtype, n);
     at::Tensor y = at::empty(x.sizes(), x.options());
-    at::Tensor mean = at::empty({n.batch, groups}, x.options().dtype(at::kFloat));
-    at::Tensor rstd = at::empty_like(mean);
-    at::Tensor codes = at::empty(keep8 ? x.sizes() : at::IntArrayRef({0}), x.options().dtype(at::kChar));
-    at::Tensor scales = at::empty(keep8 ? scale_shape(x) : std::vector<int64_t>{0}, x.options().dtype(at::kFloat));
+    at::Tensor stats;
+    at::Tensor codes;
+    at::Tensor scales;
+    if (keep_stats) {
+        stats = at::empty({2, n.batch, groups}, x.options().dtype(at::kFloat));
+    }
+    if (keep8) {
+        codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+        scales = at::empty(scale_shape(x), x.options().dtype(at::kFloat));
+    }
     if (x.numel() == 0) {
-        mean.zero_();
-        rstd.zero_();
-        return {y, mean, rstd, codes, scales};
+        if (keep_stats) {
+            stats.zero_();
+        }
+        return {y, stats, codes, scales};
     }
     size_t count = 0;
     check_status(spectral_group_norm_act_workspace(dtype, n.batch, n.points, n.channels, n.groups, &count));
     at::Tensor work = workspace(count, x);
-    check_status(spectral_group_norm_act(cptr(xc), fptr(w), fptr(b), mptr(y), static_cast<float*>(mptr(mean)),
-                                         static_cast<float*>(mptr(rstd)), keep8 ? mptr(codes) : nullptr,
+    float* mean = keep_stats ? static_cast<float*>(mptr(stats)) : nullptr;
+    check_status(spectral_group_norm_act(cptr(xc), fptr(w), fptr(b), mptr(y), mean,
+                                         keep_stats ? mean + n.batch * groups : nullptr, keep8 ? mptr(codes) : nullptr,
                                          keep8 ? static_cast<float*>(mptr(scales)) : nullptr, dtype, first ? 1 : 0, n.batch,
                                          n.points, n.channels, n.groups, static_cast<float>(eps), act, mptr(work), stream()));
-    return {y, mean, rstd, codes, scales};
+    return {y, stats, codes, scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+group_norm_act_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                    const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation, bool keep8)
+{
+    const NormResult r = norm_forward(x, groups, weight, bias, eps, activation, keep8, true);
+    return {r.y, r.stats.select(0, 0), r.stats.select(0, 1), r.codes, r.scales};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor>
-group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x,
-                             const c10::optional<at::Tensor>& codes, const c10::optional<at::Tensor>& scales,
-                             const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
-                             const at::Tensor& mean, const at::Tensor& rstd, int64_t groups, c10::string_view activation)
+norm_backward(const at::Tensor& dy, const c10::optional<at::Tensor>& x, const c10::optional<at::Tensor>& codes,
+              const c10::optional<at::Tensor>& scales, const c10::optional<at::Tensor>& weight,
+              const c10::optional<at::Tensor>& bias, const float* mean, const float* rstd, int64_t groups,
+              c10::string_view activation)
 {
     constexpr const char* op = "group_norm_act_backward";
     const int dtype = dtype_code(dy, op, "dy");
@@ -742,11 +767,6 @@ group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tenso
         cc = codes->contiguous();
         sc = scales->contiguous();
     }
-    for (const at::Tensor* t : {&mean, &rstd}) {
-        TORCH_CHECK(t->is_cuda() && t->device() == dy.device() && t->scalar_type() == at::kFloat && t->dim() == 2
-                        && t->size(0) == n.batch && t->size(1) == groups && t->is_contiguous(),
-                    op, ": mean and rstd must be contiguous float32 (batch, groups) on the device of dy");
-    }
     const at::Tensor w = channel_parameter(weight, dy, n.channels, op, "weight");
     const at::Tensor b = channel_parameter(bias, dy, n.channels, op, "bias");
     const at::Tensor dyc = last_contiguous(dy, dtype, n);
@@ -758,9 +778,25 @@ group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tenso
     at::Tensor work = workspace(count, dy);
     check_status(spectral_group_norm_act_backward(
         cptr(dyc), xc.defined() ? cptr(xc) : nullptr, cc.defined() ? cptr(cc) : nullptr, fptr(sc), fptr(w), fptr(b),
-        fptr(mean), fptr(rstd), mptr(dx), static_cast<float*>(mptr(dweight)), static_cast<float*>(mptr(dbias)), dtype,
-        n.batch, n.points, n.channels, n.groups, act, mptr(work), stream()));
+        mean, rstd, mptr(dx), static_cast<float*>(mptr(dweight)), static_cast<float*>(mptr(dbias)), dtype, n.batch, n.points,
+        n.channels, n.groups, act, mptr(work), stream()));
     return {dx, dweight, dbias};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+group_norm_act_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x,
+                             const c10::optional<at::Tensor>& codes, const c10::optional<at::Tensor>& scales,
+                             const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
+                             const at::Tensor& mean, const at::Tensor& rstd, int64_t groups, c10::string_view activation)
+{
+    constexpr const char* op = "group_norm_act_backward";
+    const NormSizes n = norm_sizes(dy, groups, op);
+    for (const at::Tensor* t : {&mean, &rstd}) {
+        TORCH_CHECK(t->is_cuda() && t->device() == dy.device() && t->scalar_type() == at::kFloat && t->dim() == 2
+                        && t->size(0) == n.batch && t->size(1) == groups && t->is_contiguous(),
+                    op, ": mean and rstd must be contiguous float32 (batch, groups) on the device of dy");
+    }
+    return norm_backward(dy, x, codes, scales, weight, bias, fptr(mean), fptr(rstd), groups, activation);
 }
 
 struct MlpSizes {
@@ -858,6 +894,135 @@ gated_mlp_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x
     return {dx, dwg, dwu, dwd};
 }
 
+// --- the same with gradients: what spectral.nn calls ----------------------------------------------
+// Functions of torch's autograd engine in C++ (the Python class's bookkeeping took longer than the
+// kernels of a small layer). Each keeps only its input for the backward pass, in 8 bits if asked.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients of gradients are not computed: asking for them is an error, not a silent zero.
+void check_once(const variable_list& grads, const char* op)
+{
+    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].defined() && grads[0].requires_grad()), op,
+                ": the backward pass is not differentiable itself");
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor*> tensors)
+{
+    if (!at::GradMode::is_enabled()) {
+        return false;
+    }
+    for (const at::Tensor* t : tensors) {
+        if (t->defined() && t->requires_grad()) {
+            return true;
+        }
+    }
+    return false;
+}
+
+c10::optional<at::Tensor> optional_of(const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
+
+struct GroupNormActFunction : torch::autograd::Function<GroupNormActFunction> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                              const c10::optional<at::Tensor>& bias, int64_t groups, double eps, std::string activation,
+                              bool checkpoint8)
+    {
+        at::AutoDispatchBelowAutograd guard;
+        const NormResult r = norm_forward(x, groups, weight, bias, eps, activation, checkpoint8, true);
+        const at::Tensor w = weight.value_or(at::Tensor());
+        const at::Tensor b = bias.value_or(at::Tensor());
+        ctx->save_for_backward(checkpoint8 ? variable_list{w, b, r.stats, r.codes, r.scales}
+                                           : variable_list{w, b, r.stats, x});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["activation"] = activation;
+        return r.y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        check_once(grads, "group_norm_act");
+        const variable_list kept = ctx->get_saved_variables();
+        const bool packed = kept.size() == 5;
+        const std::string activation = ctx->saved_data["activation"].toStringRef();
+        const at::Tensor& stats = kept[2];
+        const float* mean = fptr(stats);
+        auto [dx, dweight, dbias] = norm_backward(
+            grads[0], packed ? c10::nullopt : optional_of(kept[3]), packed ? optional_of(kept[3]) : c10::nullopt,
+            packed ? optional_of(kept[4]) : c10::nullopt, optional_of(kept[0]), optional_of(kept[1]), mean,
+            mean == nullptr ? nullptr : mean + stats.numel() / 2, ctx->saved_data["groups"].toInt(), activation);
+        const at::Tensor none;
+        return {dx, kept[0].defined() ? dweight : none, kept[1].defined() ? dbias : none, none, none, none, none};
+    }
+};
+
+at::Tensor group_norm_act_layer_cuda(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                                     const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation, bool)
+{
+    return norm_forward(x, groups, weight, bias, eps, activation, false, false).y;
+}
+
+at::Tensor group_norm_act_layer_autograd(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                                         const c10::optional<at::Tensor>& bias, double eps, c10::string_view activation,
+                                         bool checkpoint8)
+{
+    const at::Tensor w = weight.value_or(at::Tensor());
+    const at::Tensor b = bias.value_or(at::Tensor());
+    if (wants_grad({&x, &w, &b})) {
+        return GroupNormActFunction::apply(x, weight, bias, groups, eps, std::string(activation.data(), activation.size()), checkpoint8);
+    }
+    at::AutoDispatchBelowAutograd guard;
+    return group_norm_act_layer_cuda(x, groups, weight, bias, eps, activation, checkpoint8);
+}
+
+struct GatedMlpFunction : torch::autograd::Function<GatedMlpFunction> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up,
+                              const at::Tensor& w_down, std::string activation, bool checkpoint8)
+    {
+        at::AutoDispatchBelowAutograd guard;
+        const at::Tensor y = gated_mlp_cuda(x, w_gate, w_up, w_down, activation);
+        variable_list kept{w_gate, w_up, w_down};
+        if (checkpoint8) {
+            auto [codes, scales] = pack8_cuda(x);
+            kept.push_back(codes);
+            kept.push_back(scales);
+        } else {
+            kept.push_back(x);
+        }
+        ctx->save_for_backward(std::move(kept));
+        ctx->saved_data["activation"] = activation;
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        check_once(grads, "gated_mlp");
+        const variable_list kept = ctx->get_saved_variables();
+        const bool packed = kept.size() == 5;
+        const std::string activation = ctx->saved_data["activation"].toStringRef();
+        auto [dx, dwg, dwu, dwd] = gated_mlp_backward_cuda(
+            grads[0], packed ? c10::nullopt : optional_of(kept[3]), packed ? optional_of(kept[3]) : c10::nullopt,
+            packed ? optional_of(kept[4]) : c10::nullopt, kept[0], kept[1], kept[2], activation);
+        return {dx, dwg, dwu, dwd, at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor gated_mlp_layer_cuda(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up,
+                                const at::Tensor& w_down, c10::string_view activation, bool)
+{
+    return gated_mlp_cuda(x, w_gate, w_up, w_down, activation);
+}
+
+at::Tensor gated_mlp_layer_autograd(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up,
+                                    const at::Tensor& w_down, c10::string_view activation, bool checkpoint8)
+{
+    if (wants_grad({&x, &w_gate, &w_up, &w_down})) {
+        return GatedMlpFunction::apply(x, w_gate, w_up, w_down, std::string(activation.data(), activation.size()), checkpoint8);
+    }
+    at::AutoDispatchBelowAutograd guard;
+    return gated_mlp_layer_cuda(x, w_gate, w_up, w_down, activation, checkpoint8);
+}
+
 // spectral._C.fft_impls(): the registry's names, in order, as a tuple of str.
 PyObject* py_fft_impls(PyObject*, PyObject*)
 {
@@ -914,6 +1079,10 @@ TORCH_LIBRARY(spectral, m)
     m.def("gated_mlp(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation=\"silu\") -> Tensor");
     m.def("gated_mlp_backward(Tensor dy, Tensor? x, Tensor? codes, Tensor? scales, Tensor w_gate, Tensor w_up,"
           " Tensor w_down, str activation) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("group_norm_act_layer(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, str activation,"
+          " bool checkpoint8) -> Tensor");
+    m.def("gated_mlp_layer(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation, bool checkpoint8)"
+          " -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(spectral, CUDA, m)
@@ -938,6 +1107,14 @@ TORCH_LIBRARY_IMPL(spectral, CUDA, m)
     m.impl("group_norm_act_backward", &group_norm_act_backward_cuda);
     m.impl("gated_mlp", &gated_mlp_cuda);
     m.impl("gated_mlp_backward", &gated_mlp_backward_cuda);
+    m.impl("group_norm_act_layer", &group_norm_act_layer_cuda);
+    m.impl("gated_mlp_layer", &gated_mlp_layer_cuda);
+}
+
+TORCH_LIBRARY_IMPL(spectral, AutogradCUDA, m)
+{
+    m.impl("group_norm_act_layer", &group_norm_act_layer_autograd);
+    m.impl("gated_mlp_layer", &gated_mlp_layer_autograd);
 }
 
 PyMODINIT_FUNC PyInit__C(void)

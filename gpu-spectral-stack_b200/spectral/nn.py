@@ -119,31 +119,6 @@ class SpectralConv2d(torch.nn.Module):
         return f"{self.in_channels}, {self.out_channels}, m1={self.m1}, m2={self.m2}, impl={self.impl!r}"
 
 
-def _wants_grad(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _GroupNormActFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups: int, eps: float, activation: str, checkpoint8: bool):
-        y, mean, rstd, codes, scales = torch.ops.spectral.group_norm_act.default(
-            x, groups, weight, bias, eps, activation, checkpoint8)
-        kept = (codes, scales) if checkpoint8 else (x,)
-        ctx.save_for_backward(weight, bias, mean, rstd, *kept)
-        ctx.groups, ctx.activation = groups, activation
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad: torch.Tensor):
-        weight, bias, mean, rstd, *kept = ctx.saved_tensors
-        x, codes, scales = (None, *kept) if len(kept) == 2 else (kept[0], None, None)
-        dx, dweight, dbias = torch.ops.spectral.group_norm_act_backward.default(
-            grad, x, codes, scales, weight, bias, mean, rstd, ctx.groups, ctx.activation)
-        return (dx, dweight if weight is not None else None, dbias if bias is not None else None,
-                None, None, None, None)
-
-
 def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
                    bias: torch.Tensor | None = None, *, eps: float = 1e-5, activation: str = "none",
                    checkpoint8: bool = False) -> torch.Tensor:
@@ -151,28 +126,7 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
     sample and group of c / groups channels over all points; weight and bias float32 (c,) or None;
     activation "none", "silu" or "gelu" (the exact one). Returns a contiguous tensor of x's type.
     Differentiable in x, weight and bias; checkpoint8=True keeps x for that in 8 bits."""
-    if _wants_grad(x, weight, bias):
-        return _GroupNormActFunction.apply(x, weight, bias, groups, eps, activation, checkpoint8)
-    return torch.ops.spectral.group_norm_act.default(x, groups, weight, bias, eps, activation, False)[0]
-
-
-class _GatedMLPFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation: str, checkpoint8: bool):
-        y = torch.ops.spectral.gated_mlp.default(x, w_gate, w_up, w_down, activation)
-        kept = torch.ops.spectral.pack8.default(x) if checkpoint8 else (x,)
-        ctx.save_for_backward(w_gate, w_up, w_down, *kept)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad: torch.Tensor):
-        w_gate, w_up, w_down, *kept = ctx.saved_tensors
-        x, codes, scales = (None, *kept) if len(kept) == 2 else (kept[0], None, None)
-        grads = torch.ops.spectral.gated_mlp_backward.default(
-            grad, x, codes, scales, w_gate, w_up, w_down, ctx.activation)
-        return (*grads, None, None)
+    return torch.ops.spectral.group_norm_act_layer.default(x, groups, weight, bias, eps, activation, checkpoint8)
 
 
 def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
@@ -181,9 +135,7 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     and w_up (hidden, channels), w_down (outputs, hidden), all of x's type. Differentiable in all
     four; only x is kept for that (in 8 bits with checkpoint8=True), the hidden values are
     recomputed."""
-    if _wants_grad(x, w_gate, w_up, w_down):
-        return _GatedMLPFunction.apply(x, w_gate, w_up, w_down, activation, checkpoint8)
-    return torch.ops.spectral.gated_mlp.default(x, w_gate, w_up, w_down, activation)
+    return torch.ops.spectral.gated_mlp_layer.default(x, w_gate, w_up, w_down, activation, checkpoint8)
 
 
 class GroupNormAct(torch.nn.Module):

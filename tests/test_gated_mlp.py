@@ -330,3 +330,18 @@ def test_wrong_arguments_are_refused():
         gated_mlp(x, w[0], w, d)
     with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
         gated_mlp(x.double(), w.double(), w.double(), d.double())
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused_and_unused_ones_cost_nothing_else():
+    *args, dy = inputs(20, 16, 24, 16, torch.float32)
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    up = dy.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not differentiable itself"):
+        torch.autograd.grad(gated_mlp(*leaves), leaves, up, create_graph=True)
+    with torch.no_grad():
+        assert gated_mlp(*leaves).grad_fn is None
+    # Only some inputs want gradients.
+    frozen = [args[0].clone().requires_grad_(True), *args[1:]]
+    (dx,) = torch.autograd.grad(gated_mlp(*frozen), frozen[:1], dy)
+    assert torch.equal(dx, torch.autograd.grad(gated_mlp(*leaves), leaves[:1], dy)[0])
