@@ -37,7 +37,6 @@
 #include "mlp.cuh"
 
 #include <algorithm>
-#include <climits>
 
 namespace spectral {
 
@@ -52,13 +51,30 @@ constexpr long long kMaxTokens = 0x7fffff00LL;  // 32-bit TMA coordinates
 
 // --- staging ---------------------------------------------------------------------------------------
 
-// Copies a rows x cols matrix of T into the operand form: planes of the operand type, `pitch`
-// values a row (a multiple of 8). For arrays TMA cannot read as they lie: float32, or rows that
-// are not 16-byte pieces.
+// Matrices of T to copy into the operand form: planes of the operand type, `pitch` values a row (a
+// multiple of 8). For arrays TMA cannot read as they lie: float32, or rows that are not 16-byte
+// pieces. One launch for all of a call's (blockIdx.y).
+struct StageJob {
+    const void* src;
+    void* dst;
+    long long rows;
+    int cols;
+    int pitch;
+};
+struct StageJobs {
+    StageJob job[5];
+    int count = 0;
+};
+
 template <class T>
-__global__ void __launch_bounds__(256)
-    stage_kernel(const T* __restrict__ src, typename Operand<T>::Type* __restrict__ dst, long long rows, int cols, int pitch)
+__global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ StageJobs jobs)
 {
+    const StageJob& job = jobs.job[blockIdx.y];
+    const T* __restrict__ src = static_cast<const T*>(job.src);
+    auto* __restrict__ dst = static_cast<typename Operand<T>::Type*>(job.dst);
+    const long long rows = job.rows;
+    const int cols = job.cols;
+    const int pitch = job.pitch;
     allow_next_grid();
     wait_for_previous_grid();
     const int pieces = pitch / 8;
@@ -154,18 +170,25 @@ struct Args {
     unsigned* fault = nullptr;
 };
 
-template <Kind K, int BN>
+// A tile is MT x 128 rows by BN columns (of each accumulator). Two accumulator sets where tensor memory
+// holds them, so that a tile's epilogue runs under the next tile's products.
+template <Kind K, int BN, int MT>
 struct Config {
     static constexpr bool kAMn = K == Kind::kWeight;
     static constexpr int kSets = K == Kind::kGate ? 2 : K == Kind::kGateBack ? 3 : 1;  // accumulators of BN columns
     static constexpr int kBRows = K == Kind::kGate || K == Kind::kGateBack ? 2 * BN : BN;
+    static constexpr int kRows = MT * kTileM;
+    static constexpr int kABytes = MT * kTileABytes;
     static constexpr int kBBytes = kBRows * umma::kRowBytes;
-    static constexpr int kStageBytes = kTileABytes + kBBytes;
+    static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kStages = (kMaxSmem - 2048) / kStageBytes > 6 ? 6 : (kMaxSmem - 2048) / kStageBytes;
-    static constexpr int kCols = kSets * BN;
-    static constexpr int kTmemCols = 2 * kCols <= 64 ? 64 : 2 * kCols <= 128 ? 128 : 2 * kCols <= 256 ? 256 : 512;
+    static constexpr int kCols = kSets * BN * MT;
+    static constexpr int kSlots = 2 * kCols <= 512 ? 2 : 1;
+    static constexpr int kUsed = kSlots * kCols;
+    static constexpr int kTmemCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static constexpr int kSmem = kStages * kStageBytes + 2048;  // barriers, and slack for the 1 KiB base
-    static_assert(2 * kCols <= 512, "two accumulator sets in tensor memory");
+    static_assert(kUsed <= 512, "tensor memory");
+    static_assert(MT == 1 || kSets == 1, "row tiles of one accumulator each");
 };
 
 // Tile t: output rows from m0, columns from n0, chunks [k0, k1) (kWeight: of problem p and part `part`).
@@ -189,7 +212,7 @@ __device__ __forceinline__ void pass_range(const Args& g, const Tile& tile, int 
     end = min(begin + kStep, last);
 }
 
-template <Kind K, int BN, class T>
+template <Kind K, int BN, int MT, class T>
 __device__ __forceinline__ Tile locate(const Args& g, long long t)
 {
     Tile tile{0, 0, 0, g.chunks[0], 0, 0, 1};
@@ -198,12 +221,12 @@ __device__ __forceinline__ Tile locate(const Args& g, long long t)
         const long long r = t - tile.part * g.first[3];
         tile.problem = r >= g.first[2] ? 2 : r >= g.first[1] ? 1 : 0;
         const int i = static_cast<int>(r - g.first[tile.problem]);
-        tile.m0 = i / g.n_tiles_of[tile.problem] * kTileM;
+        tile.m0 = i / g.n_tiles_of[tile.problem] * (MT * kTileM);
         tile.n0 = i % g.n_tiles_of[tile.problem] * BN;
         tile.k0 = tile.part * g.part_chunks;
         tile.k1 = min(tile.k0 + g.part_chunks, g.chunks[0]);
     } else {
-        tile.m0 = static_cast<int>(t / g.n_tiles) * kTileM;
+        tile.m0 = static_cast<int>(t / g.n_tiles) * (MT * kTileM);
         tile.n0 = static_cast<int>(t % g.n_tiles) * BN;
     }
     if constexpr (sizeof(T) == 4) {
@@ -254,10 +277,10 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
     }
 }
 
-template <Kind K, int BN, class T, int Act>
+template <Kind K, int BN, int MT, class T, int Act>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g)
 {
-    using Cfg = Config<K, BN>;
+    using Cfg = Config<K, BN, MT>;
     using Op = Operand<T>;
     constexpr bool kBf16 = std::is_same_v<typename Op::Type, bf16>;
     constexpr int kStages = Cfg::kStages;
@@ -300,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         long long issued = 0;
         bool ok = true;
         for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
-            const Tile tile = locate<K, BN, T>(g, t);
+            const Tile tile = locate<K, BN, MT, T>(g, t);
             constexpr int kPairs = K == Kind::kGateBack || K == Kind::kInput ? 2 : 1;
             for (int turn = 0; ok && turn < tile.passes * kPairs; ++turn) {
                 const int pair = turn % kPairs;
@@ -314,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             break;
                         }
                         const uint32_t a = base + stage * Cfg::kStageBytes;
-                        const uint32_t b = a + kTileABytes;
+                        const uint32_t b = a + Cfg::kABytes;
                         uint64_t* bar = &full[stage];
                         if (umma::elect_one()) {
                             const int kc = k * kChunk;
@@ -322,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                 const int q = tile.problem;
                                 tma::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
 #pragma unroll
-                                for (int j = 0; j < kTileM / 64; ++j) {
+                                for (int j = 0; j < MT * kTileM / 64; ++j) {
                                     umma::load_3d(a + j * 8192, &maps.a[q], tile.m0 + 64 * j, kc, pa, bar);
                                 }
 #pragma unroll
@@ -346,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                 umma::load_3d(b, &maps.b[0], kc, tile.n0, pb, bar);
                                 umma::load_3d(b + BN * umma::kRowBytes, &maps.b[1], kc, tile.n0, pb, bar);
                             } else {
-                                tma::mbar_arrive_expect_tx(bar, kTileABytes + BN * umma::kRowBytes);
+                                tma::mbar_arrive_expect_tx(bar, Cfg::kABytes + BN * umma::kRowBytes);
                                 umma::load_3d(a, &maps.a[1], kc, tile.m0, pa, bar);
 #pragma unroll
                                 for (int j = 0; j < BN / 64; ++j) {
@@ -390,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         unsigned slot_phase = 0;
         bool ok = true;
         for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
-            const Tile tile = locate<K, BN, T>(g, t);
+            const Tile tile = locate<K, BN, MT, T>(g, t);
             constexpr int kPairs = K == Kind::kGateBack || K == Kind::kInput ? 2 : 1;
             for (int pass = 0; ok && pass < tile.passes; ++pass) {
                 ok = tma::mbar_wait(&freed[slot], slot_phase ^ 1u);
@@ -412,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         }
                         umma::fence_after_sync();
                         const uint32_t a = base + stage * Cfg::kStageBytes;
-                        const uint32_t b = a + kTileABytes;
+                        const uint32_t b = a + Cfg::kABytes;
                         if (umma::elect_one()) {
                             const uint64_t da = Cfg::kAMn ? umma::desc_mn<8192>(a) : umma::desc_k(a);
                             constexpr uint64_t kStepA = Cfg::kAMn ? umma::kStepMn : umma::kStepK;
@@ -427,7 +450,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                 constexpr uint64_t kStepB = kBMnFirst ? umma::kStepMn : umma::kStepK;
 #pragma unroll
                                 for (int s = 0; s < kChunk / 16; ++s) {
-                                    umma::mma(d, da + kStepA * s, db + kStepB * s, kFirst, !fresh || i > 0 || s > 0);
+#pragma unroll
+                                    for (int m = 0; m < MT; ++m) {
+                                        umma::mma(d + m * BN, da + kStepA * s + m * (kTileABytes >> 4), db + kStepB * s, kFirst,
+                                                  !fresh || i > 0 || s > 0);
+                                    }
                                 }
                             }
                             umma::commit(&empty[stage]);
@@ -444,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         umma::commit(&done[slot]);
                     }
                     __syncwarp();
-                    slot ^= 1;
+                    slot = (slot + 1) % Cfg::kSlots;
                     slot_phase ^= slot == 0 ? 1u : 0u;
                 }
             }
@@ -471,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         unsigned slot_phase = 0;
         bool ok = true;
         for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
-            const Tile tile = locate<K, BN, T>(g, t);
+            const Tile tile = locate<K, BN, MT, T>(g, t);
             const int row = tile.m0 + quad * 32 + lane;
             const int rows = K == Kind::kWeight ? g.rows_of[tile.problem] : g.rows;
             const int cols = K == Kind::kWeight ? g.cols_of[tile.problem] : g.cols;
@@ -509,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         }
                     }
                     release(&freed[slot], lane);
-                    slot ^= 1;
+                    slot = (slot + 1) % Cfg::kSlots;
                     slot_phase ^= slot == 0 ? 1u : 0u;
                 }
                 const int col = tile.n0 + half * 32;
@@ -522,26 +549,28 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     umma::fence_after_sync();
                     const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
-                    for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                    for (int i = 0; i < MT * (BN / 64); ++i) {
+                        const int m = i / (BN / 64);  // row tile
+                        const int c = half * (BN / 2) + i % (BN / 64) * 32;
                         if (tile.n0 + c >= cols) {
-                            break;
+                            continue;
                         }
                         float acc[Cfg::kSets][32];
 #pragma unroll
                         for (int q = 0; q < Cfg::kSets; ++q) {
-                            umma::load32(d + q * BN + c, acc[q]);
+                            umma::load32(d + (m * Cfg::kSets + q) * BN + c, acc[q]);
                         }
 #pragma unroll
                         for (int q = 0; q < Cfg::kSets; ++q) {
                             umma::load_wait(acc[q]);
                         }
-                        if (row < rows) {
-                            finish<K, T, Act>(g, tile, row, tile.n0 + c, cols, acc);
+                        if (row + m * kTileM < rows) {
+                            finish<K, T, Act>(g, tile, row + m * kTileM, tile.n0 + c, cols, acc);
                         }
                         __syncwarp();
                     }
                     release(&freed[slot], lane);
-                    slot ^= 1;
+                    slot = (slot + 1) % Cfg::kSlots;
                     slot_phase ^= slot == 0 ? 1u : 0u;
                 }
             }
@@ -620,34 +649,66 @@ __global__ void __launch_bounds__(256)
 
 // --- a few tokens --------------------------------------------------------------------------------------
 
-constexpr int kFewTokens = 8;
+constexpr int kFewAtOnce = 8;  // tokens of one launch
 constexpr int kFewThreads = 256;
 
-// acc[m] += sum over a warp's share of w[0 .. n) . v[m][0 .. n), lanes striding 16-byte pieces (or
-// single values where the rows are not whole aligned pieces).
-template <class W, class X, int M>
-__device__ __forceinline__ void row_dot(const W* __restrict__ w, const X* __restrict__ v, long long pitch, int n, int first,
-                                        int step, bool wide, float (&acc)[M])
+// The most tokens that take this path: past them the tensor cores are faster. float32, whose weights would
+// have to be split first, stays here longer (four launches).
+template <class T>
+constexpr int kFewTokens = sizeof(T) == 4 ? 32 : 8;
+
+// N consecutive values as floats, by 16-byte loads.
+template <class X, int N>
+__device__ __forceinline__ void load_floats(const X* p, float (&v)[N])
+{
+    constexpr int kPer = 16 / static_cast<int>(sizeof(X));
+#pragma unroll
+    for (int i = 0; i < N / kPer; ++i) {
+        const Vec<X, kPer> q = reinterpret_cast<const Vec<X, kPer>*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            v[i * kPer + j] = to_float(q.v[j]);
+        }
+    }
+}
+
+// acc[r][m] += the share of lane `first` of `step` of w[r][0 .. n) . v[m][0 .. n), for R rows of weights at
+// once: lanes stride 16-byte pieces, or single values where rows are not whole aligned pieces.
+template <class W, class X, int R, int M>
+__device__ __forceinline__ void row_dots(const W* const (&w)[R], const X* __restrict__ v, long long pitch, int n, int first,
+                                         int step, bool wide, float (&acc)[R][M])
 {
     constexpr int kV = 16 / static_cast<int>(sizeof(W));
     if (wide) {
-#pragma unroll 4
+#pragma unroll 2
         for (int c = first * kV; c < n; c += step * kV) {
-            const Vec<W, kV> p = *reinterpret_cast<const Vec<W, kV>*>(w + c);
+            float p[R][kV];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                load_floats<W, kV>(w[r] + c, p[r]);
+            }
 #pragma unroll
             for (int m = 0; m < M; ++m) {
+                float q[kV];
+                load_floats<X, kV>(v + m * pitch + c, q);
 #pragma unroll
-                for (int j = 0; j < kV; ++j) {
-                    acc[m] = fmaf(to_float(p.v[j]), to_float(v[m * pitch + c + j]), acc[m]);
+                for (int r = 0; r < R; ++r) {
+#pragma unroll
+                    for (int j = 0; j < kV; ++j) {
+                        acc[r][m] = fmaf(p[r][j], q[j], acc[r][m]);
+                    }
                 }
             }
         }
     } else {
         for (int c = first; c < n; c += step) {
-            const float p = to_float(w[c]);
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                acc[m] = fmaf(p, to_float(v[m * pitch + c]), acc[m]);
+                const float q = to_float(v[m * pitch + c]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    acc[r][m] = fmaf(to_float(w[r][c]), q, acc[r][m]);
+                }
             }
         }
     }
@@ -666,23 +727,18 @@ __global__ void __launch_bounds__(kFewThreads)
     if (f >= hidden) {
         return;
     }
-    float a[M], b[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        a[m] = 0.0f;
-        b[m] = 0.0f;
-    }
-    row_dot<T, T, M>(w_gate + static_cast<long long>(f) * channels, x, channels, channels, lane, 32, wide, a);
-    row_dot<T, T, M>(w_up + static_cast<long long>(f) * channels, x, channels, channels, lane, 32, wide, b);
+    float acc[2][M] = {};
+    const T* const rows[2] = {w_gate + static_cast<long long>(f) * channels, w_up + static_cast<long long>(f) * channels};
+    row_dots<T, T, 2, M>(rows, x, channels, channels, lane, 32, wide, acc);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            a[m] += __shfl_xor_sync(0xffffffffu, a[m], o);
-            b[m] += __shfl_xor_sync(0xffffffffu, b[m], o);
+            acc[0][m] += __shfl_xor_sync(0xffffffffu, acc[0][m], o);
+            acc[1][m] += __shfl_xor_sync(0xffffffffu, acc[1][m], o);
         }
         if (lane == 0) {
-            h[static_cast<long long>(m) * hidden + f] = activate<Act>(a[m]) * b[m];
+            h[static_cast<long long>(m) * hidden + f] = activate<Act>(acc[0][m]) * acc[1][m];
         }
     }
 }
@@ -697,21 +753,17 @@ __global__ void __launch_bounds__(kFewThreads)
     allow_next_grid();
     wait_for_previous_grid();
     const int o = blockIdx.x;
-    float a[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        a[m] = 0.0f;
-    }
-    row_dot<T, float, M>(w_down + static_cast<long long>(o) * hidden, h, hidden, hidden, static_cast<int>(threadIdx.x),
-                         kFewThreads, wide, a);
+    float acc[1][M] = {};
+    const T* const row[1] = {w_down + static_cast<long long>(o) * hidden};
+    row_dots<T, float, 1, M>(row, h, hidden, hidden, static_cast<int>(threadIdx.x), kFewThreads, wide, acc);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) {
-            a[m] += __shfl_xor_sync(0xffffffffu, a[m], k);
+            acc[0][m] += __shfl_xor_sync(0xffffffffu, acc[0][m], k);
         }
         if ((threadIdx.x & 31) == 0) {
-            sums[threadIdx.x >> 5][m] = a[m];
+            sums[threadIdx.x >> 5][m] = acc[0][m];
         }
     }
     __syncthreads();
@@ -757,9 +809,10 @@ std::size_t staged_bytes(long long rows, int cols)
     return static_cast<std::size_t>(rows) * round_up(cols, 8) * 2 * Operand<T>::kPlanes;
 }
 
-// The operand form of a rows x cols array, staged into the arena where TMA cannot read it in place.
+// The operand form of a rows x cols array; where TMA cannot read it in place, in the arena, filled once
+// `jobs` have run.
 template <class T>
-Matrix operand(const void* p, long long rows, int cols, Arena& arena, cudaStream_t stream)
+Matrix operand(const void* p, long long rows, int cols, Arena& arena, StageJobs& jobs)
 {
     constexpr bool kBf16 = std::is_same_v<typename Operand<T>::Type, bf16>;
     if (direct<T>(p, cols)) {
@@ -767,11 +820,22 @@ Matrix operand(const void* p, long long rows, int cols, Arena& arena, cudaStream
     }
     const int pitch = round_up(cols, 8);
     void* dst = arena.take(staged_bytes<T>(rows, cols));
-    const long long pieces = rows * (pitch / 8);
-    const unsigned grid = static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, 148 * 16));
-    launch_pdl(stage_kernel<T>, dim3(grid), dim3(256), 0, stream, static_cast<const T*>(p),
-               static_cast<typename Operand<T>::Type*>(dst), rows, cols, pitch);
+    jobs.job[jobs.count++] = {p, dst, rows, cols, pitch};
     return {dst, rows, cols, pitch, Operand<T>::kPlanes, kBf16};
+}
+
+template <class T>
+void run_jobs(const StageJobs& jobs, cudaStream_t stream)
+{
+    if (jobs.count == 0) {
+        return;
+    }
+    long long pieces = 1;
+    for (int i = 0; i < jobs.count; ++i) {
+        pieces = std::max(pieces, jobs.job[i].rows * (jobs.job[i].pitch / 8));
+    }
+    const unsigned grid = static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, 148 * 16));
+    launch_pdl(stage_kernel<T>, dim3(grid, static_cast<unsigned>(jobs.count)), dim3(256), 0, stream, jobs);
 }
 
 // hidden values (tokens x hidden) in the arena, in the operand form.
@@ -783,13 +847,13 @@ Matrix hidden_matrix(const MlpShape& n, Arena& arena)
     return {p, n.tokens, n.hidden, pitch, Operand<T>::kPlanes, std::is_same_v<typename Operand<T>::Type, bf16>};
 }
 
-template <Kind K, int BN, class T, int Act>
+template <Kind K, int BN, int MT, class T, int Act>
 void launch_product(const Maps& maps, Args& g, cudaStream_t stream)
 {
-    using Cfg = Config<K, BN>;
+    using Cfg = Config<K, BN, MT>;
     static std::atomic<bool> opted[kMaxDevices];
     const int device = current_device();
-    const auto kernel = product_kernel<K, BN, T, Act>;
+    const auto kernel = product_kernel<K, BN, MT, T, Act>;
     if (!opted[device].load(std::memory_order_relaxed)) {
         SPECTRAL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
         opted[device].store(true, std::memory_order_relaxed);
@@ -825,29 +889,29 @@ void set_tiles(Args& g, long long rows, int cols, int bn)
 }
 
 template <class T, int Act>
-void mlp_few(const void* x, const void* wg, const void* wu, const void* wd, void* y, const MlpShape& n, float* h,
-             cudaStream_t stream)
+void mlp_few(const T* x, const T* wg, const T* wu, const T* wd, T* y, const MlpShape& n, float* h, cudaStream_t stream)
 {
     constexpr int kV = 16 / static_cast<int>(sizeof(T));
-    const bool wide_c = n.channels % kV == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
-    const bool wide_f = n.hidden % kV == 0 && aligned_to(wd, 16);
-    const auto run = [&](auto m) {
-        constexpr int M = decltype(m)::value;
-        launch_pdl(few_gate_kernel<T, Act, M>, dim3(static_cast<unsigned>(tiles_of(n.hidden, kFewThreads / 32))),
-                   dim3(kFewThreads), 0, stream, static_cast<const T*>(x), static_cast<const T*>(wg),
-                   static_cast<const T*>(wu), h, n.channels, n.hidden, wide_c);
-        launch_pdl(few_down_kernel<T, M>, dim3(static_cast<unsigned>(n.outputs)), dim3(kFewThreads), 0, stream,
-                   static_cast<const float*>(h), static_cast<const T*>(wd), static_cast<T*>(y), n.hidden, n.outputs, wide_f);
-    };
-    switch (n.tokens) {
-        case 1: run(std::integral_constant<int, 1>{}); return;
-        case 2: run(std::integral_constant<int, 2>{}); return;
-        case 3: run(std::integral_constant<int, 3>{}); return;
-        case 4: run(std::integral_constant<int, 4>{}); return;
-        case 5: run(std::integral_constant<int, 5>{}); return;
-        case 6: run(std::integral_constant<int, 6>{}); return;
-        case 7: run(std::integral_constant<int, 7>{}); return;
-        default: run(std::integral_constant<int, 8>{}); return;
+    const bool wide_c = n.channels % kV == 0 && aligned_to(x, 16) && aligned_to(wg, 16) && aligned_to(wu, 16);
+    const bool wide_f = n.hidden % 8 == 0 && aligned_to(wd, 16);  // h: rows of whole 16-byte pieces too
+    for (long long t = 0; t < n.tokens; t += kFewAtOnce) {
+        const auto run = [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            launch_pdl(few_gate_kernel<T, Act, M>, dim3(static_cast<unsigned>(tiles_of(n.hidden, kFewThreads / 32))),
+                       dim3(kFewThreads), 0, stream, x + t * n.channels, wg, wu, h, n.channels, n.hidden, wide_c);
+            launch_pdl(few_down_kernel<T, M>, dim3(static_cast<unsigned>(n.outputs)), dim3(kFewThreads), 0, stream,
+                       static_cast<const float*>(h), wd, y + t * n.outputs, n.hidden, n.outputs, wide_f);
+        };
+        switch (std::min<long long>(n.tokens - t, kFewAtOnce)) {
+            case 1: run(std::integral_constant<int, 1>{}); break;
+            case 2: run(std::integral_constant<int, 2>{}); break;
+            case 3: run(std::integral_constant<int, 3>{}); break;
+            case 4: run(std::integral_constant<int, 4>{}); break;
+            case 5: run(std::integral_constant<int, 5>{}); break;
+            case 6: run(std::integral_constant<int, 6>{}); break;
+            case 7: run(std::integral_constant<int, 7>{}); break;
+            default: run(std::integral_constant<int, 8>{}); break;
+        }
     }
 }
 
@@ -860,7 +924,7 @@ std::size_t forward_bytes(const MlpShape& n)
     arena.take(staged_bytes<T>(n.hidden, n.channels));
     arena.take(staged_bytes<T>(n.outputs, n.hidden));
     hidden_matrix<T>(n, arena);
-    arena.take(sizeof(float) * kFewTokens * static_cast<std::size_t>(n.hidden));
+    arena.take(sizeof(float) * kFewAtOnce * static_cast<std::size_t>(n.hidden));
     return arena.used + 256;
 }
 
@@ -869,15 +933,20 @@ void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, 
                  void* work, cudaStream_t stream)
 {
     Arena arena{reinterpret_cast<unsigned char*>((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255})};
-    if (n.tokens <= kFewTokens) {
-        float* h = static_cast<float*>(arena.take(sizeof(float) * kFewTokens * static_cast<std::size_t>(n.hidden)));
-        with_activation(n.act, [&](auto act) { mlp_few<T, decltype(act)::value>(x, wg, wu, wd, y, n, h, stream); });
+    if (n.tokens <= kFewTokens<T>) {
+        float* h = static_cast<float*>(arena.take(sizeof(float) * kFewAtOnce * static_cast<std::size_t>(n.hidden)));
+        with_activation(n.act, [&](auto act) {
+            mlp_few<T, decltype(act)::value>(static_cast<const T*>(x), static_cast<const T*>(wg), static_cast<const T*>(wu),
+                                             static_cast<const T*>(wd), static_cast<T*>(y), n, h, stream);
+        });
         return;
     }
-    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, stream);
-    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, stream);
-    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, stream);
-    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, stream);
+    StageJobs jobs;
+    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, jobs);
+    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, jobs);
+    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, jobs);
+    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, jobs);
+    run_jobs<T>(jobs, stream);
     if constexpr (sizeof(T) == 2) {
         if (narrow_forward_fits(n, dtype)) {
             narrow_forward(mx, mg, mu, md, y, dtype, n, stream);
@@ -897,7 +966,7 @@ void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, 
         g.out[0] = const_cast<void*>(mh.base);
         g.pitch = mh.pitch;
         g.plane = mh.rows * mh.pitch;
-        with_activation(n.act, [&](auto act) { launch_product<Kind::kGate, BN, T, decltype(act)::value>(maps, g, stream); });
+        with_activation(n.act, [&](auto act) { launch_product<Kind::kGate, BN, 1, T, decltype(act)::value>(maps, g, stream); });
     }
     with_width<T>(n.outputs, [&](auto width) {
         constexpr int BN = decltype(width)::value;
@@ -909,26 +978,36 @@ void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, 
         g.chunks[0] = tiles_of(n.hidden, kChunk);
         g.out[0] = y;
         g.pitch = n.outputs;
-        launch_product<Kind::kDown, BN, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        launch_product<Kind::kDown, BN, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
     });
 }
 
+// Tiles of the weight products: 256 x 256 where every side is longer than that (a tile of 128 x 128 reads
+// twice as much per product), else 128 x 128, whose epilogue overlaps. Backward passes measured with the large
+// and the small tiles, us: 8192 x 512 x 2048 149 and 159, 8192 x 1024 x 4096 519 and 538, but
+// 32768 x 256 x 512 114 and 106.
 template <class T>
-constexpr int kWeightBN = sizeof(T) == 4 ? 64 : 128;
+bool large_weight_tiles(const MlpShape& n)
+{
+    return sizeof(T) == 2 && n.hidden > 256 && n.channels > 256 && n.outputs > 256;
+}
 
 // The weight products' tiles and parts: as many parts as keep the SMs busy over whole waves, each
 // at least eight chunks (512 tokens) long.
 template <class T>
 void set_weight_tiles(Args& g, const MlpShape& n)
 {
+    const bool large = large_weight_tiles<T>(n);
+    const int tile_rows = large ? 256 : 128;
+    const int tile_cols = large ? 256 : sizeof(T) == 4 ? 64 : 128;
     const int rows[3] = {n.hidden, n.hidden, n.outputs};
     const int cols[3] = {n.channels, n.channels, n.hidden};
     g.first[0] = 0;
     for (int p = 0; p < 3; ++p) {
         g.rows_of[p] = rows[p];
         g.cols_of[p] = cols[p];
-        g.n_tiles_of[p] = tiles_of(cols[p], kWeightBN<T>);
-        g.first[p + 1] = g.first[p] + static_cast<long long>(tiles_of(rows[p], kTileM)) * g.n_tiles_of[p];
+        g.n_tiles_of[p] = tiles_of(cols[p], tile_cols);
+        g.first[p + 1] = g.first[p] + static_cast<long long>(tiles_of(rows[p], tile_rows)) * g.n_tiles_of[p];
     }
     const long long size = static_cast<long long>(n.hidden) * n.channels;
     g.offset[0] = 0;
@@ -936,12 +1015,13 @@ void set_weight_tiles(Args& g, const MlpShape& n)
     g.offset[2] = 2 * size;
     g.part_size = 2 * size + static_cast<long long>(n.outputs) * n.hidden;
     g.chunks[0] = std::max(1, tiles_of(n.tokens, kChunk));  // no tokens: sized for, never launched
-    // A part of k chunks costs its tiles k units and an epilogue of about four.
+    // A part of k chunks costs its tiles k units and an epilogue of about four (eight for a large tile).
+    const int epilogue = large ? 8 : 4;
     double best = 0.0;
     for (int parts = 1; parts <= 148 && (parts == 1 || g.chunks[0] / parts >= 8); ++parts) {
         const int k = tiles_of(g.chunks[0], parts);
         const long long waves = (g.first[3] * tiles_of(g.chunks[0], k) + 147) / 148;
-        const double cost = static_cast<double>(waves) * (k + 4);
+        const double cost = static_cast<double>(waves) * (k + epilogue);
         if (parts == 1 || cost < 0.97 * best) {
             best = cost;
             g.parts = tiles_of(g.chunks[0], k);
@@ -981,11 +1061,13 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         unpack8(codes, scales, restored, dtype, n.tokens, n.channels, stream);
         x = restored;
     }
-    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, stream);
-    const Matrix mdy = operand<T>(dy, n.tokens, n.outputs, arena, stream);
-    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, stream);
-    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, stream);
-    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, stream);
+    StageJobs jobs;
+    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, jobs);
+    const Matrix mdy = operand<T>(dy, n.tokens, n.outputs, arena, jobs);
+    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, jobs);
+    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, jobs);
+    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, jobs);
+    run_jobs<T>(jobs, stream);
     const long long size0 = static_cast<long long>(n.hidden) * n.channels;
     const long long size2 = static_cast<long long>(n.outputs) * n.hidden;
     const long long part_size = 2 * size0 + size2;
@@ -1013,8 +1095,8 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
     const Matrix mdg = hidden_matrix<T>(n, arena);
     const Matrix mdu = hidden_matrix<T>(n, arena);
     const Matrix mh = hidden_matrix<T>(n, arena);
-    {
-        constexpr int BN = 64;
+    const auto gate_back = [&](auto width) {
+        constexpr int BN = decltype(width)::value;
         Maps maps;
         maps.a[0] = mx.map(kTileM);
         maps.b[0] = mg.map(BN);
@@ -1031,7 +1113,18 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         g.pitch = mh.pitch;
         g.plane = mh.rows * mh.pitch;
         with_activation(n.act,
-                        [&](auto act) { launch_product<Kind::kGateBack, BN, T, decltype(act)::value>(maps, g, stream); });
+                        [&](auto act) { launch_product<Kind::kGateBack, BN, 1, T, decltype(act)::value>(maps, g, stream); });
+    };
+    // 128 columns leave one accumulator set (384 of 512), so the epilogue does not overlap, but an MMA of N = 64
+    // takes nearly as long as one of 128 and a wider tile reads its tokens fewer times: worth it where the
+    // products are long. Backward passes with 128 and 64 columns, us: 8192 x 1024 x 4096 519 and 551,
+    // 8192 x 512 x 2048 149 and 150, 16384 x 256 x 1024 142 and 115.
+    if constexpr (sizeof(T) == 4) {
+        gate_back(std::integral_constant<int, 64>{});  // the passes' sums stay in registers
+    } else if (n.channels + n.outputs >= 1024) {
+        gate_back(std::integral_constant<int, 128>{});
+    } else {
+        gate_back(std::integral_constant<int, 64>{});
     }
     with_width<T>(n.channels, [&](auto width) {
         constexpr int BN = decltype(width)::value;
@@ -1046,7 +1139,7 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         g.chunks[1] = g.chunks[0];
         g.out[0] = dx;
         g.pitch = n.channels;
-        launch_product<Kind::kInput, BN, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        launch_product<Kind::kInput, BN, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
     });
     {
         Maps maps;
@@ -1060,7 +1153,13 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         set_weight_tiles<T>(g, n);
         float* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts));
         g.out[0] = partial;
-        launch_product<Kind::kWeight, kWeightBN<T>, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        if constexpr (sizeof(T) == 4) {
+            launch_product<Kind::kWeight, 64, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        } else if (large_weight_tiles<T>(n)) {
+            launch_product<Kind::kWeight, 256, 2, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        } else {
+            launch_product<Kind::kWeight, 128, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        }
         add_parts(partial, g.parts);
     }
 }
