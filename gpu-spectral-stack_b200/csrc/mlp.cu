@@ -503,14 +503,18 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             const int rows = K == Kind::kWeight ? g.rows_of[tile.problem] : g.rows;
             const int cols = K == Kind::kWeight ? g.cols_of[tile.problem] : g.cols;
             if constexpr (sizeof(T) == 4) {
-                // The passes' accumulators add up in registers: BN = 64, 32 columns per warp.
-                static_assert(BN == 64, "one run of 32 columns per warp");
-                float acc[Cfg::kSets][32];
+                // The passes' accumulators add up in registers: BN / 2 columns of each per warp, in runs of 32.
+                static_assert(MT == 1 && Cfg::kSets * BN <= 256, "the sums fit in registers");
+                constexpr int kRuns = BN / 64;
+                float acc[kRuns][Cfg::kSets][32];
 #pragma unroll
-                for (int q = 0; q < Cfg::kSets; ++q) {
+                for (int r = 0; r < kRuns; ++r) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        acc[q][j] = 0.0f;
+                    for (int q = 0; q < Cfg::kSets; ++q) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            acc[r][q][j] = 0.0f;
+                        }
                     }
                 }
                 for (int pass = 0; ok && pass < tile.passes; ++pass) {
@@ -519,19 +523,22 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         break;
                     }
                     umma::fence_after_sync();
-                    const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16) + half * 32;
+                    const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16) + half * (BN / 2);
 #pragma unroll
                     for (int q = 0; q < Cfg::kSets; ++q) {
                         // An operand pair that ended in an earlier pass has nothing new here.
                         int begin, end;
                         pass_range<T>(g, tile, K == Kind::kGateBack && q == 2 ? 1 : 0, pass, begin, end);
                         if (begin < end) {
-                            float v[32];
-                            umma::load32(d + q * BN, v);
-                            umma::load_wait(v);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                acc[q][j] += v[j];
+                            for (int r = 0; r < kRuns; ++r) {
+                                float v[32];
+                                umma::load32(d + q * BN + 32 * r, v);
+                                umma::load_wait(v);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    acc[r][q][j] += v[j];
+                                }
                             }
                         }
                     }
@@ -539,9 +546,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     slot = (slot + 1) % Cfg::kSlots;
                     slot_phase ^= slot == 0 ? 1u : 0u;
                 }
-                const int col = tile.n0 + half * 32;
-                if (ok && row < rows && col < cols) {
-                    finish<K, T, Act>(g, tile, row, col, cols, acc);
+#pragma unroll
+                for (int r = 0; r < kRuns; ++r) {
+                    const int col = tile.n0 + half * (BN / 2) + 32 * r;
+                    if (ok && row < rows && col < cols) {
+                        finish<K, T, Act>(g, tile, row, col, cols, acc[r]);
+                    }
                 }
             } else {
                 ok = tma::mbar_wait(&done[slot], slot_phase);
@@ -863,19 +873,21 @@ void launch_product(const Maps& maps, Args& g, cudaStream_t stream)
     launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), static_cast<std::size_t>(Cfg::kSmem), stream, maps, g);
 }
 
-// Calls f(integral_constant<BN>) with the widest tile of 64, 128 or 256 columns that `cols` fills:
-// wider tiles read each row of A fewer times.
-template <class T, class F>
-void with_width(int cols, F&& f)
+// Calls f(integral_constant<BN>) with the widest tile of 64, 128 or 256 columns that `cols` fills and that
+// still leaves about two thirds of the SMs a tile: wider tiles read each row of A fewer times and run
+// longer MMAs (float32 8192 x 512 x 2048 forward 440 us at 64 columns, 255 us at 256), but few tokens
+// would leave SMs idle (float32 128 x 512 x 2048: 83 us at 64, 110 us at 256).
+constexpr long long kEnoughTiles = 96;
+template <class F>
+void with_width(long long rows, int cols, F&& f)
 {
-    if constexpr (sizeof(T) == 4) {
-        f(std::integral_constant<int, 64>{});  // the passes' sums stay in registers
-    } else if (cols <= 64) {
-        f(std::integral_constant<int, 64>{});
-    } else if (cols <= 128) {
+    const auto enough = [&](int bn) { return static_cast<long long>(tiles_of(rows, kTileM)) * tiles_of(cols, bn) >= kEnoughTiles; };
+    if (cols > 128 && enough(256)) {
+        f(std::integral_constant<int, 256>{});
+    } else if (cols > 64 && enough(128)) {
         f(std::integral_constant<int, 128>{});
     } else {
-        f(std::integral_constant<int, 256>{});
+        f(std::integral_constant<int, 64>{});
     }
 }
 
@@ -954,8 +966,8 @@ void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, 
         }
     }
     const Matrix mh = hidden_matrix<T>(n, arena);
-    {
-        constexpr int BN = sizeof(T) == 4 ? 64 : 128;
+    const auto gate = [&](auto width) {
+        constexpr int BN = decltype(width)::value;
         Maps maps;
         maps.a[0] = mx.map(kTileM);
         maps.b[0] = mg.map(BN);
@@ -967,8 +979,17 @@ void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, 
         g.pitch = mh.pitch;
         g.plane = mh.rows * mh.pitch;
         with_activation(n.act, [&](auto act) { launch_product<Kind::kGate, BN, 1, T, decltype(act)::value>(maps, g, stream); });
+    };
+    // As with_width, up to 128; float32 with short products is bound by its epilogue, which two narrow tiles
+    // overlap better (262144 x 64 x 128: 166 us at 64 columns, 184 us at 128).
+    const bool wide = n.hidden > 64 && static_cast<long long>(tiles_of(n.tokens, kTileM)) * tiles_of(n.hidden, 128) >= kEnoughTiles
+                      && (sizeof(T) == 2 || n.channels >= 128);
+    if (wide) {
+        gate(std::integral_constant<int, 128>{});
+    } else {
+        gate(std::integral_constant<int, 64>{});
     }
-    with_width<T>(n.outputs, [&](auto width) {
+    with_width(n.tokens, n.outputs, [&](auto width) {
         constexpr int BN = decltype(width)::value;
         Maps maps;
         maps.a[0] = mh.map(kTileM);
@@ -999,7 +1020,7 @@ void set_weight_tiles(Args& g, const MlpShape& n)
 {
     const bool large = large_weight_tiles<T>(n);
     const int tile_rows = large ? 256 : 128;
-    const int tile_cols = large ? 256 : sizeof(T) == 4 ? 64 : 128;
+    const int tile_cols = large ? 256 : 128;
     const int rows[3] = {n.hidden, n.hidden, n.outputs};
     const int cols[3] = {n.channels, n.channels, n.hidden};
     g.first[0] = 0;
@@ -1126,7 +1147,7 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
     } else {
         gate_back(std::integral_constant<int, 64>{});
     }
-    with_width<T>(n.channels, [&](auto width) {
+    with_width(n.tokens, n.channels, [&](auto width) {
         constexpr int BN = decltype(width)::value;
         Maps maps;
         maps.a[0] = mdg.map(kTileM);
@@ -1153,10 +1174,12 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         set_weight_tiles<T>(g, n);
         float* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts));
         g.out[0] = partial;
-        if constexpr (sizeof(T) == 4) {
-            launch_product<Kind::kWeight, 64, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
-        } else if (large_weight_tiles<T>(n)) {
-            launch_product<Kind::kWeight, 256, 2, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+        if constexpr (sizeof(T) == 2) {
+            if (large_weight_tiles<T>(n)) {
+                launch_product<Kind::kWeight, 256, 2, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+            } else {
+                launch_product<Kind::kWeight, 128, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
+            }
         } else {
             launch_product<Kind::kWeight, 128, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
         }
