@@ -1151,6 +1151,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     const T* src = x + (sample * n.channels + c0) * n.points + chunk * s.rows;
     T* dst = y + (sample * n.points + chunk * s.rows) * n.channels + c0;
+    const bool whole = (reinterpret_cast<std::uintptr_t>(dst) & 31u) == 0;  // then every point's eight values are a sector
     for (int r = (warp / across * 32 + lane) * V; r < count; r += along * 32 * V) {
         Vec<T, V> in[kChannels];
 #pragma unroll
@@ -1177,7 +1178,9 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             T* at = dst + static_cast<long long>(r + j) * n.channels;
-            if constexpr (sizeof(T) == 4) {
+            if (sizeof(T) == 4 && whole) {
+                store32(at, *reinterpret_cast<const uint32_t(*)[8]>(&out[j]));
+            } else if constexpr (sizeof(T) == 4) {
                 reinterpret_cast<Vec<T, 4>*>(at)[0] = *reinterpret_cast<const Vec<T, 4>*>(&out[j].v[0]);
                 reinterpret_cast<Vec<T, 4>*>(at)[1] = *reinterpret_cast<const Vec<T, 4>*>(&out[j].v[4]);
             } else {
@@ -1628,6 +1631,9 @@ extern "C" int spectral_group_norm_act(const void* x, const float* weight, const
     const int status = check("group_norm_act", dtype, batch, points, channels, groups, activation);
     if (status != SPECTRAL_OK || batch == 0 || points == 0) {
         return status;
+    }
+    if (!(eps >= 0.0f)) {
+        return invalid("group_norm_act: eps must be at least 0");
     }
     if (x == nullptr || y == nullptr || work == nullptr || (mean == nullptr) != (rstd == nullptr)
         || (codes == nullptr) != (scales == nullptr)) {

@@ -345,3 +345,33 @@ def test_gradients_of_gradients_are_refused_and_unused_ones_cost_nothing_else():
     frozen = [args[0].clone().requires_grad_(True), *args[1:]]
     (dx,) = torch.autograd.grad(gated_mlp(*frozen), frozen[:1], dy)
     assert torch.equal(dx, torch.autograd.grad(gated_mlp(*leaves), leaves[:1], dy)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("tokens", "channels"), [(4, 64), (1000, 64), (1000, 200)])
+def test_a_captured_training_step_replays_with_new_inputs(tokens, channels):
+    # Norm, feed-forward block and their backward passes in one CUDA graph, after a first call outside it.
+    *args, dy = inputs(tokens, channels, 96, channels, torch.bfloat16)
+    x = args[0].view(1, tokens, channels)
+    weight = torch.ones(channels, device="cuda")
+
+    def step(x, dy):
+        leaves = [x.detach().requires_grad_(True), weight.detach().requires_grad_(True), *(a.detach().requires_grad_(True) for a in args[1:])]
+        y = gated_mlp(spectral.nn.group_norm_act(leaves[0], 2, leaves[1], activation="gelu", checkpoint8=True), *leaves[2:])
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    static_x, static_dy = x.clone(), dy.view(1, tokens, channels).clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static_x, static_dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static_x, static_dy)
+    new_x, new_dy = x * 0.5 + 0.25, static_dy.flip(1)
+    static_x.copy_(new_x)
+    static_dy.copy_(new_dy)
+    graph.replay()
+    for a, b in zip(out, step(new_x, new_dy)):
+        assert torch.equal(a, b)

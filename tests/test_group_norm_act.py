@@ -277,7 +277,7 @@ def forward_args(**change):
 @pytest.mark.parametrize(
     ("change", "message"),
     [(dict(dtype=5), "dtype must be"), (dict(activation=9), "activation must be"), (dict(groups=3), "groups dividing channels"),
-     (dict(groups=0), "groups dividing channels"), (dict(batch=-1), "batch >= 0"), (dict(work=None), "must be given"),
+     (dict(groups=0), "groups dividing channels"), (dict(eps=-1.0), "eps must be"), (dict(eps=math.nan), "eps must be"), (dict(batch=-1), "batch >= 0"), (dict(work=None), "must be given"),
      (dict(mean=4096), "mean with rstd"), (dict(codes=4096), "codes with scales"), (dict(x=4098), "aligned"),
      (dict(y=4096 + 64), "must not overlap"), (dict(channels_first=1, points=5), "channels first needs"),
      (dict(channels_first=1, codes=1 << 20, scales=1 << 21), "channels first needs"), (dict(batch=1 << 31, x=1 << 60), "at most 2\\^30 samples")])
