@@ -318,3 +318,75 @@ def test_wrong_arguments_are_refused():
         group_norm_act(x.double(), 2)
     with pytest.raises(RuntimeError, match="must be \\(batch"):
         group_norm_act(x[0, 0], 2)
+
+
+# Fields with the channels first in memory, as a convolution leaves them: (batch, channels, points along two axes), groups.
+FIRST = [((2, 16, 8, 8), 4), ((3, 24, 12, 16), 3), ((2, 8, 1, 8), 1), ((1, 72, 64, 96), 72), ((1, 136, 50, 40), 2), ((2, 64, 72, 1000), 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("checkpoint8", [False, True])
+@pytest.mark.parametrize(("shape", "groups"), FIRST)
+def test_channels_first_in_memory(shape, groups, checkpoint8, dtype):
+    b, c, *points = shape
+    x, weight, bias, dy = inputs((b, *points, c), dtype, sum(shape) + groups)
+    first = x.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1)  # the same values, channels first
+    dy_first = dy.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1)
+    leaves = [t.detach().requires_grad_(True) for t in (first, weight, bias)]
+    y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], activation="gelu", checkpoint8=checkpoint8)
+    assert y.is_contiguous() and y.shape == x.shape
+    got = torch.autograd.grad(y, leaves, dy_first)
+    close(group_norm_act(first, groups, weight, bias, activation="gelu"), y, TOL[torch.float32] + (0 if dtype == torch.float32 else TOL[dtype]))
+    close(y, formula(x.double(), groups, weight.double(), bias.double(), 1e-5, "gelu"),
+          TOL[dtype] + first_single(x, groups))
+    at = spectral.unpack8(*spectral.pack8(x), dtype=dtype) if checkpoint8 else x
+    want = gradients_at(at.double(), x.double(), groups, weight.double(), bias.double(), 1e-5, "gelu", dy.double())
+    single = first_single(x, groups)
+    v = x.double().reshape(b, -1, groups, c // groups)
+    std = (v.var((1, 3), unbiased=False) + 1e-5).sqrt()
+    terms = float(((1.0 / std)[:, None, :, None] * (dy.double() * weight.double()).reshape(v.shape)).norm())
+    err = float((got[0].double() - want[0]).norm())
+    assert err <= (TOL[dtype] + single) * float(want[0].norm()) + single * 2 * terms, f"dx: {err:.3g}"
+    for name, g, w, factor in (("dweight", got[1], want[1], 4), ("dbias", got[2], want[2], 2)):
+        size = float((dy.double().abs() * factor).sum()) / c ** 0.5
+        assert float((g.double() - w).abs().max()) <= single * (float(w.abs().max()) + size), name
+
+
+def first_single(x, groups):
+    v = x.double().reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
+    std = (v.var((1, 3), unbiased=False) + 1e-5).sqrt()
+    return TOL[torch.float32] * (1.0 + float((v.mean((1, 3)).abs() / std).max()))
+
+
+@pytest.mark.gpu
+def test_channels_first_statistics_of_a_large_mean_and_non_finite_values():
+    g = torch.Generator().manual_seed(7)
+    x = (torch.randn(2, 16, 40, 30, generator=g) + 3000.0).cuda().permute(0, 2, 3, 1)
+    close(group_norm_act(x, 2), formula(x.double(), 2, None, None, 1e-5, "none"), 64 * 3001 * 2.0 ** -24)
+    clean = group_norm_act(x, 2)
+    x[0, 3, 1, 2] = float("nan")
+    y = group_norm_act(x, 2)
+    assert y[0, ..., :8].isnan().all() and torch.equal(y[0, ..., 8:], clean[0, ..., 8:]) and torch.equal(y[1], clean[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("batch", "points", "channels"), [(1, 8, 8), (3, 200, 24), (2, 5000, 136), (70000, 8, 8)])
+def test_the_c_abi_lays_channels_last(batch, points, channels, dtype):
+    x = torch.randn(batch, channels, points, generator=torch.Generator().manual_seed(points)).to(dtype).cuda()
+    y = torch.empty(batch, points, channels, dtype=dtype, device="cuda")
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    native.call("spectral_channels_last", x.data_ptr(), y.data_ptr(), code, batch, points, channels, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(y, x.transpose(1, 2))
+
+
+@pytest.mark.parametrize(
+    ("change", "message"),
+    [(dict(dtype=4), "dtype must be"), (dict(points=5), "points of 16 bytes"), (dict(channels=12), "multiple of 8"), (dict(x=4104), "aligned"),
+     (dict(x=None), "needs"), (dict(y=4096 + 32), "must not overlap"), (dict(batch=-1), "batch >= 0")])
+def test_the_c_abi_refuses_to_lay_channels_last(change, message):
+    a = dict(x=4096, y=1 << 20, dtype=0, batch=2, points=8, channels=8, stream=None)
+    a.update(change)
+    with pytest.raises(ValueError, match=message):
+        native.call("spectral_channels_last", *a.values())
