@@ -8,7 +8,7 @@
 // Backward, from x (or its 8-bit checkpoint) and dy alone:
 //   gate back  G, U and dh = dy Wd in one kernel; its epilogue stores dU = dh act(G),
 //              dG = dh U act'(G) and h
-//   input      dx = dG Wg + dU Wu, one accumulator over both products
+//   input      dx = dG Wg + dU Wu, one sum over both products
 //   weights    dWg = dG^T x, dWu = dU^T x, dWd = dy^T h, K = tokens: the token range is cut into
 //              parts, FP32 partial products are added up in a fixed order by a last kernel
 // Weights and activations are used as they lie: a product that needs a transposed operand reads
@@ -201,6 +201,11 @@ struct Tile {
     int part;
     int passes;
 };
+
+// float32 dx: its two products take passes of their own, alternately, or the second's small products
+// would be cut against the first's sum (an error of 1.3e-6 instead of 3e-7).
+template <Kind K, class T>
+constexpr bool kApart = K == Kind::kInput && sizeof(T) == 4;
 
 // The chunks of operand pair `pair` that pass `pass` of a tile covers.
 template <class T>
@@ -415,18 +420,20 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         for (long long t = blockIdx.x; ok && t < g.tiles; t += gridDim.x) {
             const Tile tile = locate<K, BN, MT, T>(g, t);
             constexpr int kPairs = K == Kind::kGateBack || K == Kind::kInput ? 2 : 1;
-            for (int pass = 0; ok && pass < tile.passes; ++pass) {
+            const int passes = tile.passes * (kApart<K, T> ? 2 : 1);
+            for (int pass = 0; ok && pass < passes; ++pass) {
                 ok = tma::mbar_wait(&freed[slot], slot_phase ^ 1u);
                 if (!ok) {
                     break;
                 }
                 umma::fence_after_sync();
-                for (int pair = 0; ok && pair < kPairs; ++pair) {
+                const int first = kApart<K, T> ? pass & 1 : 0;
+                for (int pair = first; ok && pair < (kApart<K, T> ? first + 1 : kPairs); ++pair) {
                     int k0, k1;
-                    pass_range<T>(g, tile, pair, pass, k0, k1);
+                    pass_range<T>(g, tile, pair, kApart<K, T> ? pass >> 1 : pass, k0, k1);
                     const int steps = (k1 - k0) * Op::kProducts;
-                    // kInput's two products share an accumulator; kGateBack's second has its own.
-                    const bool fresh = pair == 0 || K == Kind::kGateBack;
+                    // kInput's two products share an accumulator (16-bit types); kGateBack's second has its own.
+                    const bool fresh = kApart<K, T> || pair == 0 || K == Kind::kGateBack;
                     const uint32_t d = tmem + slot * Cfg::kCols + (K == Kind::kGateBack && pair == 1 ? 2 * BN : 0);
                     for (int i = 0; i < steps; ++i) {
                         ok = tma::mbar_wait(&full[stage], phase);
@@ -517,7 +524,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         }
                     }
                 }
-                for (int pass = 0; ok && pass < tile.passes; ++pass) {
+                const int passes = tile.passes * (kApart<K, T> ? 2 : 1);
+                for (int pass = 0; ok && pass < passes; ++pass) {
                     ok = tma::mbar_wait(&done[slot], slot_phase);
                     if (!ok) {
                         break;
@@ -528,7 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     for (int q = 0; q < Cfg::kSets; ++q) {
                         // An operand pair that ended in an earlier pass has nothing new here.
                         int begin, end;
-                        pass_range<T>(g, tile, K == Kind::kGateBack && q == 2 ? 1 : 0, pass, begin, end);
+                        pass_range<T>(g, tile, kApart<K, T> ? pass & 1 : K == Kind::kGateBack && q == 2 ? 1 : 0,
+                                      kApart<K, T> ? pass >> 1 : pass, begin, end);
                         if (begin < end) {
 #pragma unroll
                             for (int r = 0; r < kRuns; ++r) {

@@ -375,3 +375,19 @@ def test_a_captured_training_step_replays_with_new_inputs(tokens, channels):
     graph.replay()
     for a, b in zip(out, step(new_x, new_dy)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("tokens", "channels", "hidden"), [(300, 100, 270), (700, 240, 2000), (40, 16, 130)])
+def test_float32_products_stay_at_float32_error(tokens, channels, hidden):
+    # A pass of 128 values of K ends with eight products on the full-size sum, each cut by at most a unit in
+    # the last place, 2^-23, half of it on average: 8 units of 2^-24; 4 more for the small products, the
+    # operands' rounding and the sums of passes.
+    *args, dy = inputs(tokens, channels, hidden, channels, torch.float32)
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    y = gated_mlp(*leaves, activation="silu")
+    wide = [a.double().requires_grad_(True) for a in args]
+    want = formula(*wide, "silu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    for got, exact in zip((y, *grads), (want, *torch.autograd.grad(want, wide, dy.double()))):
+        assert float((got.detach().double() - exact.detach()).norm()) <= 12 * 2.0 ** -24 * float(exact.detach().norm())
