@@ -262,7 +262,7 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
             float2 slope;
             const float2 up = make_float2(acc[1][j], acc[1][j + 1]);
             const float2 dh = make_float2(acc[2][j], acc[2][j + 1]);
-            const float2 a = activate_slope2<Act>(make_float2(acc[0][j], acc[0][j + 1]), slope);
+            const float2 a = activate_slope2<Act, T>(make_float2(acc[0][j], acc[0][j + 1]), slope);
             const float2 dg = dh * up * slope, h = a * up, du = dh * a;
             acc[0][j] = dg.x;
             acc[0][j + 1] = dg.y;

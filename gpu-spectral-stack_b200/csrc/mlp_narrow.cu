@@ -21,11 +21,12 @@
 // x, dy, the weights and the hidden tiles each serve as K-major and as MN-major operands from the
 // one copy in shared memory (umma.cuh).
 //
-// What bounds them (64 channels, 128 hidden). Forward: gelu, whose two special functions a value (16 a cycle)
-// are 2048 of a tile's 2900 cycles; a polynomial without any measured the same, bound by its
-// multiply-adds (31 us against 18.5 us with no activation; HBM alone 10 us). Backward: the tensor
-// cores' reads of shared memory; a tile's 56 MMAs of N = 64 or 128 take some 85 cycles each, 4800 in
-// all, which is a tile's period (60 us with gelu, 50 us without).
+// What bounds them (262144 tokens, 64 channels, 128 hidden). Forward: the instructions of the epilogue
+// warps (31 us with gelu, 29 us with silu, 20.5 us with no activation; HBM alone 10 us). gelu without
+// special functions, a polynomial, and with one reciprocal for two values measured the same: what they
+// save there they spend on multiply-adds. Backward: the tensor cores' reads of shared memory; a tile's 56
+// MMAs of N = 64 or 128 take some 85 cycles each, 4800 in all, which is a tile's period (58 us with gelu,
+// 55 us without).
 
 #include "mlp.cuh"
 
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
                     float2 slope;
                     const float2 up = make_float2(u[i], u[i + 1]);
                     const float2 d = make_float2(dh[i], dh[i + 1]);
-                    const float2 v = activate_slope2<Act>(make_float2(a[i], a[i + 1]), slope);
+                    const float2 v = activate_slope2<Act, T>(make_float2(a[i], a[i + 1]), slope);
                     const float2 dg = d * up * slope, h = v * up, du = d * v;
                     a[i] = dg.x;
                     a[i + 1] = dg.y;

@@ -21,8 +21,10 @@
 // Two-pass form: chunks of a sample's rows give partial results (means and squares about them, joined
 // block by block, so that neither a large mean nor an outlier cancels), a small kernel joins them, and
 // the outputs are computed from a second read, which runs backwards to meet what is still in L2.
-// Same array: 86 us forward (402 MB in three passes: 4.7 TB/s), 150 us backward (671 MB: 4.5 TB/s);
-// float32 138 us (5.8 TB/s) and 221 us (6.1 TB/s).
+// Same array with gelu: 85 us forward (402 MB in three passes: 4.7 TB/s; 74 us with no activation), 148 us
+// backward (671 MB: 4.5 TB/s; 134 us), from an 8-bit checkpoint 185 us (141 us); float32 135 us (6.0 TB/s) and
+// 223 us (6.0 TB/s). Cutting the batch so that a part's second read stays in L2 measured slower at every
+// cut (2 to 16 parts: 105 to 330 us forward, 180 to 470 us backward): each part pays its launches' ends.
 // Keeping the second read in L2, with persistent CTAs that take sum and apply tasks a few samples
 // apart, measured 97 us and 207 us: a sample's statistics take some 10 us from its last sum to its
 // first output (fences, atomics, flags), and at this bandwidth 65 MB pass in that time.
@@ -351,12 +353,12 @@ struct Channels {
         }
     }
     // xhat and dz = dy act'(z) of pair j.
-    template <int Act>
+    template <int Act, class T>
     __device__ __forceinline__ float2 slope(float2 x, float2 dy, int j, float2& xhat) const
     {
         xhat = (x - mean.p[j]) * rstd.p[j];
         float2 s;
-        activate_slope2<Act>(fma2(xhat, weight.p[j], bias.p[j]), s);
+        activate_slope2<Act, T>(fma2(xhat, weight.p[j], bias.p[j]), s);
         return dy * s;
     }
 };
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < Floats<V>::kPairs; ++j) {
             float2 xhat;
-            const float2 dz = ch.template slope<Act>(f.p[j], g.p[j], j, xhat);
+            const float2 dz = ch.template slope<Act, T>(f.p[j], g.p[j], j, xhat);
             part_dz.p[j] = part_dz.p[j] + dz;
             part_dzx.p[j] = fma2(dz, xhat, part_dzx.p[j]);
         }
@@ -477,7 +479,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < Floats<V>::kPairs; ++j) {
             float2 xhat;
-            const float2 dz = ch.template slope<Act>(f.p[j], g.p[j], j, xhat);
+            const float2 dz = ch.template slope<Act, T>(f.p[j], g.p[j], j, xhat);
             const float2 t = fma2(dz, ch.weight.p[j], pair(0.0f) - mt.p[j]);
             f.p[j] = ch.rstd.p[j] * (t - xhat * mtx.p[j]);
         }
@@ -970,7 +972,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < Floats<V>::kPairs; ++j) {
             float2 xhat;
-            const float2 dz = ch.template slope<Act>(x.p[j], g.p[j], j, xhat);
+            const float2 dz = ch.template slope<Act, T>(x.p[j], g.p[j], j, xhat);
             a.p[j] = a.p[j] + dz;
             b.p[j] = fma2(dz, xhat, b.p[j]);
         }
@@ -1039,7 +1041,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < Floats<V>::kPairs; ++j) {
             float2 xhat;
-            const float2 dz = ch.template slope<Act>(x.p[j], g.p[j], j, xhat);
+            const float2 dz = ch.template slope<Act, T>(x.p[j], g.p[j], j, xhat);
             f.p[j] = ch.rstd.p[j] * (dz * ch.weight.p[j] - mt.p[j] - xhat * mtx.p[j]);
         }
         *reinterpret_cast<Vec<T, V>*>(dst) = narrow<T>(f);

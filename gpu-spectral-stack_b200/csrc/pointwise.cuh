@@ -161,43 +161,34 @@ __device__ __forceinline__ float2 sigmoid2(float2 z)
     return make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
 }
 
-// The normal distribution function Phi(z), and e = exp(-z^2 / 2), which its density shares.
-// 1 - Phi(|z|) = e t P(t) with t = 1 / (1 + 0.28 |z|), the form of Hastings' approximations; P
-// (degree 5) is a least-squares fit of this library's own, off by less than 1.5e-8. One power and
-// one reciprocal give the value and the slope of gelu, about ten instructions a value; erff and
-// expf measured 47 against 22 for the whole normalisation of a value.
-__device__ __forceinline__ float2 normal_cdf2(float2 z, float2& e)
+// Phi(|z|) - 1/2 of the normal distribution function, with az = |z| and e = exp(-z^2 / 2), which the
+// density shares: 1 - Phi(|z|) = e t P(t) with t = 1 / (1 + c |z|), the form of Hastings' approximations.
+// c and P are least-squares fits of this library's own: degree 5, off by less than 1.5e-8, and for
+// results that are rounded to 16 bits degree 4, off by less than 7e-8 (of z Phi(z) at z = -3: 5e-5 of its
+// size; a bf16 or f16 rounding is 2^-9, 2^-12).
+template <class T>
+__device__ __forceinline__ float2 normal_half2(float2 z, float2& az, float2& e)
 {
+    constexpr bool kShort = sizeof(T) == 2;
     const float2 x = (z * pair(-0.7213475204444817f)) * z;
     e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-    const float2 t = make_float2(reciprocal_fast(fmaf(0.28f, fabsf(z.x), 1.0f)), reciprocal_fast(fmaf(0.28f, fabsf(z.y), 1.0f)));
-    float2 p = pair(-0.10655131936073303f);
-    p = fma2(p, t, pair(0.3929559588432312f));
-    p = fma2(p, t, pair(-0.2420753836631775f));
-    p = fma2(p, t, pair(0.27307337522506714f));
-    p = fma2(p, t, pair(0.06580273061990738f));
-    p = fma2(p, t, pair(0.11679460108280182f));
-    const float2 half = fma2(p * t, e * pair(-1.0f), pair(0.5f));  // Phi(|z|) - 1/2
-    return pair(0.5f) + make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y));
-}
-
-// Phi(z) for results that are rounded to 16 bits: the logistic function of z P(z^2), P (degree 6, a
-// least-squares fit of this library's own) the even part of log(Phi(z) / Phi(-z)) / z. z Phi(z) is off
-// by less than 6e-7 in all and by 5e-5 of its own size for z > -3 (a bf16 or f16 rounding: 2^-9, 2^-12).
-// Seven instructions a value against normal_cdf2's ten, every one of them packed.
-__device__ __forceinline__ float2 normal_cdf16(float2 z)
-{
-    const float2 u = z * z;
-    float2 p = pair(-4.304068657035032e-09f);  // times -log2(e)
-    p = fma2(p, u, pair(3.4366911449978943e-07f));
-    p = fma2(p, u, pair(-1.07983396446798e-05f));
-    p = fma2(p, u, pair(0.0001548998843645677f));
-    p = fma2(p, u, pair(0.00010911076969932765f));
-    p = fma2(p, u, pair(-0.1048540323972702f));
-    p = fma2(p, u, pair(-2.3022031784057617f));
-    p = p * z;
-    const float2 d = make_float2(exp2_fast(p.x), exp2_fast(p.y)) + pair(1.0f);
-    return make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+    az = make_float2(fabsf(z.x), fabsf(z.y));
+    const float2 d = fma2(az, pair(kShort ? 0.33f : 0.28f), pair(1.0f));
+    const float2 t = make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+    float2 p;  // -P
+    if constexpr (kShort) {
+        p = fma2(pair(0.11067703366279602f), t, pair(-0.3792961835861206f));
+        p = fma2(p, t, pair(0.09625490754842758f));
+        p = fma2(p, t, pair(-0.20623883605003357f));
+        p = fma2(p, t, pair(-0.12139694392681122f));
+    } else {
+        p = fma2(pair(0.10655131936073303f), t, pair(-0.3929559588432312f));
+        p = fma2(p, t, pair(0.2420753836631775f));
+        p = fma2(p, t, pair(-0.27307337522506714f));
+        p = fma2(p, t, pair(-0.06580273061990738f));
+        p = fma2(p, t, pair(-0.11679460108280182f));
+    }
+    return fma2(p * t, e, pair(0.5f));
 }
 
 // The activation of a value that is then rounded to T.
@@ -206,18 +197,17 @@ __device__ __forceinline__ float2 activate2(float2 z)
 {
     if constexpr (Act == SPECTRAL_ACT_SILU) {
         return z * sigmoid2(z);
-    } else if constexpr (Act == SPECTRAL_ACT_GELU && sizeof(T) == 2) {
-        return z * normal_cdf16(z);
     } else if constexpr (Act == SPECTRAL_ACT_GELU) {
-        float2 e;
-        return z * normal_cdf2(z, e);
+        float2 az, e;
+        const float2 half = normal_half2<T>(z, az, e);
+        return fma2(az, half, z * pair(0.5f));  // z Phi(z) = z / 2 + |z| (Phi(|z|) - 1/2)
     } else {
         return z;
     }
 }
 
-// The activation's values and slopes at z.
-template <int Act>
+// The activation's values and slopes at z, of which T results are made.
+template <int Act, class T>
 __device__ __forceinline__ float2 activate_slope2(float2 z, float2& slope)
 {
     if constexpr (Act == SPECTRAL_ACT_SILU) {
@@ -226,10 +216,11 @@ __device__ __forceinline__ float2 activate_slope2(float2 z, float2& slope)
         slope = fma2(a, pair(1.0f) - s, s);
         return a;
     } else if constexpr (Act == SPECTRAL_ACT_GELU) {
-        float2 e;
-        const float2 phi = normal_cdf2(z, e);
-        slope = fma2(z * pair(0.3989422804014327f), e, phi);
-        return z * phi;
+        float2 az, e;
+        const float2 half = normal_half2<T>(z, az, e);
+        const float2 odd = fma2(az * pair(0.3989422804014327f), e, half);  // of Phi(z) + z phi(z) - 1/2
+        slope = pair(0.5f) + make_float2(copysignf(odd.x, z.x), copysignf(odd.y, z.y));
+        return fma2(az, half, z * pair(0.5f));
     } else {
         slope = pair(1.0f);
         return z;
