@@ -15,12 +15,14 @@
 // the same TMA tile through an MN-major descriptor (umma.cuh), nothing is transposed in memory.
 //
 // One kernel template serves the products: persistent CTAs (one per SM), a TMA warp, an MMA warp
-// (one elected lane issues) and eight epilogue warps; tiles of 128 rows, K in chunks of 64,
-// kStages chunks in flight; two accumulator sets in tensor memory, so a tile's epilogue runs under
-// the next tile's products. Every wait is bounded (tma.cuh).
+// (one elected lane issues) and eight epilogue warps; tiles of 128 rows (256 where that pays), K in
+// chunks of 64, kStages chunks in flight; two accumulator sets in tensor memory where they fit, so a
+// tile's epilogue runs under the next tile's products. 8192 x 512 x 2048 bf16: forward 43 us (51.5
+// GFLOP, 1.2 PFLOP/s), backward 149 us (with the recomputed products 137 GFLOP, 0.92 PFLOP/s). Every wait is bounded (tma.cuh).
 //
 // Types: bf16 and f16 run as they are, accumulated in FP32; h, dG and dU are rounded once to the
-// type, as they feed the next product. float32 operands are split into three bf16 parts
+// type, as they feed the next product. With the rounding of the result that is 1.4 times the error of
+// rounding the result alone; a second 16-bit part of them would double those products. float32 operands are split into three bf16 parts
 // (24 significand bits, bf16 has FP32's range) and the six products of order up to 2 (hi hi, hi
 // mid, mid hi, mid mid, hi lo, lo hi) are taken: the dropped ones are below 2^-24 of the product.
 // The tensor core cuts its FP32 accumulator once per MMA, an error that grows with K, so float32

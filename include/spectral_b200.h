@@ -321,9 +321,9 @@ SPECTRAL_API int spectral_mode_contract_method(const void* x, const void* w, voi
  * SPECTRAL_PACK8_BLOCK values (the last may be shorter). With m = max(|v|, 2^-100) over a block,
  *   scale = m / 127,  code = round(v * (127 / m)) to nearest, ties to even,  value = code * scale
  * (each operation in FP32, the value at most the largest float), so a restored value is off by at
- * most half a scale. A block with an
- * infinity or NaN restores as NaN throughout. codes: rows x width int8; scales: rows x
- * ceil(width / 64) floats. spectral_unpack8 writes the values in `dtype`. */
+ * most half a scale. A block with an infinity or NaN restores as NaN throughout. codes: rows x
+ * width int8; scales: rows x ceil(width / 64) floats. spectral_unpack8 writes the values in
+ * `dtype`. */
 #define SPECTRAL_PACK8_BLOCK 64
 SPECTRAL_API int spectral_pack8(const void* x, int dtype, void* codes, float* scales, long long rows, int width,
                                 void* stream);
@@ -333,7 +333,7 @@ SPECTRAL_API int spectral_unpack8(const void* codes, const float* scales, void* 
 /* Group norm with an activation: x and y (batch, points, channels),
  *   y = act((x - mean) rstd weight + bias),  rstd = 1 / sqrt(var + eps),
  * mean and var (biased) per sample over the points x (channels / groups) values of each group.
- * weight and bias: `channels` floats, or NULL for 1 and 0. mean and rstd (batch x groups floats)
+ * eps >= 0. weight and bias: `channels` floats, or NULL for 1 and 0. mean and rstd (batch x groups floats)
  * receive the statistics for the backward pass; both may be NULL. codes and scales (both or
  * neither) receive x's 8-bit checkpoint (rows of `channels`). x and y must not overlap. With
  * channels_first, x is (batch, channels, points), as a spectral convolution leaves it, and is read
@@ -366,7 +366,9 @@ SPECTRAL_API int spectral_channels_last(const void* x, void* y, int dtype, long 
  *   y = (act(x w_gate^T) * (x w_up^T)) w_down^T
  * x (tokens, channels), w_gate and w_up (hidden, channels), w_down (outputs, hidden),
  * y (tokens, outputs), all of `dtype`. Products run on the tensor cores with FP32 accumulators;
- * FP32 operands are split into three bf16 parts (FP32-level error). */
+ * FP32 operands are split into three bf16 parts (FP32-level error). In the 16-bit types the hidden
+ * values (backward: also the gradients of both products) are rounded once to the type between the
+ * products, and have its range: an FP16 hidden value beyond 65504 is infinite. */
 SPECTRAL_API int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
                                               size_t* count);
 SPECTRAL_API int spectral_gated_mlp(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* y,
