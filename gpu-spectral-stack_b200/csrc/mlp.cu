@@ -15,10 +15,10 @@
 // the same TMA tile through an MN-major descriptor (umma.cuh), nothing is transposed in memory.
 //
 // One kernel template serves the products: persistent CTAs (one per SM), a TMA warp, an MMA warp
-// (one elected lane issues) and eight epilogue warps; tiles of 128 rows (256 where that pays), K in
+// (one elected lane issues) and eight or sixteen epilogue warps; tiles of 128 rows (256 where that pays), K in
 // chunks of 64, kStages chunks in flight; two accumulator sets in tensor memory where they fit, so a
 // tile's epilogue runs under the next tile's products. 8192 x 512 x 2048 bf16: forward 43 us (51.5
-// GFLOP, 1.2 PFLOP/s), backward 149 us (with the recomputed products 137 GFLOP, 0.92 PFLOP/s). Every wait is bounded (tma.cuh).
+// GFLOP, 1.2 PFLOP/s), backward 146 us (with the recomputed products 137 GFLOP, 0.94 PFLOP/s). Every wait is bounded (tma.cuh).
 //
 // Types: bf16 and f16 run as they are, accumulated in FP32; h, dG and dU are rounded once to the
 // type, as they feed the next product. With the rounding of the result that is 1.4 times the error of
@@ -113,22 +113,22 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ Stag
 // --- epilogue stores ---------------------------------------------------------------------------------
 
 // A run of hidden values in the operand form (planes `plane` values apart).
-template <class T>
-__device__ __forceinline__ void store_hidden(typename Operand<T>::Type* p, long long plane, const float (&v)[32], int valid)
+template <class T, int N>
+__device__ __forceinline__ void store_hidden(typename Operand<T>::Type* p, long long plane, const float (&v)[N], int valid)
 {
     if constexpr (sizeof(T) == 4) {
-        bf16 hi[32], mid[32], lo[32];
+        bf16 hi[N], mid[N], lo[N];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             split3(v[j], hi[j], mid[j], lo[j]);
         }
         store_run(p, hi, valid);
         store_run(p + plane, mid, valid);
         store_run(p + 2 * plane, lo, valid);
     } else {
-        T out[32];
+        T out[N];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             out[j] = from_float<T>(v[j]);
         }
         store_run(p, out, valid);
@@ -174,8 +174,16 @@ struct Args {
 
 // A tile is MT x 128 rows by BN columns (of each accumulator). Two accumulator sets where tensor memory
 // holds them, so that a tile's epilogue runs under the next tile's products.
-template <Kind K, int BN, int MT>
+template <Kind K, int BN, int MT, class T>
 struct Config {
+    // The activation's epilogues wait on special functions and tensor memory: sixteen warps in 16-bit types, each
+    // a quarter of the columns in runs of 16 (16384 x 256 x 1024 backward 100 us, with eight 115 us; float32
+    // sums need the registers of eight).
+    static constexpr bool kActs = sizeof(T) == 2 && (K == Kind::kGate || K == Kind::kGateBack);
+    static constexpr int kEpilogueWarps = kActs ? 16 : 8;
+    static constexpr int kThreads = 32 * (kEpilogueWarps + 2);
+    static constexpr int kRun = kActs ? 16 : 32;                   // columns of a row at a time
+    static constexpr int kColumns = BN / (kEpilogueWarps / 4);     // a warp's
     static constexpr bool kAMn = K == Kind::kWeight;
     static constexpr int kSets = K == Kind::kGate ? 2 : K == Kind::kGateBack ? 3 : 1;  // accumulators of BN columns
     static constexpr int kBRows = K == Kind::kGate || K == Kind::kGateBack ? 2 * BN : BN;
@@ -243,16 +251,16 @@ __device__ __forceinline__ Tile locate(const Args& g, long long t)
     return tile;
 }
 
-// The epilogue of 32 columns of one row, from col on: acc holds each accumulator's values.
-template <Kind K, class T, int Act, int Sets>
-__device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row, int col, int cols, float (&acc)[Sets][32])
+// The epilogue of N columns of one row, from col on: acc holds each accumulator's values.
+template <Kind K, class T, int Act, int Sets, int N>
+__device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row, int col, int cols, float (&acc)[Sets][N])
 {
     using Op = typename Operand<T>::Type;
-    const int valid = min(32, cols - col);
+    const int valid = min(N, cols - col);
     const long long at = row * g.pitch + col;
     if constexpr (K == Kind::kGate) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
+        for (int j = 0; j < N; j += 2) {
             const float2 h = activate2<Act, T>(make_float2(acc[0][j], acc[0][j + 1])) * make_float2(acc[1][j], acc[1][j + 1]);
             acc[0][j] = h.x;
             acc[0][j + 1] = h.y;
@@ -260,7 +268,7 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
         store_hidden<T>(static_cast<Op*>(g.out[0]) + at, g.plane, acc[0], valid);
     } else if constexpr (K == Kind::kGateBack) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
+        for (int j = 0; j < N; j += 2) {
             float2 slope;
             const float2 up = make_float2(acc[1][j], acc[1][j + 1]);
             const float2 dh = make_float2(acc[2][j], acc[2][j + 1]);
@@ -285,9 +293,9 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
 }
 
 template <Kind K, int BN, int MT, class T, int Act>
-__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g)
+__global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g)
 {
-    using Cfg = Config<K, BN, MT>;
+    using Cfg = Config<K, BN, MT, T>;
     using Op = Operand<T>;
     constexpr bool kBf16 = std::is_same_v<typename Op::Type, bf16>;
     constexpr int kStages = Cfg::kStages;
@@ -300,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == kEpilogueWarps) {
+    if (warp == Cfg::kEpilogueWarps) {
         umma::alloc<Cfg::kTmemCols>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
@@ -310,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         }
         for (int s = 0; s < 2; ++s) {
             tma::mbar_init(&done[s], 1);
-            tma::mbar_init(&freed[s], kEpilogueWarps);
+            tma::mbar_init(&freed[s], Cfg::kEpilogueWarps);
         }
         tma::mbar_init(&drain, 1);
         gave_up = 0;
@@ -322,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     const uint32_t tmem = tmem_slot;
     wait_for_previous_grid();
 
-    if (warp == kEpilogueWarps) {
+    if (warp == Cfg::kEpilogueWarps) {
         // The TMA warp. The previous kernels' plain stores come before these async-proxy reads.
         asm volatile("fence.proxy.async.global;" ::: "memory");
         int stage = 0;
@@ -407,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                 }
             }
         }
-    } else if (warp == kEpilogueWarps + 1) {
+    } else if (warp == Cfg::kEpilogueWarps + 1) {
         // The MMA warp: converged, so that addresses and descriptors stay warp-uniform, one elected lane
         // issues (one lane throughout measured 10 % slower).
         constexpr bool kBMnFirst = K == Kind::kWeight || K == Kind::kInput;
@@ -499,10 +507,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             }
         }
     } else {
-        // The epilogue warps: warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half the
+        // The epilogue warps: warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and its kColumns
         // columns of each accumulator.
         const int quad = warp & 3;
-        const int half = warp >> 2;
+        const int first = (warp >> 2) * Cfg::kColumns;
         int slot = 0;
         unsigned slot_phase = 0;
         bool ok = true;
@@ -533,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         break;
                     }
                     umma::fence_after_sync();
-                    const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16) + half * (BN / 2);
+                    const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16) + first;
 #pragma unroll
                     for (int q = 0; q < Cfg::kSets; ++q) {
                         // An operand pair that ended in an earlier pass has nothing new here.
@@ -559,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                 }
 #pragma unroll
                 for (int r = 0; r < kRuns; ++r) {
-                    const int col = tile.n0 + half * (BN / 2) + 32 * r;
+                    const int col = tile.n0 + first + 32 * r;
                     if (ok && row < rows && col < cols) {
                         finish<K, T, Act>(g, tile, row, col, cols, acc[r]);
                     }
@@ -570,16 +578,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     umma::fence_after_sync();
                     const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
-                    for (int i = 0; i < MT * (BN / 64); ++i) {
-                        const int m = i / (BN / 64);  // row tile
-                        const int c = half * (BN / 2) + i % (BN / 64) * 32;
+                    for (int i = 0; i < MT * (Cfg::kColumns / Cfg::kRun); ++i) {
+                        const int m = i / (Cfg::kColumns / Cfg::kRun);  // row tile
+                        const int c = first + i % (Cfg::kColumns / Cfg::kRun) * Cfg::kRun;
                         if (tile.n0 + c >= cols) {
                             continue;
                         }
-                        float acc[Cfg::kSets][32];
+                        float acc[Cfg::kSets][Cfg::kRun];
 #pragma unroll
                         for (int q = 0; q < Cfg::kSets; ++q) {
-                            umma::load32(d + (m * Cfg::kSets + q) * BN + c, acc[q]);
+                            umma::load_run(d + (m * Cfg::kSets + q) * BN + c, acc[q]);
                         }
 #pragma unroll
                         for (int q = 0; q < Cfg::kSets; ++q) {
@@ -606,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     if (threadIdx.x == 0 && gave_up != 0) {
         atomicOr(g.fault, tma::kFaultWaitTimeout);
     }
-    if (warp == kEpilogueWarps) {
+    if (warp == Cfg::kEpilogueWarps) {
         umma::dealloc<Cfg::kTmemCols>(tmem);
     }
 }
@@ -871,7 +879,7 @@ Matrix hidden_matrix(const MlpShape& n, Arena& arena)
 template <Kind K, int BN, int MT, class T, int Act>
 void launch_product(const Maps& maps, Args& g, cudaStream_t stream)
 {
-    using Cfg = Config<K, BN, MT>;
+    using Cfg = Config<K, BN, MT, T>;
     static std::atomic<bool> opted[kMaxDevices];
     const int device = current_device();
     const auto kernel = product_kernel<K, BN, MT, T, Act>;
@@ -881,7 +889,7 @@ void launch_product(const Maps& maps, Args& g, cudaStream_t stream)
     }
     g.fault = device_fault_word();
     const long long grid = std::min<long long>(g.tiles, device_sm_count(device));
-    launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), static_cast<std::size_t>(Cfg::kSmem), stream, maps, g);
+    launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(Cfg::kThreads), static_cast<std::size_t>(Cfg::kSmem), stream, maps, g);
 }
 
 // Calls f(integral_constant<BN>) with the widest tile of 64, 128 or 256 columns that `cols` fills and that
@@ -1149,8 +1157,9 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
     };
     // 128 columns leave one accumulator set (384 of 512), so the epilogue does not overlap, but an MMA of N = 64
     // takes nearly as long as one of 128 and a wider tile reads its tokens fewer times: worth it where the
-    // products are long. Backward passes with 128 and 64 columns, us: 8192 x 1024 x 4096 519 and 551,
-    // 8192 x 512 x 2048 149 and 150, 16384 x 256 x 1024 142 and 115.
+    // products are long. Backward passes with 128 and 64 columns, us: 8192 x 1024 x 4096 536 and 557,
+    // 8192 x 512 x 2048 147 and 150, 32768 x 256 x 512 105 and 99. At 128 the tiles' operands are what counts:
+    // 650 MB from L2 to shared memory in the 72 us of 8192 x 512 x 2048, 9 TB/s.
     if constexpr (sizeof(T) == 4) {
         gate_back(std::integral_constant<int, 64>{});  // the passes' sums stay in registers
     } else if (n.channels + n.outputs >= 1024) {

@@ -12,8 +12,6 @@ namespace spectral::mlp {
 
 constexpr int kTileM = 128;
 constexpr int kChunk = umma::kAtom;  // K per stage
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kTileABytes = kTileM * umma::kRowBytes;
 constexpr int kMaxSmem = 227 * 1024;
 

@@ -127,6 +127,8 @@ __device__ __forceinline__ void load16(uint32_t taddr, float (&v)[16])
           "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(taddr));
 }
+__device__ __forceinline__ void load_run(uint32_t taddr, float (&v)[16]) { load16(taddr, v); }
+__device__ __forceinline__ void load_run(uint32_t taddr, float (&v)[32]) { load32(taddr, v); }
 __device__ __forceinline__ void load_wait(float (&v)[16])
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
