@@ -901,50 +901,83 @@ __global__ void __launch_bounds__(kThreads)
     });
 }
 
-// Backward: calls f(dy, x, i) for the thread's rows, Run of them loaded at once.
-template <class T, int V, bool Packed, int Run, class F>
-__device__ __forceinline__ void for_gradient_rows(const T* dy, const Input<T, V, Packed>& in, const Place& at, int channel,
-                                                  const NormShape& n, int rows_per_pass, F&& f)
+// Rows of dy and x on their way to a thread of the backward kernels, kAhead of them in flight. Each thread
+// copies its own pieces and reads only those, so nothing but its own wait is needed. In registers, two
+// rows ahead, they left two CTAs of 120 registers a thread on an SM and half the bandwidth unused.
+constexpr int kAhead = 4;
+template <class T, int V, bool Packed>
+struct Ring {
+    Vec<T, V> g[kAhead + 1][kThreads];
+    typename Input<T, V, Packed>::Raw v[kAhead + 1][kThreads];
+    float scale[Packed ? kAhead + 1 : 1][kThreads];
+};
+
+// Backward: calls f(dy, x) for the thread's rows.
+template <class T, int V, bool Packed, class F>
+__device__ __forceinline__ void for_gradient_rows(Ring<T, V, Packed>& ring, const T* dy, const Input<T, V, Packed>& in,
+                                                  const Place& at, int channel, const NormShape& n, int rows_per_pass, F&& f)
 {
     using Piece = Vec<T, V>;
     using Raw = typename Input<T, V, Packed>::Raw;
-    struct Rows {
-        Piece g[Run];
-        Raw v[Run];
-        float scale[Run];
-    };
+    const int tid = threadIdx.x;
     // One pointer per array, moved by a constant: the addresses were a third of the instructions.
     const int step = rows_per_pass * n.channels;
     const int scale_step = rows_per_pass * ((n.channels + kPackBlock - 1) / kPackBlock);
     const T* g = dy + at.base;
     const auto* v = static_cast<const typename Input<T, V, Packed>::Value*>(in.at(at.base));
     const float* scale = Packed ? in.scale_at(at.row, channel, n.channels) : nullptr;
-    const auto load = [&](Rows& r, int left) {
-#pragma unroll
-        for (int k = 0; k < Run; ++k) {
-            if (k < left) {
-                r.g[k] = *reinterpret_cast<const Piece*>(g);
-                r.v[k] = *reinterpret_cast<const Raw*>(v);
-                r.scale[k] = Packed ? *scale : 1.0f;
+    int left = at.mine;
+    const auto issue = [&](int slot) {
+        if (left > 0) {
+            copy_async<sizeof(Piece)>(&ring.g[slot][tid], g);
+            copy_async<sizeof(Raw)>(&ring.v[slot][tid], v);
+            if constexpr (Packed) {
+                copy_async<4>(&ring.scale[slot][tid], scale);
             }
-            g += step;
-            v += step;
-            scale += Packed ? scale_step : 0;
         }
+        --left;
+        g += step;
+        v += step;
+        scale += Packed ? scale_step : 0;
+        cp_async_commit();
     };
-    Rows now, next;
-    load(now, at.mine);
-    for (int left = at.mine; left > 0; left -= Run) {
-        load(next, left - Run);
 #pragma unroll
-        for (int k = 0; k < Run; ++k) {
-            if (k < left) {
-                f(widen(now.g[k]), Input<T, V, Packed>::values(now.v[k], now.scale[k]));
-            }
-        }
-        now = next;
+    for (int k = 0; k < kAhead; ++k) {
+        issue(k);
+    }
+    int slot = 0;
+    for (int i = 0; i < at.mine; ++i) {
+        cp_async_wait<kAhead - 1>();
+        const Piece dyv = ring.g[slot][tid];
+        const Raw raw = ring.v[slot][tid];
+        const float s = Packed ? ring.scale[slot][tid] : 1.0f;
+        issue(slot == 0 ? kAhead : slot - 1);  // the slot of the row before, which has been used
+        slot = slot == kAhead ? 0 : slot + 1;
+        f(widen(dyv), Input<T, V, Packed>::values(raw, s));
     }
 }
+
+// What the backward kernels need of a thread's channels: dz = dy act'(z) with z = d w rstd + b, d = x - mean.
+template <int V>
+struct Folded {
+    Floats<V> mean, scale, bias;
+
+    __device__ __forceinline__ explicit Folded(const Channels<V>& c) : mean(c.mean), bias(c.bias)
+    {
+#pragma unroll
+        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+            scale.p[j] = c.weight.p[j] * c.rstd.p[j];
+        }
+    }
+    template <int Act, class T>
+    __device__ __forceinline__ float2 slope(float2 x, float2 dy, int j, float2& d) const
+    {
+        d = x - mean.p[j];
+        float2 s;
+        activate_slope2<Act, T>(fma2(d, scale.p[j], bias.p[j]), s);
+        return dy * s;
+    }
+};
 
 // Backward, first pass: sum dz and sum dz xhat of a chunk per channel.
 template <class T, int V, bool Packed, int Act>
@@ -954,7 +987,11 @@ __global__ void __launch_bounds__(kThreads)
                              const float* __restrict__ rstd, float2* __restrict__ partial, NormShape n, Chunking s)
 {
     allow_next_grid();
-    __shared__ Sums<V> sums;
+    __shared__ union {
+        Ring<T, V, Packed> ring;
+        Sums<V> sums;
+    } shared;
+    Sums<V>& sums = shared.sums;
     const int tid = threadIdx.x;
     const int lane = tid & 31;
     const int warp = tid >> 5;
@@ -963,20 +1000,31 @@ __global__ void __launch_bounds__(kThreads)
     const int rows_per_pass = kThreads / s.lanes;
     const Place at = place_of(t, s, n, lane_c, tid / s.lanes);
     wait_for_previous_grid();
-    Channels<V> ch;
-    ch.load(mean, rstd, weight, bias, n, t.sample, t.c0 + lane_c, at.mine > 0);
     Floats<V> a, b;
     a.fill(0.0f);
     b.fill(0.0f);
-    for_gradient_rows<T, V, Packed, 2>(dy, in, at, t.c0 + lane_c, n, rows_per_pass, [&](const Floats<V>& g, const Floats<V>& x) {
+    {
+        Channels<V> all;
+        all.load(mean, rstd, weight, bias, n, t.sample, t.c0 + lane_c, at.mine > 0);
+        const Folded<V> ch(all);
+        for_gradient_rows<T, V, Packed>(shared.ring, dy, in, at, t.c0 + lane_c, n, rows_per_pass,
+                                        [&](const Floats<V>& g, const Floats<V>& x) {
 #pragma unroll
-        for (int j = 0; j < Floats<V>::kPairs; ++j) {
-            float2 xhat;
-            const float2 dz = ch.template slope<Act, T>(x.p[j], g.p[j], j, xhat);
-            a.p[j] = a.p[j] + dz;
-            b.p[j] = fma2(dz, xhat, b.p[j]);
+            for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                float2 d;
+                const float2 dz = ch.template slope<Act, T>(x.p[j], g.p[j], j, d);
+                a.p[j] = a.p[j] + dz;
+                b.p[j] = fma2(dz, d, b.p[j]);
+            }
+        });
+    }
+    if (at.mine > 0) {  // sum dz xhat = rstd sum dz (x - mean)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            b.set(j, b.at(j) * rstd[t.sample * n.groups + (t.c0 + lane_c + j) / n.per_group]);
         }
-    });
+    }
+    __syncthreads();  // the sums lie where the rows did
     for (int o = 16; o >= s.lanes; o >>= 1) {
 #pragma unroll
         for (int j = 0; j < Floats<V>::kPairs; ++j) {
@@ -1014,6 +1062,7 @@ __global__ void __launch_bounds__(kThreads)
                                T* __restrict__ dx, NormShape n, Chunking s)
 {
     allow_next_grid();
+    __shared__ Ring<T, V, Packed> ring;
     const int tid = threadIdx.x;
     const Task t = task_of(s, n, true);
     const int lane_c = (tid % s.lanes) * V;
@@ -1023,26 +1072,29 @@ __global__ void __launch_bounds__(kThreads)
     if (at.mine == 0) {
         return;
     }
-    Channels<V> ch;
-    ch.load(mean, rstd, weight, bias, n, t.sample, t.c0 + lane_c, true);
-    Floats<V> mt, mtx;
-    mt.fill(0.0f);
-    mtx.fill(0.0f);
+    Channels<V> all;
+    all.load(mean, rstd, weight, bias, n, t.sample, t.c0 + lane_c, true);
+    const Folded<V> ch(all);
+    // dx = rstd (w dz - mean(t) - xhat mean(t xhat)) = scale dz - c0 - d c1
+    Floats<V> c0, c1;
+    c0.fill(0.0f);
+    c1.fill(0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const float2 gm = group_means[t.sample * n.groups + (t.c0 + lane_c + j) / n.per_group];
-        mt.set(j, gm.x);
-        mtx.set(j, gm.y);
+        const float r = all.rstd.at(j);
+        c0.set(j, -r * gm.x);
+        c1.set(j, -r * (r * gm.y));
     }
     T* dst = dx + at.base;
     const long long step = static_cast<long long>(rows_per_pass) * n.channels;
-    for_gradient_rows<T, V, Packed, 2>(dy, in, at, t.c0 + lane_c, n, rows_per_pass, [&](const Floats<V>& g, const Floats<V>& x) {
+    for_gradient_rows<T, V, Packed>(ring, dy, in, at, t.c0 + lane_c, n, rows_per_pass, [&](const Floats<V>& g, const Floats<V>& x) {
         Floats<V> f;
 #pragma unroll
         for (int j = 0; j < Floats<V>::kPairs; ++j) {
-            float2 xhat;
-            const float2 dz = ch.template slope<Act, T>(x.p[j], g.p[j], j, xhat);
-            f.p[j] = ch.rstd.p[j] * (dz * ch.weight.p[j] - mt.p[j] - xhat * mtx.p[j]);
+            float2 d;
+            const float2 dz = ch.template slope<Act, T>(x.p[j], g.p[j], j, d);
+            f.p[j] = fma2(ch.scale.p[j], dz, fma2(d, c1.p[j], c0.p[j]));
         }
         *reinterpret_cast<Vec<T, V>*>(dst) = narrow<T>(f);
         dst += step;
