@@ -21,10 +21,11 @@
 // Two-pass form: chunks of a sample's rows give partial results (means and squares about them, joined
 // block by block, so that neither a large mean nor an outlier cancels), a small kernel joins them, and
 // the outputs are computed from a second read, which runs backwards to meet what is still in L2.
-// Same array with gelu: 85 us forward (402 MB in three passes: 4.7 TB/s; 74 us with no activation), 148 us
-// backward (671 MB: 4.5 TB/s; 134 us), from an 8-bit checkpoint 185 us (141 us); float32 135 us (6.0 TB/s) and
-// 223 us (6.0 TB/s). Cutting the batch so that a part's second read stays in L2 measured slower at every
-// cut (2 to 16 parts: 105 to 330 us forward, 180 to 470 us backward): each part pays its launches' ends.
+// Same array with gelu: 77 us forward (402 MB in three passes: 5.2 TB/s; 69 us with no activation), 136 us
+// backward (671 MB: 4.9 TB/s; 113 us), from an 8-bit checkpoint 165 us (103 us); float32 134 us (6.0 TB/s) and
+// 214 us (6.3 TB/s). What bounds the 16-bit types with gelu are its instructions, computed twice in the backward pass.
+// Cutting the batch so that a part's second read stays in L2 measured slower at every cut (2 to 16
+// parts: 105 to 330 us forward, 180 to 470 us backward): each part pays its launches' ends.
 // Keeping the second read in L2, with persistent CTAs that take sum and apply tasks a few samples
 // apart, measured 97 us and 207 us: a sample's statistics take some 10 us from its last sum to its
 // first output (fences, atomics, flags), and at this bandwidth 65 MB pass in that time.
@@ -708,35 +709,48 @@ __device__ __forceinline__ void to_shared(float* p, const Floats<V>& f)
     }
 }
 
-// Calls f(pieces, i) for the thread's passes i ..: Run rows at a time, the next Run loaded before they
-// are used, then row by row.
-template <class T, int V, int Run, class F>
-__device__ __forceinline__ void for_rows(const T* src, long long step, int mine, F&& f)
+// Rows of x on their way to a thread of the forward kernels: blocks of kRun rows, two in flight while one is
+// used. As in Ring, a thread reads only what it has copied.
+constexpr int kRun = 4;
+template <class T, int V>
+struct RowRing {
+    Vec<T, V> x[3 * kRun][kThreads];
+};
+
+// Calls f(pieces, i) for the thread's passes i ..: kRun rows at a time, then row by row.
+template <class T, int V, class F>
+__device__ __forceinline__ void for_rows(RowRing<T, V>& ring, const T* src, long long step, int mine, F&& f)
 {
     using Piece = Vec<T, V>;
-    const auto load = [&](Piece (&raw)[Run]) {
+    const int tid = threadIdx.x;
+    const int blocks = mine / kRun;
+    int ahead = 0;  // blocks issued
+    const auto issue = [&](int slot) {
+        if (ahead < blocks) {
 #pragma unroll
-        for (int k = 0; k < Run; ++k) {
-            raw[k] = *reinterpret_cast<const Piece*>(src + k * step);
-        }
-        src += Run * step;
-    };
-    int i = 0;
-    if (mine >= Run) {
-        Piece now[Run], next[Run];
-        load(now);
-        for (; i + 2 * Run <= mine; i += Run) {
-            load(next);
-            f(now, i);
-#pragma unroll
-            for (int k = 0; k < Run; ++k) {
-                now[k] = next[k];
+            for (int k = 0; k < kRun; ++k) {
+                copy_async<sizeof(Piece)>(&ring.x[slot * kRun + k][tid], src);
+                src += step;
             }
+            ++ahead;
         }
-        f(now, i);
-        i += Run;
+        cp_async_commit();
+    };
+    issue(0);
+    issue(1);
+    int slot = 0;
+    for (int b = 0; b < blocks; ++b) {
+        cp_async_wait<1>();
+        Piece raw[kRun];
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            raw[k] = ring.x[slot * kRun + k][tid];
+        }
+        issue(slot == 0 ? 2 : slot - 1);  // the slot of the block before, which has been used
+        slot = slot == 2 ? 0 : slot + 1;
+        f(raw, b * kRun);
     }
-    for (; i < mine; ++i) {
+    for (int i = blocks * kRun; i < mine; ++i) {
         const Piece raw[1] = {*reinterpret_cast<const Piece*>(src)};
         f(raw, i);
         src += step;
@@ -752,7 +766,11 @@ __global__ void __launch_bounds__(kThreads)
 {
     using Piece = Vec<T, V>;
     allow_next_grid();
-    __shared__ Sums<V> sums;
+    __shared__ union {
+        RowRing<T, V> ring;
+        Sums<V> sums;
+    } shared;
+    Sums<V>& sums = shared.sums;
     const int tid = threadIdx.x;
     const int lane = tid & 31;
     const int warp = tid >> 5;
@@ -766,7 +784,7 @@ __global__ void __launch_bounds__(kThreads)
     Floats<V> m, q;
     m.fill(0.0f);
     q.fill(0.0f);
-    for_rows<T, V, (V >= 8 ? 4 : 8)>(x + at.base, step, at.mine, [&](const auto& raw, int i) {
+    for_rows<T, V>(shared.ring, x + at.base, step, at.mine, [&](const auto& raw, int i) {
         constexpr int K = sizeof(raw) / sizeof(Piece);
         Floats<V> f[K];
 #pragma unroll
@@ -788,6 +806,7 @@ __global__ void __launch_bounds__(kThreads)
     });
     // The warp's rows of each channel joined about one of them: means and squares are then plain
     // sums (a reference this close costs at most a bit or two).
+    __syncthreads();  // the sums lie where the rows did
     float count = static_cast<float>(at.mine);
     if (s.lanes < 32) {
         float total = count;
@@ -869,6 +888,7 @@ __global__ void __launch_bounds__(kThreads)
 {
     using Piece = Vec<T, V>;
     allow_next_grid();
+    __shared__ RowRing<T, V> ring;
     const int tid = threadIdx.x;
     const Task t = task_of(s, n, true);
     const int lane_c = (tid % s.lanes) * V;
@@ -886,7 +906,7 @@ __global__ void __launch_bounds__(kThreads)
         ch.weight.p[j] = ch.weight.p[j] * ch.rstd.p[j];
     }
     T* dst = y + at.base;
-    for_rows<T, V, 4>(x + at.base, step, at.mine, [&](const auto& raw, int) {
+    for_rows<T, V>(ring, x + at.base, step, at.mine, [&](const auto& raw, int) {
         constexpr int K = sizeof(raw) / sizeof(Piece);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -1114,6 +1134,7 @@ __global__ void __launch_bounds__(kThreads)
 {
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     allow_next_grid();
+    __shared__ RowRing<T, V> ring;
     const int lane = threadIdx.x & 31;
     const int c = static_cast<int>(blockIdx.x % static_cast<unsigned>(s.tiles)) * kWarps + static_cast<int>(threadIdx.x >> 5);
     const long long i = blockIdx.x / static_cast<unsigned>(s.tiles);
@@ -1128,7 +1149,7 @@ __global__ void __launch_bounds__(kThreads)
     Floats<V> m, q;
     m.fill(0.0f);
     q.fill(0.0f);
-    for_rows<T, V, (V >= 8 ? 4 : 8)>(x + (sample * n.channels + c) * n.points + chunk * s.rows + lane * V, 32 * V, mine,
+    for_rows<T, V>(ring, x + (sample * n.channels + c) * n.points + chunk * s.rows + lane * V, 32 * V, mine,
                                      [&](const auto& raw, int k0) {
                                          constexpr int K = sizeof(raw) / sizeof(Vec<T, V>);
                                          Floats<V> f[K];
@@ -1244,20 +1265,22 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// dbias[c] and dweight[c]: the samples' sums added up. Eight row lanes per channel, joined in
-// a fixed order.
-__global__ void __launch_bounds__(kThreads)
+// dbias[c] and dweight[c]: the samples' sums added up. 32 row lanes per channel, joined in a fixed order
+// (4096 samples: eight took 150 us of a backward pass).
+constexpr int kSumLanes = 32;
+__global__ void __launch_bounds__(32 * kSumLanes)
     norm_parameter_kernel(const float* __restrict__ sample_sums, float* __restrict__ dweight, float* __restrict__ dbias,
                           long long batch, int channels)
 {
-    __shared__ float sb[8][33], sw[8][33];
+    __shared__ float sb[kSumLanes][33], sw[kSumLanes][33];
     allow_next_grid();
     wait_for_previous_grid();
     const int c = static_cast<int>(blockIdx.x) * 32 + static_cast<int>(threadIdx.x & 31);
     const int part = static_cast<int>(threadIdx.x >> 5);
     float b = 0.0f, w = 0.0f;
     if (c < channels) {
-        for (long long k = part; k < batch; k += 8) {
+#pragma unroll 4
+        for (long long k = part; k < batch; k += kSumLanes) {
             b += sample_sums[k * channels + c];
             w += sample_sums[(batch + k) * channels + c];
         }
@@ -1266,7 +1289,7 @@ __global__ void __launch_bounds__(kThreads)
     sw[part][threadIdx.x & 31] = w;
     __syncthreads();
     if (part == 0 && c < channels) {
-        for (int k = 1; k < 8; ++k) {
+        for (int k = 1; k < kSumLanes; ++k) {
             b += sb[k][threadIdx.x & 31];
             w += sw[k][threadIdx.x & 31];
         }
@@ -1562,7 +1585,7 @@ void norm_backward_typed(const T* dy, const Input<T, V, Packed>& in, const float
                    weight, bias, mean, rstd, static_cast<const float2*>(group_means), dx, n, st);
     }
     if (dweight != nullptr || dbias != nullptr) {
-        launch_pdl(norm_parameter_kernel, dim3(static_cast<unsigned>((n.channels + 31) / 32)), dim3(kThreads), 0, stream,
+        launch_pdl(norm_parameter_kernel, dim3(static_cast<unsigned>((n.channels + 31) / 32)), dim3(32 * kSumLanes), 0, stream,
                    static_cast<const float*>(sample_sums), dweight, dbias, n.batch, n.channels);
     }
 }
