@@ -68,9 +68,15 @@ struct StageJobs {
     int count = 0;
 };
 
+// A warp copies 256 values at a time, some whole rows or a part of one: single values loaded in a row,
+// through shared memory, eight stored at once. (Eight loads side by side per thread took 262 us for 47519 x 895
+// bf16.)
+constexpr int kStageValues = 256;
+
 template <class T>
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ StageJobs jobs)
 {
+    __shared__ float rows_of[8][kStageValues];
     const StageJob& job = jobs.job[blockIdx.y];
     const T* __restrict__ src = static_cast<const T*>(job.src);
     auto* __restrict__ dst = static_cast<typename Operand<T>::Type*>(job.dst);
@@ -79,34 +85,55 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ Stag
     const int pitch = job.pitch;
     allow_next_grid();
     wait_for_previous_grid();
-    const int pieces = pitch / 8;
-    const long long total = rows * pieces;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
-         i += static_cast<long long>(gridDim.x) * 256) {
-        const long long row = i / pieces;
-        const int c0 = static_cast<int>(i - row * pieces) * 8;
-        float v[8];
+    const int lane = threadIdx.x & 31;
+    float* buf = rows_of[threadIdx.x >> 5];
+    const int at_once = pitch <= kStageValues ? kStageValues / pitch : 1;  // rows
+    const int parts = (pitch + kStageValues - 1) / kStageValues;           // of a row
+    const long long total = (rows + at_once - 1) / at_once * parts;
+    // This lane's eight values, among the rows at once or in the part.
+    const int r = parts == 1 ? lane * 8 / pitch : 0;
+    const int c = lane * 8 - r * pitch;
+    for (long long i = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total;
+         i += static_cast<long long>(gridDim.x) * 8) {
+        const long long first = i / parts;
+        const long long row0 = first * at_once;
+        const int c0 = static_cast<int>(i - first * parts) * kStageValues;
+        const int have = parts == 1 ? static_cast<int>(min(static_cast<long long>(at_once), rows - row0)) * cols
+                                    : min(kStageValues, cols - c0);
+        const T* from = src + row0 * cols + c0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = c0 + j < cols ? to_float(src[row * cols + c0 + j]) : 0.0f;
+        for (int j = 0; j < kStageValues / 32; ++j) {
+            const int e = 32 * j + lane;
+            buf[e] = e < have ? to_float(from[e]) : 0.0f;
         }
-        if constexpr (sizeof(T) == 4) {
-            Vec<bf16, 8> hi, mid, lo;
+        __syncwarp();
+        const long long row = row0 + r;
+        if (r < at_once && row < rows && c0 + c < pitch) {
+            float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                split3(v[j], hi.v[j], mid.v[j], lo.v[j]);
+                v[j] = c0 + c + j < cols ? buf[r * cols + c + j] : 0.0f;
             }
-            *reinterpret_cast<Vec<bf16, 8>*>(dst + row * pitch + c0) = hi;
-            *reinterpret_cast<Vec<bf16, 8>*>(dst + (rows + row) * pitch + c0) = mid;
-            *reinterpret_cast<Vec<bf16, 8>*>(dst + (2 * rows + row) * pitch + c0) = lo;
-        } else {
-            Vec<T, 8> out;
+            const long long at = row * pitch + c0 + c;
+            if constexpr (sizeof(T) == 4) {
+                Vec<bf16, 8> hi, mid, lo;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                out.v[j] = from_float<T>(v[j]);
+                for (int j = 0; j < 8; ++j) {
+                    split3(v[j], hi.v[j], mid.v[j], lo.v[j]);
+                }
+                *reinterpret_cast<Vec<bf16, 8>*>(dst + at) = hi;
+                *reinterpret_cast<Vec<bf16, 8>*>(dst + rows * pitch + at) = mid;
+                *reinterpret_cast<Vec<bf16, 8>*>(dst + 2 * rows * pitch + at) = lo;
+            } else {
+                Vec<T, 8> out;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    out.v[j] = from_float<T>(v[j]);
+                }
+                *reinterpret_cast<Vec<T, 8>*>(dst + at) = out;
             }
-            *reinterpret_cast<Vec<T, 8>*>(dst + row * pitch + c0) = out;
         }
+        __syncwarp();
     }
 }
 
@@ -251,7 +278,50 @@ __device__ __forceinline__ Tile locate(const Args& g, long long t)
     return tile;
 }
 
-// The epilogue of N columns of one row, from col on: acc holds each accumulator's values.
+// A warp's 32 x 32 values, lane l holding row l, to rows whose stores would not be whole sectors: transposed by
+// shuffles, so that a store is 32 values side by side (47519 x 895 bf16 results of 8 hidden values: single
+// values of 32 rows at a time took 440 us).
+template <class T>
+__device__ __forceinline__ void store_across(T* p, long long pitch, float (&v)[32], long long rows, int cols)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        const bool upper = (lane & s) != 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if ((j & s) == 0) {
+                const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j | s], s);
+                v[j] = upper ? other : v[j];
+                v[j | s] = upper ? v[j | s] : other;
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        if (j < rows && lane < cols) {
+            p[j * pitch + lane] = from_float<T>(v[j]);
+        }
+    }
+}
+
+// Results of one accumulator: the warp's 32 rows from row - lane on, 32 columns from col on.
+template <Kind K, class T>
+__device__ __forceinline__ void store_results(const Args& g, const Tile& tile, int row, int rows, int col, int cols, float (&acc)[32])
+{
+    using Out = std::conditional_t<K == Kind::kWeight, float, T>;
+    const int lane = threadIdx.x & 31;
+    const long long pitch = K == Kind::kWeight ? cols : g.pitch;
+    Out* out = static_cast<Out*>(g.out[0]) + (K == Kind::kWeight ? tile.part * g.part_size + g.offset[tile.problem] : 0)
+               + static_cast<long long>(row - lane) * pitch + col;
+    if (((reinterpret_cast<std::uintptr_t>(out) | static_cast<std::uintptr_t>(pitch * sizeof(Out))) & 31u) != 0) {
+        store_across(out, pitch, acc, rows - (row - lane), cols - col);
+    } else if (row < rows) {
+        store_values<Out>(out + lane * pitch, acc, min(32, cols - col));
+    }
+}
+
+// The epilogue of the gate kernels, N columns of one row from col on: acc holds each accumulator's values.
 template <Kind K, class T, int Act, int Sets, int N>
 __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row, int col, int cols, float (&acc)[Sets][N])
 {
@@ -284,11 +354,6 @@ __device__ __forceinline__ void finish(const Args& g, const Tile& tile, int row,
         store_hidden<T>(static_cast<Op*>(g.out[0]) + at, g.plane, acc[0], valid);
         store_hidden<T>(static_cast<Op*>(g.out[1]) + at, g.plane, acc[2], valid);
         store_hidden<T>(static_cast<Op*>(g.out[2]) + at, g.plane, acc[1], valid);
-    } else if constexpr (K == Kind::kWeight) {
-        float* out = static_cast<float*>(g.out[0]) + tile.part * g.part_size + g.offset[tile.problem];
-        store_values<float>(out + static_cast<long long>(row) * cols + col, acc[0], valid);
-    } else {
-        store_values<T>(static_cast<T*>(g.out[0]) + at, acc[0], valid);
     }
 }
 
@@ -568,7 +633,12 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
 #pragma unroll
                 for (int r = 0; r < kRuns; ++r) {
                     const int col = tile.n0 + first + 32 * r;
-                    if (ok && row < rows && col < cols) {
+                    if (!ok || col >= cols) {
+                        continue;
+                    }
+                    if constexpr (Cfg::kSets == 1) {
+                        store_results<K, T>(g, tile, row, rows, col, cols, acc[r][0]);
+                    } else if (row < rows) {
                         finish<K, T, Act>(g, tile, row, col, cols, acc[r]);
                     }
                 }
@@ -593,7 +663,9 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
                         for (int q = 0; q < Cfg::kSets; ++q) {
                             umma::load_wait(acc[q]);
                         }
-                        if (row + m * kTileM < rows) {
+                        if constexpr (Cfg::kSets == 1) {
+                            store_results<K, T>(g, tile, row + m * kTileM, rows, tile.n0 + c, cols, acc[0]);
+                        } else if (row + m * kTileM < rows) {
                             finish<K, T, Act>(g, tile, row + m * kTileM, tile.n0 + c, cols, acc);
                         }
                         __syncwarp();
