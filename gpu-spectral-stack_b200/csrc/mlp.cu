@@ -278,33 +278,6 @@ __device__ __forceinline__ Tile locate(const Args& g, long long t)
     return tile;
 }
 
-// A warp's 32 x 32 values, lane l holding row l, to rows whose stores would not be whole sectors: transposed by
-// shuffles, so that a store is 32 values side by side (47519 x 895 bf16 results of 8 hidden values: single
-// values of 32 rows at a time took 440 us).
-template <class T>
-__device__ __forceinline__ void store_across(T* p, long long pitch, float (&v)[32], long long rows, int cols)
-{
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-        const bool upper = (lane & s) != 0;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            if ((j & s) == 0) {
-                const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j | s], s);
-                v[j] = upper ? other : v[j];
-                v[j | s] = upper ? v[j | s] : other;
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        if (j < rows && lane < cols) {
-            p[j * pitch + lane] = from_float<T>(v[j]);
-        }
-    }
-}
-
 // Results of one accumulator: the warp's 32 rows from row - lane on, 32 columns from col on.
 template <Kind K, class T>
 __device__ __forceinline__ void store_results(const Args& g, const Tile& tile, int row, int rows, int col, int cols, float (&acc)[32])
@@ -312,13 +285,9 @@ __device__ __forceinline__ void store_results(const Args& g, const Tile& tile, i
     using Out = std::conditional_t<K == Kind::kWeight, float, T>;
     const int lane = threadIdx.x & 31;
     const long long pitch = K == Kind::kWeight ? cols : g.pitch;
-    Out* out = static_cast<Out*>(g.out[0]) + (K == Kind::kWeight ? tile.part * g.part_size + g.offset[tile.problem] : 0)
-               + static_cast<long long>(row - lane) * pitch + col;
-    if (((reinterpret_cast<std::uintptr_t>(out) | static_cast<std::uintptr_t>(pitch * sizeof(Out))) & 31u) != 0) {
-        store_across(out, pitch, acc, rows - (row - lane), cols - col);
-    } else if (row < rows) {
-        store_values<Out>(out + lane * pitch, acc, min(32, cols - col));
-    }
+    Out* out = static_cast<Out*>(g.out[0]) + (K == Kind::kWeight ? tile.part * g.part_size + g.offset[tile.problem] : 0);
+    const int first = row - lane;
+    store_rows(out + static_cast<long long>(first) * pitch + col, pitch, acc, rows - first, cols - col);
 }
 
 // The epilogue of the gate kernels, N columns of one row from col on: acc holds each accumulator's values.

@@ -324,9 +324,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
                 const int col = 64 * d + 32 * half;
                 umma::load32(tmem_y + lanes + group * F::kYCols + col, v);
                 umma::load_wait(v);
-                if (token < g.tokens && col < g.outputs) {
-                    store_values<T>(static_cast<T*>(g.out) + token * g.outputs + col, v, min(32, g.outputs - col));
-                }
+                store_rows(static_cast<T*>(g.out) + (token - lane) * g.outputs + col, g.outputs, v, g.tokens - (token - lane),
+                           g.outputs - col);
             }
             warp_arrive(&y_empty[group], false);
         };
@@ -610,9 +609,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
             dx.next();
             const long long token = static_cast<long long>(t) * kTileM + row;
             const int col = 16 * part;
-            if (token < g.tokens && col < g.channels) {
-                store_values<T>(static_cast<T*>(g.out) + token * g.channels + col, v, min(16, g.channels - col));
-            }
+            store_rows(static_cast<T*>(g.out) + (token - lane) * g.channels + col, g.channels, v, g.tokens - (token - lane),
+                       g.channels - col);
         };
         int before = -1;
         for (int k = 0; ok && k < mine; ++k) {
