@@ -57,6 +57,7 @@ constexpr int kCtaBytes = 200 * 1024;    // the most of a unit one CTA holds
 constexpr int kGoodBytes = 64 * 1024;    // of a CTA's part: three share an SM
 constexpr int kChunkBytes = 128 * 1024;  // two-pass form: of a CTA's chunk (64 KiB measured 5 % slower)
 constexpr long long kResidentBytes = 8LL << 20;  // the resident form's largest array
+constexpr long long kSmallSample = 32 * 1024;    // and the largest samples of larger arrays
 
 // What the kernels need of one call. x holds values of T, or codes8 / scales their checkpoint.
 struct NormShape {
@@ -1310,8 +1311,9 @@ __global__ void __launch_bounds__(32 * kSumLanes)
 //
 // The rule, from both forms measured over 16 KB to 270 MB (forward, silu and gelu): arrays up to 8 MiB are
 // resident if a unit fits a cluster (one launch instead of three: 12 against 17 us at 2 MB, 15 against
-// 17 us at 8 MB, where 17 MB are 31 against 19 us), and larger ones only where a unit fits one CTA, whose
-// barriers cost little.
+// 17 us at 8 MB, where 17 MB are 31 against 19 us), and larger ones only where the
+// samples are small (4096 x 64 x 64 bf16: 65 against 121 us, backward 152 against 220 us; 2048 x 256 x 64, at
+// the limit: 78 and 81 us, 163 and 162 us; 64 x 1000 x 512: 59 against 51 us, backward 113 against 86 us).
 bool slice(const NormShape& n, int vec, int elem, int held, int arrays, int group_arrays, Slicing& s)
 {
     s.width = 0;
@@ -1342,7 +1344,8 @@ bool slice(const NormShape& n, int vec, int elem, int held, int arrays, int grou
         const bool small = bytes <= kGoodBytes || (s.cluster >= 8 && s.smem <= kCtaBytes);
         const bool spread = units * s.cluster >= 2 * 148 || s.passes <= 4;
         if ((small && spread) || (s.cluster == kMaxCluster && s.smem <= kCtaBytes)) {
-            const bool worth = s.cluster == 1 || n.batch * n.points * n.channels * elem <= kResidentBytes;
+            const long long sample = n.points * n.channels * elem;
+            const bool worth = (s.cluster == 1 && sample <= kSmallSample) || n.batch * sample <= kResidentBytes;
             return worth && units * s.cluster <= 0x7fffffffLL;
         }
     }
