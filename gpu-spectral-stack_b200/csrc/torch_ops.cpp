@@ -901,11 +901,47 @@ gated_mlp_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Gradients of gradients are not computed: asking for them is an error, not a silent zero.
+// Gradients of gradients are not computed: asking for them is an error, not a silent zero. In a backward pass
+// with create_graph, the results depend on the forward pass's inputs and on the upstream gradient; they get
+// this node as their history, whose edges lead to all of those, so that differentiating them raises
+// wherever the answer would need it, and using their values alone does not.
+struct NotDifferentiable : torch::autograd::Node {
+    explicit NotDifferentiable(std::string name) : op(std::move(name)) {}
+    variable_list apply(variable_list&&) override { TORCH_CHECK(false, op, ": the backward pass is not differentiable itself"); }
+    std::string op;
+};
+
+// An upstream gradient that is a leaf can only ask for gradients of gradients: refused at once.
 void check_once(const variable_list& grads, const char* op)
 {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].defined() && grads[0].requires_grad()), op,
+    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].defined() && grads[0].requires_grad() && !grads[0].grad_fn()), op,
                 ": the backward pass is not differentiable itself");
+}
+
+// The end of a backward pass: `results` with the history above if there is to be one. `create_graph` is grad mode
+// as the pass was entered.
+variable_list finish_once(bool create_graph, const char* op, const variable_list& grads, variable_list results)
+{
+    if (!create_graph) {
+        return results;
+    }
+    torch::autograd::edge_list edges;
+    for (const torch::autograd::Edge& e : torch::autograd::get_current_node()->next_edges()) {
+        if (e.is_valid()) {
+            edges.push_back(e);
+        }
+    }
+    if (grads[0].defined() && grads[0].requires_grad()) {
+        edges.push_back(torch::autograd::impl::gradient_edge(grads[0]));
+    }
+    const auto node = std::make_shared<NotDifferentiable>(op);
+    node->set_next_edges(std::move(edges));
+    for (at::Tensor& t : results) {
+        if (t.defined()) {
+            torch::autograd::impl::set_gradient_edge(t, {node, node->add_input_metadata(t)});
+        }
+    }
+    return results;
 }
 
 bool wants_grad(std::initializer_list<const at::Tensor*> tensors)
@@ -942,6 +978,8 @@ struct GroupNormActFunction : torch::autograd::Function<GroupNormActFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         check_once(grads, "group_norm_act");
+        const bool create_graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
         const variable_list kept = ctx->get_saved_variables();
         const bool packed = kept.size() == 5;
         const std::string activation = ctx->saved_data["activation"].toStringRef();
@@ -952,7 +990,8 @@ struct GroupNormActFunction : torch::autograd::Function<GroupNormActFunction> {
             packed ? optional_of(kept[4]) : c10::nullopt, optional_of(kept[0]), optional_of(kept[1]), mean,
             mean == nullptr ? nullptr : mean + stats.numel() / 2, ctx->saved_data["groups"].toInt(), activation);
         const at::Tensor none;
-        return {dx, kept[0].defined() ? dweight : none, kept[1].defined() ? dbias : none, none, none, none, none};
+        return finish_once(create_graph, "group_norm_act", grads,
+                           {dx, kept[0].defined() ? dweight : none, kept[1].defined() ? dbias : none, none, none, none, none});
     }
 };
 
@@ -997,13 +1036,15 @@ struct GatedMlpFunction : torch::autograd::Function<GatedMlpFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         check_once(grads, "gated_mlp");
+        const bool create_graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
         const variable_list kept = ctx->get_saved_variables();
         const bool packed = kept.size() == 5;
         const std::string activation = ctx->saved_data["activation"].toStringRef();
         auto [dx, dwg, dwu, dwd] = gated_mlp_backward_cuda(
             grads[0], packed ? c10::nullopt : optional_of(kept[3]), packed ? optional_of(kept[3]) : c10::nullopt,
             packed ? optional_of(kept[4]) : c10::nullopt, kept[0], kept[1], kept[2], activation);
-        return {dx, dwg, dwu, dwd, at::Tensor(), at::Tensor()};
+        return finish_once(create_graph, "gated_mlp", grads, {dx, dwg, dwu, dwd, at::Tensor(), at::Tensor()});
     }
 };
 

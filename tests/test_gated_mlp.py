@@ -391,3 +391,30 @@ def test_float32_products_stay_at_float32_error(tokens, channels, hidden):
     grads = torch.autograd.grad(y, leaves, dy)
     for got, exact in zip((y, *grads), (want, *torch.autograd.grad(want, wide, dy.double()))):
         assert float((got.detach().double() - exact.detach()).norm()) <= 12 * 2.0 ** -24 * float(exact.detach().norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_gradients_of_gradients_under_a_constant_upstream_gradient_are_refused(checkpoint8):
+    *args, _ = inputs(20, 16, 24, 16, torch.float32)
+    leaves = [a.requires_grad_(True) for a in args]
+
+    def layer(x):
+        return gated_mlp(x, *leaves[1:], checkpoint8=checkpoint8)
+
+    y = layer(leaves[0])
+    plain = torch.autograd.grad(y.sum(), leaves, retain_graph=True)
+    grads = torch.autograd.grad(y.sum(), leaves, create_graph=True)
+    for g, p in zip(grads, plain):  # the values are there, without a way back through them
+        assert torch.equal(g, p)
+        for wrt in leaves:
+            with pytest.raises(RuntimeError, match="not differentiable itself"):
+                torch.autograd.grad(y.mean() + g.pow(2).sum(), wrt, retain_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable itself"):
+        (y.mean() + grads[0].pow(2).sum()).backward()
+    # Through two layers, and with an upstream gradient that depends on another tensor.
+    scale = torch.ones((), device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad((layer(layer(leaves[0])) * scale).sum(), leaves[0], create_graph=True)
+    for wrt in (leaves[0], leaves[3], scale):
+        with pytest.raises(RuntimeError, match="not differentiable itself"):
+            torch.autograd.grad(g.sum(), wrt, retain_graph=True)

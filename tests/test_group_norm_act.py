@@ -390,3 +390,30 @@ def test_the_c_abi_refuses_to_lay_channels_last(change, message):
     a.update(change)
     with pytest.raises(ValueError, match=message):
         native.call("spectral_channels_last", *a.values())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_gradients_of_gradients_under_a_constant_upstream_gradient_are_refused(checkpoint8):
+    x, weight, bias, _ = inputs((2, 9, 16), torch.float32, 5)
+    leaves = [t.requires_grad_(True) for t in (x, weight, bias)]
+
+    def layer():
+        return group_norm_act(leaves[0], 2, leaves[1], leaves[2], activation="gelu", checkpoint8=checkpoint8)
+
+    y = layer()
+    plain = torch.autograd.grad(y.sum(), leaves, retain_graph=True)
+    grads = torch.autograd.grad(y.sum(), leaves, create_graph=True)
+    for g, p in zip(grads, plain):  # the values are there, without a way back through them
+        assert torch.equal(g, p)
+        for wrt in leaves:
+            with pytest.raises(RuntimeError, match="not differentiable itself"):
+                torch.autograd.grad(y.mean() + g.pow(2).sum(), wrt, retain_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable itself"):
+        (layer().mean() + grads[0].pow(2).sum()).backward()
+    # Through two layers, and with an upstream gradient that depends on another tensor.
+    scale = torch.ones((), device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad((group_norm_act(layer(), 4) * scale).sum(), leaves[0], create_graph=True)
+    for wrt in (leaves[0], scale):
+        with pytest.raises(RuntimeError, match="not differentiable itself"):
+            torch.autograd.grad(g.sum(), wrt, retain_graph=True)
