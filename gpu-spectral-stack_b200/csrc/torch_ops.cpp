@@ -957,6 +957,16 @@ bool wants_grad(std::initializer_list<const at::Tensor*> tensors)
     return false;
 }
 
+// Nor are forward-mode derivatives: a result without its tangent would be a silent zero too. (These do not depend
+// on requires_grad or on grad mode.)
+void check_no_tangent(const char* op, std::initializer_list<const at::Tensor*> tensors)
+{
+    for (const at::Tensor* t : tensors) {
+        TORCH_CHECK(!(t->defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined()), op,
+                    ": forward-mode derivatives are not computed");
+    }
+}
+
 c10::optional<at::Tensor> optional_of(const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
 
 struct GroupNormActFunction : torch::autograd::Function<GroupNormActFunction> {
@@ -1007,6 +1017,7 @@ at::Tensor group_norm_act_layer_autograd(const at::Tensor& x, int64_t groups, co
 {
     const at::Tensor w = weight.value_or(at::Tensor());
     const at::Tensor b = bias.value_or(at::Tensor());
+    check_no_tangent("group_norm_act", {&x, &w, &b});
     if (wants_grad({&x, &w, &b})) {
         return GroupNormActFunction::apply(x, weight, bias, groups, eps, std::string(activation.data(), activation.size()), checkpoint8);
     }
@@ -1057,6 +1068,7 @@ at::Tensor gated_mlp_layer_cuda(const at::Tensor& x, const at::Tensor& w_gate, c
 at::Tensor gated_mlp_layer_autograd(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up,
                                     const at::Tensor& w_down, c10::string_view activation, bool checkpoint8)
 {
+    check_no_tangent("gated_mlp", {&x, &w_gate, &w_up, &w_down});
     if (wants_grad({&x, &w_gate, &w_up, &w_down})) {
         return GatedMlpFunction::apply(x, w_gate, w_up, w_down, std::string(activation.data(), activation.size()), checkpoint8);
     }

@@ -417,3 +417,14 @@ def test_gradients_of_gradients_under_a_constant_upstream_gradient_are_refused(c
     for wrt in (leaves[0], scale):
         with pytest.raises(RuntimeError, match="not differentiable itself"):
             torch.autograd.grad(g.sum(), wrt, retain_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_tangents_are_refused(which, grad_mode):
+    args = list(inputs((2, 9, 16), torch.float32, 5)[:3])
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            group_norm_act(args[0], 2, args[1], args[2], activation="gelu")
