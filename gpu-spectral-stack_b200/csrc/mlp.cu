@@ -853,24 +853,29 @@ int tiles_of(long long v, int tile) { return static_cast<int>((v + tile - 1) / t
 int hidden_pitch(const MlpShape& n) { return round_up(n.hidden, 16); }  // 32-byte rows for the epilogue's stores
 int planes_of(int dtype) { return dtype == SPECTRAL_FLOAT32 ? 3 : 1; }
 
-// A workspace handed out piece by piece, each 256-byte aligned; with a null base it only counts.
+// A workspace handed out piece by piece, each 256-byte aligned. A call lays its pieces out in the same steps
+// in which the workspace queries counted them (then at an address that nothing reads or writes).
 struct Arena {
-    unsigned char* base;
+    std::uintptr_t base = 256;
     std::size_t used = 0;
 
+    Arena() = default;
+    explicit Arena(void* work) : base((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255}) {}
     void* take(std::size_t bytes)
     {
-        void* p = base != nullptr ? base + used : nullptr;
+        void* p = reinterpret_cast<void*>(base + used);
         used += (bytes + 255) / 256 * 256;
         return p;
     }
+    std::size_t total() const { return used + 256; }  // whatever the workspace's own alignment
 };
 
-// TMA reads the array as it lies: 16-bit values in 16-byte aligned rows.
+// TMA reads the array as it lies: 16-bit values in 16-byte aligned rows. (A workspace query that does not know
+// the array passes nullptr.)
 template <class T>
 bool direct(const void* p, int cols)
 {
-    return sizeof(T) == 2 && cols % 8 == 0 && aligned_to(p, 16);
+    return sizeof(T) == 2 && cols % 8 == 0 && p != nullptr && aligned_to(p, 16);
 }
 
 template <class T>
@@ -987,45 +992,62 @@ void mlp_few(const T* x, const T* wg, const T* wu, const T* wd, T* y, const MlpS
     }
 }
 
+// The arrays a call gives.
+struct Arrays {
+    const void* dy = nullptr;  // backward
+    const void* x = nullptr;
+    const void* wg = nullptr;
+    const void* wu = nullptr;
+    const void* wd = nullptr;
+};
+
+// A forward call's workspace: the few-token form's hidden values, or the operands TMA does not read in place and,
+// unless they stay on chip, the hidden values.
 template <class T>
-std::size_t forward_bytes(const MlpShape& n)
-{
-    Arena arena{nullptr};
-    arena.take(staged_bytes<T>(n.tokens, n.channels));
-    arena.take(staged_bytes<T>(n.hidden, n.channels));
-    arena.take(staged_bytes<T>(n.hidden, n.channels));
-    arena.take(staged_bytes<T>(n.outputs, n.hidden));
-    hidden_matrix<T>(n, arena);
-    arena.take(sizeof(float) * kFewAtOnce * static_cast<std::size_t>(n.hidden));
-    return arena.used + 256;
-}
+struct ForwardLayout {
+    bool few = false, narrow = false;
+    float* few_hidden = nullptr;
+    StageJobs jobs;
+    Matrix x, wg, wu, wd, h;
+
+    ForwardLayout(Arena& arena, const Arrays& in, int dtype, const MlpShape& n)
+        : few(n.tokens <= kFewTokens<T>), narrow(narrow_forward_fits(n, dtype))
+    {
+        if (few) {
+            few_hidden = static_cast<float*>(arena.take(sizeof(float) * kFewAtOnce * static_cast<std::size_t>(n.hidden)));
+            return;
+        }
+        x = operand<T>(in.x, n.tokens, n.channels, arena, jobs);
+        wg = operand<T>(in.wg, n.hidden, n.channels, arena, jobs);
+        wu = operand<T>(in.wu, n.hidden, n.channels, arena, jobs);
+        wd = operand<T>(in.wd, n.outputs, n.hidden, arena, jobs);
+        if (!narrow) {
+            h = hidden_matrix<T>(n, arena);
+        }
+    }
+};
 
 template <class T>
-void mlp_forward(const void* x, const void* wg, const void* wu, const void* wd, void* y, int dtype, const MlpShape& n,
-                 void* work, cudaStream_t stream)
+void mlp_forward(const Arrays& in, void* y, int dtype, const MlpShape& n, void* work, cudaStream_t stream)
 {
-    Arena arena{reinterpret_cast<unsigned char*>((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255})};
-    if (n.tokens <= kFewTokens<T>) {
-        float* h = static_cast<float*>(arena.take(sizeof(float) * kFewAtOnce * static_cast<std::size_t>(n.hidden)));
+    Arena arena(work);
+    const ForwardLayout<T> lay(arena, in, dtype, n);
+    if (lay.few) {
         with_activation(n.act, [&](auto act) {
-            mlp_few<T, decltype(act)::value>(static_cast<const T*>(x), static_cast<const T*>(wg), static_cast<const T*>(wu),
-                                             static_cast<const T*>(wd), static_cast<T*>(y), n, h, stream);
+            mlp_few<T, decltype(act)::value>(static_cast<const T*>(in.x), static_cast<const T*>(in.wg),
+                                             static_cast<const T*>(in.wu), static_cast<const T*>(in.wd), static_cast<T*>(y), n,
+                                             lay.few_hidden, stream);
         });
         return;
     }
-    StageJobs jobs;
-    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, jobs);
-    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, jobs);
-    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, jobs);
-    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, jobs);
-    run_jobs<T>(jobs, stream);
+    const Matrix &mx = lay.x, &mg = lay.wg, &mu = lay.wu, &md = lay.wd, &mh = lay.h;
+    run_jobs<T>(lay.jobs, stream);
     if constexpr (sizeof(T) == 2) {
-        if (narrow_forward_fits(n, dtype)) {
+        if (lay.narrow) {
             narrow_forward(mx, mg, mu, md, y, dtype, n, stream);
             return;
         }
     }
-    const Matrix mh = hidden_matrix<T>(n, arena);
     const auto gate = [&](auto width) {
         constexpr int BN = decltype(width)::value;
         Maps maps;
@@ -1112,51 +1134,64 @@ void set_weight_tiles(Args& g, const MlpShape& n)
     g.tiles = g.first[3] * g.parts;
 }
 
+// A backward call's workspace: x restored from its checkpoint, the operands TMA does not read in place, the hidden
+// values and their gradients unless they stay on chip, and the FP32 parts of the weight gradients.
 template <class T>
-std::size_t backward_bytes(const MlpShape& n)
-{
-    Arena arena{nullptr};
-    arena.take(static_cast<std::size_t>(n.tokens) * n.channels * sizeof(T));  // x restored
-    arena.take(staged_bytes<T>(n.tokens, n.channels));
-    arena.take(staged_bytes<T>(n.tokens, n.outputs));
-    arena.take(staged_bytes<T>(n.hidden, n.channels));
-    arena.take(staged_bytes<T>(n.hidden, n.channels));
-    arena.take(staged_bytes<T>(n.outputs, n.hidden));
-    for (int i = 0; i < 3; ++i) {
-        hidden_matrix<T>(n, arena);
+struct BackwardLayout {
+    bool narrow = false;
+    int parts = 0;
+    void* restored = nullptr;
+    StageJobs jobs;
+    Matrix dy, x, wg, wu, wd, dg, du, h;
+    Args weights;  // the weight products' tiles, where they are products of their own
+    float* partial = nullptr;
+
+    BackwardLayout(Arena& arena, const Arrays& in, bool packed, int dtype, const MlpShape& n)
+        : narrow(narrow_backward_fits(n, dtype))
+    {
+        if (packed) {
+            restored = arena.take(static_cast<std::size_t>(n.tokens) * n.channels * sizeof(T));
+        }
+        x = operand<T>(packed ? restored : in.x, n.tokens, n.channels, arena, jobs);
+        dy = operand<T>(in.dy, n.tokens, n.outputs, arena, jobs);
+        wg = operand<T>(in.wg, n.hidden, n.channels, arena, jobs);
+        wu = operand<T>(in.wu, n.hidden, n.channels, arena, jobs);
+        wd = operand<T>(in.wd, n.outputs, n.hidden, arena, jobs);
+        if (narrow) {
+            parts = narrow_backward_parts(n);
+        } else {
+            dg = hidden_matrix<T>(n, arena);
+            du = hidden_matrix<T>(n, arena);
+            h = hidden_matrix<T>(n, arena);
+            set_weight_tiles<T>(weights, n);
+            parts = weights.parts;
+        }
+        const std::size_t part = static_cast<std::size_t>(n.hidden) * (2 * static_cast<std::size_t>(n.channels) + n.outputs);
+        partial = static_cast<float*>(arena.take(sizeof(float) * part * parts));
     }
-    Args g;
-    set_weight_tiles<T>(g, n);
-    arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * std::max(g.parts, narrow_backward_parts(n)));
-    return arena.used + 256;
-}
+};
 
 template <class T>
-void mlp_backward(const void* dy, const void* x, const signed char* codes, const float* scales, const void* wg,
-                  const void* wu, const void* wd, void* dx, void* dwg, void* dwu, void* dwd, int dtype, const MlpShape& n,
-                  void* work, cudaStream_t stream)
+void mlp_backward(const Arrays& in, const signed char* codes, const float* scales, void* dx, void* dwg, void* dwu, void* dwd,
+                  int dtype, const MlpShape& n, void* work, cudaStream_t stream)
 {
-    Arena arena{reinterpret_cast<unsigned char*>((reinterpret_cast<std::uintptr_t>(work) + 255) & ~std::uintptr_t{255})};
+    Arena arena(work);
+    BackwardLayout<T> lay(arena, in, codes != nullptr, dtype, n);
     if (codes != nullptr) {
-        void* restored = arena.take(static_cast<std::size_t>(n.tokens) * n.channels * sizeof(T));
-        unpack8(codes, scales, restored, dtype, n.tokens, n.channels, stream);
-        x = restored;
+        unpack8(codes, scales, lay.restored, dtype, n.tokens, n.channels, stream);
     }
-    StageJobs jobs;
-    const Matrix mx = operand<T>(x, n.tokens, n.channels, arena, jobs);
-    const Matrix mdy = operand<T>(dy, n.tokens, n.outputs, arena, jobs);
-    const Matrix mg = operand<T>(wg, n.hidden, n.channels, arena, jobs);
-    const Matrix mu = operand<T>(wu, n.hidden, n.channels, arena, jobs);
-    const Matrix md = operand<T>(wd, n.outputs, n.hidden, arena, jobs);
-    run_jobs<T>(jobs, stream);
+    const Matrix &mx = lay.x, &mdy = lay.dy, &mg = lay.wg, &mu = lay.wu, &md = lay.wd;
+    const Matrix &mdg = lay.dg, &mdu = lay.du, &mh = lay.h;
+    float* const partial = lay.partial;
+    run_jobs<T>(lay.jobs, stream);
     const long long size0 = static_cast<long long>(n.hidden) * n.channels;
     const long long size2 = static_cast<long long>(n.outputs) * n.hidden;
     const long long part_size = 2 * size0 + size2;
-    const auto add_parts = [&](const float* partial, int parts) {
+    const auto add_parts = [&](int parts) {
         const auto launch = [&](auto many, int per_cta) {
             const unsigned grid = static_cast<unsigned>(std::min<long long>((part_size + per_cta - 1) / per_cta, 148 * 16));
-            launch_pdl(weight_sum_kernel<T, decltype(many)::value>, dim3(grid), dim3(256), 0, stream, partial,
-                       static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dwd), size0, size2, part_size, parts);
+            launch_pdl(weight_sum_kernel<T, decltype(many)::value>, dim3(grid), dim3(256), 0, stream,
+                       static_cast<const float*>(partial), static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dwd), size0, size2, part_size, parts);
         };
         if (parts > 8) {
             launch(std::true_type{}, 32);
@@ -1165,17 +1200,12 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         }
     };
     if constexpr (sizeof(T) == 2) {
-        if (narrow_backward_fits(n, dtype)) {
-            const int parts = narrow_backward_parts(n);
-            auto* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(part_size) * parts));
+        if (lay.narrow) {
             narrow_backward(mdy, mx, mg, mu, md, dx, partial, dtype, n, stream);
-            add_parts(partial, parts);
+            add_parts(lay.parts);
             return;
         }
     }
-    const Matrix mdg = hidden_matrix<T>(n, arena);
-    const Matrix mdu = hidden_matrix<T>(n, arena);
-    const Matrix mh = hidden_matrix<T>(n, arena);
     const auto gate_back = [&](auto width) {
         constexpr int BN = decltype(width)::value;
         Maps maps;
@@ -1231,9 +1261,7 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         maps.b[0] = mx.map(kChunk);
         maps.b[1] = mx.map(kChunk);
         maps.b[2] = mh.map(kChunk);
-        Args g;
-        set_weight_tiles<T>(g, n);
-        float* partial = static_cast<float*>(arena.take(sizeof(float) * static_cast<std::size_t>(g.part_size) * g.parts));
+        Args& g = lay.weights;
         g.out[0] = partial;
         if constexpr (sizeof(T) == 2) {
             if (large_weight_tiles<T>(n)) {
@@ -1244,7 +1272,7 @@ void mlp_backward(const void* dy, const void* x, const signed char* codes, const
         } else {
             launch_product<Kind::kWeight, 128, 1, T, SPECTRAL_ACT_NONE>(maps, g, stream);
         }
-        add_parts(partial, g.parts);
+        add_parts(lay.parts);
     }
 }
 
@@ -1278,7 +1306,9 @@ bool overlap(const void* a, unsigned long long a_bytes, const void* b, unsigned 
 }  // namespace
 }  // namespace spectral
 
-extern "C" int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs, size_t* count)
+extern "C" int spectral_gated_mlp_workspace_for(const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                                                int dtype, long long tokens, int channels, int hidden, int outputs,
+                                                size_t* count)
 {
     using namespace spectral;
     const int status = check("gated_mlp_workspace", dtype, tokens, channels, hidden, outputs);
@@ -1286,12 +1316,22 @@ extern "C" int spectral_gated_mlp_workspace(int dtype, long long tokens, int cha
         return status != SPECTRAL_OK ? status : invalid("gated_mlp_workspace: null count");
     }
     const MlpShape n{tokens, channels, hidden, outputs, 0};
-    with_dtype(dtype, [&](auto t) { *count = (forward_bytes<decltype(t)>(n) + 7) / 8; });
+    with_dtype(dtype, [&](auto t) {
+        Arena arena;
+        const ForwardLayout<decltype(t)> lay(arena, {nullptr, x, w_gate, w_up, w_down}, dtype, n);
+        *count = (arena.total() + 7) / 8;
+    });
     return SPECTRAL_OK;
 }
 
-extern "C" int spectral_gated_mlp_backward_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
-                                                     size_t* count)
+extern "C" int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs, size_t* count)
+{
+    return spectral_gated_mlp_workspace_for(nullptr, nullptr, nullptr, nullptr, dtype, tokens, channels, hidden, outputs, count);
+}
+
+extern "C" int spectral_gated_mlp_backward_workspace_for(const void* dy, const void* x, int packed, const void* w_gate,
+                                                         const void* w_up, const void* w_down, int dtype, long long tokens,
+                                                         int channels, int hidden, int outputs, size_t* count)
 {
     using namespace spectral;
     const int status = check("gated_mlp_backward_workspace", dtype, tokens, channels, hidden, outputs);
@@ -1299,7 +1339,26 @@ extern "C" int spectral_gated_mlp_backward_workspace(int dtype, long long tokens
         return status != SPECTRAL_OK ? status : invalid("gated_mlp_backward_workspace: null count");
     }
     const MlpShape n{tokens, channels, hidden, outputs, 0};
-    with_dtype(dtype, [&](auto t) { *count = (backward_bytes<decltype(t)>(n) + 7) / 8; });
+    with_dtype(dtype, [&](auto t) {
+        Arena arena;
+        const BackwardLayout<decltype(t)> lay(arena, {dy, x, w_gate, w_up, w_down}, packed != 0, dtype, n);
+        *count = (arena.total() + 7) / 8;
+    });
+    return SPECTRAL_OK;
+}
+
+extern "C" int spectral_gated_mlp_backward_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
+                                                     size_t* count)
+{
+    size_t plain = 0, packed = 0;
+    for (size_t* c : {&plain, &packed}) {
+        const int status = spectral_gated_mlp_backward_workspace_for(nullptr, nullptr, c == &packed, nullptr, nullptr, nullptr, dtype,
+                                                                     tokens, channels, hidden, outputs, count != nullptr ? c : nullptr);
+        if (status != SPECTRAL_OK) {
+            return status;
+        }
+    }
+    *count = std::max(plain, packed);
     return SPECTRAL_OK;
 }
 
@@ -1333,7 +1392,7 @@ extern "C" int spectral_gated_mlp(const void* x, const void* w_gate, const void*
     try {
         const MlpShape n{tokens, channels, hidden, outputs, activation};
         with_dtype(dtype, [&](auto t) {
-            mlp_forward<decltype(t)>(x, w_gate, w_up, w_down, y, dtype, n, work, static_cast<cudaStream_t>(stream));
+            mlp_forward<decltype(t)>({nullptr, x, w_gate, w_up, w_down}, y, dtype, n, work, static_cast<cudaStream_t>(stream));
         });
         return SPECTRAL_OK;
     } catch (const std::exception& e) {
@@ -1383,8 +1442,8 @@ extern "C" int spectral_gated_mlp_backward(const void* dy, const void* x, const 
         }
         const MlpShape n{tokens, channels, hidden, outputs, activation};
         with_dtype(dtype, [&](auto t) {
-            mlp_backward<decltype(t)>(dy, x, static_cast<const signed char*>(codes), scales, w_gate, w_up, w_down, dx,
-                                      dw_gate, dw_up, dw_down, dtype, n, work, s);
+            mlp_backward<decltype(t)>({dy, x, w_gate, w_up, w_down}, static_cast<const signed char*>(codes), scales, dx, dw_gate,
+                                      dw_up, dw_down, dtype, n, work, s);
         });
         return SPECTRAL_OK;
     } catch (const std::exception& e) {

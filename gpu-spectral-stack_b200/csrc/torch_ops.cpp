@@ -838,7 +838,7 @@ at::Tensor gated_mlp_cuda(const at::Tensor& x, const at::Tensor& w_gate, const a
     const at::Tensor wu = w_up.contiguous();
     const at::Tensor wd = w_down.contiguous();
     size_t count = 0;
-    check_status(spectral_gated_mlp_workspace(dtype, n.tokens, n.channels, n.hidden, n.outputs, &count));
+    check_status(spectral_gated_mlp_workspace_for(cptr(xc), cptr(wg), cptr(wu), cptr(wd), dtype, n.tokens, n.channels, n.hidden, n.outputs, &count));
     at::Tensor work = workspace(count, x);
     check_status(spectral_gated_mlp(cptr(xc), cptr(wg), cptr(wu), cptr(wd), mptr(y), dtype, n.tokens, n.channels, n.hidden,
                                     n.outputs, act, mptr(work), stream()));
@@ -885,7 +885,8 @@ gated_mlp_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x
     at::Tensor dwu = at::empty(wg.sizes(), dy.options());
     at::Tensor dwd = at::empty(wd.sizes(), dy.options());
     size_t count = 0;
-    check_status(spectral_gated_mlp_backward_workspace(dtype, n.tokens, n.channels, n.hidden, n.outputs, &count));
+    check_status(spectral_gated_mlp_backward_workspace_for(cptr(dyc), xc.defined() ? cptr(xc) : nullptr, cc.defined() ? 1 : 0,
+                                                           cptr(wg), cptr(wu), cptr(wd), dtype, n.tokens, n.channels, n.hidden, n.outputs, &count));
     at::Tensor work = workspace(count, dy);
     check_status(spectral_gated_mlp_backward(cptr(dyc), xc.defined() ? cptr(xc) : nullptr, cc.defined() ? cptr(cc) : nullptr,
                                              fptr(sc), cptr(wg), cptr(wu), cptr(wd), mptr(dx), mptr(dwg), mptr(dwu),

@@ -87,8 +87,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spectral_group_norm_act_backward": (_i, [_p] * 11 + [_i, _ll, _ll, _i, _i, _i, _p, _p]),
     "spectral_channels_last": (_i, [_p, _p, _i, _ll, _ll, _i, _p]),
     "spectral_gated_mlp_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),
+    "spectral_gated_mlp_workspace_for": (_i, [_p] * 4 + [_i, _ll, _i, _i, _i, _szp]),
     "spectral_gated_mlp": (_i, [_p] * 5 + [_i, _ll, _i, _i, _i, _i, _p, _p]),
     "spectral_gated_mlp_backward_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),
+    "spectral_gated_mlp_backward_workspace_for": (_i, [_p, _p, _i, _p, _p, _p, _i, _ll, _i, _i, _i, _szp]),
     "spectral_gated_mlp_backward": (_i, [_p] * 11 + [_i, _ll, _i, _i, _i, _i, _p, _p]),
     "spectral_fp32_ceiling": (_i, [_p, _i, _i, _p, ctypes.POINTER(ctypes.c_double)]),
     "spectral_spectrum": (_i, [_s, _p, _p, _p, _ll, _i, _ll, _p]),

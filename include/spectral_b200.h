@@ -371,6 +371,11 @@ SPECTRAL_API int spectral_channels_last(const void* x, void* y, int dtype, long 
  * products, and have its range: an FP16 hidden value beyond 65504 is infinite. */
 SPECTRAL_API int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
                                               size_t* count);
+/* The same for the arrays a call will be given: smaller where they need no staging copy (16-bit values in rows of
+ * 16 bytes, 16-byte aligned). NULL is an array of unknown alignment. */
+SPECTRAL_API int spectral_gated_mlp_workspace_for(const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                                                  int dtype, long long tokens, int channels, int hidden, int outputs,
+                                                  size_t* count);
 SPECTRAL_API int spectral_gated_mlp(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* y,
                                     int dtype, long long tokens, int channels, int hidden, int outputs,
                                     int activation, void* work, void* stream);
@@ -379,6 +384,11 @@ SPECTRAL_API int spectral_gated_mlp(const void* x, const void* w_gate, const voi
  * The products of the forward pass are recomputed, nothing but x is kept. Fixed summation order. */
 SPECTRAL_API int spectral_gated_mlp_backward_workspace(int dtype, long long tokens, int channels, int hidden,
                                                        int outputs, size_t* count);
+/* The same for the arrays a call will be given, from x or, if `packed` is not 0, its checkpoint. */
+SPECTRAL_API int spectral_gated_mlp_backward_workspace_for(const void* dy, const void* x, int packed, const void* w_gate,
+                                                           const void* w_up, const void* w_down, int dtype,
+                                                           long long tokens, int channels, int hidden, int outputs,
+                                                           size_t* count);
 SPECTRAL_API int spectral_gated_mlp_backward(const void* dy, const void* x, const void* codes, const float* scales,
                                              const void* w_gate, const void* w_up, const void* w_down, void* dx,
                                              void* dw_gate, void* dw_up, void* dw_down, int dtype, long long tokens,

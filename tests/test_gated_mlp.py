@@ -429,3 +429,55 @@ def test_forward_mode_tangents_are_refused(which, grad_mode):
         args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             gated_mlp(*args)
+
+
+# bf16: tokens, channels, hidden, outputs; a shape whose forward pass stays on chip, ones whose backward pass does not.
+@pytest.mark.parametrize(("tokens", "channels", "hidden", "outputs"), [(262144, 64, 128, 64), (262144, 128, 256, 128), (8192, 512, 2048, 512),
+                                                                       (8192, 1024, 4096, 1024), (8192, 4096, 11008, 4096),
+                                                                       (32768, 4096, 14336, 4096), (100, 24, 40, 8)])
+def test_workspaces_hold_what_a_call_uses(tokens, channels, hidden, outputs):
+    small = 4096 + 512 * hidden  # roundings to 256 bytes, and a few rows
+    operands = 2 * (tokens * channels + 2 * hidden * channels + hidden * outputs)
+    hidden_values = 2 * tokens * (hidden + 15) // 16 * 16
+    gradients = 4 * hidden * (2 * channels + outputs)
+    on_chip = channels <= 64 and outputs <= 64 and hidden <= 128
+    # Parts of the weight gradients: one per CTA on chip, else what fills a few whole waves of 148 SMs.
+    tiles = 2 * -(-hidden // 256) * -(-channels // 256) + -(-outputs // 256) * -(-hidden // 256)
+    parts = min(148, -(-tokens // 128)) if on_chip else 1 + 4 * 148 // tiles
+    forward = 8 * native.workspace("spectral_gated_mlp_workspace", 1, tokens, channels, hidden, outputs)
+    assert forward <= operands + (0 if channels <= 64 and hidden <= 256 else hidden_values) + small
+    backward = 8 * native.workspace("spectral_gated_mlp_backward_workspace", 1, tokens, channels, hidden, outputs)
+    most = 2 * tokens * outputs + operands + (0 if on_chip else 3 * hidden_values) + parts * gradients + small
+    assert backward <= most
+    # For arrays that are read in place: no copies of them, x restored only from a checkpoint.
+    shape = (1, tokens, channels, hidden, outputs)
+    at = 4096
+    assert 8 * native.workspace("spectral_gated_mlp_workspace_for", at, at, at, at, *shape) <= forward - operands + small
+    for packed in (0, 1):
+        exact = 8 * native.workspace("spectral_gated_mlp_backward_workspace_for", at, None if packed else at, packed, at, at, at, *shape)
+        assert exact <= backward - operands - 2 * tokens * outputs + packed * 2 * tokens * channels + small
+
+
+def test_a_checkpoint_saves_memory_in_the_backward_pass():
+    # What a backward pass from 8 bits needs beside its operands is no more than one restored x.
+    for shape in [(1, 262144, 64, 128, 64), (1, 8192, 512, 2048, 512), (0, 8192, 512, 2048, 512), (2, 999, 37, 50, 37)]:
+        plain, packed = (native.workspace("spectral_gated_mlp_backward_workspace_for", 4096, None if p else 4096, p, 4096, 4096, 4096, *shape)
+                         for p in (0, 1))
+        size = (4 if shape[0] == 0 else 2) * shape[1] * shape[2]
+        assert 8 * (packed - plain) <= size + 4096
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_a_training_step_allocates_what_it_needs(checkpoint8):
+    tokens, channels, hidden = 8192, 512, 2048
+    *args, dy = inputs(tokens, channels, hidden, channels, torch.bfloat16)
+    leaves = [a.requires_grad_(True) for a in args]
+    y = gated_mlp(*leaves, checkpoint8=checkpoint8)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(y, leaves, dy)
+    peak = torch.cuda.max_memory_allocated() - before
+    # The results, three hidden arrays, a restored x, and FP32 parts of the weight gradients (48 tiles: seven at most).
+    assert peak <= sum(g.numel() * 2 for g in grads) + 3 * 2 * tokens * hidden + 2 * tokens * channels + 7 * 4 * 3 * hidden * channels + (1 << 22)
