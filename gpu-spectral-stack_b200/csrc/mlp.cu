@@ -244,11 +244,15 @@ struct Tile {
 template <Kind K, class T>
 constexpr bool kApart = K == Kind::kInput && sizeof(T) == 4;
 
+// Chunks of K whose products share an accumulator.
+template <Kind K, class T>
+constexpr int kPass = K == Kind::kWeight && sizeof(T) == 2 ? kLongSum * 16 / kChunk : Operand<T>::kPassChunks;
+
 // The chunks of operand pair `pair` that pass `pass` of a tile covers.
-template <class T>
+template <Kind K, class T>
 __device__ __forceinline__ void pass_range(const Args& g, const Tile& tile, int pair, int pass, int& begin, int& end)
 {
-    constexpr int kStep = Operand<T>::kPassChunks;
+    constexpr int kStep = kPass<K, T>;
     const int last = pair == 0 ? tile.k1 : g.chunks[1];
     begin = min((pair == 0 ? tile.k0 : 0) + pass * kStep, last);
     end = min(begin + kStep, last);
@@ -271,23 +275,26 @@ __device__ __forceinline__ Tile locate(const Args& g, long long t)
         tile.m0 = static_cast<int>(t / g.n_tiles) * (MT * kTileM);
         tile.n0 = static_cast<int>(t % g.n_tiles) * BN;
     }
-    if constexpr (sizeof(T) == 4) {
-        constexpr int kStep = Operand<T>::kPassChunks;
+    if constexpr (sizeof(T) == 4 || K == Kind::kWeight) {
+        constexpr int kStep = kPass<K, T>;
         tile.passes = (max(tile.k1 - tile.k0, g.chunks[1]) + kStep - 1) / kStep;
     }
     return tile;
 }
 
-// Results of one accumulator: the warp's 32 rows from row - lane on, 32 columns from col on.
+// Results of one accumulator: the warp's 32 rows from row - lane on, 32 columns from col on; `add` (kWeight): to those
+// of the passes before.
 template <Kind K, class T>
-__device__ __forceinline__ void store_results(const Args& g, const Tile& tile, int row, int rows, int col, int cols, float (&acc)[32])
+__device__ __forceinline__ void store_results(const Args& g, const Tile& tile, int row, int rows, int col, int cols, float (&acc)[32],
+                                              bool add = false)
 {
     using Out = std::conditional_t<K == Kind::kWeight, float, T>;
     const int lane = threadIdx.x & 31;
     const long long pitch = K == Kind::kWeight ? cols : g.pitch;
     Out* out = static_cast<Out*>(g.out[0]) + (K == Kind::kWeight ? tile.part * g.part_size + g.offset[tile.problem] : 0);
     const int first = row - lane;
-    store_rows(out + static_cast<long long>(first) * pitch + col, pitch, acc, rows - first, cols - col);
+    store_rows(out + static_cast<long long>(first) * pitch + col, pitch, acc, rows - first, cols - col,
+               K == Kind::kWeight && add);
 }
 
 // The epilogue of the gate kernels, N columns of one row from col on: acc holds each accumulator's values.
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
             for (int turn = 0; ok && turn < tile.passes * kPairs; ++turn) {
                 const int pair = turn % kPairs;
                 int k0, k1;
-                pass_range<T>(g, tile, pair, turn / kPairs, k0, k1);
+                pass_range<K, T>(g, tile, pair, turn / kPairs, k0, k1);
                 for (int p = 0; ok && p < Op::kProducts; ++p) {
                     const int pa = part_a<T>(p), pb = part_b<T>(p);
                     for (int k = k0; k < k1; ++k) {
@@ -474,7 +481,7 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
                 const int first = kApart<K, T> ? pass & 1 : 0;
                 for (int pair = first; ok && pair < (kApart<K, T> ? first + 1 : kPairs); ++pair) {
                     int k0, k1;
-                    pass_range<T>(g, tile, pair, kApart<K, T> ? pass >> 1 : pass, k0, k1);
+                    pass_range<K, T>(g, tile, pair, kApart<K, T> ? pass >> 1 : pass, k0, k1);
                     const int steps = (k1 - k0) * Op::kProducts;
                     // kInput's two products share an accumulator (16-bit types); kGateBack's second has its own.
                     const bool fresh = kApart<K, T> || pair == 0 || K == Kind::kGateBack;
@@ -580,7 +587,7 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
                     for (int q = 0; q < Cfg::kSets; ++q) {
                         // An operand pair that ended in an earlier pass has nothing new here.
                         int begin, end;
-                        pass_range<T>(g, tile, kApart<K, T> ? pass & 1 : K == Kind::kGateBack && q == 2 ? 1 : 0,
+                        pass_range<K, T>(g, tile, kApart<K, T> ? pass & 1 : K == Kind::kGateBack && q == 2 ? 1 : 0,
                                       kApart<K, T> ? pass >> 1 : pass, begin, end);
                         if (begin < end) {
 #pragma unroll
@@ -612,8 +619,11 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
                     }
                 }
             } else {
-                ok = tma::mbar_wait(&done[slot], slot_phase);
-                if (ok) {
+                for (int pass = 0; ok && pass < tile.passes; ++pass) {
+                    ok = tma::mbar_wait(&done[slot], slot_phase);
+                    if (!ok) {
+                        break;
+                    }
                     umma::fence_after_sync();
                     const uint32_t d = tmem + slot * Cfg::kCols + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
@@ -633,7 +643,7 @@ __global__ void __launch_bounds__(Config<K, BN, MT, T>::kThreads, 1) product_ker
                             umma::load_wait(acc[q]);
                         }
                         if constexpr (Cfg::kSets == 1) {
-                            store_results<K, T>(g, tile, row + m * kTileM, rows, tile.n0 + c, cols, acc[0]);
+                            store_results<K, T>(g, tile, row + m * kTileM, rows, tile.n0 + c, cols, acc[0], pass > 0);
                         } else if (row + m * kTileM < rows) {
                             finish<K, T, Act>(g, tile, row + m * kTileM, tile.n0 + c, cols, acc);
                         }

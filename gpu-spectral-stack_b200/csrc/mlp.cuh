@@ -51,6 +51,14 @@ __device__ __forceinline__ void split3(float v, bf16& hi, bf16& mid, bf16& lo)
     lo = __float2bfloat16_rn(r - __bfloat162float(mid));
 }
 
+// The tensor core cuts its FP32 accumulator once per MMA, which pulls a long sum towards zero: by 1.1e-7 of it per
+// MMA (16 values of K) where the terms have one sign, 5.8e-4 at 87000 tokens, more than a rounding to f16. Sums
+// over tokens therefore leave the accumulator after this many MMAs and add up in FP32 (rounded to
+// nearest): 5.5e-5 at most, a fifth of that rounding. Sums over channels or hidden values stay in one accumulator:
+// they would need 8192 to get there. (Backward passes past that, with and without: 262144 x 512 x 2048 bf16 4.75 and 4.57 ms,
+// narrow at 4.2 M tokens 785 and 745 us; shorter sums are not touched.)
+constexpr int kLongSum = 512;
+
 // A run of N (16 or 32) values of one row; only the first `valid` exist.
 template <class T, int N>
 __device__ __forceinline__ void store_run(T* p, const T (&v)[N], int valid)
@@ -98,13 +106,32 @@ __device__ __forceinline__ void store_values(T* p, const float (&v)[N], int vali
 // A warp's N columns (16 or 32) of 32 rows, lane l holding row l; p is the first row's first value, and `rows` rows and
 // `cols` columns from there on exist. Where the rows' runs are whole sectors each lane stores its own. Else
 // the values are transposed by shuffles and stored side by side (47519 x 895 bf16 results of 8 hidden
-// values: 94 us, with single values of 32 rows at a time 440 us).
+// values: 94 us, with single values of 32 rows at a time 440 us). `add` (FP32 results): to what an earlier
+// call stored there; each lane meets only its own stores again.
 template <class T, int N>
-__device__ __forceinline__ void store_rows(T* p, long long pitch, float (&v)[N], long long rows, int cols)
+__device__ __forceinline__ void store_rows(T* p, long long pitch, float (&v)[N], long long rows, int cols, bool add = false)
 {
     const int lane = threadIdx.x & 31;
     if (((reinterpret_cast<std::uintptr_t>(p) | static_cast<std::uintptr_t>(pitch * sizeof(T))) & 31u) == 0) {
         if (lane < rows && cols > 0) {
+            if (add) {
+                const T* before = p + lane * pitch;
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    if (j + 4 <= cols) {
+                        const Vec<T, 4> b = *reinterpret_cast<const Vec<T, 4>*>(before + j);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[j + i] += to_float(b.v[i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[j + i] += j + i < cols ? to_float(before[j + i]) : 0.0f;
+                        }
+                    }
+                }
+            }
             store_values<T>(p + lane * pitch, v, min(N, cols));
         }
         return;
@@ -126,7 +153,8 @@ __device__ __forceinline__ void store_rows(T* p, long long pitch, float (&v)[N],
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         if (row + j < rows && col < cols) {
-            p[(row + j) * pitch + col] = from_float<T>(v[j]);
+            T* at = p + (row + j) * pitch + col;
+            *at = from_float<T>(add ? v[j] + to_float(*at) : v[j]);
         }
     }
 }

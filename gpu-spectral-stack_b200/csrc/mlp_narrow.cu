@@ -17,7 +17,8 @@
 //          per tile: dWd^T += [h_0 h_1]^T dy
 // The weight gradients stay in tensor memory over all of a CTA's tiles (512 columns in all: 192 for a
 // chunk's three products, 2 x 64 for dx, 128 and 64 for the gradients) and leave it once, as the
-// CTA's part of a sum that a last kernel adds up in order.
+// CTA's part of a sum that a last kernel adds up in order. (Past 64 tiles a CTA, ranges of tokens are launched
+// one by one.)
 // x, dy, the weights and the hidden tiles each serve as K-major and as MN-major operands from the
 // one copy in shared memory (umma.cuh).
 //
@@ -807,27 +808,51 @@ bool narrow_backward_fits(const MlpShape& n, int dtype)
     return dtype != SPECTRAL_FLOAT32 && n.channels <= kBackWidth && n.outputs <= kBackWidth && n.hidden <= kBackHidden;
 }
 
-int narrow_backward_parts(const MlpShape& n) { return std::min(tile_count(n), 148); }
+// The weight gradients' accumulators take 8 MMAs per tile (128 tokens) over all of a CTA's tiles, so a call of very
+// many tokens is cut into ranges of as many tiles each, a launch with parts of its own (kLongSum; 1.2 M tokens).
+constexpr int kBackCtas = 148;
+constexpr int kRangeTiles = kLongSum / (kTileM / 16) * kBackCtas;
+int backward_ranges(const MlpShape& n) { return std::max(1, (tile_count(n) + kRangeTiles - 1) / kRangeTiles); }
+int range_tiles(const MlpShape& n) { return (tile_count(n) + backward_ranges(n) - 1) / backward_ranges(n); }
+
+int narrow_backward_parts(const MlpShape& n)
+{
+    const int ranges = backward_ranges(n), each = range_tiles(n);
+    return (ranges - 1) * std::min(each, kBackCtas) + std::min(tile_count(n) - (ranges - 1) * each, kBackCtas);
+}
 
 void narrow_backward(const Matrix& dy, const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd, void* dx,
                      float* partial, int dtype, const MlpShape& n, cudaStream_t stream)
 {
-    NarrowMaps maps{};
-    maps.x = x.map(kTileM);
-    maps.dy = dy.map(kTileM);
-    maps.wg = wg.map(kHiddenChunk);
-    maps.wu = wu.map(kHiddenChunk);
-    maps.wd = wd.map(64);
-    NarrowArgs g = arguments(n, dx);
-    g.partial = partial;
-    g.part_size = 2LL * n.hidden * n.channels + static_cast<long long>(n.outputs) * n.hidden;
-    with_16_bits(dtype, [&](auto type) {
-        using T = decltype(type);
-        with_activation(n.act, [&](auto act) {
-            constexpr int Act = decltype(act)::value;
-            launch<narrow_backward_kernel<T, Act>>(narrow_backward_parts(n), kBackSmem, maps, g, stream);
+    const int each = range_tiles(n);
+    for (int first = 0; first < tile_count(n); first += each) {
+        const long long start = static_cast<long long>(first) * kTileM;
+        MlpShape part = n;
+        part.tokens = std::min(n.tokens - start, static_cast<long long>(each) * kTileM);
+        const auto rows = [&](Matrix m) {  // the range's rows of x or dy
+            m.base = static_cast<const char*>(m.base) + start * m.pitch * 2;
+            m.rows = part.tokens;
+            return m.map(kTileM);
+        };
+        NarrowMaps maps{};
+        maps.x = rows(x);
+        maps.dy = rows(dy);
+        maps.wg = wg.map(kHiddenChunk);
+        maps.wu = wu.map(kHiddenChunk);
+        maps.wd = wd.map(64);
+        NarrowArgs g = arguments(part, static_cast<char*>(dx) + start * n.channels * 2);
+        const int ctas = std::min(g.tiles, kBackCtas);
+        g.partial = partial;
+        g.part_size = 2LL * n.hidden * n.channels + static_cast<long long>(n.outputs) * n.hidden;
+        with_16_bits(dtype, [&](auto type) {
+            using T = decltype(type);
+            with_activation(n.act, [&](auto act) {
+                constexpr int Act = decltype(act)::value;
+                launch<narrow_backward_kernel<T, Act>>(ctas, kBackSmem, maps, g, stream);
+            });
         });
-    });
+        partial += ctas * g.part_size;
+    }
 }
 
 }  // namespace spectral::mlp

@@ -481,3 +481,41 @@ def test_a_training_step_allocates_what_it_needs(checkpoint8):
     peak = torch.cuda.max_memory_allocated() - before
     # The results, three hidden arrays, a restored x, and FP32 parts of the weight gradients (48 tiles: seven at most).
     assert peak <= sum(g.numel() * 2 for g in grads) + 3 * 2 * tokens * hidden + 2 * tokens * channels + 7 * 4 * 3 * hidden * channels + (1 << 22)
+
+
+# Sums over many tokens, of terms of one sign: the wide kernels with 128 and with 256 columns a tile, and the narrow one.
+@pytest.mark.gpu
+@pytest.mark.parametrize(("tokens", "channels", "hidden", "outputs"), [(262144 + 77, 200, 401, 201), (262144, 320, 512, 320),
+                                                                       ((1 << 24) + 77, 64, 128, 64)])
+def test_weight_gradients_of_many_tokens_are_not_pulled_towards_zero(tokens, channels, hidden, outputs):
+    dtype = torch.float16
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def positive(rows, cols, scale):
+        return torch.rand(rows, cols, generator=g, device="cuda").add_(0.5).mul_(scale).to(dtype)
+
+    args = [positive(tokens, channels, 1.0), positive(hidden, channels, 1 / channels), positive(hidden, channels, 1 / channels),
+            positive(outputs, hidden, 1 / hidden)]
+    dy = positive(tokens, outputs, 64 / tokens)
+    leaves = [a.requires_grad_(True) for a in args]
+    got = torch.autograd.grad(gated_mlp(*leaves, activation="none"), leaves, dy)
+    with torch.no_grad():
+        wg, wu, wd = (a.double() for a in args[1:])
+        want = [torch.zeros_like(w) for w in (wg, wu, wd)]
+        for i in range(0, tokens, 1 << 17):
+            x, d = args[0][i:i + (1 << 17)].double(), dy[i:i + (1 << 17)].double()
+            gate, up, dh = x @ wg.T, x @ wu.T, d @ wd
+            want[0] += (dh * up).T @ x
+            want[1] += (dh * gate).T @ x
+            want[2] += d.T @ (gate * up)
+    # An MMA of 16 tokens cuts its sum by less than 2^-23 of what it ends up as, and 512 follow one another at most;
+    # roundings to the type (of the hidden values, their gradients and the results) are to nearest and leave a mean of
+    # 2^-17 at most over these many values.
+    for name, a, b in zip(("dw_gate", "dw_up", "dw_down"), got[1:], want):
+        mean = float(((a.double() - b) / b).mean())
+        assert abs(mean) <= 512 * 2.0 ** -23 + 2.0 ** -17, f"{name}: {mean:.3g}"
+    # dx, wherever the call was cut: the rows' own values.
+    for i in (0, tokens // 14 // 128 * 128, tokens // 2, tokens - 301):
+        rows = [args[0][i:i + 300].detach().requires_grad_(True), *leaves[1:]]
+        (alone,) = torch.autograd.grad(gated_mlp(*rows, activation="none"), rows[:1], dy[i:i + 300])
+        assert torch.equal(got[0][i:i + 300], alone)
