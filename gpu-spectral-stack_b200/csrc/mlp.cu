@@ -1446,6 +1446,9 @@ extern "C" int spectral_gated_mlp_backward(const void* dy, const void* x, const 
                 return invalid("gated_mlp_backward: arrays must be aligned to their element size");
             }
         }
+        if (!aligned_to(scales, sizeof(float))) {
+            return invalid("gated_mlp_backward: scales must be aligned to 4 bytes");
+        }
         if (overlap(dx, tokens * channels * size, dy, tokens * outputs * size)
             || (x != nullptr && overlap(dx, tokens * channels * size, x, tokens * channels * size))) {
             return invalid("gated_mlp_backward: dx must not overlap dy or x");

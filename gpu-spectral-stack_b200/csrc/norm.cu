@@ -1650,6 +1650,17 @@ bool overlap(const void* a, const void* b, unsigned long long bytes)
     return p < q + bytes && q < p + bytes;
 }
 
+// The float arrays beside the values: parameters, statistics, scales (null ones are not given).
+bool floats_aligned(std::initializer_list<const void*> arrays)
+{
+    for (const void* p : arrays) {
+        if (!aligned_to(p, sizeof(float))) {
+            return false;
+        }
+    }
+    return true;
+}
+
 }  // namespace
 }  // namespace spectral
 
@@ -1719,7 +1730,8 @@ extern "C" int spectral_group_norm_act(const void* x, const float* weight, const
         || (codes == nullptr) != (scales == nullptr)) {
         return invalid("group_norm_act: x, y and work must be given, mean with rstd, and codes with scales");
     }
-    if (!aligned_to(x, dtype_size(dtype)) || !aligned_to(y, dtype_size(dtype)) || !aligned_to(work, 8)) {
+    if (!aligned_to(x, dtype_size(dtype)) || !aligned_to(y, dtype_size(dtype)) || !aligned_to(work, 8)
+        || !floats_aligned({weight, bias, mean, rstd, scales})) {
         return invalid("group_norm_act: arrays must be aligned to their element size, work to 8 bytes");
     }
     if (overlap(x, y, static_cast<unsigned long long>(batch * points) * channels * dtype_size(dtype))) {
@@ -1758,6 +1770,9 @@ extern "C" int spectral_group_norm_act_backward(const void* dy, const void* x, c
     const auto s = static_cast<cudaStream_t>(stream);
     try {
         if (batch == 0 || points == 0) {  // sums over nothing
+            if (!floats_aligned({dweight, dbias})) {
+                return invalid("group_norm_act_backward: arrays must be aligned to their element size");
+            }
             if (dweight != nullptr) {
                 SPECTRAL_CUDA(cudaMemsetAsync(dweight, 0, sizeof(float) * channels, s));
             }
@@ -1771,7 +1786,8 @@ extern "C" int spectral_group_norm_act_backward(const void* dy, const void* x, c
             return invalid("group_norm_act_backward: dy, dx, mean, rstd and work must be given, and either x or codes with scales");
         }
         const std::size_t size = dtype_size(dtype);
-        if (!aligned_to(dy, size) || !aligned_to(dx, size) || !aligned_to(x, size) || !aligned_to(work, 8)) {
+        if (!aligned_to(dy, size) || !aligned_to(dx, size) || !aligned_to(x, size) || !aligned_to(work, 8)
+            || !floats_aligned({scales, weight, bias, mean, rstd, dweight, dbias})) {
             return invalid("group_norm_act_backward: arrays must be aligned to their element size, work to 8 bytes");
         }
         const unsigned long long bytes = static_cast<unsigned long long>(batch * points) * channels * size;

@@ -519,3 +519,11 @@ def test_weight_gradients_of_many_tokens_are_not_pulled_towards_zero(tokens, cha
         rows = [args[0][i:i + 300].detach().requires_grad_(True), *leaves[1:]]
         (alone,) = torch.autograd.grad(gated_mlp(*rows, activation="none"), rows[:1], dy[i:i + 300])
         assert torch.equal(got[0][i:i + 300], alone)
+
+
+def test_the_c_abi_refuses_unaligned_scales():
+    a = dict(dy=1 << 20, x=None, codes=1 << 21, scales=(1 << 18) + 2, w_gate=1 << 22, w_up=1 << 23, w_down=1 << 24, dx=1 << 25,
+             dw_gate=1 << 26, dw_up=1 << 27, dw_down=1 << 29, dtype=1, tokens=4, channels=8, hidden=16, outputs=8, activation=1,
+             work=1 << 30, stream=None)
+    with pytest.raises(ValueError, match="aligned"):
+        native.call("spectral_gated_mlp_backward", *a.values())

@@ -428,3 +428,22 @@ def test_forward_mode_tangents_are_refused(which, grad_mode):
         args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             group_norm_act(args[0], 2, args[1], args[2], activation="gelu")
+
+
+@pytest.mark.parametrize("change", [dict(weight=(1 << 20) + 2), dict(bias=(1 << 20) + 1), dict(mean=(1 << 20) + 2, rstd=1 << 21),
+                                    dict(mean=1 << 20, rstd=(1 << 21) + 2), dict(codes=1 << 20, scales=(1 << 21) + 2)])
+def test_the_c_abi_refuses_unaligned_float_arrays(change):
+    with pytest.raises(ValueError, match="aligned"):
+        native.call("spectral_group_norm_act", *forward_args(**change))
+
+
+@pytest.mark.parametrize(
+    ("change", "message"),
+    [({name: (1 << 24) + 2}, "aligned") for name in ("weight", "bias", "mean", "rstd", "dweight", "dbias")]
+    + [(dict(x=None, codes=1 << 21, scales=(1 << 23) + 2), "aligned"), (dict(dweight=(1 << 24) + 2, points=0), "aligned")])
+def test_the_c_abi_refuses_unaligned_float_arrays_backward(change, message):
+    a = dict(dy=1 << 20, x=1 << 21, codes=None, scales=None, weight=None, bias=None, mean=4096, rstd=8192, dx=1 << 22,
+             dweight=None, dbias=None, dtype=0, batch=1, points=4, channels=8, groups=2, activation=0, work=65536, stream=None)
+    a.update(change)
+    with pytest.raises(ValueError, match=message):
+        native.call("spectral_group_norm_act_backward", *a.values())
