@@ -1643,12 +1643,14 @@ int check(const char* op, int dtype, long long batch, long long points, int chan
     return SPECTRAL_OK;
 }
 
-bool overlap(const void* a, const void* b, unsigned long long bytes)
+bool overlap(const void* a, unsigned long long a_bytes, const void* b, unsigned long long b_bytes)
 {
     const auto p = reinterpret_cast<unsigned long long>(a);
     const auto q = reinterpret_cast<unsigned long long>(b);
-    return p < q + bytes && q < p + bytes;
+    return p < q + b_bytes && q < p + a_bytes;
 }
+
+bool overlap(const void* a, const void* b, unsigned long long bytes) { return overlap(a, bytes, b, bytes); }
 
 // The float arrays beside the values: parameters, statistics, scales (null ones are not given).
 bool floats_aligned(std::initializer_list<const void*> arrays)
@@ -1793,6 +1795,12 @@ extern "C" int spectral_group_norm_act_backward(const void* dy, const void* x, c
         const unsigned long long bytes = static_cast<unsigned long long>(batch * points) * channels * size;
         if (overlap(dx, dy, bytes) || (x != nullptr && overlap(dx, x, bytes))) {
             return invalid("group_norm_act_backward: dx must not overlap dy or x");
+        }
+        const unsigned long long rows = static_cast<unsigned long long>(batch * points);
+        if (codes != nullptr
+            && (overlap(dx, bytes, codes, rows * channels)
+                || overlap(dx, bytes, scales, rows * ((channels + kPackBlock - 1) / kPackBlock) * sizeof(float)))) {
+            return invalid("group_norm_act_backward: dx must not overlap the checkpoint");
         }
         const NormShape n{batch, points, channels, groups, channels / groups, activation, 0.0f};
         norm_backward(dy, x, static_cast<const signed char*>(codes), scales, weight, bias, mean, rstd, dx, dweight, dbias,

@@ -347,7 +347,7 @@ SPECTRAL_API int spectral_group_norm_act(const void* x, const float* weight, con
                                          int activation, void* work, void* stream);
 /* Its gradients for the upstream gradient dy, from the forward call's mean and rstd and either x
  * or its checkpoint (codes and scales, x NULL): dx, and dweight and dbias (`channels` floats each;
- * either may be NULL). Every sum has a fixed order: equal inputs give equal bits. */
+ * either may be NULL). dx must not overlap dy, x or the checkpoint. Every sum has a fixed order: equal inputs give equal bits. */
 SPECTRAL_API int spectral_group_norm_act_backward_workspace(int dtype, long long batch, long long points,
                                                             int channels, int groups, size_t* count);
 SPECTRAL_API int spectral_group_norm_act_backward(const void* dy, const void* x, const void* codes,

@@ -442,6 +442,15 @@ def test_the_c_abi_refuses_unaligned_float_arrays(change):
     [({name: (1 << 24) + 2}, "aligned") for name in ("weight", "bias", "mean", "rstd", "dweight", "dbias")]
     + [(dict(x=None, codes=1 << 21, scales=(1 << 23) + 2), "aligned"), (dict(dweight=(1 << 24) + 2, points=0), "aligned")])
 def test_the_c_abi_refuses_unaligned_float_arrays_backward(change, message):
+    backward_refuses(change, message)
+
+
+@pytest.mark.parametrize("change", [dict(codes=(1 << 22) + 100, scales=1 << 23), dict(codes=1 << 23, scales=(1 << 22) + 124)])
+def test_the_c_abi_refuses_dx_over_the_checkpoint(change):
+    backward_refuses(dict(x=None, **change), "must not overlap the checkpoint")
+
+
+def backward_refuses(change, message):
     a = dict(dy=1 << 20, x=1 << 21, codes=None, scales=None, weight=None, bias=None, mean=4096, rstd=8192, dx=1 << 22,
              dweight=None, dbias=None, dtype=0, batch=1, points=4, channels=8, groups=2, activation=0, work=65536, stream=None)
     a.update(change)
