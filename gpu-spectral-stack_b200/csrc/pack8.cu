@@ -235,7 +235,7 @@ int check(const char* op, const void* x, const void* codes, const void* scales, 
 
 void pack8(const void* x, int dtype, signed char* codes, float* scales, long long rows, int width, cudaStream_t stream)
 {
-    const int per_row = (width + kPackBlock - 1) / kPackBlock;
+    const int per_row = (width - 1) / kPackBlock + 1;
     const long long blocks = rows * per_row;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
@@ -255,7 +255,7 @@ void pack8(const void* x, int dtype, signed char* codes, float* scales, long lon
 void unpack8(const signed char* codes, const float* scales, void* x, int dtype, long long rows, int width,
              cudaStream_t stream)
 {
-    const int per_row = (width + kPackBlock - 1) / kPackBlock;
+    const int per_row = (width - 1) / kPackBlock + 1;
     const long long blocks = rows * per_row;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);

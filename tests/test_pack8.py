@@ -114,6 +114,24 @@ def test_past_two_to_the_31_values():
     assert torch.equal(back[-5:].cpu(), torch.from_numpy(want_codes.astype(np.float32) * want_scales).to(torch.bfloat16))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [2 ** 31 - 8, 2 ** 31 - 1])  # whole 16-byte pieces, and not
+def test_the_longest_rows(width):
+    first = (width - 1) // 64 * 64 - 128  # of the last blocks
+    tail = values(1, width - first, torch.float16, 3)
+    x = torch.zeros(1, width, dtype=torch.float16, device="cuda")
+    x[0, first:] = tail[0].cuda()
+    codes, scales = spectral.pack8(x)
+    want_codes, want_scales = definition(tail.float().numpy())
+    np.testing.assert_array_equal(codes[:, first:].cpu().numpy(), want_codes)
+    np.testing.assert_array_equal(scales[:, first // 64:].cpu().numpy(), want_scales)
+    assert not codes[:, :first].any()
+    del x
+    back = spectral.unpack8(codes, scales, dtype=torch.float16)
+    step = np.repeat(want_scales, 64, axis=1)[:, :width - first]
+    assert torch.equal(back[:, first:].cpu(), torch.from_numpy(want_codes.astype(np.float32) * step).to(torch.float16))
+
+
 @pytest.mark.parametrize(
     ("fn", "args", "message"),
     [
