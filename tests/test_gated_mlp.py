@@ -527,3 +527,19 @@ def test_the_c_abi_refuses_unaligned_scales():
              work=1 << 30, stream=None)
     with pytest.raises(ValueError, match="aligned"):
         native.call("spectral_gated_mlp_backward", *a.values())
+
+
+# Enough tokens for the wide tiles: 256 columns down and to the input, 128 at the gate both ways, weight tiles of 256 x 256 in
+# the 16-bit types; then 128 columns down and to the input, with weight tiles of 128 x 128.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize(("tokens", "channels", "hidden", "outputs"), [(8200, 520, 2050, 530), (12300, 120, 300, 120), (12289, 121, 299, 130)])
+def test_wide_tiles(tokens, channels, hidden, outputs, activation, dtype):
+    test_values_and_gradients(tokens, channels, hidden, outputs, activation, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_wide_tiles_from_an_8_bit_checkpoint(dtype):
+    test_gradients_from_an_8_bit_checkpoint(8200, 520, 2050, 530, dtype)

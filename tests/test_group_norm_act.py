@@ -456,3 +456,39 @@ def backward_refuses(change, message):
     a.update(change)
     with pytest.raises(ValueError, match=message):
         native.call("spectral_group_norm_act_backward", *a.values())
+
+
+# The two-pass form where rows are no whole 16-byte pieces (single values; pairs), and wide rows in tiles that hold whole groups.
+TWO_PASS = [((2, 70001, 37), 1), ((2, 50001, 54), 6), ((2, 1100, 4608), 144)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("shape", "groups"), TWO_PASS)
+def test_two_passes_over_odd_and_wide_rows(shape, groups, dtype):
+    assert math.prod(shape) * (4 if dtype == torch.float32 else 2) > 8 << 20  # smaller arrays stay on chip
+    test_values_and_gradients(shape, groups, "gelu", dtype)
+    test_gradients_from_an_8_bit_checkpoint(shape, groups, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_two_passes_over_unaligned_views(dtype, checkpoint8):
+    x, weight, bias, dy = inputs((2, 40001, 64), dtype, 6)
+
+    def step(x, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, weight, bias)]
+        y = group_norm_act(leaves[0], 8, leaves[1], leaves[2], activation="silu", checkpoint8=checkpoint8)
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    def shifted(t, by):  # the same values a few elements off a 16-byte boundary
+        flat = torch.empty(t.numel() + by, dtype=t.dtype, device=t.device)
+        flat[by:] = t.reshape(-1)
+        return flat[by:].view(t.shape)
+
+    want = step(x, dy)
+    for by in (1, 2):
+        for got, w in zip(step(shifted(x, by), shifted(dy, by)), want):
+            # Sums in another order, and a rounding that may then fall the other way.
+            close(got, w, 4 * TOL[torch.float32] + (0 if got.dtype == torch.float32 else TOL[dtype]))
