@@ -1097,8 +1097,9 @@ void mlp_forward(const Arrays& in, void* y, int dtype, const MlpShape& n, void* 
 
 // Tiles of the weight products: 256 x 256 where every side is longer than that (a tile of 128 x 128 reads
 // twice as much per product), else 128 x 128, whose epilogue overlaps. Backward passes measured with the large
-// and the small tiles, us: 8192 x 512 x 2048 149 and 159, 8192 x 1024 x 4096 519 and 538, but
-// 32768 x 256 x 512 114 and 106.
+// and the small tiles, us: 8192 x 512 x 2048 146 and 156, 8192 x 1024 x 4096 519 and 538, 8192 x 448 x 1792 140 and 152, but
+// 32768 x 256 x 512 114 and 106. From 257 to 384 neither wins by much (8192 x 384 x 1536 113 and 112, 8192 x 320 x 1280 89 and 85,
+// 65536 x 384 x 768 405 and 418).
 template <class T>
 bool large_weight_tiles(const MlpShape& n)
 {
@@ -1239,7 +1240,8 @@ void mlp_backward(const Arrays& in, const signed char* codes, const float* scale
     // 128 columns leave one accumulator set (384 of 512), so the epilogue does not overlap, but an MMA of N = 64
     // takes nearly as long as one of 128 and a wider tile reads its tokens fewer times: worth it where the
     // products are long. Backward passes with 128 and 64 columns, us: 8192 x 1024 x 4096 536 and 557,
-    // 8192 x 512 x 2048 147 and 150, 32768 x 256 x 512 105 and 99. At 128 the tiles' operands are what counts:
+    // 8192 x 512 x 2048 146 and 149, 8192 x 448 x 1792 150 and 142, 8192 x 384 x 1536 118 and 113, 32768 x 256 x 512 105 and 99;
+    // unequal sides, 16384 x 1024 x 300 with 512 outputs 118 and 120. At 128 the tiles' operands are what counts:
     // 650 MB from L2 to shared memory in the 72 us of 8192 x 512 x 2048, 9 TB/s.
     if constexpr (sizeof(T) == 4) {
         gate_back(std::integral_constant<int, 64>{});  // the passes' sums stay in registers

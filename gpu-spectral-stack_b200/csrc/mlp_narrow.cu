@@ -22,12 +22,12 @@
 // x, dy, the weights and the hidden tiles each serve as K-major and as MN-major operands from the
 // one copy in shared memory (umma.cuh).
 //
-// What bounds them (262144 tokens, 64 channels, 128 hidden). Forward: the instructions of the epilogue
-// warps (31 us with gelu, 29 us with silu, 20.5 us with no activation; HBM alone 10 us). gelu without
-// special functions, a polynomial, and with one reciprocal for two values measured the same: what they
-// save there they spend on multiply-adds. Backward: the tensor cores' reads of shared memory; a tile's 56
-// MMAs of N = 64 or 128 take some 85 cycles each, 4800 in all, which is a tile's period (58 us with gelu,
-// 55 us without).
+// What bounds them (262144 tokens, 64 channels, 128 hidden). Forward: a chunk's way from one stage to the next
+// (accumulator, activation, shared memory, second product; 30 us with gelu, 28 us with silu, 18 us with no activation;
+// HBM alone 10 us): the issue slots are 46 % busy, the tensor pipe 19 %, and the warps wait longest for tensor memory and barriers.
+// gelu without special functions, a polynomial, and with one reciprocal for two values measured the same. Backward: the
+// tensor cores' reads of shared memory; a tile's 56 MMAs of N = 64 or 128 take some 85 cycles each, 4800 in all, which is
+// a tile's period (with the sum of the CTAs' parts 58 us with gelu, 51 us without).
 
 #include "mlp.cuh"
 
@@ -148,6 +148,8 @@ struct Forward {
     static constexpr int kFixed = kXStages * kXBytes + 2 * kTileBytes + 2048;
     static constexpr int kYCols = DK * 64;
     static constexpr int smem(int chunks) { return kFixed + chunks * kChunkBytes; }
+    // Each CTA takes all of tensor memory: no second one fits an SM's 228 KiB beside it.
+    static_assert(2 * (kFixed + kChunkBytes) > 228 * 1024, "one CTA per SM");
 };
 
 template <class T, int Act, int CK, int DK>
@@ -390,6 +392,7 @@ constexpr int kBackStages = 3;
 constexpr int kBackChunkWeights = 3 * kWeightBytes;
 constexpr int kBackSmem = 2 * kBackStages * kTileBytes + 2 * kBackChunkWeights + 4 * kTileBytes + 2048;
 static_assert(kBackSmem <= kMaxSmem, "shared memory");
+static_assert(2 * kBackSmem > 228 * 1024, "one CTA per SM, which takes all of tensor memory");
 // Tensor memory columns.
 constexpr int kColDx = 192;        // two accumulators of 64
 constexpr int kColGateUp = 320;    // two chunks of 64

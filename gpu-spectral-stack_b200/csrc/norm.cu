@@ -21,14 +21,17 @@
 // Two-pass form: chunks of a sample's rows give partial results (means and squares about them, joined
 // block by block, so that neither a large mean nor an outlier cancels), a small kernel joins them, and
 // the outputs are computed from a second read, which runs backwards to meet what is still in L2.
-// Same array with gelu: 77 us forward (402 MB in three passes: 5.2 TB/s; 69 us with no activation), 136 us
-// backward (671 MB: 4.9 TB/s; 113 us), from an 8-bit checkpoint 165 us (103 us); float32 134 us (6.0 TB/s) and
-// 214 us (6.3 TB/s). What bounds the 16-bit types with gelu are its instructions, computed twice in the backward pass.
+// Same array with gelu, calls in a graph: 77 us forward (402 MB in three passes: 5.2 TB/s; 67 us with no activation),
+// 138 us backward (671 MB: 4.9 TB/s; 111 us), from an 8-bit checkpoint 169 us (100 us); float32 132 us (6.1 TB/s) and
+// 209 us (6.4 TB/s), from a checkpoint 201 us. What bounds the 16-bit types with gelu are its instructions, computed
+// twice in the backward pass: their kernels fill 61 to 71 % of the issue slots with a third of the warps.
 // Cutting the batch so that a part's second read stays in L2 measured slower at every cut (2 to 16
 // parts: 105 to 330 us forward, 180 to 470 us backward): each part pays its launches' ends.
 // Keeping the second read in L2, with persistent CTAs that take sum and apply tasks a few samples
 // apart, measured 97 us and 207 us: a sample's statistics take some 10 us from its last sum to its
 // first output (fences, atomics, flags), and at this bandwidth 65 MB pass in that time.
+//
+// Samples of a few values each are the weak side of both: a CTA each, whatever they hold (65536 x 16 x 64: 850 us).
 //
 // All sums are FP32; 16-bit types are widened when read and rounded once when written.
 

@@ -27,8 +27,9 @@ transposes, conjugations and per-column weights.
 
 The pointwise half (additions of this library) works on channels-last fields (b, ..., c), float32,
 bfloat16 or float16. Each layer keeps only its input for the backward pass; with checkpoint8=True
-it keeps that input in 8 bits (ops.pack8), a half or a quarter of the memory, and the gradients
-are those at the restored input.
+it keeps that input in 8 bits (ops.pack8), a half or a quarter of the memory. The feed-forward
+block's gradients are then those at the restored input; the norm's are its formula with the restored
+values under the mean and standard deviation of the original ones, which the forward pass keeps.
 """
 
 from __future__ import annotations

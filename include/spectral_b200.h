@@ -366,9 +366,10 @@ SPECTRAL_API int spectral_channels_last(const void* x, void* y, int dtype, long 
  *   y = (act(x w_gate^T) * (x w_up^T)) w_down^T
  * x (tokens, channels), w_gate and w_up (hidden, channels), w_down (outputs, hidden),
  * y (tokens, outputs), all of `dtype`. Products run on the tensor cores with FP32 accumulators;
- * FP32 operands are split into three bf16 parts (FP32-level error). In the 16-bit types the hidden
- * values (backward: also the gradients of both products) are rounded once to the type between the
- * products, and have its range: an FP16 hidden value beyond 65504 is infinite. */
+ * FP32 operands are split into three bf16 parts (FP32-level error; what an infinite operand enters
+ * is infinite or NaN). In the 16-bit types the hidden values (backward: also the gradients of both
+ * products) are rounded once to the type between the products, and have its range: an FP16 hidden
+ * value beyond 65504 is infinite. (Up to 8 tokens they stay in FP32.) */
 SPECTRAL_API int spectral_gated_mlp_workspace(int dtype, long long tokens, int channels, int hidden, int outputs,
                                               size_t* count);
 /* The same for the arrays a call will be given: smaller where they need no staging copy (16-bit values in rows of

@@ -568,3 +568,18 @@ def test_fno_block_at_its_own_size(dtype, tol):
     close(packed, want_y, tol)
     for g, w in zip(torch.autograd.grad(packed, [leaf, *params], up), got):
         close(g, w.double(), 0.05)
+
+
+@pytest.mark.gpu
+def test_mixed_types_are_refused_by_the_layers():
+    # The norm's parameters are float32 whatever the fields are; the feed-forward weights have the fields' type. Autocast casts neither.
+    x = torch.zeros(2, 3, 16, device="cuda")
+    with pytest.raises(RuntimeError, match="weight must be a float32"):
+        spectral.nn.GroupNormAct(4, 16, device="cuda").bfloat16()(x.bfloat16())
+    mlp = GatedMLP(16, 32, device="cuda")
+    with pytest.raises(RuntimeError, match="w_gate must be"):
+        mlp(x.bfloat16())
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert mlp(x).dtype == torch.float32
+        with pytest.raises(RuntimeError, match="w_gate must be"):
+            mlp(x.bfloat16())
