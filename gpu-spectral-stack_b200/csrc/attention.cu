@@ -1,0 +1,979 @@
+// Attention to states of another length: the C ABI (include/spectral_b200.h: spectral_cross_attention and
+// its backward), the float32 kernels, and the kernels around the 16-bit ones.
+//
+// Float32 products run on the CUDA cores: FP32 multiply-adds two to an instruction, tiles of rows x 64 keys,
+// operands staged through shared memory as float32 with what must not count as zeros. A pass over the keys keeps the
+// running maximum and sum of each row. The backward pass recomputes the scores twice, once for the
+// keys' gradients (a CTA per 64 keys, a loop over rows) and once for the queries' (a CTA per 64 rows, a loop over
+// keys): every sum has one owner, so nothing is atomic and equal inputs give equal bits.
+
+#include "attention.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace spectral::attention {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kKeys = 64;  // per tile
+
+// A tile of `Rows` rows of float32 in shared memory; the pitch keeps reads of 16 rows apart.
+template <int Dim>
+constexpr int kPitch = Dim + 4;
+constexpr int kScorePitch = kKeys + 4;
+
+// Rows [first, first + Rows) of queries (or of an array of their shape), zeros past the end.
+template <class T, int Dim, int Rows>
+__device__ __forceinline__ void load_rows(float* tile, const Call& c, const void* base, const Strides& s, int b, int head,
+                                          long long first)
+{
+    const T* p = static_cast<const T*>(base) + b * s.sample;
+    for (int i = threadIdx.x; i < Rows * Dim; i += kThreads) {
+        const int row = i / Dim, d = i - row * Dim;
+        const long long r = first + row;
+        float v = 0.0f;
+        if (r < c.rows() && d < c.dim) {
+            const long long t = r / c.group;
+            v = to_float(p[t * s.token + (head * c.group + (r - t * c.group)) * s.head + d]);
+        }
+        tile[row * kPitch<Dim> + d] = v;
+    }
+}
+
+// Keys [first, first + kKeys) of k or v, zeros where `valid` is not set.
+template <class T, int Dim>
+__device__ __forceinline__ void load_keys(float* tile, const Call& c, const void* base, const Strides& s, int b, int head,
+                                          long long first, unsigned long long valid)
+{
+    const T* p = static_cast<const T*>(base) + b * s.sample + head * s.head;
+    for (int i = threadIdx.x; i < kKeys * Dim; i += kThreads) {
+        const int key = i / Dim, d = i - key * Dim;
+        tile[key * kPitch<Dim> + d] = (valid >> key & 1) != 0 && d < c.dim ? to_float(p[(first + key) * s.token + d]) : 0.0f;
+    }
+}
+
+// One bit per key of the tile at `first` that counts (the same in every thread). `votes`: two words.
+__device__ __forceinline__ unsigned long long valid_keys(const Call& c, int b, int length, long long first, unsigned* votes)
+{
+    const int key = threadIdx.x;
+    __syncthreads();
+    if (key < kKeys) {
+        bool ok = first + key < length;
+        if (ok && c.mask != nullptr) {
+            ok = c.mask[static_cast<long long>(b) * c.keys + first + key] != 0;
+        }
+        const unsigned word = __ballot_sync(0xffffffffu, ok);
+        if ((key & 31) == 0) {
+            votes[key >> 5] = word;
+        }
+    }
+    __syncthreads();
+    return votes[0] | static_cast<unsigned long long>(votes[1]) << 32;
+}
+
+// R x 4 dot products over Dim: rows row0 .. of a, rows col + 16 j of b.
+template <int Dim, int R>
+__device__ __forceinline__ void products(const float* a, const float* b, int row0, int col, float (&out)[R][4])
+{
+    float2 acc[R][4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[i][j] = pair(0.0f);
+        }
+    }
+#pragma unroll 4
+    for (int d = 0; d < Dim; d += 4) {
+        float4 x[R], y[4];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            x[i] = *reinterpret_cast<const float4*>(a + (row0 + i) * kPitch<Dim> + d);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            y[j] = *reinterpret_cast<const float4*>(b + (col + 16 * j) * kPitch<Dim> + d);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[i][j] = fma2(make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y), acc[i][j]);
+                acc[i][j] = fma2(make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w), acc[i][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            out[i][j] = acc[i][j].x + acc[i][j].y;
+        }
+    }
+}
+
+// The pairs of values a thread holds of a row of Dim: p * 32 + 2 col and the next.
+template <int Dim>
+constexpr int kPairs = Dim / 32;
+
+// acc[i] += sum over keys of s[row0 + i][key] * m[key][its values].
+template <int Dim, int R>
+__device__ __forceinline__ void weigh_rows(const float* s, const float* m, int row0, int col, float2 (&acc)[R][kPairs<Dim>])
+{
+#pragma unroll 2
+    for (int key = 0; key < kKeys; key += 4) {
+        float4 w[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            w[i] = *reinterpret_cast<const float4*>(s + (row0 + i) * kScorePitch + key);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 v[kPairs<Dim>];
+#pragma unroll
+            for (int p = 0; p < kPairs<Dim>; ++p) {
+                v[p] = *reinterpret_cast<const float2*>(m + (key + j) * kPitch<Dim> + p * 32 + 2 * col);
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const float f = j == 0 ? w[i].x : j == 1 ? w[i].y : j == 2 ? w[i].z : w[i].w;
+#pragma unroll
+                for (int p = 0; p < kPairs<Dim>; ++p) {
+                    acc[i][p] = fma2(pair(f), v[p], acc[i][p]);
+                }
+            }
+        }
+    }
+}
+
+// acc[i] += sum over rows of s[row][key0 + i] * m[row][its values], four keys.
+template <int Dim, int Rows>
+__device__ __forceinline__ void weigh_keys(const float* s, const float* m, int key0, int col, float2 (&acc)[4][kPairs<Dim>])
+{
+#pragma unroll 4
+    for (int row = 0; row < Rows; ++row) {
+        const float4 w = *reinterpret_cast<const float4*>(s + row * kScorePitch + key0);
+#pragma unroll
+        for (int p = 0; p < kPairs<Dim>; ++p) {
+            const float2 v = *reinterpret_cast<const float2*>(m + row * kPitch<Dim> + p * 32 + 2 * col);
+            acc[0][p] = fma2(pair(w.x), v, acc[0][p]);
+            acc[1][p] = fma2(pair(w.y), v, acc[1][p]);
+            acc[2][p] = fma2(pair(w.z), v, acc[2][p]);
+            acc[3][p] = fma2(pair(w.w), v, acc[3][p]);
+        }
+    }
+}
+
+template <class T, int Dim>
+__device__ __forceinline__ void store_pairs(T* p, int dim, int col, const float2 (&v)[kPairs<Dim>], float factor)
+{
+#pragma unroll
+    for (int j = 0; j < kPairs<Dim>; ++j) {
+        const int d = j * 32 + 2 * col;
+        if (d < dim) {
+            p[d] = from_float<T>(v[j].x * factor);
+        }
+        if (d + 1 < dim) {
+            p[d + 1] = from_float<T>(v[j].y * factor);
+        }
+    }
+}
+
+__device__ __forceinline__ float lanes16_max(float v)
+{
+#pragma unroll
+    for (int o = 8; o > 0; o /= 2) {
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    return v;
+}
+__device__ __forceinline__ float lanes16_sum(float v)
+{
+#pragma unroll
+    for (int o = 8; o > 0; o /= 2) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+
+// Where a kernel's results go: the call's arrays, or float32 parts of them.
+struct Parts {
+    int count = 1;
+    long long span = 0;       // keys (forward, dq) or rows (dk, dv) of a part
+    float* first = nullptr;   // sum p v, dq or dk: (part, pair, row, dim)
+    float* second = nullptr;  // dv
+    float2* stats = nullptr;  // forward: (part, pair, row)
+};
+
+// Forward: 16 R rows per CTA, thread (row group, column) of a 16 x 16 grid.
+template <class T, int Dim, int R>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const Parts parts)
+{
+    constexpr int kRows = 16 * R;
+    extern __shared__ __align__(16) float shared[];
+    float* sq = shared;
+    float* sk = sq + kRows * kPitch<Dim>;
+    float* sv = sk + kKeys * kPitch<Dim>;
+    float* sp = sv + kKeys * kPitch<Dim>;
+    __shared__ unsigned votes[2];
+    const int col = threadIdx.x & 15;
+    const int row0 = (threadIdx.x >> 4) * R;
+    const long long at = blockIdx.y;
+    const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
+    const long long first = static_cast<long long>(blockIdx.x) * kRows;
+    const int part = blockIdx.z;
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int length = length_of(c, b);
+    const long long begin = part * parts.span;
+    const long long end = min(static_cast<long long>(length), begin + parts.span);
+    load_rows<T, Dim, kRows>(sq, c, c.q, c.qs, b, head, first);
+    const float scale = c.scale * kLog2e;
+    float most[R], total[R];
+    float2 acc[R][kPairs<Dim>];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        most[i] = -INFINITY;
+        total[i] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < kPairs<Dim>; ++p) {
+            acc[i][p] = pair(0.0f);
+        }
+    }
+    for (long long key0 = begin; key0 < end; key0 += kKeys) {
+        const unsigned long long valid = valid_keys(c, b, static_cast<int>(end), key0, votes);
+        if (valid == 0) {
+            continue;
+        }
+        load_keys<T, Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
+        load_keys<T, Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+        __syncthreads();
+        float s[R][4];
+        products<Dim, R>(sq, sk, row0, col, s);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = (valid >> (col + 16 * j) & 1) != 0 ? s[i][j] * scale : -INFINITY;
+                m = fmaxf(m, s[i][j]);
+            }
+            m = fmaxf(most[i], lanes16_max(m));
+            const float base = m == -INFINITY ? 0.0f : m;
+            const float keep = exp2f(most[i] - base);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(s[i][j] - base);
+                sum += p;
+                sp[(row0 + i) * kScorePitch + col + 16 * j] = p;
+            }
+            most[i] = m;
+            total[i] = total[i] * keep + lanes16_sum(sum);
+#pragma unroll
+            for (int p = 0; p < kPairs<Dim>; ++p) {
+                acc[i][p] = acc[i][p] * pair(keep);
+            }
+        }
+        __syncwarp();  // a row's scores are written and read by one warp
+        weigh_rows<Dim, R>(sp, sv, row0, col, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const long long r = first + row0 + i;
+        if (r >= c.rows()) {
+            continue;
+        }
+        const float base = most[i] == -INFINITY ? 0.0f : most[i];
+        if (parts.count == 1) {
+            store_pairs<T, Dim>(static_cast<T*>(c.out) + c.row_at(b, head, r), c.dim, col, acc[i], total[i] == 0.0f ? 0.0f : 1.0f / total[i]);
+            if (c.stats != nullptr && col == 0) {
+                c.stats[at * c.rows() + r] = make_float2(base, total[i]);
+            }
+        } else {
+            const long long to = (part * c.pairs() + at) * c.rows() + r;
+            store_pairs<float, Dim>(parts.first + to * c.dim, c.dim, col, acc[i], 1.0f);
+            if (col == 0) {
+                parts.stats[to] = make_float2(most[i], total[i]);
+            }
+        }
+    }
+}
+
+// Scores of a tile, turned into p and p (dp - delta): what both backward kernels need.
+template <int Dim>
+__device__ __forceinline__ void score_gradients(const float* sq, const float* sk, const float* sv, const float* sdo, int row0, int col,
+                                                float scale, unsigned long long valid, const float2 (&stats)[4], const float (&delta)[4],
+                                                float (&p)[4][4], float (&ds)[4][4])
+{
+    products<Dim, 4>(sq, sk, row0, col, p);
+    products<Dim, 4>(sdo, sv, row0, col, ds);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool ok = (valid >> (col + 16 * j) & 1) != 0;
+            p[i][j] = ok ? exp2f(p[i][j] * scale - stats[i].x) * stats[i].y : 0.0f;
+            ds[i][j] = ok ? p[i][j] * (ds[i][j] - delta[i]) : 0.0f;
+        }
+    }
+}
+
+// m and 1 / sum p, and delta, of rows row0 .. of the tile at `first`; zeros past the end and for empty rows.
+__device__ __forceinline__ void row_constants(const Call& c, long long at, long long first, int row0, float2 (&stats)[4], float (&delta)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long r = first + row0 + i;
+        stats[i] = make_float2(0.0f, 0.0f);
+        delta[i] = 0.0f;
+        if (r < c.rows()) {
+            const float2 s = c.stats[at * c.rows() + r];
+            stats[i] = make_float2(s.x, s.y == 0.0f ? 0.0f : 1.0f / s.y);
+            delta[i] = c.delta[at * c.rows() + r];
+        }
+    }
+}
+
+template <class T, int Dim>
+__global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, const Parts parts)
+{
+    extern __shared__ __align__(16) float shared[];
+    float* sk = shared;
+    float* sv = sk + kKeys * kPitch<Dim>;
+    float* sq = sv + kKeys * kPitch<Dim>;
+    float* sdo = sq + 64 * kPitch<Dim>;
+    float* sp = sdo + 64 * kPitch<Dim>;
+    float* sds = sp + 64 * kScorePitch;
+    __shared__ unsigned votes[2];
+    const int col = threadIdx.x & 15;
+    const int row0 = (threadIdx.x >> 4) * 4;
+    const long long at = blockIdx.y;
+    const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
+    const long long key0 = static_cast<long long>(blockIdx.x) * kKeys;
+    const int part = blockIdx.z;
+    allow_next_grid();
+    wait_for_previous_grid();
+    const unsigned long long valid = valid_keys(c, b, length_of(c, b), key0, votes);
+    load_keys<T, Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
+    load_keys<T, Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+    const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
+                        c.dim};
+    float2 dk[4][kPairs<Dim>], dv[4][kPairs<Dim>];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int p = 0; p < kPairs<Dim>; ++p) {
+            dk[i][p] = pair(0.0f);
+            dv[i][p] = pair(0.0f);
+        }
+    }
+    const long long end = min(c.rows(), (part + 1) * parts.span);
+    for (long long first = part * parts.span; first < end && valid != 0; first += 64) {
+        __syncthreads();
+        load_rows<T, Dim, 64>(sq, c, c.q, c.qs, b, head, first);
+        load_rows<T, Dim, 64>(sdo, c, c.dout, dense, b, head, first);
+        float2 stats[4];
+        float delta[4], p[4][4], ds[4][4];
+        row_constants(c, at, first, row0, stats, delta);
+        __syncthreads();
+        score_gradients<Dim>(sq, sk, sv, sdo, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sp[(row0 + i) * kScorePitch + col + 16 * j] = p[i][j];
+                sds[(row0 + i) * kScorePitch + col + 16 * j] = ds[i][j];
+            }
+        }
+        __syncthreads();
+        weigh_keys<Dim, 64>(sp, sdo, row0, col, dv);
+        weigh_keys<Dim, 64>(sds, sq, row0, col, dk);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long key = key0 + row0 + i;
+        if (key >= c.keys) {
+            continue;
+        }
+        if (parts.count == 1) {
+            const long long to = ((static_cast<long long>(b) * c.keys + key) * c.kv_heads + head) * c.dim;
+            store_pairs<T, Dim>(static_cast<T*>(c.dk) + to, c.dim, col, dk[i], c.scale);
+            store_pairs<T, Dim>(static_cast<T*>(c.dv) + to, c.dim, col, dv[i], 1.0f);
+        } else {
+            const long long to = ((part * c.pairs() + at) * c.keys + key) * c.dim;
+            store_pairs<float, Dim>(parts.first + to, c.dim, col, dk[i], 1.0f);
+            store_pairs<float, Dim>(parts.second + to, c.dim, col, dv[i], 1.0f);
+        }
+    }
+}
+
+template <class T, int Dim>
+__global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, const Parts parts)
+{
+    extern __shared__ __align__(16) float shared[];
+    float* sk = shared;
+    float* sv = sk + kKeys * kPitch<Dim>;
+    float* sq = sv + kKeys * kPitch<Dim>;
+    float* sdo = sq + 64 * kPitch<Dim>;
+    float* sds = sdo + 64 * kPitch<Dim>;
+    __shared__ unsigned votes[2];
+    const int col = threadIdx.x & 15;
+    const int row0 = (threadIdx.x >> 4) * 4;
+    const long long at = blockIdx.y;
+    const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
+    const long long first = static_cast<long long>(blockIdx.x) * 64;
+    const int part = blockIdx.z;
+    allow_next_grid();
+    wait_for_previous_grid();
+    const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
+                        c.dim};
+    load_rows<T, Dim, 64>(sq, c, c.q, c.qs, b, head, first);
+    load_rows<T, Dim, 64>(sdo, c, c.dout, dense, b, head, first);
+    float2 stats[4];
+    float delta[4];
+    row_constants(c, at, first, row0, stats, delta);
+    float2 dq[4][kPairs<Dim>];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int p = 0; p < kPairs<Dim>; ++p) {
+            dq[i][p] = pair(0.0f);
+        }
+    }
+    const long long begin = part * parts.span;
+    const long long end = min(static_cast<long long>(length_of(c, b)), begin + parts.span);
+    for (long long key0 = begin; key0 < end; key0 += kKeys) {
+        const unsigned long long valid = valid_keys(c, b, static_cast<int>(end), key0, votes);
+        if (valid == 0) {
+            continue;
+        }
+        load_keys<T, Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
+        load_keys<T, Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+        __syncthreads();
+        float p[4][4], ds[4][4];
+        score_gradients<Dim>(sq, sk, sv, sdo, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sds[(row0 + i) * kScorePitch + col + 16 * j] = ds[i][j];
+            }
+        }
+        __syncwarp();
+        weigh_rows<Dim, 4>(sds, sk, row0, col, dq);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long r = first + row0 + i;
+        if (r >= c.rows()) {
+            continue;
+        }
+        if (parts.count == 1) {
+            store_pairs<T, Dim>(static_cast<T*>(c.dq) + c.row_at(b, head, r), c.dim, col, dq[i], c.scale);
+        } else {
+            const long long to = ((part * c.pairs() + at) * c.rows() + r) * c.dim;
+            store_pairs<float, Dim>(parts.first + to, c.dim, col, dq[i], 1.0f);
+        }
+    }
+}
+
+// --- around them -------------------------------------------------------------------------------------
+
+// A warp per row.
+template <class T>
+__global__ void __launch_bounds__(kThreads) row_products_kernel(const Call c)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int lane = threadIdx.x & 31;
+    const long long all = static_cast<long long>(c.batch) * c.queries * c.kv_heads * c.group;
+    const T* __restrict__ o = static_cast<const T*>(c.out);
+    const T* __restrict__ g = static_cast<const T*>(c.dout);
+    for (long long i = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); i < all;
+         i += static_cast<long long>(gridDim.x) * (kThreads / 32)) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < SPECTRAL_HEAD_DIM_MAX / 32; ++k) {
+            const int d = lane + 32 * k;
+            if (d < c.dim) {
+                sum = fmaf(to_float(o[i * c.dim + d]), to_float(g[i * c.dim + d]), sum);
+            }
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s /= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        }
+        if (lane == 0) {
+            // (sample, token, head) to (sample, key head, row).
+            const int heads = c.kv_heads * c.group;
+            const long long token = i / heads;  // of all samples
+            const int h = static_cast<int>(i - token * heads);
+            const long long b = token / c.queries;
+            const int kv = h / c.group;
+            c.delta[(b * c.kv_heads + kv) * c.rows() + (token - b * c.queries) * c.group + (h - kv * c.group)] = sum;
+        }
+    }
+}
+
+// A thread per result value.
+template <class T>
+__global__ void __launch_bounds__(kThreads) add_parts_kernel(const Call c, const float* __restrict__ partial, int parts, bool of_keys,
+                                                             void* result, float factor)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const long long count = of_keys ? c.keys : c.rows();
+    const long long all = c.pairs() * count * c.dim;
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * kThreads) {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            sum += partial[p * all + i];
+        }
+        const long long row = i / c.dim;
+        const int d = static_cast<int>(i - row * c.dim);
+        const long long at = row / count;
+        const long long r = row - at * count;
+        const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
+        const long long to = of_keys ? ((static_cast<long long>(b) * c.keys + r) * c.kv_heads + head) * c.dim : c.row_at(b, head, r);
+        static_cast<T*>(result)[to + d] = from_float<T>(sum * factor);
+    }
+}
+
+// A warp per row.
+template <class T>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Call c, const float* __restrict__ partial, const float2* __restrict__ stats,
+                                                        int splits)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int lane = threadIdx.x & 31;
+    const long long all = c.pairs() * c.rows();
+    for (long long i = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); i < all;
+         i += static_cast<long long>(gridDim.x) * (kThreads / 32)) {
+        float most = -INFINITY;
+        for (int s = lane; s < splits; s += 32) {
+            most = fmaxf(most, stats[s * all + i].x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        const float base = most == -INFINITY ? 0.0f : most;
+        float total = 0.0f;
+        float acc[SPECTRAL_HEAD_DIM_MAX / 32] = {};
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const float2 st = stats[s * all + i];
+            const float w = exp2f(st.x - base);
+            total = fmaf(st.y, w, total);
+#pragma unroll
+            for (int k = 0; k < SPECTRAL_HEAD_DIM_MAX / 32; ++k) {
+                const int d = lane + 32 * k;
+                if (d < c.dim) {
+                    acc[k] = fmaf(partial[(s * all + i) * c.dim + d], w, acc[k]);
+                }
+            }
+        }
+        const long long at = i / c.rows();
+        const long long r = i - at * c.rows();
+        const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+        T* out = static_cast<T*>(c.out) + c.row_at(b, head, r);
+#pragma unroll
+        for (int k = 0; k < SPECTRAL_HEAD_DIM_MAX / 32; ++k) {
+            const int d = lane + 32 * k;
+            if (d < c.dim) {
+                out[d] = from_float<T>(acc[k] * f);
+            }
+        }
+        if (c.stats != nullptr && lane == 0) {
+            c.stats[i] = make_float2(base, total);
+        }
+    }
+}
+
+}  // namespace
+
+void add_parts(const Call& c, const float* partial, int parts, bool of_keys, void* result, float factor, cudaStream_t stream)
+{
+    const long long all = c.pairs() * (of_keys ? c.keys : c.rows()) * c.dim;
+    const auto grid = static_cast<unsigned>(std::min<long long>((all + kThreads - 1) / kThreads, 148 * 16));
+    with_dtype(c.dtype, [&](auto t) {
+        launch_pdl(add_parts_kernel<decltype(t)>, dim3(grid), dim3(kThreads), 0, stream, c, partial, parts, of_keys, result, factor);
+    });
+}
+
+void join_splits(const Call& c, const float* partial, const float2* stats, int splits, cudaStream_t stream)
+{
+    const auto grid = static_cast<unsigned>(std::min<long long>((c.pairs() * c.rows() + 7) / 8, 148 * 16));
+    with_dtype(c.dtype, [&](auto t) {
+        launch_pdl(join_kernel<decltype(t)>, dim3(grid), dim3(kThreads), 0, stream, c, partial, stats, splits);
+    });
+}
+
+void row_products(const Call& c, cudaStream_t stream)
+{
+    const auto grid = static_cast<unsigned>(std::min<long long>((c.pairs() * c.rows() + 7) / 8, 148 * 16));
+    with_dtype(c.dtype, [&](auto t) { launch_pdl(row_products_kernel<decltype(t)>, dim3(grid), dim3(kThreads), 0, stream, c); });
+}
+
+namespace {
+
+constexpr int kSms = 148;
+
+// Calls f(integral_constant<Dim>) with the padded head size.
+template <class F>
+void with_dim(int dim, F&& f)
+{
+    if (dim <= 32) {
+        f(std::integral_constant<int, 32>{});
+    } else if (dim <= 64) {
+        f(std::integral_constant<int, 64>{});
+    } else {
+        f(std::integral_constant<int, 128>{});
+    }
+}
+
+// Rows per forward CTA: 64, or 16 where there are no more (a single query's rows).
+int forward_rows(const Call& c) { return c.rows() <= 16 ? 16 : 64; }
+
+// Parts of an axis of `length` in tiles of 64, so that `tiles` CTAs per part fill the GPU about twice; a part's
+// span is a whole number of tiles.
+Parts split(long long tiles, long long length)
+{
+    Parts p;
+    const long long all = pieces(length, 64);
+    const long long wanted = std::max(1LL, std::min({all, (2LL * kSms + tiles - 1) / tiles, 256LL}));
+    p.span = (all + wanted - 1) / wanted * 64;
+    p.count = static_cast<int>(std::max(1LL, (length + p.span - 1) / std::max(1LL, p.span)));
+    return p;
+}
+
+struct ForwardPlan {
+    Parts parts;
+    Arena arena;
+    std::size_t partial = 0, stats = 0;
+
+    explicit ForwardPlan(const Call& c)
+    {
+        parts = split(c.pairs() * pieces(c.rows(), forward_rows(c)), c.keys);
+        if (parts.count > 1) {
+            const std::size_t rows = static_cast<std::size_t>(c.pairs()) * c.rows() * parts.count;
+            partial = arena.take(rows * c.dim * sizeof(float));
+            stats = arena.take(rows * sizeof(float2));
+        }
+    }
+};
+
+struct BackwardPlan {
+    Parts of_rows, of_keys;
+    Arena arena;
+    std::size_t delta = 0, dq = 0, dk = 0, dv = 0;
+
+    explicit BackwardPlan(const Call& c)
+    {
+        const std::size_t rows = static_cast<std::size_t>(c.pairs()) * c.rows();
+        const std::size_t keys = static_cast<std::size_t>(c.pairs()) * c.keys;
+        delta = arena.take(rows * sizeof(float));
+        of_keys = split(c.pairs() * pieces(c.rows(), 64), c.keys);
+        of_rows = split(c.pairs() * pieces(c.keys, 64), c.rows());
+        if (of_keys.count > 1) {
+            dq = arena.take(rows * c.dim * of_keys.count * sizeof(float));
+        }
+        if (of_rows.count > 1) {
+            dk = arena.take(keys * c.dim * of_rows.count * sizeof(float));
+            dv = arena.take(keys * c.dim * of_rows.count * sizeof(float));
+        }
+    }
+};
+
+template <class K, class... A>
+void launch(K kernel, dim3 grid, std::size_t smem, cudaStream_t stream, const A&... args)
+{
+    if (smem > 48 * 1024) {
+        SPECTRAL_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    }
+    launch_pdl(kernel, grid, dim3(kThreads), smem, stream, args...);
+}
+
+template <class T>
+void forward(const Call& c, char* work, cudaStream_t stream)
+{
+    ForwardPlan plan(c);
+    plan.parts.first = reinterpret_cast<float*>(work + plan.partial);
+    plan.parts.stats = reinterpret_cast<float2*>(work + plan.stats);
+    const int rows = forward_rows(c);
+    const dim3 grid(pieces(c.rows(), rows), static_cast<unsigned>(c.pairs()), plan.parts.count);
+    with_dim(c.dim, [&](auto d) {
+        constexpr int Dim = decltype(d)::value;
+        const std::size_t smem = ((rows + 2 * kKeys) * kPitch<Dim> + rows * kScorePitch) * sizeof(float);
+        if (rows == 16) {
+            launch(forward_kernel<T, Dim, 1>, grid, smem, stream, c, plan.parts);
+        } else {
+            launch(forward_kernel<T, Dim, 4>, grid, smem, stream, c, plan.parts);
+        }
+    });
+    if (plan.parts.count > 1) {
+        join_splits(c, plan.parts.first, plan.parts.stats, plan.parts.count, stream);
+    }
+}
+
+template <class T>
+void backward(Call c, char* work, cudaStream_t stream)
+{
+    BackwardPlan plan(c);
+    c.delta = reinterpret_cast<float*>(work + plan.delta);
+    plan.of_keys.first = reinterpret_cast<float*>(work + plan.dq);
+    plan.of_rows.first = reinterpret_cast<float*>(work + plan.dk);
+    plan.of_rows.second = reinterpret_cast<float*>(work + plan.dv);
+    row_products(c, stream);
+    with_dim(c.dim, [&](auto d) {
+        constexpr int Dim = decltype(d)::value;
+        const std::size_t tiles = 4 * 64 * kPitch<Dim> * sizeof(float);
+        constexpr std::size_t kScores = 64 * kScorePitch * sizeof(float);
+        launch(keys_backward_kernel<T, Dim>, dim3(pieces(c.keys, 64), static_cast<unsigned>(c.pairs()), plan.of_rows.count), tiles + 2 * kScores, stream,
+               c, plan.of_rows);
+        launch(rows_backward_kernel<T, Dim>, dim3(pieces(c.rows(), 64), static_cast<unsigned>(c.pairs()), plan.of_keys.count), tiles + kScores, stream, c,
+               plan.of_keys);
+    });
+    if (plan.of_rows.count > 1) {
+        add_parts(c, plan.of_rows.first, plan.of_rows.count, true, c.dk, c.scale, stream);
+        add_parts(c, plan.of_rows.second, plan.of_rows.count, true, c.dv, 1.0f, stream);
+    }
+    if (plan.of_keys.count > 1) {
+        add_parts(c, plan.of_keys.first, plan.of_keys.count, false, c.dq, c.scale, stream);
+    }
+}
+
+int invalid(const std::string& message)
+{
+    set_last_error(message);
+    return SPECTRAL_INVALID_ARGUMENT;
+}
+
+// Sizes into `c`; strides may be NULL (contiguous arrays).
+int sizes(const char* op, Call& c, const long long* strides, int dtype, long long batch, long long queries, long long keys, int heads,
+          int kv_heads, int dim)
+{
+    const std::string name(op);
+    if (!dtype_known(dtype)) {
+        return invalid(name + ": dtype must be SPECTRAL_FLOAT32, SPECTRAL_BFLOAT16 or SPECTRAL_FLOAT16");
+    }
+    if (dim < 1 || dim > SPECTRAL_HEAD_DIM_MAX) {
+        return invalid(name + ": need 1 <= dim <= " + std::to_string(SPECTRAL_HEAD_DIM_MAX));
+    }
+    if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0) {
+        return invalid(name + ": heads must be a multiple of kv_heads, both at least 1");
+    }
+    if (heads / kv_heads > 128) {
+        return invalid(name + ": at most 128 query heads may share a head of k and v");
+    }
+    constexpr long long kMost = (1LL << 31) - 256;
+    if (batch < 0 || queries < 0 || keys < 0 || keys > kMost || queries > kMost / (heads / kv_heads) || batch > 65535 / kv_heads) {
+        return invalid(name + ": need batch * kv_heads <= 65535, and keys and queries * heads / kv_heads below 2^31 - 256");
+    }
+    c.dtype = dtype;
+    c.batch = static_cast<int>(batch);
+    c.queries = static_cast<int>(queries);
+    c.keys = static_cast<int>(keys);
+    c.kv_heads = kv_heads;
+    c.group = heads / kv_heads;
+    c.dim = dim;
+    const long long d = dim;
+    c.qs = {queries * heads * d, heads * d, d};
+    c.ks = {keys * kv_heads * d, kv_heads * d, d};
+    c.vs = c.ks;
+    if (strides != nullptr) {
+        c.qs = {strides[0], strides[1], strides[2]};
+        c.ks = {strides[3], strides[4], strides[5]};
+        c.vs = {strides[6], strides[7], strides[8]};
+    }
+    return SPECTRAL_OK;
+}
+
+// Whether a contiguous result of `bytes` at `out` shares memory with a strided input.
+bool overlaps(const void* out, unsigned long long bytes, const void* in, const Strides& s, const long long (&extent)[3], int dim, std::size_t size)
+{
+    long long low = 0, high = dim - 1;
+    const long long step[3] = {s.sample, s.token, s.head};
+    for (int i = 0; i < 3; ++i) {
+        (step[i] < 0 ? low : high) += step[i] * (extent[i] - 1);
+    }
+    const auto o = reinterpret_cast<unsigned long long>(out), p = reinterpret_cast<unsigned long long>(in);
+    return p + low * static_cast<long long>(size) < o + bytes && o < p + (high + 1) * static_cast<long long>(size);
+}
+
+}  // namespace
+}  // namespace spectral::attention
+
+extern "C" int spectral_cross_attention_workspace(const void* q, const void* k, const void* v, const long long* strides, int dtype,
+                                                  long long batch, long long queries, long long keys, int heads, int kv_heads, int dim,
+                                                  size_t* count)
+{
+    using namespace spectral;
+    using namespace spectral::attention;
+    Call c;
+    const int status = sizes("cross_attention_workspace", c, strides, dtype, batch, queries, keys, heads, kv_heads, dim);
+    if (status != SPECTRAL_OK || count == nullptr) {
+        return status != SPECTRAL_OK ? status : invalid("cross_attention_workspace: null count");
+    }
+    c.q = q;
+    c.k = k;
+    c.v = v;
+    *count = 0;
+    if (c.pairs() * c.rows() > 0) {
+        *count = ForwardPlan(c).arena.size() / 8;
+    }
+    return SPECTRAL_OK;
+}
+
+extern "C" int spectral_cross_attention(const void* q, const void* k, const void* v, const long long* strides, const void* lengths,
+                                        int lengths64, const void* mask, void* out, float* stats, int dtype, long long batch,
+                                        long long queries, long long keys, int heads, int kv_heads, int dim, float scale, void* work,
+                                        void* stream)
+{
+    using namespace spectral;
+    using namespace spectral::attention;
+    Call c;
+    const int status = sizes("cross_attention", c, strides, dtype, batch, queries, keys, heads, kv_heads, dim);
+    if (status != SPECTRAL_OK) {
+        return status;
+    }
+    if (c.pairs() * c.rows() == 0) {
+        return SPECTRAL_OK;
+    }
+    const std::size_t size = dtype_size(dtype);
+    if (q == nullptr || out == nullptr || (keys > 0 && (k == nullptr || v == nullptr))) {
+        return invalid("cross_attention: null array");
+    }
+    for (const void* p : {q, k, v, static_cast<const void*>(out)}) {
+        if (!aligned_to(p, size)) {
+            return invalid("cross_attention: arrays must be aligned to their element size");
+        }
+    }
+    if (!aligned_to(stats, 8) || !aligned_to(lengths, lengths64 != 0 ? 8 : 4) || !aligned_to(work, 8)) {
+        return invalid("cross_attention: stats and work must be 8-byte aligned, lengths to their element size");
+    }
+    c.q = q;
+    c.k = k;
+    c.v = v;
+    const unsigned long long bytes = static_cast<unsigned long long>(batch) * queries * heads * dim * size;
+    const long long of_q[3] = {batch, queries, heads}, of_k[3] = {batch, keys, kv_heads};
+    if (overlaps(out, bytes, q, c.qs, of_q, dim, size)
+        || (keys > 0 && (overlaps(out, bytes, k, c.ks, of_k, dim, size) || overlaps(out, bytes, v, c.vs, of_k, dim, size)))) {
+        return invalid("cross_attention: out must not overlap q, k or v");
+    }
+    c.lengths = lengths;
+    c.lengths64 = lengths64;
+    c.mask = static_cast<const unsigned char*>(mask);
+    c.out = out;
+    c.stats = reinterpret_cast<float2*>(stats);
+    c.scale = scale;
+    try {
+        if (work == nullptr && ForwardPlan(c).arena.size() > 0) {
+            return invalid("cross_attention: needs a workspace");
+        }
+        with_dtype(dtype, [&](auto t) { forward<decltype(t)>(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream)); });
+        return SPECTRAL_OK;
+    } catch (const InvalidArgument& e) {
+        return invalid(e.what());
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return SPECTRAL_CUDA_ERROR;
+    }
+}
+
+extern "C" int spectral_cross_attention_backward_workspace(const void* q, const void* k, const void* v, const long long* strides, int dtype,
+                                                           long long batch, long long queries, long long keys, int heads, int kv_heads,
+                                                           int dim, size_t* count)
+{
+    using namespace spectral;
+    using namespace spectral::attention;
+    Call c;
+    const int status = sizes("cross_attention_backward_workspace", c, strides, dtype, batch, queries, keys, heads, kv_heads, dim);
+    if (status != SPECTRAL_OK || count == nullptr) {
+        return status != SPECTRAL_OK ? status : invalid("cross_attention_backward_workspace: null count");
+    }
+    c.q = q;
+    c.k = k;
+    c.v = v;
+    *count = 0;
+    if (c.pairs() * c.rows() > 0 && keys > 0) {
+        *count = BackwardPlan(c).arena.size() / 8;
+    }
+    return SPECTRAL_OK;
+}
+
+extern "C" int spectral_cross_attention_backward(const void* dout, const void* q, const void* k, const void* v, const long long* strides,
+                                                 const void* out, const float* stats, const void* lengths, int lengths64, const void* mask,
+                                                 void* dq, void* dk, void* dv, int dtype, long long batch, long long queries, long long keys,
+                                                 int heads, int kv_heads, int dim, float scale, void* work, void* stream)
+{
+    using namespace spectral;
+    using namespace spectral::attention;
+    Call c;
+    const int status = sizes("cross_attention_backward", c, strides, dtype, batch, queries, keys, heads, kv_heads, dim);
+    if (status != SPECTRAL_OK) {
+        return status;
+    }
+    const std::size_t size = dtype_size(dtype);
+    const unsigned long long q_bytes = static_cast<unsigned long long>(batch) * queries * heads * dim * size;
+    const unsigned long long k_bytes = static_cast<unsigned long long>(batch) * keys * kv_heads * dim * size;
+    if ((q_bytes > 0 && dq == nullptr) || (k_bytes > 0 && (dk == nullptr || dv == nullptr))) {
+        return invalid("cross_attention_backward: null array");
+    }
+    const auto s = static_cast<cudaStream_t>(stream);
+    try {
+        if (q_bytes == 0 || k_bytes == 0) {  // nothing attends, or to nothing
+            for (const auto& z : {std::pair<void*, unsigned long long>{dq, q_bytes}, {dk, k_bytes}, {dv, k_bytes}}) {
+                if (z.second > 0) {
+                    SPECTRAL_CUDA(cudaMemsetAsync(z.first, 0, z.second, s));
+                }
+            }
+            return SPECTRAL_OK;
+        }
+        if (dout == nullptr || q == nullptr || k == nullptr || v == nullptr || out == nullptr || stats == nullptr || work == nullptr) {
+            return invalid("cross_attention_backward: null array");
+        }
+        for (const void* p : {dout, q, k, v, out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)}) {
+            if (!aligned_to(p, size)) {
+                return invalid("cross_attention_backward: arrays must be aligned to their element size");
+            }
+        }
+        if (!aligned_to(stats, 8) || !aligned_to(lengths, lengths64 != 0 ? 8 : 4) || !aligned_to(work, 8)) {
+            return invalid("cross_attention_backward: stats and work must be 8-byte aligned, lengths to their element size");
+        }
+        const long long of_q[3] = {batch, queries, heads}, of_k[3] = {batch, keys, kv_heads};
+        const Strides dense{static_cast<long long>(queries) * heads * dim, static_cast<long long>(heads) * dim, dim};
+        for (const auto& z : {std::pair<void*, unsigned long long>{dq, q_bytes}, {dk, k_bytes}, {dv, k_bytes}}) {
+            if (overlaps(z.first, z.second, q, c.qs, of_q, dim, size) || overlaps(z.first, z.second, k, c.ks, of_k, dim, size)
+                || overlaps(z.first, z.second, v, c.vs, of_k, dim, size) || overlaps(z.first, z.second, dout, dense, of_q, dim, size)
+                || overlaps(z.first, z.second, out, dense, of_q, dim, size)) {
+                return invalid("cross_attention_backward: a gradient must not overlap dout, q, k, v or out");
+            }
+        }
+        c.q = q;
+        c.k = k;
+        c.v = v;
+        c.lengths = lengths;
+        c.lengths64 = lengths64;
+        c.mask = static_cast<const unsigned char*>(mask);
+        c.out = const_cast<void*>(out);
+        c.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+        c.dout = dout;
+        c.dq = dq;
+        c.dk = dk;
+        c.dv = dv;
+        c.scale = scale;
+        with_dtype(dtype, [&](auto t) { backward<decltype(t)>(c, static_cast<char*>(work), s); });
+        return SPECTRAL_OK;
+    } catch (const InvalidArgument& e) {
+        return invalid(e.what());
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return SPECTRAL_CUDA_ERROR;
+    }
+}

@@ -1,0 +1,99 @@
+#pragma once
+
+// What the attention kernels share: the call's arrays and sizes, which keys count, and the joining of
+// results that were split over an axis.
+//
+// out = softmax(scale q k^T) v, with the rows of a key head's queries side by side: `group` = heads / kv_heads query
+// heads read the same keys and values, and row r = token * group + (head in the group) of `rows` = queries * group.
+// Scores are taken in base 2: p = 2^(c s - m), c = scale log2(e), m the row's largest c s (or an earlier one),
+// out = sum p v / sum p. A row without keys has sum p = 0 and the result 0.
+
+#include "../../include/spectral_b200.h"
+
+#include "backend.hpp"
+#include "launch.cuh"
+#include "pointwise.cuh"
+
+namespace spectral::attention {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Strides {
+    long long sample = 0;
+    long long token = 0;
+    long long head = 0;
+};
+
+struct Call {
+    const void* q = nullptr;
+    const void* k = nullptr;
+    const void* v = nullptr;
+    Strides qs, ks, vs;
+    const void* lengths = nullptr;
+    int lengths64 = 0;
+    const unsigned char* mask = nullptr;
+    void* out = nullptr;       // (batch, queries, heads, dim)
+    float2* stats = nullptr;   // (batch, kv_heads, rows): m and sum p; NULL: not kept
+    // backward
+    const void* dout = nullptr;  // (batch, queries, heads, dim)
+    void* dq = nullptr;
+    void* dk = nullptr;
+    void* dv = nullptr;
+    float* delta = nullptr;    // (batch, kv_heads, rows): sum over dim of dout out
+    int dtype = 0;
+    int batch = 0;
+    int queries = 0;
+    int keys = 0;
+    int kv_heads = 0;
+    int group = 1;
+    int dim = 0;
+    float scale = 1.0f;
+    __host__ __device__ long long rows() const { return static_cast<long long>(queries) * group; }
+    __host__ __device__ long long pairs() const { return static_cast<long long>(batch) * kv_heads; }
+    // Values from the start of a (sample, key head)'s results to row r's.
+    __host__ __device__ long long row_at(int b, int head, long long r) const
+    {
+        const long long t = r / group;
+        return ((b * static_cast<long long>(queries) + t) * kv_heads + head) * group * dim + (r - t * group) * dim;
+    }
+};
+
+// How many keys sample b has before its mask.
+__device__ __forceinline__ int length_of(const Call& c, int b)
+{
+    if (c.lengths == nullptr) {
+        return c.keys;
+    }
+    const long long n = c.lengths64 != 0 ? static_cast<const long long*>(c.lengths)[b] : static_cast<const int*>(c.lengths)[b];
+    return static_cast<int>(max(0LL, min(n, static_cast<long long>(c.keys))));
+}
+
+// Sums of `parts` float32 arrays of a result, in order, rounded once. Partial arrays are (part, pair, row, dim);
+// the result's rows are those of Call::row_at (queries) or (sample, key, head) (keys).
+void add_parts(const Call& c, const float* partial, int parts, bool of_keys, void* result, float factor, cudaStream_t stream);
+
+// Joins the splits of a forward pass: partial (split, pair, row, dim) holds sum p v, stats (split, pair, row) m and
+// sum p.
+void join_splits(const Call& c, const float* partial, const float2* stats, int splits, cudaStream_t stream);
+
+// delta = sum over dim of dout out.
+void row_products(const Call& c, cudaStream_t stream);
+
+inline int pieces(long long n, long long per) { return static_cast<int>((n + per - 1) / per); }
+
+// A part of a workspace, in bytes; every array starts on 256.
+class Arena {
+public:
+    std::size_t take(std::size_t bytes)
+    {
+        const std::size_t at = size_;
+        size_ += (bytes + 255) / 256 * 256;
+        return at;
+    }
+    std::size_t size() const { return size_; }
+
+private:
+    std::size_t size_ = 0;
+};
+
+}  // namespace spectral::attention

@@ -1,0 +1,667 @@
+// Queries and keys before an attention: the norm of each head and the rotation by position, in one
+// pass over both (include/spectral_b200.h: spectral_qk_norm_rotary and its backward).
+//
+// Over one head x of `dim` values, with r = 1 / sqrt(mean(x^2) + eps):
+//   u = x r w,  and of each pair (u1, u2) turned by its angle a: (u1 cos a - u2 sin a, u1 sin a + u2 cos a)
+// Backward, with g the upstream gradient turned back by -a:
+//   dw = sum over rows of g x r,  dx = r (g w - x r^2 mean(g w x))
+//
+// Memory bounds it: a value is read and written once (backward: two reads, one write), some ten operations
+// each. A lane holds one 16-byte piece of a head (8 bytes or 4 where rows are aligned to no more), a head's
+// lanes sit side by side, so its sums are a few shuffles and so is the exchange of the pairs that lie half
+// an axis apart. The angles of a token serve all of its heads: a CTA takes as many tokens as give each
+// thread a few pieces, asks for those pieces, fills a table of (cos, sin) in shared memory while they
+// arrive, then works through the heads. An angle is position * frequency in turns, in 64 bits until whole turns
+// are taken off (a position of 2^20 leaves an angle of 2^-4 in 32 bits), then float32.
+// Sums over dim, and those of the weights' gradients over rows, are float32 in a fixed order.
+
+#include "../../include/spectral_b200.h"
+
+#include "backend.hpp"
+#include "launch.cuh"
+#include "pointwise.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace spectral {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxDim = SPECTRAL_HEAD_DIM_MAX;
+constexpr int kTableBytes = 16 * 1024;
+
+struct Side {
+    const void* x = nullptr;
+    const void* dy = nullptr;
+    void* out = nullptr;  // y, or dx
+    const float* weight = nullptr;
+    const void* positions = nullptr;
+    float* partial = nullptr;  // backward: a row of dim sums per CTA
+    long long stride[3] = {0, 0, 0};
+    long long position_stride[3] = {0, 0, 0};
+    int position_type = 0;
+    int heads = 0;
+    long long tokens = 0;  // of a sample
+    long long total = 0;   // of all samples
+    int tile_tokens = 1;
+    int ctas = 0;
+};
+
+struct Plan {
+    Side side[2];
+    int dim = 0;
+    int rotated = 0;
+    int axes = 1;
+    int per_axis = 0;  // pairs
+    int table_pairs = 0;
+    bool neighbours = false;
+    float eps = 0.0f;
+    double turns[kMaxDim / 2];  // angle per position, in turns, of an axis's pairs
+};
+
+__device__ __forceinline__ double position_at(const Side& s, long long at)
+{
+    switch (s.position_type) {
+        case SPECTRAL_POSITIONS_FLOAT32: return static_cast<double>(static_cast<const float*>(s.positions)[at]);
+        case SPECTRAL_POSITIONS_INT32: return static_cast<double>(static_cast<const int*>(s.positions)[at]);
+        default: return static_cast<double>(static_cast<const long long*>(s.positions)[at]);
+    }
+}
+
+// (cos, sin) of an angle in turns. For results rounded to 16 bits the hardware's functions on [-pi, pi], off by
+// 2^-20 at most, do.
+template <class T>
+__device__ __forceinline__ float2 unit(double turns)
+{
+    const float f = static_cast<float>(turns - rint(turns));
+    float2 cs;
+    if constexpr (sizeof(T) == 4) {
+        sincospif(2.0f * f, &cs.y, &cs.x);
+    } else {
+        __sincosf(6.283185307179586f * f, &cs.y, &cs.x);
+    }
+    return cs;
+}
+
+template <class W>
+__device__ __forceinline__ W shuffle_words(const W& v, int src)
+{
+    static_assert(sizeof(W) % 4 == 0, "whole words");
+    W out;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(W) / 4); ++i) {
+        reinterpret_cast<uint32_t*>(&out)[i] = __shfl_sync(0xffffffffu, reinterpret_cast<const uint32_t*>(&v)[i], src);
+    }
+    return out;
+}
+
+__device__ __forceinline__ float sum_lanes(float v, int lanes)
+{
+    for (int o = lanes / 2; o > 0; o /= 2) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+
+// V values of a head per lane, `lanes` (a power of two) lanes a head; V = 1: any dim and alignment, a warp a head and
+// up to four values a lane. Forward needs x, backward also dy.
+template <class T, int V, bool Back>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Plan plan, int lanes)
+{
+    constexpr int kUnits = V == 1 ? kMaxDim / 32 : 1;  // pieces of a head a lane holds
+    constexpr int kRows = V == 1 ? 1 : Back ? 2 : 4;   // heads in flight per lane
+    using Piece = Vec<T, V>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float exchange[V == 1 ? kThreads / 32 : 1][V == 1 ? kMaxDim : 1];
+    const bool second_side = static_cast<int>(blockIdx.x) >= plan.side[0].ctas;
+    const Side& s = plan.side[second_side ? 1 : 0];
+    const int cta = blockIdx.x - (second_side ? plan.side[0].ctas : 0);
+    const int dim = plan.dim;
+    const int rotated = s.positions != nullptr ? plan.rotated : 0;
+    const int n = plan.per_axis;
+    const int pairs = plan.table_pairs;
+    auto* table = reinterpret_cast<float2*>(smem);
+    auto* offsets = reinterpret_cast<long long*>(smem + (static_cast<size_t>(s.tile_tokens) * pairs * 8 + 15) / 16 * 16);
+
+    const int lane = threadIdx.x & 31;
+    const int sub = lane & (lanes - 1);
+    const int group = threadIdx.x / lanes;
+    const int groups = kThreads / lanes;
+    // This lane's pieces: where in the head, which pairs of the table, where the partners are (halves) and which of
+    // the two it holds.
+    int d[kUnits], pair_at[kUnits], partner[kUnits];
+    bool live[kUnits], turned[kUnits], first[kUnits];
+    Floats<V> w[kUnits], wp[kUnits], dw[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+        d[k] = (sub + k * lanes) * V;
+        live[k] = d[k] < dim;
+        turned[k] = live[k] && d[k] < rotated;
+        first[k] = true;
+        partner[k] = d[k];
+        pair_at[k] = d[k] / 2;
+        if (plan.neighbours) {
+            if (V == 1) {
+                first[k] = d[k] % 2 == 0;
+                partner[k] = d[k] ^ 1;
+            }
+        } else if (turned[k]) {
+            const int axis = d[k] / (2 * n);
+            const int off = d[k] - axis * 2 * n;
+            first[k] = off < n;
+            partner[k] = first[k] ? d[k] + n : d[k] - n;
+            pair_at[k] = axis * n + (first[k] ? off : off - n);
+        }
+        w[k].fill(1.0f);
+        wp[k].fill(1.0f);
+        dw[k].fill(0.0f);
+    }
+    allow_next_grid();
+    wait_for_previous_grid();
+    if (s.weight != nullptr) {
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (live[k]) {
+                    w[k].set(j, s.weight[d[k] + j]);
+                    wp[k].set(j, turned[k] ? s.weight[partner[k] + j] : 0.0f);
+                }
+            }
+        }
+    }
+    const T* __restrict__ x = static_cast<const T*>(s.x);
+    const T* __restrict__ dy = static_cast<const T*>(s.dy);
+    T* __restrict__ out = static_cast<T*>(s.out);
+    const int heads = s.heads;
+    const int step_tokens = groups / heads;
+    const int step_heads = groups - step_tokens * heads;
+
+    for (long long start = static_cast<long long>(cta) * s.tile_tokens; start < s.total;
+         start += static_cast<long long>(s.ctas) * s.tile_tokens) {
+        const int tokens = static_cast<int>(min(static_cast<long long>(s.tile_tokens), s.total - start));
+        for (int t = threadIdx.x; t < tokens; t += kThreads) {
+            const long long b = (start + t) / s.tokens;
+            offsets[t] = b * s.stride[0] + (start + t - b * s.tokens) * s.stride[1];
+        }
+        __syncthreads();
+        const long long rows = static_cast<long long>(tokens) * heads;
+        int token = group / heads;
+        int head = group - token * heads;
+        for (long long base = 0; base < rows; base += static_cast<long long>(kRows) * groups) {
+            Piece px[kRows][kUnits], pg[kRows][kUnits];
+            int token_of[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const long long row = base + group + i * groups;
+                token_of[i] = min(token, tokens - 1);
+                const long long from = offsets[token_of[i]] + head * s.stride[2];
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    px[i][k] = Piece{};
+                    pg[i][k] = Piece{};
+                    if (row < rows && live[k]) {
+                        px[i][k] = *reinterpret_cast<const Piece*>(x + from + d[k]);
+                        if constexpr (Back) {
+                            pg[i][k] = *reinterpret_cast<const Piece*>(dy + (start * heads + row) * dim + d[k]);
+                        }
+                    }
+                }
+                token += step_tokens;
+                head += step_heads;
+                if (head >= heads) {
+                    head -= heads;
+                    ++token;
+                }
+            }
+            if (base == 0) {
+                if (rotated > 0) {
+                    for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
+                        const int t = i / pairs;
+                        const int p = i - t * pairs;
+                        float2 cs = make_float2(1.0f, 0.0f);
+                        if (p < rotated / 2) {
+                            const int axis = p / n;
+                            const long long b = (start + t) / s.tokens;
+                            const double pos = position_at(s, b * s.position_stride[0] + (start + t - b * s.tokens) * s.position_stride[1]
+                                                                  + axis * s.position_stride[2]);
+                            cs = unit<T>(pos * plan.turns[p - axis * n]);
+                        }
+                        table[i] = cs;
+                    }
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const long long row = base + group + i * groups;
+                if (base + i * groups >= rows) {  // none in the whole CTA
+                    break;
+                }
+                float2 square = pair(0.0f);
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    const Floats<V> f = widen(px[i][k]);
+#pragma unroll
+                    for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                        square = fma2(f.p[j], f.p[j], square);
+                    }
+                }
+                const float mean = sum_lanes(square.x + square.y, lanes) / static_cast<float>(dim);
+                const float r = rsqrtf(mean + plan.eps);
+                // What is turned: x r w forward, the upstream gradient (the other way) backward.
+                Floats<V> f[kUnits], other[kUnits];
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    f[k] = widen(Back ? pg[i][k] : px[i][k]);
+                    if constexpr (!Back) {
+#pragma unroll
+                        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                            f[k].p[j] = f[k].p[j] * pair(r) * w[k].p[j];
+                        }
+                    }
+                }
+                if (rotated > 0) {
+                    const float2* cs = table + token_of[i] * pairs;
+                    if constexpr (V == 1) {
+                        float* buf = exchange[threadIdx.x >> 5];
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < kUnits; ++k) {
+                            if (live[k]) {
+                                buf[d[k]] = f[k].p[0].x;
+                            }
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < kUnits; ++k) {
+                            if (turned[k]) {
+                                const float2 c = cs[pair_at[k]];
+                                f[k].p[0].x = f[k].p[0].x * c.x + buf[partner[k]] * (first[k] != Back ? -c.y : c.y);
+                            }
+                        }
+                    } else if (plan.neighbours) {
+                        if (turned[0]) {
+#pragma unroll
+                            for (int j = 0; j < V / 2; ++j) {
+                                const float2 c = cs[pair_at[0] + j];
+                                const float sine = Back ? -c.y : c.y;
+                                const float2 v = f[0].p[j];
+                                f[0].p[j] = make_float2(v.x * c.x - v.y * sine, v.y * c.x + v.x * sine);
+                            }
+                        }
+                    } else {
+                        const int src = lane - sub + partner[0] / V;
+                        other[0] = widen(shuffle_words(Back ? pg[i][0] : px[i][0], src));
+                        if (turned[0]) {
+                            const float sign = first[0] != Back ? -1.0f : 1.0f;
+#pragma unroll
+                            for (int j = 0; j < V; ++j) {
+                                const float2 c = cs[pair_at[0] + j];
+                                float o = other[0].at(j);
+                                if constexpr (!Back) {
+                                    o *= r * wp[0].at(j);
+                                }
+                                f[0].set(j, f[0].at(j) * c.x + o * (sign * c.y));
+                            }
+                        }
+                    }
+                }
+                if constexpr (Back) {
+                    float2 dot = pair(0.0f);
+                    Floats<V> xs[kUnits];
+#pragma unroll
+                    for (int k = 0; k < kUnits; ++k) {
+                        xs[k] = widen(px[i][k]);
+#pragma unroll
+                        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                            const float2 gx = f[k].p[j] * xs[k].p[j];
+                            dw[k].p[j] = fma2(gx, pair(r), dw[k].p[j]);
+                            dot = fma2(gx, w[k].p[j], dot);
+                        }
+                    }
+                    const float c = -sum_lanes(dot.x + dot.y, lanes) / static_cast<float>(dim) * r * r;
+#pragma unroll
+                    for (int k = 0; k < kUnits; ++k) {
+#pragma unroll
+                        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                            f[k].p[j] = fma2(xs[k].p[j], pair(c), f[k].p[j] * w[k].p[j]) * pair(r);
+                        }
+                    }
+                }
+                if (row < rows) {
+#pragma unroll
+                    for (int k = 0; k < kUnits; ++k) {
+                        if (live[k]) {
+                            *reinterpret_cast<Piece*>(out + (start * heads + row) * dim + d[k]) = narrow<T>(f[k]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if constexpr (Back) {
+        if (s.partial == nullptr) {
+            return;
+        }
+        // The groups' sums of each value, in order: through shared memory, a value a thread.
+        auto* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (live[k]) {
+                    sums[group * dim + d[k] + j] = dw[k].at(j);
+                }
+            }
+        }
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < dim) {
+            float total = 0.0f;
+            for (int g = 0; g < groups; ++g) {
+                total += sums[g * dim + threadIdx.x];
+            }
+            s.partial[static_cast<long long>(cta) * dim + threadIdx.x] = total;
+        }
+    }
+}
+
+// dweight = the sum of the CTAs' rows; a CTA per side and 32 values, eight warps side by side over the rows.
+struct Sums {
+    const float* partial[2];
+    float* out[2];
+    int rows[2];
+    int dim;
+};
+
+__global__ void __launch_bounds__(256) weight_sum_kernel(const Sums g)
+{
+    __shared__ float part[8][32];
+    wait_for_previous_grid();
+    const int side = blockIdx.y;
+    const int d = blockIdx.x * 32 + (threadIdx.x & 31);
+    const int warp = threadIdx.x >> 5;
+    if (g.out[side] == nullptr) {
+        return;
+    }
+    float total = 0.0f;
+    if (d < g.dim) {
+#pragma unroll 4
+        for (int r = warp; r < g.rows[side]; r += 8) {
+            total += g.partial[side][static_cast<long long>(r) * g.dim + d];
+        }
+    }
+    part[warp][threadIdx.x & 31] = total;
+    __syncthreads();
+    if (warp == 0 && d < g.dim) {
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            total += part[i][threadIdx.x];
+        }
+        g.out[side][d] = total;
+    }
+}
+
+// --- host ------------------------------------------------------------------------------------------
+
+int invalid(const std::string& message)
+{
+    set_last_error(message);
+    return SPECTRAL_INVALID_ARGUMENT;
+}
+
+// Values per access that every row of the call allows: whole pieces in a head (and in half an axis's values, where
+// partners lie that far apart), at most a warp's worth, aligned.
+int vector_width(const spectral_heads* const (&sides)[2], int dtype, long long batch, int dim, int rotated, int axes, int pairs)
+{
+    const int size = static_cast<int>(dtype_size(dtype));
+    const int n = rotated / (2 * axes);
+    for (int v = 16 / size; v >= 2; v /= 2) {
+        bool ok = dim % v == 0 && dim / v <= 32 && (rotated == 0 || pairs == SPECTRAL_PAIRS_NEIGHBOURS || n % v == 0);
+        for (const spectral_heads* s : sides) {
+            if (s == nullptr) {
+                continue;
+            }
+            ok = ok && aligned_to(s->x, v * size) && aligned_to(s->out, v * size) && aligned_to(s->dy, v * size)
+                 && (batch <= 1 || s->stride[0] % v == 0) && (s->tokens <= 1 || s->stride[1] % v == 0)
+                 && (s->heads <= 1 || s->stride[2] % v == 0);
+        }
+        if (ok) {
+            return v;
+        }
+    }
+    return 1;
+}
+
+int lanes_for(int dim, int v)
+{
+    int lanes = 1;
+    while (lanes < 32 && lanes * v < dim) {
+        lanes *= 2;
+    }
+    return lanes;
+}
+
+// CTAs that are resident at once with room for registers and tables, the most a call has.
+int most_ctas() { return device_sm_count(current_device()) * 4; }
+
+int check(const char* op, const spectral_heads* const (&sides)[2], bool back, int dtype, long long batch, int dim, int rotated,
+          int axes, int pairs, float eps, float theta)
+{
+    const std::string name(op);
+    if (!dtype_known(dtype)) {
+        return invalid(name + ": dtype must be SPECTRAL_FLOAT32, SPECTRAL_BFLOAT16 or SPECTRAL_FLOAT16");
+    }
+    if (dim < 1 || dim > kMaxDim) {
+        return invalid(name + ": need 1 <= dim <= " + std::to_string(kMaxDim));
+    }
+    if (axes < 1 || rotated < 0 || rotated > dim || rotated % (2 * axes) != 0) {
+        return invalid(name + ": rotated must be a multiple of 2 * axes from 0 to dim");
+    }
+    if (pairs != SPECTRAL_PAIRS_HALVES && pairs != SPECTRAL_PAIRS_NEIGHBOURS) {
+        return invalid(name + ": pairs must be SPECTRAL_PAIRS_HALVES or SPECTRAL_PAIRS_NEIGHBOURS");
+    }
+    if (!(eps >= 0.0f) || !(theta > 0.0f) || std::isinf(theta)) {
+        return invalid(name + ": need eps >= 0 and a finite theta > 0");
+    }
+    if (sides[0] == nullptr && sides[1] == nullptr) {
+        return invalid(name + ": needs q or k");
+    }
+    for (const spectral_heads* s : sides) {
+        if (s == nullptr) {
+            continue;
+        }
+        if (batch < 0 || s->tokens < 0 || s->heads < 1 || s->heads > (1 << 20) || batch >= (1LL << 31) || s->tokens >= (1LL << 31)
+            || (s->tokens > 0 && batch > (1LL << 40) / s->tokens)) {
+            return invalid(name + ": need 0 <= batch, tokens < 2^31, batch * tokens <= 2^40 and heads from 1 to 2^20");
+        }
+        if (batch * s->tokens == 0) {
+            continue;
+        }
+        const std::size_t size = dtype_size(dtype);
+        if (s->x == nullptr || s->out == nullptr || (back && s->dy == nullptr)) {
+            return invalid(name + ": null array");
+        }
+        if (!aligned_to(s->x, size) || !aligned_to(s->out, size) || !aligned_to(s->dy, size) || !aligned_to(s->weight, 4)
+            || !aligned_to(s->dweight, 4)) {
+            return invalid(name + ": arrays must be aligned to their element size");
+        }
+        if (s->positions != nullptr && rotated > 0) {
+            if (s->position_type < SPECTRAL_POSITIONS_FLOAT32 || s->position_type > SPECTRAL_POSITIONS_INT64) {
+                return invalid(name + ": position_type must be SPECTRAL_POSITIONS_FLOAT32, _INT32 or _INT64");
+            }
+            if (!aligned_to(s->positions, s->position_type == SPECTRAL_POSITIONS_INT64 ? 8 : 4)) {
+                return invalid(name + ": positions must be aligned to their element size");
+            }
+        }
+        // The results are contiguous; the input may be a strided view, whose extent bounds what it can touch.
+        const auto p = reinterpret_cast<std::uintptr_t>(s->x);
+        long long low = 0, high = dim - 1;
+        const long long extent[3] = {batch, s->tokens, s->heads};
+        for (int i = 0; i < 3; ++i) {
+            (s->stride[i] < 0 ? low : high) += s->stride[i] * (extent[i] - 1);
+        }
+        const std::uintptr_t count = static_cast<std::uintptr_t>(batch) * s->tokens * s->heads * dim * size;
+        const auto o = reinterpret_cast<std::uintptr_t>(s->out);
+        const auto g = reinterpret_cast<std::uintptr_t>(s->dy);
+        if ((p + low * static_cast<long long>(size) < o + count && o < p + (high + 1) * static_cast<long long>(size))
+            || (back && g < o + count && o < g + count)) {
+            return invalid(name + ": the result must not overlap the input" + (back ? " or dy" : ""));
+        }
+    }
+    return SPECTRAL_OK;
+}
+
+void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long long batch, int dim, int rotated, int axes,
+         int pairs, float eps, float theta, float* work, cudaStream_t stream)
+{
+    Plan plan;
+    plan.dim = dim;
+    plan.axes = axes;
+    plan.neighbours = pairs == SPECTRAL_PAIRS_NEIGHBOURS;
+    plan.eps = eps;
+    bool any = false;
+    for (const spectral_heads* s : sides) {
+        any = any || (s != nullptr && s->positions != nullptr);
+    }
+    plan.rotated = any ? rotated : 0;
+    plan.per_axis = std::max(1, plan.rotated / (2 * axes));
+    // A piece that reaches past `rotated` (neighbours only) finds angles of zero there.
+    plan.table_pairs = plan.rotated == 0 ? 0 : plan.neighbours ? (dim + 1) / 2 : plan.rotated / 2;
+    for (int i = 0; i < plan.per_axis && plan.rotated > 0; ++i) {
+        plan.turns[i] = std::pow(static_cast<double>(theta), -static_cast<double>(i) / plan.per_axis) / 6.283185307179586476925;
+    }
+    const int v = vector_width(sides, dtype, batch, dim, plan.rotated, axes, pairs);
+    const int lanes = v == 1 ? 32 : lanes_for(dim, v);
+    const int groups = kThreads / lanes;
+    const int in_flight = v == 1 ? 4 : back ? 2 : 4;
+    const int most = most_ctas();
+    long long tiles[2] = {0, 0};
+    int table_tokens = 1;
+    for (int i = 0; i < 2; ++i) {
+        const spectral_heads* s = sides[i];
+        if (s == nullptr || batch * s->tokens == 0) {
+            continue;
+        }
+        Side& t = plan.side[i];
+        t.x = s->x;
+        t.dy = s->dy;
+        t.out = s->out;
+        t.weight = s->weight;
+        t.positions = plan.rotated > 0 ? s->positions : nullptr;
+        t.position_type = s->position_type;
+        std::copy(s->stride, s->stride + 3, t.stride);
+        std::copy(s->position_stride, s->position_stride + 3, t.position_stride);
+        t.heads = s->heads;
+        t.tokens = s->tokens;
+        t.total = batch * s->tokens;
+        const long long cap = plan.table_pairs > 0 ? std::max(1, kTableBytes / (8 * plan.table_pairs)) : 256;
+        t.tile_tokens = static_cast<int>(std::max(1LL, std::min<long long>(cap, static_cast<long long>(groups) * in_flight / s->heads)));
+        t.tile_tokens = static_cast<int>(std::min<long long>(t.tile_tokens, t.total));
+        tiles[i] = (t.total + t.tile_tokens - 1) / t.tile_tokens;
+        table_tokens = std::max(table_tokens, t.tile_tokens);
+    }
+    // CTAs in proportion to the sides' values.
+    const long long all = tiles[0] + tiles[1];
+    if (all > 0) {
+        const long long ctas = std::min<long long>(all, most);
+        for (int i = 0; i < 2; ++i) {
+            plan.side[i].ctas = tiles[i] == 0 ? 0 : static_cast<int>(std::max(1LL, std::min(tiles[i], (ctas * tiles[i] + all / 2) / all)));
+        }
+    }
+    Sums sums{};
+    sums.dim = dim;
+    float* at = work;
+    for (int i = 0; i < 2; ++i) {
+        if (back && sides[i] != nullptr && sides[i]->dweight != nullptr) {
+            sums.partial[i] = at;
+            sums.out[i] = sides[i]->dweight;
+            sums.rows[i] = plan.side[i].ctas;
+            plan.side[i].partial = at;
+            at += static_cast<long long>(plan.side[i].ctas) * dim;
+        }
+    }
+    const int ctas = plan.side[0].ctas + plan.side[1].ctas;
+    if (ctas > 0) {
+        std::size_t smem = (static_cast<std::size_t>(table_tokens) * plan.table_pairs * 8 + 15) / 16 * 16 + table_tokens * sizeof(long long);
+        if (back) {
+            smem = std::max(smem, static_cast<std::size_t>(groups) * dim * sizeof(float));
+        }
+        with_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            const auto launch = [&](auto width) {
+                constexpr int V = decltype(width)::value;
+                launch_pdl(back ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>, dim3(ctas), dim3(kThreads), smem, stream, plan, lanes);
+            };
+            switch (v) {
+                case 8:
+                    if constexpr (sizeof(T) == 2) {
+                        launch(std::integral_constant<int, 8>{});
+                    }
+                    break;
+                case 4: launch(std::integral_constant<int, 4>{}); break;
+                case 2: launch(std::integral_constant<int, 2>{}); break;
+                default: launch(std::integral_constant<int, 1>{}); break;
+            }
+        });
+    }
+    if (sums.out[0] != nullptr || sums.out[1] != nullptr) {
+        launch_pdl(weight_sum_kernel, dim3((dim + 31) / 32, 2), dim3(256), 0, stream, sums);
+    }
+}
+
+int entry(const char* op, const spectral_heads* q, const spectral_heads* k, bool back, int dtype, long long batch, int dim, int rotated,
+          int axes, int pairs, float eps, float theta, void* work, void* stream)
+{
+    const spectral_heads* const sides[2] = {q, k};
+    const int status = check(op, sides, back, dtype, batch, dim, rotated, axes, pairs, eps, theta);
+    if (status != SPECTRAL_OK) {
+        return status;
+    }
+    const bool sums = back && ((q != nullptr && q->dweight != nullptr) || (k != nullptr && k->dweight != nullptr));
+    if (sums && (work == nullptr || !aligned_to(work, 8))) {
+        return invalid(std::string(op) + ": needs a workspace, 8-byte aligned");
+    }
+    try {
+        run(sides, back, dtype, batch, dim, rotated, axes, pairs, eps, theta, static_cast<float*>(work), static_cast<cudaStream_t>(stream));
+        return SPECTRAL_OK;
+    } catch (const InvalidArgument& e) {
+        return invalid(e.what());
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return SPECTRAL_CUDA_ERROR;
+    }
+}
+
+}  // namespace
+}  // namespace spectral
+
+extern "C" int spectral_qk_norm_rotary(const spectral_heads* q, const spectral_heads* k, int dtype, long long batch, int dim,
+                                       int rotated, int axes, int pairs, float eps, float theta, void* stream)
+{
+    return spectral::entry("qk_norm_rotary", q, k, false, dtype, batch, dim, rotated, axes, pairs, eps, theta, nullptr, stream);
+}
+
+extern "C" int spectral_qk_norm_rotary_backward_workspace(int dim, size_t* count)
+{
+    using namespace spectral;
+    if (count == nullptr || dim < 1 || dim > kMaxDim) {
+        return invalid("qk_norm_rotary_backward_workspace: need 1 <= dim <= " + std::to_string(kMaxDim) + " and a count");
+    }
+    try {
+        *count = (static_cast<std::size_t>(most_ctas() + 2) * dim + 1) / 2;
+        return SPECTRAL_OK;
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return SPECTRAL_CUDA_ERROR;
+    }
+}
+
+extern "C" int spectral_qk_norm_rotary_backward(const spectral_heads* q, const spectral_heads* k, int dtype, long long batch, int dim,
+                                                int rotated, int axes, int pairs, float eps, float theta, void* work, void* stream)
+{
+    return spectral::entry("qk_norm_rotary_backward", q, k, true, dtype, batch, dim, rotated, axes, pairs, eps, theta, work, stream);
+}

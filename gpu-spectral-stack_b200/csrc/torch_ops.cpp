@@ -6,7 +6,7 @@
 // made here raise RuntimeError (TORCH_CHECK), the C ABI's SPECTRAL_INVALID_ARGUMENT is rethrown
 // as std::invalid_argument (ValueError), as the reference's drivers do. Every operator is
 // registered for the CUDA dispatch key only, so CPU tensors get the dispatcher's
-// NotImplementedError (two also have gradients, through the AutogradCUDA key). A binding checks, makes its input contiguous, allocates the output and
+// NotImplementedError (four also have gradients, through the AutogradCUDA key). A binding checks, makes its input contiguous, allocates the output and
 // any workspace with at::empty (torch's caching allocator, stream-ordered), and launches on the
 // current stream under a device guard. Nothing here runs on the CPU.
 
@@ -20,7 +20,9 @@
 
 #include "../../include/spectral_b200.h"
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -28,6 +30,8 @@
 #include <vector>
 
 namespace {
+
+using variable_list_t = std::vector<at::Tensor>;
 
 void check_status(int status)
 {
@@ -895,6 +899,306 @@ gated_mlp_backward_cuda(const at::Tensor& dy, const c10::optional<at::Tensor>& x
     return {dx, dwg, dwu, dwd};
 }
 
+// --- reading from states of another length: additions of this library ---------------------------
+
+// The values of a head side by side; other strides are the kernels' business.
+at::Tensor head_rows(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+struct RotarySettings {
+    int64_t rotated;
+    double eps;
+    double theta;
+    std::string pairs;
+};
+
+int pairs_code(const std::string& pairs, const char* op)
+{
+    if (pairs == "halves") {
+        return SPECTRAL_PAIRS_HALVES;
+    }
+    TORCH_CHECK(pairs == "neighbours", op, ": pairs must be 'halves' or 'neighbours', got '", pairs, "'");
+    return SPECTRAL_PAIRS_NEIGHBOURS;
+}
+
+// One side of the call: x (batch, tokens, heads, dim), an optional weight and optional positions. Keeps what the
+// descriptor points to.
+struct RotarySide {
+    at::Tensor x, weight, positions, dy, out, dweight;
+    spectral_heads heads{};
+    int axes = 0;
+};
+
+// `like`: the first side, whose type, device, batch and dim the others have.
+RotarySide rotary_side(const at::Tensor& x, const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& positions,
+                       const at::Tensor& like, const char* op, const char* name)
+{
+    TORCH_CHECK(x.dim() == 4, op, ": ", name, " must be (batch, tokens, heads, dim), got ", x.sizes());
+    dtype_code(x, op, name);
+    check_like(x, like, op, name);
+    TORCH_CHECK(x.size(0) == like.size(0) && x.size(3) == like.size(3), op, ": q and k must agree in batch and dim, got ",
+                like.sizes(), " and ", x.sizes());
+    RotarySide s;
+    s.x = head_rows(x);
+    s.weight = channel_parameter(weight, x, x.size(3), op, name == std::string("q") ? "q_weight" : "k_weight");
+    s.heads.x = cptr(s.x);
+    for (int i = 0; i < 3; ++i) {
+        s.heads.stride[i] = s.x.stride(i);
+    }
+    s.heads.weight = fptr(s.weight);
+    s.heads.heads = small_int(x.size(2), op, "the number of heads");
+    s.heads.tokens = x.size(1);
+    if (positions.has_value() && positions->defined()) {
+        s.positions = *positions;
+        const at::Tensor& p = s.positions;
+        TORCH_CHECK(p.is_cuda() && p.device() == x.device(), op, ": ", name, "_positions must be on the device of ", name);
+        const bool shared = p.dim() == 2;
+        TORCH_CHECK((shared || (p.dim() == 3 && p.size(0) == x.size(0))) && p.size(-2) == x.size(1) && p.size(-1) >= 1, op, ": ", name,
+                    "_positions must be (tokens, axes) or (batch, tokens, axes) for ", name, " ", x.sizes(), ", got ", p.sizes());
+        switch (p.scalar_type()) {
+            case at::kFloat: s.heads.position_type = SPECTRAL_POSITIONS_FLOAT32; break;
+            case at::kInt: s.heads.position_type = SPECTRAL_POSITIONS_INT32; break;
+            case at::kLong: s.heads.position_type = SPECTRAL_POSITIONS_INT64; break;
+            default: TORCH_CHECK(false, op, ": ", name, "_positions must be float32, int32 or int64, got ", p.scalar_type());
+        }
+        s.heads.positions = cptr(p);
+        s.heads.position_stride[0] = shared ? 0 : p.stride(0);
+        s.heads.position_stride[1] = p.stride(-2);
+        s.heads.position_stride[2] = p.stride(-1);
+        s.axes = small_int(p.size(-1), op, "the number of axes");
+    }
+    return s;
+}
+
+// The axes of the call: those of its positions (1 if there are none).
+int rotary_axes(const std::vector<RotarySide>& sides, const char* op)
+{
+    int axes = 0;
+    for (const RotarySide& s : sides) {
+        TORCH_CHECK(axes == 0 || s.axes == 0 || s.axes == axes, op, ": q_positions and k_positions must have the same axes");
+        axes = std::max(axes, s.axes);
+    }
+    return std::max(axes, 1);
+}
+
+// As many values of a head as `axes` spans of pairs hold, unless the caller says how many.
+int rotary_values(int64_t rotated, int64_t dim, int axes, const char* op)
+{
+    if (rotated < 0) {
+        return static_cast<int>(dim / (2 * axes) * (2 * axes));
+    }
+    return small_int(rotated, op, "rotated");
+}
+
+const char* side_name(size_t i) { return i == 1 ? "k" : "q"; }
+
+variable_list_t rotary_forward(const variable_list_t& x, const std::vector<c10::optional<at::Tensor>>& weight,
+                               const std::vector<c10::optional<at::Tensor>>& positions, const RotarySettings& set)
+{
+    constexpr const char* op = "qk_norm_rotary";
+    const int dtype = dtype_code(x[0], op, "q");
+    const int pairs = pairs_code(set.pairs, op);
+    std::vector<RotarySide> sides;
+    for (size_t i = 0; i < x.size(); ++i) {
+        sides.push_back(rotary_side(x[i], weight[i], positions[i], x[0], op, side_name(i)));
+    }
+    const int axes = rotary_axes(sides, op);
+    const int dim = small_int(x[0].size(3), op, "dim");
+    const c10::cuda::CUDAGuard guard(x[0].device());
+    variable_list_t out;
+    for (RotarySide& s : sides) {
+        out.push_back(at::empty(s.x.sizes(), s.x.options()));
+        s.heads.out = mptr(out.back());
+    }
+    check_status(spectral_qk_norm_rotary(&sides[0].heads, sides.size() > 1 ? &sides[1].heads : nullptr, dtype, x[0].size(0), dim,
+                                         rotary_values(set.rotated, dim, axes, op), axes, pairs, static_cast<float>(set.eps),
+                                         static_cast<float>(set.theta), stream()));
+    return out;
+}
+
+// dx of each side, then dweight of each (undefined without a weight). A side whose dy is undefined has neither.
+variable_list_t rotary_backward(const variable_list_t& dy, const variable_list_t& x, const std::vector<c10::optional<at::Tensor>>& weight,
+                                const std::vector<c10::optional<at::Tensor>>& positions, const RotarySettings& set)
+{
+    constexpr const char* op = "qk_norm_rotary_backward";
+    const int dtype = dtype_code(x[0], op, "q");
+    const int pairs = pairs_code(set.pairs, op);
+    std::vector<RotarySide> sides;
+    for (size_t i = 0; i < x.size(); ++i) {
+        sides.push_back(rotary_side(x[i], weight[i], positions[i], x[0], op, side_name(i)));
+    }
+    const int axes = rotary_axes(sides, op);
+    const int dim = small_int(x[0].size(3), op, "dim");
+    const c10::cuda::CUDAGuard guard(x[0].device());
+    const spectral_heads* given[2] = {nullptr, nullptr};
+    size_t count = 0;
+    check_status(spectral_qk_norm_rotary_backward_workspace(dim, &count));
+    for (size_t i = 0; i < sides.size(); ++i) {
+        RotarySide& s = sides[i];
+        if (!dy[i].defined()) {
+            continue;
+        }
+        check_like(dy[i], x[i], op, "dy");
+        TORCH_CHECK(dy[i].sizes() == x[i].sizes(), op, ": dy must be ", x[i].sizes(), ", got ", dy[i].sizes());
+        s.dy = dy[i].contiguous();
+        s.out = at::empty(s.x.sizes(), s.x.options());
+        s.heads.dy = cptr(s.dy);
+        s.heads.out = mptr(s.out);
+        if (s.weight.defined()) {
+            s.dweight = at::empty(s.weight.sizes(), s.weight.options());
+            s.heads.dweight = static_cast<float*>(mptr(s.dweight));
+        }
+        given[i] = &s.heads;
+    }
+    variable_list_t results;
+    if (given[0] != nullptr || given[1] != nullptr) {
+        at::Tensor work = workspace(count, x[0]);
+        check_status(spectral_qk_norm_rotary_backward(given[0], given[1], dtype, x[0].size(0), dim, rotary_values(set.rotated, dim, axes, op), axes,
+                                                      pairs, static_cast<float>(set.eps), static_cast<float>(set.theta), mptr(work), stream()));
+    }
+    for (const RotarySide& s : sides) {
+        results.push_back(s.out);
+    }
+    for (const RotarySide& s : sides) {
+        results.push_back(s.dweight);
+    }
+    return results;
+}
+
+std::vector<c10::optional<at::Tensor>> two(const c10::optional<at::Tensor>& a, const c10::optional<at::Tensor>& b) { return {a, b}; }
+
+variable_list_t qk_norm_rotary_cuda(const at::Tensor& q, const c10::optional<at::Tensor>& k, const c10::optional<at::Tensor>& q_weight,
+                                    const c10::optional<at::Tensor>& k_weight, const c10::optional<at::Tensor>& q_positions,
+                                    const c10::optional<at::Tensor>& k_positions, double eps, double theta, int64_t rotated,
+                                    c10::string_view pairs)
+{
+    variable_list_t x{q};
+    if (k.has_value() && k->defined()) {
+        x.push_back(*k);
+    }
+    return rotary_forward(x, two(q_weight, k_weight), two(q_positions, k_positions),
+                          {rotated, eps, theta, std::string(pairs.data(), pairs.size())});
+}
+
+struct AttentionSizes {
+    int64_t batch, queries, keys;
+    int heads, kv_heads, dim;
+};
+
+AttentionSizes attention_sizes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const char* op)
+{
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(3) == k.size(3), op,
+                ": q (batch, queries, heads, dim) and k and v (batch, keys, kv_heads, dim) do not match: ", q.sizes(), ", ", k.sizes(), ", ",
+                v.sizes());
+    return {q.size(0), q.size(1), k.size(1), small_int(q.size(2), op, "heads"), small_int(k.size(2), op, "kv_heads"), small_int(q.size(3), op, "dim")};
+}
+
+// The call's arrays as the C ABI takes them.
+struct AttentionArrays {
+    at::Tensor q, k, v, lengths, mask;
+    long long strides[9];
+    AttentionSizes n;
+    int dtype;
+    float scale;
+    int lengths64() const { return lengths.defined() && lengths.scalar_type() == at::kLong ? 1 : 0; }
+    const void* lengths_ptr() const { return lengths.defined() && lengths.numel() > 0 ? cptr(lengths) : nullptr; }
+    const void* mask_ptr() const { return mask.defined() && mask.numel() > 0 ? cptr(mask) : nullptr; }
+
+    AttentionArrays(const at::Tensor& q0, const at::Tensor& k0, const at::Tensor& v0, const c10::optional<at::Tensor>& lengths0,
+                    const c10::optional<at::Tensor>& mask0, c10::optional<double> scale0, const char* op)
+    {
+        dtype = dtype_code(q0, op, "q");
+        check_like(k0, q0, op, "k");
+        check_like(v0, q0, op, "v");
+        n = attention_sizes(q0, k0, v0, op);
+        q = head_rows(q0);
+        k = head_rows(k0);
+        v = head_rows(v0);
+        const at::Tensor* arrays[3] = {&q, &k, &v};
+        for (int i = 0; i < 9; ++i) {
+            strides[i] = arrays[i / 3]->stride(i % 3);
+        }
+        scale = scale0.has_value() ? static_cast<float>(*scale0) : 1.0f / std::sqrt(static_cast<float>(n.dim));
+        if (lengths0.has_value() && lengths0->defined()) {
+            const at::Tensor& l = *lengths0;
+            TORCH_CHECK(l.is_cuda() && l.device() == q.device() && (l.scalar_type() == at::kInt || l.scalar_type() == at::kLong)
+                            && l.dim() == 1 && l.size(0) == n.batch,
+                        op, ": lengths must be an int32 or int64 tensor of ", n.batch, " values on the device of q");
+            lengths = l.contiguous();
+        }
+        if (mask0.has_value() && mask0->defined()) {
+            const at::Tensor& m = *mask0;
+            TORCH_CHECK(m.is_cuda() && m.device() == q.device() && m.scalar_type() == at::kBool && m.dim() == 2
+                            && (m.size(0) == n.batch || m.size(0) == 1) && m.size(1) == n.keys,
+                        op, ": mask must be a bool tensor (batch, keys) or (1, keys) on the device of q, got ", m.scalar_type(), " ", m.sizes());
+            mask = m.expand({n.batch, n.keys}).contiguous();
+        }
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                     const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
+                                                     c10::optional<double> scale, bool keep)
+{
+    constexpr const char* op = "cross_attention";
+    TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(q.device());
+    const AttentionArrays a(q, k, v, lengths, mask, scale, op);
+    const AttentionSizes& n = a.n;
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    at::Tensor stats;
+    if (keep) {
+        stats = at::empty({n.batch, n.kv_heads, n.kv_heads > 0 ? n.queries * (n.heads / n.kv_heads) : 0, 2}, q.options().dtype(at::kFloat));
+    }
+    size_t count = 0;
+    check_status(spectral_cross_attention_workspace(cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.dtype, n.batch, n.queries, n.keys, n.heads,
+                                                    n.kv_heads, n.dim, &count));
+    at::Tensor work = workspace(count, q);
+    check_status(spectral_cross_attention(cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.lengths_ptr(), a.lengths64(), a.mask_ptr(), mptr(out),
+                                          keep ? static_cast<float*>(mptr(stats)) : nullptr, a.dtype, n.batch, n.queries, n.keys, n.heads,
+                                          n.kv_heads, n.dim, a.scale, mptr(work), stream()));
+    return {out, stats};
+}
+
+std::tuple<at::Tensor, at::Tensor> cross_attention_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                        const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
+                                                        c10::optional<double> scale)
+{
+    return attention_forward(q, k, v, lengths, mask, scale, true);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+cross_attention_backward_cuda(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
+                              const at::Tensor& stats, const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
+                              c10::optional<double> scale)
+{
+    constexpr const char* op = "cross_attention_backward";
+    TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(q.device());
+    const AttentionArrays a(q, k, v, lengths, mask, scale, op);
+    const AttentionSizes& n = a.n;
+    check_like(dout, q, op, "dout");
+    check_like(out, q, op, "out");
+    TORCH_CHECK(dout.sizes() == q.sizes() && out.sizes() == q.sizes(), op, ": dout and out must be ", q.sizes(), ", got ", dout.sizes(), " and ",
+                out.sizes());
+    TORCH_CHECK(stats.is_cuda() && stats.device() == q.device() && stats.scalar_type() == at::kFloat && n.kv_heads > 0
+                    && stats.numel() == 2 * n.batch * n.queries * n.heads,
+                op, ": stats must be what cross_attention returned");
+    const at::Tensor dc = dout.contiguous();
+    const at::Tensor oc = out.contiguous();
+    const at::Tensor sc = stats.contiguous();
+    at::Tensor dq = at::empty(q.sizes(), q.options());
+    at::Tensor dk = at::empty(k.sizes(), q.options());
+    at::Tensor dv = at::empty(v.sizes(), q.options());
+    size_t count = 0;
+    check_status(spectral_cross_attention_backward_workspace(cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.dtype, n.batch, n.queries, n.keys,
+                                                             n.heads, n.kv_heads, n.dim, &count));
+    at::Tensor work = workspace(count, q);
+    check_status(spectral_cross_attention_backward(cptr(dc), cptr(a.q), cptr(a.k), cptr(a.v), a.strides, cptr(oc), fptr(sc), a.lengths_ptr(),
+                                                   a.lengths64(), a.mask_ptr(), mptr(dq), mptr(dk), mptr(dv), a.dtype, n.batch, n.queries, n.keys,
+                                                   n.heads, n.kv_heads, n.dim, a.scale, mptr(work), stream()));
+    return {dq, dk, dv};
+}
+
 // --- the same with gradients: what spectral.nn calls ----------------------------------------------
 // Functions of torch's autograd engine in C++ (the Python class's bookkeeping took longer than the
 // kernels of a small layer). Each keeps only its input for the backward pass, in 8 bits if asked.
@@ -915,8 +1219,10 @@ struct NotDifferentiable : torch::autograd::Node {
 // An upstream gradient that is a leaf can only ask for gradients of gradients: refused at once.
 void check_once(const variable_list& grads, const char* op)
 {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].defined() && grads[0].requires_grad() && !grads[0].grad_fn()), op,
-                ": the backward pass is not differentiable itself");
+    for (const at::Tensor& g : grads) {
+        TORCH_CHECK(!(at::GradMode::is_enabled() && g.defined() && g.requires_grad() && !g.grad_fn()), op,
+                    ": the backward pass is not differentiable itself");
+    }
 }
 
 // The end of a backward pass: `results` with the history above if there is to be one. `create_graph` is grad mode
@@ -932,8 +1238,10 @@ variable_list finish_once(bool create_graph, const char* op, const variable_list
             edges.push_back(e);
         }
     }
-    if (grads[0].defined() && grads[0].requires_grad()) {
-        edges.push_back(torch::autograd::impl::gradient_edge(grads[0]));
+    for (const at::Tensor& g : grads) {
+        if (g.defined() && g.requires_grad()) {
+            edges.push_back(torch::autograd::impl::gradient_edge(g));
+        }
     }
     const auto node = std::make_shared<NotDifferentiable>(op);
     node->set_next_edges(std::move(edges));
@@ -1077,6 +1385,108 @@ at::Tensor gated_mlp_layer_autograd(const at::Tensor& x, const at::Tensor& w_gat
     return gated_mlp_layer_cuda(x, w_gate, w_up, w_down, activation, checkpoint8);
 }
 
+struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const c10::optional<at::Tensor>& k,
+                                 const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+                                 const c10::optional<at::Tensor>& q_positions, const c10::optional<at::Tensor>& k_positions, double eps,
+                                 double theta, int64_t rotated, std::string pairs)
+    {
+        at::AutoDispatchBelowAutograd guard;
+        variable_list out = qk_norm_rotary_cuda(q, k, q_weight, k_weight, q_positions, k_positions, eps, theta, rotated, pairs);
+        const at::Tensor none;
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k.value_or(none), q_weight.value_or(none), k_weight.value_or(none), q_positions.value_or(none),
+                                k_positions.value_or(none)});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["theta"] = theta;
+        ctx->saved_data["rotated"] = rotated;
+        ctx->saved_data["pairs"] = pairs;
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        check_once(grads, "qk_norm_rotary");
+        const bool create_graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
+        const variable_list kept = ctx->get_saved_variables();
+        variable_list x{kept[0]};
+        if (kept[1].defined()) {
+            x.push_back(kept[1]);
+        }
+        variable_list d = rotary_backward(grads, x, two(optional_of(kept[2]), optional_of(kept[3])), two(optional_of(kept[4]), optional_of(kept[5])),
+                                          {ctx->saved_data["rotated"].toInt(), ctx->saved_data["eps"].toDouble(),
+                                           ctx->saved_data["theta"].toDouble(), ctx->saved_data["pairs"].toStringRef()});
+        const at::Tensor none;
+        const bool both = x.size() == 2;
+        return finish_once(create_graph, "qk_norm_rotary", grads,
+                           {d[0], both ? d[1] : none, both ? d[2] : d[1], both ? d[3] : none, none, none, none, none, none, none});
+    }
+};
+
+variable_list qk_norm_rotary_layer_autograd(const at::Tensor& q, const c10::optional<at::Tensor>& k, const c10::optional<at::Tensor>& q_weight,
+                                            const c10::optional<at::Tensor>& k_weight, const c10::optional<at::Tensor>& q_positions,
+                                            const c10::optional<at::Tensor>& k_positions, double eps, double theta, int64_t rotated,
+                                            c10::string_view pairs)
+{
+    const at::Tensor kt = k.value_or(at::Tensor());
+    const at::Tensor qw = q_weight.value_or(at::Tensor());
+    const at::Tensor kw = k_weight.value_or(at::Tensor());
+    const at::Tensor qp = q_positions.value_or(at::Tensor());
+    const at::Tensor kp = k_positions.value_or(at::Tensor());
+    check_no_tangent("qk_norm_rotary", {&q, &kt, &qw, &kw, &qp, &kp});
+    TORCH_CHECK(!wants_grad({&qp, &kp}), "qk_norm_rotary: positions have no gradient; detach them");
+    // Without keys their weight has no part in the call, so no gradient either.
+    if (wants_grad({&q, &kt, &qw}) || (kt.defined() && wants_grad({&kw}))) {
+        return QkNormRotaryFunction::apply(q, k, q_weight, k_weight, q_positions, k_positions, eps, theta, rotated,
+                                           std::string(pairs.data(), pairs.size()));
+    }
+    at::AutoDispatchBelowAutograd guard;
+    return qk_norm_rotary_cuda(q, k, q_weight, k_weight, q_positions, k_positions, eps, theta, rotated, pairs);
+}
+
+struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                              const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask, c10::optional<double> scale)
+    {
+        at::AutoDispatchBelowAutograd guard;
+        auto [out, stats] = attention_forward(q, k, v, lengths, mask, scale, true);
+        const at::Tensor none;
+        ctx->save_for_backward({q, k, v, out, stats, lengths.value_or(none), mask.value_or(none)});
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        check_once(grads, "cross_attention");
+        const bool create_graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
+        const variable_list kept = ctx->get_saved_variables();
+        auto [dq, dk, dv] = cross_attention_backward_cuda(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], optional_of(kept[5]),
+                                                          optional_of(kept[6]), ctx->saved_data["scale"].toOptional<double>());
+        const at::Tensor none;
+        return finish_once(create_graph, "cross_attention", grads, {dq, dk, dv, none, none, none});
+    }
+};
+
+at::Tensor cross_attention_layer_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
+                                      const c10::optional<at::Tensor>& mask, c10::optional<double> scale)
+{
+    return std::get<0>(attention_forward(q, k, v, lengths, mask, scale, false));
+}
+
+at::Tensor cross_attention_layer_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
+                                          const c10::optional<at::Tensor>& mask, c10::optional<double> scale)
+{
+    check_no_tangent("cross_attention", {&q, &k, &v});
+    if (wants_grad({&q, &k, &v})) {
+        return CrossAttentionFunction::apply(q, k, v, lengths, mask, scale);
+    }
+    at::AutoDispatchBelowAutograd guard;
+    return cross_attention_layer_cuda(q, k, v, lengths, mask, scale);
+}
+
 // spectral._C.fft_impls(): the registry's names, in order, as a tuple of str.
 PyObject* py_fft_impls(PyObject*, PyObject*)
 {
@@ -1137,6 +1547,13 @@ TORCH_LIBRARY(spectral, m)
           " bool checkpoint8) -> Tensor");
     m.def("gated_mlp_layer(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation, bool checkpoint8)"
           " -> Tensor");
+    m.def("qk_norm_rotary_layer(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_positions,"
+          " Tensor? k_positions, float eps, float theta, int rotated, str pairs) -> Tensor[]");
+    m.def("cross_attention(Tensor q, Tensor k, Tensor v, Tensor? lengths=None, Tensor? mask=None, float? scale=None)"
+          " -> (Tensor, Tensor)");
+    m.def("cross_attention_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor stats,"
+          " Tensor? lengths=None, Tensor? mask=None, float? scale=None) -> (Tensor, Tensor, Tensor)");
+    m.def("cross_attention_layer(Tensor q, Tensor k, Tensor v, Tensor? lengths, Tensor? mask, float? scale) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(spectral, CUDA, m)
@@ -1163,12 +1580,18 @@ TORCH_LIBRARY_IMPL(spectral, CUDA, m)
     m.impl("gated_mlp_backward", &gated_mlp_backward_cuda);
     m.impl("group_norm_act_layer", &group_norm_act_layer_cuda);
     m.impl("gated_mlp_layer", &gated_mlp_layer_cuda);
+    m.impl("qk_norm_rotary_layer", &qk_norm_rotary_cuda);
+    m.impl("cross_attention", &cross_attention_cuda);
+    m.impl("cross_attention_backward", &cross_attention_backward_cuda);
+    m.impl("cross_attention_layer", &cross_attention_layer_cuda);
 }
 
 TORCH_LIBRARY_IMPL(spectral, AutogradCUDA, m)
 {
     m.impl("group_norm_act_layer", &group_norm_act_layer_autograd);
     m.impl("gated_mlp_layer", &gated_mlp_layer_autograd);
+    m.impl("qk_norm_rotary_layer", &qk_norm_rotary_layer_autograd);
+    m.impl("cross_attention_layer", &cross_attention_layer_autograd);
 }
 
 PyMODINIT_FUNC PyInit__C(void)

@@ -31,6 +31,19 @@ _f = ctypes.c_float
 _szp = ctypes.POINTER(ctypes.c_size_t)
 _ip = ctypes.POINTER(ctypes.c_int)
 
+
+class Heads(ctypes.Structure):
+    """spectral_heads: the queries, or the keys, of spectral_qk_norm_rotary and its backward."""
+
+    _fields_ = [
+        ("x", _p), ("stride", _ll * 3), ("weight", _p), ("positions", _p), ("position_stride", _ll * 3),
+        ("position_type", _i), ("heads", _i), ("tokens", _ll), ("out", _p), ("dy", _p), ("dweight", _p),
+    ]
+
+
+_heads = ctypes.POINTER(Heads)
+_strides = ctypes.POINTER(_ll)
+
 # name -> (restype, argtypes), in the order of include/spectral_b200.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spectral_last_error": (_s, []),
@@ -92,6 +105,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spectral_gated_mlp_backward_workspace": (_i, [_i, _ll, _i, _i, _i, _szp]),
     "spectral_gated_mlp_backward_workspace_for": (_i, [_p, _p, _i, _p, _p, _p, _i, _ll, _i, _i, _i, _szp]),
     "spectral_gated_mlp_backward": (_i, [_p] * 11 + [_i, _ll, _i, _i, _i, _i, _p, _p]),
+    "spectral_qk_norm_rotary": (_i, [_heads, _heads, _i, _ll, _i, _i, _i, _i, _f, _f, _p]),
+    "spectral_qk_norm_rotary_backward_workspace": (_i, [_i, _szp]),
+    "spectral_qk_norm_rotary_backward": (_i, [_heads, _heads, _i, _ll, _i, _i, _i, _i, _f, _f, _p, _p]),
+    "spectral_cross_attention_workspace": (_i, [_p] * 3 + [_strides, _i, _ll, _ll, _ll, _i, _i, _i, _szp]),
+    "spectral_cross_attention": (_i, [_p] * 3 + [_strides, _p, _i, _p, _p, _p, _i, _ll, _ll, _ll, _i, _i, _i, _f, _p, _p]),
+    "spectral_cross_attention_backward_workspace": (_i, [_p] * 3 + [_strides, _i, _ll, _ll, _ll, _i, _i, _i, _szp]),
+    "spectral_cross_attention_backward": (
+        _i, [_p] * 4 + [_strides, _p, _p, _p, _i] + [_p] * 4 + [_i, _ll, _ll, _ll, _i, _i, _i, _f, _p, _p]),
     "spectral_fp32_ceiling": (_i, [_p, _i, _i, _p, ctypes.POINTER(ctypes.c_double)]),
     "spectral_spectrum": (_i, [_s, _p, _p, _p, _ll, _i, _ll, _p]),
     "spectral_fir": (_i, [_s, _p, _p, _p, _ll, _i, _i, _ll, _p]),

@@ -1,6 +1,7 @@
 """Layers of a Fourier neural operator on this library's kernels, with hand-derived backwards:
-SpectralConv2d, the spectral convolution, and the pointwise half of an FNO block around it
-(GroupNormAct, GatedMLP, and FNOBlock, which joins the three).
+SpectralConv2d, the spectral convolution; the pointwise half of an FNO block around it (GroupNormAct,
+GatedMLP); CrossAttention, by which a field reads from states of another length; and FNOBlock, which
+joins them.
 
 SpectralConv2d.
 
@@ -139,6 +140,43 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     return torch.ops.spectral.gated_mlp_layer.default(x, w_gate, w_up, w_down, activation, checkpoint8)
 
 
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                   k_weight: torch.Tensor | None = None, q_positions: torch.Tensor | None = None,
+                   k_positions: torch.Tensor | None = None, *, eps: float = 1e-6, theta: float = 10000.0,
+                   rotated: int | None = None, pairs: str = "halves") -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Queries and keys ready for an attention, in one pass: each head x becomes u = x / sqrt(mean(x^2) + eps) *
+    weight, then its first `rotated` values are turned by position.
+
+    q (batch, tokens, heads, dim), dim at most 128, and k of the same batch and dim (or None: returns (q', None)),
+    strided views included; weights float32 (dim,) or None for 1. Positions (tokens, axes) or (batch, tokens,
+    axes), float32, int32 or int64; None: not turned. The rotated values fall into `axes` equal spans, one
+    for each axis; of a span's n pairs the i-th is turned by position * theta^(-i / n). pairs="halves" pairs value i
+    of a span with value i + n, "neighbours" value 2i with 2i + 1. rotated=None: as many values as 2 * axes
+    divides. Returns contiguous tensors of q's type. Differentiable in q, k and the weights."""
+    out = torch.ops.spectral.qk_norm_rotary_layer.default(
+        q, k, q_weight, k_weight, q_positions, k_positions, eps, theta, _rotated(rotated), pairs)
+    return out[0], out[1] if k is not None else None
+
+
+def _rotated(rotated: int | None) -> int:
+    if rotated is not None and rotated < 0:
+        raise ValueError(f"qk_norm_rotary: rotated must not be negative, got {rotated}")
+    return -1 if rotated is None else rotated
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: torch.Tensor | None = None,
+                    mask: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v for each sample and head: q (batch, queries, heads, dim) reads k and v (batch, keys,
+    kv_heads, dim), heads / kv_heads neighbouring query heads sharing a head of k and v; dim at most 128,
+    strided views included. scale: 1 / sqrt(dim) if None.
+
+    Only a sample's first lengths[sample] keys count (int32 or int64, (batch,)), and of them those where mask
+    ((batch, keys) or (1, keys) bool) is True; what lies in other places has no effect, whatever it is, and gets zero
+    gradients. A sample without keys gives zeros. Returns a contiguous tensor of q's shape and type.
+    Differentiable in q, k and v."""
+    return torch.ops.spectral.cross_attention_layer.default(q, k, v, lengths, mask, scale)
+
+
 class GroupNormAct(torch.nn.Module):
     """Group norm with learned scale and offset per channel, then the activation, on channels-last
     fields (group_norm_act)."""
@@ -183,22 +221,97 @@ class GatedMLP(torch.nn.Module):
                 f"checkpoint8={self.checkpoint8}")
 
 
+class CrossAttention(torch.nn.Module):
+    """Points x (b, ..., channels) read from states context (b, states, context_channels): queries from x, keys and
+    values from the context, queries and keys normalised for each head and turned by position (qk_norm_rotary), then
+    cross_attention and a projection back to `channels`.
+
+    Positions are coordinates on `axes` axes, for x (points, axes) or (b, points, axes) with its middle dimensions
+    flattened to points, for the context (states, axes) or (b, states, axes); None: not turned. lengths and mask say
+    which states count. Weights start iid N(0, 1 / fan-in); `dtype` is theirs and x's and the context's."""
+
+    def __init__(self, channels: int, context_channels: int, heads: int, *, kv_heads: int | None = None,
+                 head_dim: int | None = None, theta: float = 10000.0, pairs: str = "halves", eps: float = 1e-6,
+                 device=None, dtype=None):
+        super().__init__()
+        self.heads, self.kv_heads = heads, heads if kv_heads is None else kv_heads
+        if head_dim is None:
+            if channels % heads:
+                raise ValueError(f"CrossAttention: {heads} heads do not divide {channels} channels; give head_dim")
+            head_dim = channels // heads
+        self.head_dim, self.theta, self.pairs, self.eps = head_dim, theta, pairs, eps
+
+        def weight(rows: int, cols: int) -> torch.nn.Parameter:
+            return torch.nn.Parameter(torch.randn(rows, cols, device=device, dtype=dtype) / math.sqrt(max(1, cols)))
+
+        self.w_q = weight(heads * head_dim, channels)
+        self.w_k = weight(self.kv_heads * head_dim, context_channels)
+        self.w_v = weight(self.kv_heads * head_dim, context_channels)
+        self.w_out = weight(channels, heads * head_dim)
+        self.q_norm = torch.nn.Parameter(torch.ones(head_dim, device=device))
+        self.k_norm = torch.nn.Parameter(torch.ones(head_dim, device=device))
+
+    def forward(self, x: torch.Tensor, context: torch.Tensor, *, positions: torch.Tensor | None = None,
+                context_positions: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                mask: torch.Tensor | None = None) -> torch.Tensor:
+        b, states = x.shape[0], context.shape[1]
+        linear = torch.nn.functional.linear
+        q = linear(x, self.w_q).reshape(b, -1, self.heads, self.head_dim)
+        k = linear(context, self.w_k).reshape(b, states, self.kv_heads, self.head_dim)
+        v = linear(context, self.w_v).reshape(b, states, self.kv_heads, self.head_dim)
+        q, k = qk_norm_rotary(q, k, self.q_norm, self.k_norm, positions, context_positions, eps=self.eps, theta=self.theta,
+                              pairs=self.pairs)
+        out = cross_attention(q, k, v, lengths=lengths, mask=mask)
+        return linear(out.reshape(*x.shape[:-1], self.heads * self.head_dim), self.w_out)
+
+    def extra_repr(self) -> str:
+        return (f"{self.w_q.shape[1]}, {self.w_k.shape[1]}, heads={self.heads}, kv_heads={self.kv_heads}, "
+                f"head_dim={self.head_dim}")
+
+
 class FNOBlock(torch.nn.Module):
     """One Fourier-neural-operator block on real fields u (b, channels, n1, n2), float32:
 
         v = SpectralConv2d(u) as channels-last fields, in `dtype`
-        out = u + GatedMLP(GroupNormAct(v)), channels first again, float32
+        h = GroupNormAct(v)
+        h = h + CrossAttention(h, context)                 if the block has context_channels
+        out = u + GatedMLP(h), channels first again, float32
 
-    `dtype` is the pointwise half's type; checkpoint8=True keeps its two inputs in 8 bits."""
+    `dtype` is the pointwise half's type; checkpoint8=True keeps its two inputs in 8 bits.
+
+    With context_channels the points also read from states context (b, states, context_channels): sensors,
+    observations, another network's tokens. context_positions (states, 2) or (b, states, 2) place them in the domain,
+    whose extent is 1 along both axes; they and the grid's points, times `position_scale`, turn keys and queries."""
 
     def __init__(self, channels: int, hidden: int, m1: int, m2: int, *, groups: int = 8, activation: str = "gelu",
-                 checkpoint8: bool = False, impl: str = "stockham_r8", device=None, dtype: torch.dtype = torch.float32):
+                 checkpoint8: bool = False, impl: str = "stockham_r8", device=None, dtype: torch.dtype = torch.float32,
+                 context_channels: int | None = None, heads: int = 2, kv_heads: int | None = None,
+                 position_scale: float = 128.0):
         super().__init__()
         self.conv = SpectralConv2d(channels, channels, m1, m2, impl=impl, device=device)
         self.norm = GroupNormAct(groups, channels, activation=activation, checkpoint8=checkpoint8, device=device)
         self.mlp = GatedMLP(channels, hidden, activation=activation, checkpoint8=checkpoint8, device=device, dtype=dtype)
         self.dtype = dtype
+        self.position_scale = position_scale
+        self.attention = None
+        if context_channels is not None:
+            self.attention = CrossAttention(channels, context_channels, heads, kv_heads=kv_heads, device=device, dtype=dtype)
 
-    def forward(self, u: torch.Tensor) -> torch.Tensor:
+    def _grid(self, n1: int, n2: int, device) -> torch.Tensor:
+        first = torch.arange(n1, device=device, dtype=torch.float32) * (self.position_scale / n1)
+        second = torch.arange(n2, device=device, dtype=torch.float32) * (self.position_scale / n2)
+        return torch.stack(torch.meshgrid(first, second, indexing="ij"), -1).reshape(n1 * n2, 2)
+
+    def forward(self, u: torch.Tensor, context: torch.Tensor | None = None, *, context_positions: torch.Tensor | None = None,
+                lengths: torch.Tensor | None = None, mask: torch.Tensor | None = None) -> torch.Tensor:
         v = self.conv(u).permute(0, 2, 3, 1).to(self.dtype)
-        return u + self.mlp(self.norm(v)).permute(0, 3, 1, 2).to(u.dtype)
+        h = self.norm(v)
+        if (context is None) != (self.attention is None):
+            raise ValueError("FNOBlock: a context is given if, and only if, the block was made with context_channels")
+        if self.attention is not None:
+            places = grid = None
+            if context_positions is not None:
+                places = context_positions.float() * self.position_scale
+                grid = self._grid(u.shape[-2], u.shape[-1], u.device)
+            h = h + self.attention(h, context.to(self.dtype), positions=grid, context_positions=places, lengths=lengths, mask=mask)
+        return u + self.mlp(h).permute(0, 3, 1, 2).to(u.dtype)

@@ -396,6 +396,76 @@ SPECTRAL_API int spectral_gated_mlp_backward(const void* dy, const void* x, cons
                                              int channels, int hidden, int outputs, int activation, void* work,
                                              void* stream);
 
+/* --- reading from states of another length -------------------------------------------------------- */
+/* A field conditioned on sensors, observations or an encoder's tokens: its points make queries, those
+ * states make keys and values. No counterparts in the reference. Values of the three types above, sums and
+ * softmax statistics FP32, heads of at most SPECTRAL_HEAD_DIM_MAX values. */
+#define SPECTRAL_HEAD_DIM_MAX 128
+#define SPECTRAL_PAIRS_HALVES 0     /* value i of an axis's span with value i + span / 2 */
+#define SPECTRAL_PAIRS_NEIGHBOURS 1 /* value 2 i with value 2 i + 1 */
+#define SPECTRAL_POSITIONS_FLOAT32 0
+#define SPECTRAL_POSITIONS_INT32 1
+#define SPECTRAL_POSITIONS_INT64 2
+
+/* The queries, or the keys, of a spectral_qk_norm_rotary call. */
+typedef struct spectral_heads {
+    const void* x;                /* (batch, tokens, heads, dim), the values of a head side by side */
+    long long stride[3];          /* of sample, token and head, in values */
+    const float* weight;          /* dim floats, NULL for 1 */
+    const void* positions;        /* a position per sample, token and axis; NULL: no rotation */
+    long long position_stride[3]; /* of sample (0: shared), token and axis */
+    int position_type;            /* SPECTRAL_POSITIONS_* */
+    int heads;
+    long long tokens;
+    void* out;                    /* y, backward dx: (batch, tokens, heads, dim), contiguous */
+    const void* dy;               /* backward: of the same form */
+    float* dweight;               /* backward: dim floats, or NULL */
+} spectral_heads;
+
+/* The norm of each head and the rotation by position, of queries and keys in one pass (either may be
+ * NULL): u = x / sqrt(mean(x^2) + eps) * weight over a head; its first `rotated` values in `axes` equal spans,
+ * each for one axis of the positions; of a span's n = rotated / (2 axes) pairs (u1, u2) the i-th is turned by
+ * a = position * theta^(-i / n) to (u1 cos a - u2 sin a, u1 sin a + u2 cos a). Angles are formed in 64 bits;
+ * whole-number positions count up to 2^53. Results must not overlap inputs. */
+SPECTRAL_API int spectral_qk_norm_rotary(const spectral_heads* q, const spectral_heads* k, int dtype, long long batch, int dim,
+                                         int rotated, int axes, int pairs, float eps, float theta, void* stream);
+/* Its gradients from x and dy: out receives dx, dweight the weight's. Fixed summation order. work: as many
+ * complex values as spectral_qk_norm_rotary_backward_workspace says for the current device (NULL if no
+ * dweight is asked for). */
+SPECTRAL_API int spectral_qk_norm_rotary_backward_workspace(int dim, size_t* count);
+SPECTRAL_API int spectral_qk_norm_rotary_backward(const spectral_heads* q, const spectral_heads* k, int dtype, long long batch,
+                                                  int dim, int rotated, int axes, int pairs, float eps, float theta, void* work,
+                                                  void* stream);
+
+/* out = softmax(scale q k^T) v for each sample and head: q (batch, queries, heads, dim), k and v (batch, keys,
+ * kv_heads, dim), out (batch, queries, heads, dim). heads / kv_heads (1 to 128) neighbouring query heads share a
+ * head of k and v. strides: nine, of sample, token and head of q, k and v, in values (the values of a head lie side
+ * by side); NULL for contiguous arrays. A key counts if its index is below lengths[sample] (`batch`
+ * int32, or int64 if lengths64 is not 0; NULL: keys) and mask[sample * keys + key] is not 0 (bytes; NULL: all);
+ * what lies in the others' places, infinities and NaN among it, has no effect. A row without keys gives zeros.
+ * out is contiguous and must not overlap the inputs. stats (batch x kv_heads x queries heads / kv_heads pairs of
+ * floats, or NULL) is kept for the backward pass. Products of 16-bit values run on the tensor cores with FP32
+ * accumulators, the softmax's weights rounded to the type in between; float32 runs in FP32 throughout.
+ * work: as many complex values as the workspace function says for the same arrays (NULL is an array of unknown
+ * alignment). */
+SPECTRAL_API int spectral_cross_attention_workspace(const void* q, const void* k, const void* v, const long long* strides, int dtype,
+                                                    long long batch, long long queries, long long keys, int heads, int kv_heads,
+                                                    int dim, size_t* count);
+SPECTRAL_API int spectral_cross_attention(const void* q, const void* k, const void* v, const long long* strides, const void* lengths,
+                                          int lengths64, const void* mask, void* out, float* stats, int dtype, long long batch,
+                                          long long queries, long long keys, int heads, int kv_heads, int dim, float scale,
+                                          void* work, void* stream);
+/* Its gradients for dout, from the forward call's out and stats: dq, dk and dv, contiguous, of the type and shapes
+ * of q, k and v (zeros for keys that do not count). dout is contiguous. Fixed summation order. */
+SPECTRAL_API int spectral_cross_attention_backward_workspace(const void* q, const void* k, const void* v, const long long* strides,
+                                                             int dtype, long long batch, long long queries, long long keys, int heads,
+                                                             int kv_heads, int dim, size_t* count);
+SPECTRAL_API int spectral_cross_attention_backward(const void* dout, const void* q, const void* k, const void* v,
+                                                   const long long* strides, const void* out, const float* stats, const void* lengths,
+                                                   int lengths64, const void* mask, void* dq, void* dk, void* dv, int dtype,
+                                                   long long batch, long long queries, long long keys, int heads, int kv_heads, int dim,
+                                                   float scale, void* work, void* stream);
+
 /* The FP32 arithmetic ceiling, for the roofline of FP32-bound kernels such as the contraction
  * (reference: csrc/tools/peaks.cu:46-70, a separate tool there). Launches one full wave of CTAs
  * that run independent fused multiply-add chains and nothing else: scalar FFMA (packed == 0) or
