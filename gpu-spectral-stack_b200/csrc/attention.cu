@@ -668,6 +668,8 @@ struct ForwardPlan {
     }
 };
 
+std::size_t forward_workspace(const Call& c) { return c.dtype == SPECTRAL_FLOAT32 ? ForwardPlan(c).arena.size() : tensor_forward_workspace(c); }
+
 struct BackwardPlan {
     Parts of_rows, of_keys;
     Arena arena;
@@ -825,7 +827,7 @@ extern "C" int spectral_cross_attention_workspace(const void* q, const void* k, 
     c.v = v;
     *count = 0;
     if (c.pairs() * c.rows() > 0) {
-        *count = ForwardPlan(c).arena.size() / 8;
+        *count = forward_workspace(c) / 8;
     }
     return SPECTRAL_OK;
 }
@@ -873,10 +875,14 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
     c.stats = reinterpret_cast<float2*>(stats);
     c.scale = scale;
     try {
-        if (work == nullptr && ForwardPlan(c).arena.size() > 0) {
+        if (work == nullptr && forward_workspace(c) > 0) {
             return invalid("cross_attention: needs a workspace");
         }
-        with_dtype(dtype, [&](auto t) { forward<decltype(t)>(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream)); });
+        if (dtype == SPECTRAL_FLOAT32) {
+            forward<float>(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+        } else {
+            tensor_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+        }
         return SPECTRAL_OK;
     } catch (const InvalidArgument& e) {
         return invalid(e.what());

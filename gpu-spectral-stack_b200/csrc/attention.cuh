@@ -79,6 +79,10 @@ void join_splits(const Call& c, const float* partial, const float2* stats, int s
 // delta = sum over dim of dout out.
 void row_products(const Call& c, cudaStream_t stream);
 
+// The 16-bit kernels (attention_tc.cu).
+std::size_t tensor_forward_workspace(const Call& c);
+void tensor_forward(const Call& c, char* work, cudaStream_t stream);
+
 inline int pieces(long long n, long long per) { return static_cast<int>((n + per - 1) / per); }
 
 // A part of a workspace, in bytes; every array starts on 256.

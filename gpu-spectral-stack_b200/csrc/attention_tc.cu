@@ -1,0 +1,665 @@
+// Attention forward for 16-bit values on the 5th-generation tensor cores.
+//
+// A CTA keeps two tiles of 128 query rows and walks over tiles of 128 keys. Both products run on tcgen05: the
+// scores S = Q K^T into tensor memory, from where a thread per row takes its 128 scores to registers, and
+// O += P V with the weights P written back over S as the 16-bit operand. While one row tile's threads work on
+// their scores the tensor cores multiply for the other. A warp brings tiles of K and V in by TMA through a ring, a
+// warp issues the products, and with a length or a mask a warp wipes the values of keys that do not count.
+//
+// Softmax in one pass: a row's weights are 2^(c s - m) with m the largest c s when it was last moved, and m moves only
+// if a later score passes it by more than 2^8; then O in tensor memory and the sum are scaled. Weights reach 2^8 that way,
+// which changes nothing in bf16; float16 has them times 2^7, so that the smallest it keeps is 2^-31 of the largest.
+//
+// Work items are (row tiles, split of the keys, sample and key head); CTAs, one per SM, stay and take every
+// 148th. Few rows over many keys are split so that all SMs read, and the parts joined by a second kernel.
+
+#include "attention_tc.cuh"
+#include "mlp.cuh"
+
+#include <algorithm>
+
+namespace spectral::attention {
+namespace {
+
+constexpr float kSlack = 8.0f;  // in powers of two, see above
+
+struct Forward {
+    HeadMap q, k, v;
+    Call c;
+    int rows_per_tile = 0;    // 128 / group * group
+    int tokens_per_tile = 0;
+    int row_items = 0;        // pairs of row tiles
+    int splits = 1;
+    int split_tiles = 0;      // key tiles of a split
+    long long items = 0;
+    float factor = 1.0f;      // |scale| log2(e)
+    bool negative = false;    // scale < 0
+    float* partial = nullptr;
+    float2* part_stats = nullptr;
+    unsigned* fault = nullptr;
+};
+
+struct Item {
+    int b;
+    int head;
+    int split;
+    int row_tile;   // the first of the two
+    int tiles;      // of keys
+    int key0;
+    int end;        // keys before this count, but for the mask
+    int slots;      // row tiles with rows
+};
+
+__device__ __forceinline__ Item item_at(const Forward& g, long long i)
+{
+    Item it;
+    const long long r = i / g.row_items;
+    it.row_tile = static_cast<int>(i - r * g.row_items) * 2;
+    const long long pair = r / g.splits;
+    it.split = static_cast<int>(r - pair * g.splits);
+    it.b = static_cast<int>(pair / g.c.kv_heads);
+    it.head = static_cast<int>(pair - static_cast<long long>(it.b) * g.c.kv_heads);
+    it.key0 = it.split * g.split_tiles * kTile;
+    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * kTile);
+    it.tiles = it.end > it.key0 ? (it.end - it.key0 + kTile - 1) / kTile : 0;
+    it.slots = static_cast<long long>(it.row_tile + 1) * g.rows_per_tile < g.c.rows() ? 2 : 1;
+    return it;
+}
+
+template <int Boxes, bool Cut>
+struct Config {
+    static constexpr int kThreads = Cut ? 352 : 320;
+    static constexpr int kTileBytes = Boxes * kBox;
+    static constexpr int kStages = Boxes == 1 ? 8 : 5;  // of K and V tiles
+    static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
+    static constexpr int kO = 256;                       // tensor memory: S and P 0 and 1, then O 0 and 1
+    static constexpr int kCols = 512;
+    static_assert(kSmem <= kSmemMost - 1024, "shared memory");
+};
+
+template <class T, int Boxes, bool Cut>
+__global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kernel(const __grid_constant__ Forward g)
+{
+    using Cfg = Config<Boxes, Cut>;
+    constexpr bool kBf16 = std::is_same_v<T, bf16>;
+    constexpr float kOffset = kBf16 ? 0.0f : 7.0f;  // weights times 2^7
+    constexpr int kStages = Cfg::kStages;
+    extern __shared__ unsigned char smem_base[];
+    const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
+    const uint32_t ring = base + 2 * Cfg::kTileBytes;
+    __shared__ uint64_t q_full, q_empty, full[kStages], empty[kStages], clean[kStages], s_full[2], p_full[2], o_full[2], o_free[2], drain;
+    __shared__ uint32_t tmem_slot;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (warp == 8) {
+        umma::alloc<Cfg::kCols>(&tmem_slot);
+    }
+    if (threadIdx.x == 0) {
+        tma::mbar_init(&q_full, 1);
+        tma::mbar_init(&q_empty, 1);
+        for (int s = 0; s < kStages; ++s) {
+            tma::mbar_init(&full[s], 1);
+            tma::mbar_init(&empty[s], 1);
+            tma::mbar_init(&clean[s], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            tma::mbar_init(&s_full[x], 1);
+            tma::mbar_init(&p_full[x], 4);
+            tma::mbar_init(&o_full[x], 1);
+            tma::mbar_init(&o_free[x], 4);
+        }
+        tma::mbar_init(&drain, 1);
+        tma::fence_mbar_init();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    // The next grid may start from here: its CTAs cannot take this one's tensor memory any more.
+    allow_next_grid();
+    wait_for_previous_grid();
+    const Call& c = g.c;
+    bool ok = true;
+
+    if (warp == 8) {
+        // The TMA warp: Q of an item as soon as the one before is read, then its K and V tiles in turn.
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        const unsigned q_bytes = static_cast<unsigned>(g.rows_per_tile) * umma::kRowBytes * Boxes;
+        int stage = 0;
+        unsigned phase = 0, q_phase = 0;
+        long long issued = 0, q_issued = 0;
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at(g, i);
+            if (it.tiles == 0) {
+                continue;
+            }
+            ok = tma::mbar_wait(&q_empty, q_phase ^ 1u);
+            if (!ok) {
+                break;
+            }
+            q_phase ^= 1u;
+            if (umma::elect_one()) {
+                tma::mbar_arrive_expect_tx(&q_full, q_bytes * it.slots);
+                for (int x = 0; x < it.slots; ++x) {
+#pragma unroll
+                    for (int j = 0; j < Boxes; ++j) {
+                        load_heads(base + x * Cfg::kTileBytes + j * kBox, g.q, j * umma::kAtom, it.head * c.group,
+                                   (it.row_tile + x) * g.tokens_per_tile, it.b, &q_full);
+                    }
+                }
+            }
+            __syncwarp();
+            ++q_issued;
+            for (int t = 0; ok && t < 2 * it.tiles; ++t) {
+                ok = tma::mbar_wait(&empty[stage], phase ^ 1u);
+                if (!ok) {
+                    break;
+                }
+                if (umma::elect_one()) {
+                    tma::mbar_arrive_expect_tx(&full[stage], Cfg::kTileBytes);
+#pragma unroll
+                    for (int j = 0; j < Boxes; ++j) {
+                        load_heads(ring + stage * Cfg::kTileBytes + j * kBox, (t & 1) != 0 ? g.v : g.k, j * umma::kAtom, it.head,
+                                   it.key0 + (t >> 1) * kTile, it.b, &full[stage]);
+                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok) {  // the loads in flight land (bounded) before the shared memory is given up
+            bool drained = q_issued == 0 || tma::mbar_wait(&q_full, static_cast<unsigned>(q_issued - 1) & 1u);
+            for (long long i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+                drained = tma::mbar_wait(&full[i % kStages], static_cast<unsigned>(i / kStages) & 1u) && drained;
+            }
+            if (lane == 0) {
+                atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
+            }
+        }
+    } else if (warp == 9) {
+        // The MMA warp, one elected lane issues.
+        const int steps = (c.dim + 15) / 16;
+        const uint32_t score = umma::instruction(kBf16, false, false, kTile, kTile);
+        const uint32_t weigh = umma::instruction(kBf16, false, true, kTile, steps * 16);
+        int stage = 0;
+        unsigned phase = 0, q_phase = 0, cleaned = 0;
+        unsigned slot_items[2] = {0, 0};
+        unsigned p_phases[2] = {0, 0};
+        const auto scores = [&](int x, uint32_t k_tile) {
+            if (umma::elect_one()) {
+                const uint64_t a = umma::desc_k(base + x * Cfg::kTileBytes), b = umma::desc_k(k_tile);
+                for (int s = 0; s < steps; ++s) {
+                    const uint64_t step = (s & 3) * umma::kStepK + (s >> 2) * (kBox >> 4);
+                    umma::mma(tmem + x * kTile, a + step, b + step, score, s > 0);
+                }
+                umma::commit(&s_full[x]);
+            }
+            __syncwarp();
+        };
+        const auto advance = [&] {
+            if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        };
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at(g, i);
+            if (it.tiles == 0) {
+                continue;
+            }
+            ok = tma::mbar_wait(&q_full, q_phase) && tma::mbar_wait(&full[stage], phase);
+            if (!ok) {
+                break;
+            }
+            q_phase ^= 1u;
+            umma::fence_after_sync();
+            for (int x = 0; x < it.slots; ++x) {
+                scores(x, ring + stage * Cfg::kTileBytes);
+            }
+            if (umma::elect_one()) {
+                umma::commit(&empty[stage]);
+                if (it.tiles == 1) {
+                    umma::commit(&q_empty);
+                }
+            }
+            __syncwarp();
+            advance();
+            for (int t = 0; ok && t < it.tiles; ++t) {
+                const int v_stage = stage;
+                // Only V tiles pass the wiping warp, so their barriers count their own phases.
+                ok = Cut ? tma::mbar_wait(&clean[stage], cleaned >> stage & 1u) : tma::mbar_wait(&full[stage], phase);
+                cleaned ^= 1u << stage;
+                advance();
+                const bool more = t + 1 < it.tiles;
+                const int k_stage = stage;
+                if (ok && more) {
+                    ok = tma::mbar_wait(&full[stage], phase);
+                    advance();
+                }
+                if (!ok) {
+                    break;
+                }
+                for (int x = 0; ok && x < it.slots; ++x) {
+                    ok = tma::mbar_wait(&p_full[x], p_phases[x]) && (t > 0 || tma::mbar_wait(&o_free[x], (slot_items[x] & 1u) ^ 1u));
+                    if (!ok) {
+                        break;
+                    }
+                    p_phases[x] ^= 1u;
+                    umma::fence_after_sync();
+                    if (umma::elect_one()) {
+                        const uint64_t b = umma::desc_mn<kBox>(ring + v_stage * Cfg::kTileBytes);
+#pragma unroll
+                        for (int s = 0; s < kTile / 16; ++s) {
+                            mma_tmem(tmem + Cfg::kO + x * Boxes * 64, tmem + x * kTile + s * 8, b + umma::kStepMn * s, weigh, t > 0 || s > 0);
+                        }
+                        if (!more) {
+                            umma::commit(&o_full[x]);
+                        }
+                    }
+                    __syncwarp();
+                    if (more) {
+                        scores(x, ring + k_stage * Cfg::kTileBytes);
+                    }
+                }
+                if (!ok) {
+                    break;
+                }
+                if (umma::elect_one()) {
+                    umma::commit(&empty[v_stage]);
+                    if (more) {
+                        umma::commit(&empty[k_stage]);
+                        if (t + 2 == it.tiles) {
+                            umma::commit(&q_empty);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            for (int x = 0; x < it.slots; ++x) {
+                ++slot_items[x];
+            }
+        }
+        if (!ok) {
+            if (umma::elect_one()) {
+                umma::commit(&drain);
+            }
+            __syncwarp();
+            const bool drained = tma::mbar_wait(&drain, 0);
+            if (lane == 0) {
+                atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
+            }
+        }
+    } else if (Cut && warp == 10) {
+        // The wiping warp: every V tile passes through it.
+        int stage = 0;
+        unsigned phase = 0;
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at(g, i);
+            for (int t = 0; ok && t < it.tiles; ++t) {
+                uint32_t w[4];
+                tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
+                if (++stage == kStages) {  // past the K tile
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                ok = tma::mbar_wait(&full[stage], phase);
+                if (ok && !all_count(w)) {
+                    wipe_rows(ring + stage * Cfg::kTileBytes, Boxes, w);
+                }
+                __syncwarp();
+                if (ok && lane == 0) {
+                    umma::arrive(&clean[stage]);
+                }
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(g.fault, tma::kFaultWaitTimeout);
+        }
+    } else if (warp < 8) {
+        // A thread per row: warps 0 to 3 the first tile's, 4 to 7 the second's.
+        const int x = warp >> 2;
+        const int quad = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+        const uint32_t s_at = tmem + lanes + x * kTile;
+        const uint32_t o_at = tmem + lanes + Cfg::kO + x * Boxes * 64;
+        const int local = quad * 32 + lane;
+        unsigned s_phase = 0, o_phase = 0;
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at(g, i);
+            if (x >= it.slots) {
+                continue;
+            }
+            const long long row = static_cast<long long>(it.row_tile + x) * g.rows_per_tile + local;
+            const bool live = local < g.rows_per_tile && row < c.rows();
+            // A warp without rows only keeps the barriers going; what lies in its lanes reaches no one.
+            const bool idle = quad * 32 >= g.rows_per_tile || static_cast<long long>(it.row_tile + x) * g.rows_per_tile + quad * 32 >= c.rows();
+            float m = -INFINITY, sum = 0.0f;
+            for (int t = 0; ok && t < it.tiles; ++t) {
+                uint32_t w[4];
+                if (!idle) {
+                    tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
+                }
+                ok = tma::mbar_wait(&s_full[x], s_phase);
+                if (!ok) {
+                    break;
+                }
+                s_phase ^= 1u;
+                umma::fence_after_sync();
+                if (!idle) {
+                    float s[4][32];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        umma::load32(s_at + 32 * j, s[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        umma::load_wait(s[j]);
+                    }
+                    if (g.negative) {
+#pragma unroll
+                        for (int j = 0; j < 128; ++j) {
+                            s[j / 32][j % 32] = -s[j / 32][j % 32];
+                        }
+                    }
+                    if (!all_count(w)) {
+#pragma unroll
+                        for (int j = 0; j < 128; ++j) {
+                            s[j / 32][j % 32] = (w[j / 32] >> (j % 32) & 1u) != 0 ? s[j / 32][j % 32] : -INFINITY;
+                        }
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        top[j] = s[j][0];
+#pragma unroll
+                        for (int k = 1; k < 32; ++k) {
+                            top[j] = fmaxf(top[j], s[j][k]);
+                        }
+                    }
+                    const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.factor;
+                    const bool move = largest > m + kSlack || (m == -INFINITY && largest > -INFINITY);
+                    if (__any_sync(0xffffffffu, move)) {
+                        // Each row by its own scores alone: its bits do not depend on its neighbours.
+                        const float keep = !move ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - largest);
+                        m = move ? largest : m;
+                        sum *= keep;
+                        if (t > 0) {  // the products before are done: their commit came with these scores
+                            for (int d = 0; d < c.dim; d += 16) {
+                                float o[16];
+                                umma::load16(o_at + d, o);
+                                umma::load_wait(o);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) {
+                                    o[k] *= keep;
+                                }
+                                store16(o_at + d, o);
+                            }
+                        }
+                    }
+                    const float2 shift = pair((m == -INFINITY ? 0.0f : -m) + kOffset);
+                    float2 total = pair(0.0f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 e = fma2(make_float2(s[j][2 * k], s[j][2 * k + 1]), pair(g.factor), shift);
+                            const float2 v = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            total = total + v;
+                            p[k] = pack2<T>(v);
+                        }
+                        store16(s_at + 16 * j, p);
+                    }
+                    sum += total.x + total.y;
+                    store_wait();
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    umma::arrive(&p_full[x]);
+                }
+            }
+            if (!ok) {
+                break;
+            }
+            if (it.tiles > 0) {
+                ok = tma::mbar_wait(&o_full[x], o_phase);
+                if (!ok) {
+                    break;
+                }
+                o_phase ^= 1u;
+                umma::fence_after_sync();
+            }
+            const long long at = static_cast<long long>(it.b) * c.kv_heads + it.head;
+            const float base_m = m == -INFINITY ? (g.splits > 1 ? m : 0.0f) : m - kOffset;
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const long long part_row = (it.split * c.pairs() + at) * c.rows() + row;
+            T* out = live ? static_cast<T*>(c.out) + c.row_at(it.b, it.head, row) : nullptr;
+            if (!idle) {
+                for (int d = 0; d < c.dim; d += 16) {
+                    float o[16];
+                    if (it.tiles > 0) {
+                        umma::load16(o_at + d, o);
+                        umma::load_wait(o);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            o[k] = 0.0f;
+                        }
+                    }
+                    if (live) {
+                        const int valid = min(16, c.dim - d);
+                        if (g.splits > 1) {
+                            mlp::store_values<float>(g.partial + part_row * c.dim + d, o, valid);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                o[k] *= inverse;
+                            }
+                            mlp::store_values<T>(out + d, o, valid);
+                        }
+                    }
+                }
+                if (live && g.splits > 1) {
+                    g.part_stats[part_row] = make_float2(base_m, sum);
+                } else if (live && c.stats != nullptr) {
+                    c.stats[at * c.rows() + row] = make_float2(base_m, sum);
+                }
+            }
+            if (it.tiles > 0) {
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    umma::arrive(&o_free[x]);
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(g.fault, tma::kFaultWaitTimeout);
+        }
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    if (warp == 8) {
+        umma::dealloc<Cfg::kCols>(tmem);
+    }
+}
+
+// --- staging -------------------------------------------------------------------------------------------
+
+struct StageJob {
+    const void* source;
+    void* target;
+    Strides stride;
+    long long tokens;
+    int heads;
+    long long values;  // of the target
+};
+struct StageJobs {
+    StageJob job[4];
+    int dim;
+    int pitch;
+};
+
+// 16-bit values, whatever their type: a thread per target value, zeros in the padding.
+__global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ StageJobs g)
+{
+    allow_next_grid();
+    wait_for_previous_grid();
+    const StageJob& j = g.job[blockIdx.y];
+    const auto* source = static_cast<const unsigned short*>(j.source);
+    auto* target = static_cast<unsigned short*>(j.target);
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < j.values; i += static_cast<long long>(gridDim.x) * 256) {
+        const long long row = i / g.pitch;
+        const int d = static_cast<int>(i - row * g.pitch);
+        const long long token = row / j.heads;
+        const long long b = token / j.tokens;
+        target[i] = d < g.dim ? source[b * j.stride.sample + (token - b * j.tokens) * j.stride.token + (row - token * j.heads) * j.stride.head + d]
+                              : static_cast<unsigned short>(0);
+    }
+}
+
+// --- host ------------------------------------------------------------------------------------------------
+
+constexpr int kSms = 148;
+
+struct Plan {
+    Operand q, k, v;
+    int row_items = 0;
+    int splits = 1;
+    int split_tiles = 0;
+    std::size_t partial = 0, stats = 0;
+    Arena arena;
+
+    explicit Plan(const Call& c)
+    {
+        q = operand(arena, c.q, c.qs, c.batch, c.queries, c.kv_heads * c.group, c.dim, false);
+        k = operand(arena, c.k, c.ks, c.batch, c.keys, c.kv_heads, c.dim, true);
+        v = operand(arena, c.v, c.vs, c.batch, c.keys, c.kv_heads, c.dim, true);
+        const int rows = kTile / c.group * c.group;
+        row_items = pieces(pieces(c.rows(), rows), 2);
+        // Splits of the keys: the fewest turns of the busiest CTA, counted in key tiles, where an item costs about two
+        // more (its first loads and scores, its last products and stores); parts are written and joined.
+        const long long tiles = pieces(c.keys, kTile);
+        const long long base = c.pairs() * row_items;
+        const long long least = std::max(1LL, (tiles + kLongestSum / kTile - 1) / (kLongestSum / kTile));
+        double best = 0.0;
+        for (long long s = least; s <= std::max(least, std::min(tiles, 128LL)); ++s) {
+            const long long span = (tiles + s - 1) / s;
+            if (s > least && (tiles + span - 1) / span != s) {
+                continue;  // the same span as fewer splits
+            }
+            const double turns = static_cast<double>((base * s + kSms - 1) / kSms) * (static_cast<double>(span) + 2.0) + (s > 1 ? 4.0 + 0.02 * s : 0.0);
+            if (s == least || turns < best) {
+                best = turns;
+                splits = static_cast<int>(s);
+                split_tiles = static_cast<int>(span);
+            }
+        }
+        splits = static_cast<int>(std::max(1LL, split_tiles == 0 ? 1LL : (tiles + split_tiles - 1) / split_tiles));
+        if (splits > 1) {
+            const std::size_t all = static_cast<std::size_t>(c.pairs()) * c.rows() * splits;
+            partial = arena.take(all * c.dim * sizeof(float));
+            stats = arena.take(all * sizeof(float2));
+        }
+    }
+};
+
+template <class T, int Boxes, bool Cut>
+void launch(const Forward& g, cudaStream_t stream)
+{
+    using Cfg = Config<Boxes, Cut>;
+    const auto kernel = forward_kernel<T, Boxes, Cut>;
+    static std::atomic<int> cache[kMaxDevices];
+    const unsigned grid = persistent_grid(reinterpret_cast<const void*>(kernel), Cfg::kThreads, Cfg::kSmem, cache, g.items);
+    launch_pdl(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, g);
+}
+
+}  // namespace
+
+void stage(const Operand* const* operands, int count, int batch, int dim, char* work, cudaStream_t stream)
+{
+    StageJobs g;
+    g.dim = dim;
+    g.pitch = (dim + 7) / 8 * 8;
+    int jobs = 0;
+    long long most = 0;
+    for (int i = 0; i < count; ++i) {
+        const Operand& o = *operands[i];
+        if (o.staged && batch * o.tokens > 0) {
+            const long long values = batch * o.tokens * o.heads * g.pitch;
+            g.job[jobs++] = {o.source, work + o.at, o.stride, o.tokens, o.heads, values};
+            most = std::max(most, values);
+        }
+    }
+    if (jobs > 0) {
+        const auto grid = static_cast<unsigned>(std::min<long long>((most + 255) / 256, kSms * 16));
+        launch_pdl(stage_kernel, dim3(grid, jobs), dim3(256), 0, stream, g);
+    }
+}
+
+std::size_t tensor_forward_workspace(const Call& c) { return Plan(c).arena.size(); }
+
+void tensor_forward(const Call& c, char* work, cudaStream_t stream)
+{
+    const Plan plan(c);
+    const Operand* const operands[3] = {&plan.q, &plan.k, &plan.v};
+    stage(operands, 3, c.batch, c.dim, work, stream);
+    const bool is_bf16 = c.dtype == SPECTRAL_BFLOAT16;
+    Forward g;
+    g.c = c;
+    g.tokens_per_tile = kTile / c.group;
+    g.rows_per_tile = g.tokens_per_tile * c.group;
+    g.row_items = plan.row_items;
+    g.splits = plan.splits;
+    g.split_tiles = plan.split_tiles;
+    g.items = c.pairs() * plan.row_items * plan.splits;
+    g.negative = c.scale < 0.0f;
+    // A factor of 0 would turn the -infinity of a key that does not count into a NaN.
+    g.factor = std::max(std::abs(c.scale) * kLog2e, 1.17549435e-38f);
+    g.partial = reinterpret_cast<float*>(work + plan.partial);
+    g.part_stats = reinterpret_cast<float2*>(work + plan.stats);
+    g.fault = device_fault_word();
+    g.q = head_map(plan.q.base(work), is_bf16, plan.q.strides(c.dim), c.batch, c.queries, c.kv_heads * c.group, c.dim, c.group, g.tokens_per_tile);
+    const void* keys[2] = {plan.k.base(work), plan.v.base(work)};
+    if (c.keys > 0) {
+        g.k = head_map(keys[0], is_bf16, plan.k.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile);
+        g.v = head_map(keys[1], is_bf16, plan.v.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile);
+    }
+    const bool cut = c.lengths != nullptr || c.mask != nullptr;
+    const auto run = [&](auto t, auto boxes) {
+        using T = decltype(t);
+        constexpr int Boxes = decltype(boxes)::value;
+        if (cut) {
+            launch<T, Boxes, true>(g, stream);
+        } else {
+            launch<T, Boxes, false>(g, stream);
+        }
+    };
+    const auto with_boxes = [&](auto t) {
+        if (c.dim <= 64) {
+            run(t, std::integral_constant<int, 1>{});
+        } else {
+            run(t, std::integral_constant<int, 2>{});
+        }
+    };
+    if (is_bf16) {
+        with_boxes(bf16{});
+    } else {
+        with_boxes(f16{});
+    }
+    if (plan.splits > 1) {
+        join_splits(c, g.partial, g.part_stats, plan.splits, stream);
+    }
+}
+
+}  // namespace spectral::attention

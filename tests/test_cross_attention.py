@@ -332,11 +332,14 @@ def test_the_same_bits_every_time_on_a_side_stream_and_from_a_graph(queries, key
 def test_past_two_to_the_31_values():
     keys = (1 << 25) + 77
     k = torch.zeros(1, keys, 1, 64, dtype=torch.bfloat16, device="cuda")
-    q, k1, v1, _ = inputs(1, 1, 200, 1, 1, 64, torch.bfloat16)
+    q, k1, _, _ = inputs(1, 1, 200, 1, 1, 64, torch.bfloat16)
     mask = torch.zeros(1, keys, dtype=torch.bool, device="cuda")
     mask[:, -200:] = True
     k[:, -200:] = k1
-    assert torch.equal(cross_attention(q, k, k, mask=mask)[0, 0], cross_attention(q, k1, k1)[0, 0])
+    # Which keys share a tile differs from that of the 200 alone, and with it where a running maximum moves: not the
+    # same bits, the same bounds.
+    all_count = torch.ones(1, 200, dtype=torch.bool, device="cuda")
+    within(cross_attention(q, k, k, mask=mask), formula(q, k1, k1, q, all_count, 0.125, torch.bfloat16)[0], "out")
 
 
 @pytest.mark.gpu
