@@ -24,32 +24,32 @@ constexpr int kPitch = Dim + 4;
 constexpr int kScorePitch = kKeys + 4;
 
 // Rows [first, first + Rows) of queries (or of an array of their shape), zeros past the end.
-template <class T, int Dim, int Rows>
+template <int Dim, int Rows>
 __device__ __forceinline__ void load_rows(float* tile, const Call& c, const void* base, const Strides& s, int b, int head,
                                           long long first)
 {
-    const T* p = static_cast<const T*>(base) + b * s.sample;
+    const float* p = static_cast<const float*>(base) + b * s.sample;
     for (int i = threadIdx.x; i < Rows * Dim; i += kThreads) {
         const int row = i / Dim, d = i - row * Dim;
         const long long r = first + row;
         float v = 0.0f;
         if (r < c.rows() && d < c.dim) {
             const long long t = r / c.group;
-            v = to_float(p[t * s.token + (head * c.group + (r - t * c.group)) * s.head + d]);
+            v = p[t * s.token + (head * c.group + (r - t * c.group)) * s.head + d];
         }
         tile[row * kPitch<Dim> + d] = v;
     }
 }
 
 // Keys [first, first + kKeys) of k or v, zeros where `valid` is not set.
-template <class T, int Dim>
+template <int Dim>
 __device__ __forceinline__ void load_keys(float* tile, const Call& c, const void* base, const Strides& s, int b, int head,
                                           long long first, unsigned long long valid)
 {
-    const T* p = static_cast<const T*>(base) + b * s.sample + head * s.head;
+    const float* p = static_cast<const float*>(base) + b * s.sample + head * s.head;
     for (int i = threadIdx.x; i < kKeys * Dim; i += kThreads) {
         const int key = i / Dim, d = i - key * Dim;
-        tile[key * kPitch<Dim> + d] = (valid >> key & 1) != 0 && d < c.dim ? to_float(p[(first + key) * s.token + d]) : 0.0f;
+        tile[key * kPitch<Dim> + d] = (valid >> key & 1) != 0 && d < c.dim ? p[(first + key) * s.token + d] : 0.0f;
     }
 }
 
@@ -165,17 +165,17 @@ __device__ __forceinline__ void weigh_keys(const float* s, const float* m, int k
     }
 }
 
-template <class T, int Dim>
-__device__ __forceinline__ void store_pairs(T* p, int dim, int col, const float2 (&v)[kPairs<Dim>], float factor)
+template <int Dim>
+__device__ __forceinline__ void store_pairs(float* p, int dim, int col, const float2 (&v)[kPairs<Dim>], float factor)
 {
 #pragma unroll
     for (int j = 0; j < kPairs<Dim>; ++j) {
         const int d = j * 32 + 2 * col;
         if (d < dim) {
-            p[d] = from_float<T>(v[j].x * factor);
+            p[d] = v[j].x * factor;
         }
         if (d + 1 < dim) {
-            p[d + 1] = from_float<T>(v[j].y * factor);
+            p[d + 1] = v[j].y * factor;
         }
     }
 }
@@ -207,7 +207,7 @@ struct Parts {
 };
 
 // Forward: 16 R rows per CTA, thread (row group, column) of a 16 x 16 grid.
-template <class T, int Dim, int R>
+template <int Dim, int R>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const Parts parts)
 {
     constexpr int kRows = 16 * R;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const P
     const int length = length_of(c, b);
     const long long begin = part * parts.span;
     const long long end = min(static_cast<long long>(length), begin + parts.span);
-    load_rows<T, Dim, kRows>(sq, c, c.q, c.qs, b, head, first);
+    load_rows<Dim, kRows>(sq, c, c.q, c.qs, b, head, first);
     const float scale = c.scale * kLog2e;
     float most[R], total[R];
     float2 acc[R][kPairs<Dim>];
@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const P
         if (valid == 0) {
             continue;
         }
-        load_keys<T, Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
-        load_keys<T, Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+        load_keys<Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
+        load_keys<Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
         __syncthreads();
         float s[R][4];
         products<Dim, R>(sq, sk, row0, col, s);
@@ -287,13 +287,13 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const P
         }
         const float base = most[i] == -INFINITY ? 0.0f : most[i];
         if (parts.count == 1) {
-            store_pairs<T, Dim>(static_cast<T*>(c.out) + c.row_at(b, head, r), c.dim, col, acc[i], total[i] == 0.0f ? 0.0f : 1.0f / total[i]);
+            store_pairs<Dim>(static_cast<float*>(c.out) + c.row_at(b, head, r), c.dim, col, acc[i], total[i] == 0.0f ? 0.0f : 1.0f / total[i]);
             if (c.stats != nullptr && col == 0) {
                 c.stats[at * c.rows() + r] = make_float2(base, total[i]);
             }
         } else {
             const long long to = (part * c.pairs() + at) * c.rows() + r;
-            store_pairs<float, Dim>(parts.first + to * c.dim, c.dim, col, acc[i], 1.0f);
+            store_pairs<Dim>(parts.first + to * c.dim, c.dim, col, acc[i], 1.0f);
             if (col == 0) {
                 parts.stats[to] = make_float2(most[i], total[i]);
             }
@@ -336,7 +336,7 @@ __device__ __forceinline__ void row_constants(const Call& c, long long at, long 
     }
 }
 
-template <class T, int Dim>
+template <int Dim>
 __global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, const Parts parts)
 {
     extern __shared__ __align__(16) float shared[];
@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, c
     allow_next_grid();
     wait_for_previous_grid();
     const unsigned long long valid = valid_keys(c, b, length_of(c, b), key0, votes);
-    load_keys<T, Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
-    load_keys<T, Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+    load_keys<Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
+    load_keys<Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
     const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
                         c.dim};
     float2 dk[4][kPairs<Dim>], dv[4][kPairs<Dim>];
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, c
     const long long end = min(c.rows(), (part + 1) * parts.span);
     for (long long first = part * parts.span; first < end && valid != 0; first += 64) {
         __syncthreads();
-        load_rows<T, Dim, 64>(sq, c, c.q, c.qs, b, head, first);
-        load_rows<T, Dim, 64>(sdo, c, c.dout, dense, b, head, first);
+        load_rows<Dim, 64>(sq, c, c.q, c.qs, b, head, first);
+        load_rows<Dim, 64>(sdo, c, c.dout, dense, b, head, first);
         float2 stats[4];
         float delta[4], p[4][4], ds[4][4];
         row_constants(c, at, first, row0, stats, delta);
@@ -399,17 +399,17 @@ __global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, c
         }
         if (parts.count == 1) {
             const long long to = ((static_cast<long long>(b) * c.keys + key) * c.kv_heads + head) * c.dim;
-            store_pairs<T, Dim>(static_cast<T*>(c.dk) + to, c.dim, col, dk[i], c.scale);
-            store_pairs<T, Dim>(static_cast<T*>(c.dv) + to, c.dim, col, dv[i], 1.0f);
+            store_pairs<Dim>(static_cast<float*>(c.dk) + to, c.dim, col, dk[i], c.scale);
+            store_pairs<Dim>(static_cast<float*>(c.dv) + to, c.dim, col, dv[i], 1.0f);
         } else {
             const long long to = ((part * c.pairs() + at) * c.keys + key) * c.dim;
-            store_pairs<float, Dim>(parts.first + to, c.dim, col, dk[i], 1.0f);
-            store_pairs<float, Dim>(parts.second + to, c.dim, col, dv[i], 1.0f);
+            store_pairs<Dim>(parts.first + to, c.dim, col, dk[i], 1.0f);
+            store_pairs<Dim>(parts.second + to, c.dim, col, dv[i], 1.0f);
         }
     }
 }
 
-template <class T, int Dim>
+template <int Dim>
 __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, const Parts parts)
 {
     extern __shared__ __align__(16) float shared[];
@@ -429,8 +429,8 @@ __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, c
     wait_for_previous_grid();
     const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
                         c.dim};
-    load_rows<T, Dim, 64>(sq, c, c.q, c.qs, b, head, first);
-    load_rows<T, Dim, 64>(sdo, c, c.dout, dense, b, head, first);
+    load_rows<Dim, 64>(sq, c, c.q, c.qs, b, head, first);
+    load_rows<Dim, 64>(sdo, c, c.dout, dense, b, head, first);
     float2 stats[4];
     float delta[4];
     row_constants(c, at, first, row0, stats, delta);
@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, c
         if (valid == 0) {
             continue;
         }
-        load_keys<T, Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
-        load_keys<T, Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+        load_keys<Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
+        load_keys<Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
         __syncthreads();
         float p[4][4], ds[4][4];
         score_gradients<Dim>(sq, sk, sv, sdo, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
@@ -471,10 +471,10 @@ __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, c
             continue;
         }
         if (parts.count == 1) {
-            store_pairs<T, Dim>(static_cast<T*>(c.dq) + c.row_at(b, head, r), c.dim, col, dq[i], c.scale);
+            store_pairs<Dim>(static_cast<float*>(c.dq) + c.row_at(b, head, r), c.dim, col, dq[i], c.scale);
         } else {
             const long long to = ((part * c.pairs() + at) * c.rows() + r) * c.dim;
-            store_pairs<float, Dim>(parts.first + to, c.dim, col, dq[i], 1.0f);
+            store_pairs<Dim>(parts.first + to, c.dim, col, dq[i], 1.0f);
         }
     }
 }
@@ -482,15 +482,14 @@ __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, c
 // --- around them -------------------------------------------------------------------------------------
 
 // A warp per row.
-template <class T>
 __global__ void __launch_bounds__(kThreads) row_products_kernel(const Call c)
 {
     allow_next_grid();
     wait_for_previous_grid();
     const int lane = threadIdx.x & 31;
     const long long all = static_cast<long long>(c.batch) * c.queries * c.kv_heads * c.group;
-    const T* __restrict__ o = static_cast<const T*>(c.out);
-    const T* __restrict__ g = static_cast<const T*>(c.dout);
+    const float* __restrict__ o = static_cast<const float*>(c.out);
+    const float* __restrict__ g = static_cast<const float*>(c.dout);
     for (long long i = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); i < all;
          i += static_cast<long long>(gridDim.x) * (kThreads / 32)) {
         float sum = 0.0f;
@@ -498,7 +497,7 @@ __global__ void __launch_bounds__(kThreads) row_products_kernel(const Call c)
         for (int k = 0; k < SPECTRAL_HEAD_DIM_MAX / 32; ++k) {
             const int d = lane + 32 * k;
             if (d < c.dim) {
-                sum = fmaf(to_float(o[i * c.dim + d]), to_float(g[i * c.dim + d]), sum);
+                sum = fmaf(o[i * c.dim + d], g[i * c.dim + d], sum);
             }
         }
 #pragma unroll
@@ -614,13 +613,14 @@ void join_splits(const Call& c, const float* partial, const float2* stats, int s
     });
 }
 
+namespace {
+
+// delta = sum over dim of dout out.
 void row_products(const Call& c, cudaStream_t stream)
 {
     const auto grid = static_cast<unsigned>(std::min<long long>((c.pairs() * c.rows() + 7) / 8, 148 * 16));
-    with_dtype(c.dtype, [&](auto t) { launch_pdl(row_products_kernel<decltype(t)>, dim3(grid), dim3(kThreads), 0, stream, c); });
+    launch_pdl(row_products_kernel, dim3(grid), dim3(kThreads), 0, stream, c);
 }
-
-namespace {
 
 constexpr int kSms = 148;
 
@@ -701,7 +701,6 @@ void launch(K kernel, dim3 grid, std::size_t smem, cudaStream_t stream, const A&
     launch_pdl(kernel, grid, dim3(kThreads), smem, stream, args...);
 }
 
-template <class T>
 void forward(const Call& c, char* work, cudaStream_t stream)
 {
     ForwardPlan plan(c);
@@ -713,9 +712,9 @@ void forward(const Call& c, char* work, cudaStream_t stream)
         constexpr int Dim = decltype(d)::value;
         const std::size_t smem = ((rows + 2 * kKeys) * kPitch<Dim> + rows * kScorePitch) * sizeof(float);
         if (rows == 16) {
-            launch(forward_kernel<T, Dim, 1>, grid, smem, stream, c, plan.parts);
+            launch(forward_kernel<Dim, 1>, grid, smem, stream, c, plan.parts);
         } else {
-            launch(forward_kernel<T, Dim, 4>, grid, smem, stream, c, plan.parts);
+            launch(forward_kernel<Dim, 4>, grid, smem, stream, c, plan.parts);
         }
     });
     if (plan.parts.count > 1) {
@@ -723,7 +722,6 @@ void forward(const Call& c, char* work, cudaStream_t stream)
     }
 }
 
-template <class T>
 void backward(Call c, char* work, cudaStream_t stream)
 {
     BackwardPlan plan(c);
@@ -736,9 +734,9 @@ void backward(Call c, char* work, cudaStream_t stream)
         constexpr int Dim = decltype(d)::value;
         const std::size_t tiles = 4 * 64 * kPitch<Dim> * sizeof(float);
         constexpr std::size_t kScores = 64 * kScorePitch * sizeof(float);
-        launch(keys_backward_kernel<T, Dim>, dim3(pieces(c.keys, 64), static_cast<unsigned>(c.pairs()), plan.of_rows.count), tiles + 2 * kScores, stream,
+        launch(keys_backward_kernel<Dim>, dim3(pieces(c.keys, 64), static_cast<unsigned>(c.pairs()), plan.of_rows.count), tiles + 2 * kScores, stream,
                c, plan.of_rows);
-        launch(rows_backward_kernel<T, Dim>, dim3(pieces(c.rows(), 64), static_cast<unsigned>(c.pairs()), plan.of_keys.count), tiles + kScores, stream, c,
+        launch(rows_backward_kernel<Dim>, dim3(pieces(c.rows(), 64), static_cast<unsigned>(c.pairs()), plan.of_keys.count), tiles + kScores, stream, c,
                plan.of_keys);
     });
     if (plan.of_rows.count > 1) {
@@ -879,7 +877,7 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
             return invalid("cross_attention: needs a workspace");
         }
         if (dtype == SPECTRAL_FLOAT32) {
-            forward<float>(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+            forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
         } else {
             tensor_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
         }
@@ -892,7 +890,7 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
     }
 }
 
-extern "C" int spectral_cross_attention_backward_workspace(const void* q, const void* k, const void* v, const long long* strides, int dtype,
+extern "C" int spectral_cross_attention_backward_workspace(const void* dout, const void* q, const void* k, const void* v, const long long* strides, int dtype,
                                                            long long batch, long long queries, long long keys, int heads, int kv_heads,
                                                            int dim, size_t* count)
 {
@@ -903,12 +901,13 @@ extern "C" int spectral_cross_attention_backward_workspace(const void* q, const 
     if (status != SPECTRAL_OK || count == nullptr) {
         return status != SPECTRAL_OK ? status : invalid("cross_attention_backward_workspace: null count");
     }
+    c.dout = dout;
     c.q = q;
     c.k = k;
     c.v = v;
     *count = 0;
     if (c.pairs() * c.rows() > 0 && keys > 0) {
-        *count = BackwardPlan(c).arena.size() / 8;
+        *count = (dtype == SPECTRAL_FLOAT32 ? BackwardPlan(c).arena.size() : tensor_backward_workspace(c)) / 8;
     }
     return SPECTRAL_OK;
 }
@@ -974,7 +973,11 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         c.dk = dk;
         c.dv = dv;
         c.scale = scale;
-        with_dtype(dtype, [&](auto t) { backward<decltype(t)>(c, static_cast<char*>(work), s); });
+        if (dtype == SPECTRAL_FLOAT32) {
+            backward(c, static_cast<char*>(work), s);
+        } else {
+            tensor_backward(c, static_cast<char*>(work), s);
+        }
         return SPECTRAL_OK;
     } catch (const InvalidArgument& e) {
         return invalid(e.what());

@@ -76,12 +76,11 @@ void add_parts(const Call& c, const float* partial, int parts, bool of_keys, voi
 // sum p.
 void join_splits(const Call& c, const float* partial, const float2* stats, int splits, cudaStream_t stream);
 
-// delta = sum over dim of dout out.
-void row_products(const Call& c, cudaStream_t stream);
-
-// The 16-bit kernels (attention_tc.cu).
+// The 16-bit kernels (attention_tc.cu, attention_tc_backward.cu).
 std::size_t tensor_forward_workspace(const Call& c);
 void tensor_forward(const Call& c, char* work, cudaStream_t stream);
+std::size_t tensor_backward_workspace(const Call& c);
+void tensor_backward(const Call& c, char* work, cudaStream_t stream);
 
 inline int pieces(long long n, long long per) { return static_cast<int>((n + per - 1) / per); }
 

@@ -1,0 +1,872 @@
+// Attention backward for 16-bit values on the 5th-generation tensor cores.
+//
+// With p = 2^(c s - lse) (c = scale log2(e), lse = m + log2(sum) of the forward pass), g the upstream gradient,
+// delta = sum over dim of g out and ds = p (g v^T - delta):
+//   dv = p^T g,   dk = scale ds^T q,   dq = scale ds k
+// Two kernels of one form, each sum with one owner, so that nothing is atomic and equal inputs give equal bits. A CTA
+// owns 128 keys (their k and v stay in shared memory) and walks over row tiles for dk and dv, or owns 128 rows (q
+// and g) and walks over key tiles for dq; the scores are computed in both. Per step, on tcgen05:
+//   S = X0 Y0^T and D = X1 Y1^T into tensor memory (X owned, Y the tiles of the walk)
+//   P over S and dS over D, as 16-bit operands; A1 += P Y1 (keys), A0 += dS Y0, accumulators in tensor memory.
+// Eight warps, a thread per owned row and half of the columns, first turn S to P, then D to dS; the products that
+// need P and the next S run under the second half of that, those that need dS and the next D under the first half of the
+// next step. A warp brings the tiles by TMA, one issues the products, and where keys are cut and walked over a warp wipes
+// the values of those that do not count.
+//
+// float16 keeps p times 2^15 and ds times a power of two that no |ds| takes past 2^15: |g v - delta| is at most
+// 2 max|g| max|v| (norms of rows and keys that count), which the kernel before these finds. Unscaled, weights of 2^-14 and
+// less (16384 keys and more) would be subnormal, and small gradients zero.
+
+#include "attention_tc.cuh"
+#include "mlp.cuh"
+
+#include <algorithm>
+
+namespace spectral::attention {
+namespace {
+
+constexpr int kSms = 148;
+constexpr int kConstants = 2 * kTile;        // floats per row tile: lse of its rows, then delta
+constexpr int kNormCtas = 4 * kSms;          // of the constants kernel, at most
+constexpr float kWeightPower = 15.0f;        // float16's p times 2^15
+
+struct Backward {
+    HeadMap x0, x1, y0, y1;
+    Call c;
+    int rows_per_tile = 0;
+    int tokens_per_tile = 0;
+    int row_tiles = 0;
+    int key_tiles = 0;
+    int parts = 1;
+    int part_tiles = 0;   // tiles walked over per part
+    long long items = 0;
+    float factor = 1.0f;  // c
+    const float* constants = nullptr;  // (pair, row tile, kConstants)
+    const float* norms = nullptr;      // float16: the CTAs' largest squares of rows of g, then of v
+    int norm_count = 0;
+    float* partial0 = nullptr;
+    float* partial1 = nullptr;
+    unsigned* fault = nullptr;
+};
+
+struct Item {
+    int b;
+    int head;
+    int part;
+    int tile;    // owned
+    int first;   // tile walked over first
+    int tiles;   // how many
+    int end;     // keys before this count, but for the mask
+};
+
+// Rows: the CTA owns rows and walks over keys.
+template <bool Rows>
+__device__ __forceinline__ Item item_at(const Backward& g, long long i)
+{
+    Item it;
+    const int owned = Rows ? g.row_tiles : g.key_tiles;
+    const long long r = i / owned;
+    it.tile = static_cast<int>(i - r * owned);
+    const long long pair = r / g.parts;
+    it.part = static_cast<int>(r - pair * g.parts);
+    it.b = static_cast<int>(pair / g.c.kv_heads);
+    it.head = static_cast<int>(pair - static_cast<long long>(it.b) * g.c.kv_heads);
+    it.end = length_of(g.c, it.b);
+    it.first = it.part * g.part_tiles;
+    const int walked = Rows ? (it.end + kTile - 1) / kTile : it.tile * kTile < it.end ? g.row_tiles : 0;
+    it.tiles = max(0, min(g.part_tiles, walked - it.first));
+    return it;
+}
+
+template <int Boxes, bool Rows, bool Wipe>
+struct Config {
+    static constexpr int kThreads = Wipe ? 352 : 320;
+    static constexpr int kTileBytes = Boxes * kBox;
+    static constexpr int kConstantBytes = Rows ? 0 : kConstants * 4;
+    static constexpr int kStageBytes = 2 * kTileBytes;  // Y0, Y1
+    static constexpr int kStages = Boxes == 1 ? 4 : 2;
+    static constexpr int kSmem = 2 * kTileBytes + kStages * (kStageBytes + kConstantBytes) + 1024;
+    static constexpr int kD = 128;                       // tensor memory: S and P, D and dS, A0, A1
+    static constexpr int kA0 = 256;
+    static constexpr int kA1 = 256 + Boxes * 64;
+    static constexpr int kCols = 512;
+    static_assert(kSmem <= kSmemMost - 1024, "shared memory");
+};
+
+template <class T, int Boxes, bool Rows, bool Wipe>
+__global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backward_kernel(const __grid_constant__ Backward g)
+{
+    using Cfg = Config<Boxes, Rows, Wipe>;
+    constexpr bool kBf16 = std::is_same_v<T, bf16>;
+    constexpr int kStages = Cfg::kStages;
+    extern __shared__ unsigned char smem_base[];
+    const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
+    unsigned char* const generic = smem_base + (base - tma::smem_addr(smem_base));
+    const uint32_t ring = base + 2 * Cfg::kTileBytes;
+    const float* const constants = reinterpret_cast<const float*>(generic + 2 * Cfg::kTileBytes + kStages * Cfg::kStageBytes);
+    __shared__ uint64_t x_full, x_empty, full[kStages], empty[kStages], clean[kStages], s_full, d_full, p_ready, ds_ready, acc_full, acc_free, drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ float norm_of[2][12];
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (warp == 8) {
+        umma::alloc<Cfg::kCols>(&tmem_slot);
+    }
+    if (threadIdx.x == 0) {
+        tma::mbar_init(&x_full, 1);
+        tma::mbar_init(&x_empty, 1);
+        for (int s = 0; s < kStages; ++s) {
+            tma::mbar_init(&full[s], 1);
+            tma::mbar_init(&empty[s], 1);
+            tma::mbar_init(&clean[s], 1);
+        }
+        tma::mbar_init(&s_full, 1);
+        tma::mbar_init(&d_full, 1);
+        tma::mbar_init(&p_ready, 8);
+        tma::mbar_init(&ds_ready, 8);
+        tma::mbar_init(&acc_full, 1);
+        tma::mbar_init(&acc_free, 8);
+        tma::mbar_init(&drain, 1);
+        tma::fence_mbar_init();
+    }
+    if constexpr (!Rows) {
+        // Rows of a tile that no box writes (128 % group) are reduced over: zeros, once.
+        const int spare = kTile - g.rows_per_tile;
+        for (int i = threadIdx.x; i < 2 * kStages * Boxes * spare * 8; i += Cfg::kThreads) {
+            const int box = i / (spare * 8), at = i - box * spare * 8;
+            *reinterpret_cast<uint4*>(generic + (2 * Boxes + box) * kBox + (g.rows_per_tile + at / 8) * umma::kRowBytes + at % 8 * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+        tma::fence_proxy_async();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    // The next grid may start from here: its CTAs cannot take this one's tensor memory any more.
+    allow_next_grid();
+    wait_for_previous_grid();
+    const Call& c = g.c;
+    bool ok = true;
+
+    // float16: the power of two that ds is held in.
+    float ds_scale = 1.0f;
+    if constexpr (!kBf16) {
+        float top[2] = {0.0f, 0.0f};
+        for (int i = threadIdx.x; i < 2 * g.norm_count; i += Cfg::kThreads) {
+            const int which = i >= g.norm_count ? 1 : 0;
+            top[which] = fmaxf(top[which], g.norms[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2) {
+                top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+            }
+            if (lane == 0) {
+                norm_of[k][warp] = top[k];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            top[k] = 0.0f;
+            for (int i = 0; i < Cfg::kThreads / 32; ++i) {
+                top[k] = fmaxf(top[k], norm_of[k][i]);
+            }
+        }
+        const float most = 2.0f * sqrtf(top[0]) * sqrtf(top[1]);
+        // 2^(14 - floor(log2(most))) times most is below 2^15.
+        const int power = most > 0.0f ? 14 - ilogbf(most) : 0;
+        ds_scale = exp2f(static_cast<float>(max(-60, min(60, power))));
+    }
+
+    if (warp == 8) {
+        // The TMA warp: the owned tiles as soon as the item before has no more use for its own, then Y0, Y1 in turn.
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        const unsigned row_bytes = static_cast<unsigned>(g.rows_per_tile) * umma::kRowBytes * Boxes;
+        const unsigned owned_bytes = 2 * (Rows ? row_bytes : Cfg::kTileBytes);
+        const unsigned walked_bytes = 2 * (Rows ? Cfg::kTileBytes : row_bytes) + Cfg::kConstantBytes;
+        int stage = 0;
+        unsigned phase = 0, x_phase = 0;
+        long long issued = 0, x_issued = 0;
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows>(g, i);
+            if (it.tiles == 0) {
+                continue;
+            }
+            ok = tma::mbar_wait(&x_empty, x_phase ^ 1u);
+            if (!ok) {
+                break;
+            }
+            x_phase ^= 1u;
+            const int x_head = Rows ? it.head * c.group : it.head;
+            const int y_head = Rows ? it.head : it.head * c.group;
+            const int x_token = it.tile * (Rows ? g.tokens_per_tile : kTile);
+            if (umma::elect_one()) {
+                tma::mbar_arrive_expect_tx(&x_full, owned_bytes);
+#pragma unroll
+                for (int j = 0; j < Boxes; ++j) {
+                    load_heads(base + j * kBox, g.x0, j * umma::kAtom, x_head, x_token, it.b, &x_full);
+                    load_heads(base + Cfg::kTileBytes + j * kBox, g.x1, j * umma::kAtom, x_head, x_token, it.b, &x_full);
+                }
+            }
+            __syncwarp();
+            ++x_issued;
+            for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
+                ok = tma::mbar_wait(&empty[stage], phase ^ 1u);
+                if (!ok) {
+                    break;
+                }
+                if (umma::elect_one()) {
+                    const uint32_t y = ring + stage * Cfg::kStageBytes;
+                    const int y_token = t * (Rows ? kTile : g.tokens_per_tile);
+                    tma::mbar_arrive_expect_tx(&full[stage], walked_bytes);
+#pragma unroll
+                    for (int j = 0; j < Boxes; ++j) {
+                        load_heads(y + j * kBox, g.y0, j * umma::kAtom, y_head, y_token, it.b, &full[stage]);
+                        load_heads(y + Cfg::kTileBytes + j * kBox, g.y1, j * umma::kAtom, y_head, y_token, it.b, &full[stage]);
+                    }
+                    if constexpr (!Rows) {
+                        const long long at = (static_cast<long long>(it.b) * c.kv_heads + it.head) * g.row_tiles + t;
+                        tma::bulk_g2s(const_cast<float*>(constants) + stage * kConstants, g.constants + at * kConstants, Cfg::kConstantBytes,
+                                      &full[stage]);
+                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok) {  // the loads in flight land (bounded) before the shared memory is given up
+            bool drained = x_issued == 0 || tma::mbar_wait(&x_full, static_cast<unsigned>(x_issued - 1) & 1u);
+            for (long long i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+                drained = tma::mbar_wait(&full[i % kStages], static_cast<unsigned>(i / kStages) & 1u) && drained;
+            }
+            if (lane == 0) {
+                atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
+            }
+        }
+    } else if (warp == 9) {
+        // The MMA warp, one elected lane issues.
+        const int steps = (c.dim + 15) / 16;
+        const uint32_t score = umma::instruction(kBf16, false, false, kTile, kTile);
+        const uint32_t weigh = umma::instruction(kBf16, false, true, kTile, steps * 16);
+        int stage = 0;
+        unsigned phase = 0, x_phase = 0, step_phase = 0, acc_phase = 0;
+        // S (k = 0) or D (k = 1) from the owned tiles and a stage's.
+        const auto scores = [&](int k, int y_stage, uint64_t* done) {
+            if (umma::elect_one()) {
+                const uint64_t a = umma::desc_k(base + k * Cfg::kTileBytes);
+                const uint64_t b = umma::desc_k(ring + y_stage * Cfg::kStageBytes + k * Cfg::kTileBytes);
+                for (int s = 0; s < steps; ++s) {
+                    const uint64_t step = (s & 3) * umma::kStepK + (s >> 2) * (kBox >> 4);
+                    umma::mma(tmem + k * Cfg::kD, a + step, b + step, score, s > 0);
+                }
+                umma::commit(done);
+            }
+            __syncwarp();
+        };
+        // A0 += dS Y0 (k = 0), A1 += P Y1 (k = 1). The halves of P and dS lie 64 columns apart.
+        const auto weighed = [&](int k, int y_stage, bool accumulate) {
+            const uint64_t b = umma::desc_mn<kBox>(ring + y_stage * Cfg::kStageBytes + k * Cfg::kTileBytes);
+            const uint32_t a = tmem + (k == 0 ? Cfg::kD : 0);
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s) {
+                mma_tmem(tmem + (k == 0 ? Cfg::kA0 : Cfg::kA1), a + (s >> 2) * 64 + (s & 3) * 8, b + umma::kStepMn * s, weigh, accumulate || s > 0);
+            }
+        };
+        const auto arrived = [&](int y_stage, unsigned y_phase) { return tma::mbar_wait(Wipe ? &clean[y_stage] : &full[y_stage], y_phase); };
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows>(g, i);
+            if (it.tiles == 0) {
+                continue;
+            }
+            ok = tma::mbar_wait(&x_full, x_phase) && arrived(stage, phase);
+            if (!ok) {
+                break;
+            }
+            x_phase ^= 1u;
+            umma::fence_after_sync();
+            scores(0, stage, &s_full);
+            scores(1, stage, &d_full);
+            for (int t = 0; ok && t < it.tiles; ++t) {
+                const bool more = t + 1 < it.tiles;
+                const int now = stage;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                ok = tma::mbar_wait(&p_ready, step_phase) && (t > 0 || tma::mbar_wait(&acc_free, acc_phase ^ 1u)) && (!more || arrived(stage, phase));
+                if (!ok) {
+                    break;
+                }
+                umma::fence_after_sync();
+                if constexpr (!Rows) {
+                    if (umma::elect_one()) {
+                        weighed(1, now, t > 0);
+                    }
+                    __syncwarp();
+                }
+                if (more) {
+                    scores(0, stage, &s_full);
+                }
+                ok = tma::mbar_wait(&ds_ready, step_phase);
+                if (!ok) {
+                    break;
+                }
+                step_phase ^= 1u;
+                umma::fence_after_sync();
+                if (umma::elect_one()) {
+                    weighed(0, now, t > 0);
+                    umma::commit(&empty[now]);
+                    if (!more) {
+                        umma::commit(&acc_full);
+                        umma::commit(&x_empty);
+                    }
+                }
+                __syncwarp();
+                if (more) {
+                    scores(1, stage, &d_full);
+                }
+            }
+            acc_phase ^= 1u;
+        }
+        if (!ok) {
+            if (umma::elect_one()) {
+                umma::commit(&drain);
+            }
+            __syncwarp();
+            const bool drained = tma::mbar_wait(&drain, 0);
+            if (lane == 0) {
+                atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
+            }
+        }
+    } else if (Wipe && warp == 10) {
+        // The wiping warp: every stage passes through it. (Only k is reduced over; masked scores are dropped.)
+        int stage = 0;
+        unsigned phase = 0;
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows>(g, i);
+            for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
+                uint32_t w[4];
+                tile_bits(c, it.b, it.end, t * kTile, w);
+                ok = tma::mbar_wait(&full[stage], phase);
+                if (ok && !all_count(w)) {
+                    wipe_rows(ring + stage * Cfg::kStageBytes, Boxes, w);
+                }
+                __syncwarp();
+                if (ok && lane == 0) {
+                    umma::arrive(&clean[stage]);
+                }
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(g.fault, tma::kFaultWaitTimeout);
+        }
+    } else if (warp < 8) {
+        // A thread per owned row: warps 0 to 3 the first 64 columns, 4 to 7 the others.
+        const int half = warp >> 2;
+        const int local = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + half * 64;
+        const uint32_t d_at = s_at + Cfg::kD;
+        int stage = 0;
+        unsigned phase = 0, step_phase = 0, acc_phase = 0;
+        const float power = kBf16 ? 0.0f : kWeightPower;
+        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows>(g, i);
+            const long long pair_at = static_cast<long long>(it.b) * c.kv_heads + it.head;
+            // Rows: this row's constants. Keys: whether this key counts.
+            float2 shift = pair(0.0f), delta = pair(0.0f);
+            bool counts = true;
+            const long long row = static_cast<long long>(it.tile) * (Rows ? g.rows_per_tile : kTile) + local;
+            if constexpr (Rows) {
+                const float* at = g.constants + (pair_at * g.row_tiles + it.tile) * kConstants + local;
+                shift = pair(-at[0]);
+                delta = pair(at[kTile]);
+            } else {
+                counts = row < it.end && (c.mask == nullptr || c.mask[static_cast<long long>(it.b) * c.keys + row] != 0);
+            }
+            const bool whole = __all_sync(0xffffffffu, counts);
+            for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
+                uint32_t w[4];
+                if constexpr (Rows) {
+                    tile_bits(c, it.b, it.end, t * kTile, w);
+                } else {
+                    ok = tma::mbar_wait(&full[stage], phase);
+                }
+                const float* lse = constants + stage * kConstants + half * 64;
+                ok = ok && tma::mbar_wait(&s_full, step_phase);
+                if (!ok) {
+                    break;
+                }
+                umma::fence_after_sync();
+                float p[2][32];
+                umma::load32(s_at, p[0]);
+                umma::load32(s_at + 32, p[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    umma::load_wait(p[j]);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float2 a = shift, b = shift;
+                        if constexpr (!Rows) {
+                            const float4 l = *reinterpret_cast<const float4*>(lse + 32 * j + k);
+                            a = make_float2(-l.x, -l.y);
+                            b = make_float2(-l.z, -l.w);
+                        }
+                        a = fma2(make_float2(p[j][k], p[j][k + 1]), pair(g.factor), a);
+                        b = fma2(make_float2(p[j][k + 2], p[j][k + 3]), pair(g.factor), b);
+                        p[j][k] = exp2_fast(a.x);
+                        p[j][k + 1] = exp2_fast(a.y);
+                        p[j][k + 2] = exp2_fast(b.x);
+                        p[j][k + 3] = exp2_fast(b.y);
+                    }
+                }
+                if constexpr (Rows) {
+                    if (!all_count(w)) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) {
+                            const uint32_t word = half == 0 ? w[j / 32] : w[2 + j / 32];
+                            p[j / 32][j % 32] = (word >> (j % 32) & 1u) != 0 ? p[j / 32][j % 32] : 0.0f;
+                        }
+                    }
+                } else {
+                    if (!whole) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) {
+                            p[j / 32][j % 32] = counts ? p[j / 32][j % 32] : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t out[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float2 v = make_float2(p[j][2 * k], p[j][2 * k + 1]);
+                            if constexpr (!kBf16) {
+                                v = v * pair(exp2f(kWeightPower));
+                            }
+                            out[k] = pack2<T>(v);
+                        }
+                        store16(s_at + 16 * j, out);
+                    }
+                    store_wait();
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    umma::arrive(&p_ready);
+                }
+                ok = tma::mbar_wait(&d_full, step_phase);
+                if (!ok) {
+                    break;
+                }
+                step_phase ^= 1u;
+                umma::fence_after_sync();
+                float d[2][32];
+                umma::load32(d_at, d[0]);
+                umma::load32(d_at + 32, d[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    umma::load_wait(d[j]);
+                    uint32_t out[16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float2 a = delta, b = delta;
+                        if constexpr (!Rows) {
+                            const float4 l = *reinterpret_cast<const float4*>(lse + kTile + 32 * j + k);
+                            a = make_float2(l.x, l.y);
+                            b = make_float2(l.z, l.w);
+                        }
+                        a = (make_float2(d[j][k], d[j][k + 1]) - a) * make_float2(p[j][k], p[j][k + 1]);
+                        b = (make_float2(d[j][k + 2], d[j][k + 3]) - b) * make_float2(p[j][k + 2], p[j][k + 3]);
+                        if constexpr (!kBf16) {
+                            a = a * pair(ds_scale);
+                            b = b * pair(ds_scale);
+                        }
+                        d[j][k] = a.x;
+                        d[j][k + 1] = a.y;
+                        d[j][k + 2] = b.x;
+                        d[j][k + 3] = b.y;
+                    }
+                    // A key that does not count may have made D anything.
+                    if constexpr (Rows) {
+                        if (!all_count(w)) {
+                            const uint32_t word = half == 0 ? w[j] : w[2 + j];
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                d[j][k] = (word >> k & 1u) != 0 ? d[j][k] : 0.0f;
+                            }
+                        }
+                    } else if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            d[j][k] = counts ? d[j][k] : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        out[k] = pack2<T>(make_float2(d[j][2 * k], d[j][2 * k + 1]));
+                    }
+                    store16(d_at + 16 * j, out);
+                }
+                store_wait();
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    umma::arrive(&ds_ready);
+                }
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!ok) {
+                break;
+            }
+            if (it.tiles > 0) {
+                ok = tma::mbar_wait(&acc_full, acc_phase);
+                if (!ok) {
+                    break;
+                }
+                acc_phase ^= 1u;
+                umma::fence_after_sync();
+            }
+            // Keys: the first warps store dk, the others dv. Rows: each half of dq.
+            const bool of_v = !Rows && half == 1;
+            const int span = (c.dim + 15) / 16;
+            const int from = Rows ? (half == 0 ? 0 : (span + 1) / 2 * 16) : 0;
+            const int to = Rows && half == 0 ? (span + 1) / 2 * 16 : c.dim;
+            const float factor = it.tiles == 0 || !counts ? 0.0f : of_v ? exp2f(-power) : (g.parts > 1 ? 1.0f : c.scale) / ds_scale;
+            const bool live = Rows ? local < g.rows_per_tile && row < c.rows() : row < c.keys;
+            const long long entries = Rows ? c.rows() : c.keys;
+            const long long part_row = (it.part * c.pairs() + pair_at) * entries + row;
+            float* partial = of_v ? g.partial1 : g.partial0;
+            T* result = static_cast<T*>(Rows ? c.dq : of_v ? c.dv : c.dk);
+            const long long at = Rows ? c.row_at(it.b, it.head, row) : ((static_cast<long long>(it.b) * c.keys + row) * c.kv_heads + it.head) * c.dim;
+            for (int d = from; d < to && d < c.dim; d += 16) {
+                float a[16];
+                if (it.tiles > 0) {
+                    umma::load16(tmem + lanes + (of_v ? Cfg::kA1 : Cfg::kA0) + d, a);
+                    umma::load_wait(a);
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    a[k] = it.tiles == 0 || !counts ? 0.0f : a[k] * factor;
+                }
+                if (live) {
+                    if (g.parts > 1) {
+                        mlp::store_values<float>(partial + part_row * c.dim + d, a, min(16, c.dim - d));
+                    } else {
+                        mlp::store_values<T>(result + at + d, a, min(16, c.dim - d));
+                    }
+                }
+            }
+            if (it.tiles > 0) {
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    umma::arrive(&acc_free);
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(g.fault, tma::kFaultWaitTimeout);
+        }
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    if (warp == 8) {
+        umma::dealloc<Cfg::kCols>(tmem);
+    }
+}
+
+// --- the rows' constants -----------------------------------------------------------------------------------
+
+// lse (infinite for rows that are not there or have no keys, so that their weights are 0) and delta of every entry of
+// every row tile, `lanes` lanes of eight values a row. float16: also the largest squares of g's rows and v's
+// keys that this CTA met (finite ones).
+template <class T, bool Vectors>
+__global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __restrict__ out, float* __restrict__ norms, int rows_per_tile,
+                                                        int row_tiles, int lanes)
+{
+    __shared__ float top_of[2][8];
+    allow_next_grid();
+    wait_for_previous_grid();
+    const int lane = threadIdx.x & 31;
+    const int sub = lane & (lanes - 1);
+    const int per_cta = 256 / lanes;
+    const T* __restrict__ o = static_cast<const T*>(c.out);
+    const T* __restrict__ g = static_cast<const T*>(c.dout);
+    const auto fetch = [&](const T* p) {
+        Vec<T, 8> v{};
+        if (sub * 8 < c.dim) {
+            if constexpr (Vectors) {
+                v = *reinterpret_cast<const Vec<T, 8>*>(p + sub * 8);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v.v[j] = sub * 8 + j < c.dim ? p[sub * 8 + j] : from_float<T>(0.0f);
+                }
+            }
+        }
+        return widen(v);
+    };
+    const auto total = [&](float2 v) {
+        float s = v.x + v.y;
+        for (int k = lanes / 2; k > 0; k /= 2) {
+            s += __shfl_xor_sync(0xffffffffu, s, k);
+        }
+        return s;
+    };
+    float top[2] = {0.0f, 0.0f};
+    const long long all = c.pairs() * row_tiles * kTile;
+    // Whole warps stay in the loops together: they shuffle.
+    for (long long base = static_cast<long long>(blockIdx.x) * per_cta; base < all; base += static_cast<long long>(gridDim.x) * per_cta) {
+        const long long i = base + threadIdx.x / lanes;
+        const int local = static_cast<int>(i % kTile);
+        const long long tile = i / kTile;
+        const long long pair_at = tile / row_tiles;
+        const long long r = (tile - pair_at * row_tiles) * rows_per_tile + local;
+        const bool there = i < all && local < rows_per_tile && r < c.rows();
+        float2 dot = pair(0.0f), square = pair(0.0f);
+        if (there) {
+            const int b = static_cast<int>(pair_at / c.kv_heads);
+            const long long at = c.row_at(b, static_cast<int>(pair_at - static_cast<long long>(b) * c.kv_heads), r);
+            const Floats<8> x = fetch(o + at), y = fetch(g + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                dot = fma2(x.p[j], y.p[j], dot);
+                square = fma2(y.p[j], y.p[j], square);
+            }
+        }
+        const float delta = total(dot);
+        if constexpr (std::is_same_v<T, f16>) {
+            const float s = total(square);
+            top[0] = s < INFINITY ? fmaxf(top[0], s) : top[0];
+        }
+        if (sub == 0 && i < all) {
+            float lse = INFINITY;
+            if (there) {
+                const float2 s = c.stats[pair_at * c.rows() + r];
+                lse = s.y == 0.0f ? INFINITY : s.x + log2f(s.y);
+            }
+            float* at = out + tile * kConstants + local;
+            at[0] = lse;
+            at[kTile] = delta;
+        }
+    }
+    if constexpr (std::is_same_v<T, f16>) {
+        const T* __restrict__ v = static_cast<const T*>(c.v);
+        const long long keys = c.pairs() * c.keys;
+        for (long long base = static_cast<long long>(blockIdx.x) * per_cta; base < keys; base += static_cast<long long>(gridDim.x) * per_cta) {
+            const long long i = base + threadIdx.x / lanes;
+            const long long pair_at = i / c.keys;
+            const int key = static_cast<int>(i - pair_at * c.keys);
+            const int b = static_cast<int>(pair_at / c.kv_heads);
+            float2 square = pair(0.0f);
+            if (i < keys && key < length_of(c, b) && (c.mask == nullptr || c.mask[static_cast<long long>(b) * c.keys + key] != 0)) {
+                const T* at = v + b * c.vs.sample + key * c.vs.token + (pair_at - static_cast<long long>(b) * c.kv_heads) * c.vs.head;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = sub * 8 + j < c.dim ? to_float(at[sub * 8 + j]) : 0.0f;
+                    square.x = fmaf(x, x, square.x);
+                }
+            }
+            const float s = total(square);
+            top[1] = s < INFINITY ? fmaxf(top[1], s) : top[1];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int s = 16; s > 0; s /= 2) {
+                top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], s));
+            }
+            if (lane == 0) {
+                top_of[k][threadIdx.x >> 5] = top[k];
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            float m = 0.0f;
+            for (int w = 0; w < 8; ++w) {
+                m = fmaxf(m, top_of[threadIdx.x][w]);
+            }
+            norms[threadIdx.x * gridDim.x + blockIdx.x] = m;
+        }
+    }
+}
+
+// --- host --------------------------------------------------------------------------------------------------
+
+// How many parts `walked` tiles are cut into for `owned` items of one part each: the fewest turns of the busiest CTA,
+// counted in tiles (an item costs about two more), at most kLongestSum entries a part.
+void cut(long long owned, int walked, int& parts, int& part_tiles)
+{
+    const long long least = std::max(1, (walked + kLongestSum / kTile - 1) / (kLongestSum / kTile));
+    double best = 0.0;
+    for (long long s = least; s <= std::max<long long>(least, std::min(walked, 64)); ++s) {
+        const long long span = (walked + s - 1) / s;
+        if (s > least && (walked + span - 1) / span != s) {
+            continue;
+        }
+        const double turns = static_cast<double>((owned * s + kSms - 1) / kSms) * (static_cast<double>(span) + 2.0) + (s > 1 ? 3.0 + 0.1 * s : 0.0);
+        if (s == least || turns < best) {
+            best = turns;
+            parts = static_cast<int>(s);
+            part_tiles = static_cast<int>(span);
+        }
+    }
+    parts = std::max(1, (walked + part_tiles - 1) / part_tiles);
+}
+
+struct Plan {
+    Operand q, k, v, dout;
+    int rows_per_tile = 0, row_tiles = 0, key_tiles = 0;
+    int row_parts = 1, row_span = 0;   // keys' kernel: parts of the rows
+    int key_parts = 1, key_span = 0;   // rows' kernel: parts of the keys
+    std::size_t constants = 0, norms = 0, dq = 0, dk = 0, dv = 0;
+    Arena arena;
+
+    explicit Plan(const Call& c)
+    {
+        const int heads = c.kv_heads * c.group;
+        const Strides dense{static_cast<long long>(c.queries) * heads * c.dim, static_cast<long long>(heads) * c.dim, c.dim};
+        q = operand(arena, c.q, c.qs, c.batch, c.queries, heads, c.dim, false);
+        k = operand(arena, c.k, c.ks, c.batch, c.keys, c.kv_heads, c.dim, true);
+        v = operand(arena, c.v, c.vs, c.batch, c.keys, c.kv_heads, c.dim, true);
+        dout = operand(arena, c.dout, dense, c.batch, c.queries, heads, c.dim, false);
+        rows_per_tile = kTile / c.group * c.group;
+        row_tiles = pieces(c.rows(), rows_per_tile);
+        key_tiles = pieces(c.keys, kTile);
+        cut(c.pairs() * key_tiles, row_tiles, row_parts, row_span);
+        cut(c.pairs() * row_tiles, key_tiles, key_parts, key_span);
+        constants = arena.take(static_cast<std::size_t>(c.pairs()) * row_tiles * kConstants * sizeof(float));
+        norms = arena.take(2 * kNormCtas * sizeof(float));
+        if (key_parts > 1) {
+            dq = arena.take(static_cast<std::size_t>(c.pairs()) * c.rows() * c.dim * key_parts * sizeof(float));
+        }
+        if (row_parts > 1) {
+            dk = arena.take(static_cast<std::size_t>(c.pairs()) * c.keys * c.dim * row_parts * sizeof(float));
+            dv = arena.take(static_cast<std::size_t>(c.pairs()) * c.keys * c.dim * row_parts * sizeof(float));
+        }
+    }
+};
+
+template <class T, int Boxes, bool Rows, bool Wipe>
+void launch(const Backward& g, cudaStream_t stream)
+{
+    using Cfg = Config<Boxes, Rows, Wipe>;
+    const auto kernel = backward_kernel<T, Boxes, Rows, Wipe>;
+    static std::atomic<int> cache[kMaxDevices];
+    const unsigned grid = persistent_grid(reinterpret_cast<const void*>(kernel), Cfg::kThreads, Cfg::kSmem, cache, g.items);
+    launch_pdl(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, g);
+}
+
+template <class T, int Boxes>
+void both(Backward g, const Plan& plan, const HeadMap (&rows)[2], const HeadMap (&keys)[2], char* work, cudaStream_t stream)
+{
+    const Call& c = g.c;
+    const bool cut = c.lengths != nullptr || c.mask != nullptr;
+    // dk and dv.
+    g.x0 = keys[0];
+    g.x1 = keys[1];
+    g.y0 = rows[0];
+    g.y1 = rows[1];
+    g.parts = plan.row_parts;
+    g.part_tiles = plan.row_span;
+    g.items = c.pairs() * plan.key_tiles * plan.row_parts;
+    g.partial0 = reinterpret_cast<float*>(work + plan.dk);
+    g.partial1 = reinterpret_cast<float*>(work + plan.dv);
+    launch<T, Boxes, false, false>(g, stream);
+    // dq.
+    g.x0 = rows[0];
+    g.x1 = rows[1];
+    g.y0 = keys[0];
+    g.y1 = keys[1];
+    g.parts = plan.key_parts;
+    g.part_tiles = plan.key_span;
+    g.items = c.pairs() * plan.row_tiles * plan.key_parts;
+    g.partial0 = reinterpret_cast<float*>(work + plan.dq);
+    if (cut) {
+        launch<T, Boxes, true, true>(g, stream);
+    } else {
+        launch<T, Boxes, true, false>(g, stream);
+    }
+}
+
+}  // namespace
+
+std::size_t tensor_backward_workspace(const Call& c) { return Plan(c).arena.size(); }
+
+void tensor_backward(const Call& c, char* work, cudaStream_t stream)
+{
+    const Plan plan(c);
+    const Operand* const operands[4] = {&plan.q, &plan.k, &plan.v, &plan.dout};
+    stage(operands, 4, c.batch, c.dim, work, stream);
+    const bool is_bf16 = c.dtype == SPECTRAL_BFLOAT16;
+    Backward g;
+    g.c = c;
+    g.tokens_per_tile = kTile / c.group;
+    g.rows_per_tile = plan.rows_per_tile;
+    g.row_tiles = plan.row_tiles;
+    g.key_tiles = plan.key_tiles;
+    g.factor = c.scale * kLog2e;
+    auto* constants = reinterpret_cast<float*>(work + plan.constants);
+    auto* norms = reinterpret_cast<float*>(work + plan.norms);
+    g.constants = constants;
+    g.norms = norms;
+    g.fault = device_fault_word();
+    int lanes = 1;
+    while (lanes * 8 < c.dim) {
+        lanes *= 2;
+    }
+    const long long entries = std::max(c.pairs() * plan.row_tiles * kTile, is_bf16 ? 0LL : c.pairs() * c.keys);
+    const auto grid = static_cast<unsigned>(std::min<long long>((entries * lanes + 255) / 256, kNormCtas));
+    g.norm_count = static_cast<int>(grid);
+    const bool vectors = c.dim % 8 == 0 && aligned_to(c.out, 16) && aligned_to(c.dout, 16);
+    const int heads = c.kv_heads * c.group;
+    const auto rows_map = [&](const Operand& o) {
+        return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.queries, heads, c.dim, c.group, g.tokens_per_tile);
+    };
+    const auto keys_map = [&](const Operand& o) { return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile); };
+    const HeadMap rows[2] = {rows_map(plan.q), rows_map(plan.dout)};
+    const HeadMap keys[2] = {keys_map(plan.k), keys_map(plan.v)};
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        if (vectors) {
+            launch_pdl(constants_kernel<T, true>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.rows_per_tile, plan.row_tiles, lanes);
+        } else {
+            launch_pdl(constants_kernel<T, false>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.rows_per_tile, plan.row_tiles, lanes);
+        }
+        if (c.dim <= 64) {
+            both<T, 1>(g, plan, rows, keys, work, stream);
+        } else {
+            both<T, 2>(g, plan, rows, keys, work, stream);
+        }
+    };
+    if (is_bf16) {
+        run(bf16{});
+    } else {
+        run(f16{});
+    }
+    if (plan.row_parts > 1) {
+        add_parts(c, reinterpret_cast<const float*>(work + plan.dk), plan.row_parts, true, c.dk, c.scale, stream);
+        add_parts(c, reinterpret_cast<const float*>(work + plan.dv), plan.row_parts, true, c.dv, 1.0f, stream);
+    }
+    if (plan.key_parts > 1) {
+        add_parts(c, reinterpret_cast<const float*>(work + plan.dq), plan.key_parts, false, c.dq, c.scale, stream);
+    }
+}
+
+}  // namespace spectral::attention

@@ -1190,7 +1190,7 @@ cross_attention_backward_cuda(const at::Tensor& dout, const at::Tensor& q, const
     at::Tensor dk = at::empty(k.sizes(), q.options());
     at::Tensor dv = at::empty(v.sizes(), q.options());
     size_t count = 0;
-    check_status(spectral_cross_attention_backward_workspace(cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.dtype, n.batch, n.queries, n.keys,
+    check_status(spectral_cross_attention_backward_workspace(cptr(dc), cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.dtype, n.batch, n.queries, n.keys,
                                                              n.heads, n.kv_heads, n.dim, &count));
     at::Tensor work = workspace(count, q);
     check_status(spectral_cross_attention_backward(cptr(dc), cptr(a.q), cptr(a.k), cptr(a.v), a.strides, cptr(oc), fptr(sc), a.lengths_ptr(),

@@ -457,9 +457,9 @@ SPECTRAL_API int spectral_cross_attention(const void* q, const void* k, const vo
                                           void* work, void* stream);
 /* Its gradients for dout, from the forward call's out and stats: dq, dk and dv, contiguous, of the type and shapes
  * of q, k and v (zeros for keys that do not count). dout is contiguous. Fixed summation order. */
-SPECTRAL_API int spectral_cross_attention_backward_workspace(const void* q, const void* k, const void* v, const long long* strides,
-                                                             int dtype, long long batch, long long queries, long long keys, int heads,
-                                                             int kv_heads, int dim, size_t* count);
+SPECTRAL_API int spectral_cross_attention_backward_workspace(const void* dout, const void* q, const void* k, const void* v,
+                                                             const long long* strides, int dtype, long long batch, long long queries,
+                                                             long long keys, int heads, int kv_heads, int dim, size_t* count);
 SPECTRAL_API int spectral_cross_attention_backward(const void* dout, const void* q, const void* k, const void* v,
                                                    const long long* strides, const void* out, const float* stats, const void* lengths,
                                                    int lengths64, const void* mask, void* dq, void* dk, void* dv, int dtype,
