@@ -54,7 +54,8 @@ struct Plan {
     int rotated = 0;
     int axes = 1;
     int per_axis = 0;  // pairs
-    int table_pairs = 0;
+    int table_pitch = 0;    // pairs of a token in the table, a multiple of 4
+    int table_columns = 1;  // the power of two from there on
     bool neighbours = false;
     float eps = 0.0f;
     double turns[kMaxDim / 2];  // angle per position, in turns, of an axis's pairs
@@ -104,64 +105,73 @@ __device__ __forceinline__ float sum_lanes(float v, int lanes)
     return v;
 }
 
-// V values of a head per lane, `lanes` (a power of two) lanes a head; V = 1: any dim and alignment, a warp a head and
-// up to four values a lane. Forward needs x, backward also dy.
-template <class T, int V, bool Back>
+// V values of a head per piece, `lanes` (a power of two) lanes a head with U pieces each, piece k of lane l the
+// (l + k lanes)th; V = 1: any dim and alignment. Forward needs x, backward also dy.
+template <class T, int V, int U, bool Back>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Plan plan, int lanes)
 {
-    constexpr int kUnits = V == 1 ? kMaxDim / 32 : 1;  // pieces of a head a lane holds
-    constexpr int kRows = V == 1 ? 1 : Back ? 2 : 4;   // heads in flight per lane
+    constexpr int kRows = U > 1 ? (Back ? 1 : 2) : Back ? 2 : 4;  // heads in flight per lane
     using Piece = Vec<T, V>;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float exchange[V == 1 ? kThreads / 32 : 1][V == 1 ? kMaxDim : 1];
+    __shared__ __align__(16) float exchange[U > 1 ? kThreads / 32 : 1][U > 1 ? kMaxDim : 4];
     const bool second_side = static_cast<int>(blockIdx.x) >= plan.side[0].ctas;
     const Side& s = plan.side[second_side ? 1 : 0];
     const int cta = blockIdx.x - (second_side ? plan.side[0].ctas : 0);
     const int dim = plan.dim;
     const int rotated = s.positions != nullptr ? plan.rotated : 0;
     const int n = plan.per_axis;
-    const int pairs = plan.table_pairs;
-    auto* table = reinterpret_cast<float2*>(smem);
-    auto* offsets = reinterpret_cast<long long*>(smem + (static_cast<size_t>(s.tile_tokens) * pairs * 8 + 15) / 16 * 16);
+    const int pitch = plan.table_pitch;
+    // Of each token of a tile: where it starts, where its positions are, the cosines of its pairs, the sines.
+    auto* offsets = reinterpret_cast<long long*>(smem);
+    auto* position_offsets = offsets + s.tile_tokens;
+    auto* cosines = reinterpret_cast<float*>(smem + static_cast<size_t>(s.tile_tokens) * 16);
+    auto* sines = cosines + s.tile_tokens * pitch;
 
     const int lane = threadIdx.x & 31;
     const int sub = lane & (lanes - 1);
     const int group = threadIdx.x / lanes;
     const int groups = kThreads / lanes;
-    // This lane's pieces: where in the head, which pairs of the table, where the partners are (halves) and which of
-    // the two it holds.
-    int d[kUnits], pair_at[kUnits], partner[kUnits];
-    bool live[kUnits], turned[kUnits], first[kUnits];
-    Floats<V> w[kUnits], wp[kUnits], dw[kUnits];
+    // This lane's pieces: where in the head, which pairs of the table, where the partners are (halves) and the sign of
+    // their sines.
+    int d[U], pair_at[U], partner[U];
+    bool live[U], turned[U];
+    float sign[U];
+    Floats<V> w[U], wp[U], dw[U];
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
+    for (int k = 0; k < U; ++k) {
         d[k] = (sub + k * lanes) * V;
         live[k] = d[k] < dim;
         turned[k] = live[k] && d[k] < rotated;
-        first[k] = true;
+        bool first = true;
         partner[k] = d[k];
         pair_at[k] = d[k] / 2;
         if (plan.neighbours) {
             if (V == 1) {
-                first[k] = d[k] % 2 == 0;
+                first = d[k] % 2 == 0;
                 partner[k] = d[k] ^ 1;
             }
         } else if (turned[k]) {
             const int axis = d[k] / (2 * n);
             const int off = d[k] - axis * 2 * n;
-            first[k] = off < n;
-            partner[k] = first[k] ? d[k] + n : d[k] - n;
-            pair_at[k] = axis * n + (first[k] ? off : off - n);
+            first = off < n;
+            partner[k] = first ? d[k] + n : d[k] - n;
+            pair_at[k] = axis * n + (first ? off : off - n);
         }
+        sign[k] = first != Back ? -1.0f : 1.0f;
         w[k].fill(1.0f);
         wp[k].fill(1.0f);
         dw[k].fill(0.0f);
     }
+    // This thread's column of the table: one pair, every `table_rows`-th token.
+    const int column = threadIdx.x % plan.table_columns;
+    const int table_rows = kThreads / plan.table_columns;
+    const int column_axis = column / n;
+    const double turns = column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0;
     allow_next_grid();
     wait_for_previous_grid();
     if (s.weight != nullptr) {
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
+        for (int k = 0; k < U; ++k) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 if (live[k]) {
@@ -171,40 +181,50 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
             }
         }
     }
-    const T* __restrict__ x = static_cast<const T*>(s.x);
-    const T* __restrict__ dy = static_cast<const T*>(s.dy);
-    T* __restrict__ out = static_cast<T*>(s.out);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {  // what a partner's value meets: weight and sign (backward: the sign)
+#pragma unroll
+        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+            wp[k].p[j] = Back ? pair(sign[k]) : wp[k].p[j] * pair(sign[k]);
+        }
+    }
     const int heads = s.heads;
     const int step_tokens = groups / heads;
     const int step_heads = groups - step_tokens * heads;
+    const float per_dim = 1.0f / static_cast<float>(dim);
 
     for (long long start = static_cast<long long>(cta) * s.tile_tokens; start < s.total;
          start += static_cast<long long>(s.ctas) * s.tile_tokens) {
         const int tokens = static_cast<int>(min(static_cast<long long>(s.tile_tokens), s.total - start));
         for (int t = threadIdx.x; t < tokens; t += kThreads) {
             const long long b = (start + t) / s.tokens;
-            offsets[t] = b * s.stride[0] + (start + t - b * s.tokens) * s.stride[1];
+            const long long at = start + t - b * s.tokens;
+            offsets[t] = b * s.stride[0] + at * s.stride[1];
+            position_offsets[t] = b * s.position_stride[0] + at * s.position_stride[1];
         }
         __syncthreads();
-        const long long rows = static_cast<long long>(tokens) * heads;
+        const T* __restrict__ x = static_cast<const T*>(s.x);
+        const T* __restrict__ dy = static_cast<const T*>(s.dy) + start * heads * dim;
+        T* __restrict__ out = static_cast<T*>(s.out) + start * heads * dim;
+        const int rows = tokens * heads;  // tile_tokens * heads * dim stays below 2^31
         int token = group / heads;
         int head = group - token * heads;
-        for (long long base = 0; base < rows; base += static_cast<long long>(kRows) * groups) {
-            Piece px[kRows][kUnits], pg[kRows][kUnits];
+        for (int base = 0; base < rows; base += kRows * groups) {
+            Piece px[kRows][U], pg[kRows][U];
             int token_of[kRows];
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
-                const long long row = base + group + i * groups;
+                const int row = base + group + i * groups;
                 token_of[i] = min(token, tokens - 1);
-                const long long from = offsets[token_of[i]] + head * s.stride[2];
+                const T* from = x + offsets[token_of[i]] + head * s.stride[2];
 #pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
+                for (int k = 0; k < U; ++k) {
                     px[i][k] = Piece{};
                     pg[i][k] = Piece{};
                     if (row < rows && live[k]) {
-                        px[i][k] = *reinterpret_cast<const Piece*>(x + from + d[k]);
+                        px[i][k] = *reinterpret_cast<const Piece*>(from + d[k]);
                         if constexpr (Back) {
-                            pg[i][k] = *reinterpret_cast<const Piece*>(dy + (start * heads + row) * dim + d[k]);
+                            pg[i][k] = *reinterpret_cast<const Piece*>(dy + row * dim + d[k]);
                         }
                     }
                 }
@@ -216,104 +236,116 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
                 }
             }
             if (base == 0) {
-                if (rotated > 0) {
-                    for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
-                        const int t = i / pairs;
-                        const int p = i - t * pairs;
+                if (rotated > 0 && column < pitch) {
+                    for (int t = threadIdx.x / plan.table_columns; t < tokens; t += table_rows) {
                         float2 cs = make_float2(1.0f, 0.0f);
-                        if (p < rotated / 2) {
-                            const int axis = p / n;
-                            const long long b = (start + t) / s.tokens;
-                            const double pos = position_at(s, b * s.position_stride[0] + (start + t - b * s.tokens) * s.position_stride[1]
-                                                                  + axis * s.position_stride[2]);
-                            cs = unit<T>(pos * plan.turns[p - axis * n]);
+                        if (column < rotated / 2) {
+                            cs = unit<T>(position_at(s, position_offsets[t] + column_axis * s.position_stride[2]) * turns);
                         }
-                        table[i] = cs;
+                        cosines[t * pitch + column] = cs.x;
+                        sines[t * pitch + column] = cs.y;
                     }
                 }
                 __syncthreads();
             }
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
-                const long long row = base + group + i * groups;
+                const int row = base + group + i * groups;
                 if (base + i * groups >= rows) {  // none in the whole CTA
                     break;
                 }
+                Floats<V> xs[U], f[U];
                 float2 square = pair(0.0f);
 #pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
-                    const Floats<V> f = widen(px[i][k]);
+                for (int k = 0; k < U; ++k) {
+                    xs[k] = widen(px[i][k]);
 #pragma unroll
                     for (int j = 0; j < Floats<V>::kPairs; ++j) {
-                        square = fma2(f.p[j], f.p[j], square);
+                        square = fma2(xs[k].p[j], xs[k].p[j], square);
                     }
                 }
-                const float mean = sum_lanes(square.x + square.y, lanes) / static_cast<float>(dim);
-                const float r = rsqrtf(mean + plan.eps);
-                // What is turned: x r w forward, the upstream gradient (the other way) backward.
-                Floats<V> f[kUnits], other[kUnits];
+                const float r = rsqrtf(fmaf(sum_lanes(square.x + square.y, lanes), per_dim, plan.eps));
+                // What is turned: x w forward (r comes at the end), the upstream gradient (the other way) backward.
 #pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
-                    f[k] = widen(Back ? pg[i][k] : px[i][k]);
-                    if constexpr (!Back) {
-#pragma unroll
-                        for (int j = 0; j < Floats<V>::kPairs; ++j) {
-                            f[k].p[j] = f[k].p[j] * pair(r) * w[k].p[j];
-                        }
-                    }
+                for (int k = 0; k < U; ++k) {
+                    f[k] = Back ? widen(pg[i][k]) : xs[k];
                 }
                 if (rotated > 0) {
-                    const float2* cs = table + token_of[i] * pairs;
-                    if constexpr (V == 1) {
+                    const float* c = cosines + token_of[i] * pitch;
+                    const float* e = sines + token_of[i] * pitch;
+                    if constexpr (U > 1) {
                         float* buf = exchange[threadIdx.x >> 5];
                         __syncwarp();
 #pragma unroll
-                        for (int k = 0; k < kUnits; ++k) {
+                        for (int k = 0; k < U; ++k) {
                             if (live[k]) {
-                                buf[d[k]] = f[k].p[0].x;
+#pragma unroll
+                                for (int j = 0; j < V; ++j) {
+                                    buf[d[k] + j] = f[k].at(j);
+                                }
                             }
                         }
                         __syncwarp();
+                    }
 #pragma unroll
-                        for (int k = 0; k < kUnits; ++k) {
-                            if (turned[k]) {
-                                const float2 c = cs[pair_at[k]];
-                                f[k].p[0].x = f[k].p[0].x * c.x + buf[partner[k]] * (first[k] != Back ? -c.y : c.y);
-                            }
-                        }
-                    } else if (plan.neighbours) {
-                        if (turned[0]) {
+                    for (int k = 0; k < U; ++k) {
+                        if (V > 1 && plan.neighbours) {
+                            if constexpr (!Back) {
 #pragma unroll
-                            for (int j = 0; j < V / 2; ++j) {
-                                const float2 c = cs[pair_at[0] + j];
-                                const float sine = Back ? -c.y : c.y;
-                                const float2 v = f[0].p[j];
-                                f[0].p[j] = make_float2(v.x * c.x - v.y * sine, v.y * c.x + v.x * sine);
-                            }
-                        }
-                    } else {
-                        const int src = lane - sub + partner[0] / V;
-                        other[0] = widen(shuffle_words(Back ? pg[i][0] : px[i][0], src));
-                        if (turned[0]) {
-                            const float sign = first[0] != Back ? -1.0f : 1.0f;
-#pragma unroll
-                            for (int j = 0; j < V; ++j) {
-                                const float2 c = cs[pair_at[0] + j];
-                                float o = other[0].at(j);
-                                if constexpr (!Back) {
-                                    o *= r * wp[0].at(j);
+                                for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                                    f[k].p[j] = f[k].p[j] * w[k].p[j];
                                 }
-                                f[0].set(j, f[0].at(j) * c.x + o * (sign * c.y));
                             }
+                            if (turned[k]) {
+                                const auto cs = *reinterpret_cast<const Vec<float, V / 2 + (V == 1)>*>(c + pair_at[k]);
+                                const auto sn = *reinterpret_cast<const Vec<float, V / 2 + (V == 1)>*>(e + pair_at[k]);
+#pragma unroll
+                                for (int j = 0; j < V / 2; ++j) {
+                                    const float sine = Back ? -sn.v[j] : sn.v[j];
+                                    const float2 v = f[k].p[j];
+                                    f[k].p[j] = fma2(v, pair(cs.v[j]), make_float2(-v.y * sine, v.x * sine));
+                                }
+                            }
+                        } else {
+                            Floats<V> other;
+                            if constexpr (U > 1) {
+#pragma unroll
+                                for (int j = 0; j < V; ++j) {
+                                    other.set(j, exchange[threadIdx.x >> 5][live[k] ? partner[k] + j : 0]);
+                                }
+                            } else {
+                                other = widen(shuffle_words(Back ? pg[i][k] : px[i][k], lane - sub + partner[k] / V));
+                            }
+                            if (turned[k]) {
+                                const auto cs = *reinterpret_cast<const Vec<float, V>*>(c + pair_at[k]);
+                                const auto sn = *reinterpret_cast<const Vec<float, V>*>(e + pair_at[k]);
+                                const Floats<V> c2 = widen(cs), s2 = widen(sn);
+#pragma unroll
+                                for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                                    const float2 a = Back ? c2.p[j] : c2.p[j] * w[k].p[j];
+                                    f[k].p[j] = fma2(f[k].p[j], a, other.p[j] * (s2.p[j] * wp[k].p[j]));
+                                }
+                            } else if constexpr (!Back) {
+#pragma unroll
+                                for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                                    f[k].p[j] = f[k].p[j] * w[k].p[j];
+                                }
+                            }
+                        }
+                    }
+                } else if constexpr (!Back) {
+#pragma unroll
+                    for (int k = 0; k < U; ++k) {
+#pragma unroll
+                        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                            f[k].p[j] = f[k].p[j] * w[k].p[j];
                         }
                     }
                 }
                 if constexpr (Back) {
                     float2 dot = pair(0.0f);
-                    Floats<V> xs[kUnits];
 #pragma unroll
-                    for (int k = 0; k < kUnits; ++k) {
-                        xs[k] = widen(px[i][k]);
+                    for (int k = 0; k < U; ++k) {
 #pragma unroll
                         for (int j = 0; j < Floats<V>::kPairs; ++j) {
                             const float2 gx = f[k].p[j] * xs[k].p[j];
@@ -321,20 +353,24 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
                             dot = fma2(gx, w[k].p[j], dot);
                         }
                     }
-                    const float c = -sum_lanes(dot.x + dot.y, lanes) / static_cast<float>(dim) * r * r;
+                    const float c = -sum_lanes(dot.x + dot.y, lanes) * per_dim * r * r;
 #pragma unroll
-                    for (int k = 0; k < kUnits; ++k) {
+                    for (int k = 0; k < U; ++k) {
 #pragma unroll
                         for (int j = 0; j < Floats<V>::kPairs; ++j) {
-                            f[k].p[j] = fma2(xs[k].p[j], pair(c), f[k].p[j] * w[k].p[j]) * pair(r);
+                            f[k].p[j] = fma2(xs[k].p[j], pair(c), f[k].p[j] * w[k].p[j]);
                         }
                     }
                 }
                 if (row < rows) {
 #pragma unroll
-                    for (int k = 0; k < kUnits; ++k) {
+                    for (int k = 0; k < U; ++k) {
                         if (live[k]) {
-                            *reinterpret_cast<Piece*>(out + (start * heads + row) * dim + d[k]) = narrow<T>(f[k]);
+#pragma unroll
+                            for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                                f[k].p[j] = f[k].p[j] * pair(r);
+                            }
+                            *reinterpret_cast<Piece*>(out + row * dim + d[k]) = narrow<T>(f[k]);
                         }
                     }
                 }
@@ -349,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         // The groups' sums of each value, in order: through shared memory, a value a thread.
         auto* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
+        for (int k = 0; k < U; ++k) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 if (live[k]) {
@@ -420,7 +456,7 @@ int vector_width(const spectral_heads* const (&sides)[2], int dtype, long long b
     const int size = static_cast<int>(dtype_size(dtype));
     const int n = rotated / (2 * axes);
     for (int v = 16 / size; v >= 2; v /= 2) {
-        bool ok = dim % v == 0 && dim / v <= 32 && (rotated == 0 || pairs == SPECTRAL_PAIRS_NEIGHBOURS || n % v == 0);
+        bool ok = dim % v == 0 && dim / v <= (v == 2 ? 64 : 32) && (rotated == 0 || pairs == SPECTRAL_PAIRS_NEIGHBOURS || n % v == 0);
         for (const spectral_heads* s : sides) {
             if (s == nullptr) {
                 continue;
@@ -530,14 +566,18 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     plan.rotated = any ? rotated : 0;
     plan.per_axis = std::max(1, plan.rotated / (2 * axes));
     // A piece that reaches past `rotated` (neighbours only) finds angles of zero there.
-    plan.table_pairs = plan.rotated == 0 ? 0 : plan.neighbours ? (dim + 1) / 2 : plan.rotated / 2;
+    plan.table_pitch = plan.rotated == 0 ? 0 : ((plan.neighbours ? (dim + 1) / 2 : plan.rotated / 2) + 3) / 4 * 4;
+    while (plan.table_columns < plan.table_pitch) {
+        plan.table_columns *= 2;
+    }
     for (int i = 0; i < plan.per_axis && plan.rotated > 0; ++i) {
         plan.turns[i] = std::pow(static_cast<double>(theta), -static_cast<double>(i) / plan.per_axis) / 6.283185307179586476925;
     }
     const int v = vector_width(sides, dtype, batch, dim, plan.rotated, axes, pairs);
+    const int units = v == 1 ? 4 : v == 2 && dim > 64 ? 2 : 1;
     const int lanes = v == 1 ? 32 : lanes_for(dim, v);
     const int groups = kThreads / lanes;
-    const int in_flight = v == 1 ? 4 : back ? 2 : 4;
+    const int in_flight = back ? 2 : 4;
     const int most = most_ctas();
     long long tiles[2] = {0, 0};
     int table_tokens = 1;
@@ -558,7 +598,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
         t.heads = s->heads;
         t.tokens = s->tokens;
         t.total = batch * s->tokens;
-        const long long cap = plan.table_pairs > 0 ? std::max(1, kTableBytes / (8 * plan.table_pairs)) : 256;
+        const long long cap = plan.table_pitch > 0 ? std::max(1, kTableBytes / (8 * plan.table_pitch)) : 256;
         t.tile_tokens = static_cast<int>(std::max(1LL, std::min<long long>(cap, static_cast<long long>(groups) * in_flight / s->heads)));
         t.tile_tokens = static_cast<int>(std::min<long long>(t.tile_tokens, t.total));
         tiles[i] = (t.total + t.tile_tokens - 1) / t.tile_tokens;
@@ -586,25 +626,35 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     }
     const int ctas = plan.side[0].ctas + plan.side[1].ctas;
     if (ctas > 0) {
-        std::size_t smem = (static_cast<std::size_t>(table_tokens) * plan.table_pairs * 8 + 15) / 16 * 16 + table_tokens * sizeof(long long);
+        std::size_t smem = static_cast<std::size_t>(table_tokens) * (plan.table_pitch * 8 + 16);
         if (back) {
             smem = std::max(smem, static_cast<std::size_t>(groups) * dim * sizeof(float));
         }
         with_dtype(dtype, [&](auto t) {
             using T = decltype(t);
-            const auto launch = [&](auto width) {
+            const auto launch = [&](auto width, auto pieces) {
                 constexpr int V = decltype(width)::value;
-                launch_pdl(back ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>, dim3(ctas), dim3(kThreads), smem, stream, plan, lanes);
+                constexpr int U = decltype(pieces)::value;
+                launch_pdl(back ? rotary_kernel<T, V, U, true> : rotary_kernel<T, V, U, false>, dim3(ctas), dim3(kThreads), smem, stream, plan, lanes);
             };
+            constexpr std::integral_constant<int, 1> one;
+            constexpr std::integral_constant<int, 2> two;
+            constexpr std::integral_constant<int, 4> four;
             switch (v) {
                 case 8:
                     if constexpr (sizeof(T) == 2) {
-                        launch(std::integral_constant<int, 8>{});
+                        launch(std::integral_constant<int, 8>{}, one);
                     }
                     break;
-                case 4: launch(std::integral_constant<int, 4>{}); break;
-                case 2: launch(std::integral_constant<int, 2>{}); break;
-                default: launch(std::integral_constant<int, 1>{}); break;
+                case 4: launch(four, one); break;
+                case 2:
+                    if (units == 2) {
+                        launch(two, two);
+                    } else {
+                        launch(two, one);
+                    }
+                    break;
+                default: launch(one, four); break;
             }
         });
     }
