@@ -29,7 +29,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = SPECTRAL_HEAD_DIM_MAX;
-constexpr int kTableBytes = 16 * 1024;
+constexpr int kTableBytes = 40 * 1024;  // places and tables, at most
+
+// Heads a lane works on at a time, while it waits for as many more.
+__host__ __device__ constexpr int rows_in_flight(int units, bool back) { return units > 1 ? (back ? 1 : 2) : back ? 2 : 4; }
 
 struct Side {
     const void* x = nullptr;
@@ -61,28 +64,41 @@ struct Plan {
     double turns[kMaxDim / 2];  // angle per position, in turns, of an axis's pairs
 };
 
-__device__ __forceinline__ double position_at(const Side& s, long long at)
-{
-    switch (s.position_type) {
-        case SPECTRAL_POSITIONS_FLOAT32: return static_cast<double>(static_cast<const float*>(s.positions)[at]);
-        case SPECTRAL_POSITIONS_INT32: return static_cast<double>(static_cast<const int*>(s.positions)[at]);
-        default: return static_cast<double>(static_cast<const long long*>(s.positions)[at]);
-    }
-}
-
-// (cos, sin) of an angle in turns. For results rounded to 16 bits the hardware's functions on [-pi, pi], off by
-// 2^-20 at most, do.
+// (cos, sin) of a fraction of a turn between -1/2 and 1/2. For results rounded to 16 bits the hardware's functions on
+// [-pi, pi], off by 2^-20 at most, do.
 template <class T>
-__device__ __forceinline__ float2 unit(double turns)
+__device__ __forceinline__ float2 unit(float turn)
 {
-    const float f = static_cast<float>(turns - rint(turns));
     float2 cs;
     if constexpr (sizeof(T) == 4) {
-        sincospif(2.0f * f, &cs.y, &cs.x);
+        sincospif(2.0f * turn, &cs.y, &cs.x);
     } else {
-        __sincosf(6.283185307179586f * f, &cs.y, &cs.x);
+        __sincosf(6.283185307179586f * turn, &cs.y, &cs.x);
     }
     return cs;
+}
+
+// A pair's frequency in turns per position: in 64 bits, and as the sum of two floats.
+struct Frequency {
+    double turns;
+    float high;
+    float low;
+};
+
+// What is left of position * frequency without its whole turns. A float's product with the two floats is exact but for
+// 2^-48 of it; whole numbers go through 64 bits.
+template <class P>
+__device__ __forceinline__ float turn_of(P position, const Frequency& f)
+{
+    if constexpr (std::is_same_v<P, float>) {
+        const float a = position * f.high;
+        const float rest = fmaf(position, f.low, fmaf(position, f.high, -a));
+        const float turn = (a - rintf(a)) + rest;
+        return turn - rintf(turn);
+    } else {
+        const double a = static_cast<double>(position) * f.turns;
+        return static_cast<float>(a - rint(a));
+    }
 }
 
 template <class W>
@@ -108,9 +124,9 @@ __device__ __forceinline__ float sum_lanes(float v, int lanes)
 // V values of a head per piece, `lanes` (a power of two) lanes a head with U pieces each, piece k of lane l the
 // (l + k lanes)th; V = 1: any dim and alignment. Forward needs x, backward also dy.
 template <class T, int V, int U, bool Back>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Plan plan, int lanes)
+__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_constant__ Plan plan, int lanes)
 {
-    constexpr int kRows = U > 1 ? (Back ? 1 : 2) : Back ? 2 : 4;  // heads in flight per lane
+    constexpr int kRows = rows_in_flight(U, Back);
     using Piece = Vec<T, V>;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) float exchange[U > 1 ? kThreads / 32 : 1][U > 1 ? kMaxDim : 4];
@@ -121,11 +137,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const int rotated = s.positions != nullptr ? plan.rotated : 0;
     const int n = plan.per_axis;
     const int pitch = plan.table_pitch;
+    const int span = s.tile_tokens;
     // Of each token of a tile: where it starts, where its positions are, the cosines of its pairs, the sines.
-    auto* offsets = reinterpret_cast<long long*>(smem);
-    auto* position_offsets = offsets + s.tile_tokens;
-    auto* cosines = reinterpret_cast<float*>(smem + static_cast<size_t>(s.tile_tokens) * 16);
-    auto* sines = cosines + s.tile_tokens * pitch;
+    auto* const places = reinterpret_cast<long long*>(smem);
+    auto* const position_places = places + span;
+    auto* const cosines = reinterpret_cast<float*>(smem + static_cast<size_t>(span) * 16);
 
     const int lane = threadIdx.x & 31;
     const int sub = lane & (lanes - 1);
@@ -166,7 +182,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const int column = threadIdx.x % plan.table_columns;
     const int table_rows = kThreads / plan.table_columns;
     const int column_axis = column / n;
-    const double turns = column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0;
+    Frequency frequency{column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0, 0.0f, 0.0f};
+    frequency.high = static_cast<float>(frequency.turns);
+    frequency.low = static_cast<float>(frequency.turns - frequency.high);
     allow_next_grid();
     wait_for_previous_grid();
     if (s.weight != nullptr) {
@@ -192,87 +210,112 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const int step_tokens = groups / heads;
     const int step_heads = groups - step_tokens * heads;
     const float per_dim = 1.0f / static_cast<float>(dim);
+    float* const sines = cosines + span * pitch;
 
-    for (long long start = static_cast<long long>(cta) * s.tile_tokens; start < s.total;
-         start += static_cast<long long>(s.ctas) * s.tile_tokens) {
-        const int tokens = static_cast<int>(min(static_cast<long long>(s.tile_tokens), s.total - start));
+    for (long long start = static_cast<long long>(cta) * span; start < s.total; start += static_cast<long long>(s.ctas) * span) {
+        const int tokens = static_cast<int>(min(static_cast<long long>(span), s.total - start));
         for (int t = threadIdx.x; t < tokens; t += kThreads) {
-            const long long b = (start + t) / s.tokens;
-            const long long at = start + t - b * s.tokens;
-            offsets[t] = b * s.stride[0] + at * s.stride[1];
-            position_offsets[t] = b * s.position_stride[0] + at * s.position_stride[1];
+            const long long token = start + t;
+            const long long b = s.total < (1LL << 31) ? static_cast<unsigned>(token) / static_cast<unsigned>(s.tokens) : token / s.tokens;
+            const long long in = token - b * s.tokens;
+            places[t] = b * s.stride[0] + in * s.stride[1];
+            position_places[t] = b * s.position_stride[0] + in * s.position_stride[1];
         }
         __syncthreads();
         const T* __restrict__ x = static_cast<const T*>(s.x);
         const T* __restrict__ dy = static_cast<const T*>(s.dy) + start * heads * dim;
         T* __restrict__ out = static_cast<T*>(s.out) + start * heads * dim;
-        const int rows = tokens * heads;  // tile_tokens * heads * dim stays below 2^31
-        int token = group / heads;
-        int head = group - token * heads;
+        const int rows = tokens * heads;  // the tile's values stay below 2^31
+        int next_token = group / heads;
+        int next_head = group - next_token * heads;
         for (int base = 0; base < rows; base += kRows * groups) {
             Piece px[kRows][U], pg[kRows][U];
             int token_of[kRows];
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const int row = base + group + i * groups;
-                token_of[i] = min(token, tokens - 1);
-                const T* from = x + offsets[token_of[i]] + head * s.stride[2];
+            for (int r = 0; r < kRows; ++r) {
+                const int row = base + group + r * groups;
+                token_of[r] = min(next_token, tokens - 1);
+                const T* from = x + places[token_of[r]] + next_head * s.stride[2];
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    px[i][k] = Piece{};
-                    pg[i][k] = Piece{};
+                    px[r][k] = Piece{};
+                    pg[r][k] = Piece{};
                     if (row < rows && live[k]) {
-                        px[i][k] = *reinterpret_cast<const Piece*>(from + d[k]);
+                        px[r][k] = *reinterpret_cast<const Piece*>(from + d[k]);
                         if constexpr (Back) {
-                            pg[i][k] = *reinterpret_cast<const Piece*>(dy + row * dim + d[k]);
+                            pg[r][k] = *reinterpret_cast<const Piece*>(dy + row * dim + d[k]);
                         }
                     }
                 }
-                token += step_tokens;
-                head += step_heads;
-                if (head >= heads) {
-                    head -= heads;
-                    ++token;
+                next_token += step_tokens;
+                next_head += step_heads;
+                if (next_head >= heads) {
+                    next_head -= heads;
+                    ++next_token;
                 }
             }
-            if (base == 0) {
+            if (base == 0) {  // the first pieces are on their way
                 if (rotated > 0 && column < pitch) {
-                    for (int t = threadIdx.x / plan.table_columns; t < tokens; t += table_rows) {
-                        float2 cs = make_float2(1.0f, 0.0f);
-                        if (column < rotated / 2) {
-                            cs = unit<T>(position_at(s, position_offsets[t] + column_axis * s.position_stride[2]) * turns);
+            const bool turning = column < rotated / 2;
+            const long long mine = column_axis * s.position_stride[2];
+            // Several at a time: their positions are asked for together. (One after the other took half of the kernel's time.)
+            const auto fill = [&](auto type) {
+                using P = decltype(type);
+                constexpr int kBatch = sizeof(P) == 8 ? 4 : 8;
+                const P* __restrict__ positions = static_cast<const P*>(s.positions) + mine;
+                for (int t0 = threadIdx.x / plan.table_columns; t0 < tokens; t0 += kBatch * table_rows) {
+                    P position[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int t = t0 + j * table_rows;
+                        position[j] = turning && t < tokens ? __ldg(positions + position_places[t]) : P(0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int t = t0 + j * table_rows;
+                        if (t < tokens) {
+                            const float2 cs = unit<T>(turn_of(position[j], frequency));
+                            cosines[t * pitch + column] = cs.x;
+                            sines[t * pitch + column] = cs.y;
                         }
-                        cosines[t * pitch + column] = cs.x;
-                        sines[t * pitch + column] = cs.y;
                     }
                 }
+            };
+            if (s.position_type == SPECTRAL_POSITIONS_FLOAT32) {
+                fill(float{});
+            } else if (s.position_type == SPECTRAL_POSITIONS_INT32) {
+                fill(int{});
+            } else {
+                fill(0LL);
+            }
+        }
                 __syncthreads();
             }
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const int row = base + group + i * groups;
-                if (base + i * groups >= rows) {  // none in the whole CTA
+            for (int r = 0; r < kRows; ++r) {
+                const int row = base + group + r * groups;
+                if (base + r * groups >= rows) {  // none in the whole CTA
                     break;
                 }
                 Floats<V> xs[U], f[U];
                 float2 square = pair(0.0f);
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    xs[k] = widen(px[i][k]);
+                    xs[k] = widen(px[r][k]);
 #pragma unroll
                     for (int j = 0; j < Floats<V>::kPairs; ++j) {
                         square = fma2(xs[k].p[j], xs[k].p[j], square);
                     }
                 }
-                const float r = rsqrtf(fmaf(sum_lanes(square.x + square.y, lanes), per_dim, plan.eps));
-                // What is turned: x w forward (r comes at the end), the upstream gradient (the other way) backward.
+                const float inv = rsqrtf(fmaf(sum_lanes(square.x + square.y, lanes), per_dim, plan.eps));
+                // What is turned: x w forward (inv comes at the end), the upstream gradient (the other way) backward.
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    f[k] = Back ? widen(pg[i][k]) : xs[k];
+                    f[k] = Back ? widen(pg[r][k]) : xs[k];
                 }
                 if (rotated > 0) {
-                    const float* c = cosines + token_of[i] * pitch;
-                    const float* e = sines + token_of[i] * pitch;
+                    const float* c = cosines + token_of[r] * pitch;
+                    const float* e = sines + token_of[r] * pitch;
                     if constexpr (U > 1) {
                         float* buf = exchange[threadIdx.x >> 5];
                         __syncwarp();
@@ -314,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
                                     other.set(j, exchange[threadIdx.x >> 5][live[k] ? partner[k] + j : 0]);
                                 }
                             } else {
-                                other = widen(shuffle_words(Back ? pg[i][k] : px[i][k], lane - sub + partner[k] / V));
+                                other = widen(shuffle_words(Back ? pg[r][k] : px[r][k], lane - sub + partner[k] / V));
                             }
                             if (turned[k]) {
                                 const auto cs = *reinterpret_cast<const Vec<float, V>*>(c + pair_at[k]);
@@ -349,11 +392,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 #pragma unroll
                         for (int j = 0; j < Floats<V>::kPairs; ++j) {
                             const float2 gx = f[k].p[j] * xs[k].p[j];
-                            dw[k].p[j] = fma2(gx, pair(r), dw[k].p[j]);
+                            dw[k].p[j] = fma2(gx, pair(inv), dw[k].p[j]);
                             dot = fma2(gx, w[k].p[j], dot);
                         }
                     }
-                    const float c = -sum_lanes(dot.x + dot.y, lanes) * per_dim * r * r;
+                    const float c = -sum_lanes(dot.x + dot.y, lanes) * per_dim * inv * inv;
 #pragma unroll
                     for (int k = 0; k < U; ++k) {
 #pragma unroll
@@ -368,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
                         if (live[k]) {
 #pragma unroll
                             for (int j = 0; j < Floats<V>::kPairs; ++j) {
-                                f[k].p[j] = f[k].p[j] * pair(r);
+                                f[k].p[j] = f[k].p[j] * pair(inv);
                             }
                             *reinterpret_cast<Piece*>(out + row * dim + d[k]) = narrow<T>(f[k]);
                         }
@@ -481,8 +524,46 @@ int lanes_for(int dim, int v)
     return lanes;
 }
 
-// CTAs that are resident at once with room for registers and tables, the most a call has.
-int most_ctas() { return device_sm_count(current_device()) * 4; }
+constexpr int kMostResident = 4;  // CTAs of an SM, by the tables
+int most_ctas() { return device_sm_count(current_device()) * kMostResident; }
+
+// Calls f(kernel, cache of its residency) for the variant of a call.
+template <class F>
+void with_kernel(int dtype, int v, int units, bool back, F&& f)
+{
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const auto pick = [&](auto width, auto pieces) {
+            constexpr int V = decltype(width)::value;
+            constexpr int U = decltype(pieces)::value;
+            static std::atomic<int> cache[2][kMaxDevices];
+            if (back) {
+                f(rotary_kernel<T, V, U, true>, cache[1]);
+            } else {
+                f(rotary_kernel<T, V, U, false>, cache[0]);
+            }
+        };
+        constexpr std::integral_constant<int, 1> one;
+        constexpr std::integral_constant<int, 2> two;
+        constexpr std::integral_constant<int, 4> four;
+        switch (v) {
+            case 8:
+                if constexpr (sizeof(T) == 2) {
+                    pick(std::integral_constant<int, 8>{}, one);
+                }
+                break;
+            case 4: pick(four, one); break;
+            case 2:
+                if (units == 2) {
+                    pick(two, two);
+                } else {
+                    pick(two, one);
+                }
+                break;
+            default: pick(one, four); break;
+        }
+    });
+}
 
 int check(const char* op, const spectral_heads* const (&sides)[2], bool back, int dtype, long long batch, int dim, int rotated,
           int axes, int pairs, float eps, float theta)
@@ -577,8 +658,12 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     const int units = v == 1 ? 4 : v == 2 && dim > 64 ? 2 : 1;
     const int lanes = v == 1 ? 32 : lanes_for(dim, v);
     const int groups = kThreads / lanes;
-    const int in_flight = back ? 2 : 4;
-    const int most = most_ctas();
+    const int in_flight = rows_in_flight(units, back);
+    int most = 0;
+    with_kernel(dtype, v, units, back, [&](auto kernel, std::atomic<int>* cache) {
+        const int device = current_device();
+        most = device_sm_count(device) * std::min(kMostResident, resident_ctas(reinterpret_cast<const void*>(kernel), kThreads, kTableBytes, cache, device));
+    });
     long long tiles[2] = {0, 0};
     int table_tokens = 1;
     for (int i = 0; i < 2; ++i) {
@@ -598,9 +683,11 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
         t.heads = s->heads;
         t.tokens = s->tokens;
         t.total = batch * s->tokens;
-        const long long cap = plan.table_pitch > 0 ? std::max(1, kTableBytes / (8 * plan.table_pitch)) : 256;
-        t.tile_tokens = static_cast<int>(std::max(1LL, std::min<long long>(cap, static_cast<long long>(groups) * in_flight / s->heads)));
-        t.tile_tokens = static_cast<int>(std::min<long long>(t.tile_tokens, t.total));
+        // As many tokens as the table holds, fewer if that leaves CTAs without any, but enough to keep all lanes busy.
+        const long long cap = kTableBytes / (plan.table_pitch * 8 + 16);
+        const long long busy = std::max(1, groups * in_flight / s->heads);
+        const long long share = (t.total + most - 1) / most;
+        t.tile_tokens = static_cast<int>(std::min(cap, std::min(t.total, std::max(busy, share))));
         tiles[i] = (t.total + t.tile_tokens - 1) / t.tile_tokens;
         table_tokens = std::max(table_tokens, t.tile_tokens);
     }
@@ -630,32 +717,8 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
         if (back) {
             smem = std::max(smem, static_cast<std::size_t>(groups) * dim * sizeof(float));
         }
-        with_dtype(dtype, [&](auto t) {
-            using T = decltype(t);
-            const auto launch = [&](auto width, auto pieces) {
-                constexpr int V = decltype(width)::value;
-                constexpr int U = decltype(pieces)::value;
-                launch_pdl(back ? rotary_kernel<T, V, U, true> : rotary_kernel<T, V, U, false>, dim3(ctas), dim3(kThreads), smem, stream, plan, lanes);
-            };
-            constexpr std::integral_constant<int, 1> one;
-            constexpr std::integral_constant<int, 2> two;
-            constexpr std::integral_constant<int, 4> four;
-            switch (v) {
-                case 8:
-                    if constexpr (sizeof(T) == 2) {
-                        launch(std::integral_constant<int, 8>{}, one);
-                    }
-                    break;
-                case 4: launch(four, one); break;
-                case 2:
-                    if (units == 2) {
-                        launch(two, two);
-                    } else {
-                        launch(two, one);
-                    }
-                    break;
-                default: launch(one, four); break;
-            }
+        with_kernel(dtype, v, units, back, [&](auto kernel, std::atomic<int>*) {
+            launch_pdl(kernel, dim3(ctas), dim3(kThreads), smem, stream, plan, lanes);
         });
     }
     if (sums.out[0] != nullptr || sums.out[1] != nullptr) {
