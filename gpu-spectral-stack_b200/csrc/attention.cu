@@ -580,12 +580,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Call c, const floa
         const long long r = i - at * c.rows();
         const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
         const float f = total == 0.0f ? 0.0f : 1.0f / total;
-        T* out = static_cast<T*>(c.out) + c.row_at(b, head, r);
+        const long long to = c.row_at(b, head, r);
+        T* out = static_cast<T*>(c.out) + to;
 #pragma unroll
         for (int k = 0; k < SPECTRAL_HEAD_DIM_MAX / 32; ++k) {
             const int d = lane + 32 * k;
             if (d < c.dim) {
                 out[d] = from_float<T>(acc[k] * f);
+                if constexpr (sizeof(T) == 2) {
+                    if (c.rest != nullptr) {
+                        c.rest[to + d] = Rest<T>::code(acc[k] * f);
+                    }
+                }
             }
         }
         if (c.stats != nullptr && lane == 0) {
@@ -831,7 +837,7 @@ extern "C" int spectral_cross_attention_workspace(const void* q, const void* k, 
 }
 
 extern "C" int spectral_cross_attention(const void* q, const void* k, const void* v, const long long* strides, const void* lengths,
-                                        int lengths64, const void* mask, void* out, float* stats, int dtype, long long batch,
+                                        int lengths64, const void* mask, void* out, void* rest, float* stats, int dtype, long long batch,
                                         long long queries, long long keys, int heads, int kv_heads, int dim, float scale, void* work,
                                         void* stream)
 {
@@ -870,6 +876,7 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
     c.lengths64 = lengths64;
     c.mask = static_cast<const unsigned char*>(mask);
     c.out = out;
+    c.rest = static_cast<signed char*>(rest);
     c.stats = reinterpret_cast<float2*>(stats);
     c.scale = scale;
     try {
@@ -913,7 +920,7 @@ extern "C" int spectral_cross_attention_backward_workspace(const void* dout, con
 }
 
 extern "C" int spectral_cross_attention_backward(const void* dout, const void* q, const void* k, const void* v, const long long* strides,
-                                                 const void* out, const float* stats, const void* lengths, int lengths64, const void* mask,
+                                                 const void* out, const void* rest, const float* stats, const void* lengths, int lengths64, const void* mask,
                                                  void* dq, void* dk, void* dv, int dtype, long long batch, long long queries, long long keys,
                                                  int heads, int kv_heads, int dim, float scale, void* work, void* stream)
 {
@@ -967,6 +974,7 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         c.lengths64 = lengths64;
         c.mask = static_cast<const unsigned char*>(mask);
         c.out = const_cast<void*>(out);
+        c.rest = const_cast<signed char*>(static_cast<const signed char*>(rest));
         c.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
         c.dout = dout;
         c.dq = dq;

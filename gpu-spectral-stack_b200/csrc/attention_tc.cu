@@ -23,6 +23,26 @@ namespace {
 
 constexpr float kSlack = 8.0f;  // in powers of two, see above
 
+template <class T>
+__device__ __forceinline__ void store_rest(signed char* p, const float (&o)[16], int valid)
+{
+    Vec<signed char, 16> v;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        v.v[j] = Rest<T>::code(o[j]);
+    }
+    if (valid == 16 && (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0) {
+        *reinterpret_cast<Vec<signed char, 16>*>(p) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (j < valid) {
+                p[j] = v.v[j];
+            }
+        }
+    }
+}
+
 struct Forward {
     HeadMap q, k, v;
     Call c;
@@ -442,7 +462,8 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
             const float base_m = m == -INFINITY ? (g.splits > 1 ? m : 0.0f) : m - kOffset;
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
             const long long part_row = (it.split * c.pairs() + at) * c.rows() + row;
-            T* out = live ? static_cast<T*>(c.out) + c.row_at(it.b, it.head, row) : nullptr;
+            const long long out_at = live ? c.row_at(it.b, it.head, row) : 0;
+            T* out = static_cast<T*>(c.out) + out_at;
             if (!idle) {
                 for (int d = 0; d < c.dim; d += 16) {
                     float o[16];
@@ -465,6 +486,9 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
                                 o[k] *= inverse;
                             }
                             mlp::store_values<T>(out + d, o, valid);
+                            if (c.rest != nullptr) {
+                                store_rest<T>(c.rest + out_at + d, o, valid);
+                            }
                         }
                     }
                 }

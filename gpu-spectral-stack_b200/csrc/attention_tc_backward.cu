@@ -643,7 +643,23 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
         if (there) {
             const int b = static_cast<int>(pair_at / c.kv_heads);
             const long long at = c.row_at(b, static_cast<int>(pair_at - static_cast<long long>(b) * c.kv_heads), r);
-            const Floats<8> x = fetch(o + at), y = fetch(g + at);
+            Floats<8> x = fetch(o + at);
+            const Floats<8> y = fetch(g + at);
+            if (c.rest != nullptr && sub * 8 < c.dim) {
+                Vec<signed char, 8> code{};
+                if constexpr (Vectors) {
+                    code = *reinterpret_cast<const Vec<signed char, 8>*>(c.rest + at + sub * 8);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        code.v[j] = sub * 8 + j < c.dim ? c.rest[at + sub * 8 + j] : static_cast<signed char>(0);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x.set(j, Rest<T>::restored(x.at(j), code.v[j]));
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 dot = fma2(x.p[j], y.p[j], dot);
@@ -834,7 +850,7 @@ void tensor_backward(const Call& c, char* work, cudaStream_t stream)
     const long long entries = std::max(c.pairs() * plan.row_tiles * kTile, is_bf16 ? 0LL : c.pairs() * c.keys);
     const auto grid = static_cast<unsigned>(std::min<long long>((entries * lanes + 255) / 256, kNormCtas));
     g.norm_count = static_cast<int>(grid);
-    const bool vectors = c.dim % 8 == 0 && aligned_to(c.out, 16) && aligned_to(c.dout, 16);
+    const bool vectors = c.dim % 8 == 0 && aligned_to(c.out, 16) && aligned_to(c.dout, 16) && aligned_to(c.rest, 8);
     const int heads = c.kv_heads * c.group;
     const auto rows_map = [&](const Operand& o) {
         return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.queries, heads, c.dim, c.group, g.tokens_per_tile);

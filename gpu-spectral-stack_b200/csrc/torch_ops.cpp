@@ -1135,7 +1135,12 @@ struct AttentionArrays {
     }
 };
 
-std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+// out; stats and, for 16-bit types, rest if they are kept.
+struct AttentionResult {
+    at::Tensor out, stats, rest;
+};
+
+AttentionResult attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                      const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
                                                      c10::optional<double> scale, bool keep)
 {
@@ -1146,29 +1151,32 @@ std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const 
     const AttentionSizes& n = a.n;
     at::Tensor out = at::empty(q.sizes(), q.options());
     at::Tensor stats;
+    at::Tensor rest;
     if (keep) {
         stats = at::empty({n.batch, n.kv_heads, n.kv_heads > 0 ? n.queries * (n.heads / n.kv_heads) : 0, 2}, q.options().dtype(at::kFloat));
+        rest = at::empty(q.scalar_type() == at::kFloat ? at::IntArrayRef({0}) : q.sizes(), q.options().dtype(at::kChar));
     }
     size_t count = 0;
     check_status(spectral_cross_attention_workspace(cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.dtype, n.batch, n.queries, n.keys, n.heads,
                                                     n.kv_heads, n.dim, &count));
     at::Tensor work = workspace(count, q);
     check_status(spectral_cross_attention(cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.lengths_ptr(), a.lengths64(), a.mask_ptr(), mptr(out),
-                                          keep ? static_cast<float*>(mptr(stats)) : nullptr, a.dtype, n.batch, n.queries, n.keys, n.heads,
+                                          keep ? mptr(rest) : nullptr, keep ? static_cast<float*>(mptr(stats)) : nullptr, a.dtype, n.batch, n.queries, n.keys, n.heads,
                                           n.kv_heads, n.dim, a.scale, mptr(work), stream()));
-    return {out, stats};
+    return {out, stats, rest};
 }
 
-std::tuple<at::Tensor, at::Tensor> cross_attention_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attention_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                         const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
                                                         c10::optional<double> scale)
 {
-    return attention_forward(q, k, v, lengths, mask, scale, true);
+    AttentionResult r = attention_forward(q, k, v, lengths, mask, scale, true);
+    return {r.out, r.stats, r.rest};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor>
 cross_attention_backward_cuda(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
-                              const at::Tensor& stats, const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
+                              const at::Tensor& stats, const at::Tensor& rest, const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
                               c10::optional<double> scale)
 {
     constexpr const char* op = "cross_attention_backward";
@@ -1183,9 +1191,12 @@ cross_attention_backward_cuda(const at::Tensor& dout, const at::Tensor& q, const
     TORCH_CHECK(stats.is_cuda() && stats.device() == q.device() && stats.scalar_type() == at::kFloat && n.kv_heads > 0
                     && stats.numel() == 2 * n.batch * n.queries * n.heads,
                 op, ": stats must be what cross_attention returned");
+    TORCH_CHECK(rest.is_cuda() && rest.device() == q.device() && rest.scalar_type() == at::kChar && (rest.numel() == 0 || rest.sizes() == q.sizes()),
+                op, ": rest must be what cross_attention returned");
     const at::Tensor dc = dout.contiguous();
     const at::Tensor oc = out.contiguous();
     const at::Tensor sc = stats.contiguous();
+    const at::Tensor rc = rest.contiguous();
     at::Tensor dq = at::empty(q.sizes(), q.options());
     at::Tensor dk = at::empty(k.sizes(), q.options());
     at::Tensor dv = at::empty(v.sizes(), q.options());
@@ -1193,7 +1204,7 @@ cross_attention_backward_cuda(const at::Tensor& dout, const at::Tensor& q, const
     check_status(spectral_cross_attention_backward_workspace(cptr(dc), cptr(a.q), cptr(a.k), cptr(a.v), a.strides, a.dtype, n.batch, n.queries, n.keys,
                                                              n.heads, n.kv_heads, n.dim, &count));
     at::Tensor work = workspace(count, q);
-    check_status(spectral_cross_attention_backward(cptr(dc), cptr(a.q), cptr(a.k), cptr(a.v), a.strides, cptr(oc), fptr(sc), a.lengths_ptr(),
+    check_status(spectral_cross_attention_backward(cptr(dc), cptr(a.q), cptr(a.k), cptr(a.v), a.strides, cptr(oc), rc.numel() > 0 ? cptr(rc) : nullptr, fptr(sc), a.lengths_ptr(),
                                                    a.lengths64(), a.mask_ptr(), mptr(dq), mptr(dk), mptr(dv), a.dtype, n.batch, n.queries, n.keys,
                                                    n.heads, n.kv_heads, n.dim, a.scale, mptr(work), stream()));
     return {dq, dk, dv};
@@ -1450,11 +1461,11 @@ struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction
                               const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask, c10::optional<double> scale)
     {
         at::AutoDispatchBelowAutograd guard;
-        auto [out, stats] = attention_forward(q, k, v, lengths, mask, scale, true);
+        const AttentionResult r = attention_forward(q, k, v, lengths, mask, scale, true);
         const at::Tensor none;
-        ctx->save_for_backward({q, k, v, out, stats, lengths.value_or(none), mask.value_or(none)});
+        ctx->save_for_backward({q, k, v, r.out, r.stats, r.rest, lengths.value_or(none), mask.value_or(none)});
         ctx->saved_data["scale"] = scale;
-        return out;
+        return r.out;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
@@ -1463,8 +1474,8 @@ struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction
         const bool create_graph = at::GradMode::is_enabled();
         const at::NoGradGuard no_grad;
         const variable_list kept = ctx->get_saved_variables();
-        auto [dq, dk, dv] = cross_attention_backward_cuda(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], optional_of(kept[5]),
-                                                          optional_of(kept[6]), ctx->saved_data["scale"].toOptional<double>());
+        auto [dq, dk, dv] = cross_attention_backward_cuda(grads[0], kept[0], kept[1], kept[2], kept[3], kept[4], kept[5], optional_of(kept[6]),
+                                                          optional_of(kept[7]), ctx->saved_data["scale"].toOptional<double>());
         const at::Tensor none;
         return finish_once(create_graph, "cross_attention", grads, {dq, dk, dv, none, none, none});
     }
@@ -1473,7 +1484,7 @@ struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction
 at::Tensor cross_attention_layer_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
                                       const c10::optional<at::Tensor>& mask, c10::optional<double> scale)
 {
-    return std::get<0>(attention_forward(q, k, v, lengths, mask, scale, false));
+    return attention_forward(q, k, v, lengths, mask, scale, false).out;
 }
 
 at::Tensor cross_attention_layer_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
@@ -1550,8 +1561,8 @@ TORCH_LIBRARY(spectral, m)
     m.def("qk_norm_rotary_layer(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_positions,"
           " Tensor? k_positions, float eps, float theta, int rotated, str pairs) -> Tensor[]");
     m.def("cross_attention(Tensor q, Tensor k, Tensor v, Tensor? lengths=None, Tensor? mask=None, float? scale=None)"
-          " -> (Tensor, Tensor)");
-    m.def("cross_attention_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor stats,"
+          " -> (Tensor, Tensor, Tensor)");
+    m.def("cross_attention_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor stats, Tensor rest,"
           " Tensor? lengths=None, Tensor? mask=None, float? scale=None) -> (Tensor, Tensor, Tensor)");
     m.def("cross_attention_layer(Tensor q, Tensor k, Tensor v, Tensor? lengths, Tensor? mask, float? scale) -> Tensor");
 }

@@ -109,10 +109,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spectral_qk_norm_rotary_backward_workspace": (_i, [_i, _szp]),
     "spectral_qk_norm_rotary_backward": (_i, [_heads, _heads, _i, _ll, _i, _i, _i, _i, _f, _f, _p, _p]),
     "spectral_cross_attention_workspace": (_i, [_p] * 3 + [_strides, _i, _ll, _ll, _ll, _i, _i, _i, _szp]),
-    "spectral_cross_attention": (_i, [_p] * 3 + [_strides, _p, _i, _p, _p, _p, _i, _ll, _ll, _ll, _i, _i, _i, _f, _p, _p]),
+    "spectral_cross_attention": (_i, [_p] * 3 + [_strides, _p, _i, _p, _p, _p, _p, _i, _ll, _ll, _ll, _i, _i, _i, _f, _p, _p]),
     "spectral_cross_attention_backward_workspace": (_i, [_p] * 4 + [_strides, _i, _ll, _ll, _ll, _i, _i, _i, _szp]),
     "spectral_cross_attention_backward": (
-        _i, [_p] * 4 + [_strides, _p, _p, _p, _i] + [_p] * 4 + [_i, _ll, _ll, _ll, _i, _i, _i, _f, _p, _p]),
+        _i, [_p] * 4 + [_strides, _p, _p, _p, _p, _i] + [_p] * 4 + [_i, _ll, _ll, _ll, _i, _i, _i, _f, _p, _p]),
     "spectral_fp32_ceiling": (_i, [_p, _i, _i, _p, ctypes.POINTER(ctypes.c_double)]),
     "spectral_spectrum": (_i, [_s, _p, _p, _p, _ll, _i, _ll, _p]),
     "spectral_fir": (_i, [_s, _p, _p, _p, _ll, _i, _i, _ll, _p]),

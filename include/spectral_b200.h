@@ -443,7 +443,8 @@ SPECTRAL_API int spectral_qk_norm_rotary_backward(const spectral_heads* q, const
  * by side); NULL for contiguous arrays. A key counts if its index is below lengths[sample] (`batch`
  * int32, or int64 if lengths64 is not 0; NULL: keys) and mask[sample * keys + key] is not 0 (bytes; NULL: all);
  * what lies in the others' places, infinities and NaN among it, has no effect. A row without keys gives zeros.
- * out is contiguous and must not overlap the inputs. stats (batch x kv_heads x queries heads / kv_heads pairs of
+ * out is contiguous and must not overlap the inputs. rest (16-bit types, a byte per value of out, or NULL) receives what
+ * out's rounding took, for the accuracy of the backward pass. stats (batch x kv_heads x queries heads / kv_heads pairs of
  * floats, or NULL) is kept for the backward pass. Products of 16-bit values run on the tensor cores with FP32
  * accumulators, the softmax's weights rounded to the type in between; float32 runs in FP32 throughout.
  * work: as many complex values as the workspace function says for the same arrays (NULL is an array of unknown
@@ -452,16 +453,16 @@ SPECTRAL_API int spectral_cross_attention_workspace(const void* q, const void* k
                                                     long long batch, long long queries, long long keys, int heads, int kv_heads,
                                                     int dim, size_t* count);
 SPECTRAL_API int spectral_cross_attention(const void* q, const void* k, const void* v, const long long* strides, const void* lengths,
-                                          int lengths64, const void* mask, void* out, float* stats, int dtype, long long batch,
+                                          int lengths64, const void* mask, void* out, void* rest, float* stats, int dtype, long long batch,
                                           long long queries, long long keys, int heads, int kv_heads, int dim, float scale,
                                           void* work, void* stream);
-/* Its gradients for dout, from the forward call's out and stats: dq, dk and dv, contiguous, of the type and shapes
+/* Its gradients for dout, from the forward call's out, rest (or NULL: out as rounded) and stats: dq, dk and dv, contiguous, of the type and shapes
  * of q, k and v (zeros for keys that do not count). dout is contiguous. Fixed summation order. */
 SPECTRAL_API int spectral_cross_attention_backward_workspace(const void* dout, const void* q, const void* k, const void* v,
                                                              const long long* strides, int dtype, long long batch, long long queries,
                                                              long long keys, int heads, int kv_heads, int dim, size_t* count);
 SPECTRAL_API int spectral_cross_attention_backward(const void* dout, const void* q, const void* k, const void* v,
-                                                   const long long* strides, const void* out, const float* stats, const void* lengths,
+                                                   const long long* strides, const void* out, const void* rest, const float* stats, const void* lengths,
                                                    int lengths64, const void* mask, void* dq, void* dk, void* dv, int dtype,
                                                    long long batch, long long queries, long long keys, int heads, int kv_heads, int dim,
                                                    float scale, void* work, void* stream);

@@ -470,7 +470,7 @@ def test_fno_block_with_a_context():
 
 
 def arguments(**change):
-    a = dict(q=1 << 20, k=1 << 21, v=1 << 22, strides=None, lengths=None, lengths64=0, mask=None, out=1 << 23, stats=1 << 24, dtype=1, batch=2,
+    a = dict(q=1 << 20, k=1 << 21, v=1 << 22, strides=None, lengths=None, lengths64=0, mask=None, out=1 << 23, rest=None, stats=1 << 24, dtype=1, batch=2,
              queries=4, keys=8, heads=4, kv_heads=2, dim=16, scale=1.0, work=1 << 25, stream=None)
     a.update(change)
     return tuple(a.values())
@@ -494,7 +494,7 @@ def test_the_c_abi_refuses(change, message):
      (dict(dq=(1 << 27) + 1), "aligned"), (dict(dq=(1 << 20) + 64), "must not overlap"), (dict(dv=(1 << 19) + 64), "must not overlap"),
      (dict(dtype=-1), "dtype must be")])
 def test_the_c_abi_refuses_backward(change, message):
-    a = dict(dout=1 << 19, q=1 << 20, k=1 << 21, v=1 << 22, strides=None, out=1 << 23, stats=1 << 24, lengths=None, lengths64=0, mask=None,
+    a = dict(dout=1 << 19, q=1 << 20, k=1 << 21, v=1 << 22, strides=None, out=1 << 23, rest=None, stats=1 << 24, lengths=None, lengths64=0, mask=None,
              dq=1 << 27, dk=1 << 28, dv=1 << 29, dtype=1, batch=2, queries=4, keys=8, heads=4, kv_heads=2, dim=16, scale=1.0, work=1 << 30,
              stream=None)
     a.update(change)
