@@ -46,12 +46,11 @@ __device__ __forceinline__ void store_rest(signed char* p, const float (&o)[16],
 struct Forward {
     HeadMap q, k, v;
     Call c;
-    int rows_per_tile = 0;    // 128 / group * group
-    int tokens_per_tile = 0;
-    int row_items = 0;        // pairs of row tiles
-    int splits = 1;
+    int tokens_per_tile = 0;  // 128 / group
+    unsigned row_items = 0;   // pairs of row tiles
+    unsigned splits = 1;
     int split_tiles = 0;      // key tiles of a split
-    long long items = 0;
+    unsigned items = 0;
     float factor = 1.0f;      // |scale| log2(e)
     bool negative = false;    // scale < 0
     float* partial = nullptr;
@@ -70,19 +69,19 @@ struct Item {
     int slots;      // row tiles with rows
 };
 
-__device__ __forceinline__ Item item_at(const Forward& g, long long i)
+__device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
 {
     Item it;
-    const long long r = i / g.row_items;
+    const unsigned r = i / g.row_items;
     it.row_tile = static_cast<int>(i - r * g.row_items) * 2;
-    const long long pair = r / g.splits;
+    const unsigned pair = r / g.splits;
     it.split = static_cast<int>(r - pair * g.splits);
-    it.b = static_cast<int>(pair / g.c.kv_heads);
-    it.head = static_cast<int>(pair - static_cast<long long>(it.b) * g.c.kv_heads);
+    it.b = static_cast<int>(pair / static_cast<unsigned>(g.c.kv_heads));
+    it.head = static_cast<int>(pair) - it.b * g.c.kv_heads;
     it.key0 = it.split * g.split_tiles * kTile;
     it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * kTile);
     it.tiles = it.end > it.key0 ? (it.end - it.key0 + kTile - 1) / kTile : 0;
-    it.slots = static_cast<long long>(it.row_tile + 1) * g.rows_per_tile < g.c.rows() ? 2 : 1;
+    it.slots = (it.row_tile + 1) * g.tokens_per_tile < g.c.queries ? 2 : 1;
     return it;
 }
 
@@ -91,7 +90,8 @@ struct Config {
     static constexpr int kThreads = Cut ? 352 : 320;
     static constexpr int kTileBytes = Boxes * kBox;
     static constexpr int kStages = Boxes == 1 ? 8 : 5;  // of K and V tiles
-    static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
+    static constexpr int kQueries = Boxes == 1 ? 2 : 1;   // items whose queries are kept
+    static constexpr int kSmem = (2 * kQueries + kStages) * kTileBytes + 1024;
     static constexpr int kO = 256;                       // tensor memory: S and P 0 and 1, then O 0 and 1
     static constexpr int kCols = 512;
     static_assert(kSmem <= kSmemMost - 1024, "shared memory");
@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
     constexpr int kStages = Cfg::kStages;
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
-    const uint32_t ring = base + 2 * Cfg::kTileBytes;
-    __shared__ uint64_t q_full, q_empty, full[kStages], empty[kStages], clean[kStages], s_full[2], p_full[2], o_full[2], o_free[2], drain;
+    const uint32_t ring = base + 2 * Cfg::kQueries * Cfg::kTileBytes;
+    __shared__ uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], clean[kStages], s_full[2], p_full[2], o_full[2], o_free[2], drain;
     __shared__ uint32_t tmem_slot;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -115,14 +115,14 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         umma::alloc<Cfg::kCols>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
-        tma::mbar_init(&q_full, 1);
-        tma::mbar_init(&q_empty, 1);
         for (int s = 0; s < kStages; ++s) {
             tma::mbar_init(&full[s], 1);
             tma::mbar_init(&empty[s], 1);
             tma::mbar_init(&clean[s], 1);
         }
         for (int x = 0; x < 2; ++x) {
+            tma::mbar_init(&q_full[x], 1);
+            tma::mbar_init(&q_empty[x], 1);
             tma::mbar_init(&s_full[x], 1);
             tma::mbar_init(&p_full[x], 4);
             tma::mbar_init(&o_full[x], 1);
@@ -144,27 +144,27 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
     if (warp == 8) {
         // The TMA warp: Q of an item as soon as the one before is read, then its K and V tiles in turn.
         asm volatile("fence.proxy.async.global;" ::: "memory");
-        const unsigned q_bytes = static_cast<unsigned>(g.rows_per_tile) * umma::kRowBytes * Boxes;
+        const unsigned q_bytes = static_cast<unsigned>(g.tokens_per_tile * c.group) * umma::kRowBytes * Boxes;
         int stage = 0;
-        unsigned phase = 0, q_phase = 0;
+        unsigned phase = 0;
         long long issued = 0, q_issued = 0;
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at(g, i);
             if (it.tiles == 0) {
                 continue;
             }
-            ok = tma::mbar_wait(&q_empty, q_phase ^ 1u);
+            const int kept = static_cast<int>(q_issued % Cfg::kQueries);
+            ok = tma::mbar_wait(&q_empty[kept], (static_cast<unsigned>(q_issued / Cfg::kQueries) & 1u) ^ 1u);
             if (!ok) {
                 break;
             }
-            q_phase ^= 1u;
             if (umma::elect_one()) {
-                tma::mbar_arrive_expect_tx(&q_full, q_bytes * it.slots);
+                tma::mbar_arrive_expect_tx(&q_full[kept], q_bytes * it.slots);
                 for (int x = 0; x < it.slots; ++x) {
 #pragma unroll
                     for (int j = 0; j < Boxes; ++j) {
-                        load_heads(base + x * Cfg::kTileBytes + j * kBox, g.q, j * umma::kAtom, it.head * c.group,
-                                   (it.row_tile + x) * g.tokens_per_tile, it.b, &q_full);
+                        load_heads(base + (2 * kept + x) * Cfg::kTileBytes + j * kBox, g.q, j * umma::kAtom, it.head * c.group,
+                                   (it.row_tile + x) * g.tokens_per_tile, it.b, &q_full[kept]);
                     }
                 }
             }
@@ -192,7 +192,10 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
             }
         }
         if (!ok) {  // the loads in flight land (bounded) before the shared memory is given up
-            bool drained = q_issued == 0 || tma::mbar_wait(&q_full, static_cast<unsigned>(q_issued - 1) & 1u);
+            bool drained = true;
+            for (long long i = q_issued > Cfg::kQueries ? q_issued - Cfg::kQueries : 0; i < q_issued; ++i) {
+                drained = tma::mbar_wait(&q_full[i % Cfg::kQueries], static_cast<unsigned>(i / Cfg::kQueries) & 1u) && drained;
+            }
             for (long long i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
                 drained = tma::mbar_wait(&full[i % kStages], static_cast<unsigned>(i / kStages) & 1u) && drained;
             }
@@ -206,12 +209,13 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         const uint32_t score = umma::instruction(kBf16, false, false, kTile, kTile);
         const uint32_t weigh = umma::instruction(kBf16, false, true, kTile, steps * 16);
         int stage = 0;
-        unsigned phase = 0, q_phase = 0, cleaned = 0;
+        unsigned phase = 0, cleaned = 0, taken = 0;  // items
         unsigned slot_items[2] = {0, 0};
         unsigned p_phases[2] = {0, 0};
+        int kept = 0;
         const auto scores = [&](int x, uint32_t k_tile) {
             if (umma::elect_one()) {
-                const uint64_t a = umma::desc_k(base + x * Cfg::kTileBytes), b = umma::desc_k(k_tile);
+                const uint64_t a = umma::desc_k(base + (2 * kept + x) * Cfg::kTileBytes), b = umma::desc_k(k_tile);
                 for (int s = 0; s < steps; ++s) {
                     const uint64_t step = (s & 3) * umma::kStepK + (s >> 2) * (kBox >> 4);
                     umma::mma(tmem + x * kTile, a + step, b + step, score, s > 0);
@@ -226,16 +230,17 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
                 phase ^= 1u;
             }
         };
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at(g, i);
             if (it.tiles == 0) {
                 continue;
             }
-            ok = tma::mbar_wait(&q_full, q_phase) && tma::mbar_wait(&full[stage], phase);
+            kept = static_cast<int>(taken % Cfg::kQueries);
+            ok = tma::mbar_wait(&q_full[kept], taken / Cfg::kQueries & 1u) && tma::mbar_wait(&full[stage], phase);
             if (!ok) {
                 break;
             }
-            q_phase ^= 1u;
+            ++taken;
             umma::fence_after_sync();
             for (int x = 0; x < it.slots; ++x) {
                 scores(x, ring + stage * Cfg::kTileBytes);
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
             if (umma::elect_one()) {
                 umma::commit(&empty[stage]);
                 if (it.tiles == 1) {
-                    umma::commit(&q_empty);
+                    umma::commit(&q_empty[kept]);
                 }
             }
             __syncwarp();
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
                     if (more) {
                         umma::commit(&empty[k_stage]);
                         if (t + 2 == it.tiles) {
-                            umma::commit(&q_empty);
+                            umma::commit(&q_empty[kept]);
                         }
                     }
                 }
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         // The wiping warp: every V tile passes through it.
         int stage = 0;
         unsigned phase = 0;
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at(g, i);
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
@@ -351,16 +356,20 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         const uint32_t s_at = tmem + lanes + x * kTile;
         const uint32_t o_at = tmem + lanes + Cfg::kO + x * Boxes * 64;
         const int local = quad * 32 + lane;
+        const int row_token = local / c.group;
+        const int row_head = local - row_token * c.group;
         unsigned s_phase = 0, o_phase = 0;
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at(g, i);
             if (x >= it.slots) {
                 continue;
             }
-            const long long row = static_cast<long long>(it.row_tile + x) * g.rows_per_tile + local;
-            const bool live = local < g.rows_per_tile && row < c.rows();
+            const int first_token = (it.row_tile + x) * g.tokens_per_tile;
+            const int token = first_token + row_token;
+            const int row = token * c.group + row_head;
+            const bool live = row_token < g.tokens_per_tile && token < c.queries;
             // A warp without rows only keeps the barriers going; what lies in its lanes reaches no one.
-            const bool idle = quad * 32 >= g.rows_per_tile || static_cast<long long>(it.row_tile + x) * g.rows_per_tile + quad * 32 >= c.rows();
+            const bool idle = quad * 32 >= min(g.tokens_per_tile, c.queries - first_token) * c.group;
             float m = -INFINITY, sum = 0.0f;
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
@@ -462,7 +471,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
             const float base_m = m == -INFINITY ? (g.splits > 1 ? m : 0.0f) : m - kOffset;
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
             const long long part_row = (it.split * c.pairs() + at) * c.rows() + row;
-            const long long out_at = live ? c.row_at(it.b, it.head, row) : 0;
+            const long long out_at = ((static_cast<long long>(it.b) * c.queries + token) * c.kv_heads + it.head) * c.group * c.dim + row_head * c.dim;
             T* out = static_cast<T*>(c.out) + out_at;
             if (!idle) {
                 for (int d = 0; d < c.dim; d += 16) {
@@ -569,8 +578,7 @@ struct Plan {
         q = operand(arena, c.q, c.qs, c.batch, c.queries, c.kv_heads * c.group, c.dim, false);
         k = operand(arena, c.k, c.ks, c.batch, c.keys, c.kv_heads, c.dim, true);
         v = operand(arena, c.v, c.vs, c.batch, c.keys, c.kv_heads, c.dim, true);
-        const int rows = kTile / c.group * c.group;
-        row_items = pieces(pieces(c.rows(), rows), 2);
+        row_items = pieces(pieces(c.queries, kTile / c.group), 2);
         // Splits of the keys: the fewest turns of the busiest CTA, counted in key tiles, where an item costs about two
         // more (its first loads and scores, its last products and stores); parts are written and joined.
         const long long tiles = pieces(c.keys, kTile);
@@ -642,11 +650,14 @@ void tensor_forward(const Call& c, char* work, cudaStream_t stream)
     Forward g;
     g.c = c;
     g.tokens_per_tile = kTile / c.group;
-    g.rows_per_tile = g.tokens_per_tile * c.group;
     g.row_items = plan.row_items;
     g.splits = plan.splits;
     g.split_tiles = plan.split_tiles;
-    g.items = c.pairs() * plan.row_items * plan.splits;
+    const long long items = c.pairs() * plan.row_items * plan.splits;
+    if (items >= (1LL << 31)) {
+        throw InvalidArgument("cross_attention: too many tiles for one call");
+    }
+    g.items = static_cast<unsigned>(items);
     g.negative = c.scale < 0.0f;
     // A factor of 0 would turn the -infinity of a key that does not count into a NaN.
     g.factor = std::max(std::abs(c.scale) * kLog2e, 1.17549435e-38f);

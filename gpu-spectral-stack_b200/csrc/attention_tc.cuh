@@ -93,18 +93,24 @@ __device__ __forceinline__ void tile_bits(const Call& c, int b, int end, int key
     }
 }
 
-__device__ __forceinline__ bool all_count(const uint32_t (&w)[4]) { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
+// Whether the first 32 Words keys all do.
+template <int Words = 4>
+__device__ __forceinline__ bool all_count(const uint32_t (&w)[4])
+{
+    return (Words == 4 ? w[0] & w[1] & w[2] & w[3] : w[0] & w[1]) == 0xffffffffu;
+}
 
-// Zeros into the rows of a tile (`boxes` boxes) whose keys do not count, by one warp: a masked weight of 0 times an
+// Zeros into the rows of a tile (`boxes` boxes of Rows rows) whose keys do not count, by one warp: a masked weight of 0 times an
 // infinity or NaN would be a NaN. The async proxy's reads of the tile come after.
+template <int Rows = kTile>
 __device__ __forceinline__ void wipe_rows(uint32_t tile, int boxes, const uint32_t (&w)[4])
 {
     const int lane = threadIdx.x & 31;
-    for (int r = lane / 8; r < kTile; r += 4) {
+    for (int r = lane / 8; r < Rows; r += 4) {
         const uint32_t word = r < 64 ? (r < 32 ? w[0] : w[1]) : (r < 96 ? w[2] : w[3]);
         if ((word >> (r & 31) & 1u) == 0) {
             for (int box = 0; box < boxes; ++box) {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + box * kBox + r * umma::kRowBytes + (lane & 7) * 16), "r"(0)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (box * Rows + r) * umma::kRowBytes + (lane & 7) * 16), "r"(0)
                              : "memory");
             }
         }

@@ -26,22 +26,23 @@ namespace spectral::attention {
 namespace {
 
 constexpr int kSms = 148;
-constexpr int kConstants = 2 * kTile;        // floats per row tile: lse of its rows, then delta
 constexpr int kNormCtas = 4 * kSms;          // of the constants kernel, at most
 constexpr float kWeightPower = 15.0f;        // float16's p times 2^15
 
 struct Backward {
     HeadMap x0, x1, y0, y1;
     Call c;
-    int rows_per_tile = 0;
-    int tokens_per_tile = 0;
-    int row_tiles = 0;
-    int key_tiles = 0;
-    int parts = 1;
-    int part_tiles = 0;   // tiles walked over per part
-    long long items = 0;
-    float factor = 1.0f;  // c
-    const float* constants = nullptr;  // (pair, row tile, kConstants)
+    // Rows come in whole tokens: of the tiles that are owned, and of those walked over.
+    int owned_tokens = 0;
+    int walked_tokens = 0;
+    unsigned owned = 0;        // tiles that are owned
+    int walked = 0;            // tiles of rows to walk over (keys' kernel)
+    int row_walks = 0;         // tiles of rows in `constants`
+    unsigned parts = 1;
+    int part_tiles = 0;        // tiles walked over per part
+    unsigned items = 0;
+    float factor = 1.0f;       // c
+    const float* constants = nullptr;  // (pair, tile of walked_tokens): lse of its rows, then delta
     const float* norms = nullptr;      // float16: the CTAs' largest squares of rows of g, then of v
     int norm_count = 0;
     float* partial0 = nullptr;
@@ -59,57 +60,67 @@ struct Item {
     int end;     // keys before this count, but for the mask
 };
 
-// Rows: the CTA owns rows and walks over keys.
-template <bool Rows>
-__device__ __forceinline__ Item item_at(const Backward& g, long long i)
+// Rows: the CTA owns rows and walks over keys, `Width` at a time.
+template <bool Rows, int Width>
+__device__ __forceinline__ Item item_at(const Backward& g, unsigned i)
 {
     Item it;
-    const int owned = Rows ? g.row_tiles : g.key_tiles;
-    const long long r = i / owned;
-    it.tile = static_cast<int>(i - r * owned);
-    const long long pair = r / g.parts;
+    const unsigned r = i / g.owned;
+    it.tile = static_cast<int>(i - r * g.owned);
+    const unsigned pair = r / g.parts;
     it.part = static_cast<int>(r - pair * g.parts);
-    it.b = static_cast<int>(pair / g.c.kv_heads);
-    it.head = static_cast<int>(pair - static_cast<long long>(it.b) * g.c.kv_heads);
+    it.b = static_cast<int>(pair / static_cast<unsigned>(g.c.kv_heads));
+    it.head = static_cast<int>(pair) - it.b * g.c.kv_heads;
     it.end = length_of(g.c, it.b);
     it.first = it.part * g.part_tiles;
-    const int walked = Rows ? (it.end + kTile - 1) / kTile : it.tile * kTile < it.end ? g.row_tiles : 0;
+    const int walked = Rows ? (it.end + Width - 1) / Width : it.tile * kTile < it.end ? g.walked : 0;
     it.tiles = max(0, min(g.part_tiles, walked - it.first));
     return it;
 }
 
+// Heads of up to 64 values: 64 entries of the walk at a time, four warps on them, two CTAs per SM that fill each other's
+// waits (one CTA with 128 at a time and eight warps: see the table of the design notes). Wider heads: 128 at a time, one CTA.
 template <int Boxes, bool Rows, bool Wipe>
 struct Config {
-    static constexpr int kThreads = Wipe ? 352 : 320;
-    static constexpr int kTileBytes = Boxes * kBox;
+    static constexpr int kWidth = Boxes == 1 ? 64 : 128;
+    static constexpr int kCtas = Boxes == 1 ? 2 : 1;
+    static constexpr int kWarps = kWidth / 16;           // that turn scores: a thread per owned row and 64 columns
+    static constexpr int kThreads = 32 * (kWarps + (Wipe ? 3 : 2));
+    static constexpr int kOwnedBytes = Boxes * kBox;
+    static constexpr int kWalkedBox = kWidth * umma::kRowBytes;
+    static constexpr int kWalkedBytes = Boxes * kWalkedBox;
+    static constexpr int kConstants = 2 * kWidth;        // floats per tile of rows
     static constexpr int kConstantBytes = Rows ? 0 : kConstants * 4;
-    static constexpr int kStageBytes = 2 * kTileBytes;  // Y0, Y1
+    static constexpr int kStageBytes = 2 * kWalkedBytes;  // Y0, Y1
     static constexpr int kStages = Boxes == 1 ? 4 : 2;
-    static constexpr int kSmem = 2 * kTileBytes + kStages * (kStageBytes + kConstantBytes) + 1024;
-    static constexpr int kD = 128;                       // tensor memory: S and P, D and dS, A0, A1
-    static constexpr int kA0 = 256;
-    static constexpr int kA1 = 256 + Boxes * 64;
-    static constexpr int kCols = 512;
-    static_assert(kSmem <= kSmemMost - 1024, "shared memory");
+    static constexpr int kSmem = 2 * kOwnedBytes + kStages * (kStageBytes + kConstantBytes) + 1024;
+    static constexpr int kD = kWidth;                    // tensor memory: S and P, D and dS, A0, A1
+    static constexpr int kA0 = 2 * kWidth;
+    static constexpr int kA1 = 2 * kWidth + Boxes * 64;
+    static constexpr int kCols = Boxes == 1 ? 256 : 512;
+    static_assert(kCtas * (kSmem + 1024) <= kSmemMost, "shared memory");
+    static_assert(kCtas * kCols <= 512 && kA1 + Boxes * 64 <= kCols, "tensor memory");
 };
 
 template <class T, int Boxes, bool Rows, bool Wipe>
-__global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backward_kernel(const __grid_constant__ Backward g)
+__global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Boxes, Rows, Wipe>::kCtas) backward_kernel(const __grid_constant__ Backward g)
 {
     using Cfg = Config<Boxes, Rows, Wipe>;
     constexpr bool kBf16 = std::is_same_v<T, bf16>;
     constexpr int kStages = Cfg::kStages;
+    constexpr int kWidth = Cfg::kWidth;
+    constexpr int kWarps = Cfg::kWarps;
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
     unsigned char* const generic = smem_base + (base - tma::smem_addr(smem_base));
-    const uint32_t ring = base + 2 * Cfg::kTileBytes;
-    const float* const constants = reinterpret_cast<const float*>(generic + 2 * Cfg::kTileBytes + kStages * Cfg::kStageBytes);
+    const uint32_t ring = base + 2 * Cfg::kOwnedBytes;
+    const float* const constants = reinterpret_cast<const float*>(generic + 2 * Cfg::kOwnedBytes + kStages * Cfg::kStageBytes);
     __shared__ uint64_t x_full, x_empty, full[kStages], empty[kStages], clean[kStages], s_full, d_full, p_ready, ds_ready, acc_full, acc_free, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ float norm_of[2][12];
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::alloc<Cfg::kCols>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
@@ -122,19 +133,20 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
         }
         tma::mbar_init(&s_full, 1);
         tma::mbar_init(&d_full, 1);
-        tma::mbar_init(&p_ready, 8);
-        tma::mbar_init(&ds_ready, 8);
+        tma::mbar_init(&p_ready, kWarps);
+        tma::mbar_init(&ds_ready, kWarps);
         tma::mbar_init(&acc_full, 1);
-        tma::mbar_init(&acc_free, 8);
+        tma::mbar_init(&acc_free, kWarps);
         tma::mbar_init(&drain, 1);
         tma::fence_mbar_init();
     }
     if constexpr (!Rows) {
-        // Rows of a tile that no box writes (128 % group) are reduced over: zeros, once.
-        const int spare = kTile - g.rows_per_tile;
+        // Rows of a tile that no box writes (width % group) are reduced over: zeros, once.
+        const int used = g.walked_tokens * g.c.group;
+        const int spare = kWidth - used;
         for (int i = threadIdx.x; i < 2 * kStages * Boxes * spare * 8; i += Cfg::kThreads) {
             const int box = i / (spare * 8), at = i - box * spare * 8;
-            *reinterpret_cast<uint4*>(generic + (2 * Boxes + box) * kBox + (g.rows_per_tile + at / 8) * umma::kRowBytes + at % 8 * 16) =
+            *reinterpret_cast<uint4*>(generic + 2 * Cfg::kOwnedBytes + box * Cfg::kWalkedBox + (used + at / 8) * umma::kRowBytes + at % 8 * 16) =
                 make_uint4(0, 0, 0, 0);
         }
         tma::fence_proxy_async();
@@ -181,17 +193,17 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
         ds_scale = exp2f(static_cast<float>(max(-60, min(60, power))));
     }
 
-    if (warp == 8) {
+    if (warp == kWarps) {
         // The TMA warp: the owned tiles as soon as the item before has no more use for its own, then Y0, Y1 in turn.
         asm volatile("fence.proxy.async.global;" ::: "memory");
-        const unsigned row_bytes = static_cast<unsigned>(g.rows_per_tile) * umma::kRowBytes * Boxes;
-        const unsigned owned_bytes = 2 * (Rows ? row_bytes : Cfg::kTileBytes);
-        const unsigned walked_bytes = 2 * (Rows ? Cfg::kTileBytes : row_bytes) + Cfg::kConstantBytes;
+        const unsigned token_bytes = static_cast<unsigned>(c.group) * umma::kRowBytes * Boxes;
+        const unsigned owned_bytes = 2 * (Rows ? g.owned_tokens * token_bytes : Cfg::kOwnedBytes);
+        const unsigned walked_bytes = 2 * (Rows ? Cfg::kWalkedBytes : g.walked_tokens * token_bytes) + Cfg::kConstantBytes;
         int stage = 0;
         unsigned phase = 0, x_phase = 0;
         long long issued = 0, x_issued = 0;
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at<Rows>(g, i);
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows, kWidth>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
@@ -202,13 +214,13 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
             x_phase ^= 1u;
             const int x_head = Rows ? it.head * c.group : it.head;
             const int y_head = Rows ? it.head : it.head * c.group;
-            const int x_token = it.tile * (Rows ? g.tokens_per_tile : kTile);
+            const int x_token = it.tile * (Rows ? g.owned_tokens : kTile);
             if (umma::elect_one()) {
                 tma::mbar_arrive_expect_tx(&x_full, owned_bytes);
 #pragma unroll
                 for (int j = 0; j < Boxes; ++j) {
                     load_heads(base + j * kBox, g.x0, j * umma::kAtom, x_head, x_token, it.b, &x_full);
-                    load_heads(base + Cfg::kTileBytes + j * kBox, g.x1, j * umma::kAtom, x_head, x_token, it.b, &x_full);
+                    load_heads(base + Cfg::kOwnedBytes + j * kBox, g.x1, j * umma::kAtom, x_head, x_token, it.b, &x_full);
                 }
             }
             __syncwarp();
@@ -220,16 +232,16 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                 }
                 if (umma::elect_one()) {
                     const uint32_t y = ring + stage * Cfg::kStageBytes;
-                    const int y_token = t * (Rows ? kTile : g.tokens_per_tile);
+                    const int y_token = t * (Rows ? kWidth : g.walked_tokens);
                     tma::mbar_arrive_expect_tx(&full[stage], walked_bytes);
 #pragma unroll
                     for (int j = 0; j < Boxes; ++j) {
-                        load_heads(y + j * kBox, g.y0, j * umma::kAtom, y_head, y_token, it.b, &full[stage]);
-                        load_heads(y + Cfg::kTileBytes + j * kBox, g.y1, j * umma::kAtom, y_head, y_token, it.b, &full[stage]);
+                        load_heads(y + j * Cfg::kWalkedBox, g.y0, j * umma::kAtom, y_head, y_token, it.b, &full[stage]);
+                        load_heads(y + Cfg::kWalkedBytes + j * Cfg::kWalkedBox, g.y1, j * umma::kAtom, y_head, y_token, it.b, &full[stage]);
                     }
                     if constexpr (!Rows) {
-                        const long long at = (static_cast<long long>(it.b) * c.kv_heads + it.head) * g.row_tiles + t;
-                        tma::bulk_g2s(const_cast<float*>(constants) + stage * kConstants, g.constants + at * kConstants, Cfg::kConstantBytes,
+                        const long long at = (static_cast<long long>(it.b) * c.kv_heads + it.head) * g.row_walks + t;
+                        tma::bulk_g2s(const_cast<float*>(constants) + stage * Cfg::kConstants, g.constants + at * Cfg::kConstants, Cfg::kConstantBytes,
                                       &full[stage]);
                     }
                 }
@@ -250,21 +262,21 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == kWarps + 1) {
         // The MMA warp, one elected lane issues.
         const int steps = (c.dim + 15) / 16;
-        const uint32_t score = umma::instruction(kBf16, false, false, kTile, kTile);
+        const uint32_t score = umma::instruction(kBf16, false, false, kTile, kWidth);
         const uint32_t weigh = umma::instruction(kBf16, false, true, kTile, steps * 16);
         int stage = 0;
         unsigned phase = 0, x_phase = 0, step_phase = 0, acc_phase = 0;
         // S (k = 0) or D (k = 1) from the owned tiles and a stage's.
         const auto scores = [&](int k, int y_stage, uint64_t* done) {
             if (umma::elect_one()) {
-                const uint64_t a = umma::desc_k(base + k * Cfg::kTileBytes);
-                const uint64_t b = umma::desc_k(ring + y_stage * Cfg::kStageBytes + k * Cfg::kTileBytes);
+                const uint64_t a = umma::desc_k(base + k * Cfg::kOwnedBytes);
+                const uint64_t b = umma::desc_k(ring + y_stage * Cfg::kStageBytes + k * Cfg::kWalkedBytes);
                 for (int s = 0; s < steps; ++s) {
-                    const uint64_t step = (s & 3) * umma::kStepK + (s >> 2) * (kBox >> 4);
-                    umma::mma(tmem + k * Cfg::kD, a + step, b + step, score, s > 0);
+                    const uint64_t step = (s & 3) * umma::kStepK;
+                    umma::mma(tmem + k * Cfg::kD, a + step + (s >> 2) * (kBox >> 4), b + step + (s >> 2) * (Cfg::kWalkedBox >> 4), score, s > 0);
                 }
                 umma::commit(done);
             }
@@ -272,16 +284,16 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
         };
         // A0 += dS Y0 (k = 0), A1 += P Y1 (k = 1). The halves of P and dS lie 64 columns apart.
         const auto weighed = [&](int k, int y_stage, bool accumulate) {
-            const uint64_t b = umma::desc_mn<kBox>(ring + y_stage * Cfg::kStageBytes + k * Cfg::kTileBytes);
+            const uint64_t b = umma::desc_mn<Cfg::kWalkedBox>(ring + y_stage * Cfg::kStageBytes + k * Cfg::kWalkedBytes);
             const uint32_t a = tmem + (k == 0 ? Cfg::kD : 0);
 #pragma unroll
-            for (int s = 0; s < kTile / 16; ++s) {
+            for (int s = 0; s < kWidth / 16; ++s) {
                 mma_tmem(tmem + (k == 0 ? Cfg::kA0 : Cfg::kA1), a + (s >> 2) * 64 + (s & 3) * 8, b + umma::kStepMn * s, weigh, accumulate || s > 0);
             }
         };
         const auto arrived = [&](int y_stage, unsigned y_phase) { return tma::mbar_wait(Wipe ? &clean[y_stage] : &full[y_stage], y_phase); };
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at<Rows>(g, i);
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows, kWidth>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
@@ -293,6 +305,14 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
             umma::fence_after_sync();
             scores(0, stage, &s_full);
             scores(1, stage, &d_full);
+            // After its last scores an item has no more use for the owned tiles.
+            const auto release = [&](int t) {
+                if (t + 1 == it.tiles && umma::elect_one()) {
+                    umma::commit(&x_empty);
+                }
+                __syncwarp();
+            };
+            release(0);
             for (int t = 0; ok && t < it.tiles; ++t) {
                 const bool more = t + 1 < it.tiles;
                 const int now = stage;
@@ -325,12 +345,12 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                     umma::commit(&empty[now]);
                     if (!more) {
                         umma::commit(&acc_full);
-                        umma::commit(&x_empty);
                     }
                 }
                 __syncwarp();
                 if (more) {
                     scores(1, stage, &d_full);
+                    release(t + 1);
                 }
             }
             acc_phase ^= 1u;
@@ -345,18 +365,18 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (Wipe && warp == 10) {
+    } else if (Wipe && warp == kWarps + 2) {
         // The wiping warp: every stage passes through it. (Only k is reduced over; masked scores are dropped.)
         int stage = 0;
         unsigned phase = 0;
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at<Rows>(g, i);
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows, kWidth>(g, i);
             for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
                 uint32_t w[4];
-                tile_bits(c, it.b, it.end, t * kTile, w);
+                tile_bits(c, it.b, it.end, t * kWidth, w);
                 ok = tma::mbar_wait(&full[stage], phase);
-                if (ok && !all_count(w)) {
-                    wipe_rows(ring + stage * Cfg::kStageBytes, Boxes, w);
+                if (ok && !all_count<kWidth / 32>(w)) {
+                    wipe_rows<kWidth>(ring + stage * Cfg::kStageBytes, Boxes, w);
                 }
                 __syncwarp();
                 if (ok && lane == 0) {
@@ -371,8 +391,8 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
         if (!ok && lane == 0) {
             atomicOr(g.fault, tma::kFaultWaitTimeout);
         }
-    } else if (warp < 8) {
-        // A thread per owned row: warps 0 to 3 the first 64 columns, 4 to 7 the others.
+    } else if (warp < kWarps) {
+        // A thread per owned row and 64 columns: with 128 at a time warps 0 to 3 the first, 4 to 7 the others.
         const int half = warp >> 2;
         const int local = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -381,17 +401,25 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
         int stage = 0;
         unsigned phase = 0, step_phase = 0, acc_phase = 0;
         const float power = kBf16 ? 0.0f : kWeightPower;
-        for (long long i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at<Rows>(g, i);
+        // Where an owned row lies: token and head in the group.
+        const int row_token = local / c.group;
+        const int row_head = local - row_token * c.group;
+        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+            const Item it = item_at<Rows, kWidth>(g, i);
             const long long pair_at = static_cast<long long>(it.b) * c.kv_heads + it.head;
             // Rows: this row's constants. Keys: whether this key counts.
             float2 shift = pair(0.0f), delta = pair(0.0f);
             bool counts = true;
-            const long long row = static_cast<long long>(it.tile) * (Rows ? g.rows_per_tile : kTile) + local;
+            const int token = it.tile * g.owned_tokens + row_token;
+            const int row = Rows ? token * c.group + row_head : it.tile * kTile + local;
+            const bool live = Rows ? row_token < g.owned_tokens && token < c.queries : row < c.keys;
             if constexpr (Rows) {
-                const float* at = g.constants + (pair_at * g.row_tiles + it.tile) * kConstants + local;
-                shift = pair(-at[0]);
-                delta = pair(at[kTile]);
+                if (live) {
+                    const int tile = token / g.walked_tokens;
+                    const float* at = g.constants + (pair_at * g.row_walks + tile) * Cfg::kConstants + (token - tile * g.walked_tokens) * c.group + row_head;
+                    shift = pair(-at[0]);
+                    delta = pair(at[kWidth]);
+                }
             } else {
                 counts = row < it.end && (c.mask == nullptr || c.mask[static_cast<long long>(it.b) * c.keys + row] != 0);
             }
@@ -399,11 +427,11 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
             for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
                 uint32_t w[4];
                 if constexpr (Rows) {
-                    tile_bits(c, it.b, it.end, t * kTile, w);
+                    tile_bits(c, it.b, it.end, t * kWidth, w);
                 } else {
                     ok = tma::mbar_wait(&full[stage], phase);
                 }
-                const float* lse = constants + stage * kConstants + half * 64;
+                const float* lse = constants + stage * Cfg::kConstants + half * 64;
                 ok = ok && tma::mbar_wait(&s_full, step_phase);
                 if (!ok) {
                     break;
@@ -432,7 +460,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                     }
                 }
                 if constexpr (Rows) {
-                    if (!all_count(w)) {
+                    if (!all_count<kWidth / 32>(w)) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) {
                             const uint32_t word = half == 0 ? w[j / 32] : w[2 + j / 32];
@@ -472,50 +500,49 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                 }
                 step_phase ^= 1u;
                 umma::fence_after_sync();
-                float d[2][32];
-                umma::load32(d_at, d[0]);
-                umma::load32(d_at + 32, d[1]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    umma::load_wait(d[j]);
+                    float d[1][32];
+                    umma::load32(d_at + 32 * j, d[0]);
+                    umma::load_wait(d[0]);
                     uint32_t out[16];
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
                         float2 a = delta, b = delta;
                         if constexpr (!Rows) {
-                            const float4 l = *reinterpret_cast<const float4*>(lse + kTile + 32 * j + k);
+                            const float4 l = *reinterpret_cast<const float4*>(lse + kWidth + 32 * j + k);
                             a = make_float2(l.x, l.y);
                             b = make_float2(l.z, l.w);
                         }
-                        a = (make_float2(d[j][k], d[j][k + 1]) - a) * make_float2(p[j][k], p[j][k + 1]);
-                        b = (make_float2(d[j][k + 2], d[j][k + 3]) - b) * make_float2(p[j][k + 2], p[j][k + 3]);
+                        a = (make_float2(d[0][k], d[0][k + 1]) - a) * make_float2(p[j][k], p[j][k + 1]);
+                        b = (make_float2(d[0][k + 2], d[0][k + 3]) - b) * make_float2(p[j][k + 2], p[j][k + 3]);
                         if constexpr (!kBf16) {
                             a = a * pair(ds_scale);
                             b = b * pair(ds_scale);
                         }
-                        d[j][k] = a.x;
-                        d[j][k + 1] = a.y;
-                        d[j][k + 2] = b.x;
-                        d[j][k + 3] = b.y;
+                        d[0][k] = a.x;
+                        d[0][k + 1] = a.y;
+                        d[0][k + 2] = b.x;
+                        d[0][k + 3] = b.y;
                     }
                     // A key that does not count may have made D anything.
                     if constexpr (Rows) {
-                        if (!all_count(w)) {
+                        if (!all_count<kWidth / 32>(w)) {
                             const uint32_t word = half == 0 ? w[j] : w[2 + j];
 #pragma unroll
                             for (int k = 0; k < 32; ++k) {
-                                d[j][k] = (word >> k & 1u) != 0 ? d[j][k] : 0.0f;
+                                d[0][k] = (word >> k & 1u) != 0 ? d[0][k] : 0.0f;
                             }
                         }
                     } else if (!whole) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
-                            d[j][k] = counts ? d[j][k] : 0.0f;
+                            d[0][k] = counts ? d[0][k] : 0.0f;
                         }
                     }
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        out[k] = pack2<T>(make_float2(d[j][2 * k], d[j][2 * k + 1]));
+                        out[k] = pack2<T>(make_float2(d[0][2 * k], d[0][2 * k + 1]));
                     }
                     store16(d_at + 16 * j, out);
                 }
@@ -541,33 +568,37 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
                 acc_phase ^= 1u;
                 umma::fence_after_sync();
             }
-            // Keys: the first warps store dk, the others dv. Rows: each half of dq.
-            const bool of_v = !Rows && half == 1;
+            // With eight warps the first four store dk (dq: the first half of it), the others dv; four store it all.
             const int span = (c.dim + 15) / 16;
-            const int from = Rows ? (half == 0 ? 0 : (span + 1) / 2 * 16) : 0;
-            const int to = Rows && half == 0 ? (span + 1) / 2 * 16 : c.dim;
-            const float factor = it.tiles == 0 || !counts ? 0.0f : of_v ? exp2f(-power) : (g.parts > 1 ? 1.0f : c.scale) / ds_scale;
-            const bool live = Rows ? local < g.rows_per_tile && row < c.rows() : row < c.keys;
-            const long long entries = Rows ? c.rows() : c.keys;
-            const long long part_row = (it.part * c.pairs() + pair_at) * entries + row;
-            float* partial = of_v ? g.partial1 : g.partial0;
-            T* result = static_cast<T*>(Rows ? c.dq : of_v ? c.dv : c.dk);
-            const long long at = Rows ? c.row_at(it.b, it.head, row) : ((static_cast<long long>(it.b) * c.keys + row) * c.kv_heads + it.head) * c.dim;
-            for (int d = from; d < to && d < c.dim; d += 16) {
-                float a[16];
-                if (it.tiles > 0) {
-                    umma::load16(tmem + lanes + (of_v ? Cfg::kA1 : Cfg::kA0) + d, a);
-                    umma::load_wait(a);
-                }
+            const int cut = kWarps == 8 ? (span + 1) / 2 * 16 : c.dim;
+            const long long part_row = (it.part * c.pairs() + pair_at) * (Rows ? c.rows() : c.keys) + row;
+            const long long at = Rows ? ((static_cast<long long>(it.b) * c.queries + token) * c.kv_heads + it.head) * c.group * c.dim + row_head * c.dim
+                                      : ((static_cast<long long>(it.b) * c.keys + row) * c.kv_heads + it.head) * c.dim;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    a[k] = it.tiles == 0 || !counts ? 0.0f : a[k] * factor;
+            for (int which = 0; which < (Rows ? 1 : 2); ++which) {
+                const bool of_v = which == 1;
+                if (!Rows && kWarps == 8 && which != half) {
+                    continue;
                 }
-                if (live) {
-                    if (g.parts > 1) {
-                        mlp::store_values<float>(partial + part_row * c.dim + d, a, min(16, c.dim - d));
-                    } else {
-                        mlp::store_values<T>(result + at + d, a, min(16, c.dim - d));
+                const float factor = of_v ? exp2f(-power) : (g.parts > 1 ? 1.0f : c.scale) / ds_scale;
+                float* partial = of_v ? g.partial1 : g.partial0;
+                T* result = static_cast<T*>(Rows ? c.dq : of_v ? c.dv : c.dk);
+                for (int d = Rows && half == 1 ? cut : 0; d < (Rows && half == 0 ? min(cut, c.dim) : c.dim); d += 16) {
+                    float a[16];
+                    if (it.tiles > 0) {
+                        umma::load16(tmem + lanes + (of_v ? Cfg::kA1 : Cfg::kA0) + d, a);
+                        umma::load_wait(a);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        a[k] = it.tiles == 0 || !counts ? 0.0f : a[k] * factor;
+                    }
+                    if (live) {
+                        if (g.parts > 1) {
+                            mlp::store_values<float>(partial + part_row * c.dim + d, a, min(16, c.dim - d));
+                        } else {
+                            mlp::store_values<T>(result + at + d, a, min(16, c.dim - d));
+                        }
                     }
                 }
             }
@@ -586,7 +617,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::dealloc<Cfg::kCols>(tmem);
     }
 }
@@ -597,7 +628,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, 1) backwa
 // every row tile, `lanes` lanes of eight values a row. float16: also the largest squares of g's rows and v's
 // keys that this CTA met (finite ones).
 template <class T, bool Vectors>
-__global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __restrict__ out, float* __restrict__ norms, int rows_per_tile,
+__global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __restrict__ out, float* __restrict__ norms, int width, int rows_per_tile,
                                                         int row_tiles, int lanes)
 {
     __shared__ float top_of[2][8];
@@ -630,12 +661,12 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
         return s;
     };
     float top[2] = {0.0f, 0.0f};
-    const long long all = c.pairs() * row_tiles * kTile;
+    const long long all = c.pairs() * row_tiles * width;
     // Whole warps stay in the loops together: they shuffle.
     for (long long base = static_cast<long long>(blockIdx.x) * per_cta; base < all; base += static_cast<long long>(gridDim.x) * per_cta) {
         const long long i = base + threadIdx.x / lanes;
-        const int local = static_cast<int>(i % kTile);
-        const long long tile = i / kTile;
+        const int local = static_cast<int>(i % width);
+        const long long tile = i / width;
         const long long pair_at = tile / row_tiles;
         const long long r = (tile - pair_at * row_tiles) * rows_per_tile + local;
         const bool there = i < all && local < rows_per_tile && r < c.rows();
@@ -677,9 +708,9 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
                 const float2 s = c.stats[pair_at * c.rows() + r];
                 lse = s.y == 0.0f ? INFINITY : s.x + log2f(s.y);
             }
-            float* at = out + tile * kConstants + local;
+            float* at = out + tile * 2 * width + local;
             at[0] = lse;
-            at[kTile] = delta;
+            at[width] = delta;
         }
     }
     if constexpr (std::is_same_v<T, f16>) {
@@ -727,16 +758,17 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
 
 // How many parts `walked` tiles are cut into for `owned` items of one part each: the fewest turns of the busiest CTA,
 // counted in tiles (an item costs about two more), at most kLongestSum entries a part.
-void cut(long long owned, int walked, int& parts, int& part_tiles)
+void cut(long long owned, int walked, int width, int ctas, int& parts, int& part_tiles)
 {
-    const long long least = std::max(1, (walked + kLongestSum / kTile - 1) / (kLongestSum / kTile));
+    const int most = kLongestSum / width;
+    const long long least = std::max(1, (walked + most - 1) / most);
     double best = 0.0;
     for (long long s = least; s <= std::max<long long>(least, std::min(walked, 64)); ++s) {
         const long long span = (walked + s - 1) / s;
         if (s > least && (walked + span - 1) / span != s) {
             continue;
         }
-        const double turns = static_cast<double>((owned * s + kSms - 1) / kSms) * (static_cast<double>(span) + 2.0) + (s > 1 ? 3.0 + 0.1 * s : 0.0);
+        const double turns = static_cast<double>((owned * s + ctas - 1) / ctas) * (static_cast<double>(span) + 2.0) + (s > 1 ? 3.0 + 0.1 * s : 0.0);
         if (s == least || turns < best) {
             best = turns;
             parts = static_cast<int>(s);
@@ -748,7 +780,10 @@ void cut(long long owned, int walked, int& parts, int& part_tiles)
 
 struct Plan {
     Operand q, k, v, dout;
-    int rows_per_tile = 0, row_tiles = 0, key_tiles = 0;
+    int boxes = 1, width = 64;
+    int owned_tokens = 0, walked_tokens = 0;
+    int row_tiles = 0, key_tiles = 0;  // owned
+    int row_walks = 0, key_walks = 0;
     int row_parts = 1, row_span = 0;   // keys' kernel: parts of the rows
     int key_parts = 1, key_span = 0;   // rows' kernel: parts of the keys
     std::size_t constants = 0, norms = 0, dq = 0, dk = 0, dv = 0;
@@ -762,12 +797,18 @@ struct Plan {
         k = operand(arena, c.k, c.ks, c.batch, c.keys, c.kv_heads, c.dim, true);
         v = operand(arena, c.v, c.vs, c.batch, c.keys, c.kv_heads, c.dim, true);
         dout = operand(arena, c.dout, dense, c.batch, c.queries, heads, c.dim, false);
-        rows_per_tile = kTile / c.group * c.group;
-        row_tiles = pieces(c.rows(), rows_per_tile);
+        boxes = c.dim <= 64 && c.group <= 64 ? 1 : 2;  // a tile that is walked over holds a token's heads
+        width = boxes == 1 ? 64 : 128;
+        owned_tokens = kTile / c.group;
+        walked_tokens = width / c.group;
+        row_tiles = pieces(c.queries, owned_tokens);
         key_tiles = pieces(c.keys, kTile);
-        cut(c.pairs() * key_tiles, row_tiles, row_parts, row_span);
-        cut(c.pairs() * row_tiles, key_tiles, key_parts, key_span);
-        constants = arena.take(static_cast<std::size_t>(c.pairs()) * row_tiles * kConstants * sizeof(float));
+        row_walks = pieces(c.queries, walked_tokens);
+        key_walks = pieces(c.keys, width);
+        const int ctas = kSms * (boxes == 1 ? 2 : 1);
+        cut(c.pairs() * key_tiles, row_walks, width, ctas, row_parts, row_span);
+        cut(c.pairs() * row_tiles, key_walks, width, ctas, key_parts, key_span);
+        constants = arena.take(static_cast<std::size_t>(c.pairs()) * row_walks * 2 * width * sizeof(float));
         norms = arena.take(2 * kNormCtas * sizeof(float));
         if (key_parts > 1) {
             dq = arena.take(static_cast<std::size_t>(c.pairs()) * c.rows() * c.dim * key_parts * sizeof(float));
@@ -779,42 +820,60 @@ struct Plan {
     }
 };
 
+unsigned item_count(long long items)
+{
+    if (items >= (1LL << 31)) {
+        throw InvalidArgument("cross_attention_backward: too many tiles for one call");
+    }
+    return static_cast<unsigned>(items);
+}
+
 template <class T, int Boxes, bool Rows, bool Wipe>
 void launch(const Backward& g, cudaStream_t stream)
 {
     using Cfg = Config<Boxes, Rows, Wipe>;
     const auto kernel = backward_kernel<T, Boxes, Rows, Wipe>;
-    static std::atomic<int> cache[kMaxDevices];
-    const unsigned grid = persistent_grid(reinterpret_cast<const void*>(kernel), Cfg::kThreads, Cfg::kSmem, cache, g.items);
+    static std::atomic<bool> ready[kMaxDevices];
+    const int device = current_device();
+    if (!ready[device].load(std::memory_order_relaxed)) {
+        const auto* f = reinterpret_cast<const void*>(kernel);
+        SPECTRAL_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+        // All of the SM's memory, or the occupancy is one CTA where two fit.
+        SPECTRAL_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+        ready[device].store(true, std::memory_order_relaxed);
+    }
+    const unsigned grid = std::min(g.items, static_cast<unsigned>(device_sm_count(device) * Cfg::kCtas));
     launch_pdl(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, g);
 }
 
 template <class T, int Boxes>
-void both(Backward g, const Plan& plan, const HeadMap (&rows)[2], const HeadMap (&keys)[2], char* work, cudaStream_t stream)
+void both(Backward g, const Plan& plan, const HeadMap (&rows)[2], const HeadMap (&row_walk)[2], const HeadMap (&keys)[2], const HeadMap (&key_walk)[2],
+          char* work, cudaStream_t stream)
 {
     const Call& c = g.c;
-    const bool cut = c.lengths != nullptr || c.mask != nullptr;
     // dk and dv.
     g.x0 = keys[0];
     g.x1 = keys[1];
-    g.y0 = rows[0];
-    g.y1 = rows[1];
+    g.y0 = row_walk[0];
+    g.y1 = row_walk[1];
+    g.owned = plan.key_tiles;
     g.parts = plan.row_parts;
     g.part_tiles = plan.row_span;
-    g.items = c.pairs() * plan.key_tiles * plan.row_parts;
+    g.items = item_count(c.pairs() * plan.key_tiles * plan.row_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dk);
     g.partial1 = reinterpret_cast<float*>(work + plan.dv);
     launch<T, Boxes, false, false>(g, stream);
     // dq.
     g.x0 = rows[0];
     g.x1 = rows[1];
-    g.y0 = keys[0];
-    g.y1 = keys[1];
+    g.y0 = key_walk[0];
+    g.y1 = key_walk[1];
+    g.owned = plan.row_tiles;
     g.parts = plan.key_parts;
     g.part_tiles = plan.key_span;
-    g.items = c.pairs() * plan.row_tiles * plan.key_parts;
+    g.items = item_count(c.pairs() * plan.row_tiles * plan.key_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dq);
-    if (cut) {
+    if (c.lengths != nullptr || c.mask != nullptr) {
         launch<T, Boxes, true, true>(g, stream);
     } else {
         launch<T, Boxes, true, false>(g, stream);
@@ -833,10 +892,10 @@ void tensor_backward(const Call& c, char* work, cudaStream_t stream)
     const bool is_bf16 = c.dtype == SPECTRAL_BFLOAT16;
     Backward g;
     g.c = c;
-    g.tokens_per_tile = kTile / c.group;
-    g.rows_per_tile = plan.rows_per_tile;
-    g.row_tiles = plan.row_tiles;
-    g.key_tiles = plan.key_tiles;
+    g.owned_tokens = plan.owned_tokens;
+    g.walked_tokens = plan.walked_tokens;
+    g.walked = plan.row_walks;
+    g.row_walks = plan.row_walks;
     g.factor = c.scale * kLog2e;
     auto* constants = reinterpret_cast<float*>(work + plan.constants);
     auto* norms = reinterpret_cast<float*>(work + plan.norms);
@@ -847,28 +906,34 @@ void tensor_backward(const Call& c, char* work, cudaStream_t stream)
     while (lanes * 8 < c.dim) {
         lanes *= 2;
     }
-    const long long entries = std::max(c.pairs() * plan.row_tiles * kTile, is_bf16 ? 0LL : c.pairs() * c.keys);
+    const long long entries = std::max(c.pairs() * plan.row_walks * plan.width, is_bf16 ? 0LL : c.pairs() * c.keys);
     const auto grid = static_cast<unsigned>(std::min<long long>((entries * lanes + 255) / 256, kNormCtas));
     g.norm_count = static_cast<int>(grid);
     const bool vectors = c.dim % 8 == 0 && aligned_to(c.out, 16) && aligned_to(c.dout, 16) && aligned_to(c.rest, 8);
     const int heads = c.kv_heads * c.group;
-    const auto rows_map = [&](const Operand& o) {
-        return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.queries, heads, c.dim, c.group, g.tokens_per_tile);
+    const auto rows_map = [&](const Operand& o, int tokens) {
+        return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.queries, heads, c.dim, c.group, tokens);
     };
-    const auto keys_map = [&](const Operand& o) { return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile); };
-    const HeadMap rows[2] = {rows_map(plan.q), rows_map(plan.dout)};
-    const HeadMap keys[2] = {keys_map(plan.k), keys_map(plan.v)};
+    const auto keys_map = [&](const Operand& o, int keys) {
+        return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, keys);
+    };
+    const HeadMap rows[2] = {rows_map(plan.q, plan.owned_tokens), rows_map(plan.dout, plan.owned_tokens)};
+    const HeadMap row_walk[2] = {rows_map(plan.q, plan.walked_tokens), rows_map(plan.dout, plan.walked_tokens)};
+    const HeadMap keys[2] = {keys_map(plan.k, kTile), keys_map(plan.v, kTile)};
+    const HeadMap key_walk[2] = {keys_map(plan.k, plan.width), keys_map(plan.v, plan.width)};
     const auto run = [&](auto t) {
         using T = decltype(t);
         if (vectors) {
-            launch_pdl(constants_kernel<T, true>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.rows_per_tile, plan.row_tiles, lanes);
+            launch_pdl(constants_kernel<T, true>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.width, plan.walked_tokens * c.group,
+                       plan.row_walks, lanes);
         } else {
-            launch_pdl(constants_kernel<T, false>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.rows_per_tile, plan.row_tiles, lanes);
+            launch_pdl(constants_kernel<T, false>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.width, plan.walked_tokens * c.group,
+                       plan.row_walks, lanes);
         }
-        if (c.dim <= 64) {
-            both<T, 1>(g, plan, rows, keys, work, stream);
+        if (plan.boxes == 1) {
+            both<T, 1>(g, plan, rows, row_walk, keys, key_walk, work, stream);
         } else {
-            both<T, 2>(g, plan, rows, keys, work, stream);
+            both<T, 2>(g, plan, rows, row_walk, keys, key_walk, work, stream);
         }
     };
     if (is_bf16) {
