@@ -4,7 +4,7 @@
 // scores S = Q K^T into tensor memory, from where a thread per row takes its 128 scores to registers, and
 // O += P V with the weights P written back over S as the 16-bit operand. While one row tile's threads work on
 // their scores the tensor cores multiply for the other. A warp brings tiles of K and V in by TMA through a ring, a
-// warp issues the products, and with a length or a mask a warp wipes the values of keys that do not count.
+// warp issues the products.
 //
 // Softmax in one pass: a row's weights are 2^(c s - m) with m the largest c s when it was last moved, and m moves only
 // if a later score passes it by more than 2^8; then O in tensor memory and the sum are scaled. Weights reach 2^8 that way,
@@ -85,9 +85,9 @@ __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
     return it;
 }
 
-template <int Boxes, bool Cut>
+template <int Boxes>
 struct Config {
-    static constexpr int kThreads = Cut ? 352 : 320;
+    static constexpr int kThreads = 320;
     static constexpr int kTileBytes = Boxes * kBox;
     static constexpr int kStages = Boxes == 1 ? 8 : 5;  // of K and V tiles
     static constexpr int kQueries = Boxes == 1 ? 2 : 1;   // items whose queries are kept
@@ -97,17 +97,17 @@ struct Config {
     static_assert(kSmem <= kSmemMost - 1024, "shared memory");
 };
 
-template <class T, int Boxes, bool Cut>
-__global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kernel(const __grid_constant__ Forward g)
+template <class T, int Boxes>
+__global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(const __grid_constant__ Forward g)
 {
-    using Cfg = Config<Boxes, Cut>;
+    using Cfg = Config<Boxes>;
     constexpr bool kBf16 = std::is_same_v<T, bf16>;
     constexpr float kOffset = kBf16 ? 0.0f : 7.0f;  // weights times 2^7
     constexpr int kStages = Cfg::kStages;
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
     const uint32_t ring = base + 2 * Cfg::kQueries * Cfg::kTileBytes;
-    __shared__ uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], clean[kStages], s_full[2], p_full[2], o_full[2], o_free[2], drain;
+    __shared__ uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[2], p_full[2], o_full[2], o_free[2], drain;
     __shared__ uint32_t tmem_slot;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -118,7 +118,6 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         for (int s = 0; s < kStages; ++s) {
             tma::mbar_init(&full[s], 1);
             tma::mbar_init(&empty[s], 1);
-            tma::mbar_init(&clean[s], 1);
         }
         for (int x = 0; x < 2; ++x) {
             tma::mbar_init(&q_full[x], 1);
@@ -209,7 +208,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         const uint32_t score = umma::instruction(kBf16, false, false, kTile, kTile);
         const uint32_t weigh = umma::instruction(kBf16, false, true, kTile, steps * 16);
         int stage = 0;
-        unsigned phase = 0, cleaned = 0, taken = 0;  // items
+        unsigned phase = 0, taken = 0;  // items
         unsigned slot_items[2] = {0, 0};
         unsigned p_phases[2] = {0, 0};
         int kept = 0;
@@ -255,9 +254,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
             advance();
             for (int t = 0; ok && t < it.tiles; ++t) {
                 const int v_stage = stage;
-                // Only V tiles pass the wiping warp, so their barriers count their own phases.
-                ok = Cut ? tma::mbar_wait(&clean[stage], cleaned >> stage & 1u) : tma::mbar_wait(&full[stage], phase);
-                cleaned ^= 1u << stage;
+                ok = tma::mbar_wait(&full[stage], phase);
                 advance();
                 const bool more = t + 1 < it.tiles;
                 const int k_stage = stage;
@@ -318,37 +315,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (Cut && warp == 10) {
-        // The wiping warp: every V tile passes through it.
-        int stage = 0;
-        unsigned phase = 0;
-        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
-            for (int t = 0; ok && t < it.tiles; ++t) {
-                uint32_t w[4];
-                tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
-                if (++stage == kStages) {  // past the K tile
-                    stage = 0;
-                    phase ^= 1u;
-                }
-                ok = tma::mbar_wait(&full[stage], phase);
-                if (ok && !all_count(w)) {
-                    wipe_rows(ring + stage * Cfg::kTileBytes, Boxes, w);
-                }
-                __syncwarp();
-                if (ok && lane == 0) {
-                    umma::arrive(&clean[stage]);
-                }
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            }
-        }
-        if (!ok && lane == 0) {
-            atomicOr(g.fault, tma::kFaultWaitTimeout);
-        }
-    } else if (warp < 8) {
+    } else {
         // A thread per row: warps 0 to 3 the first tile's, 4 to 7 the second's.
         const int x = warp >> 2;
         const int quad = warp & 3;
@@ -359,9 +326,11 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
         const int row_token = local / c.group;
         const int row_head = local - row_token * c.group;
         unsigned s_phase = 0, o_phase = 0;
+        unsigned entry = 0;  // of the ring: the next K tile
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at(g, i);
             if (x >= it.slots) {
+                entry += 2 * it.tiles;
                 continue;
             }
             const int first_token = (it.row_tile + x) * g.tokens_per_tile;
@@ -373,9 +342,7 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
             float m = -INFINITY, sum = 0.0f;
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
-                if (!idle) {
-                    tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
-                }
+                tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
                 ok = tma::mbar_wait(&s_full[x], s_phase);
                 if (!ok) {
                     break;
@@ -450,6 +417,13 @@ __global__ void __launch_bounds__(Config<Boxes, Cut>::kThreads, 1) forward_kerne
                     sum += total.x + total.y;
                     store_wait();
                 }
+                if (!all_count(w)) {
+                    // Both row tiles wipe all of V: the other's products may come first.
+                    const unsigned v_entry = entry + 1;
+                    ok = tma::mbar_wait(&full[v_entry % kStages], v_entry / kStages & 1u);
+                    wipe_rows<kTile, 4>(ring + v_entry % kStages * Cfg::kTileBytes, Boxes, w, quad);
+                }
+                entry += 2;
                 umma::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
@@ -535,7 +509,7 @@ struct StageJob {
     Strides stride;
     long long tokens;
     int heads;
-    long long values;  // of the target
+    long long rows;  // heads of all tokens
 };
 struct StageJobs {
     StageJob job[4];
@@ -543,21 +517,49 @@ struct StageJobs {
     int pitch;
 };
 
-// 16-bit values, whatever their type: a thread per target value, zeros in the padding.
+// 16-bit values, whatever their type: a warp takes four heads at a time, all their values asked for before one is stored.
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ StageJobs g)
 {
+    constexpr int kHeads = 4;
+    constexpr int kPer = SPECTRAL_HEAD_DIM_MAX / 32;
     allow_next_grid();
     wait_for_previous_grid();
     const StageJob& j = g.job[blockIdx.y];
-    const auto* source = static_cast<const unsigned short*>(j.source);
-    auto* target = static_cast<unsigned short*>(j.target);
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < j.values; i += static_cast<long long>(gridDim.x) * 256) {
-        const long long row = i / g.pitch;
-        const int d = static_cast<int>(i - row * g.pitch);
-        const long long token = row / j.heads;
-        const long long b = token / j.tokens;
-        target[i] = d < g.dim ? source[b * j.stride.sample + (token - b * j.tokens) * j.stride.token + (row - token * j.heads) * j.stride.head + d]
-                              : static_cast<unsigned short>(0);
+    const auto* __restrict__ source = static_cast<const unsigned short*>(j.source);
+    auto* __restrict__ target = static_cast<unsigned short*>(j.target);
+    const int lane = threadIdx.x & 31;
+    const unsigned heads = j.heads, tokens = static_cast<unsigned>(j.tokens);
+    for (long long first = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * kHeads; first < j.rows;
+         first += static_cast<long long>(gridDim.x) * 8 * kHeads) {
+        unsigned short v[kHeads][kPer];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const long long row = first + h;
+            long long token, b;
+            if (j.rows < (1LL << 31)) {
+                token = static_cast<unsigned>(row) / heads;
+                b = static_cast<unsigned>(token) / tokens;
+            } else {
+                token = row / heads;
+                b = token / tokens;
+            }
+            const auto* from = source + b * j.stride.sample + (token - b * tokens) * j.stride.token + (row - token * heads) * j.stride.head;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int d = lane + 32 * k;
+                v[h][k] = row < j.rows && d < g.dim ? from[d] : static_cast<unsigned short>(0);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int d = lane + 32 * k;
+                if (first + h < j.rows && d < g.pitch) {
+                    target[(first + h) * g.pitch + d] = v[h][k];
+                }
+            }
+        }
     }
 }
 
@@ -606,11 +608,11 @@ struct Plan {
     }
 };
 
-template <class T, int Boxes, bool Cut>
+template <class T, int Boxes>
 void launch(const Forward& g, cudaStream_t stream)
 {
-    using Cfg = Config<Boxes, Cut>;
-    const auto kernel = forward_kernel<T, Boxes, Cut>;
+    using Cfg = Config<Boxes>;
+    const auto kernel = forward_kernel<T, Boxes>;
     static std::atomic<int> cache[kMaxDevices];
     const unsigned grid = persistent_grid(reinterpret_cast<const void*>(kernel), Cfg::kThreads, Cfg::kSmem, cache, g.items);
     launch_pdl(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, g);
@@ -628,13 +630,13 @@ void stage(const Operand* const* operands, int count, int batch, int dim, char* 
     for (int i = 0; i < count; ++i) {
         const Operand& o = *operands[i];
         if (o.staged && batch * o.tokens > 0) {
-            const long long values = batch * o.tokens * o.heads * g.pitch;
-            g.job[jobs++] = {o.source, work + o.at, o.stride, o.tokens, o.heads, values};
-            most = std::max(most, values);
+            const long long rows = batch * o.tokens * o.heads;
+            g.job[jobs++] = {o.source, work + o.at, o.stride, o.tokens, o.heads, rows};
+            most = std::max(most, rows);
         }
     }
     if (jobs > 0) {
-        const auto grid = static_cast<unsigned>(std::min<long long>((most + 255) / 256, kSms * 16));
+        const auto grid = static_cast<unsigned>(std::min<long long>((most + 31) / 32, kSms * 8));
         launch_pdl(stage_kernel, dim3(grid, jobs), dim3(256), 0, stream, g);
     }
 }
@@ -670,21 +672,11 @@ void tensor_forward(const Call& c, char* work, cudaStream_t stream)
         g.k = head_map(keys[0], is_bf16, plan.k.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile);
         g.v = head_map(keys[1], is_bf16, plan.v.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile);
     }
-    const bool cut = c.lengths != nullptr || c.mask != nullptr;
-    const auto run = [&](auto t, auto boxes) {
-        using T = decltype(t);
-        constexpr int Boxes = decltype(boxes)::value;
-        if (cut) {
-            launch<T, Boxes, true>(g, stream);
-        } else {
-            launch<T, Boxes, false>(g, stream);
-        }
-    };
     const auto with_boxes = [&](auto t) {
         if (c.dim <= 64) {
-            run(t, std::integral_constant<int, 1>{});
+            launch<decltype(t), 1>(g, stream);
         } else {
-            run(t, std::integral_constant<int, 2>{});
+            launch<decltype(t), 2>(g, stream);
         }
     };
     if (is_bf16) {

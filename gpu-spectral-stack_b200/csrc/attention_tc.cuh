@@ -100,13 +100,14 @@ __device__ __forceinline__ bool all_count(const uint32_t (&w)[4])
     return (Words == 4 ? w[0] & w[1] & w[2] & w[3] : w[0] & w[1]) == 0xffffffffu;
 }
 
-// Zeros into the rows of a tile (`boxes` boxes of Rows rows) whose keys do not count, by one warp: a masked weight of 0 times an
-// infinity or NaN would be a NaN. The async proxy's reads of the tile come after.
-template <int Rows = kTile>
-__device__ __forceinline__ void wipe_rows(uint32_t tile, int boxes, const uint32_t (&w)[4])
+// Zeros into the rows of a tile (`boxes` boxes of Rows rows) whose keys do not count: a masked weight of 0 times an infinity
+// or NaN would be a NaN. The Warps warps that are about to hand over the weights each take a share, `warp` of them;
+// the tile has landed, and the product that reads it comes after their arrivals.
+template <int Rows, int Warps>
+__device__ __forceinline__ void wipe_rows(uint32_t tile, int boxes, const uint32_t (&w)[4], int warp)
 {
     const int lane = threadIdx.x & 31;
-    for (int r = lane / 8; r < Rows; r += 4) {
+    for (int r = warp * (Rows / Warps) + lane / 8; r < (warp + 1) * (Rows / Warps); r += 4) {
         const uint32_t word = r < 64 ? (r < 32 ? w[0] : w[1]) : (r < 96 ? w[2] : w[3]);
         if ((word >> (r & 31) & 1u) == 0) {
             for (int box = 0; box < boxes; ++box) {
@@ -116,7 +117,6 @@ __device__ __forceinline__ void wipe_rows(uint32_t tile, int boxes, const uint32
         }
     }
     tma::fence_proxy_async();
-    __syncwarp();
 }
 
 // --- host ------------------------------------------------------------------------------------------

@@ -8,10 +8,9 @@
 // and g) and walks over key tiles for dq; the scores are computed in both. Per step, on tcgen05:
 //   S = X0 Y0^T and D = X1 Y1^T into tensor memory (X owned, Y the tiles of the walk)
 //   P over S and dS over D, as 16-bit operands; A1 += P Y1 (keys), A0 += dS Y0, accumulators in tensor memory.
-// Eight warps, a thread per owned row and half of the columns, first turn S to P, then D to dS; the products that
+// Warps with a thread per owned row and 32 columns first turn S to P, then D to dS; the products that
 // need P and the next S run under the second half of that, those that need dS and the next D under the first half of the
-// next step. A warp brings the tiles by TMA, one issues the products, and where keys are cut and walked over a warp wipes
-// the values of those that do not count.
+// next step. A warp brings the tiles by TMA, one issues the products.
 //
 // float16 keeps p times 2^15 and ds times a power of two that no |ds| takes past 2^15: |g v - delta| is at most
 // 2 max|g| max|v| (norms of rows and keys that count), which the kernel before these finds. Unscaled, weights of 2^-14 and
@@ -42,7 +41,7 @@ struct Backward {
     int part_tiles = 0;        // tiles walked over per part
     unsigned items = 0;
     float factor = 1.0f;       // c
-    const float* constants = nullptr;  // (pair, tile of walked_tokens): lse of its rows, then delta
+    const float* constants = nullptr;  // (pair, tile of walked_tokens): -lse of its rows, then -delta
     const float* norms = nullptr;      // float16: the CTAs' largest squares of rows of g, then of v
     int norm_count = 0;
     float* partial0 = nullptr;
@@ -78,14 +77,16 @@ __device__ __forceinline__ Item item_at(const Backward& g, unsigned i)
     return it;
 }
 
-// Heads of up to 64 values: 64 entries of the walk at a time, four warps on them, two CTAs per SM that fill each other's
-// waits (one CTA with 128 at a time and eight warps: see the table of the design notes). Wider heads: 128 at a time, one CTA.
-template <int Boxes, bool Rows, bool Wipe>
+// Heads of up to 64 values: 64 entries of the walk at a time and two CTAs per SM that fill each other's waits. Wider heads: 128
+// at a time, one CTA. Either way sixteen warps of an SM work on scores: their instructions follow from each other, and
+// with eight (64 columns a thread) an SM issued one in four cycles per scheduler.
+template <int Boxes, bool Rows>
 struct Config {
     static constexpr int kWidth = Boxes == 1 ? 64 : 128;
     static constexpr int kCtas = Boxes == 1 ? 2 : 1;
-    static constexpr int kWarps = kWidth / 16;           // that turn scores: a thread per owned row and 64 columns
-    static constexpr int kThreads = 32 * (kWarps + (Wipe ? 3 : 2));
+    static constexpr int kParts = kWidth / 32;           // of a row of scores: a thread per owned row and 32 columns
+    static constexpr int kWarps = 4 * kParts;            // that turn scores
+    static constexpr int kThreads = 32 * (kWarps + 2);
     static constexpr int kOwnedBytes = Boxes * kBox;
     static constexpr int kWalkedBox = kWidth * umma::kRowBytes;
     static constexpr int kWalkedBytes = Boxes * kWalkedBox;
@@ -102,10 +103,10 @@ struct Config {
     static_assert(kCtas * kCols <= 512 && kA1 + Boxes * 64 <= kCols, "tensor memory");
 };
 
-template <class T, int Boxes, bool Rows, bool Wipe>
-__global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Boxes, Rows, Wipe>::kCtas) backward_kernel(const __grid_constant__ Backward g)
+template <class T, int Boxes, bool Rows>
+__global__ void __launch_bounds__(Config<Boxes, Rows>::kThreads, Config<Boxes, Rows>::kCtas) backward_kernel(const __grid_constant__ Backward g)
 {
-    using Cfg = Config<Boxes, Rows, Wipe>;
+    using Cfg = Config<Boxes, Rows>;
     constexpr bool kBf16 = std::is_same_v<T, bf16>;
     constexpr int kStages = Cfg::kStages;
     constexpr int kWidth = Cfg::kWidth;
@@ -115,9 +116,9 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
     unsigned char* const generic = smem_base + (base - tma::smem_addr(smem_base));
     const uint32_t ring = base + 2 * Cfg::kOwnedBytes;
     const float* const constants = reinterpret_cast<const float*>(generic + 2 * Cfg::kOwnedBytes + kStages * Cfg::kStageBytes);
-    __shared__ uint64_t x_full, x_empty, full[kStages], empty[kStages], clean[kStages], s_full, d_full, p_ready, ds_ready, acc_full, acc_free, drain;
+    __shared__ uint64_t x_full, x_empty, full[kStages], empty[kStages], s_full, d_full, p_ready, ds_ready, acc_full, acc_free, drain;
     __shared__ uint32_t tmem_slot;
-    __shared__ float norm_of[2][12];
+    __shared__ float norm_of[2][20];
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     if (warp == kWarps) {
@@ -129,7 +130,6 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
         for (int s = 0; s < kStages; ++s) {
             tma::mbar_init(&full[s], 1);
             tma::mbar_init(&empty[s], 1);
-            tma::mbar_init(&clean[s], 1);
         }
         tma::mbar_init(&s_full, 1);
         tma::mbar_init(&d_full, 1);
@@ -282,22 +282,21 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
             }
             __syncwarp();
         };
-        // A0 += dS Y0 (k = 0), A1 += P Y1 (k = 1). The halves of P and dS lie 64 columns apart.
+        // A0 += dS Y0 (k = 0), A1 += P Y1 (k = 1). Each 32 columns of scores leave theirs in the first 16 of the same place.
         const auto weighed = [&](int k, int y_stage, bool accumulate) {
             const uint64_t b = umma::desc_mn<Cfg::kWalkedBox>(ring + y_stage * Cfg::kStageBytes + k * Cfg::kWalkedBytes);
             const uint32_t a = tmem + (k == 0 ? Cfg::kD : 0);
 #pragma unroll
             for (int s = 0; s < kWidth / 16; ++s) {
-                mma_tmem(tmem + (k == 0 ? Cfg::kA0 : Cfg::kA1), a + (s >> 2) * 64 + (s & 3) * 8, b + umma::kStepMn * s, weigh, accumulate || s > 0);
+                mma_tmem(tmem + (k == 0 ? Cfg::kA0 : Cfg::kA1), a + (s >> 1) * 32 + (s & 1) * 8, b + umma::kStepMn * s, weigh, accumulate || s > 0);
             }
         };
-        const auto arrived = [&](int y_stage, unsigned y_phase) { return tma::mbar_wait(Wipe ? &clean[y_stage] : &full[y_stage], y_phase); };
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at<Rows, kWidth>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
-            ok = tma::mbar_wait(&x_full, x_phase) && arrived(stage, phase);
+            ok = tma::mbar_wait(&x_full, x_phase) && tma::mbar_wait(&full[stage], phase);
             if (!ok) {
                 break;
             }
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
                     stage = 0;
                     phase ^= 1u;
                 }
-                ok = tma::mbar_wait(&p_ready, step_phase) && (t > 0 || tma::mbar_wait(&acc_free, acc_phase ^ 1u)) && (!more || arrived(stage, phase));
+                ok = tma::mbar_wait(&p_ready, step_phase) && (t > 0 || tma::mbar_wait(&acc_free, acc_phase ^ 1u)) && (!more || tma::mbar_wait(&full[stage], phase));
                 if (!ok) {
                     break;
                 }
@@ -365,38 +364,12 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (Wipe && warp == kWarps + 2) {
-        // The wiping warp: every stage passes through it. (Only k is reduced over; masked scores are dropped.)
-        int stage = 0;
-        unsigned phase = 0;
-        for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at<Rows, kWidth>(g, i);
-            for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
-                uint32_t w[4];
-                tile_bits(c, it.b, it.end, t * kWidth, w);
-                ok = tma::mbar_wait(&full[stage], phase);
-                if (ok && !all_count<kWidth / 32>(w)) {
-                    wipe_rows<kWidth>(ring + stage * Cfg::kStageBytes, Boxes, w);
-                }
-                __syncwarp();
-                if (ok && lane == 0) {
-                    umma::arrive(&clean[stage]);
-                }
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            }
-        }
-        if (!ok && lane == 0) {
-            atomicOr(g.fault, tma::kFaultWaitTimeout);
-        }
-    } else if (warp < kWarps) {
-        // A thread per owned row and 64 columns: with 128 at a time warps 0 to 3 the first, 4 to 7 the others.
-        const int half = warp >> 2;
+    } else {
+        // A thread per owned row and 32 columns: warps 4 k to 4 k + 3 the k-th.
+        const int part = warp >> 2;
         const int local = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + half * 64;
+        const uint32_t s_at = tmem + lanes + part * 32;
         const uint32_t d_at = s_at + Cfg::kD;
         int stage = 0;
         unsigned phase = 0, step_phase = 0, acc_phase = 0;
@@ -407,7 +380,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Item it = item_at<Rows, kWidth>(g, i);
             const long long pair_at = static_cast<long long>(it.b) * c.kv_heads + it.head;
-            // Rows: this row's constants. Keys: whether this key counts.
+            // Rows: this row's -lse and -delta. Keys: whether this key counts.
             float2 shift = pair(0.0f), delta = pair(0.0f);
             bool counts = true;
             const int token = it.tile * g.owned_tokens + row_token;
@@ -417,7 +390,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
                 if (live) {
                     const int tile = token / g.walked_tokens;
                     const float* at = g.constants + (pair_at * g.row_walks + tile) * Cfg::kConstants + (token - tile * g.walked_tokens) * c.group + row_head;
-                    shift = pair(-at[0]);
+                    shift = pair(at[0]);
                     delta = pair(at[kWidth]);
                 }
             } else {
@@ -425,68 +398,54 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
             }
             const bool whole = __all_sync(0xffffffffu, counts);
             for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
-                uint32_t w[4];
+                uint32_t w[4] = {0, 0, 0, 0};
                 if constexpr (Rows) {
                     tile_bits(c, it.b, it.end, t * kWidth, w);
-                } else {
-                    ok = tma::mbar_wait(&full[stage], phase);
                 }
-                const float* lse = constants + stage * Cfg::kConstants + half * 64;
+                ok = tma::mbar_wait(&full[stage], phase);
+                const float* less = constants + stage * Cfg::kConstants + part * 32;  // -lse, then -delta
+                const uint32_t word = Rows ? (part == 0 ? w[0] : part == 1 ? w[1] : part == 2 ? w[2] : w[3]) : counts ? 0xffffffffu : 0u;
+                const bool all = Rows ? word == 0xffffffffu : whole;
                 ok = ok && tma::mbar_wait(&s_full, step_phase);
                 if (!ok) {
                     break;
                 }
                 umma::fence_after_sync();
-                float p[2][32];
-                umma::load32(s_at, p[0]);
-                umma::load32(s_at + 32, p[1]);
+                float p[32];
+                umma::load32(s_at, p);
+                umma::load_wait(p);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    umma::load_wait(p[j]);
+                for (int k = 0; k < 32; k += 4) {
+                    float2 a = shift, b = shift;
+                    if constexpr (!Rows) {
+                        const float4 l = *reinterpret_cast<const float4*>(less + k);
+                        a = make_float2(l.x, l.y);
+                        b = make_float2(l.z, l.w);
+                    }
+                    a = fma2(make_float2(p[k], p[k + 1]), pair(g.factor), a);
+                    b = fma2(make_float2(p[k + 2], p[k + 3]), pair(g.factor), b);
+                    p[k] = exp2_fast(a.x);
+                    p[k + 1] = exp2_fast(a.y);
+                    p[k + 2] = exp2_fast(b.x);
+                    p[k + 3] = exp2_fast(b.y);
+                }
+                if (!all) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        float2 a = shift, b = shift;
-                        if constexpr (!Rows) {
-                            const float4 l = *reinterpret_cast<const float4*>(lse + 32 * j + k);
-                            a = make_float2(-l.x, -l.y);
-                            b = make_float2(-l.z, -l.w);
-                        }
-                        a = fma2(make_float2(p[j][k], p[j][k + 1]), pair(g.factor), a);
-                        b = fma2(make_float2(p[j][k + 2], p[j][k + 3]), pair(g.factor), b);
-                        p[j][k] = exp2_fast(a.x);
-                        p[j][k + 1] = exp2_fast(a.y);
-                        p[j][k + 2] = exp2_fast(b.x);
-                        p[j][k + 3] = exp2_fast(b.y);
+                    for (int k = 0; k < 32; ++k) {
+                        p[k] = (word >> k & 1u) != 0 ? p[k] : 0.0f;
                     }
                 }
-                if constexpr (Rows) {
-                    if (!all_count<kWidth / 32>(w)) {
+                if constexpr (!Rows) {
+                    uint32_t out[16];
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) {
-                            const uint32_t word = half == 0 ? w[j / 32] : w[2 + j / 32];
-                            p[j / 32][j % 32] = (word >> (j % 32) & 1u) != 0 ? p[j / 32][j % 32] : 0.0f;
+                    for (int k = 0; k < 16; ++k) {
+                        float2 v = make_float2(p[2 * k], p[2 * k + 1]);
+                        if constexpr (!kBf16) {
+                            v = v * pair(32768.0f);  // 2^kWeightPower
                         }
+                        out[k] = pack2<T>(v);
                     }
-                } else {
-                    if (!whole) {
-#pragma unroll
-                        for (int j = 0; j < 64; ++j) {
-                            p[j / 32][j % 32] = counts ? p[j / 32][j % 32] : 0.0f;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t out[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            float2 v = make_float2(p[j][2 * k], p[j][2 * k + 1]);
-                            if constexpr (!kBf16) {
-                                v = v * pair(exp2f(kWeightPower));
-                            }
-                            out[k] = pack2<T>(v);
-                        }
-                        store16(s_at + 16 * j, out);
-                    }
+                    store16(s_at, out);
                     store_wait();
                 }
                 umma::fence_before_sync();
@@ -500,53 +459,49 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
                 }
                 step_phase ^= 1u;
                 umma::fence_after_sync();
+                float d[32];
+                umma::load32(d_at, d);
+                umma::load_wait(d);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float d[1][32];
-                    umma::load32(d_at + 32 * j, d[0]);
-                    umma::load_wait(d[0]);
+                for (int k = 0; k < 32; k += 4) {
+                    float2 a = delta, b = delta;
+                    if constexpr (!Rows) {
+                        const float4 l = *reinterpret_cast<const float4*>(less + kWidth + k);
+                        a = make_float2(l.x, l.y);
+                        b = make_float2(l.z, l.w);
+                    }
+                    a = (make_float2(d[k], d[k + 1]) + a) * make_float2(p[k], p[k + 1]);
+                    b = (make_float2(d[k + 2], d[k + 3]) + b) * make_float2(p[k + 2], p[k + 3]);
+                    if constexpr (!kBf16) {
+                        a = a * pair(ds_scale);
+                        b = b * pair(ds_scale);
+                    }
+                    d[k] = a.x;
+                    d[k + 1] = a.y;
+                    d[k + 2] = b.x;
+                    d[k + 3] = b.y;
+                }
+                // A key that does not count may have made D anything.
+                if (!all) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        d[k] = (word >> k & 1u) != 0 ? d[k] : 0.0f;
+                    }
+                }
+                {
                     uint32_t out[16];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        float2 a = delta, b = delta;
-                        if constexpr (!Rows) {
-                            const float4 l = *reinterpret_cast<const float4*>(lse + kWidth + 32 * j + k);
-                            a = make_float2(l.x, l.y);
-                            b = make_float2(l.z, l.w);
-                        }
-                        a = (make_float2(d[0][k], d[0][k + 1]) - a) * make_float2(p[j][k], p[j][k + 1]);
-                        b = (make_float2(d[0][k + 2], d[0][k + 3]) - b) * make_float2(p[j][k + 2], p[j][k + 3]);
-                        if constexpr (!kBf16) {
-                            a = a * pair(ds_scale);
-                            b = b * pair(ds_scale);
-                        }
-                        d[0][k] = a.x;
-                        d[0][k + 1] = a.y;
-                        d[0][k + 2] = b.x;
-                        d[0][k + 3] = b.y;
-                    }
-                    // A key that does not count may have made D anything.
-                    if constexpr (Rows) {
-                        if (!all_count<kWidth / 32>(w)) {
-                            const uint32_t word = half == 0 ? w[j] : w[2 + j];
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                d[0][k] = (word >> k & 1u) != 0 ? d[0][k] : 0.0f;
-                            }
-                        }
-                    } else if (!whole) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            d[0][k] = counts ? d[0][k] : 0.0f;
-                        }
-                    }
-#pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        out[k] = pack2<T>(make_float2(d[0][2 * k], d[0][2 * k + 1]));
+                        out[k] = pack2<T>(make_float2(d[2 * k], d[2 * k + 1]));
                     }
-                    store16(d_at + 16 * j, out);
+                    store16(d_at, out);
+                    store_wait();
                 }
-                store_wait();
+                if constexpr (Rows) {  // of k, which ds meets; v has only been read for scores that were dropped
+                    if (!all_count<kWidth / 32>(w)) {
+                        wipe_rows<kWidth, kWarps>(ring + stage * Cfg::kStageBytes, Boxes, w, warp);
+                    }
+                }
                 umma::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
@@ -568,22 +523,19 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
                 acc_phase ^= 1u;
                 umma::fence_after_sync();
             }
-            // With eight warps the first four store dk (dq: the first half of it), the others dv; four store it all.
-            const int span = (c.dim + 15) / 16;
-            const int cut = kWarps == 8 ? (span + 1) / 2 * 16 : c.dim;
+            // The warps share the stores: rows, each part some of dq; keys, the first half of the parts dk, the others dv.
+            constexpr int kSharers = Rows ? Cfg::kParts : Cfg::kParts / 2;
+            const int span = ((c.dim + 15) / 16 + kSharers - 1) / kSharers * 16;
             const long long part_row = (it.part * c.pairs() + pair_at) * (Rows ? c.rows() : c.keys) + row;
             const long long at = Rows ? ((static_cast<long long>(it.b) * c.queries + token) * c.kv_heads + it.head) * c.group * c.dim + row_head * c.dim
                                       : ((static_cast<long long>(it.b) * c.keys + row) * c.kv_heads + it.head) * c.dim;
-#pragma unroll
-            for (int which = 0; which < (Rows ? 1 : 2); ++which) {
-                const bool of_v = which == 1;
-                if (!Rows && kWarps == 8 && which != half) {
-                    continue;
-                }
+            {
+                const bool of_v = !Rows && part >= kSharers;
+                const int from = part % kSharers * span;
                 const float factor = of_v ? exp2f(-power) : (g.parts > 1 ? 1.0f : c.scale) / ds_scale;
                 float* partial = of_v ? g.partial1 : g.partial0;
                 T* result = static_cast<T*>(Rows ? c.dq : of_v ? c.dv : c.dk);
-                for (int d = Rows && half == 1 ? cut : 0; d < (Rows && half == 0 ? min(cut, c.dim) : c.dim); d += 16) {
+                for (int d = from; d < min(from + span, c.dim); d += 16) {
                     float a[16];
                     if (it.tiles > 0) {
                         umma::load16(tmem + lanes + (of_v ? Cfg::kA1 : Cfg::kA0) + d, a);
@@ -624,7 +576,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows, Wipe>::kThreads, Config<Bo
 
 // --- the rows' constants -----------------------------------------------------------------------------------
 
-// lse (infinite for rows that are not there or have no keys, so that their weights are 0) and delta of every entry of
+// -lse (infinite for rows that are not there or have no keys, so that their weights are 0) and -delta of every entry of
 // every row tile, `lanes` lanes of eight values a row. float16: also the largest squares of g's rows and v's
 // keys that this CTA met (finite ones).
 template <class T, bool Vectors>
@@ -709,8 +661,8 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
                 lse = s.y == 0.0f ? INFINITY : s.x + log2f(s.y);
             }
             float* at = out + tile * 2 * width + local;
-            at[0] = lse;
-            at[width] = delta;
+            at[0] = -lse;
+            at[width] = -delta;
         }
     }
     if constexpr (std::is_same_v<T, f16>) {
@@ -828,11 +780,11 @@ unsigned item_count(long long items)
     return static_cast<unsigned>(items);
 }
 
-template <class T, int Boxes, bool Rows, bool Wipe>
+template <class T, int Boxes, bool Rows>
 void launch(const Backward& g, cudaStream_t stream)
 {
-    using Cfg = Config<Boxes, Rows, Wipe>;
-    const auto kernel = backward_kernel<T, Boxes, Rows, Wipe>;
+    using Cfg = Config<Boxes, Rows>;
+    const auto kernel = backward_kernel<T, Boxes, Rows>;
     static std::atomic<bool> ready[kMaxDevices];
     const int device = current_device();
     if (!ready[device].load(std::memory_order_relaxed)) {
@@ -862,7 +814,7 @@ void both(Backward g, const Plan& plan, const HeadMap (&rows)[2], const HeadMap 
     g.items = item_count(c.pairs() * plan.key_tiles * plan.row_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dk);
     g.partial1 = reinterpret_cast<float*>(work + plan.dv);
-    launch<T, Boxes, false, false>(g, stream);
+    launch<T, Boxes, false>(g, stream);
     // dq.
     g.x0 = rows[0];
     g.x1 = rows[1];
@@ -873,11 +825,7 @@ void both(Backward g, const Plan& plan, const HeadMap (&rows)[2], const HeadMap 
     g.part_tiles = plan.key_span;
     g.items = item_count(c.pairs() * plan.row_tiles * plan.key_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dq);
-    if (c.lengths != nullptr || c.mask != nullptr) {
-        launch<T, Boxes, true, true>(g, stream);
-    } else {
-        launch<T, Boxes, true, false>(g, stream);
-    }
+    launch<T, Boxes, true>(g, stream);
 }
 
 }  // namespace
