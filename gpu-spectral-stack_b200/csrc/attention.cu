@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 namespace spectral::attention {
 namespace {
@@ -23,33 +24,69 @@ template <int Dim>
 constexpr int kPitch = Dim + 4;
 constexpr int kScorePitch = kKeys + 4;
 
-// Rows [first, first + Rows) of queries (or of an array of their shape), zeros past the end.
-template <int Dim, int Rows>
-__device__ __forceinline__ void load_rows(float* tile, const Call& c, const void* base, const Strides& s, int b, int head,
-                                          long long first)
+// A row of `dim` values into a tile's row, `Lanes` lanes side by side, zeros behind it; zeros throughout without a source.
+// `vectors`: source rows are 16-byte aligned and dim is a multiple of 4.
+template <int Dim, bool Vectors>
+__device__ __forceinline__ void load_row(float* to, const float* from, int dim, int at)
 {
-    const float* p = static_cast<const float*>(base) + b * s.sample;
-    for (int i = threadIdx.x; i < Rows * Dim; i += kThreads) {
-        const int row = i / Dim, d = i - row * Dim;
-        const long long r = first + row;
-        float v = 0.0f;
-        if (r < c.rows() && d < c.dim) {
-            const long long t = r / c.group;
-            v = p[t * s.token + (head * c.group + (r - t * c.group)) * s.head + d];
-        }
-        tile[row * kPitch<Dim> + d] = v;
+    if constexpr (Vectors) {
+        const int d = 4 * at;
+        const float4 v = from != nullptr && d < dim ? *reinterpret_cast<const float4*>(from + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        *reinterpret_cast<float4*>(to + d) = v;
+    } else {
+        to[at] = from != nullptr && at < dim ? from[at] : 0.0f;
+    }
+}
+
+// Rows [first, first + Rows) of queries (or of an array of their shape), zeros past the end.
+template <int Dim, int Rows, bool Vectors>
+__device__ __forceinline__ void fill_rows(float* tile, const Call& c, const float* base, const Strides& s, long long first)
+{
+    constexpr int kLanes = Vectors ? Dim / 4 : Dim;  // per row
+    constexpr int kAtOnce = kThreads / kLanes;
+    const int at = threadIdx.x % kLanes;
+#pragma unroll 8
+    for (int row = threadIdx.x / kLanes; row < Rows; row += kAtOnce) {
+        const unsigned r = static_cast<unsigned>(first) + row;  // rows stay below 2^31
+        const unsigned t = r / static_cast<unsigned>(c.group);
+        const float* from = base + t * s.token + static_cast<int>(r - t * c.group) * s.head;
+        load_row<Dim, Vectors>(tile + row * kPitch<Dim>, r < c.rows() ? from : nullptr, c.dim, at);
+    }
+}
+
+template <int Dim, int Rows>
+__device__ __forceinline__ void load_rows(float* tile, const Call& c, const void* p, const Strides& s, bool vectors, int b, int head, long long first)
+{
+    const float* base = static_cast<const float*>(p) + b * s.sample + head * c.group * s.head;
+    if (vectors) {
+        fill_rows<Dim, Rows, true>(tile, c, base, s, first);
+    } else {
+        fill_rows<Dim, Rows, false>(tile, c, base, s, first);
     }
 }
 
 // Keys [first, first + kKeys) of k or v, zeros where `valid` is not set.
-template <int Dim>
-__device__ __forceinline__ void load_keys(float* tile, const Call& c, const void* base, const Strides& s, int b, int head,
-                                          long long first, unsigned long long valid)
+template <int Dim, bool Vectors>
+__device__ __forceinline__ void fill_keys(float* tile, const Call& c, const float* base, const Strides& s, unsigned long long valid)
 {
-    const float* p = static_cast<const float*>(base) + b * s.sample + head * s.head;
-    for (int i = threadIdx.x; i < kKeys * Dim; i += kThreads) {
-        const int key = i / Dim, d = i - key * Dim;
-        tile[key * kPitch<Dim> + d] = (valid >> key & 1) != 0 && d < c.dim ? p[(first + key) * s.token + d] : 0.0f;
+    constexpr int kLanes = Vectors ? Dim / 4 : Dim;
+    constexpr int kAtOnce = kThreads / kLanes;
+    const int at = threadIdx.x % kLanes;
+#pragma unroll 8
+    for (int key = threadIdx.x / kLanes; key < kKeys; key += kAtOnce) {
+        load_row<Dim, Vectors>(tile + key * kPitch<Dim>, (valid >> key & 1) != 0 ? base + key * s.token : nullptr, c.dim, at);
+    }
+}
+
+template <int Dim>
+__device__ __forceinline__ void load_keys(float* tile, const Call& c, const void* p, const Strides& s, bool vectors, int b, int head, long long first,
+                                          unsigned long long valid)
+{
+    const float* base = static_cast<const float*>(p) + b * s.sample + head * s.head + first * s.token;
+    if (vectors) {
+        fill_keys<Dim, true>(tile, c, base, s, valid);
+    } else {
+        fill_keys<Dim, false>(tile, c, base, s, valid);
     }
 }
 
@@ -72,9 +109,9 @@ __device__ __forceinline__ unsigned long long valid_keys(const Call& c, int b, i
     return votes[0] | static_cast<unsigned long long>(votes[1]) << 32;
 }
 
-// R x 4 dot products over Dim: rows row0 .. of a, rows col + 16 j of b.
+// R x 4 dot products over dim: rows row0 .. of a, rows col + 16 j of b.
 template <int Dim, int R>
-__device__ __forceinline__ void products(const float* a, const float* b, int row0, int col, float (&out)[R][4])
+__device__ __forceinline__ void products(const float* a, const float* b, int dim, int row0, int col, float (&out)[R][4])
 {
     float2 acc[R][4];
 #pragma unroll
@@ -84,8 +121,8 @@ __device__ __forceinline__ void products(const float* a, const float* b, int row
             acc[i][j] = pair(0.0f);
         }
     }
-#pragma unroll 4
-    for (int d = 0; d < Dim; d += 4) {
+#pragma unroll 2
+    for (int d = 0; d < dim; d += 4) {  // what lies between dim and the next 4 is zero
         float4 x[R], y[4];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -147,20 +184,25 @@ __device__ __forceinline__ void weigh_rows(const float* s, const float* m, int r
     }
 }
 
-// acc[i] += sum over rows of s[row][key0 + i] * m[row][its values], four keys.
+// acc[i] += sum over rows of s[row][key0 + i] * m[row][its values], eight keys.
 template <int Dim, int Rows>
-__device__ __forceinline__ void weigh_keys(const float* s, const float* m, int key0, int col, float2 (&acc)[4][kPairs<Dim>])
+__device__ __forceinline__ void weigh_keys(const float* s, const float* m, int key0, int col, float2 (&acc)[8][kPairs<Dim>])
 {
 #pragma unroll 4
     for (int row = 0; row < Rows; ++row) {
-        const float4 w = *reinterpret_cast<const float4*>(s + row * kScorePitch + key0);
+        const float4 a = *reinterpret_cast<const float4*>(s + row * kScorePitch + key0);
+        const float4 b = *reinterpret_cast<const float4*>(s + row * kScorePitch + key0 + 4);
 #pragma unroll
         for (int p = 0; p < kPairs<Dim>; ++p) {
             const float2 v = *reinterpret_cast<const float2*>(m + row * kPitch<Dim> + p * 32 + 2 * col);
-            acc[0][p] = fma2(pair(w.x), v, acc[0][p]);
-            acc[1][p] = fma2(pair(w.y), v, acc[1][p]);
-            acc[2][p] = fma2(pair(w.z), v, acc[2][p]);
-            acc[3][p] = fma2(pair(w.w), v, acc[3][p]);
+            acc[0][p] = fma2(pair(a.x), v, acc[0][p]);
+            acc[1][p] = fma2(pair(a.y), v, acc[1][p]);
+            acc[2][p] = fma2(pair(a.z), v, acc[2][p]);
+            acc[3][p] = fma2(pair(a.w), v, acc[3][p]);
+            acc[4][p] = fma2(pair(b.x), v, acc[4][p]);
+            acc[5][p] = fma2(pair(b.y), v, acc[5][p]);
+            acc[6][p] = fma2(pair(b.z), v, acc[6][p]);
+            acc[7][p] = fma2(pair(b.w), v, acc[7][p]);
         }
     }
 }
@@ -199,6 +241,7 @@ __device__ __forceinline__ float lanes16_sum(float v)
 
 // Where a kernel's results go: the call's arrays, or float32 parts of them.
 struct Parts {
+    bool vectors = false;     // every array's rows are 16-byte aligned
     int count = 1;
     long long span = 0;       // keys (forward, dq) or rows (dk, dv) of a part
     float* first = nullptr;   // sum p v, dq or dk: (part, pair, row, dim)
@@ -208,7 +251,7 @@ struct Parts {
 
 // Forward: 16 R rows per CTA, thread (row group, column) of a 16 x 16 grid.
 template <int Dim, int R>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const Parts parts)
+__global__ void __launch_bounds__(kThreads, R == 8 || Dim == 128 ? 1 : 2) forward_kernel(const Call c, const Parts parts)
 {
     constexpr int kRows = 16 * R;
     extern __shared__ __align__(16) float shared[];
@@ -228,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const P
     const int length = length_of(c, b);
     const long long begin = part * parts.span;
     const long long end = min(static_cast<long long>(length), begin + parts.span);
-    load_rows<Dim, kRows>(sq, c, c.q, c.qs, b, head, first);
+    load_rows<Dim, kRows>(sq, c, c.q, c.qs, parts.vectors, b, head, first);
     const float scale = c.scale * kLog2e;
     float most[R], total[R];
     float2 acc[R][kPairs<Dim>];
@@ -246,11 +289,11 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const P
         if (valid == 0) {
             continue;
         }
-        load_keys<Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
-        load_keys<Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+        load_keys<Dim>(sk, c, c.k, c.ks, parts.vectors, b, head, key0, valid);
+        load_keys<Dim>(sv, c, c.v, c.vs, parts.vectors, b, head, key0, valid);
         __syncthreads();
         float s[R][4];
-        products<Dim, R>(sq, sk, row0, col, s);
+        products<Dim, R>(sq, sk, c.dim, row0, col, s);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float m = -INFINITY;
@@ -302,15 +345,15 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Call c, const P
 }
 
 // Scores of a tile, turned into p and p (dp - delta): what both backward kernels need.
-template <int Dim>
-__device__ __forceinline__ void score_gradients(const float* sq, const float* sk, const float* sv, const float* sdo, int row0, int col,
-                                                float scale, unsigned long long valid, const float2 (&stats)[4], const float (&delta)[4],
-                                                float (&p)[4][4], float (&ds)[4][4])
+template <int Dim, int R>
+__device__ __forceinline__ void score_gradients(const float* sq, const float* sk, const float* sv, const float* sdo, int dim, int row0, int col,
+                                                float scale, unsigned long long valid, const float2 (&stats)[R], const float (&delta)[R],
+                                                float (&p)[R][4], float (&ds)[R][4])
 {
-    products<Dim, 4>(sq, sk, row0, col, p);
-    products<Dim, 4>(sdo, sv, row0, col, ds);
+    products<Dim, R>(sq, sk, dim, row0, col, p);
+    products<Dim, R>(sdo, sv, dim, row0, col, ds);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const bool ok = (valid >> (col + 16 * j) & 1) != 0;
@@ -321,10 +364,11 @@ __device__ __forceinline__ void score_gradients(const float* sq, const float* sk
 }
 
 // m and 1 / sum p, and delta, of rows row0 .. of the tile at `first`; zeros past the end and for empty rows.
-__device__ __forceinline__ void row_constants(const Call& c, long long at, long long first, int row0, float2 (&stats)[4], float (&delta)[4])
+template <int R>
+__device__ __forceinline__ void row_constants(const Call& c, long long at, long long first, int row0, float2 (&stats)[R], float (&delta)[R])
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
         const long long r = first + row0 + i;
         stats[i] = make_float2(0.0f, 0.0f);
         delta[i] = 0.0f;
@@ -337,7 +381,7 @@ __device__ __forceinline__ void row_constants(const Call& c, long long at, long 
 }
 
 template <int Dim>
-__global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, const Parts parts)
+__global__ void __launch_bounds__(kThreads, Dim == 128 ? 1 : 2) keys_backward_kernel(const Call c, const Parts parts)
 {
     extern __shared__ __align__(16) float shared[];
     float* sk = shared;
@@ -356,29 +400,31 @@ __global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, c
     allow_next_grid();
     wait_for_previous_grid();
     const unsigned long long valid = valid_keys(c, b, length_of(c, b), key0, votes);
-    load_keys<Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
-    load_keys<Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+    load_keys<Dim>(sk, c, c.k, c.ks, parts.vectors, b, head, key0, valid);
+    load_keys<Dim>(sv, c, c.v, c.vs, parts.vectors, b, head, key0, valid);
     const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
                         c.dim};
-    float2 dk[4][kPairs<Dim>], dv[4][kPairs<Dim>];
+    // Half of the threads sum dv, the others dk: eight keys each.
+    const bool of_v = threadIdx.x < kThreads / 2;
+    const int keys0 = (threadIdx.x % (kThreads / 2) >> 4) * 8;
+    float2 acc[8][kPairs<Dim>];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
 #pragma unroll
         for (int p = 0; p < kPairs<Dim>; ++p) {
-            dk[i][p] = pair(0.0f);
-            dv[i][p] = pair(0.0f);
+            acc[i][p] = pair(0.0f);
         }
     }
     const long long end = min(c.rows(), (part + 1) * parts.span);
     for (long long first = part * parts.span; first < end && valid != 0; first += 64) {
         __syncthreads();
-        load_rows<Dim, 64>(sq, c, c.q, c.qs, b, head, first);
-        load_rows<Dim, 64>(sdo, c, c.dout, dense, b, head, first);
+        load_rows<Dim, 64>(sq, c, c.q, c.qs, parts.vectors, b, head, first);
+        load_rows<Dim, 64>(sdo, c, c.dout, dense, parts.vectors, b, head, first);
         float2 stats[4];
         float delta[4], p[4][4], ds[4][4];
         row_constants(c, at, first, row0, stats, delta);
         __syncthreads();
-        score_gradients<Dim>(sq, sk, sv, sdo, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
+        score_gradients<Dim, 4>(sq, sk, sv, sdo, c.dim, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -388,55 +434,54 @@ __global__ void __launch_bounds__(kThreads) keys_backward_kernel(const Call c, c
             }
         }
         __syncthreads();
-        weigh_keys<Dim, 64>(sp, sdo, row0, col, dv);
-        weigh_keys<Dim, 64>(sds, sq, row0, col, dk);
+        weigh_keys<Dim, 64>(of_v ? sp : sds, of_v ? sdo : sq, keys0, col, acc);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long key = key0 + row0 + i;
+    for (int i = 0; i < 8; ++i) {
+        const long long key = key0 + keys0 + i;
         if (key >= c.keys) {
             continue;
         }
         if (parts.count == 1) {
             const long long to = ((static_cast<long long>(b) * c.keys + key) * c.kv_heads + head) * c.dim;
-            store_pairs<Dim>(static_cast<float*>(c.dk) + to, c.dim, col, dk[i], c.scale);
-            store_pairs<Dim>(static_cast<float*>(c.dv) + to, c.dim, col, dv[i], 1.0f);
+            store_pairs<Dim>(static_cast<float*>(of_v ? c.dv : c.dk) + to, c.dim, col, acc[i], of_v ? 1.0f : c.scale);
         } else {
             const long long to = ((part * c.pairs() + at) * c.keys + key) * c.dim;
-            store_pairs<Dim>(parts.first + to, c.dim, col, dk[i], 1.0f);
-            store_pairs<Dim>(parts.second + to, c.dim, col, dv[i], 1.0f);
+            store_pairs<Dim>((of_v ? parts.second : parts.first) + to, c.dim, col, acc[i], 1.0f);
         }
     }
 }
 
-template <int Dim>
-__global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, const Parts parts)
+// 16 R rows per CTA.
+template <int Dim, int R>
+__global__ void __launch_bounds__(kThreads, R == 8 || Dim == 128 ? 1 : 2) rows_backward_kernel(const Call c, const Parts parts)
 {
+    constexpr int kRows = 16 * R;
     extern __shared__ __align__(16) float shared[];
     float* sk = shared;
     float* sv = sk + kKeys * kPitch<Dim>;
     float* sq = sv + kKeys * kPitch<Dim>;
-    float* sdo = sq + 64 * kPitch<Dim>;
-    float* sds = sdo + 64 * kPitch<Dim>;
+    float* sdo = sq + kRows * kPitch<Dim>;
+    float* sds = sdo + kRows * kPitch<Dim>;
     __shared__ unsigned votes[2];
     const int col = threadIdx.x & 15;
-    const int row0 = (threadIdx.x >> 4) * 4;
+    const int row0 = (threadIdx.x >> 4) * R;
     const long long at = blockIdx.y;
     const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
-    const long long first = static_cast<long long>(blockIdx.x) * 64;
+    const long long first = static_cast<long long>(blockIdx.x) * kRows;
     const int part = blockIdx.z;
     allow_next_grid();
     wait_for_previous_grid();
     const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
                         c.dim};
-    load_rows<Dim, 64>(sq, c, c.q, c.qs, b, head, first);
-    load_rows<Dim, 64>(sdo, c, c.dout, dense, b, head, first);
-    float2 stats[4];
-    float delta[4];
+    load_rows<Dim, kRows>(sq, c, c.q, c.qs, parts.vectors, b, head, first);
+    load_rows<Dim, kRows>(sdo, c, c.dout, dense, parts.vectors, b, head, first);
+    float2 stats[R];
+    float delta[R];
     row_constants(c, at, first, row0, stats, delta);
-    float2 dq[4][kPairs<Dim>];
+    float2 dq[R][kPairs<Dim>];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
 #pragma unroll
         for (int p = 0; p < kPairs<Dim>; ++p) {
             dq[i][p] = pair(0.0f);
@@ -449,23 +494,23 @@ __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const Call c, c
         if (valid == 0) {
             continue;
         }
-        load_keys<Dim>(sk, c, c.k, c.ks, b, head, key0, valid);
-        load_keys<Dim>(sv, c, c.v, c.vs, b, head, key0, valid);
+        load_keys<Dim>(sk, c, c.k, c.ks, parts.vectors, b, head, key0, valid);
+        load_keys<Dim>(sv, c, c.v, c.vs, parts.vectors, b, head, key0, valid);
         __syncthreads();
-        float p[4][4], ds[4][4];
-        score_gradients<Dim>(sq, sk, sv, sdo, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
+        float p[R][4], ds[R][4];
+        score_gradients<Dim, R>(sq, sk, sv, sdo, c.dim, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < R; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 sds[(row0 + i) * kScorePitch + col + 16 * j] = ds[i][j];
             }
         }
         __syncwarp();
-        weigh_rows<Dim, 4>(sds, sk, row0, col, dq);
+        weigh_rows<Dim, R>(sds, sk, row0, col, dq);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
         const long long r = first + row0 + i;
         if (r >= c.rows()) {
             continue;
@@ -643,8 +688,16 @@ void with_dim(int dim, F&& f)
     }
 }
 
-// Rows per forward CTA: 64, or 16 where there are no more (a single query's rows).
-int forward_rows(const Call& c) { return c.rows() <= 16 ? 16 : 64; }
+// Rows per CTA: 128, where that leaves fewer tiles than SMs 64, and where there are no more (a single query's) 16.
+// Eight rows a thread read less shared memory per product than four.
+int tile_rows(const Call& c, bool back)
+{
+    if (c.rows() <= 16 && !back) {
+        return 16;
+    }
+    const bool fits = !back || c.dim <= 64;
+    return fits && c.pairs() * pieces(c.rows(), 128) * pieces(c.keys, 512) >= kSms ? 128 : 64;
+}
 
 // Parts of an axis of `length` in tiles of 64, so that `tiles` CTAs per part fill the GPU about twice; a part's
 // span is a whole number of tiles.
@@ -665,7 +718,7 @@ struct ForwardPlan {
 
     explicit ForwardPlan(const Call& c)
     {
-        parts = split(c.pairs() * pieces(c.rows(), forward_rows(c)), c.keys);
+        parts = split(c.pairs() * pieces(c.rows(), tile_rows(c, false)), c.keys);
         if (parts.count > 1) {
             const std::size_t rows = static_cast<std::size_t>(c.pairs()) * c.rows() * parts.count;
             partial = arena.take(rows * c.dim * sizeof(float));
@@ -686,7 +739,7 @@ struct BackwardPlan {
         const std::size_t rows = static_cast<std::size_t>(c.pairs()) * c.rows();
         const std::size_t keys = static_cast<std::size_t>(c.pairs()) * c.keys;
         delta = arena.take(rows * sizeof(float));
-        of_keys = split(c.pairs() * pieces(c.rows(), 64), c.keys);
+        of_keys = split(c.pairs() * pieces(c.rows(), tile_rows(c, true)), c.keys);
         of_rows = split(c.pairs() * pieces(c.keys, 64), c.rows());
         if (of_keys.count > 1) {
             dq = arena.take(rows * c.dim * of_keys.count * sizeof(float));
@@ -698,12 +751,24 @@ struct BackwardPlan {
     }
 };
 
+bool in_vectors(const Call& c, std::initializer_list<const void*> arrays, std::initializer_list<const Strides*> strides)
+{
+    bool ok = c.dim % 4 == 0;
+    for (const void* p : arrays) {
+        ok = ok && aligned_to(p, 16);
+    }
+    for (const Strides* s : strides) {
+        ok = ok && s->sample % 4 == 0 && s->token % 4 == 0 && s->head % 4 == 0;
+    }
+    return ok;
+}
+
 template <class K, class... A>
 void launch(K kernel, dim3 grid, std::size_t smem, cudaStream_t stream, const A&... args)
 {
-    if (smem > 48 * 1024) {
-        SPECTRAL_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    }
+    const auto* f = reinterpret_cast<const void*>(kernel);
+    SPECTRAL_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    SPECTRAL_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     launch_pdl(kernel, grid, dim3(kThreads), smem, stream, args...);
 }
 
@@ -712,13 +777,16 @@ void forward(const Call& c, char* work, cudaStream_t stream)
     ForwardPlan plan(c);
     plan.parts.first = reinterpret_cast<float*>(work + plan.partial);
     plan.parts.stats = reinterpret_cast<float2*>(work + plan.stats);
-    const int rows = forward_rows(c);
+    plan.parts.vectors = in_vectors(c, {c.q, c.k, c.v}, {&c.qs, &c.ks, &c.vs});
+    const int rows = tile_rows(c, false);
     const dim3 grid(pieces(c.rows(), rows), static_cast<unsigned>(c.pairs()), plan.parts.count);
     with_dim(c.dim, [&](auto d) {
         constexpr int Dim = decltype(d)::value;
         const std::size_t smem = ((rows + 2 * kKeys) * kPitch<Dim> + rows * kScorePitch) * sizeof(float);
         if (rows == 16) {
             launch(forward_kernel<Dim, 1>, grid, smem, stream, c, plan.parts);
+        } else if (rows == 128) {
+            launch(forward_kernel<Dim, 8>, grid, smem, stream, c, plan.parts);
         } else {
             launch(forward_kernel<Dim, 4>, grid, smem, stream, c, plan.parts);
         }
@@ -735,6 +803,7 @@ void backward(Call c, char* work, cudaStream_t stream)
     plan.of_keys.first = reinterpret_cast<float*>(work + plan.dq);
     plan.of_rows.first = reinterpret_cast<float*>(work + plan.dk);
     plan.of_rows.second = reinterpret_cast<float*>(work + plan.dv);
+    plan.of_keys.vectors = plan.of_rows.vectors = in_vectors(c, {c.q, c.k, c.v, c.dout}, {&c.qs, &c.ks, &c.vs});
     row_products(c, stream);
     with_dim(c.dim, [&](auto d) {
         constexpr int Dim = decltype(d)::value;
@@ -742,8 +811,16 @@ void backward(Call c, char* work, cudaStream_t stream)
         constexpr std::size_t kScores = 64 * kScorePitch * sizeof(float);
         launch(keys_backward_kernel<Dim>, dim3(pieces(c.keys, 64), static_cast<unsigned>(c.pairs()), plan.of_rows.count), tiles + 2 * kScores, stream,
                c, plan.of_rows);
-        launch(rows_backward_kernel<Dim>, dim3(pieces(c.rows(), 64), static_cast<unsigned>(c.pairs()), plan.of_keys.count), tiles + kScores, stream, c,
-               plan.of_keys);
+        const int rows = tile_rows(c, true);
+        const dim3 grid(pieces(c.rows(), rows), static_cast<unsigned>(c.pairs()), plan.of_keys.count);
+        const std::size_t smem = (2 * (kKeys + rows) * kPitch<Dim> + rows * kScorePitch) * sizeof(float);
+        if constexpr (Dim <= 64) {
+            if (rows == 128) {
+                launch(rows_backward_kernel<Dim, 8>, grid, smem, stream, c, plan.of_keys);
+                return;
+            }
+        }
+        launch(rows_backward_kernel<Dim, 4>, grid, smem, stream, c, plan.of_keys);
     });
     if (plan.of_rows.count > 1) {
         add_parts(c, plan.of_rows.first, plan.of_rows.count, true, c.dk, c.scale, stream);
