@@ -727,7 +727,13 @@ struct ForwardPlan {
     }
 };
 
-std::size_t forward_workspace(const Call& c) { return c.dtype == SPECTRAL_FLOAT32 ? ForwardPlan(c).arena.size() : tensor_forward_workspace(c); }
+// Float32 calls whose products are worth splitting: heads of up to 64 values and more rows than a few.
+bool on_tensor_cores(const Call& c) { return c.dim <= 64 && c.group <= 64 && c.rows() > 16 && c.keys > 0; }
+
+std::size_t forward_workspace(const Call& c)
+{
+    return c.dtype != SPECTRAL_FLOAT32 ? tensor_forward_workspace(c) : on_tensor_cores(c) ? split_forward_workspace(c) : ForwardPlan(c).arena.size();
+}
 
 struct BackwardPlan {
     Parts of_rows, of_keys;
@@ -960,7 +966,9 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
         if (work == nullptr && forward_workspace(c) > 0) {
             return invalid("cross_attention: needs a workspace");
         }
-        if (dtype == SPECTRAL_FLOAT32) {
+        if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c)) {
+            split_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+        } else if (dtype == SPECTRAL_FLOAT32) {
             forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
         } else {
             tensor_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
@@ -991,7 +999,7 @@ extern "C" int spectral_cross_attention_backward_workspace(const void* dout, con
     c.v = v;
     *count = 0;
     if (c.pairs() * c.rows() > 0 && keys > 0) {
-        *count = (dtype == SPECTRAL_FLOAT32 ? BackwardPlan(c).arena.size() : tensor_backward_workspace(c)) / 8;
+        *count = (dtype != SPECTRAL_FLOAT32 ? tensor_backward_workspace(c) : on_tensor_cores(c) ? split_backward_workspace(c) : BackwardPlan(c).arena.size()) / 8;
     }
     return SPECTRAL_OK;
 }
@@ -1058,7 +1066,9 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         c.dk = dk;
         c.dv = dv;
         c.scale = scale;
-        if (dtype == SPECTRAL_FLOAT32) {
+        if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c)) {
+            split_backward(c, static_cast<char*>(work), s);
+        } else if (dtype == SPECTRAL_FLOAT32) {
             backward(c, static_cast<char*>(work), s);
         } else {
             tensor_backward(c, static_cast<char*>(work), s);

@@ -107,6 +107,16 @@ void tensor_forward(const Call& c, char* work, cudaStream_t stream);
 std::size_t tensor_backward_workspace(const Call& c);
 void tensor_backward(const Call& c, char* work, cudaStream_t stream);
 
+// The float32 kernels on the tensor cores (attention_tc32.cu): heads of at most 64 values, at most 64 query heads to a key
+// head.
+std::size_t split_forward_workspace(const Call& c);
+void split_forward(const Call& c, char* work, cudaStream_t stream);
+std::size_t split_backward_workspace(const Call& c);
+void split_backward(const Call& c, char* work, cudaStream_t stream);
+
+// (pair, tile of `tokens` tokens): -lse of the tile's rows in `width` places, then -delta (attention_tc_backward.cu).
+void row_constants(const Call& c, float* out, int width, int tokens, int tiles, cudaStream_t stream);
+
 inline int pieces(long long n, long long per) { return static_cast<int>((n + per - 1) / per); }
 
 // A part of a workspace, in bytes; every array starts on 256.

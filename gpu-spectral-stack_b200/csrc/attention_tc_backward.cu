@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
             const long long at = c.row_at(b, static_cast<int>(pair_at - static_cast<long long>(b) * c.kv_heads), r);
             Floats<8> x = fetch(o + at);
             const Floats<8> y = fetch(g + at);
-            if (c.rest != nullptr && sub * 8 < c.dim) {
+            if (sizeof(T) == 2 && c.rest != nullptr && sub * 8 < c.dim) {
                 Vec<signed char, 8> code{};
                 if constexpr (Vectors) {
                     code = *reinterpret_cast<const Vec<signed char, 8>*>(c.rest + at + sub * 8);
@@ -828,7 +828,31 @@ void both(Backward g, const Plan& plan, const HeadMap (&rows)[2], const HeadMap 
     launch<T, Boxes, true>(g, stream);
 }
 
+// `norms` (float16): 2 x the returned count of floats.
+int launch_constants(const Call& c, float* constants, float* norms, int width, int rows_per_tile, int row_tiles, cudaStream_t stream)
+{
+    int lanes = 1;
+    while (lanes * 8 < c.dim) {
+        lanes *= 2;
+    }
+    const long long entries = std::max(c.pairs() * row_tiles * width, c.dtype == SPECTRAL_FLOAT16 ? c.pairs() * c.keys : 0LL);
+    const auto grid = static_cast<unsigned>(std::min<long long>((entries * lanes + 255) / 256, kNormCtas));
+    const std::size_t piece = 8 * dtype_size(c.dtype);
+    const bool vectors = c.dim % 8 == 0 && aligned_to(c.out, piece) && aligned_to(c.dout, piece) && aligned_to(c.rest, 8);
+    with_dtype(c.dtype, [&](auto t) {
+        using T = decltype(t);
+        launch_pdl(vectors ? constants_kernel<T, true> : constants_kernel<T, false>, dim3(grid), dim3(256), 0, stream, c, constants, norms, width,
+                   rows_per_tile, row_tiles, lanes);
+    });
+    return static_cast<int>(grid);
+}
+
 }  // namespace
+
+void row_constants(const Call& c, float* out, int width, int tokens, int tiles, cudaStream_t stream)
+{
+    launch_constants(c, out, nullptr, width, tokens * c.group, tiles, stream);
+}
 
 std::size_t tensor_backward_workspace(const Call& c) { return Plan(c).arena.size(); }
 
@@ -850,14 +874,7 @@ void tensor_backward(const Call& c, char* work, cudaStream_t stream)
     g.constants = constants;
     g.norms = norms;
     g.fault = device_fault_word();
-    int lanes = 1;
-    while (lanes * 8 < c.dim) {
-        lanes *= 2;
-    }
-    const long long entries = std::max(c.pairs() * plan.row_walks * plan.width, is_bf16 ? 0LL : c.pairs() * c.keys);
-    const auto grid = static_cast<unsigned>(std::min<long long>((entries * lanes + 255) / 256, kNormCtas));
-    g.norm_count = static_cast<int>(grid);
-    const bool vectors = c.dim % 8 == 0 && aligned_to(c.out, 16) && aligned_to(c.dout, 16) && aligned_to(c.rest, 8);
+    g.norm_count = launch_constants(c, constants, norms, plan.width, plan.walked_tokens * c.group, plan.row_walks, stream);
     const int heads = c.kv_heads * c.group;
     const auto rows_map = [&](const Operand& o, int tokens) {
         return head_map(o.base(work), is_bf16, o.strides(c.dim), c.batch, c.queries, heads, c.dim, c.group, tokens);
@@ -871,13 +888,6 @@ void tensor_backward(const Call& c, char* work, cudaStream_t stream)
     const HeadMap key_walk[2] = {keys_map(plan.k, plan.width), keys_map(plan.v, plan.width)};
     const auto run = [&](auto t) {
         using T = decltype(t);
-        if (vectors) {
-            launch_pdl(constants_kernel<T, true>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.width, plan.walked_tokens * c.group,
-                       plan.row_walks, lanes);
-        } else {
-            launch_pdl(constants_kernel<T, false>, dim3(grid), dim3(256), 0, stream, c, constants, norms, plan.width, plan.walked_tokens * c.group,
-                       plan.row_walks, lanes);
-        }
         if (plan.boxes == 1) {
             both<T, 1>(g, plan, rows, row_walk, keys, key_walk, work, stream);
         } else {
