@@ -732,7 +732,8 @@ bool on_tensor_cores(const Call& c) { return c.dim <= 64 && c.group <= 64 && c.r
 
 std::size_t forward_workspace(const Call& c)
 {
-    return c.dtype != SPECTRAL_FLOAT32 ? tensor_forward_workspace(c) : on_tensor_cores(c) ? split_forward_workspace(c) : ForwardPlan(c).arena.size();
+    return few_rows(c)                       ? few_workspace(c)
+           : c.dtype != SPECTRAL_FLOAT32 ? tensor_forward_workspace(c) : on_tensor_cores(c) ? split_forward_workspace(c) : ForwardPlan(c).arena.size();
 }
 
 struct BackwardPlan {
@@ -966,7 +967,9 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
         if (work == nullptr && forward_workspace(c) > 0) {
             return invalid("cross_attention: needs a workspace");
         }
-        if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c)) {
+        if (few_rows(c)) {
+            few_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+        } else if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c)) {
             split_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
         } else if (dtype == SPECTRAL_FLOAT32) {
             forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));

@@ -114,6 +114,11 @@ void split_forward(const Call& c, char* work, cudaStream_t stream);
 std::size_t split_backward_workspace(const Call& c);
 void split_backward(const Call& c, char* work, cudaStream_t stream);
 
+// Forward passes of at most eight rows per key head (attention_few.cu).
+bool few_rows(const Call& c);
+std::size_t few_workspace(const Call& c);
+void few_forward(const Call& c, char* work, cudaStream_t stream);
+
 // (pair, tile of `tokens` tokens): -lse of the tile's rows in `width` places, then -delta (attention_tc_backward.cu).
 void row_constants(const Call& c, float* out, int width, int tokens, int tiles, cudaStream_t stream);
 
