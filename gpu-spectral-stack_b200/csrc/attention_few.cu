@@ -2,11 +2,12 @@
 //
 // The keys and values are all there is to read, once, and two multiply-adds per value and row all there is to compute: memory
 // bounds it, and the CUDA cores keep up. (On the tensor cores such a tile leaves 120 of 128 rows empty, and its
-// softmax runs in one warp: 16 samples x 4 x 16384 keys x 64, half of them cut off, 111 us; here see the table.) A key
+// softmax runs in one warp: 16 samples x 4 x 16384 keys x 64 bf16, a quarter of them cut off, took 111 us; here
+// 70 us.) A key
 // head's keys are cut into ranges, one per CTA, and a range among its warps. `lanes` lanes hold a key, 16 bytes each
 // where rows allow; each such group of lanes walks over keys of its own with the running maximum, sum and result of
-// every row, four keys at a time: their loads first, then four scores by shuffles, one rescaling, four weighted
-// values. Groups, warps and ranges are joined at the end, in a fixed order.
+// every row, four keys at a time: four scores by shuffles, one rescaling, four weighted values, with the next two
+// fours copied to shared memory meanwhile. Groups, warps and ranges are joined at the end, in a fixed order.
 
 #include "attention.cuh"
 
@@ -18,6 +19,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
+constexpr int kBatch = 4;   // keys of a group at a time
+constexpr int kStages = 3;  // batches on their way or being worked on
+
+// Shared memory of a batch of a warp: every lane's pieces of K and V.
+template <class T, int V, int U>
+constexpr int kStageBytes = 2 * kBatch * U * 32 * V * static_cast<int>(sizeof(T));
 
 struct Few {
     Call c;
@@ -31,9 +38,9 @@ struct Few {
 template <class T, int V, int U, int R>
 __global__ void __launch_bounds__(kThreads, R >= 8 ? 1 : 2) few_kernel(const Few g)
 {
-    constexpr int kBatch = 4;
     using Piece = Vec<T, V>;
     const Call& c = g.c;
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float m_of[kWarps][R], sum_of[kWarps][R];
     __shared__ float acc_of[kWarps][R][SPECTRAL_HEAD_DIM_MAX];
     const int warp = threadIdx.x >> 5;
@@ -77,22 +84,69 @@ __global__ void __launch_bounds__(kThreads, R >= 8 ? 1 : 2) few_kernel(const Few
     const T* keys = static_cast<const T*>(c.k) + b * c.ks.sample + head * c.ks.head;
     const T* values = static_cast<const T*>(c.v) + b * c.vs.sample + head * c.vs.head;
     const unsigned char* mask = c.mask == nullptr ? nullptr : c.mask + static_cast<long long>(b) * c.keys;
-    for (long long key0 = begin + warp * groups * kBatch; key0 < end; key0 += kWarps * groups * kBatch) {
-        Piece k_piece[kBatch][U], v_piece[kBatch][U];
-        bool counts[kBatch];
+    // Each lane copies its own pieces ahead and reads them back: [stage][K, V][key][unit][lane].
+    Piece* const ring = reinterpret_cast<Piece*>(smem) + warp * kStages * (kStageBytes<T, V, U> / static_cast<int>(sizeof(Piece))) + lane;
+    const auto slot = [&](int stage, int which, int i, int k) -> Piece& { return ring[(((stage * 2 + which) * kBatch + i) * U + k) * 32]; };
+    const int step = kWarps * groups * kBatch;
+    const long long first = begin + warp * groups * kBatch + group;
+    const auto counting = [&](long long key0) {  // bit i: key i of the batch counts
+        unsigned bits = 0;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const long long key = key0 + i * groups + group;
-            counts[i] = key < end && (mask == nullptr || mask[key] != 0);
+            const long long key = key0 + i * groups;
+            bits |= (key < end && (mask == nullptr || mask[key] != 0) ? 1u : 0u) << i;
+        }
+        return bits;
+    };
+    const auto ask = [&](int stage, long long key0, unsigned bits) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const T* k_row = keys + (key0 + i * groups) * c.ks.token;
+            const T* v_row = values + (key0 + i * groups) * c.vs.token;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int d = (sub + k * lanes) * V;
-                k_piece[i][k] = Piece{};
-                v_piece[i][k] = Piece{};
-                if (counts[i] && d < c.dim) {
-                    k_piece[i][k] = *reinterpret_cast<const Piece*>(keys + key * c.ks.token + d);
-                    v_piece[i][k] = *reinterpret_cast<const Piece*>(values + key * c.vs.token + d);
+                if ((bits >> i & 1u) != 0 && d < c.dim) {
+                    copy_async<sizeof(Piece)>(&slot(stage, 0, i, k), k_row + d);
+                    copy_async<sizeof(Piece)>(&slot(stage, 1, i, k), v_row + d);
+                } else {  // what does not count may be anything
+                    slot(stage, 0, i, k) = Piece{};
+                    slot(stage, 1, i, k) = Piece{};
                 }
+            }
+        }
+        cp_async_commit();
+    };
+    unsigned bits_of[kStages];
+    long long ahead = first;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        bits_of[i] = counting(ahead);
+        ask(i, ahead, bits_of[i]);
+        ahead += step;
+    }
+    unsigned next = counting(ahead);
+    int stage = 0;
+    for (long long key0 = first - group; key0 < end; key0 += step) {
+        // The batch two ahead, into the place of the one that was left last; its mask was read a turn ago.
+        const unsigned bits = bits_of[0];
+#pragma unroll
+        for (int i = 0; i + 2 < kStages; ++i) {
+            bits_of[i] = bits_of[i + 1];
+        }
+        bits_of[kStages - 2] = next;
+        ask(stage == 0 ? kStages - 1 : stage - 1, ahead, next);
+        ahead += step;
+        next = counting(ahead);
+        cp_async_wait<kStages - 1>();
+        Piece k_piece[kBatch][U];
+        bool counts[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            counts[i] = (bits >> i & 1u) != 0;
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                k_piece[i][k] = slot(stage, 0, i, k);
             }
         }
         float s[R][kBatch];
@@ -157,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, R >= 8 ? 1 : 2) few_kernel(const Few
         for (int i = 0; i < kBatch; ++i) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const Floats<V> f = widen(v_piece[i][k]);
+                const Floats<V> f = widen(slot(stage, 1, i, k));
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -167,7 +221,9 @@ __global__ void __launch_bounds__(kThreads, R >= 8 ? 1 : 2) few_kernel(const Few
                 }
             }
         }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
     }
+    cp_async_wait_all();
     // The groups of a warp.
     for (int o = lanes; o < 32; o *= 2) {
 #pragma unroll
@@ -266,11 +322,12 @@ int piece_of(const Call& c)
     return 1;
 }
 
-// Ranges of a key head's keys: about three CTAs' worth of work per resident CTA, each with a few turns of its warps.
+// Ranges of a key head's keys: one for each resident CTA (twice and four times as many were 3 and 9 % slower on the ragged
+// case above), each with a few turns of its warps.
 int splits_of(const Call& c)
 {
     const long long most = std::max(1LL, (static_cast<long long>(c.keys) + 127) / 128);
-    const long long wanted = (6LL * kSms + c.pairs() - 1) / c.pairs();
+    const long long wanted = (2LL * kSms + c.pairs() - 1) / c.pairs();
     return static_cast<int>(std::min({most, wanted, 256LL}));
 }
 
@@ -279,7 +336,19 @@ void launch(const Few& g, cudaStream_t stream)
 {
     const int rows = static_cast<int>(g.c.rows());
     const dim3 grid(static_cast<unsigned>(g.c.pairs()), g.splits);
-    const auto run = [&](auto r) { launch_pdl(few_kernel<T, V, U, decltype(r)::value>, grid, dim3(kThreads), 0, stream, g); };
+    const auto run = [&](auto r) {
+        constexpr int kSmem = kWarps * kStages * kStageBytes<T, V, U>;
+        const auto kernel = few_kernel<T, V, U, decltype(r)::value>;
+        static std::atomic<bool> ready[kMaxDevices];
+        const int device = current_device();
+        if (!ready[device].load(std::memory_order_relaxed)) {
+            const auto* f = reinterpret_cast<const void*>(kernel);
+            SPECTRAL_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+            SPECTRAL_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+            ready[device].store(true, std::memory_order_relaxed);
+        }
+        launch_pdl(kernel, grid, dim3(kThreads), kSmem, stream, g);
+    };
     if (rows == 1) {
         run(std::integral_constant<int, 1>{});
     } else if (rows == 2) {

@@ -1,9 +1,9 @@
 // Attention forward for 16-bit values on the 5th-generation tensor cores.
 //
-// A CTA keeps two tiles of 128 query rows and walks over tiles of 128 keys. Both products run on tcgen05: the
-// scores S = Q K^T into tensor memory, from where a thread per row takes its 128 scores to registers, and
+// A CTA keeps two or four tiles of 128 query rows and walks over tiles of 128 or 64 keys. Both products run on tcgen05: the
+// scores S = Q K^T into tensor memory, from where a thread per row takes them to registers, and
 // O += P V with the weights P written back over S as the 16-bit operand. While one row tile's threads work on
-// their scores the tensor cores multiply for the other. A warp brings tiles of K and V in by TMA through a ring, a
+// their scores the tensor cores multiply for the others. A warp brings tiles of K and V in by TMA through a ring, a
 // warp issues the products.
 //
 // Softmax in one pass: a row's weights are 2^(c s - m) with m the largest c s when it was last moved, and m moves only
@@ -47,7 +47,7 @@ struct Forward {
     HeadMap q, k, v;
     Call c;
     int tokens_per_tile = 0;  // 128 / group
-    unsigned row_items = 0;   // pairs of row tiles
+    unsigned row_items = 0;   // groups of Config::kSlots row tiles
     unsigned splits = 1;
     int split_tiles = 0;      // key tiles of a split
     unsigned items = 0;
@@ -62,39 +62,49 @@ struct Item {
     int b;
     int head;
     int split;
-    int row_tile;   // the first of the two
+    int row_tile;   // the first
     int tiles;      // of keys
     int key0;
     int end;        // keys before this count, but for the mask
     int slots;      // row tiles with rows
 };
 
+template <int Slots, int Keys>
 __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
 {
     Item it;
     const unsigned r = i / g.row_items;
-    it.row_tile = static_cast<int>(i - r * g.row_items) * 2;
+    it.row_tile = static_cast<int>(i - r * g.row_items) * Slots;
     const unsigned pair = r / g.splits;
     it.split = static_cast<int>(r - pair * g.splits);
     it.b = static_cast<int>(pair / static_cast<unsigned>(g.c.kv_heads));
     it.head = static_cast<int>(pair) - it.b * g.c.kv_heads;
-    it.key0 = it.split * g.split_tiles * kTile;
-    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * kTile);
-    it.tiles = it.end > it.key0 ? (it.end - it.key0 + kTile - 1) / kTile : 0;
-    it.slots = (it.row_tile + 1) * g.tokens_per_tile < g.c.queries ? 2 : 1;
+    it.key0 = it.split * g.split_tiles * Keys;
+    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * Keys);
+    it.tiles = it.end > it.key0 ? (it.end - it.key0 + Keys - 1) / Keys : 0;
+    it.slots = min(Slots, (g.c.queries - it.row_tile * g.tokens_per_tile + g.tokens_per_tile - 1) / g.tokens_per_tile);
     return it;
 }
 
+// Heads of up to 64 values: four row tiles and 64 keys at a time, wider ones two and 128. Either way tensor memory is full; the
+// more warps, the better they fill each other's waits (128 keys and two tiles for all: 64 x 2 x 16384 x 256 x 32 took
+// 400 us, this takes what the design notes' table says).
 template <int Boxes>
 struct Config {
-    static constexpr int kThreads = 320;
-    static constexpr int kTileBytes = Boxes * kBox;
-    static constexpr int kStages = Boxes == 1 ? 8 : 5;  // of K and V tiles
-    static constexpr int kQueries = Boxes == 1 ? 2 : 1;   // items whose queries are kept
-    static constexpr int kSmem = (2 * kQueries + kStages) * kTileBytes + 1024;
-    static constexpr int kO = 256;                       // tensor memory: S and P 0 and 1, then O 0 and 1
+    static constexpr int kSlots = Boxes == 1 ? 4 : 2;
+    static constexpr int kKeys = Boxes == 1 ? 64 : 128;
+    static constexpr int kWarps = 4 * kSlots;            // of the softmax
+    static constexpr int kThreads = 32 * (kWarps + 2);
+    static constexpr int kQBytes = Boxes * kBox;
+    static constexpr int kKeyBox = kKeys * umma::kRowBytes;
+    static constexpr int kTileBytes = Boxes * kKeyBox;
+    static constexpr int kStages = Boxes == 1 ? 8 : 5;   // of K and V tiles
+    static constexpr int kQueries = Boxes == 1 ? 2 : 1;  // items whose queries are kept
+    static constexpr int kSmem = kSlots * kQueries * kQBytes + kStages * kTileBytes + 1024;
+    static constexpr int kO = kSlots * kKeys;            // tensor memory: S and P of each row tile, then O of each
     static constexpr int kCols = 512;
     static_assert(kSmem <= kSmemMost - 1024, "shared memory");
+    static_assert(kO + kSlots * Boxes * 64 <= kCols, "tensor memory");
 };
 
 template <class T, int Boxes>
@@ -104,14 +114,17 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
     constexpr bool kBf16 = std::is_same_v<T, bf16>;
     constexpr float kOffset = kBf16 ? 0.0f : 7.0f;  // weights times 2^7
     constexpr int kStages = Cfg::kStages;
+    constexpr int kSlots = Cfg::kSlots;
+    constexpr int kKeys = Cfg::kKeys;
+    constexpr int kWarps = Cfg::kWarps;
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
-    const uint32_t ring = base + 2 * Cfg::kQueries * Cfg::kTileBytes;
-    __shared__ uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[2], p_full[2], o_full[2], o_free[2], drain;
+    const uint32_t ring = base + kSlots * Cfg::kQueries * Cfg::kQBytes;
+    __shared__ uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[kSlots], p_full[kSlots], o_full[kSlots], o_free[kSlots], drain;
     __shared__ uint32_t tmem_slot;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::alloc<Cfg::kCols>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
@@ -122,6 +135,8 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
         for (int x = 0; x < 2; ++x) {
             tma::mbar_init(&q_full[x], 1);
             tma::mbar_init(&q_empty[x], 1);
+        }
+        for (int x = 0; x < kSlots; ++x) {
             tma::mbar_init(&s_full[x], 1);
             tma::mbar_init(&p_full[x], 4);
             tma::mbar_init(&o_full[x], 1);
@@ -140,7 +155,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
     const Call& c = g.c;
     bool ok = true;
 
-    if (warp == 8) {
+    if (warp == kWarps) {
         // The TMA warp: Q of an item as soon as the one before is read, then its K and V tiles in turn.
         asm volatile("fence.proxy.async.global;" ::: "memory");
         const unsigned q_bytes = static_cast<unsigned>(g.tokens_per_tile * c.group) * umma::kRowBytes * Boxes;
@@ -148,7 +163,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
         unsigned phase = 0;
         long long issued = 0, q_issued = 0;
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
+            const Item it = item_at<kSlots, kKeys>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
@@ -162,7 +177,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                 for (int x = 0; x < it.slots; ++x) {
 #pragma unroll
                     for (int j = 0; j < Boxes; ++j) {
-                        load_heads(base + (2 * kept + x) * Cfg::kTileBytes + j * kBox, g.q, j * umma::kAtom, it.head * c.group,
+                        load_heads(base + (kSlots * kept + x) * Cfg::kQBytes + j * kBox, g.q, j * umma::kAtom, it.head * c.group,
                                    (it.row_tile + x) * g.tokens_per_tile, it.b, &q_full[kept]);
                     }
                 }
@@ -178,8 +193,8 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                     tma::mbar_arrive_expect_tx(&full[stage], Cfg::kTileBytes);
 #pragma unroll
                     for (int j = 0; j < Boxes; ++j) {
-                        load_heads(ring + stage * Cfg::kTileBytes + j * kBox, (t & 1) != 0 ? g.v : g.k, j * umma::kAtom, it.head,
-                                   it.key0 + (t >> 1) * kTile, it.b, &full[stage]);
+                        load_heads(ring + stage * Cfg::kTileBytes + j * Cfg::kKeyBox, (t & 1) != 0 ? g.v : g.k, j * umma::kAtom, it.head,
+                                   it.key0 + (t >> 1) * kKeys, it.b, &full[stage]);
                     }
                 }
                 __syncwarp();
@@ -202,22 +217,21 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == kWarps + 1) {
         // The MMA warp, one elected lane issues.
         const int steps = (c.dim + 15) / 16;
-        const uint32_t score = umma::instruction(kBf16, false, false, kTile, kTile);
+        const uint32_t score = umma::instruction(kBf16, false, false, kTile, kKeys);
         const uint32_t weigh = umma::instruction(kBf16, false, true, kTile, steps * 16);
         int stage = 0;
         unsigned phase = 0, taken = 0;  // items
-        unsigned slot_items[2] = {0, 0};
-        unsigned p_phases[2] = {0, 0};
+        unsigned slot_items = 0, p_phases = 0;  // a bit per row tile
         int kept = 0;
         const auto scores = [&](int x, uint32_t k_tile) {
             if (umma::elect_one()) {
-                const uint64_t a = umma::desc_k(base + (2 * kept + x) * Cfg::kTileBytes), b = umma::desc_k(k_tile);
+                const uint64_t a = umma::desc_k(base + (kSlots * kept + x) * Cfg::kQBytes), b = umma::desc_k(k_tile);
                 for (int s = 0; s < steps; ++s) {
-                    const uint64_t step = (s & 3) * umma::kStepK + (s >> 2) * (kBox >> 4);
-                    umma::mma(tmem + x * kTile, a + step, b + step, score, s > 0);
+                    const uint64_t step = (s & 3) * umma::kStepK;
+                    umma::mma(tmem + x * kKeys, a + step + (s >> 2) * (kBox >> 4), b + step + (s >> 2) * (Cfg::kKeyBox >> 4), score, s > 0);
                 }
                 umma::commit(&s_full[x]);
             }
@@ -230,7 +244,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
             }
         };
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
+            const Item it = item_at<kSlots, kKeys>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
@@ -266,17 +280,17 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                     break;
                 }
                 for (int x = 0; ok && x < it.slots; ++x) {
-                    ok = tma::mbar_wait(&p_full[x], p_phases[x]) && (t > 0 || tma::mbar_wait(&o_free[x], (slot_items[x] & 1u) ^ 1u));
+                    ok = tma::mbar_wait(&p_full[x], p_phases >> x & 1u) && (t > 0 || tma::mbar_wait(&o_free[x], (slot_items >> x & 1u) ^ 1u));
                     if (!ok) {
                         break;
                     }
-                    p_phases[x] ^= 1u;
+                    p_phases ^= 1u << x;
                     umma::fence_after_sync();
                     if (umma::elect_one()) {
-                        const uint64_t b = umma::desc_mn<kBox>(ring + v_stage * Cfg::kTileBytes);
+                        const uint64_t b = umma::desc_mn<Cfg::kKeyBox>(ring + v_stage * Cfg::kTileBytes);
 #pragma unroll
-                        for (int s = 0; s < kTile / 16; ++s) {
-                            mma_tmem(tmem + Cfg::kO + x * Boxes * 64, tmem + x * kTile + s * 8, b + umma::kStepMn * s, weigh, t > 0 || s > 0);
+                        for (int s = 0; s < kKeys / 16; ++s) {
+                            mma_tmem(tmem + Cfg::kO + x * Boxes * 64, tmem + x * kKeys + s * 8, b + umma::kStepMn * s, weigh, t > 0 || s > 0);
                         }
                         if (!more) {
                             umma::commit(&o_full[x]);
@@ -301,9 +315,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                 }
                 __syncwarp();
             }
-            for (int x = 0; x < it.slots; ++x) {
-                ++slot_items[x];
-            }
+            slot_items ^= (1u << it.slots) - 1u;
         }
         if (!ok) {
             if (umma::elect_one()) {
@@ -316,11 +328,11 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
             }
         }
     } else {
-        // A thread per row: warps 0 to 3 the first tile's, 4 to 7 the second's.
+        // A thread per row: warps 4 x to 4 x + 3 the x-th tile's.
         const int x = warp >> 2;
         const int quad = warp & 3;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-        const uint32_t s_at = tmem + lanes + x * kTile;
+        const uint32_t s_at = tmem + lanes + x * kKeys;
         const uint32_t o_at = tmem + lanes + Cfg::kO + x * Boxes * 64;
         const int local = quad * 32 + lane;
         const int row_token = local / c.group;
@@ -328,7 +340,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
         unsigned s_phase = 0, o_phase = 0;
         unsigned entry = 0;  // of the ring: the next K tile
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
+            const Item it = item_at<kSlots, kKeys>(g, i);
             if (x >= it.slots) {
                 entry += 2 * it.tiles;
                 continue;
@@ -342,7 +354,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
             float m = -INFINITY, sum = 0.0f;
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
-                tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
+                tile_bits(c, it.b, it.end, it.key0 + t * kKeys, w);
                 ok = tma::mbar_wait(&s_full[x], s_phase);
                 if (!ok) {
                     break;
@@ -350,37 +362,36 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                 s_phase ^= 1u;
                 umma::fence_after_sync();
                 if (!idle) {
-                    float s[4][32];
+                    // 32 scores at a time, fetched twice: for the largest, then for the weights.
+                    const auto scores = [&](int j, float (&s)[32]) {
+                        umma::load32(s_at + 32 * j, s);
+                        umma::load_wait(s);
+                        if (g.negative) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        umma::load32(s_at + 32 * j, s[j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        umma::load_wait(s[j]);
-                    }
-                    if (g.negative) {
-#pragma unroll
-                        for (int j = 0; j < 128; ++j) {
-                            s[j / 32][j % 32] = -s[j / 32][j % 32];
+                            for (int k = 0; k < 32; ++k) {
+                                s[k] = -s[k];
+                            }
                         }
-                    }
-                    if (!all_count(w)) {
+                        if (w[j] != 0xffffffffu) {
 #pragma unroll
-                        for (int j = 0; j < 128; ++j) {
-                            s[j / 32][j % 32] = (w[j / 32] >> (j % 32) & 1u) != 0 ? s[j / 32][j % 32] : -INFINITY;
+                            for (int k = 0; k < 32; ++k) {
+                                s[k] = (w[j] >> k & 1u) != 0 ? s[k] : -INFINITY;
+                            }
                         }
-                    }
-                    float top[4];
+                    };
+                    float largest = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        top[j] = s[j][0];
+                    for (int j = 0; j < kKeys / 32; ++j) {
+                        float s[32];
+                        scores(j, s);
+                        float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                        for (int k = 1; k < 32; ++k) {
-                            top[j] = fmaxf(top[j], s[j][k]);
+                        for (int k = 4; k < 32; ++k) {
+                            top[k % 4] = fmaxf(top[k % 4], s[k]);
                         }
+                        largest = fmaxf(largest, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                     }
-                    const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.factor;
+                    largest *= g.factor;
                     const bool move = largest > m + kSlack || (m == -INFINITY && largest > -INFINITY);
                     if (__any_sync(0xffffffffu, move)) {
                         // Each row by its own scores alone: its bits do not depend on its neighbours.
@@ -403,11 +414,13 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                     const float2 shift = pair((m == -INFINITY ? 0.0f : -m) + kOffset);
                     float2 total = pair(0.0f);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kKeys / 32; ++j) {
+                        float s[32];
+                        scores(j, s);
                         uint32_t p[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            const float2 e = fma2(make_float2(s[j][2 * k], s[j][2 * k + 1]), pair(g.factor), shift);
+                            const float2 e = fma2(make_float2(s[2 * k], s[2 * k + 1]), pair(g.factor), shift);
                             const float2 v = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                             total = total + v;
                             p[k] = pack2<T>(v);
@@ -417,11 +430,11 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                     sum += total.x + total.y;
                     store_wait();
                 }
-                if (!all_count(w)) {
-                    // Both row tiles wipe all of V: the other's products may come first.
+                if (!all_count<kKeys / 32>(w)) {
+                    // Each row tile's warps wipe all of V: another's products may come first.
                     const unsigned v_entry = entry + 1;
                     ok = tma::mbar_wait(&full[v_entry % kStages], v_entry / kStages & 1u);
-                    wipe_rows<kTile, 4>(ring + v_entry % kStages * Cfg::kTileBytes, Boxes, w, quad);
+                    wipe_rows<kKeys, 4>(ring + v_entry % kStages * Cfg::kTileBytes, Boxes, w, quad);
                 }
                 entry += 2;
                 umma::fence_before_sync();
@@ -496,7 +509,7 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::dealloc<Cfg::kCols>(tmem);
     }
 }
@@ -580,12 +593,13 @@ struct Plan {
         q = operand(arena, c.q, c.qs, c.batch, c.queries, c.kv_heads * c.group, c.dim, false);
         k = operand(arena, c.k, c.ks, c.batch, c.keys, c.kv_heads, c.dim, true);
         v = operand(arena, c.v, c.vs, c.batch, c.keys, c.kv_heads, c.dim, true);
-        row_items = pieces(pieces(c.queries, kTile / c.group), 2);
+        const int width = c.dim <= 64 ? Config<1>::kKeys : Config<2>::kKeys;
+        row_items = pieces(pieces(c.queries, kTile / c.group), c.dim <= 64 ? Config<1>::kSlots : Config<2>::kSlots);
         // Splits of the keys: the fewest turns of the busiest CTA, counted in key tiles, where an item costs about two
         // more (its first loads and scores, its last products and stores); parts are written and joined.
-        const long long tiles = pieces(c.keys, kTile);
+        const long long tiles = pieces(c.keys, width);
         const long long base = c.pairs() * row_items;
-        const long long least = std::max(1LL, (tiles + kLongestSum / kTile - 1) / (kLongestSum / kTile));
+        const long long least = std::max(1LL, (tiles + kLongestSum / width - 1) / (kLongestSum / width));
         double best = 0.0;
         for (long long s = least; s <= std::max(least, std::min(tiles, 128LL)); ++s) {
             const long long span = (tiles + s - 1) / s;
@@ -667,10 +681,11 @@ void tensor_forward(const Call& c, char* work, cudaStream_t stream)
     g.part_stats = reinterpret_cast<float2*>(work + plan.stats);
     g.fault = device_fault_word();
     g.q = head_map(plan.q.base(work), is_bf16, plan.q.strides(c.dim), c.batch, c.queries, c.kv_heads * c.group, c.dim, c.group, g.tokens_per_tile);
+    const int width = c.dim <= 64 ? Config<1>::kKeys : Config<2>::kKeys;
     const void* keys[2] = {plan.k.base(work), plan.v.base(work)};
     if (c.keys > 0) {
-        g.k = head_map(keys[0], is_bf16, plan.k.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile);
-        g.v = head_map(keys[1], is_bf16, plan.v.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, kTile);
+        g.k = head_map(keys[0], is_bf16, plan.k.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, width);
+        g.v = head_map(keys[1], is_bf16, plan.v.strides(c.dim), c.batch, c.keys, c.kv_heads, c.dim, 1, width);
     }
     const auto with_boxes = [&](auto t) {
         if (c.dim <= 64) {
