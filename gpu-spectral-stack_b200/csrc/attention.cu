@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Call c, const floa
                 out[d] = from_float<T>(acc[k] * f);
                 if constexpr (sizeof(T) == 2) {
                     if (c.rest != nullptr) {
-                        c.rest[to + d] = Rest<T>::code(acc[k] * f);
+                        c.rest[to + d] = static_cast<unsigned char>(rest_of<T>(make_float2(acc[k] * f, 0.0f)));
                     }
                 }
             }
@@ -960,7 +960,7 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
     c.lengths64 = lengths64;
     c.mask = static_cast<const unsigned char*>(mask);
     c.out = out;
-    c.rest = static_cast<signed char*>(rest);
+    c.rest = static_cast<unsigned char*>(rest);
     c.stats = reinterpret_cast<float2*>(stats);
     c.scale = scale;
     try {
@@ -1062,7 +1062,7 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         c.lengths64 = lengths64;
         c.mask = static_cast<const unsigned char*>(mask);
         c.out = const_cast<void*>(out);
-        c.rest = const_cast<signed char*>(static_cast<const signed char*>(rest));
+        c.rest = const_cast<unsigned char*>(static_cast<const unsigned char*>(rest));
         c.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
         c.dout = dout;
         c.dq = dq;

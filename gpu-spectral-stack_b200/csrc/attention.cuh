@@ -14,6 +14,8 @@
 #include "launch.cuh"
 #include "pointwise.cuh"
 
+#include <cuda_fp8.h>
+
 namespace spectral::attention {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -34,7 +36,7 @@ struct Call {
     const unsigned char* mask = nullptr;
     void* out = nullptr;       // (batch, queries, heads, dim)
     float2* stats = nullptr;   // (batch, kv_heads, rows): m and sum p; NULL: not kept
-    signed char* rest = nullptr;  // 16-bit types: what out's rounding took, of out's shape; NULL: not kept
+    unsigned char* rest = nullptr;  // 16-bit types: what out's rounding took, of out's shape; NULL: not kept
     // backward
     const void* dout = nullptr;  // (batch, queries, heads, dim)
     void* dq = nullptr;
@@ -69,29 +71,26 @@ __device__ __forceinline__ int length_of(const Call& c, int b)
     return static_cast<int>(max(0LL, min(n, static_cast<long long>(c.keys))));
 }
 
-// What rounding to T took from `o`, in units of 1/127 of half a step of T. The backward pass needs sum over dim of
-// dout out, the weighted mean of dout v, to subtract it from each dout v: with out as rounded, dq of 512 x 16384 keys in
-// float16 was off by 5.5e-4 of its norm, with this byte by 2.9e-4 (a rounding to float16 is 2.1e-4).
+// What rounding out to its type took from it, times 2^12, as e5m2 values (two mantissa bits; from 2^-28 up to 2^3). The backward
+// pass needs sum over dim of dout out, the weighted mean of dout v, to subtract it from each dout v: with out as
+// rounded, dq of 512 x 16384 keys in float16 was off by 5.5e-4 of its norm, with this byte by 3.1e-4 (one rounding to
+// float16 is 2.1e-4, and the score gradients are rounded too).
+constexpr float kRestScale = 4096.0f;
+
+// The bytes of two values, the first the lower.
 template <class T>
-struct Rest {
-    static constexpr bool kBf16 = std::is_same_v<T, bf16>;
-    static constexpr float kUnits = 127.0f * (kBf16 ? 256.0f : 2048.0f);  // of the value's power of two
-    __device__ __forceinline__ static uint32_t exponent(float back)
-    {
-        return max(min(__float_as_uint(back) & 0x7f800000u, 253u << 23), (kBf16 ? 1u : 113u) << 23);  // float16: 2^-14 at least
-    }
-    __device__ __forceinline__ static signed char code(float o)
-    {
-        const float back = to_float(from_float<T>(o));
-        const float inverse = __uint_as_float((254u << 23) - exponent(back));
-        const int c = __float2int_rn((o - back) * inverse * kUnits);
-        return static_cast<signed char>(max(-127, min(127, c)));
-    }
-    __device__ __forceinline__ static float restored(float back, signed char c)
-    {
-        return fmaf(static_cast<float>(c) * (1.0f / kUnits), __uint_as_float(exponent(back)), back);
-    }
-};
+__device__ __forceinline__ unsigned short rest_of(float2 o)
+{
+    const Vec<T, 2> rounded = narrow<T>(Floats<2>{{o}});
+    const float2 r = (o - widen(rounded).p[0]) * pair(kRestScale);
+    return __nv_cvt_float2_to_fp8x2(r, __NV_SATFINITE, __NV_E5M2);
+}
+
+__device__ __forceinline__ float2 with_rest(float2 rounded, unsigned short bytes)
+{
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(bytes, __NV_E5M2);
+    return fma2(__half22float2(__half2(h)), pair(1.0f / kRestScale), rounded);
+}
 
 // Sums of `parts` float32 arrays of a result, in order, rounded once. Partial arrays are (part, pair, row, dim);
 // the result's rows are those of Call::row_at (queries) or (sample, key, head) (keys).

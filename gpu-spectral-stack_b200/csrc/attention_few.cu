@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, R >= 8 ? 1 : 2) few_kernel(const Few
             static_cast<T*>(c.out)[to] = from_float<T>(o);
             if constexpr (sizeof(T) == 2) {
                 if (c.rest != nullptr) {
-                    c.rest[to] = Rest<T>::code(o);
+                    c.rest[to] = static_cast<unsigned char>(rest_of<T>(make_float2(o, 0.0f)));
                 }
             }
             if (c.stats != nullptr && d == 0) {

@@ -24,15 +24,15 @@ namespace {
 constexpr float kSlack = 8.0f;  // in powers of two, see above
 
 template <class T>
-__device__ __forceinline__ void store_rest(signed char* p, const float (&o)[16], int valid)
+__device__ __forceinline__ void store_rest(unsigned char* p, const float (&o)[16], int valid)
 {
-    Vec<signed char, 16> v;
+    Vec<unsigned char, 16> v;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        v.v[j] = Rest<T>::code(o[j]);
+    for (int j = 0; j < 8; ++j) {
+        reinterpret_cast<unsigned short*>(&v)[j] = rest_of<T>(make_float2(o[2 * j], o[2 * j + 1]));
     }
     if (valid == 16 && (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0) {
-        *reinterpret_cast<Vec<signed char, 16>*>(p) = v;
+        *reinterpret_cast<Vec<unsigned char, 16>*>(p) = v;
     } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {

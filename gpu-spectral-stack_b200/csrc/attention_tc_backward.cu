@@ -629,18 +629,18 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
             Floats<8> x = fetch(o + at);
             const Floats<8> y = fetch(g + at);
             if (sizeof(T) == 2 && c.rest != nullptr && sub * 8 < c.dim) {
-                Vec<signed char, 8> code{};
+                Vec<unsigned char, 8> code{};
                 if constexpr (Vectors) {
-                    code = *reinterpret_cast<const Vec<signed char, 8>*>(c.rest + at + sub * 8);
+                    code = *reinterpret_cast<const Vec<unsigned char, 8>*>(c.rest + at + sub * 8);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        code.v[j] = sub * 8 + j < c.dim ? c.rest[at + sub * 8 + j] : static_cast<signed char>(0);
+                        code.v[j] = sub * 8 + j < c.dim ? c.rest[at + sub * 8 + j] : static_cast<unsigned char>(0);
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x.set(j, Rest<T>::restored(x.at(j), code.v[j]));
+                for (int j = 0; j < 4; ++j) {
+                    x.p[j] = with_rest(x.p[j], reinterpret_cast<const unsigned short*>(&code)[j]);
                 }
             }
 #pragma unroll
