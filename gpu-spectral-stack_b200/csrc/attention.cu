@@ -563,11 +563,14 @@ __global__ void __launch_bounds__(kThreads) row_products_kernel(const Call c)
 
 // A thread per result value.
 template <class T>
-__global__ void __launch_bounds__(kThreads) add_parts_kernel(const Call c, const float* __restrict__ partial, int parts, bool of_keys,
-                                                             void* result, float factor)
+__global__ void __launch_bounds__(kThreads) add_parts_kernel(const Call c, const __grid_constant__ Sums sums)
 {
     allow_next_grid();
     wait_for_previous_grid();
+    const Sum& job = sums.job[blockIdx.y];
+    const float* __restrict__ partial = job.partial;
+    const bool of_keys = job.of_keys;
+    const int parts = job.parts;
     const long long count = of_keys ? c.keys : c.rows();
     const long long all = c.pairs() * count * c.dim;
     for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * kThreads) {
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(kThreads) add_parts_kernel(const Call c, const
         const long long r = row - at * count;
         const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
         const long long to = of_keys ? ((static_cast<long long>(b) * c.keys + r) * c.kv_heads + head) * c.dim : c.row_at(b, head, r);
-        static_cast<T*>(result)[to + d] = from_float<T>(sum * factor);
+        static_cast<T*>(job.result)[to + d] = from_float<T>(sum * job.factor);
     }
 }
 
@@ -647,13 +650,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Call c, const floa
 
 }  // namespace
 
-void add_parts(const Call& c, const float* partial, int parts, bool of_keys, void* result, float factor, cudaStream_t stream)
+void add_parts(const Call& c, const Sums& sums, cudaStream_t stream)
 {
-    const long long all = c.pairs() * (of_keys ? c.keys : c.rows()) * c.dim;
-    const auto grid = static_cast<unsigned>(std::min<long long>((all + kThreads - 1) / kThreads, 148 * 16));
-    with_dtype(c.dtype, [&](auto t) {
-        launch_pdl(add_parts_kernel<decltype(t)>, dim3(grid), dim3(kThreads), 0, stream, c, partial, parts, of_keys, result, factor);
-    });
+    if (sums.count == 0) {
+        return;
+    }
+    const long long all = c.pairs() * std::max<long long>(c.keys, c.rows()) * c.dim;
+    const dim3 grid(static_cast<unsigned>(std::min<long long>((all + kThreads - 1) / kThreads, 148 * 16)), sums.count);
+    with_dtype(c.dtype, [&](auto t) { launch_pdl(add_parts_kernel<decltype(t)>, grid, dim3(kThreads), 0, stream, c, sums); });
 }
 
 void join_splits(const Call& c, const float* partial, const float2* stats, int splits, cudaStream_t stream)
@@ -829,13 +833,15 @@ void backward(Call c, char* work, cudaStream_t stream)
         }
         launch(rows_backward_kernel<Dim, 4>, grid, smem, stream, c, plan.of_keys);
     });
+    Sums sums;
     if (plan.of_rows.count > 1) {
-        add_parts(c, plan.of_rows.first, plan.of_rows.count, true, c.dk, c.scale, stream);
-        add_parts(c, plan.of_rows.second, plan.of_rows.count, true, c.dv, 1.0f, stream);
+        sums.add(plan.of_rows.first, plan.of_rows.count, true, c.dk, c.scale);
+        sums.add(plan.of_rows.second, plan.of_rows.count, true, c.dv, 1.0f);
     }
     if (plan.of_keys.count > 1) {
-        add_parts(c, plan.of_keys.first, plan.of_keys.count, false, c.dq, c.scale, stream);
+        sums.add(plan.of_keys.first, plan.of_keys.count, false, c.dq, c.scale);
     }
+    add_parts(c, sums, stream);
 }
 
 int invalid(const std::string& message)

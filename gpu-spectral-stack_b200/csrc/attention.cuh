@@ -92,9 +92,21 @@ __device__ __forceinline__ float2 with_rest(float2 rounded, unsigned short bytes
     return fma2(__half22float2(__half2(h)), pair(1.0f / kRestScale), rounded);
 }
 
-// Sums of `parts` float32 arrays of a result, in order, rounded once. Partial arrays are (part, pair, row, dim);
-// the result's rows are those of Call::row_at (queries) or (sample, key, head) (keys).
-void add_parts(const Call& c, const float* partial, int parts, bool of_keys, void* result, float factor, cudaStream_t stream);
+// Sums of `parts` float32 arrays of a result, in order, times `factor`, rounded once. Partial arrays are (part, pair, row,
+// dim); the result's rows are those of Call::row_at (queries) or (sample, key, head) (keys).
+struct Sum {
+    const float* partial = nullptr;
+    void* result = nullptr;
+    int parts = 0;
+    bool of_keys = false;
+    float factor = 1.0f;
+};
+struct Sums {
+    Sum job[3];
+    int count = 0;
+    void add(const float* partial, int parts, bool of_keys, void* result, float factor) { job[count++] = {partial, result, parts, of_keys, factor}; }
+};
+void add_parts(const Call& c, const Sums& sums, cudaStream_t stream);
 
 // Joins the splits of a forward pass: partial (split, pair, row, dim) holds sum p v, stats (split, pair, row) m and
 // sum p.

@@ -14,7 +14,6 @@
 // 148th. Few rows over many keys are split so that all SMs read, and the parts joined by a second kernel.
 
 #include "attention_tc.cuh"
-#include "mlp.cuh"
 
 #include <algorithm>
 
@@ -22,26 +21,6 @@ namespace spectral::attention {
 namespace {
 
 constexpr float kSlack = 8.0f;  // in powers of two, see above
-
-template <class T>
-__device__ __forceinline__ void store_rest(unsigned char* p, const float (&o)[16], int valid)
-{
-    Vec<unsigned char, 16> v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        reinterpret_cast<unsigned short*>(&v)[j] = rest_of<T>(make_float2(o[2 * j], o[2 * j + 1]));
-    }
-    if (valid == 16 && (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0) {
-        *reinterpret_cast<Vec<unsigned char, 16>*>(p) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if (j < valid) {
-                p[j] = v.v[j];
-            }
-        }
-    }
-}
 
 struct Forward {
     HeadMap q, k, v;
@@ -460,6 +439,8 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
             const long long part_row = (it.split * c.pairs() + at) * c.rows() + row;
             const long long out_at = ((static_cast<long long>(it.b) * c.queries + token) * c.kv_heads + it.head) * c.group * c.dim + row_head * c.dim;
             T* out = static_cast<T*>(c.out) + out_at;
+            const bool sectors = g.splits > 1 ? whole_sectors(g.partial, c.dim, 4)
+                                              : whole_sectors(c.out, c.dim, 2) && (c.rest == nullptr || whole_sectors(c.rest, c.dim * 2, 1));
             if (!idle) {
                 for (int d = 0; d < c.dim; d += 16) {
                     float o[16];
@@ -472,20 +453,15 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
                             o[k] = 0.0f;
                         }
                     }
-                    if (live) {
-                        const int valid = min(16, c.dim - d);
-                        if (g.splits > 1) {
-                            mlp::store_values<float>(g.partial + part_row * c.dim + d, o, valid);
-                        } else {
+                    const int valid = min(16, c.dim - d);
+                    if (g.splits > 1) {
+                        store_lanes<float>(g.partial + part_row * c.dim + d, nullptr, live, o, valid, sectors);
+                    } else {
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                o[k] *= inverse;
-                            }
-                            mlp::store_values<T>(out + d, o, valid);
-                            if (c.rest != nullptr) {
-                                store_rest<T>(c.rest + out_at + d, o, valid);
-                            }
+                        for (int k = 0; k < 16; ++k) {
+                            o[k] *= inverse;
                         }
+                        store_lanes<T>(out + d, c.rest == nullptr ? nullptr : c.rest + out_at + d, live, o, valid, sectors);
                     }
                 }
                 if (live && g.splits > 1) {

@@ -8,6 +8,7 @@
 // 128 keys. Heads are padded with zeros to 64 or 128 values by the copy; products run over whole 16s of `dim`.
 
 #include "attention.cuh"
+#include "mlp.cuh"
 #include "umma.cuh"
 
 namespace spectral::attention {
@@ -117,6 +118,70 @@ __device__ __forceinline__ void wipe_rows(uint32_t tile, int boxes, const uint32
         }
     }
     tma::fence_proxy_async();
+}
+
+// N columns of 32 rows, a row a lane: lane l's at its own p (if it is `live`), `valid` of them. `sectors` (the same in all
+// lanes): every row's run is whole 32-byte sectors, and each lane stores its own; else the values change lanes first, so that
+// a row's are stored side by side. `rest` (16-bit types, or NULL): the bytes that out's rounding leaves, at the same places.
+template <class T, int N>
+__device__ __forceinline__ void store_lanes(T* p, unsigned char* rest, bool live, float (&v)[N], int valid, bool sectors)
+{
+    if (sectors) {
+        if (live) {
+            mlp::store_values<T>(p, v, valid);
+            if constexpr (sizeof(T) == 2) {
+                if (rest != nullptr) {
+                    Vec<unsigned char, N> bytes;
+#pragma unroll
+                    for (int j = 0; j < N / 2; ++j) {
+                        reinterpret_cast<unsigned short*>(&bytes)[j] = rest_of<T>(make_float2(v[2 * j], v[2 * j + 1]));
+                    }
+                    *reinterpret_cast<Vec<unsigned char, N>*>(rest) = bytes;  // dim is a multiple of 16 then
+                }
+            }
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s = N / 2; s > 0; s >>= 1) {
+        const bool upper = (lane & s) != 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if ((j & s) == 0) {
+                const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j | s], s);
+                v[j] = upper ? other : v[j];
+                v[j | s] = upper ? v[j | s] : other;
+            }
+        }
+    }
+    const int first = lane & ~(N - 1);  // N lanes hold the columns of N rows
+    const int col = lane & (N - 1);
+    const unsigned there = __ballot_sync(0xffffffffu, live);
+    const auto at = reinterpret_cast<unsigned long long>(p);
+    const auto rest_at = reinterpret_cast<unsigned long long>(rest);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        T* row = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, at, first + j));
+        const bool stores = (there >> (first + j) & 1u) != 0 && col < valid;
+        if (stores) {
+            row[col] = from_float<T>(v[j]);
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (rest != nullptr) {
+                auto* bytes = reinterpret_cast<unsigned char*>(__shfl_sync(0xffffffffu, rest_at, first + j));
+                if (stores) {
+                    bytes[col] = static_cast<unsigned char>(rest_of<T>(make_float2(v[j], 0.0f)));
+                }
+            }
+        }
+    }
+}
+
+// Whether rows of dim values of `size` bytes from `base` on are whole sectors.
+__device__ __forceinline__ bool whole_sectors(const void* base, int dim, int size)
+{
+    return ((reinterpret_cast<std::uintptr_t>(base) | static_cast<std::uintptr_t>(dim * size)) & 31u) == 0;
 }
 
 // --- host ------------------------------------------------------------------------------------------

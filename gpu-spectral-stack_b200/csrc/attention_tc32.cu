@@ -10,7 +10,6 @@
 // tensor cores and the softmax, a thread per row; backward, one kernel that owns keys and one that owns rows.
 
 #include "attention_tc.cuh"
-#include "mlp.cuh"
 
 #include <algorithm>
 
@@ -414,10 +413,11 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                     umma::arrive(&o_free[x]);
                 }
             }
-            if (live) {
+            if (!idle) {
                 const long long at = static_cast<long long>(it.b) * c.kv_heads + it.head;
                 const float base_m = m == -INFINITY && g.splits == 1 ? 0.0f : m;
                 const float factor = g.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+                const bool sectors = whole_sectors(g.splits > 1 ? g.partial : c.out, c.dim, 4);
                 const long long part_row = (it.split * c.pairs() + at) * c.rows() + row;
                 float* to = g.splits > 1 ? g.partial + part_row * c.dim
                                          : static_cast<float*>(c.out)
@@ -430,12 +430,12 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                         for (int k = 0; k < 32; ++k) {
                             o[j][k] *= factor;
                         }
-                        mlp::store_values<float>(to + 32 * j, o[j], min(32, c.dim - 32 * j));
+                        store_lanes<float>(to + 32 * j, nullptr, live, o[j], min(32, c.dim - 32 * j), sectors);
                     }
                 }
-                if (g.splits > 1) {
+                if (live && g.splits > 1) {
                     g.part_stats[part_row] = make_float2(base_m, sum);
-                } else if (c.stats != nullptr) {
+                } else if (live && c.stats != nullptr) {
                     c.stats[at * c.rows() + row] = make_float2(base_m, sum);
                 }
             }
@@ -879,7 +879,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                     umma::arrive(&acc_free);
                 }
             }
-            if (live && holds) {
+            if (holds) {
                 const long long part_row = (it.part * c.pairs() + pair_at) * (Rows ? c.rows() : c.keys) + row;
                 const long long to = (g.parts > 1 ? part_row * c.dim
                                       : Rows
@@ -892,13 +892,15 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                 for (int k = 0; k < 32; ++k) {
                     a0[k] = counts ? a0[k] * scale : 0.0f;
                 }
-                mlp::store_values<float>((g.parts > 1 ? g.partial0 : static_cast<float*>(Rows ? c.dq : c.dk)) + to, a0, valid);
+                float* result = g.parts > 1 ? g.partial0 : static_cast<float*>(Rows ? c.dq : c.dk);
+                store_lanes<float>(result + to, nullptr, live, a0, valid, whole_sectors(result, c.dim, 4));
                 if constexpr (!Rows) {
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
                         a1[k] = counts ? a1[k] : 0.0f;
                     }
-                    mlp::store_values<float>((g.parts > 1 ? g.partial1 : static_cast<float*>(c.dv)) + to, a1, valid);
+                    result = g.parts > 1 ? g.partial1 : static_cast<float*>(c.dv);
+                    store_lanes<float>(result + to, nullptr, live, a1, valid, whole_sectors(result, c.dim, 4));
                 }
             }
         }
@@ -1205,13 +1207,15 @@ void split_backward(const Call& c, char* work, cudaStream_t stream)
     g.items = item_count(c.pairs() * plan.row_tiles * plan.key_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dq);
     launch(backward_kernel<true>, g, kBackwardThreads, kBackwardSmem, stream);
+    Sums sums;
     if (plan.row_parts > 1) {
-        add_parts(c, reinterpret_cast<const float*>(work + plan.dk), plan.row_parts, true, c.dk, c.scale, stream);
-        add_parts(c, reinterpret_cast<const float*>(work + plan.dv), plan.row_parts, true, c.dv, 1.0f, stream);
+        sums.add(reinterpret_cast<const float*>(work + plan.dk), plan.row_parts, true, c.dk, c.scale);
+        sums.add(reinterpret_cast<const float*>(work + plan.dv), plan.row_parts, true, c.dv, 1.0f);
     }
     if (plan.key_parts > 1) {
-        add_parts(c, reinterpret_cast<const float*>(work + plan.dq), plan.key_parts, false, c.dq, c.scale, stream);
+        sums.add(reinterpret_cast<const float*>(work + plan.dq), plan.key_parts, false, c.dq, c.scale);
     }
+    add_parts(c, sums, stream);
 }
 
 }  // namespace spectral::attention

@@ -17,7 +17,6 @@
 // less (16384 keys and more) would be subnormal, and small gradients zero.
 
 #include "attention_tc.cuh"
-#include "mlp.cuh"
 
 #include <algorithm>
 
@@ -545,12 +544,10 @@ __global__ void __launch_bounds__(Config<Boxes, Rows>::kThreads, Config<Boxes, R
                     for (int k = 0; k < 16; ++k) {
                         a[k] = it.tiles == 0 || !counts ? 0.0f : a[k] * factor;
                     }
-                    if (live) {
-                        if (g.parts > 1) {
-                            mlp::store_values<float>(partial + part_row * c.dim + d, a, min(16, c.dim - d));
-                        } else {
-                            mlp::store_values<T>(result + at + d, a, min(16, c.dim - d));
-                        }
+                    if (g.parts > 1) {
+                        store_lanes<float>(partial + part_row * c.dim + d, nullptr, live, a, min(16, c.dim - d), whole_sectors(partial, c.dim, 4));
+                    } else {
+                        store_lanes<T>(result + at + d, nullptr, live, a, min(16, c.dim - d), whole_sectors(result, c.dim, 2));
                     }
                 }
             }
@@ -899,13 +896,15 @@ void tensor_backward(const Call& c, char* work, cudaStream_t stream)
     } else {
         run(f16{});
     }
+    Sums sums;
     if (plan.row_parts > 1) {
-        add_parts(c, reinterpret_cast<const float*>(work + plan.dk), plan.row_parts, true, c.dk, c.scale, stream);
-        add_parts(c, reinterpret_cast<const float*>(work + plan.dv), plan.row_parts, true, c.dv, 1.0f, stream);
+        sums.add(reinterpret_cast<const float*>(work + plan.dk), plan.row_parts, true, c.dk, c.scale);
+        sums.add(reinterpret_cast<const float*>(work + plan.dv), plan.row_parts, true, c.dv, 1.0f);
     }
     if (plan.key_parts > 1) {
-        add_parts(c, reinterpret_cast<const float*>(work + plan.dq), plan.key_parts, false, c.dq, c.scale, stream);
+        sums.add(reinterpret_cast<const float*>(work + plan.dq), plan.key_parts, false, c.dq, c.scale);
     }
+    add_parts(c, sums, stream);
 }
 
 }  // namespace spectral::attention
