@@ -629,15 +629,16 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
     // Whole warps stay in the loops together: they shuffle.
     for (long long base = static_cast<long long>(blockIdx.x) * per_cta; base < all; base += static_cast<long long>(gridDim.x) * per_cta) {
         const long long i = base + threadIdx.x / lanes;
-        const int local = static_cast<int>(i % width);
-        const long long tile = i / width;
-        const long long pair_at = tile / row_tiles;
-        const long long r = (tile - pair_at * row_tiles) * rows_per_tile + local;
+        const int local = static_cast<int>(i & (width - 1));  // 64 or 128
+        const auto tile = static_cast<unsigned>(i / width);     // below 2^31: every tile is an item or a part of one
+        const unsigned pair_at = tile / static_cast<unsigned>(row_tiles);
+        const int r = static_cast<int>(tile - pair_at * row_tiles) * rows_per_tile + local;
         const bool there = i < all && local < rows_per_tile && r < c.rows();
         float2 dot = pair(0.0f), square = pair(0.0f);
         if (there) {
-            const int b = static_cast<int>(pair_at / c.kv_heads);
-            const long long at = c.row_at(b, static_cast<int>(pair_at - static_cast<long long>(b) * c.kv_heads), r);
+            const unsigned b = pair_at / static_cast<unsigned>(c.kv_heads), token = static_cast<unsigned>(r) / static_cast<unsigned>(c.group);
+            const long long at = ((static_cast<long long>(b) * c.queries + token) * c.kv_heads + (pair_at - b * c.kv_heads)) * c.group * c.dim
+                                 + (r - static_cast<int>(token) * c.group) * c.dim;
             Floats<8> x = fetch(o + at);
             const Floats<8> y = fetch(g + at);
             if (sizeof(T) == 2 && c.rest != nullptr && sub * 8 < c.dim) {
