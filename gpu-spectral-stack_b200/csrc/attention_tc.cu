@@ -331,9 +331,11 @@ __global__ void __launch_bounds__(Config<Boxes>::kThreads, 1) forward_kernel(con
             // A warp without rows only keeps the barriers going; what lies in its lanes reaches no one.
             const bool idle = quad * 32 >= min(g.tokens_per_tile, c.queries - first_token) * c.group;
             float m = -INFINITY, sum = 0.0f;
+            MaskBytes<kKeys / 32> coming = mask_bytes<kKeys / 32>(c, it.b, it.end, it.key0);
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
-                tile_bits(c, it.b, it.end, it.key0 + t * kKeys, w);
+                tile_bits<kKeys / 32>(c, coming, it.end, it.key0 + t * kKeys, w);
+                coming = mask_bytes<kKeys / 32>(c, it.b, it.end, it.key0 + (t + 1) * kKeys);
                 ok = tma::mbar_wait(&s_full[x], s_phase);
                 if (!ok) {
                     break;

@@ -70,26 +70,41 @@ __device__ __forceinline__ uint32_t pack2(float2 v)
     return *reinterpret_cast<const uint32_t*>(&two);
 }
 
+// A lane's bytes of the mask over a tile of 32 Words keys, asked for a tile ahead of their use.
+template <int Words>
+struct MaskBytes {
+    unsigned char v[Words];
+};
+
+template <int Words>
+__device__ __forceinline__ MaskBytes<Words> mask_bytes(const Call& c, int b, int end, int key0)
+{
+    MaskBytes<Words> m;
+    if (c.mask != nullptr) {
+        const unsigned char* at = c.mask + static_cast<long long>(b) * c.keys + key0;
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < Words; ++i) {
+            m.v[i] = 32 * i + lane < end - key0 ? at[32 * i + lane] : 0;
+        }
+    }
+    return m;
+}
+
 // One bit per key of the tile at key0 that counts: bit i of word w is key0 + 32 w + i. The whole warp calls it.
-__device__ __forceinline__ void tile_bits(const Call& c, int b, int end, int key0, uint32_t (&w)[4])
+template <int Words>
+__device__ __forceinline__ void tile_bits(const Call& c, const MaskBytes<Words>& m, int end, int key0, uint32_t (&w)[4])
 {
     const int left = end - key0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < Words; ++i) {
         const int n = left - 32 * i;
         w[i] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
     }
     if (c.mask != nullptr) {
-        const unsigned char* m = c.mask + static_cast<long long>(b) * c.keys + key0;
-        const int lane = threadIdx.x & 31;
-        unsigned char v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = 32 * i + lane < left ? m[32 * i + lane] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = __ballot_sync(0xffffffffu, v[i] != 0);
+        for (int i = 0; i < Words; ++i) {
+            w[i] = __ballot_sync(0xffffffffu, m.v[i] != 0);
         }
     }
 }

@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
             const bool live = row_token < g.tokens_per_tile && token < c.queries;
             const bool idle = quad * 32 >= min(g.tokens_per_tile, c.queries - first_token) * c.group;
             float m = -INFINITY, sum = 0.0f;
+            MaskBytes<4> coming = mask_bytes<4>(c, it.b, it.end, it.key0);
             float o[2][32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
@@ -332,7 +333,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
             };
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
-                tile_bits(c, it.b, it.end, it.key0 + t * kTile, w);
+                tile_bits<4>(c, coming, it.end, it.key0 + t * kTile, w);
+                coming = mask_bytes<4>(c, it.b, it.end, it.key0 + (t + 1) * kTile);
                 ok = tma::mbar_wait(&s_full[x], s_phase);
                 if (!ok) {
                     break;
@@ -796,10 +798,15 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                     }
                 }
             };
+            MaskBytes<2> mask{};
+            if constexpr (Rows) {
+                mask = mask_bytes<2>(c, it.b, it.end, it.first * kWidth);
+            }
             for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
                 uint32_t w[4] = {0, 0, 0, 0};
                 if constexpr (Rows) {
-                    tile_bits(c, it.b, it.end, t * kWidth, w);
+                    tile_bits<2>(c, mask, it.end, t * kWidth, w);
+                    mask = mask_bytes<2>(c, it.b, it.end, (t + 1) * kWidth);
                 }
                 const uint32_t word = Rows ? (part == 0 ? w[0] : w[1]) : counts ? 0xffffffffu : 0u;
                 ok = tma::mbar_wait(&full[stage], phase) && tma::mbar_wait(&s_full, step_phase);

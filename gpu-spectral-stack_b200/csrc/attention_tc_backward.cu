@@ -411,10 +411,15 @@ __global__ void __launch_bounds__(Config<Boxes, Rows>::kThreads, Config<Boxes, R
                 counts = row < it.end && (c.mask == nullptr || c.mask[static_cast<long long>(it.b) * c.keys + row] != 0);
             }
             const bool whole = __all_sync(0xffffffffu, counts);
+            MaskBytes<kWidth / 32> mask{};
+            if constexpr (Rows) {
+                mask = mask_bytes<kWidth / 32>(c, it.b, it.end, it.first * kWidth);
+            }
             for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
                 uint32_t w[4] = {0, 0, 0, 0};
                 if constexpr (Rows) {
-                    tile_bits(c, it.b, it.end, t * kWidth, w);
+                    tile_bits<kWidth / 32>(c, mask, it.end, t * kWidth, w);
+                    mask = mask_bytes<kWidth / 32>(c, it.b, it.end, (t + 1) * kWidth);
                 }
                 ok = tma::mbar_wait(&full[stage], phase);
                 const float* less = constants + stage * Cfg::kConstants + part * 32;  // -lse, then -delta
