@@ -731,8 +731,8 @@ struct ForwardPlan {
     }
 };
 
-// Float32 calls whose products are worth splitting: heads of up to 64 values and more rows than a few.
-bool on_tensor_cores(const Call& c) { return c.dim <= 64 && c.group <= 64 && c.rows() > 16 && c.keys > 0; }
+// Float32 calls whose products are worth splitting: more rows than a few.
+bool on_tensor_cores(const Call& c) { return c.group <= 64 && c.rows() > 16 && c.keys > 0; }
 
 std::size_t forward_workspace(const Call& c)
 {

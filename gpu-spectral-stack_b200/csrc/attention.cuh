@@ -118,8 +118,7 @@ void tensor_forward(const Call& c, char* work, cudaStream_t stream);
 std::size_t tensor_backward_workspace(const Call& c);
 void tensor_backward(const Call& c, char* work, cudaStream_t stream);
 
-// The float32 kernels on the tensor cores (attention_tc32.cu): heads of at most 64 values, at most 64 query heads to a key
-// head.
+// The float32 kernels on the tensor cores (attention_tc32.cu): at most 64 query heads to a key head.
 std::size_t split_forward_workspace(const Call& c);
 void split_forward(const Call& c, char* work, cudaStream_t stream);
 std::size_t split_backward_workspace(const Call& c);

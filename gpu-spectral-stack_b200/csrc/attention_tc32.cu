@@ -1,4 +1,4 @@
-// Attention for float32 heads of up to 64 values on the tensor cores, forward and backward.
+// Attention for float32 on the tensor cores, forward and backward.
 //
 // Every operand is split into three bf16 parts (their sum is the value to 2^-24 of it), every product into the six
 // that matter, the small ones first: FP32-level error. q, k, v and the upstream gradient are split by a kernel before
@@ -30,6 +30,13 @@ __device__ __forceinline__ void split_pair(float2 v, uint32_t& hi, uint32_t& mid
     lo = pack2<bf16>(r - wide(mid));
 }
 
+__device__ __forceinline__ void store8(uint32_t taddr, const uint32_t (&v)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 // 32 columns of a row into operands: parts 0 and 1 over the scores they came from, part 2 into `rest`.
 __device__ __forceinline__ void store_parts(uint32_t scores, uint32_t rest, const float (&v)[32])
 {
@@ -43,10 +50,24 @@ __device__ __forceinline__ void store_parts(uint32_t scores, uint32_t rest, cons
     store16(rest, part[2]);
 }
 
-// Where the operand's part p of 16 columns s lies.
+// The same of 16 columns.
+__device__ __forceinline__ void store_parts(uint32_t scores, uint32_t rest, const float (&v)[16])
+{
+    uint32_t part[kPlanes][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        split_pair(make_float2(v[2 * k], v[2 * k + 1]), part[0][k], part[1][k], part[2][k]);
+    }
+    store8(scores, part[0]);
+    store8(scores + 8, part[1]);
+    store8(rest, part[2]);
+}
+
+// Where the operand's part p of the s-th 16 columns lies, if threads hold Columns of them.
+template <int Columns>
 __device__ __forceinline__ uint32_t part_at(uint32_t scores, uint32_t rest, int p, int s)
 {
-    return p == 2 ? rest + s * 8 : scores + (s >> 1) * 32 + p * 16 + (s & 1) * 8;
+    return p == 2 ? rest + s * 8 : Columns == 32 ? scores + (s >> 1) * 32 + p * 16 + (s & 1) * 8 : scores + s * 16 + p * 8;
 }
 
 // --- forward -------------------------------------------------------------------------------------------
@@ -76,42 +97,59 @@ struct Item {
     int slots;
 };
 
+// Heads of up to 64 values: two row tiles and 128 keys at a time. Wider ones: their parts fill the shared memory with one row
+// tile and 64 keys.
+template <int Boxes>
+struct ForwardConfig {
+    static constexpr int kSlots = Boxes == 1 ? 2 : 1;
+    static constexpr int kKeys = Boxes == 1 ? 128 : 64;
+    static constexpr int kWarps = 4 * kSlots;
+    static constexpr int kThreads = 32 * (kWarps + 2);
+    static constexpr int kPlaneBytes = Boxes * kBox;     // of 128 rows
+    static constexpr int kTileBytes = kPlanes * kPlaneBytes;
+    static constexpr int kKeyBox = kKeys * umma::kRowBytes;
+    static constexpr int kKeyPlane = Boxes * kKeyBox;
+    static constexpr int kKeyBytes = kPlanes * kKeyPlane;
+    static constexpr int kSmem = kSlots * kTileBytes + 2 * kKeyBytes + 1024;  // Q, K, V
+    // Tensor memory of a row tile: scores (parts 0 and 1 of the weights), part 2, O.
+    static constexpr int kRest = kKeys;
+    static constexpr int kO = kKeys + kKeys / 2;
+    static constexpr int kSlotCols = 256;
+    static_assert(kSmem <= kSmemMost - 1024 && kO + Boxes * 64 <= kSlotCols, "shared and tensor memory");
+};
+
+template <int Boxes>
 __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
 {
+    using Cfg = ForwardConfig<Boxes>;
     Item it;
     const unsigned r = i / g.row_items;
-    it.row_tile = static_cast<int>(i - r * g.row_items) * 2;
+    it.row_tile = static_cast<int>(i - r * g.row_items) * Cfg::kSlots;
     const unsigned pair = r / g.splits;
     it.split = static_cast<int>(r - pair * g.splits);
     it.b = static_cast<int>(pair / static_cast<unsigned>(g.c.kv_heads));
     it.head = static_cast<int>(pair) - it.b * g.c.kv_heads;
-    it.key0 = it.split * g.split_tiles * kTile;
-    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * kTile);
-    it.tiles = it.end > it.key0 ? (it.end - it.key0 + kTile - 1) / kTile : 0;
-    it.slots = (it.row_tile + 1) * g.tokens_per_tile < g.c.queries ? 2 : 1;
+    it.key0 = it.split * g.split_tiles * Cfg::kKeys;
+    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * Cfg::kKeys);
+    it.tiles = it.end > it.key0 ? (it.end - it.key0 + Cfg::kKeys - 1) / Cfg::kKeys : 0;
+    it.slots = Cfg::kSlots == 2 && (it.row_tile + 1) * g.tokens_per_tile < g.c.queries ? 2 : 1;
     return it;
 }
 
-constexpr int kForwardThreads = 320;
-constexpr int kPlaneBytes = kBox;                  // 128 rows of 64 values
-constexpr int kTileBytes = kPlanes * kPlaneBytes;
-constexpr int kForwardSmem = 4 * kTileBytes + 1024;  // Q 0 and 1, K, V
-static_assert(kForwardSmem <= kSmemMost - 1024, "shared memory");
-// Tensor memory of a row tile: scores (parts 0 and 1 of the weights), part 2, O.
-constexpr int kSlotCols = 256;
-constexpr int kRestAt = 128;
-constexpr int kOAt = 192;
-
-__global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __grid_constant__ Forward g)
+template <int Boxes>
+__global__ void __launch_bounds__(ForwardConfig<Boxes>::kThreads, 1) forward_kernel(const __grid_constant__ Forward g)
 {
+    using Cfg = ForwardConfig<Boxes>;
+    constexpr int kWarps = Cfg::kWarps;
+    constexpr int kKeys = Cfg::kKeys;
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
-    const uint32_t kv = base + 2 * kTileBytes;  // K, then V
+    const uint32_t kv = base + Cfg::kSlots * Cfg::kTileBytes;  // K, then V
     __shared__ uint64_t q_full, q_empty, full[2], empty[2], s_full[2], p_full[2], o_full[2], o_free[2], drain;
     __shared__ uint32_t tmem_slot;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::alloc<512>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
@@ -138,13 +176,13 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
     const Call& c = g.c;
     bool ok = true;
 
-    if (warp == 8) {
+    if (warp == kWarps) {
         // The TMA warp.
         asm volatile("fence.proxy.async.global;" ::: "memory");
-        const unsigned q_bytes = static_cast<unsigned>(g.tokens_per_tile * c.group) * umma::kRowBytes * kPlanes;
+        const unsigned q_bytes = static_cast<unsigned>(g.tokens_per_tile * c.group) * umma::kRowBytes * kPlanes * Boxes;
         unsigned issued[2] = {0, 0}, items = 0;  // K, V
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
+            const Item it = item_at<Boxes>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
@@ -156,8 +194,10 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                 tma::mbar_arrive_expect_tx(&q_full, q_bytes * it.slots);
                 for (int x = 0; x < it.slots; ++x) {
                     for (int p = 0; p < kPlanes; ++p) {
-                        load_heads(base + x * kTileBytes + p * kPlaneBytes, g.q, 0, it.head * c.group, (it.row_tile + x) * g.tokens_per_tile,
-                                   p * c.batch + it.b, &q_full);
+                        for (int j = 0; j < Boxes; ++j) {
+                            load_heads(base + x * Cfg::kTileBytes + p * Cfg::kPlaneBytes + j * kBox, g.q, j * umma::kAtom, it.head * c.group,
+                                       (it.row_tile + x) * g.tokens_per_tile, p * c.batch + it.b, &q_full);
+                        }
                     }
                 }
             }
@@ -170,10 +210,12 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                         break;
                     }
                     if (umma::elect_one()) {
-                        tma::mbar_arrive_expect_tx(&full[x], kTileBytes);
+                        tma::mbar_arrive_expect_tx(&full[x], Cfg::kKeyBytes);
                         for (int p = 0; p < kPlanes; ++p) {
-                            load_heads(kv + x * kTileBytes + p * kPlaneBytes, x == 0 ? g.k : g.v, 0, it.head, it.key0 + t * kTile, p * c.batch + it.b,
-                                       &full[x]);
+                            for (int j = 0; j < Boxes; ++j) {
+                                load_heads(kv + x * Cfg::kKeyBytes + p * Cfg::kKeyPlane + j * Cfg::kKeyBox, x == 0 ? g.k : g.v, j * umma::kAtom, it.head,
+                                           it.key0 + t * kKeys, p * c.batch + it.b, &full[x]);
+                            }
                         }
                     }
                     __syncwarp();
@@ -190,20 +232,21 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == kWarps + 1) {
         // The MMA warp, one elected lane issues.
         const int steps = (c.dim + 15) / 16;
-        const uint32_t score = umma::instruction(true, false, false, kTile, kTile);
+        const uint32_t score = umma::instruction(true, false, false, kTile, kKeys);
         const uint32_t weigh = umma::instruction(true, false, true, kTile, steps * 16);
         unsigned used = 0, items = 0;
         unsigned p_phases[2] = {0, 0}, slot_items[2] = {0, 0};
         const auto scores = [&](int x) {
             if (umma::elect_one()) {
                 for (int p = 0; p < kProducts; ++p) {
-                    const uint64_t a = umma::desc_k(base + x * kTileBytes + mlp::part_a<float>(p) * kPlaneBytes);
-                    const uint64_t b = umma::desc_k(kv + mlp::part_b<float>(p) * kPlaneBytes);
+                    const uint64_t a = umma::desc_k(base + x * Cfg::kTileBytes + mlp::part_a<float>(p) * Cfg::kPlaneBytes);
+                    const uint64_t b = umma::desc_k(kv + mlp::part_b<float>(p) * Cfg::kKeyPlane);
                     for (int s = 0; s < steps; ++s) {
-                        umma::mma(tmem + x * kSlotCols, a + s * umma::kStepK, b + s * umma::kStepK, score, p > 0 || s > 0);
+                        const uint64_t step = (s & 3) * umma::kStepK;
+                        umma::mma(tmem + x * Cfg::kSlotCols, a + step + (s >> 2) * (kBox >> 4), b + step + (s >> 2) * (Cfg::kKeyBox >> 4), score, p > 0 || s > 0);
                     }
                 }
                 umma::commit(&s_full[x]);
@@ -211,7 +254,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
             __syncwarp();
         };
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
+            const Item it = item_at<Boxes>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
@@ -243,12 +286,12 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                     p_phases[x] ^= 1u;
                     umma::fence_after_sync();
                     if (umma::elect_one()) {
-                        const uint32_t at = tmem + x * kSlotCols;
+                        const uint32_t at = tmem + x * Cfg::kSlotCols;
                         for (int p = 0; p < kProducts; ++p) {
-                            const uint64_t b = umma::desc_mn<kBox>(kv + kTileBytes + mlp::part_b<float>(p) * kPlaneBytes);
+                            const uint64_t b = umma::desc_mn<Cfg::kKeyBox>(kv + Cfg::kKeyBytes + mlp::part_b<float>(p) * Cfg::kKeyPlane);
 #pragma unroll
-                            for (int s = 0; s < kTile / 16; ++s) {
-                                mma_tmem(at + kOAt, part_at(at, at + kRestAt, mlp::part_a<float>(p), s), b + umma::kStepMn * s, weigh, p > 0 || s > 0);
+                            for (int s = 0; s < kKeys / 16; ++s) {
+                                mma_tmem(at + Cfg::kO, part_at<32>(at, at + Cfg::kRest, mlp::part_a<float>(p), s), b + umma::kStepMn * s, weigh, p > 0 || s > 0);
                             }
                         }
                         if (!more) {
@@ -292,14 +335,13 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
         // A thread per row: warps 0 to 3 the first tile's, 4 to 7 the second's.
         const int x = warp >> 2;
         const int quad = warp & 3;
-        const uint32_t s_at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + x * kSlotCols;
+        const uint32_t s_at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + x * Cfg::kSlotCols;
         const int local = quad * 32 + lane;
         const int row_token = local / c.group;
         const int row_head = local - row_token * c.group;
-        const bool wide = c.dim > 32;
         unsigned s_phase = 0, o_phase = 0;
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
-            const Item it = item_at(g, i);
+            const Item it = item_at<Boxes>(g, i);
             if (x >= it.slots) {
                 continue;
             }
@@ -309,20 +351,22 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
             const bool live = row_token < g.tokens_per_tile && token < c.queries;
             const bool idle = quad * 32 >= min(g.tokens_per_tile, c.queries - first_token) * c.group;
             float m = -INFINITY, sum = 0.0f;
-            MaskBytes<4> coming = mask_bytes<4>(c, it.b, it.end, it.key0);
-            float o[2][32];
+            MaskBytes<kKeys / 32> coming = mask_bytes<kKeys / 32>(c, it.b, it.end, it.key0);
+            float o[2 * Boxes][32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-                o[0][k] = 0.0f;
-                o[1][k] = 0.0f;
+            for (int j = 0; j < 2 * Boxes; ++j) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    o[j][k] = 0.0f;
+                }
             }
             // The products of the tile before, when they are done.
             const auto collect = [&](float keep) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (j == 0 || wide) {
+                for (int j = 0; j < 2 * Boxes; ++j) {
+                    if (32 * j < c.dim) {
                         float v[32];
-                        umma::load32(s_at + kOAt + 32 * j, v);
+                        umma::load32(s_at + Cfg::kO + 32 * j, v);
                         umma::load_wait(v);
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
@@ -333,8 +377,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
             };
             for (int t = 0; ok && t < it.tiles; ++t) {
                 uint32_t w[4];
-                tile_bits<4>(c, coming, it.end, it.key0 + t * kTile, w);
-                coming = mask_bytes<4>(c, it.b, it.end, it.key0 + (t + 1) * kTile);
+                tile_bits<kKeys / 32>(c, coming, it.end, it.key0 + t * kKeys, w);
+                coming = mask_bytes<kKeys / 32>(c, it.b, it.end, it.key0 + (t + 1) * kKeys);
                 ok = tma::mbar_wait(&s_full[x], s_phase);
                 if (!ok) {
                     break;
@@ -359,7 +403,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                     };
                     float now = m;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kKeys / 32; ++j) {
                         float s[32];
                         scores(j, s);
 #pragma unroll
@@ -376,7 +420,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                     const float shift = m == -INFINITY ? 0.0f : m;
                     float2 total = pair(0.0f);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kKeys / 32; ++j) {
                         float s[32];
                         scores(j, s);
 #pragma unroll
@@ -385,7 +429,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                             s[k + 1] = exp2_fast(s[k + 1] - shift);
                             total = total + make_float2(s[k], s[k + 1]);
                         }
-                        store_parts(s_at + 32 * j, s_at + kRestAt + 16 * j, s);
+                        store_parts(s_at + 32 * j, s_at + Cfg::kRest + 16 * j, s);
                     }
                     sum += total.x + total.y;
                     store_wait();
@@ -426,7 +470,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
                                                + ((static_cast<long long>(it.b) * c.queries + token) * c.kv_heads + it.head) * c.group * c.dim
                                                + row_head * c.dim;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 2 * Boxes; ++j) {
                     if (32 * j < c.dim) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
@@ -449,7 +493,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::dealloc<512>(tmem);
     }
 }
@@ -457,16 +501,29 @@ __global__ void __launch_bounds__(kForwardThreads, 1) forward_kernel(const __gri
 // --- backward ------------------------------------------------------------------------------------------
 
 constexpr int kWidth = 64;  // entries of the walk at a time
-constexpr int kBackwardThreads = 320;
-constexpr int kWalkedPlane = kWidth * umma::kRowBytes;
-constexpr int kOwnedBytes = kPlanes * kBox;
-constexpr int kWalkedBytes = kPlanes * kWalkedPlane;
 constexpr int kConstants = 2 * kWidth;
-constexpr int kStages = 2;
-constexpr int kBackwardSmem = 2 * kOwnedBytes + kStages * (2 * kWalkedBytes + kConstants * 4) + 1024;
-static_assert(kBackwardSmem <= kSmemMost - 1024, "shared memory");
-// Tensor memory: S (parts 0, 1 of P), part 2 of P, D (parts 0, 1 of dS), part 2 of dS, A0, A1.
-constexpr int kSRest = 64, kDAt = 96, kDRest = 160, kA0 = 192, kA1 = 256;
+
+// Heads of up to 64 values: the owned tiles stay in shared memory, a thread holds 32 columns. Wider ones: the parts of the owned
+// tiles take turns in it, the first for S, the second for D of every step, read again from L2; a thread holds 16 columns,
+// so that the results' 128 fit in the registers of sixteen warps.
+template <int Boxes>
+struct BackwardConfig {
+    static constexpr int kColumns = Boxes == 1 ? 32 : 16;
+    static constexpr int kParts = kWidth / kColumns;     // of a row
+    static constexpr int kWarps = 4 * kParts;
+    static constexpr int kThreads = 32 * (kWarps + 2);
+    static constexpr int kOwnedPlane = Boxes * kBox;
+    static constexpr int kOwnedBytes = kPlanes * kOwnedPlane;
+    static constexpr int kOwned = Boxes == 1 ? 2 : 1;    // owned tiles that are there at a time
+    static constexpr int kWalkedBox = kWidth * umma::kRowBytes;
+    static constexpr int kWalkedPlane = Boxes * kWalkedBox;
+    static constexpr int kWalkedBytes = kPlanes * kWalkedPlane;
+    static constexpr int kStages = Boxes == 1 ? 2 : 1;
+    static constexpr int kSmem = kOwned * kOwnedBytes + kStages * (2 * kWalkedBytes + kConstants * 4) + 1024;
+    // Tensor memory: S (parts 0, 1 of P), part 2 of P, D (parts 0, 1 of dS), part 2 of dS, A0, A1.
+    static constexpr int kSRest = 64, kD = 96, kDRest = 160, kA0 = 192, kA1 = 192 + Boxes * 64;
+    static_assert(kSmem <= kSmemMost - 1024 && kA1 + Boxes * 64 <= 512, "shared and tensor memory");
+};
 
 struct Backward {
     HeadMap x0, x1, y0, y1;
@@ -513,19 +570,23 @@ __device__ __forceinline__ Walk walk_at(const Backward& g, unsigned i)
     return it;
 }
 
-template <bool Rows>
-__global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __grid_constant__ Backward g)
+template <bool Rows, int Boxes>
+__global__ void __launch_bounds__(BackwardConfig<Boxes>::kThreads, 1) backward_kernel(const __grid_constant__ Backward g)
 {
+    using Cfg = BackwardConfig<Boxes>;
+    constexpr int kWarps = Cfg::kWarps;
+    constexpr int kStages = Cfg::kStages;
+    constexpr int kColumns = Cfg::kColumns;
     extern __shared__ unsigned char smem_base[];
     const uint32_t base = (tma::smem_addr(smem_base) + 1023u) & ~1023u;
     unsigned char* const generic = smem_base + (base - tma::smem_addr(smem_base));
-    const uint32_t ring = base + 2 * kOwnedBytes;
-    float* const constants = reinterpret_cast<float*>(generic + 2 * kOwnedBytes + kStages * 2 * kWalkedBytes);
+    const uint32_t ring = base + Cfg::kOwned * Cfg::kOwnedBytes;
+    float* const constants = reinterpret_cast<float*>(generic + Cfg::kOwned * Cfg::kOwnedBytes + kStages * 2 * Cfg::kWalkedBytes);
     __shared__ uint64_t x_full, x_empty, full[kStages], empty[kStages], s_full, d_full, p_ready, ds_ready, acc_full, acc_free, drain;
     __shared__ uint32_t tmem_slot;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::alloc<512>(&tmem_slot);
     }
     if (threadIdx.x == 0) {
@@ -537,10 +598,10 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
         }
         tma::mbar_init(&s_full, 1);
         tma::mbar_init(&d_full, 1);
-        tma::mbar_init(&p_ready, 8);
-        tma::mbar_init(&ds_ready, 8);
+        tma::mbar_init(&p_ready, kWarps);
+        tma::mbar_init(&ds_ready, kWarps);
         tma::mbar_init(&acc_full, 1);
-        tma::mbar_init(&acc_free, 8);
+        tma::mbar_init(&acc_free, kWarps);
         tma::mbar_init(&drain, 1);
         tma::fence_mbar_init();
     }
@@ -548,9 +609,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
         // Rows of a tile that no box writes (64 % group) are reduced over: zeros, once.
         const int used = g.walked_tokens * g.c.group;
         const int spare = kWidth - used;
-        for (int i = threadIdx.x; i < kStages * 2 * kPlanes * spare * 8; i += kBackwardThreads) {
+        for (int i = threadIdx.x; i < kStages * 2 * kPlanes * Boxes * spare * 8; i += Cfg::kThreads) {
             const int box = i / (spare * 8), at = i - box * spare * 8;
-            *reinterpret_cast<uint4*>(generic + 2 * kOwnedBytes + box * kWalkedPlane + (used + at / 8) * umma::kRowBytes + at % 8 * 16) =
+            *reinterpret_cast<uint4*>(generic + Cfg::kOwned * Cfg::kOwnedBytes + box * Cfg::kWalkedBox + (used + at / 8) * umma::kRowBytes + at % 8 * 16) =
                 make_uint4(0, 0, 0, 0);
         }
         tma::fence_proxy_async();
@@ -564,48 +625,65 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
     const Call& c = g.c;
     bool ok = true;
 
-    if (warp == 8) {
+    if (warp == kWarps) {
         // The TMA warp.
         asm volatile("fence.proxy.async.global;" ::: "memory");
-        const unsigned token_bytes = static_cast<unsigned>(c.group) * umma::kRowBytes * kPlanes;
-        const unsigned owned_bytes = 2 * (Rows ? g.owned_tokens * token_bytes : kOwnedBytes);
-        const unsigned walked_bytes = 2 * (Rows ? kWalkedBytes : g.walked_tokens * token_bytes) + (Rows ? 0 : kConstants * 4);
+        const unsigned token_bytes = static_cast<unsigned>(c.group) * umma::kRowBytes * kPlanes * Boxes;
+        const unsigned owned_bytes = Rows ? g.owned_tokens * token_bytes : Cfg::kOwnedBytes;  // of one
+        const unsigned walked_bytes = 2 * (Rows ? Cfg::kWalkedBytes : g.walked_tokens * token_bytes) + (Rows ? 0 : kConstants * 4);
         int stage = 0;
         unsigned phase = 0;
-        long long issued = 0, items = 0;
+        long long issued = 0, x_issued = 0;  // steps, loads of owned tiles
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Walk it = walk_at<Rows>(g, i);
             if (it.tiles == 0) {
                 continue;
             }
-            ok = tma::mbar_wait(&x_empty, (static_cast<unsigned>(items) & 1u) ^ 1u);
-            if (!ok) {
-                break;
-            }
             const int x_head = Rows ? it.head * c.group : it.head;
             const int y_head = Rows ? it.head : it.head * c.group;
-            if (umma::elect_one()) {
-                tma::mbar_arrive_expect_tx(&x_full, owned_bytes);
-                const int token = it.tile * (Rows ? g.owned_tokens : kTile);
-                for (int p = 0; p < kPlanes; ++p) {
-                    load_heads(base + p * kBox, g.x0, 0, x_head, token, p * c.batch + it.b, &x_full);
-                    load_heads(base + kOwnedBytes + p * kBox, g.x1, 0, x_head, token, p * c.batch + it.b, &x_full);
+            const int x_token = it.tile * (Rows ? g.owned_tokens : kTile);
+            // Both owned tiles (which < 0) or one, when the ones before are done with.
+            const auto load_owned = [&](int which) {
+                ok = tma::mbar_wait(&x_empty, (static_cast<unsigned>(x_issued) & 1u) ^ 1u);
+                if (ok && umma::elect_one()) {
+                    tma::mbar_arrive_expect_tx(&x_full, which < 0 ? 2 * owned_bytes : owned_bytes);
+                    for (int k = 0; k < 2; ++k) {
+                        if (which >= 0 && k != which) {
+                            continue;
+                        }
+                        const uint32_t to = base + (which < 0 ? k * Cfg::kOwnedBytes : 0);
+                        for (int p = 0; p < kPlanes; ++p) {
+                            for (int j = 0; j < Boxes; ++j) {
+                                load_heads(to + p * Cfg::kOwnedPlane + j * kBox, k == 0 ? g.x0 : g.x1, j * umma::kAtom, x_head, x_token, p * c.batch + it.b,
+                                           &x_full);
+                            }
+                        }
+                    }
                 }
+                __syncwarp();
+                x_issued += ok ? 1 : 0;
+            };
+            if (Cfg::kOwned == 2) {
+                load_owned(-1);
             }
-            __syncwarp();
-            ++items;
             for (int t = it.first; ok && t < it.first + it.tiles; ++t) {
-                ok = tma::mbar_wait(&empty[stage], phase ^ 1u);
+                if (Cfg::kOwned == 1) {
+                    load_owned(0);
+                }
+                ok = ok && tma::mbar_wait(&empty[stage], phase ^ 1u);
                 if (!ok) {
                     break;
                 }
                 if (umma::elect_one()) {
-                    const uint32_t y = ring + stage * 2 * kWalkedBytes;
+                    const uint32_t y = ring + stage * 2 * Cfg::kWalkedBytes;
                     const int token = t * (Rows ? kWidth : g.walked_tokens);
                     tma::mbar_arrive_expect_tx(&full[stage], walked_bytes);
                     for (int p = 0; p < kPlanes; ++p) {
-                        load_heads(y + p * kWalkedPlane, g.y0, 0, y_head, token, p * c.batch + it.b, &full[stage]);
-                        load_heads(y + kWalkedBytes + p * kWalkedPlane, g.y1, 0, y_head, token, p * c.batch + it.b, &full[stage]);
+                        for (int j = 0; j < Boxes; ++j) {
+                            const uint32_t to = y + p * Cfg::kWalkedPlane + j * Cfg::kWalkedBox;
+                            load_heads(to, g.y0, j * umma::kAtom, y_head, token, p * c.batch + it.b, &full[stage]);
+                            load_heads(to + Cfg::kWalkedBytes, g.y1, j * umma::kAtom, y_head, token, p * c.batch + it.b, &full[stage]);
+                        }
                     }
                     if constexpr (!Rows) {
                         const long long at = (static_cast<long long>(it.b) * c.kv_heads + it.head) * g.row_walks + t;
@@ -618,10 +696,13 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                     stage = 0;
                     phase ^= 1u;
                 }
+                if (Cfg::kOwned == 1) {
+                    load_owned(1);
+                }
             }
         }
         if (!ok) {  // the loads in flight land (bounded) before the shared memory is given up
-            bool drained = items == 0 || tma::mbar_wait(&x_full, static_cast<unsigned>(items - 1) & 1u);
+            bool drained = x_issued == 0 || tma::mbar_wait(&x_full, static_cast<unsigned>(x_issued - 1) & 1u);
             for (long long i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
                 drained = tma::mbar_wait(&full[i % kStages], static_cast<unsigned>(i / kStages) & 1u) && drained;
             }
@@ -629,7 +710,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                 atomicOr(g.fault, drained ? tma::kFaultWaitTimeout : tma::kFaultWaitTimeout | tma::kFaultDrainTimeout);
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == kWarps + 1) {
         // The MMA warp, one elected lane issues.
         const int steps = (c.dim + 15) / 16;
         const uint32_t score = umma::instruction(true, false, false, kTile, kWidth);
@@ -640,10 +721,11 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
         const auto scores = [&](int k, int y_stage, uint64_t* done) {
             if (umma::elect_one()) {
                 for (int p = 0; p < kProducts; ++p) {
-                    const uint64_t a = umma::desc_k(base + k * kOwnedBytes + mlp::part_a<float>(p) * kBox);
-                    const uint64_t b = umma::desc_k(ring + (2 * y_stage + k) * kWalkedBytes + mlp::part_b<float>(p) * kWalkedPlane);
+                    const uint64_t a = umma::desc_k(base + (Cfg::kOwned == 2 ? k * Cfg::kOwnedBytes : 0) + mlp::part_a<float>(p) * Cfg::kOwnedPlane);
+                    const uint64_t b = umma::desc_k(ring + (2 * y_stage + k) * Cfg::kWalkedBytes + mlp::part_b<float>(p) * Cfg::kWalkedPlane);
                     for (int s = 0; s < steps; ++s) {
-                        umma::mma(tmem + k * kDAt, a + s * umma::kStepK, b + s * umma::kStepK, score, p > 0 || s > 0);
+                        const uint64_t step = (s & 3) * umma::kStepK;
+                        umma::mma(tmem + k * Cfg::kD, a + step + (s >> 2) * (kBox >> 4), b + step + (s >> 2) * (Cfg::kWalkedBox >> 4), score, p > 0 || s > 0);
                     }
                 }
                 umma::commit(done);
@@ -652,18 +734,70 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
         };
         // A0 = dS Y0 (k = 0), A1 = P Y1 (k = 1), of this tile alone.
         const auto weighed = [&](int k, int y_stage) {
-            const uint32_t from = tmem + (k == 0 ? kDAt : 0), rest = tmem + (k == 0 ? kDRest : kSRest);
+            const uint32_t from = tmem + (k == 0 ? Cfg::kD : 0), rest = tmem + (k == 0 ? Cfg::kDRest : Cfg::kSRest);
             for (int p = 0; p < kProducts; ++p) {
-                const uint64_t b = umma::desc_mn<kWalkedPlane>(ring + (2 * y_stage + k) * kWalkedBytes + mlp::part_b<float>(p) * kWalkedPlane);
+                const uint64_t b = umma::desc_mn<Cfg::kWalkedBox>(ring + (2 * y_stage + k) * Cfg::kWalkedBytes + mlp::part_b<float>(p) * Cfg::kWalkedPlane);
 #pragma unroll
                 for (int s = 0; s < kWidth / 16; ++s) {
-                    mma_tmem(tmem + (k == 0 ? kA0 : kA1), part_at(from, rest, mlp::part_a<float>(p), s), b + umma::kStepMn * s, weigh, p > 0 || s > 0);
+                    mma_tmem(tmem + (k == 0 ? Cfg::kA0 : Cfg::kA1), part_at<kColumns>(from, rest, mlp::part_a<float>(p), s), b + umma::kStepMn * s, weigh, p > 0 || s > 0);
                 }
             }
         };
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Walk it = walk_at<Rows>(g, i);
             if (it.tiles == 0) {
+                continue;
+            }
+            if constexpr (Cfg::kOwned == 1) {
+                // The owned tiles take turns, so the steps follow each other.
+                const auto turn = [&](int k, uint64_t* done) {
+                    ok = tma::mbar_wait(&x_full, x_phase) && tma::mbar_wait(&full[stage], phase);
+                    if (ok) {
+                        x_phase ^= 1u;
+                        umma::fence_after_sync();
+                        scores(k, stage, done);
+                        if (umma::elect_one()) {
+                            umma::commit(&x_empty);
+                        }
+                        __syncwarp();
+                    }
+                };
+                for (int t = 0; ok && t < it.tiles; ++t) {
+                    turn(0, &s_full);
+                    if (ok) {
+                        turn(1, &d_full);
+                    }
+                    ok = ok && tma::mbar_wait(&p_ready, step_phase) && (t > 0 || tma::mbar_wait(&acc_free, acc_phase ^ 1u));
+                    if (!ok) {
+                        break;
+                    }
+                    umma::fence_after_sync();
+                    if constexpr (!Rows) {
+                        if (umma::elect_one()) {
+                            weighed(1, stage);
+                        }
+                        __syncwarp();
+                    }
+                    ok = tma::mbar_wait(&ds_ready, step_phase);
+                    if (!ok) {
+                        break;
+                    }
+                    step_phase ^= 1u;
+                    umma::fence_after_sync();
+                    if (umma::elect_one()) {
+                        weighed(0, stage);
+                        umma::commit(&empty[stage]);
+                        if (t + 1 == it.tiles) {
+                            umma::commit(&acc_full);
+                        }
+                    }
+                    __syncwarp();
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                acc_phase ^= 1u;
                 continue;
             }
             ok = tma::mbar_wait(&x_full, x_phase) && tma::mbar_wait(&full[stage], phase);
@@ -736,7 +870,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
             }
         }
     } else {
-        // A thread per owned row and 32 columns of scores, and of the results: warps 0 to 3 the first, 4 to 7 the others.
+        // A thread per owned row and kColumns columns of scores, and 32 of the results: warps 4 k to 4 k + 3 the k-th.
         const int part = warp >> 2;
         const int local = (warp & 3) * 32 + lane;
         const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -808,36 +942,37 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                     tile_bits<2>(c, mask, it.end, t * kWidth, w);
                     mask = mask_bytes<2>(c, it.b, it.end, (t + 1) * kWidth);
                 }
-                const uint32_t word = Rows ? (part == 0 ? w[0] : w[1]) : counts ? 0xffffffffu : 0u;
+                constexpr uint32_t kAll = kColumns == 32 ? 0xffffffffu : (1u << (kColumns % 32)) - 1u;
+                const uint32_t word = (Rows ? w[part * kColumns / 32] >> (part * kColumns % 32) : counts ? 0xffffffffu : 0u) & kAll;
                 ok = tma::mbar_wait(&full[stage], phase) && tma::mbar_wait(&s_full, step_phase);
                 if (!ok) {
                     break;
                 }
                 umma::fence_after_sync();
-                const float* less = constants + stage * kConstants + part * 32;  // -lse, then -delta
+                const float* less = constants + stage * kConstants + part * kColumns;  // -lse, then -delta
                 if constexpr (!Rows) {
                     if (t > it.first) {  // its commit came before these scores'
-                        collect(kA1, a1);
+                        collect(Cfg::kA1, a1);
                     }
                 }
-                float p[32];
-                umma::load32(at + part * 32, p);
+                float p[kColumns];
+                umma::load_run(at + part * kColumns, p);
                 umma::load_wait(p);
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
+                for (int k = 0; k < kColumns; k += 2) {
                     const float2 l = Rows ? shift : *reinterpret_cast<const float2*>(less + k);
                     const float2 e = fma2(make_float2(p[k], p[k + 1]), pair(g.factor), l);
                     p[k] = exp2_fast(e.x);
                     p[k + 1] = exp2_fast(e.y);
                 }
-                if (word != 0xffffffffu) {
+                if (word != kAll) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
+                    for (int k = 0; k < kColumns; ++k) {
                         p[k] = (word >> k & 1u) != 0 ? p[k] : 0.0f;
                     }
                 }
                 if constexpr (!Rows) {
-                    store_parts(at + part * 32, at + kSRest + part * 16, p);
+                    store_parts(at + part * kColumns, at + Cfg::kSRest + part * (kColumns / 2), p);
                     store_wait();
                 }
                 umma::fence_before_sync();
@@ -852,25 +987,25 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                 step_phase ^= 1u;
                 umma::fence_after_sync();
                 if (t > it.first) {
-                    collect(kA0, a0);
+                    collect(Cfg::kA0, a0);
                 }
-                float d[32];
-                umma::load32(at + kDAt + part * 32, d);
+                float d[kColumns];
+                umma::load_run(at + Cfg::kD + part * kColumns, d);
                 umma::load_wait(d);
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
+                for (int k = 0; k < kColumns; k += 2) {
                     const float2 l = Rows ? delta : *reinterpret_cast<const float2*>(less + kWidth + k);
                     const float2 v = (make_float2(d[k], d[k + 1]) + l) * make_float2(p[k], p[k + 1]);
                     d[k] = v.x;
                     d[k + 1] = v.y;
                 }
-                if (word != 0xffffffffu) {  // a key that does not count may have made D anything
+                if (word != kAll) {  // a key that does not count may have made D anything
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
+                    for (int k = 0; k < kColumns; ++k) {
                         d[k] = (word >> k & 1u) != 0 ? d[k] : 0.0f;
                     }
                 }
-                store_parts(at + kDAt + part * 32, at + kDRest + part * 16, d);
+                store_parts(at + Cfg::kD + part * kColumns, at + Cfg::kDRest + part * (kColumns / 2), d);
                 store_wait();
                 umma::fence_before_sync();
                 __syncwarp();
@@ -892,9 +1027,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
                 }
                 acc_phase ^= 1u;
                 umma::fence_after_sync();
-                collect(kA0, a0);
+                collect(Cfg::kA0, a0);
                 if constexpr (!Rows) {
-                    collect(kA1, a1);
+                    collect(Cfg::kA1, a1);
                 }
                 umma::fence_before_sync();
                 __syncwarp();
@@ -934,7 +1069,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) backward_kernel(const __g
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == 8) {
+    if (warp == kWarps) {
         umma::dealloc<512>(tmem);
     }
 }
@@ -1104,6 +1239,8 @@ void launch(K kernel, const G& g, int threads, int smem, cudaStream_t stream)
     launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, g);
 }
 
+int forward_keys(const Call& c) { return c.dim <= 64 ? ForwardConfig<1>::kKeys : ForwardConfig<2>::kKeys; }
+
 struct ForwardPlan {
     Planes q, k, v;
     int row_items = 0, splits = 1, split_tiles = 0;
@@ -1115,8 +1252,9 @@ struct ForwardPlan {
         q = planes(arena, c, c.queries, c.kv_heads * c.group);
         k = planes(arena, c, c.keys, c.kv_heads);
         v = planes(arena, c, c.keys, c.kv_heads);
-        row_items = pieces(pieces(c.queries, kTile / c.group), 2);
-        cut(c.pairs() * row_items, pieces(c.keys, kTile), 2.0, splits, split_tiles);
+        const int slots = c.dim <= 64 ? ForwardConfig<1>::kSlots : ForwardConfig<2>::kSlots;
+        row_items = pieces(pieces(c.queries, kTile / c.group), slots);
+        cut(c.pairs() * row_items, pieces(c.keys, forward_keys(c)), 2.0, splits, split_tiles);
         if (splits > 1) {
             const std::size_t all = static_cast<std::size_t>(c.pairs()) * c.rows() * splits;
             partial = arena.take(all * c.dim * sizeof(float));
@@ -1181,9 +1319,13 @@ void split_forward(const Call& c, char* work, cudaStream_t stream)
     g.part_stats = reinterpret_cast<float2*>(work + plan.stats);
     g.fault = device_fault_word();
     g.q = plane_map(c, plan.q, work, c.group, g.tokens_per_tile);
-    g.k = plane_map(c, plan.k, work, 1, kTile);
-    g.v = plane_map(c, plan.v, work, 1, kTile);
-    launch(forward_kernel, g, kForwardThreads, kForwardSmem, stream);
+    g.k = plane_map(c, plan.k, work, 1, forward_keys(c));
+    g.v = plane_map(c, plan.v, work, 1, forward_keys(c));
+    if (c.dim <= 64) {
+        launch(forward_kernel<1>, g, ForwardConfig<1>::kThreads, ForwardConfig<1>::kSmem, stream);
+    } else {
+        launch(forward_kernel<2>, g, ForwardConfig<2>::kThreads, ForwardConfig<2>::kSmem, stream);
+    }
     if (plan.splits > 1) {
         join_splits(c, g.partial, g.part_stats, plan.splits, stream);
     }
@@ -1218,7 +1360,11 @@ void split_backward(const Call& c, char* work, cudaStream_t stream)
     g.items = item_count(c.pairs() * plan.key_tiles * plan.row_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dk);
     g.partial1 = reinterpret_cast<float*>(work + plan.dv);
-    launch(backward_kernel<false>, g, kBackwardThreads, kBackwardSmem, stream);
+    if (c.dim <= 64) {
+        launch(backward_kernel<false, 1>, g, BackwardConfig<1>::kThreads, BackwardConfig<1>::kSmem, stream);
+    } else {
+        launch(backward_kernel<false, 2>, g, BackwardConfig<2>::kThreads, BackwardConfig<2>::kSmem, stream);
+    }
     // dq.
     g.x0 = plane_map(c, plan.q, work, c.group, plan.owned_tokens);
     g.x1 = plane_map(c, plan.dout, work, c.group, plan.owned_tokens);
@@ -1229,7 +1375,11 @@ void split_backward(const Call& c, char* work, cudaStream_t stream)
     g.part_tiles = plan.key_span;
     g.items = item_count(c.pairs() * plan.row_tiles * plan.key_parts);
     g.partial0 = reinterpret_cast<float*>(work + plan.dq);
-    launch(backward_kernel<true>, g, kBackwardThreads, kBackwardSmem, stream);
+    if (c.dim <= 64) {
+        launch(backward_kernel<true, 1>, g, BackwardConfig<1>::kThreads, BackwardConfig<1>::kSmem, stream);
+    } else {
+        launch(backward_kernel<true, 2>, g, BackwardConfig<2>::kThreads, BackwardConfig<2>::kSmem, stream);
+    }
     Sums sums;
     if (plan.row_parts > 1) {
         sums.add(reinterpret_cast<const float*>(work + plan.dk), plan.row_parts, true, c.dk, c.scale);
