@@ -1,8 +1,9 @@
 // Attention to states of another length: the C ABI (include/spectral_b200.h: spectral_cross_attention and
 // its backward), the float32 kernels, and the kernels around the 16-bit ones.
 //
-// Float32 products run on the CUDA cores: FP32 multiply-adds two to an instruction, tiles of rows x 64 keys,
-// operands staged through shared memory as float32 with what must not count as zeros. A pass over the keys keeps the
+// Float32 calls that the tensor-core kernels (attention_tc32.cu) do not take, those of 9 to 16 rows per key head and
+// of more than 64 query heads to one, run on the CUDA cores: FP32 multiply-adds two to an instruction, tiles of rows x 64
+// keys, operands staged through shared memory as float32 with what must not count as zeros. A pass over the keys keeps the
 // running maximum and sum of each row. The backward pass recomputes the scores twice, once for the
 // keys' gradients (a CTA per 64 keys, a loop over rows) and once for the queries' (a CTA per 64 rows, a loop over
 // keys): every sum has one owner, so nothing is atomic and equal inputs give equal bits.
@@ -251,7 +252,7 @@ struct Parts {
 
 // Forward: 16 R rows per CTA, thread (row group, column) of a 16 x 16 grid.
 template <int Dim, int R>
-__global__ void __launch_bounds__(kThreads, R == 8 || Dim == 128 ? 1 : 2) forward_kernel(const Call c, const Parts parts)
+__global__ void __launch_bounds__(kThreads, Dim == 128 ? 1 : 2) forward_kernel(const Call c, const Parts parts)
 {
     constexpr int kRows = 16 * R;
     extern __shared__ __align__(16) float shared[];
@@ -345,15 +346,15 @@ __global__ void __launch_bounds__(kThreads, R == 8 || Dim == 128 ? 1 : 2) forwar
 }
 
 // Scores of a tile, turned into p and p (dp - delta): what both backward kernels need.
-template <int Dim, int R>
+template <int Dim>
 __device__ __forceinline__ void score_gradients(const float* sq, const float* sk, const float* sv, const float* sdo, int dim, int row0, int col,
-                                                float scale, unsigned long long valid, const float2 (&stats)[R], const float (&delta)[R],
-                                                float (&p)[R][4], float (&ds)[R][4])
+                                                float scale, unsigned long long valid, const float2 (&stats)[4], const float (&delta)[4],
+                                                float (&p)[4][4], float (&ds)[4][4])
 {
-    products<Dim, R>(sq, sk, dim, row0, col, p);
-    products<Dim, R>(sdo, sv, dim, row0, col, ds);
+    products<Dim, 4>(sq, sk, dim, row0, col, p);
+    products<Dim, 4>(sdo, sv, dim, row0, col, ds);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const bool ok = (valid >> (col + 16 * j) & 1) != 0;
@@ -364,11 +365,10 @@ __device__ __forceinline__ void score_gradients(const float* sq, const float* sk
 }
 
 // m and 1 / sum p, and delta, of rows row0 .. of the tile at `first`; zeros past the end and for empty rows.
-template <int R>
-__device__ __forceinline__ void row_constants(const Call& c, long long at, long long first, int row0, float2 (&stats)[R], float (&delta)[R])
+__device__ __forceinline__ void row_constants(const Call& c, long long at, long long first, int row0, float2 (&stats)[4], float (&delta)[4])
 {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const long long r = first + row0 + i;
         stats[i] = make_float2(0.0f, 0.0f);
         delta[i] = 0.0f;
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, Dim == 128 ? 1 : 2) keys_backward_ke
         float delta[4], p[4][4], ds[4][4];
         row_constants(c, at, first, row0, stats, delta);
         __syncthreads();
-        score_gradients<Dim, 4>(sq, sk, sv, sdo, c.dim, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
+        score_gradients<Dim>(sq, sk, sv, sdo, c.dim, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -452,36 +452,34 @@ __global__ void __launch_bounds__(kThreads, Dim == 128 ? 1 : 2) keys_backward_ke
     }
 }
 
-// 16 R rows per CTA.
-template <int Dim, int R>
-__global__ void __launch_bounds__(kThreads, R == 8 || Dim == 128 ? 1 : 2) rows_backward_kernel(const Call c, const Parts parts)
+template <int Dim>
+__global__ void __launch_bounds__(kThreads, Dim == 128 ? 1 : 2) rows_backward_kernel(const Call c, const Parts parts)
 {
-    constexpr int kRows = 16 * R;
     extern __shared__ __align__(16) float shared[];
     float* sk = shared;
     float* sv = sk + kKeys * kPitch<Dim>;
     float* sq = sv + kKeys * kPitch<Dim>;
-    float* sdo = sq + kRows * kPitch<Dim>;
-    float* sds = sdo + kRows * kPitch<Dim>;
+    float* sdo = sq + 64 * kPitch<Dim>;
+    float* sds = sdo + 64 * kPitch<Dim>;
     __shared__ unsigned votes[2];
     const int col = threadIdx.x & 15;
-    const int row0 = (threadIdx.x >> 4) * R;
+    const int row0 = (threadIdx.x >> 4) * 4;
     const long long at = blockIdx.y;
     const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
-    const long long first = static_cast<long long>(blockIdx.x) * kRows;
+    const long long first = static_cast<long long>(blockIdx.x) * 64;
     const int part = blockIdx.z;
     allow_next_grid();
     wait_for_previous_grid();
     const Strides dense{static_cast<long long>(c.queries) * c.kv_heads * c.group * c.dim, static_cast<long long>(c.kv_heads) * c.group * c.dim,
                         c.dim};
-    load_rows<Dim, kRows>(sq, c, c.q, c.qs, parts.vectors, b, head, first);
-    load_rows<Dim, kRows>(sdo, c, c.dout, dense, parts.vectors, b, head, first);
-    float2 stats[R];
-    float delta[R];
+    load_rows<Dim, 64>(sq, c, c.q, c.qs, parts.vectors, b, head, first);
+    load_rows<Dim, 64>(sdo, c, c.dout, dense, parts.vectors, b, head, first);
+    float2 stats[4];
+    float delta[4];
     row_constants(c, at, first, row0, stats, delta);
-    float2 dq[R][kPairs<Dim>];
+    float2 dq[4][kPairs<Dim>];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int p = 0; p < kPairs<Dim>; ++p) {
             dq[i][p] = pair(0.0f);
@@ -497,20 +495,20 @@ __global__ void __launch_bounds__(kThreads, R == 8 || Dim == 128 ? 1 : 2) rows_b
         load_keys<Dim>(sk, c, c.k, c.ks, parts.vectors, b, head, key0, valid);
         load_keys<Dim>(sv, c, c.v, c.vs, parts.vectors, b, head, key0, valid);
         __syncthreads();
-        float p[R][4], ds[R][4];
-        score_gradients<Dim, R>(sq, sk, sv, sdo, c.dim, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
+        float p[4][4], ds[4][4];
+        score_gradients<Dim>(sq, sk, sv, sdo, c.dim, row0, col, c.scale * kLog2e, valid, stats, delta, p, ds);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 sds[(row0 + i) * kScorePitch + col + 16 * j] = ds[i][j];
             }
         }
         __syncwarp();
-        weigh_rows<Dim, R>(sds, sk, row0, col, dq);
+        weigh_rows<Dim, 4>(sds, sk, row0, col, dq);
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const long long r = first + row0 + i;
         if (r >= c.rows()) {
             continue;
@@ -692,16 +690,8 @@ void with_dim(int dim, F&& f)
     }
 }
 
-// Rows per CTA: 128, where that leaves fewer tiles than SMs 64, and where there are no more (a single query's) 16.
-// Eight rows a thread read less shared memory per product than four.
-int tile_rows(const Call& c, bool back)
-{
-    if (c.rows() <= 16 && !back) {
-        return 16;
-    }
-    const bool fits = !back || c.dim <= 64;
-    return fits && c.pairs() * pieces(c.rows(), 128) * pieces(c.keys, 512) >= kSms ? 128 : 64;
-}
+// Rows per forward CTA: 64, or 16 where there are no more.
+int forward_rows(const Call& c) { return c.rows() <= 16 ? 16 : 64; }
 
 // Parts of an axis of `length` in tiles of 64, so that `tiles` CTAs per part fill the GPU about twice; a part's
 // span is a whole number of tiles.
@@ -722,7 +712,7 @@ struct ForwardPlan {
 
     explicit ForwardPlan(const Call& c)
     {
-        parts = split(c.pairs() * pieces(c.rows(), tile_rows(c, false)), c.keys);
+        parts = split(c.pairs() * pieces(c.rows(), forward_rows(c)), c.keys);
         if (parts.count > 1) {
             const std::size_t rows = static_cast<std::size_t>(c.pairs()) * c.rows() * parts.count;
             partial = arena.take(rows * c.dim * sizeof(float));
@@ -731,13 +721,14 @@ struct ForwardPlan {
     }
 };
 
-// Float32 calls whose products are worth splitting: more rows than a few.
-bool on_tensor_cores(const Call& c) { return c.group <= 64 && c.rows() > 16 && c.keys > 0; }
+// Float32 calls that run on the tensor cores: those whose tiles hold a token's heads, forward with more rows than a few (12
+// rows over 8192 keys, 2 x 8 heads of 64: 96 us there, 67 here; backward 190 and 400).
+bool on_tensor_cores(const Call& c, bool back) { return c.group <= 64 && c.keys > 0 && (back || c.rows() > 16); }
 
 std::size_t forward_workspace(const Call& c)
 {
     return few_rows(c)                       ? few_workspace(c)
-           : c.dtype != SPECTRAL_FLOAT32 ? tensor_forward_workspace(c) : on_tensor_cores(c) ? split_forward_workspace(c) : ForwardPlan(c).arena.size();
+           : c.dtype != SPECTRAL_FLOAT32 ? tensor_forward_workspace(c) : on_tensor_cores(c, false) ? split_forward_workspace(c) : ForwardPlan(c).arena.size();
 }
 
 struct BackwardPlan {
@@ -750,7 +741,7 @@ struct BackwardPlan {
         const std::size_t rows = static_cast<std::size_t>(c.pairs()) * c.rows();
         const std::size_t keys = static_cast<std::size_t>(c.pairs()) * c.keys;
         delta = arena.take(rows * sizeof(float));
-        of_keys = split(c.pairs() * pieces(c.rows(), tile_rows(c, true)), c.keys);
+        of_keys = split(c.pairs() * pieces(c.rows(), 64), c.keys);
         of_rows = split(c.pairs() * pieces(c.keys, 64), c.rows());
         if (of_keys.count > 1) {
             dq = arena.take(rows * c.dim * of_keys.count * sizeof(float));
@@ -789,15 +780,13 @@ void forward(const Call& c, char* work, cudaStream_t stream)
     plan.parts.first = reinterpret_cast<float*>(work + plan.partial);
     plan.parts.stats = reinterpret_cast<float2*>(work + plan.stats);
     plan.parts.vectors = in_vectors(c, {c.q, c.k, c.v}, {&c.qs, &c.ks, &c.vs});
-    const int rows = tile_rows(c, false);
+    const int rows = forward_rows(c);
     const dim3 grid(pieces(c.rows(), rows), static_cast<unsigned>(c.pairs()), plan.parts.count);
     with_dim(c.dim, [&](auto d) {
         constexpr int Dim = decltype(d)::value;
         const std::size_t smem = ((rows + 2 * kKeys) * kPitch<Dim> + rows * kScorePitch) * sizeof(float);
         if (rows == 16) {
             launch(forward_kernel<Dim, 1>, grid, smem, stream, c, plan.parts);
-        } else if (rows == 128) {
-            launch(forward_kernel<Dim, 8>, grid, smem, stream, c, plan.parts);
         } else {
             launch(forward_kernel<Dim, 4>, grid, smem, stream, c, plan.parts);
         }
@@ -822,16 +811,8 @@ void backward(Call c, char* work, cudaStream_t stream)
         constexpr std::size_t kScores = 64 * kScorePitch * sizeof(float);
         launch(keys_backward_kernel<Dim>, dim3(pieces(c.keys, 64), static_cast<unsigned>(c.pairs()), plan.of_rows.count), tiles + 2 * kScores, stream,
                c, plan.of_rows);
-        const int rows = tile_rows(c, true);
-        const dim3 grid(pieces(c.rows(), rows), static_cast<unsigned>(c.pairs()), plan.of_keys.count);
-        const std::size_t smem = (2 * (kKeys + rows) * kPitch<Dim> + rows * kScorePitch) * sizeof(float);
-        if constexpr (Dim <= 64) {
-            if (rows == 128) {
-                launch(rows_backward_kernel<Dim, 8>, grid, smem, stream, c, plan.of_keys);
-                return;
-            }
-        }
-        launch(rows_backward_kernel<Dim, 4>, grid, smem, stream, c, plan.of_keys);
+        launch(rows_backward_kernel<Dim>, dim3(pieces(c.rows(), 64), static_cast<unsigned>(c.pairs()), plan.of_keys.count), tiles + kScores, stream, c,
+               plan.of_keys);
     });
     Sums sums;
     if (plan.of_rows.count > 1) {
@@ -975,7 +956,7 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
         }
         if (few_rows(c)) {
             few_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
-        } else if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c)) {
+        } else if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c, false)) {
             split_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
         } else if (dtype == SPECTRAL_FLOAT32) {
             forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
@@ -1008,7 +989,7 @@ extern "C" int spectral_cross_attention_backward_workspace(const void* dout, con
     c.v = v;
     *count = 0;
     if (c.pairs() * c.rows() > 0 && keys > 0) {
-        *count = (dtype != SPECTRAL_FLOAT32 ? tensor_backward_workspace(c) : on_tensor_cores(c) ? split_backward_workspace(c) : BackwardPlan(c).arena.size()) / 8;
+        *count = (dtype != SPECTRAL_FLOAT32 ? tensor_backward_workspace(c) : on_tensor_cores(c, true) ? split_backward_workspace(c) : BackwardPlan(c).arena.size()) / 8;
     }
     return SPECTRAL_OK;
 }
@@ -1075,7 +1056,7 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         c.dk = dk;
         c.dv = dv;
         c.scale = scale;
-        if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c)) {
+        if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c, true)) {
             split_backward(c, static_cast<char*>(work), s);
         } else if (dtype == SPECTRAL_FLOAT32) {
             backward(c, static_cast<char*>(work), s);
