@@ -559,31 +559,51 @@ __global__ void __launch_bounds__(kThreads) row_products_kernel(const Call c)
     }
 }
 
-// A thread per result value.
-template <class T>
+// V values of a row per thread.
+template <class T, int V>
 __global__ void __launch_bounds__(kThreads) add_parts_kernel(const Call c, const __grid_constant__ Sums sums)
 {
     allow_next_grid();
     wait_for_previous_grid();
     const Sum& job = sums.job[blockIdx.y];
     const float* __restrict__ partial = job.partial;
+    T* __restrict__ result = static_cast<T*>(job.result);
     const bool of_keys = job.of_keys;
     const int parts = job.parts;
-    const long long count = of_keys ? c.keys : c.rows();
-    const long long all = c.pairs() * count * c.dim;
-    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * kThreads) {
-        float sum = 0.0f;
-#pragma unroll 4
+    const float factor = job.factor;
+    const unsigned per_row = static_cast<unsigned>(c.dim / V);
+    const unsigned count = of_keys ? c.keys : static_cast<unsigned>(c.rows());
+    const long long rows = c.pairs() * count;
+    const long long all = rows * c.dim;
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < rows * per_row; i += static_cast<long long>(gridDim.x) * kThreads) {
+        Floats<V> sum;
+        sum.fill(0.0f);
         for (int p = 0; p < parts; ++p) {
-            sum += partial[p * all + i];
+            const Floats<V> v = widen(*reinterpret_cast<const Vec<float, V>*>(partial + p * all + i * V));
+#pragma unroll
+            for (int j = 0; j < Floats<V>::kPairs; ++j) {
+                sum.p[j] = sum.p[j] + v.p[j];
+            }
         }
-        const long long row = i / c.dim;
-        const int d = static_cast<int>(i - row * c.dim);
-        const long long at = row / count;
-        const long long r = row - at * count;
-        const int b = static_cast<int>(at / c.kv_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.kv_heads);
-        const long long to = of_keys ? ((static_cast<long long>(b) * c.keys + r) * c.kv_heads + head) * c.dim : c.row_at(b, head, r);
-        static_cast<T*>(job.result)[to + d] = from_float<T>(sum * job.factor);
+#pragma unroll
+        for (int j = 0; j < Floats<V>::kPairs; ++j) {
+            sum.p[j] = sum.p[j] * pair(factor);
+        }
+        long long row, at;
+        if (rows * per_row < (1LL << 32)) {
+            row = static_cast<unsigned>(i) / per_row;
+            at = static_cast<unsigned>(row) / count;
+        } else {
+            row = i / per_row;
+            at = row / count;
+        }
+        const int d = static_cast<int>(i - row * per_row) * V;
+        const int r = static_cast<int>(row - at * count);
+        const int b = static_cast<int>(at) / c.kv_heads, head = static_cast<int>(at) - b * c.kv_heads;
+        const int token = of_keys ? r : r / c.group;
+        const long long to = of_keys ? ((static_cast<long long>(b) * c.keys + r) * c.kv_heads + head) * c.dim
+                                     : ((static_cast<long long>(b) * c.queries + token) * c.kv_heads + head) * c.group * c.dim + (r - token * c.group) * c.dim;
+        *reinterpret_cast<Vec<T, V>*>(result + to + d) = narrow<T>(sum);
     }
 }
 
@@ -653,9 +673,16 @@ void add_parts(const Call& c, const Sums& sums, cudaStream_t stream)
     if (sums.count == 0) {
         return;
     }
-    const long long all = c.pairs() * std::max<long long>(c.keys, c.rows()) * c.dim;
+    bool fours = c.dim % 4 == 0;
+    for (int i = 0; i < sums.count; ++i) {
+        fours = fours && aligned_to(sums.job[i].result, 4 * dtype_size(c.dtype));
+    }
+    const long long all = c.pairs() * std::max<long long>(c.keys, c.rows()) * c.dim / (fours ? 4 : 1);
     const dim3 grid(static_cast<unsigned>(std::min<long long>((all + kThreads - 1) / kThreads, 148 * 16)), sums.count);
-    with_dtype(c.dtype, [&](auto t) { launch_pdl(add_parts_kernel<decltype(t)>, grid, dim3(kThreads), 0, stream, c, sums); });
+    with_dtype(c.dtype, [&](auto t) {
+        using T = decltype(t);
+        launch_pdl(fours ? add_parts_kernel<T, 4> : add_parts_kernel<T, 1>, grid, dim3(kThreads), 0, stream, c, sums);
+    });
 }
 
 void join_splits(const Call& c, const float* partial, const float2* stats, int splits, cudaStream_t stream)
