@@ -879,38 +879,23 @@ __global__ void __launch_bounds__(BackwardConfig<Boxes>::kThreads, 1) backward_k
         const bool holds = part * 32 < c.dim;
         int stage = 0;
         unsigned phase = 0, step_phase = 0, acc_phase = 0;
-        // A row's constants are fetched an item ahead.
-        const auto constants_of = [&](unsigned i) {
-            float2 v = pair(0.0f);
-            if (i < g.items) {
-                const unsigned r = i / g.owned;
-                const int token = static_cast<int>(i - r * g.owned) * g.owned_tokens + row_token;
-                if (row_token < g.owned_tokens && token < c.queries) {
-                    const int tile = token / g.walked_tokens;
-                    const float* at = g.constants + (static_cast<long long>(r / g.parts) * g.row_walks + tile) * kConstants
-                                      + (token - tile * g.walked_tokens) * c.group + row_head;
-                    v = make_float2(at[0], at[kWidth]);
-                }
-            }
-            return v;
-        };
-        float2 coming = pair(0.0f);
-        if constexpr (Rows) {
-            coming = constants_of(blockIdx.x);
-        }
         for (unsigned i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
             const Walk it = walk_at<Rows>(g, i);
             const long long pair_at = static_cast<long long>(it.b) * c.kv_heads + it.head;
             // Rows: this row's -lse and -delta. Keys: whether this key counts.
-            const float2 shift = pair(coming.x), delta = pair(coming.y);
-            if constexpr (Rows) {
-                coming = constants_of(i + gridDim.x);
-            }
+            float2 shift = pair(0.0f), delta = pair(0.0f);
             bool counts = true;
             const int token = it.tile * g.owned_tokens + row_token;
             const int row = Rows ? token * c.group + row_head : it.tile * kTile + local;
             const bool live = Rows ? row_token < g.owned_tokens && token < c.queries : row < c.keys;
-            if constexpr (!Rows) {
+            if constexpr (Rows) {
+                if (live) {
+                    const int tile = token / g.walked_tokens;
+                    const float* from = g.constants + (pair_at * g.row_walks + tile) * kConstants + (token - tile * g.walked_tokens) * c.group + row_head;
+                    shift = pair(from[0]);
+                    delta = pair(from[kWidth]);
+                }
+            } else {
                 counts = row < it.end && (c.mask == nullptr || c.mask[static_cast<long long>(it.b) * c.keys + row] != 0);
             }
             float a0[32], a1[Rows ? 1 : 32];
