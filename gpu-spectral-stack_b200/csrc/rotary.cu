@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = SPECTRAL_HEAD_DIM_MAX;
-constexpr int kTableBytes = 40 * 1024;  // places and tables, at most
+constexpr int kTableBytes = 40 * 1024;  // places, positions and tables, at most
 
 // Heads a lane works on at a time, while it waits for as many more.
 __host__ __device__ constexpr int rows_in_flight(int units, bool back) { return units > 1 ? (back ? 1 : 2) : back ? 2 : 4; }
@@ -59,12 +59,13 @@ struct Plan {
     int per_axis = 0;  // pairs
     int table_pitch = 0;    // pairs of a token in the table, a multiple of 4
     int table_columns = 1;  // the power of two from there on
+    int token_bytes = 8;    // of a token's place and positions
     bool neighbours = false;
     float eps = 0.0f;
     double turns[kMaxDim / 2];  // angle per position, in turns, of an axis's pairs
 };
 
-// (cos, sin) of a fraction of a turn between -1/2 and 1/2. For results rounded to 16 bits the hardware's functions on
+// (cos, sin) of a fraction of a turn between -1/2 and 1/2 (or just past it). For results rounded to 16 bits the hardware's functions on
 // [-pi, pi], off by 2^-20 at most, do.
 template <class T>
 __device__ __forceinline__ float2 unit(float turn)
@@ -92,11 +93,9 @@ __device__ __forceinline__ float turn_of(P position, const Frequency& f)
 {
     if constexpr (std::is_same_v<P, float>) {
         const float a = position * f.high;
-        const float rest = fmaf(position, f.low, fmaf(position, f.high, -a));
-        const float turn = (a - rintf(a)) + rest;
-        return turn - rintf(turn);
+        return (a - rintf(a)) + fmaf(position, f.low, fmaf(position, f.high, -a));
     } else {
-        const double a = static_cast<double>(position) * f.turns;
+        const double a = position * f.turns;
         return static_cast<float>(a - rint(a));
     }
 }
@@ -138,10 +137,14 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
     const int n = plan.per_axis;
     const int pitch = plan.table_pitch;
     const int span = s.tile_tokens;
-    // Of each token of a tile: where it starts, where its positions are, the cosines of its pairs, the sines.
+    // Of each token of a tile: where it starts, its positions (floats, or whole numbers in 64 bits), the cosines of its
+    // pairs, the sines.
     auto* const places = reinterpret_cast<long long*>(smem);
-    auto* const position_places = places + span;
-    auto* const cosines = reinterpret_cast<float*>(smem + static_cast<size_t>(span) * 16);
+    auto* const whole_positions = reinterpret_cast<double*>(places + span);
+    auto* const float_positions = reinterpret_cast<float*>(places + span);
+    // (on 16 bytes: the tables are read in vectors)
+    auto* const cosines = reinterpret_cast<float*>(smem + (static_cast<size_t>(span) * plan.token_bytes + 15) / 16 * 16);
+    const bool floats = s.position_type == SPECTRAL_POSITIONS_FLOAT32;
 
     const int lane = threadIdx.x & 31;
     const int sub = lane & (lanes - 1);
@@ -181,8 +184,8 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
     // This thread's column of the table: one pair, every `table_rows`-th token.
     const int column = threadIdx.x % plan.table_columns;
     const int table_rows = kThreads / plan.table_columns;
-    const int column_axis = column / n;
-    Frequency frequency{column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0, 0.0f, 0.0f};
+    const int column_axis = column < rotated / 2 ? column / n : 0;
+    Frequency frequency{column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0, 0.0f, 0.0f};  // 0: not turned
     frequency.high = static_cast<float>(frequency.turns);
     frequency.low = static_cast<float>(frequency.turns - frequency.high);
     allow_next_grid();
@@ -219,7 +222,19 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
             const long long b = s.total < (1LL << 31) ? static_cast<unsigned>(token) / static_cast<unsigned>(s.tokens) : token / s.tokens;
             const long long in = token - b * s.tokens;
             places[t] = b * s.stride[0] + in * s.stride[1];
-            position_places[t] = b * s.position_stride[0] + in * s.position_stride[1];
+            if (rotated > 0) {
+                const long long at = b * s.position_stride[0] + in * s.position_stride[1];
+                for (int axis = 0; axis < plan.axes; ++axis) {
+                    const long long from = at + axis * s.position_stride[2];
+                    if (floats) {
+                        float_positions[axis * span + t] = static_cast<const float*>(s.positions)[from];
+                    } else {
+                        whole_positions[axis * span + t] = s.position_type == SPECTRAL_POSITIONS_INT32
+                                                               ? static_cast<double>(static_cast<const int*>(s.positions)[from])
+                                                               : static_cast<double>(static_cast<const long long*>(s.positions)[from]);
+                    }
+                }
+            }
         }
         __syncthreads();
         const T* __restrict__ x = static_cast<const T*>(s.x);
@@ -256,39 +271,24 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
             }
             if (base == 0) {  // the first pieces are on their way
                 if (rotated > 0 && column < pitch) {
-            const bool turning = column < rotated / 2;
-            const long long mine = column_axis * s.position_stride[2];
-            // Several at a time: their positions are asked for together. (One after the other took half of the kernel's time.)
-            const auto fill = [&](auto type) {
-                using P = decltype(type);
-                constexpr int kBatch = sizeof(P) == 8 ? 4 : 8;
-                const P* __restrict__ positions = static_cast<const P*>(s.positions) + mine;
-                for (int t0 = threadIdx.x / plan.table_columns; t0 < tokens; t0 += kBatch * table_rows) {
-                    P position[kBatch];
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int t = t0 + j * table_rows;
-                        position[j] = turning && t < tokens ? __ldg(positions + position_places[t]) : P(0);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int t = t0 + j * table_rows;
-                        if (t < tokens) {
-                            const float2 cs = unit<T>(turn_of(position[j], frequency));
-                            cosines[t * pitch + column] = cs.x;
-                            sines[t * pitch + column] = cs.y;
+                    const auto fill = [&](const auto* from) {
+                        from += column_axis * span;
+                        int t = threadIdx.x / plan.table_columns;
+                        float* to = cosines + t * pitch + column;
+                        const int step = table_rows * pitch, across = span * pitch;
+#pragma unroll 4
+                        for (; t < tokens; t += table_rows, to += step) {
+                            const float2 cs = unit<T>(turn_of(from[t], frequency));
+                            to[0] = cs.x;
+                            to[across] = cs.y;
                         }
+                    };
+                    if (floats) {
+                        fill(float_positions);
+                    } else {
+                        fill(whole_positions);
                     }
                 }
-            };
-            if (s.position_type == SPECTRAL_POSITIONS_FLOAT32) {
-                fill(float{});
-            } else if (s.position_type == SPECTRAL_POSITIONS_INT32) {
-                fill(int{});
-            } else {
-                fill(0LL);
-            }
-        }
                 __syncthreads();
             }
 #pragma unroll
@@ -651,6 +651,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     while (plan.table_columns < plan.table_pitch) {
         plan.table_columns *= 2;
     }
+    plan.token_bytes = 8 + (plan.rotated > 0 ? 8 * axes : 0);
     for (int i = 0; i < plan.per_axis && plan.rotated > 0; ++i) {
         plan.turns[i] = std::pow(static_cast<double>(theta), -static_cast<double>(i) / plan.per_axis) / 6.283185307179586476925;
     }
@@ -684,7 +685,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
         t.tokens = s->tokens;
         t.total = batch * s->tokens;
         // As many tokens as the table holds, fewer if that leaves CTAs without any, but enough to keep all lanes busy.
-        const long long cap = kTableBytes / (plan.table_pitch * 8 + 16);
+        const long long cap = kTableBytes / (plan.table_pitch * 8 + plan.token_bytes);
         const long long busy = std::max(1, groups * in_flight / s->heads);
         const long long share = (t.total + most - 1) / most;
         t.tile_tokens = static_cast<int>(std::min(cap, std::min(t.total, std::max(busy, share))));
@@ -713,7 +714,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     }
     const int ctas = plan.side[0].ctas + plan.side[1].ctas;
     if (ctas > 0) {
-        std::size_t smem = static_cast<std::size_t>(table_tokens) * (plan.table_pitch * 8 + 16);
+        std::size_t smem = static_cast<std::size_t>(table_tokens) * (plan.table_pitch * 8 + plan.token_bytes) + 16;
         if (back) {
             smem = std::max(smem, static_cast<std::size_t>(groups) * dim * sizeof(float));
         }
