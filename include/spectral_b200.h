@@ -426,7 +426,7 @@ typedef struct spectral_heads {
  * NULL): u = x / sqrt(mean(x^2) + eps) * weight over a head; its first `rotated` values in `axes` equal spans,
  * each for one axis of the positions; of a span's n = rotated / (2 axes) pairs (u1, u2) the i-th is turned by
  * a = position * theta^(-i / n) to (u1 cos a - u2 sin a, u1 sin a + u2 cos a). Angles are formed in 64 bits;
- * whole-number positions count up to 2^53. Results must not overlap inputs. */
+ * whole-number positions count up to 2^53. Results must overlap neither inputs nor each other. */
 SPECTRAL_API int spectral_qk_norm_rotary(const spectral_heads* q, const spectral_heads* k, int dtype, long long batch, int dim,
                                          int rotated, int axes, int pairs, float eps, float theta, void* stream);
 /* Its gradients from x and dy: out receives dx, dweight the weight's. Fixed summation order. work: as many
@@ -443,10 +443,11 @@ SPECTRAL_API int spectral_qk_norm_rotary_backward(const spectral_heads* q, const
  * by side); NULL for contiguous arrays. A key counts if its index is below lengths[sample] (`batch`
  * int32, or int64 if lengths64 is not 0; NULL: keys) and mask[sample * keys + key] is not 0 (bytes; NULL: all);
  * what lies in the others' places, infinities and NaN among it, has no effect. A row without keys gives zeros.
- * out is contiguous and must not overlap the inputs. rest (16-bit types, a byte per value of out, or NULL) receives what
+ * out is contiguous; out, rest, stats and work must overlap neither the inputs nor each other. rest (16-bit types, a byte per value of out, or NULL) receives what
  * out's rounding took, for the accuracy of the backward pass. stats (batch x kv_heads x queries heads / kv_heads pairs of
  * floats, or NULL) is kept for the backward pass. Products of 16-bit values run on the tensor cores with FP32
- * accumulators, the softmax's weights rounded to the type in between; float32 runs in FP32 throughout.
+ * accumulators, the softmax's weights rounded to the type in between; float32 products run in FP32, or on the tensor cores
+ * as three bf16 parts of each value, six products (what is left out is 2^-24 of a term), with FP32 sums.
  * work: as many complex values as the workspace function says for the same arrays (NULL is an array of unknown
  * alignment). */
 SPECTRAL_API int spectral_cross_attention_workspace(const void* q, const void* k, const void* v, const long long* strides, int dtype,
@@ -457,7 +458,7 @@ SPECTRAL_API int spectral_cross_attention(const void* q, const void* k, const vo
                                           long long queries, long long keys, int heads, int kv_heads, int dim, float scale,
                                           void* work, void* stream);
 /* Its gradients for dout, from the forward call's out, rest (or NULL: out as rounded) and stats: dq, dk and dv, contiguous, of the type and shapes
- * of q, k and v (zeros for keys that do not count). dout is contiguous. Fixed summation order. */
+ * of q, k and v (zeros for keys that do not count). dout is contiguous; dq, dk, dv and work must overlap no other array. Fixed summation order. */
 SPECTRAL_API int spectral_cross_attention_backward_workspace(const void* dout, const void* q, const void* k, const void* v,
                                                              const long long* strides, int dtype, long long batch, long long queries,
                                                              long long keys, int heads, int kv_heads, int dim, size_t* count);

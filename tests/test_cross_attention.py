@@ -247,12 +247,10 @@ def test_small_and_large_gradients_keep_their_accuracy(dtype):
 @pytest.mark.gpu
 def test_sums_of_one_sign_over_many_keys_and_rows():
     # Terms that do not cancel: what a sum loses on the way shows here.
-    g = torch.Generator().manual_seed(1)
     for dtype, (queries, keys) in itertools.product([torch.bfloat16, torch.float16], [(2, 60000), (60000, 40)]):
         q, k, v, dout = inputs(1, queries, keys, 1, 1, 16, dtype)
         q, v, dout = 0.1 * q, v.abs() + 1, dout.abs() + 1
         check(q, k, v, dout)
-    del g
 
 
 @pytest.mark.gpu
@@ -484,7 +482,9 @@ def arguments(**change):
      (dict(dim=0), "dim <= 128"), (dict(dim=129), "dim <= 128"), (dict(heads=3), "multiple of kv_heads"), (dict(kv_heads=0), "multiple of kv_heads"),
      (dict(heads=258), "may share"), (dict(batch=40000), "need batch"), (dict(q=None), "null array"), (dict(v=None), "null array"),
      (dict(out=None), "null array"), (dict(k=(1 << 21) + 1), "aligned"), (dict(stats=(1 << 24) + 4), "aligned"), (dict(lengths=2), "aligned"),
-     (dict(lengths=4100, lengths64=1), "aligned"), (dict(out=(1 << 20) + 64), "must not overlap"), (dict(out=(1 << 22) + 64), "must not overlap")])
+     (dict(lengths=4100, lengths64=1), "aligned"), (dict(out=(1 << 20) + 64), "must not overlap"), (dict(out=(1 << 22) + 64), "must not overlap"),
+     (dict(stats=(1 << 23) + 64), "must not overlap"), (dict(rest=(1 << 23) + 64), "must not overlap"), (dict(rest=1 << 24), "must not overlap"),
+     (dict(stats=1 << 20), "must not overlap"), (dict(mask=1 << 23), "must not overlap"), (dict(lengths=(1 << 23) + 8), "must not overlap")])
 def test_the_c_abi_refuses(change, message):
     with pytest.raises(ValueError, match=message):
         native.call("spectral_cross_attention", *arguments(**change))
@@ -494,6 +494,8 @@ def test_the_c_abi_refuses(change, message):
     ("change", "message"),
     [(dict(dout=None), "null array"), (dict(stats=None), "null array"), (dict(dk=None), "null array"), (dict(work=None), "null array"),
      (dict(dq=(1 << 27) + 1), "aligned"), (dict(dq=(1 << 20) + 64), "must not overlap"), (dict(dv=(1 << 19) + 64), "must not overlap"),
+     (dict(dk=(1 << 27) + 64), "must not overlap"), (dict(dv=1 << 28), "must not overlap"), (dict(dq=1 << 24), "must not overlap"),
+     (dict(rest=1 << 28), "must not overlap"), (dict(mask=1 << 29), "must not overlap"), (dict(work=1 << 27), "must not overlap"),
      (dict(dtype=-1), "dtype must be")])
 def test_the_c_abi_refuses_backward(change, message):
     a = dict(dout=1 << 19, q=1 << 20, k=1 << 21, v=1 << 22, strides=None, out=1 << 23, rest=None, stats=1 << 24, lengths=None, lengths64=0, mask=None,

@@ -26,10 +26,8 @@ def turn_by(t, positions, rotated, pairs, theta, sign=1.0):
     for a in range(axes):
         angle = positions[..., a, None].double() * theta ** (-torch.arange(n, device=t.device).double() / n)
         c, s = torch.cos(angle).unsqueeze(-2), sign * torch.sin(angle).unsqueeze(-2)
-        part = slice(a * span, (a + 1) * span)
         one = slice(a * span, a * span + n) if pairs == "halves" else slice(a * span, (a + 1) * span, 2)
         two = slice(a * span + n, (a + 1) * span) if pairs == "halves" else slice(a * span + 1, (a + 1) * span, 2)
-        del part
         out[..., one] = t[..., one] * c - t[..., two] * s
         out[..., two] = t[..., one] * s + t[..., two] * c
     return out
@@ -335,6 +333,17 @@ def test_the_c_abi_refuses_backward():
             native.call("spectral_qk_norm_rotary_backward", side(**change), None, *args, None, None)
     with pytest.raises(ValueError, match="needs q or k"):
         native.call("spectral_qk_norm_rotary", None, None, *args, None)
+
+
+@pytest.mark.parametrize(
+    "change", [dict(x=(1 << 21) + 64), dict(out=(1 << 20) + 64), dict(out=(1 << 21) + 64), dict(out=1 << 22), dict(out=1 << 24), dict(dweight=1 << 22),
+               dict(dweight=1 << 23), dict(weight=(1 << 21) + 64), dict(positions=(1 << 21) + 64), dict(dy=1 << 21)])
+def test_the_c_abi_refuses_keys_over_the_queries(change):
+    # The queries' arrays: x at 2^20, out 2^21, dy 2^22, dweight 2^23, weight 2^24.
+    q = side(weight=1 << 24, dweight=1 << 23)
+    k = side(**(dict(x=1 << 25, out=1 << 26, dy=1 << 27) | change))
+    with pytest.raises(ValueError, match="must not overlap"):
+        native.call("spectral_qk_norm_rotary_backward", q, k, 1, 2, 16, 16, 1, 0, 1e-6, 1e4, 1 << 30, None)
 
 
 def test_cpu_tensors_and_wrong_counts_are_refused():
