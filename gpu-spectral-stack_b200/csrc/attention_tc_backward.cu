@@ -15,6 +15,9 @@
 // float16 keeps p times 2^15 and ds times a power of two that no |ds| takes past 2^15: |g v - delta| is at most
 // 2 max|g| max|v| (norms of rows and keys that count), which the kernel before these finds. Unscaled, weights of 2^-14 and
 // less (16384 keys and more) would be subnormal, and small gradients zero.
+//
+// Measured, forward and backward in bf16: 64 x 16384 x 256 keys, 2 heads of 32, 1266 us (both kernels issue in 43 to 47 % of
+// their slots: instructions of dependent chains); 4 x 4096 x 4096, 16 and 4 heads of 128, 2524 us (tensor pipe 47 to 53 %).
 
 #include "attention_tc.cuh"
 

@@ -14,8 +14,8 @@
 // through the heads. An angle is position * frequency in turns, exact to 2^-48 or in 64 bits until whole turns
 // are taken off (a position of 2^20 leaves an angle of 2^-4 in 32 bits), then float32.
 // Sums over dim, and those of the weights' gradients over rows, are float32 in a fixed order.
-// What bounds it is the number of instructions, 28 a value at two heads a token: 64 x 16384 tokens of 2 x 32 bf16 values and
-// 256 keys a sample take 102 us (2.7 TB/s; the bytes alone 43 us), forward and backward 245 us.
+// What bounds it is the number of instructions, 31 a value at two heads a token: 64 x 16384 tokens of 2 x 32 bf16 values and
+// 256 keys a sample take 101 us (2.8 TB/s; the bytes alone 43 us), forward and backward 236 us.
 
 #include "../../include/spectral_b200.h"
 
