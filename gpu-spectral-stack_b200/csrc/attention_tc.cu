@@ -62,7 +62,9 @@ __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
     it.b = static_cast<int>(pair / static_cast<unsigned>(g.c.kv_heads));
     it.head = static_cast<int>(pair) - it.b * g.c.kv_heads;
     it.key0 = it.split * g.split_tiles * Keys;
-    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * Keys);
+    const int length = length_of(g.c, it.b);
+    const int span = g.split_tiles * Keys;
+    it.end = length - it.key0 > span ? it.key0 + span : length;  // the last split's nominal end may pass 2^31
     it.tiles = it.end > it.key0 ? (it.end - it.key0 + Keys - 1) / Keys : 0;
     it.slots = min(Slots, (g.c.queries - it.row_tile * g.tokens_per_tile + g.tokens_per_tile - 1) / g.tokens_per_tile);
     return it;

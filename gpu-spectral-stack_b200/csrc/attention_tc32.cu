@@ -133,7 +133,9 @@ __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
     it.b = static_cast<int>(pair / static_cast<unsigned>(g.c.kv_heads));
     it.head = static_cast<int>(pair) - it.b * g.c.kv_heads;
     it.key0 = it.split * g.split_tiles * Cfg::kKeys;
-    it.end = min(length_of(g.c, it.b), it.key0 + g.split_tiles * Cfg::kKeys);
+    const int length = length_of(g.c, it.b);
+    const int span = g.split_tiles * Cfg::kKeys;
+    it.end = length - it.key0 > span ? it.key0 + span : length;  // the last split's nominal end may pass 2^31
     it.tiles = it.end > it.key0 ? (it.end - it.key0 + Cfg::kKeys - 1) / Cfg::kKeys : 0;
     it.slots = Cfg::kSlots == 2 && (it.row_tile + 1) * g.tokens_per_tile < g.c.queries ? 2 : 1;
     return it;

@@ -329,6 +329,33 @@ def test_the_same_bits_every_time_on_a_side_stream_and_from_a_graph(queries, key
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [1, 40])
+def test_lengths_outside_the_keys(queries, dtype):
+    # Longer than the keys: all of them count. Negative: none.
+    q, k, v, dout = inputs(3, queries, 333, 4, 2, 64, dtype)
+    within_keys = torch.tensor([333, 0, 100], device="cuda")
+    for kind in (torch.int32, torch.int64):
+        least, most = torch.iinfo(kind).min, torch.iinfo(kind).max
+        for low, high in ((-1, 334), (least, most)):
+            got = run(q, k, v, dout, lengths=torch.tensor([high, low, 100], dtype=kind, device="cuda"))
+            assert all(torch.equal(a, b) for a, b in zip(got, run(q, k, v, dout, lengths=within_keys.to(kind))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 20])
+def test_the_last_of_the_most_keys(queries):
+    # As many keys as a call may have, all the same one: where only the last 100 count the answer is their value, with weights
+    # of one exactly, and a sum of 100 equal terms is off by far less than half a step of bf16.
+    keys = (1 << 31) - 256
+    q, k, v, _ = inputs(1, queries, 1, 1, 1, 8, torch.bfloat16)
+    mask = torch.zeros(1, keys, dtype=torch.bool, device="cuda")
+    mask[:, -100:] = True
+    out = cross_attention(q, k.expand(1, keys, 1, 8), v.expand(1, keys, 1, 8), mask=mask)
+    assert torch.equal(out, v.expand_as(out))
+
+
+@pytest.mark.gpu
 def test_past_two_to_the_31_values():
     keys = (1 << 25) + 77
     k = torch.zeros(1, keys, 1, 64, dtype=torch.bfloat16, device="cuda")
