@@ -947,7 +947,7 @@ extern "C" int spectral_cross_attention_workspace(const void* q, const void* k, 
     *count = 0;
     if (c.pairs() * c.rows() > 0) {
         try {
-            *count = forward_workspace(c) / 8;
+            *count = work_bytes(forward_workspace(c)) / 8;
         } catch (const std::exception& e) {
             set_last_error(e.what());
             return SPECTRAL_CUDA_ERROR;
@@ -999,21 +999,21 @@ extern "C" int spectral_cross_attention(const void* q, const void* k, const void
         return invalid("cross_attention: out, rest and stats must not overlap each other or the arguments");
     }
     try {
-        const std::size_t work_bytes = forward_workspace(c);
-        if (work == nullptr && work_bytes > 0) {
+        const std::size_t needed = work_bytes(forward_workspace(c));
+        if (work == nullptr && needed > 0) {
             return invalid("cross_attention: needs a workspace");
         }
-        if (any_overlap({Extent(work, work_bytes)}, {result, e.rest, e.stats, e.q, e.k, e.v, e.lengths, e.mask})) {
+        if (any_overlap({Extent(work, needed)}, {result, e.rest, e.stats, e.q, e.k, e.v, e.lengths, e.mask})) {
             return invalid("cross_attention: work must not overlap the arrays");
         }
         if (few_rows(c)) {
-            few_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+            few_forward(c, work_base(work), static_cast<cudaStream_t>(stream));
         } else if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c, false)) {
-            split_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+            split_forward(c, work_base(work), static_cast<cudaStream_t>(stream));
         } else if (dtype == SPECTRAL_FLOAT32) {
-            forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+            forward(c, work_base(work), static_cast<cudaStream_t>(stream));
         } else {
-            tensor_forward(c, static_cast<char*>(work), static_cast<cudaStream_t>(stream));
+            tensor_forward(c, work_base(work), static_cast<cudaStream_t>(stream));
         }
         return SPECTRAL_OK;
     } catch (const InvalidArgument& e) {
@@ -1042,7 +1042,7 @@ extern "C" int spectral_cross_attention_backward_workspace(const void* dout, con
     *count = 0;
     if (c.pairs() * c.rows() > 0 && keys > 0) {
         try {
-            *count = backward_workspace(c) / 8;
+            *count = work_bytes(backward_workspace(c)) / 8;
         } catch (const std::exception& e) {
             set_last_error(e.what());
             return SPECTRAL_CUDA_ERROR;
@@ -1107,16 +1107,16 @@ extern "C" int spectral_cross_attention_backward(const void* dout, const void* q
         const Extents e(c, lengths, lengths64, mask, rest, stats);
         const Extent of_dq(dq, q_bytes), of_dk(dk, k_bytes), of_dv(dv, k_bytes), of_dout(dout, q_bytes), of_out(out, q_bytes);
         if (any_overlap({of_dq, of_dk, of_dv}, {e.q, e.k, e.v, of_dout, of_out, e.rest, e.stats, e.lengths, e.mask})
-            || any_overlap({Extent(work, backward_workspace(c))},
+            || any_overlap({Extent(work, work_bytes(backward_workspace(c)))},
                            {of_dq, of_dk, of_dv, e.q, e.k, e.v, of_dout, of_out, e.rest, e.stats, e.lengths, e.mask})) {
             return invalid("cross_attention_backward: gradients and work must not overlap each other or the arguments");
         }
         if (dtype == SPECTRAL_FLOAT32 && on_tensor_cores(c, true)) {
-            split_backward(c, static_cast<char*>(work), s);
+            split_backward(c, work_base(work), s);
         } else if (dtype == SPECTRAL_FLOAT32) {
-            backward(c, static_cast<char*>(work), s);
+            backward(c, work_base(work), s);
         } else {
-            tensor_backward(c, static_cast<char*>(work), s);
+            tensor_backward(c, work_base(work), s);
         }
         return SPECTRAL_OK;
     } catch (const InvalidArgument& e) {

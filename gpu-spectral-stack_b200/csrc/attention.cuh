@@ -13,6 +13,7 @@
 #include "backend.hpp"
 #include "launch.cuh"
 #include "pointwise.cuh"
+#include "workspace.hpp"
 
 #include <cuda_fp8.h>
 
@@ -133,20 +134,5 @@ void few_forward(const Call& c, char* work, cudaStream_t stream);
 void row_constants(const Call& c, float* out, int width, int tokens, int tiles, cudaStream_t stream);
 
 inline int pieces(long long n, long long per) { return static_cast<int>((n + per - 1) / per); }
-
-// A part of a workspace, in bytes; every array starts on 256.
-class Arena {
-public:
-    std::size_t take(std::size_t bytes)
-    {
-        const std::size_t at = size_;
-        size_ += (bytes + 255) / 256 * 256;
-        return at;
-    }
-    std::size_t size() const { return size_; }
-
-private:
-    std::size_t size_ = 0;
-};
 
 }  // namespace spectral::attention

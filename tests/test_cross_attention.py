@@ -13,8 +13,12 @@ e = 2^-24, in the order the kernels compute:
 float16 weights and gradients below its smallest normal number lose relative accuracy: 2^-25 of the scale they are
 held in, at least 1 for weights (the largest is 1 or more), and 2^-40 of the largest product for gradients."""
 
+import ctypes
 import itertools
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -531,6 +535,107 @@ def test_the_c_abi_refuses_backward(change, message):
     a.update(change)
     with pytest.raises(ValueError, match=message):
         native.call("spectral_cross_attention_backward", *a.values())
+
+
+def host_program(tmp_path, source):
+    """Compiles and runs a C++ program over the kernels' host headers; its output."""
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    headers = Path(__file__).resolve().parent.parent / "gpu-spectral-stack_b200" / "csrc"
+    (tmp_path / "main.cpp").write_text(source)
+    subprocess.run(["g++", "-std=c++17", "-I", str(headers), str(tmp_path / "main.cpp"), "-o", str(tmp_path / "main")], check=True)
+    return subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True).stdout
+
+
+def test_a_workspace_starts_on_whole_256s_and_has_room_for_that(tmp_path):
+    source = """
+        #include "workspace.hpp"
+        #include <cstdio>
+        #include <initializer_list>
+        int main()
+        {
+            using namespace spectral;
+            Arena arena;
+            for (std::size_t bytes : {1, 256, 300, 0, 8}) {
+                const std::size_t at = arena.take(bytes);
+                if (at % 256 != 0) return 1;
+            }
+            if (arena.size() != 256 * 5 || work_bytes(0) != 0) return 2;
+            for (std::size_t bytes : {1, 8, 256, 1280}) {
+                for (std::uintptr_t at = 1 << 20; at < (1 << 20) + 512; at += 8) {
+                    const auto from = reinterpret_cast<std::uintptr_t>(work_base(reinterpret_cast<void*>(at)));
+                    if (from % 256 != 0 || from < at || from + bytes > at + work_bytes(bytes)) return 3;
+                }
+            }
+            std::puts("whole");
+        }
+    """
+    assert host_program(tmp_path, source) == "whole\n"
+
+
+def workspace(name, size, arrays, strides=None):
+    """Bytes that a workspace query asks for; size: dtype, batch, queries, keys, heads, kv_heads, dim."""
+    count = ctypes.c_size_t()
+    native.call(name, *arrays, strides, *size, ctypes.byref(count))
+    return 8 * count.value
+
+
+def test_workspaces_hold_their_arrays_at_any_alignment():
+    whole = lambda n: (n + 255) // 256 * 256
+    # 16-bit arrays of unknown alignment are copied: 3 samples, 40 queries of 4 heads, 70 keys of 2, 24 values; 9 rows or more
+    # and one split, so the copies are all there is.
+    size = (1, 3, 40, 70, 4, 2, 24)
+    copies = whole(3 * 40 * 4 * 24 * 2) + 2 * whole(3 * 70 * 2 * 24 * 2)
+    assert workspace("spectral_cross_attention_workspace", size, [None] * 3) == copies + 256
+    # Three bf16 parts of each in float32.
+    assert workspace("spectral_cross_attention_workspace", (0, *size[1:]), [None] * 3) >= 3 * (3 * 40 * 4 + 2 * 3 * 70 * 2) * 24 * 2 + 256
+    # Few rows over one range of keys, and a call without rows: nothing.
+    assert workspace("spectral_cross_attention_workspace", (1, 3, 1, 70, 4, 2, 24), [None] * 3) == 0
+    assert workspace("spectral_cross_attention_workspace", (1, 3, 0, 70, 4, 2, 24), [None] * 3) == 0
+    assert workspace("spectral_cross_attention_backward_workspace", size, [None] * 4) >= copies + whole(3 * 40 * 4 * 24 * 2) + 256
+
+
+@pytest.mark.parametrize("at", [8, 256])
+def test_a_workspace_over_an_array_is_refused_at_any_alignment(at):
+    # The arrays of a workspace start on the next whole 256 bytes, so the last of them ends past `count` values less 256 bytes.
+    q = 1 << 20
+    size = dict(dtype=0, batch=3, queries=40, keys=70, heads=4, kv_heads=2, dim=24)
+    bytes_ = workspace("spectral_cross_attention_workspace", tuple(size.values()), [q, 1 << 21, 1 << 22])
+    work = (1 << 25) + at
+    for out in (work + bytes_ - 8, work - 8):
+        with pytest.raises(ValueError, match="must not overlap"):
+            native.call("spectral_cross_attention", *arguments(**size, out=out, work=work, stats=1 << 27))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("queries", "keys", "heads", "kv_heads", "dim"), [(1, 5000, 4, 2, 64), (12, 700, 2, 2, 64), (40, 2500, 4, 2, 64), (200, 300, 2, 2, 36),
+                                                                    (33, 70, 2, 1, 13), (300, 150, 2, 2, 128), (2, 200, 130, 2, 32)])
+@pytest.mark.parametrize("off", [8, 136])
+def test_workspaces_of_any_alignment(off, queries, keys, heads, kv_heads, dim, dtype):
+    q, k, v, dout = inputs(2, queries, keys, heads, kv_heads, dim, dtype)
+    want = run(q, k, v, dout)
+    size = (DTYPES.index(dtype), 2, queries, keys, heads, kv_heads, dim)
+    p = lambda t: t.data_ptr() if t.numel() else None
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def work(name, *arrays):  # 8 bytes past a multiple of 128, junk in it
+        bytes_ = workspace(name, size, [p(t) for t in arrays])
+        whole = torch.full((bytes_ + 512,), 255, dtype=torch.uint8, device="cuda")
+        first = -whole.data_ptr() % 256 + off
+        return whole, (whole.data_ptr() + first if bytes_ else None), first, first + bytes_
+
+    out, dq, dk, dv = (torch.empty_like(t) for t in (q, q, k, v))
+    stats = torch.empty(2, kv_heads, queries * (heads // kv_heads), 2, device="cuda")
+    rest = torch.empty(0 if dtype == torch.float32 else q.numel(), dtype=torch.int8, device="cuda")
+    scale = 1.0 / math.sqrt(dim)
+    whole, at, first, last = work("spectral_cross_attention_workspace", q, k, v)
+    native.call("spectral_cross_attention", p(q), p(k), p(v), None, None, 0, None, p(out), p(rest), p(stats), *size, scale, at, stream)
+    assert torch.equal(out, want[0]) and bool((whole[:first] == 255).all()) and bool((whole[last:] == 255).all())
+    whole, at, first, last = work("spectral_cross_attention_backward_workspace", dout, q, k, v)
+    native.call("spectral_cross_attention_backward", p(dout), p(q), p(k), p(v), None, p(out), p(rest), p(stats), None, 0, None, p(dq), p(dk), p(dv),
+                *size, scale, at, stream)
+    assert all(torch.equal(g, w) for g, w in zip((dq, dk, dv), want[1:])) and bool((whole[:first] == 255).all()) and bool((whole[last:] == 255).all())
 
 
 def test_cpu_tensors_are_refused():
