@@ -312,7 +312,10 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
                         square = fma2(xs[k].p[j], xs[k].p[j], square);
                     }
                 }
-                const float inv = rsqrtf(fmaf(sum_lanes(square.x + square.y, lanes), per_dim, plan.eps));
+                // (A row behind the tile's last holds zeros: with eps = 0 its root's inverse would be infinite, and 0 times that a NaN
+                // in the weights' sums.)
+                const float norm = rsqrtf(fmaf(sum_lanes(square.x + square.y, lanes), per_dim, plan.eps));
+                const float inv = !Back || row < rows ? norm : 0.0f;
                 // What is turned: x w forward (inv comes at the end), the upstream gradient (the other way) backward.
 #pragma unroll
                 for (int k = 0; k < U; ++k) {

@@ -147,6 +147,16 @@ def test_settings(pairs, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+@pytest.mark.parametrize("dim", [8, 64, 36, 50, 70, 109, 128])
+def test_no_epsilon(dim, pairs, dtype):
+    # Every width of a piece, rows that do not fill a CTA's last turn: what lies behind them has no part in dweight.
+    check(2, 9, 13, 2, 1, dim, 1, None, pairs, "float", dtype, eps=0.0)
+    check(1, 301, 1, 3, 1, dim, 1, None, pairs, "none", dtype, eps=0.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("pairs", ["halves", "neighbours"])
 def test_far_positions_keep_their_angles(pairs):
     # Positions next to each other far out: 2^40 + i. Whole turns are taken off in 64 bits, so the turned vectors'
