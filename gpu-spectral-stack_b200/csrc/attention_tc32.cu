@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(BackwardConfig<Boxes>::kThreads, 1) backward_k
                     }
                     if constexpr (!Rows) {
                         const long long at = (static_cast<long long>(it.b) * c.kv_heads + it.head) * g.row_walks + t;
-                        tma::bulk_g2s(constants + stage * kConstants, g.constants + at * kConstants, kConstants * 4, &full[stage]);
+                        tma::bulk_g2s(constants + stage * kConstants, g.constants + row_constants_at(at, kWidth), kConstants * 4, &full[stage]);
                     }
                 }
                 __syncwarp();
@@ -896,7 +896,7 @@ __global__ void __launch_bounds__(BackwardConfig<Boxes>::kThreads, 1) backward_k
             if constexpr (Rows) {
                 if (live) {
                     const int tile = token / g.walked_tokens;
-                    const float* from = g.constants + (pair_at * g.row_walks + tile) * kConstants + (token - tile * g.walked_tokens) * c.group + row_head;
+                    const float* from = g.constants + row_constants_at(pair_at * g.row_walks + tile, kWidth) + (token - tile * g.walked_tokens) * c.group + row_head;
                     shift = pair(from[0]);
                     delta = pair(from[kWidth]);
                 }

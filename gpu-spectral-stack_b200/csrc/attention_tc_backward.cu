@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows>::kThreads, Config<Boxes, R
                     }
                     if constexpr (!Rows) {
                         const long long at = (static_cast<long long>(it.b) * c.kv_heads + it.head) * g.row_walks + t;
-                        tma::bulk_g2s(const_cast<float*>(constants) + stage * Cfg::kConstants, g.constants + at * Cfg::kConstants, Cfg::kConstantBytes,
+                        tma::bulk_g2s(const_cast<float*>(constants) + stage * Cfg::kConstants, g.constants + row_constants_at(at, kWidth), Cfg::kConstantBytes,
                                       &full[stage]);
                     }
                 }
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(Config<Boxes, Rows>::kThreads, Config<Boxes, R
             if constexpr (Rows) {
                 if (live) {
                     const int tile = token / g.walked_tokens;
-                    const float* from = g.constants + (pair_at * g.row_walks + tile) * Cfg::kConstants + (token - tile * g.walked_tokens) * c.group + row_head;
+                    const float* from = g.constants + row_constants_at(pair_at * g.row_walks + tile, kWidth) + (token - tile * g.walked_tokens) * c.group + row_head;
                     shift = pair(from[0]);
                     delta = pair(from[kWidth]);
                 }
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
     for (long long base = static_cast<long long>(blockIdx.x) * per_cta; base < all; base += static_cast<long long>(gridDim.x) * per_cta) {
         const long long i = base + threadIdx.x / lanes;
         const int local = static_cast<int>(i & (width - 1));  // 64 or 128
-        const auto tile = static_cast<unsigned>(i / width);     // below 2^31: every tile is an item or a part of one
+        const auto tile = static_cast<unsigned>(i / width);     // below 2^32: their constants are 512 bytes each and more
         const unsigned pair_at = tile / static_cast<unsigned>(row_tiles);
         const int r = static_cast<int>(tile - pair_at * row_tiles) * rows_per_tile + local;
         const bool there = i < all && local < rows_per_tile && r < c.rows();
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
                 const float2 s = c.stats[pair_at * c.rows() + r];
                 lse = s.y == 0.0f ? INFINITY : s.x + log2f(s.y);
             }
-            float* at = out + tile * 2 * width + local;
+            float* at = out + row_constants_at(tile, width) + local;
             at[0] = -lse;
             at[width] = -delta;
         }

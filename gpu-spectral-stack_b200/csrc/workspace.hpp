@@ -34,4 +34,8 @@ inline std::size_t work_bytes(std::size_t bytes)
     return bytes == 0 ? 0 : (bytes + 7) / 8 * 8 + kWorkAlign;
 }
 
+// Attention backward, an array of floats: where a tile of rows keeps its constants, `width` of one kind and `width` of the other.
+// (In 64 bits: 2^25 tiles of 64 rows, one token of 33 heads each, are 2^32 floats.)
+constexpr long long row_constants_at(long long tile, int width) { return tile * 2 * width; }
+
 }  // namespace spectral

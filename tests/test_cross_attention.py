@@ -573,6 +573,23 @@ def test_a_workspace_starts_on_whole_256s_and_has_room_for_that(tmp_path):
     assert host_program(tmp_path, source) == "whole\n"
 
 
+def test_row_constants_past_two_to_the_32_floats(tmp_path):
+    # As many tiles as 2^25 tokens of 33 heads make (and twice as many of twice the rows): the last one's place, and its neighbour's.
+    source = """
+        #include "workspace.hpp"
+        #include <cstdio>
+        int main()
+        {
+            const unsigned tile = (1u << 25) + 3;  // as the kernel counts them
+            const int width = 64;
+            std::printf("%lld %lld %lld\\n", spectral::row_constants_at(tile, width), spectral::row_constants_at(tile - 1, width),
+                        spectral::row_constants_at(2LL * tile, 2 * width));
+        }
+    """
+    last = ((1 << 25) + 3) * 128
+    assert host_program(tmp_path, source).split() == [str(last), str(last - 128), str(4 * last)]
+
+
 def workspace(name, size, arrays, strides=None):
     """Bytes that a workspace query asks for; size: dtype, batch, queries, keys, heads, kv_heads, dim."""
     count = ctypes.c_size_t()
