@@ -11,8 +11,8 @@
 // lanes sit side by side, so its sums are a few shuffles and so is the exchange of the pairs that lie half
 // an axis apart. The angles of a token serve all of its heads: a CTA takes as many tokens as its shared memory
 // holds tables for, asks for the first pieces, fills the table of cosines and sines while they arrive, then works
-// through the heads. An angle is position * frequency in turns, exact to 2^-48 or in 64 bits until whole turns
-// are taken off (a position of 2^20 leaves an angle of 2^-4 in 32 bits), then float32.
+// through the heads. An angle is position * frequency in turns, in two floats or in 64 bits until whole turns
+// are taken off (a position of 2^20 leaves an angle of 2^-4 in 32 bits), then float32: see turn_of.
 // Sums over dim, and those of the weights' gradients over rows, are float32 in a fixed order.
 // What bounds it is the number of instructions, 31 a value at two heads a token: 64 x 16384 tokens of 2 x 32 bf16 values and
 // 256 keys a sample take 101 us (2.8 TB/s; the bytes alone 43 us), forward and backward 236 us.
@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = SPECTRAL_HEAD_DIM_MAX;
+constexpr double kNearTurns = 65536.0;  // see turn_of
 constexpr int kTableBytes = 40 * 1024;  // places, positions and tables, at most
 
 // Heads a lane works on at a time, while it waits for as many more.
@@ -67,6 +68,7 @@ struct Plan {
     int token_bytes = 8;    // of a token's place and positions
     bool neighbours = false;
     float eps = 0.0f;
+    float near = 0.0f;  // float positions up to here make less than kNearTurns
     double turns[kMaxDim / 2];  // angle per position, in turns, of an axis's pairs
 };
 
@@ -92,7 +94,9 @@ struct Frequency {
 };
 
 // What is left of position * frequency without its whole turns. A float's product with the two floats is exact but for
-// 2^-48 of it; whole numbers go through 64 bits.
+// 2^-48 of it, and as long as it makes less than kNearTurns the rounded product's error, which is not reduced again, is below 2^-7
+// of a turn. Whole numbers, and the floats of a tile with one that makes more, go through 64 bits: off by 2^-53 of all turns for the
+// product, and by (4 + |ln frequency|) times that for the frequency.
 template <class P>
 __device__ __forceinline__ float turn_of(P position, const Frequency& f)
 {
@@ -222,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
 
     for (long long start = static_cast<long long>(cta) * span; start < s.total; start += static_cast<long long>(s.ctas) * span) {
         const int tokens = static_cast<int>(min(static_cast<long long>(span), s.total - start));
+        int close = 1;
         for (int t = threadIdx.x; t < tokens; t += kThreads) {
             const long long token = start + t;
             const long long b = s.total < (1LL << 31) ? static_cast<unsigned>(token) / static_cast<unsigned>(s.tokens) : token / s.tokens;
@@ -232,7 +237,9 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
                 for (int axis = 0; axis < plan.axes; ++axis) {
                     const long long from = at + axis * s.position_stride[2];
                     if (floats) {
-                        float_positions[axis * span + t] = static_cast<const float*>(s.positions)[from];
+                        const float position = static_cast<const float*>(s.positions)[from];
+                        float_positions[axis * span + t] = position;
+                        close &= fabsf(position) <= plan.near ? 1 : 0;
                     } else {
                         whole_positions[axis * span + t] = s.position_type == SPECTRAL_POSITIONS_INT32
                                                                ? static_cast<double>(static_cast<const int*>(s.positions)[from])
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
                 }
             }
         }
-        __syncthreads();
+        const bool near = __syncthreads_and(close) != 0;
         const T* __restrict__ x = static_cast<const T*>(s.x);
         const T* __restrict__ dy = static_cast<const T*>(s.dy) + start * heads * dim;
         T* __restrict__ out = static_cast<T*>(s.out) + start * heads * dim;
@@ -276,22 +283,24 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
             }
             if (base == 0) {  // the first pieces are on their way
                 if (rotated > 0 && column < pitch) {
-                    const auto fill = [&](const auto* from) {
+                    const auto fill = [&](const auto* from, auto wide) {
                         from += column_axis * span;
                         int t = threadIdx.x / plan.table_columns;
                         float* to = cosines + t * pitch + column;
                         const int step = table_rows * pitch, across = span * pitch;
 #pragma unroll 4
                         for (; t < tokens; t += table_rows, to += step) {
-                            const float2 cs = unit<T>(turn_of(from[t], frequency));
+                            const float2 cs = unit<T>(turn_of(static_cast<decltype(wide)>(from[t]), frequency));
                             to[0] = cs.x;
                             to[across] = cs.y;
                         }
                     };
-                    if (floats) {
-                        fill(float_positions);
+                    if (!floats) {
+                        fill(whole_positions, 0.0);
+                    } else if (near) {
+                        fill(float_positions, 0.0f);
                     } else {
-                        fill(whole_positions);
+                        fill(float_positions, 0.0);
                     }
                 }
                 __syncthreads();
@@ -675,6 +684,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     plan.token_bytes = 8 + (plan.rotated > 0 ? 8 * axes : 0);
     for (int i = 0; i < plan.per_axis && plan.rotated > 0; ++i) {
         plan.turns[i] = std::pow(static_cast<double>(theta), -static_cast<double>(i) / plan.per_axis) / 6.283185307179586476925;
+        plan.near = std::min(i == 0 ? HUGE_VALF : plan.near, static_cast<float>(kNearTurns / plan.turns[i]));
     }
     const int v = vector_width(sides, dtype, batch, dim, plan.rotated, axes, pairs);
     const int units = v == 1 ? 4 : v == 2 && dim > 64 ? 2 : 1;

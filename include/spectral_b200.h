@@ -425,8 +425,9 @@ typedef struct spectral_heads {
 /* The norm of each head and the rotation by position, of queries and keys in one pass (either may be
  * NULL): u = x / sqrt(mean(x^2) + eps) * weight over a head; its first `rotated` values in `axes` equal spans,
  * each for one axis of the positions; of a span's n = rotated / (2 axes) pairs (u1, u2) the i-th is turned by
- * a = position * theta^(-i / n) to (u1 cos a - u2 sin a, u1 sin a + u2 cos a). Angles are formed in 64 bits;
- * whole-number positions count up to 2^53. Results must overlap neither inputs nor each other. */
+ * a = position * f, f = theta^(-i / n), to (u1 cos a - u2 sin a, u1 sin a + u2 cos a). Angles are formed in 64 bits, or as
+ * closely: off by (5 + |ln f|) 2^-53 of themselves, which is float32's accuracy up to positions of about 2^28 and 2^-10 at 2^40.
+ * Results must overlap neither inputs nor each other. */
 SPECTRAL_API int spectral_qk_norm_rotary(const spectral_heads* q, const spectral_heads* k, int dtype, long long batch, int dim,
                                          int rotated, int axes, int pairs, float eps, float theta, void* stream);
 /* Its gradients from x and dy: out receives dx, dweight the weight's. Fixed summation order. work: as many

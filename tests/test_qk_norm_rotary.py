@@ -7,6 +7,9 @@ Tolerances are bounds on each value. With u the type's unit roundoff, e = 2^-24 
 (dim + 8) e of itself, a turned value by u of itself and ((dim + 12) e + t) of the magnitudes of its pair; dx likewise
 with the two terms it is made of; a weight's gradient by ((dim + rows + 12) e + t) of its terms' magnitudes."""
 
+import decimal
+import math
+
 import pytest
 import torch
 
@@ -170,6 +173,44 @@ def test_far_positions_keep_their_angles(pairs):
     (c, _), = (qk_norm_rotary(x, None, None, None, near + (1 << 20), pairs=pairs),)
     c = c[0, :, 0].double()
     assert float((a @ a.T - c @ c.T).abs().max()) <= 64 * 4 * 2.0 ** -21
+
+
+PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+def exact_angles(positions, n, theta):
+    """Angles less whole turns, and the whole angles' sizes and frequencies, of (position, pair), by 60 digits."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        frequencies = [decimal.Decimal(theta) ** (decimal.Decimal(-i) / n) for i in range(n)]
+        rest = [[float((decimal.Decimal(p) * f).remainder_near(2 * PI)) for f in frequencies] for p in positions]
+    f = torch.tensor([float(f) for f in frequencies], dtype=torch.float64)
+    return torch.tensor(rest, dtype=torch.float64), torch.tensor(positions, dtype=torch.float64)[:, None].abs() * f, f
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+@pytest.mark.parametrize(("kind", "theta"), [("float", 1e4), ("float", 2.0 ** -20), ("int", 1e4)])
+def test_angles_of_far_positions(kind, theta, pairs, dtype):
+    # Heads (1, 0) in every pair come out as (cos, sin), times sqrt(2). A frequency f in 64 bits is off by (4 + |ln f|) 2^-53 of
+    # itself (the exponent, the power, the division), its product with the position by another 2^-53; then t as above.
+    n = 16
+    places = [0, 1, -77, 5000, 400000, 500000, (1 << 23) + 1, -(1 << 26), (1 << 30) + 128, (1 << 36) + (1 << 13), -(1 << 40), (1 << 41) + (1 << 18)]
+    if kind == "float":
+        places += [0.25, 1000.5, 262143.96875]
+    x = torch.zeros(1, len(places), 1, 2 * n, dtype=dtype, device="cuda")
+    first = slice(0, n) if pairs == "halves" else slice(0, 2 * n, 2)
+    second = slice(n, 2 * n) if pairs == "halves" else slice(1, 2 * n, 2)
+    x[..., first] = 1
+    p = torch.tensor(places, dtype=torch.float32 if kind == "float" else torch.int64, device="cuda")[:, None]
+    y, _ = qk_norm_rotary(x, None, None, None, p, eps=0.0, theta=theta, pairs=pairs)
+    y = y[0, :, 0].double().cpu() / math.sqrt(2.0)
+    angle, size, f = exact_angles(places, n, theta)
+    bound = torch.finfo(dtype).eps / 2 + (2.0 ** -21 if dtype == torch.float32 else 2.0 ** -19) + size * (5 + f.log().abs()) * 2.0 ** -53
+    for got, want in ((y[:, first], torch.cos(angle)), (y[:, second], torch.sin(angle))):
+        worst = ((got - want).abs() / bound).max(1)[0]
+        assert float(worst.max()) <= 1.0, worst.tolist()
 
 
 @pytest.mark.gpu
