@@ -514,7 +514,7 @@ int invalid(const std::string& message)
 int vector_width(const spectral_heads* const (&sides)[2], int dtype, long long batch, int dim, int rotated, int axes, int pairs)
 {
     const int size = static_cast<int>(dtype_size(dtype));
-    const int n = rotated / (2 * axes);
+    const int n = static_cast<int>(rotated / (2LL * axes));
     for (int v = 16 / size; v >= 2; v /= 2) {
         bool ok = dim % v == 0 && dim / v <= (v == 2 ? 64 : 32) && (rotated == 0 || pairs == SPECTRAL_PAIRS_NEIGHBOURS || n % v == 0);
         for (const spectral_heads* s : sides) {
@@ -592,7 +592,7 @@ int check(const char* op, const spectral_heads* const (&sides)[2], bool back, in
     if (dim < 1 || dim > kMaxDim) {
         return invalid(name + ": need 1 <= dim <= " + std::to_string(kMaxDim));
     }
-    if (axes < 1 || rotated < 0 || rotated > dim || rotated % (2 * axes) != 0) {
+    if (axes < 1 || rotated < 0 || rotated > dim || rotated % (2LL * axes) != 0) {
         return invalid(name + ": rotated must be a multiple of 2 * axes from 0 to dim");
     }
     if (pairs != SPECTRAL_PAIRS_HALVES && pairs != SPECTRAL_PAIRS_NEIGHBOURS) {
@@ -675,7 +675,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
         any = any || (s != nullptr && s->positions != nullptr);
     }
     plan.rotated = any ? rotated : 0;
-    plan.per_axis = std::max(1, plan.rotated / (2 * axes));
+    plan.per_axis = static_cast<int>(std::max(1LL, plan.rotated / (2LL * axes)));
     // A piece that reaches past `rotated` (neighbours only) finds angles of zero there.
     plan.table_pitch = plan.rotated == 0 ? 0 : ((plan.neighbours ? (dim + 1) / 2 : plan.rotated / 2) + 3) / 4 * 4;
     while (plan.table_columns < plan.table_pitch) {

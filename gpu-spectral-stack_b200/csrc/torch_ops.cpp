@@ -984,7 +984,7 @@ int rotary_axes(const std::vector<RotarySide>& sides, const char* op)
 int rotary_values(int64_t rotated, int64_t dim, int axes, const char* op)
 {
     if (rotated < 0) {
-        return static_cast<int>(dim / (2 * axes) * (2 * axes));
+        return static_cast<int>(dim / (2LL * axes) * (2LL * axes));
     }
     return small_int(rotated, op, "rotated");
 }

@@ -377,6 +377,25 @@ def test_the_c_abi_refuses(change, call, message):
         native.call("spectral_qk_norm_rotary", side(**change), None, *a.values(), None)
 
 
+@pytest.mark.parametrize("axes", [(1 << 30) + 1, (1 << 31) - 1])
+def test_the_c_abi_refuses_more_axes_than_pairs(axes):
+    # Twice as many wrap in 32 bits: to 2 and to -2, which divide the head.
+    keys = side(positions=4096)
+    for name, work in (("spectral_qk_norm_rotary", ()), ("spectral_qk_norm_rotary_backward", (1 << 30,))):
+        with pytest.raises(ValueError, match="multiple of 2"):
+            native.call(name, keys, None, 1, 2, 16, 16, axes, 0, 1e-6, 1e4, *work, None)
+
+
+@pytest.mark.gpu
+def test_more_axes_than_pairs():
+    q, w, _ = inputs(1, 3, 2, 16, torch.float32)
+    many = torch.ones(3, 1, device="cuda").expand(3, (1 << 31) - 1)
+    with pytest.raises(ValueError, match="multiple of 2"):
+        qk_norm_rotary(q, None, w, None, many, rotated=16)
+    # As many values as whole pairs of every axis: none.
+    assert torch.equal(qk_norm_rotary(q, None, w, None, many)[0], qk_norm_rotary(q, None, w)[0])
+
+
 def test_the_c_abi_refuses_backward():
     args = (1, 2, 16, 16, 1, 0, 1e-6, 1e4)
     for change, message in ((dict(dy=None), "null array"), (dict(dweight=4096), "workspace"), (dict(out=(1 << 22) + 64), "must not overlap")):
