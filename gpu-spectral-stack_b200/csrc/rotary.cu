@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
     const int column = threadIdx.x % plan.table_columns;
     const int table_rows = kThreads / plan.table_columns;
     const int column_axis = column < rotated / 2 ? column / n : 0;
-    Frequency frequency{column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0, 0.0f, 0.0f};  // 0: not turned
+    Frequency frequency{column < rotated / 2 ? plan.turns[column - column_axis * n] : 0.0, 0.0f, 0.0f};
     frequency.high = static_cast<float>(frequency.turns);
     frequency.low = static_cast<float>(frequency.turns - frequency.high);
     allow_next_grid();
@@ -295,7 +295,12 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
                             to[across] = cs.y;
                         }
                     };
-                    if (!floats) {
+                    if (column >= rotated / 2) {  // of a piece that reaches past `rotated`: whatever the position, not turned
+                        for (int t = threadIdx.x / plan.table_columns; t < tokens; t += table_rows) {
+                            cosines[t * pitch + column] = 1.0f;
+                            sines[t * pitch + column] = 0.0f;
+                        }
+                    } else if (!floats) {
                         fill(whole_positions, 0.0);
                     } else if (near) {
                         fill(float_positions, 0.0f);
@@ -676,7 +681,7 @@ void run(const spectral_heads* const (&sides)[2], bool back, int dtype, long lon
     }
     plan.rotated = any ? rotated : 0;
     plan.per_axis = static_cast<int>(std::max(1LL, plan.rotated / (2LL * axes)));
-    // A piece that reaches past `rotated` (neighbours only) finds angles of zero there.
+    // A piece that reaches past `rotated` (neighbours only) finds cosines of 1 and sines of 0 there.
     plan.table_pitch = plan.rotated == 0 ? 0 : ((plan.neighbours ? (dim + 1) / 2 : plan.rotated / 2) + 3) / 4 * 4;
     while (plan.table_columns < plan.table_pitch) {
         plan.table_columns *= 2;

@@ -305,6 +305,22 @@ def test_non_finite_heads_stay_by_themselves():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+@pytest.mark.parametrize("dim", [64, 36, 70, 109])
+def test_a_position_that_is_no_number_leaves_what_is_not_turned(dim, pairs, dtype):
+    x, w, _ = inputs(1, 40, 2, dim, dtype)
+    p = place("float", 1, 40, 1)
+    clean, _ = qk_norm_rotary(x, None, w, None, p, rotated=4, pairs=pairs)
+    for junk in (float("nan"), float("inf")):
+        p[0, 7] = junk
+        y, _ = qk_norm_rotary(x, None, w, None, p, rotated=4, pairs=pairs)
+        assert y[0, 7, :, :4].isnan().all() and torch.equal(y[..., 4:], clean[..., 4:])
+        y[0, 7] = clean[0, 7]
+        assert torch.equal(y, clean)
+
+
+@pytest.mark.gpu
 def test_the_same_bits_every_time_on_a_side_stream_and_from_a_graph():
     q, wq, dq = inputs(4, 900, 4, 64, torch.bfloat16)
     k, wk, dk = inputs(4, 100, 2, 64, torch.bfloat16, 1)
