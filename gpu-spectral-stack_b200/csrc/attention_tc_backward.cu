@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(256) constants_kernel(const Call c, float* __r
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x.p[j] = with_rest(x.p[j], reinterpret_cast<const unsigned short*>(&code)[j]);
+                    x.p[j] = with_rest<T>(x.p[j], reinterpret_cast<const unsigned short*>(&code)[j]);
                 }
             }
 #pragma unroll

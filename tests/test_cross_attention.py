@@ -249,6 +249,18 @@ def test_small_and_large_gradients_keep_their_accuracy(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize(("queries", "keys", "dim"), [(1, 900, 64), (40, 300, 64), (300, 200, 32), (30, 100, 20), (200, 300, 128), (12000, 70, 16)])
+def test_the_size_of_the_values_does_not_change_the_accuracy(queries, keys, dim):
+    # bf16 values times a power of two give out, dq and dk times it, bit for bit: what out's rounding took is kept relative to out.
+    q, k, v, dout = inputs(1, queries, keys, 4, 2, dim, torch.bfloat16)
+    want = run(q, k, v, dout)
+    for size in (2.0 ** -40, 2.0 ** -20, 2.0 ** -7, 2.0 ** 15, 2.0 ** 40):
+        got = run(q, k, v * size, dout)
+        for g, w, by in zip(got, want, (size, size, size, 1.0)):
+            assert torch.equal(g.float(), w.float() * by), size
+
+
+@pytest.mark.gpu
 def test_sums_of_one_sign_over_many_keys_and_rows():
     # Terms that do not cancel: what a sum loses on the way shows here.
     for dtype, (queries, keys) in itertools.product([torch.bfloat16, torch.float16], [(2, 60000), (60000, 40)]):
