@@ -1124,6 +1124,12 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Spli
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             mlp::split3(v[k], part[0].v[k], part[1].v[k], part[2].v[k]);
+            // An infinity (or NaN) as the last part: that one meets the other side's first part alone, so a product is what it is of the
+            // whole values. As the first it would meet parts of either sign and zeros, and be NaN.
+            if (!(fabsf(v[k]) <= 3.4028234663852886e38f)) {
+                part[2].v[k] = part[0].v[k];
+                part[0].v[k] = from_float<bf16>(0.0f);
+            }
         }
 #pragma unroll
         for (int p = 0; p < kPlanes; ++p) {

@@ -184,6 +184,34 @@ def test_non_finite_values_reach_what_reads_them_and_nothing_else(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("queries", "heads", "dim"), [(1, 2, 64), (8, 2, 64), (9, 2, 64), (16, 2, 64), (17, 2, 64), (100, 2, 64), (100, 2, 128), (40, 4, 20),
+                                                 (3, 130, 32)])
+def test_infinities_that_count(queries, heads, dim, dtype):
+    # What the formula gives, whichever kernel a call's size takes. An infinite value: its weights are positive, so infinite results.
+    q, k, v, dout = inputs(2, queries, 90, heads, 2, dim, dtype)
+    clean, group, rest = cross_attention(q, k, v), heads // 2, torch.arange(dim) != 4
+    for sign in (1.0, -1.0):
+        v[1, 5, 0, 4] = sign * float("inf")
+        out = cross_attention(q, k, v)
+        assert bool((out[1, :, :group, 4] == sign * float("inf")).all())
+        assert torch.equal(out[0], clean[0]) and torch.equal(out[1, :, group:], clean[1, :, group:]) and torch.equal(out[..., rest], clean[..., rest])
+    # An infinite key: scores of either infinity by the query's sign. A weight of 0, as if the key did not count, or no number.
+    q, k, v, dout = inputs(2, queries, 90, heads, 2, dim, dtype)
+    k[1, 5, 0, 4] = float("inf")
+    out = cross_attention(q, k, v)
+    keep = torch.ones(2, 90, dtype=torch.bool, device="cuda")
+    keep[1, 5] = False
+    k[1, 5, 0, 4] = 0.0
+    want, bound = formula(q, k, v, dout, keep, 1.0 / math.sqrt(dim), dtype)[0]
+    positive = q[1, :, :group, 4] > 0
+    assert bool(out[1, :, :group][positive].isnan().all())
+    ratio = ((out.double() - want).abs() / bound)[1, :, :group][~positive]
+    assert ratio.numel() == 0 or float(ratio.max()) <= 1.0
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[1, :, group:], clean[1, :, group:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize(("queries", "keys", "dim"), [(33, 70, 64), (33, 70, 20), (1, 900, 64), (200, 200, 128)])
 def test_strided_broadcast_and_unaligned_arrays(queries, keys, dim, dtype):
     q, k, v, dout = inputs(2, queries, keys, 4, 2, dim, dtype)
