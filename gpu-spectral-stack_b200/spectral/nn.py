@@ -256,7 +256,7 @@ class CrossAttention(torch.nn.Module):
                 mask: torch.Tensor | None = None) -> torch.Tensor:
         b, states = x.shape[0], context.shape[1]
         linear = torch.nn.functional.linear
-        q = linear(x, self.w_q).reshape(b, -1, self.heads, self.head_dim)
+        q = linear(x, self.w_q).reshape(b, math.prod(x.shape[1:-1]), self.heads, self.head_dim)
         k = linear(context, self.w_k).reshape(b, states, self.kv_heads, self.head_dim)
         v = linear(context, self.w_v).reshape(b, states, self.kv_heads, self.head_dim)
         q, k = qk_norm_rotary(q, k, self.q_norm, self.k_norm, positions, context_positions, eps=self.eps, theta=self.theta,

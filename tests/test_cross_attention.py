@@ -485,6 +485,24 @@ def test_module(dtype, tol):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(0, 6, 10), (2, 0, 10), (2,)])
+def test_module_over_no_samples_no_points_and_one_point_each(shape, dtype):
+    torch.manual_seed(0)
+    m = CrossAttention(32, 24, 4, kv_heads=2, device="cuda", dtype=dtype)
+    x = torch.randn(*shape, 32, device="cuda").to(dtype).requires_grad_(True)
+    context = torch.randn(shape[0], 30, 24, device="cuda").to(dtype)
+    points = math.prod(shape[1:])
+    places = torch.rand(points, 2, device="cuda"), torch.rand(30, 2, device="cuda")
+    y = m(x, context, positions=places[0], context_positions=places[1])
+    assert y.shape == x.shape
+    y.sum().backward()
+    assert x.grad.shape == x.shape and all(p.grad is not None and bool(p.grad.isfinite().all()) for p in m.parameters())
+    if points == 1:
+        assert torch.equal(y, m(x[:, None], context, positions=places[0], context_positions=places[1])[:, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_the_passes_together(dtype):
     """Norm and rotation, then attention, and back, as a layer runs them: against the same in float64."""
     q, k, v, dout = inputs(2, 90, 140, 4, 2, 32, dtype)
