@@ -151,6 +151,38 @@ def test_values_and_gradients(batch, queries, keys, heads, kv_heads, dim, kind, 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["none", "both"])
+@pytest.mark.parametrize(("batch", "queries", "keys", "heads", "kv_heads", "dim"),
+                         [(2, 9, 65, 1, 1, 24), (1, 12, 1500, 2, 2, 64), (2, 3, 130, 8, 2, 40), (3, 16, 70, 2, 2, 128), (2, 2, 3000, 16, 2, 80),
+                          (2, 5, 150, 128, 1, 64), (2, 3, 270, 130, 2, 128), (2, 1, 200, 100, 1, 50), (2, 20, 90, 96, 1, 96), (2, 300, 40, 66, 1, 33)])
+def test_a_dozen_rows_and_many_heads_over_one(batch, queries, keys, heads, kv_heads, dim, kind, dtype):
+    q, k, v, dout = inputs(batch, queries, keys, heads, kv_heads, dim, dtype)
+    lengths, mask, keep = cuts(kind, batch, keys)
+    check(q, k, v, dout, keep, lengths=lengths, mask=mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("queries", "keys"), [(1, 700), (12, 300), (200, 300)])
+def test_the_operators_without_autograd(queries, keys, dtype):
+    q, k, v, dout = inputs(2, queries, keys, 4, 2, 64, dtype)
+    lengths, mask, keep = cuts("both", 2, keys)
+    lengths[1], mask[1, :9] = keys, True
+    keep = (torch.arange(keys, device="cuda")[None] < lengths[:, None]) & mask
+    want = run(q, k, v, dout, lengths=lengths, mask=mask)
+    ops = torch.ops.spectral
+    out, stats, rest = ops.cross_attention(q, k, v, lengths, mask)
+    assert torch.equal(out, want[0]) and rest.numel() == (0 if dtype == torch.float32 else out.numel())
+    got = ops.cross_attention_backward(dout, q, k, v, out, stats, rest, lengths, mask)
+    assert all(torch.equal(g, w) for g, w in zip(got, want[1:]))
+    # Without what out's rounding took: the bounds count a rounded out.
+    got = ops.cross_attention_backward(dout, q, k, v, out, stats, rest[:0].reshape(-1), lengths, mask)
+    for g, w, name in zip(got, formula(q, k, v, dout, keep, 0.125, dtype)[1:], ("dq", "dk", "dv")):
+        within(g, w, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize(("queries", "keys"), [(1, 700), (200, 300)])
 @pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf"), "largest"])
 def test_what_lies_in_masked_places_has_no_effect(queries, keys, junk, dtype):
