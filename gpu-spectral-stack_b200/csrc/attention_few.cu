@@ -3,7 +3,7 @@
 // The keys and values are all there is to read, once, and two multiply-adds per value and row all there is to compute: memory
 // bounds it, and the CUDA cores keep up. (On the tensor cores such a tile leaves 120 of 128 rows empty, and its
 // softmax runs in one warp: 16 samples x 4 x 16384 keys x 64 bf16, a quarter of them cut off, took 111 us; here
-// 69 us.) A key
+// 70 us.) A key
 // head's keys are cut into ranges, one per CTA, and a range among its warps. `lanes` lanes hold a key, 16 bytes each
 // where rows allow; each such group of lanes walks over keys of its own with the running maximum, sum and result of
 // every row, four keys at a time: four scores by shuffles, one rescaling, four weighted values, with the next two

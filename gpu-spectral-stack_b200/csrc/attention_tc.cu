@@ -13,8 +13,8 @@
 // Work items are (row tiles, split of the keys, sample and key head); CTAs, one per SM, stay and take every
 // 148th. Few rows over many keys are split so that all SMs read, and the parts joined by a second kernel.
 //
-// Measured in bf16: 64 x 16384 x 256 keys, 2 heads of 32, 298 us (XU 40 %, issue 38 %: the softmax bounds it); 4 x 4096 x 4096, 16
-// and 4 heads of 128, 581 us, 946 TFLOP/s (tensor pipe 44 %).
+// Measured in bf16: 64 x 16384 x 256 keys, 2 heads of 32, 297 us (XU 39 %, issue 39 %: the softmax bounds it); 4 x 4096 x 4096, 16
+// and 4 heads of 128, 597 us, 922 TFLOP/s (tensor pipe 44 %).
 
 #include "attention_tc.cuh"
 
@@ -72,7 +72,7 @@ __device__ __forceinline__ Item item_at(const Forward& g, unsigned i)
 
 // Heads of up to 64 values: four row tiles and 64 keys at a time, wider ones two and 128. Either way tensor memory is full; the
 // more warps, the better they fill each other's waits (128 keys and two tiles for all: 64 x 2 x 16384 x 256 x 32 took
-// 400 us, this takes 298).
+// 400 us, this takes 297).
 template <int Boxes>
 struct Config {
     static constexpr int kSlots = Boxes == 1 ? 4 : 2;

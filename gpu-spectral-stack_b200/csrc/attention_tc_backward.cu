@@ -16,8 +16,8 @@
 // 2 max|g| max|v| (norms of rows and keys that count), which the kernel before these finds. Unscaled, weights of 2^-14 and
 // less (16384 keys and more) would be subnormal, and small gradients zero.
 //
-// Measured, forward and backward in bf16: 64 x 16384 x 256 keys, 2 heads of 32, 1266 us (both kernels issue in 43 to 47 % of
-// their slots: instructions of dependent chains); 4 x 4096 x 4096, 16 and 4 heads of 128, 2524 us (tensor pipe 47 to 53 %).
+// Measured, forward and backward in bf16: 64 x 16384 x 256 keys, 2 heads of 32, 1228 us (both kernels issue in 44 to 48 % of
+// their slots: instructions of dependent chains); 4 x 4096 x 4096, 16 and 4 heads of 128, 2567 us (tensor pipe 48 to 54 %).
 
 #include "attention_tc.cuh"
 

@@ -152,7 +152,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None = None, q_weight: tor
     axes), float32, int32 or int64; None: not turned. The rotated values fall into `axes` equal spans, one
     for each axis; of a span's n pairs the i-th is turned by position * theta^(-i / n). pairs="halves" pairs value i
     of a span with value i + n, "neighbours" value 2i with 2i + 1. rotated=None: as many values as 2 * axes
-    divides. Returns contiguous tensors of q's type. Differentiable in q, k and the weights."""
+    divides. Angles are as exact as 64 bits make them: float32's accuracy up to
+    positions of about 2^28. Returns contiguous tensors of q's type. Differentiable in q, k and the weights."""
     out = torch.ops.spectral.qk_norm_rotary_layer.default(
         q, k, q_weight, k_weight, q_positions, k_positions, eps, theta, _rotated(rotated), pairs)
     return out[0], out[1] if k is not None else None
@@ -167,8 +168,8 @@ def _rotated(rotated: int | None) -> int:
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: torch.Tensor | None = None,
                     mask: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v for each sample and head: q (batch, queries, heads, dim) reads k and v (batch, keys,
-    kv_heads, dim), heads / kv_heads neighbouring query heads sharing a head of k and v; dim at most 128,
-    strided views included. scale: 1 / sqrt(dim) if None.
+    kv_heads, dim), heads / kv_heads (at most 128) neighbouring query heads sharing a head of k and v; dim at most 128,
+    batch * kv_heads at most 65535, strided views included. scale: 1 / sqrt(dim) if None.
 
     Only a sample's first lengths[sample] keys count (int32 or int64, (batch,)), and of them those where mask
     ((batch, keys) or (1, keys) bool) is True; what lies in other places has no effect, whatever it is, and gets zero

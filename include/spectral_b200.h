@@ -450,7 +450,7 @@ SPECTRAL_API int spectral_qk_norm_rotary_backward(const spectral_heads* q, const
  * accumulators, the softmax's weights rounded to the type in between; float32 products run in FP32, or on the tensor cores
  * as three bf16 parts of each value, six products (what is left out is 2^-24 of a term), with FP32 sums.
  * work: as many complex values as the workspace function says for the same arrays (NULL is an array of unknown
- * alignment). */
+ * alignment). batch * kv_heads is at most 65535, keys and queries * heads / kv_heads are below 2^31 - 256. */
 SPECTRAL_API int spectral_cross_attention_workspace(const void* q, const void* k, const void* v, const long long* strides, int dtype,
                                                     long long batch, long long queries, long long keys, int heads, int kv_heads,
                                                     int dim, size_t* count);
