@@ -95,7 +95,7 @@ struct Frequency {
 
 // What is left of position * frequency without its whole turns. A float's product with the two floats is exact but for
 // 2^-48 of it, and as long as it makes less than kNearTurns the rounded product's error, which is not reduced again, is below 2^-7
-// of a turn. Whole numbers, and the floats of a tile with one that makes more, go through 64 bits: off by 2^-53 of all turns for the
+// of a turn. Whole numbers, and floats that make more, go through 64 bits: off by 2^-53 of all turns for the
 // product, and by (4 + |ln frequency|) times that for the frequency.
 template <class P>
 __device__ __forceinline__ float turn_of(P position, const Frequency& f)
@@ -283,14 +283,14 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
             }
             if (base == 0) {  // the first pieces are on their way
                 if (rotated > 0 && column < pitch) {
-                    const auto fill = [&](const auto* from, auto wide) {
+                    const auto fill = [&](const auto* from, auto turn) {
                         from += column_axis * span;
                         int t = threadIdx.x / plan.table_columns;
                         float* to = cosines + t * pitch + column;
                         const int step = table_rows * pitch, across = span * pitch;
 #pragma unroll 4
                         for (; t < tokens; t += table_rows, to += step) {
-                            const float2 cs = unit<T>(turn_of(static_cast<decltype(wide)>(from[t]), frequency));
+                            const float2 cs = unit<T>(turn(from[t]));
                             to[0] = cs.x;
                             to[across] = cs.y;
                         }
@@ -301,11 +301,12 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
                             sines[t * pitch + column] = 0.0f;
                         }
                     } else if (!floats) {
-                        fill(whole_positions, 0.0);
+                        fill(whole_positions, [&](double p) { return turn_of(p, frequency); });
                     } else if (near) {
-                        fill(float_positions, 0.0f);
-                    } else {
-                        fill(float_positions, 0.0);
+                        fill(float_positions, [&](float p) { return turn_of(p, frequency); });
+                    } else {  // each by its own size: a token's bits do not depend on its neighbours
+                        fill(float_positions,
+                             [&](float p) { return fabsf(p) <= plan.near ? turn_of(p, frequency) : turn_of(static_cast<double>(p), frequency); });
                     }
                 }
                 __syncthreads();

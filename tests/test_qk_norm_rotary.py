@@ -305,6 +305,17 @@ def test_non_finite_heads_stay_by_themselves():
 
 
 @pytest.mark.gpu
+def test_a_far_position_does_not_change_its_neighbours():
+    x, w, _ = inputs(1, 60000, 1, 64, torch.float32)
+    p = place("float", 1, 60000, 1) * 1000
+    clean, _ = qk_norm_rotary(x, None, w, None, p)
+    p[0, ::50] = 1e9
+    y, _ = qk_norm_rotary(x, None, w, None, p)
+    same = torch.arange(60000) % 50 != 0
+    assert torch.equal(y[0, same], clean[0, same])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("pairs", ["halves", "neighbours"])
 @pytest.mark.parametrize("dim", [64, 36, 70, 109])
