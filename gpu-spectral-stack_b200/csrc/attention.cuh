@@ -70,13 +70,15 @@ __device__ __forceinline__ int length_of(const Call& c, int b)
     return static_cast<int>(max(0LL, min(n, static_cast<long long>(c.keys))));
 }
 
-// What rounding out to its type took from it, as a byte: a whole number of 1 / kRestSteps of the last place of the rounded value, so
-// that it is as accurate for small and large values of v, and half a place is kRestSteps / 2. (Places are counted from 2^-112 in
-// bf16, so that a step is a normal number, and in float16 from 2^-14, below which they all are 2^-24.) The backward pass needs sum over dim of
+// What rounding out to its type took from it, as a byte: in steps of 2^-kRestBits of the last place of the rounded value, 64 at
+// most, so that it is as accurate for small values of v as for large ones. (Places are counted from 2^-112 in bf16, so that a step is a
+// normal number, and in float16 from 2^-14, below which they all are 2^-24.) The backward pass needs sum over dim of
 // dout out, the weighted mean of dout v, to subtract it from each dout v: with out as
 // rounded, dq of 512 x 16384 keys in float16 was off by 5.5e-4 of its norm, with this byte by 3.1e-4 (one rounding to
 // float16 is 2.1e-4, and the score gradients are rounded too).
-constexpr float kRestSteps = 128.0f;
+constexpr unsigned kRestBits = 7;
+template <class T>
+constexpr unsigned kPlaceBits = std::is_same_v<T, bf16> ? 7 : 10;  // behind the first
 
 // The exponent bits of a rounded value, or those from which places are counted.
 template <class T>
@@ -91,11 +93,10 @@ __device__ __forceinline__ unsigned rest_exponent(float rounded)
 template <class T>
 __device__ __forceinline__ unsigned short rest_of(float2 o)
 {
-    constexpr unsigned kPlace = std::is_same_v<T, bf16> ? 7u : 10u;  // bits behind the first
     const float2 rounded = widen(narrow<T>(Floats<2>{{o}})).p[0];
     const float2 r = o - rounded;
-    // kRestSteps / place = 2^(7 + kPlace - exponent)
-    const auto scale = [](float v) { return __uint_as_float(((127u + 127u + 7u + kPlace) << 23) - rest_exponent<T>(v)); };
+    // Steps to a value of one: 2^(kRestBits + kPlaceBits - exponent).
+    const auto scale = [](float v) { return __uint_as_float(((127u + 127u + kRestBits + kPlaceBits<T>) << 23) - rest_exponent<T>(v)); };
     const float2 n = fma2(r, make_float2(scale(rounded.x), scale(rounded.y)), pair(12582912.0f));
     return static_cast<unsigned short>(__byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040));
 }
@@ -103,8 +104,7 @@ __device__ __forceinline__ unsigned short rest_of(float2 o)
 template <class T>
 __device__ __forceinline__ float2 with_rest(float2 rounded, unsigned short bytes)
 {
-    constexpr unsigned kPlace = std::is_same_v<T, bf16> ? 7u : 10u;
-    const auto step = [](float v) { return __uint_as_float(rest_exponent<T>(v) - ((7u + kPlace) << 23)); };
+    const auto step = [](float v) { return __uint_as_float(rest_exponent<T>(v) - ((kRestBits + kPlaceBits<T>) << 23)); };
     const float2 n = make_float2(static_cast<float>(static_cast<signed char>(bytes)), static_cast<float>(static_cast<signed char>(bytes >> 8)));
     return fma2(n, make_float2(step(rounded.x), step(rounded.y)), rounded);
 }

@@ -15,7 +15,7 @@
 // are taken off (a position of 2^20 leaves an angle of 2^-4 in 32 bits), then float32: see turn_of.
 // Sums over dim, and those of the weights' gradients over rows, are float32 in a fixed order.
 // What bounds it is the number of instructions, 31 a value at two heads a token: 64 x 16384 tokens of 2 x 32 bf16 values and
-// 256 keys a sample take 102 us (2.8 TB/s; the bytes alone 43 us), forward and backward 238 us.
+// 256 keys a sample take 102 us (2.8 TB/s; the bytes alone 43 us), forward and backward 239 us.
 
 #include "../../include/spectral_b200.h"
 
@@ -37,7 +37,7 @@ constexpr int kTableBytes = 40 * 1024;  // places, positions and tables, at most
 
 // Heads a lane works on at a time, while it waits for as many more.
 // (64 x 16384 x 2 x 32 bf16, measured side by side: four CTAs an SM and fewer heads a lane 105 us, backward 268; two CTAs 124 and
-// 288; this form 102 and 245, and 102 and 238 with the steps that followed.)
+// 288; this form 102 and 245, and 102 and 239 with the steps that followed.)
 __host__ __device__ constexpr int rows_in_flight(int units, bool back) { return units > 1 ? (back ? 1 : 2) : back ? 2 : 4; }
 
 struct Side {
