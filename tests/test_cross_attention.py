@@ -405,6 +405,25 @@ def test_the_same_bits_every_time_on_a_side_stream_and_from_a_graph(queries, key
 
 
 @pytest.mark.gpu
+def test_calls_on_several_streams_at_once():
+    # Kernels that share SMs and their tensor memory: one sample's worth each, so that they run side by side.
+    cases = [inputs(1, queries, keys, heads, 2, dim, dtype)
+             for dtype, (queries, keys, heads, dim) in zip(DTYPES * 2, [(300, 700, 2, 64), (500, 300, 4, 32), (200, 900, 2, 128), (100, 400, 2, 96),
+                                                                       (1, 5000, 4, 64), (700, 130, 2, 64)])]
+    want = [run(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for c, stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                got.append(run(*c))
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(results, want[i % len(cases)]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("queries", [1, 40])
 def test_lengths_outside_the_keys(queries, dtype):
